@@ -1,5 +1,6 @@
 // What the bf16 GEMM kernels share (llattn_gemm.hip: 256 x 256 tiles; llattn_gemm_tile.hip: smaller ones): the
-// launch arguments, the epilogue arithmetic, direct-to-LDS loads and the fragment reads of 64-k LDS stages.
+// launch arguments, the epilogue arithmetic, direct-to-LDS loads and the fragment reads of 64-k LDS stages.  The
+// products of the head loss (llattn_head.hip) and of the orthogonalisation (llattn_muon.hip) use the last two as well.
 #pragma once
 
 #include <type_traits>
@@ -226,6 +227,52 @@ __device__ __forceinline__ bf16x8 frag64(const unsigned char* tile, int o16, int
   }
 }
 
+constexpr int SK = 64;  // k per stage
+
+// Tile operand of O rows / columns x 64 k.  k-contiguous: rows of 128 bytes, chunk c (8 k) of row o at slot
+// c ^ pswz<PERM>(o).  m/n-contiguous: 64 k-rows of 2 O bytes, chunk c (8 columns) of k-row k at c ^ 2 (k & 3).
+template <bool KC, bool PERM, int O>
+struct TileOp {
+  static constexpr int BYTES = O * 128, NB = BYTES / 1024 / 4;  // NB: 1 KB DMA blocks per wave
+  uint32_t off[NB];
+  int kc[NB];
+  __device__ __forceinline__ void init(int64_t ld, int o0, int omax, int w4, int lane) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int bi = w4 * NB + i;
+      if constexpr (KC) {  // rows past omax are clamped to a valid row (their outputs are never stored)
+        const int row = 8 * bi + (lane >> 3), c = (lane & 7) ^ pswz<PERM>(row);
+        off[i] = (uint32_t)(((int64_t)min(o0 + row, omax - 1) * ld + 8 * c) * 2);
+        kc[i] = 8 * c;
+      } else {
+        constexpr int PER = O / 8;
+        const int q = bi * 64 + lane, k = q / PER, c = (q % PER) ^ (2 * (k & 3));
+        off[i] = step_off(((int64_t)k * ld + min(o0 + 8 * c, omax - 8)) * 2);
+        kc[i] = 0;
+      }
+    }
+  }
+  // block i of this wave; klim = K - k0 of the step: k-contiguous chunks at or past K read zero
+  __device__ __forceinline__ void dma(const i32x4& rs, unsigned char* st, int w4, int i, int klim) const {
+    dma_block(rs, KC ? kmask(off[i], kc[i], klim) : off[i], st + (w4 * NB + i) * 1024);
+  }
+  static __device__ __forceinline__ bf16x8 frag(const unsigned char* st, int o16, int r, int g, int h) {
+    if constexpr (KC) {
+      return frag64<true, PERM>(st, o16, r, g, h);
+    } else {
+      const int kb = 32 * h + 8 * g, col = o16 + 4 * (r & 3), chunk = col >> 3, inner = (col & 7) << 1;
+      bf16x4 hv[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int k = kb + 4 * half + (r >> 2);
+        const unsigned char* p = st + k * (2 * O) + ((chunk ^ (2 * (k & 3))) << 4) + inner;
+        hv[half] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(p));
+      }
+      return bf16x8{hv[0][0], hv[0][1], hv[0][2], hv[0][3], hv[1][0], hv[1][1], hv[1][2], hv[1][3]};
+    }
+  }
+};
+
 // Number of K splits of a product on 256 x 256 tiles (llattn_gemm.hip).
 int resolve_split(const llattn_gemm_desc* d);
 
@@ -233,6 +280,8 @@ int resolve_split(const llattn_gemm_desc* d);
 // (llattn_gemm_tile.hip).
 struct TilePlan { int mb, nb, kg, splits; };
 TilePlan tile_plan(const llattn_gemm_desc* d, double* us = nullptr);  // us: the time it expects
+// llattn_gemm with `b_rows` <= K rows in an m/n-contiguous B: the rows past them read zero (A holds zeros there).
+int32_t product(const llattn_gemm_desc* d, int b_rows, void* workspace, size_t workspace_bytes, hipStream_t st);
 void launch_tile(const GemmArgs& a, const TilePlan& p, bool a_kmaj, bool b_kmaj, int c_dtype, hipStream_t st);
 // Two independent products in one launch: x Wᵀ or dy W into bf16, and then dyᵀ x into fp32 or (after x Wᵀ) another x Wᵀ.
 TilePlan pair_plan(const llattn_gemm_desc* d0, const llattn_gemm_desc* d1);

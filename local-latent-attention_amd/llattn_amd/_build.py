@@ -19,7 +19,7 @@ LIB_NAME = "libllattn_gfx950.so"
 SOURCES = ("llattn_abi.cpp", "llattn_steps.cpp", "llattn_pool.hip", "llattn_latent.hip", "llattn_local.hip", "llattn_local_wide.hip",
            "llattn_gemm.hip", "llattn_gemm_tile.hip", "llattn_gemm_f32.hip",
            "llattn_colsum.hip", "llattn_cast.hip", "llattn_norm.hip",
-           "llattn_xent.hip")
+           "llattn_xent.hip", "llattn_head.hip", "llattn_muon.hip")
 ARCH = "gfx950"
 
 # -packed-fp32-ops off: hipcc must not emit packed fp32 arithmetic for this target.

@@ -8,6 +8,7 @@ on a GPU, the op raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -78,6 +79,18 @@ class LlattnFfnCfg(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("rows", "d", "d_ff", "d_out", "saved")]
 
 
+class LlattnHeadCfg(ctypes.Structure):  # include/llattn_train.h
+    _fields_ = [(n, ctypes.c_int32) for n in ("rows", "V", "D", "piece", "dw_dtype")]
+
+
+MUON_BATCH = 128  # LLATTN_MUON_BATCH
+
+
+class LlattnMuonCfg(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("batch", "rows", "cols", "g_dtype", "w_dtype", "steps", "nesterov")] + \
+        [(n, ctypes.c_float) for n in ("a", "b", "c", "eps", "mu", "keep", "step")]
+
+
 _P = ctypes.c_void_p
 _T = ctypes.POINTER(LlattnTensor)
 _G = ctypes.POINTER(LlattnGemmDesc)
@@ -132,6 +145,17 @@ STEP_SIGNATURES = {
     "llattn_ffn_bwd": (_I32, [_FC, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
 }
 
+# the same for include/llattn_train.h
+_HC, _MC, _PP = ctypes.POINTER(LlattnHeadCfg), ctypes.POINTER(LlattnMuonCfg), ctypes.POINTER(ctypes.c_void_p)
+TRAIN_SIGNATURES = {
+    "llattn_head_bytes": (_SZ, [_HC, _I32]),
+    "llattn_head_fwd": (_I32, [_HC, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "llattn_head_bwd": (_I32, [_HC, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I32, _P, _P, _P, _P, _SZ, _P]),
+    "llattn_muon_bytes": (_SZ, [_MC]),
+    "llattn_orthogonalize": (_I32, [_MC, _PP, _PP, _P, _SZ, _P]),
+    "llattn_muon_update": (_I32, [_MC, _PP, _PP, _PP, _PP, _PP, _P, _SZ, _P]),
+}
+
 _lib = None
 
 
@@ -144,7 +168,7 @@ def load() -> ctypes.CDLL:
         raise RuntimeError(f"llattn HIP library not built ({LIB_PATH} missing); run __graft_entry__.build() "
                            "or `python -m llattn_amd._build` on a machine with ROCm hipcc")
     lib = ctypes.CDLL(str(LIB_PATH))
-    for name, (res, args) in (SIGNATURES | STEP_SIGNATURES).items():
+    for name, (res, args) in (SIGNATURES | STEP_SIGNATURES | TRAIN_SIGNATURES).items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
@@ -177,6 +201,11 @@ def require_gpu(*tensors: torch.Tensor) -> None:
         if t is not None and t.device.type != "cuda":
             raise RuntimeError("llattn runs on MI355X (gfx950) GPUs only; got a tensor on "
                                f"{t.device} (there is no CPU path)")
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one, as launches on its streams need; nothing where it already is."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def stream_ptr(device: torch.device) -> ctypes.c_void_p:

@@ -15,7 +15,7 @@ implementations to compare against.
 (reference train.py:340-370, ``compute_loss_and_metrics`` for [B, T] targets);
 :meth:`LocalLatentLM.loss` computes the same from the hidden states with the
 head and the cross entropy in row chunks (no full logits tensor),
-:func:`make_optimizer` its AdamW set-up (reference train.py:851-859) and
+:func:`make_optimizer` its AdamW set-up (reference train.py:851-859; or Muon for the blocks' matrices) and
 :func:`train_step` one optimiser step as its loop runs it (reference
 train.py:960-1037, one micro-step, gradient clipping, no loss scaling in bf16).
 """
@@ -205,10 +205,17 @@ class LocalLatentLM(nn.Module):
             x, h = add_rms_norm(x, blk.ff(h2), nxt.weight, nxt.eps)
         return h
 
-    def loss(self, input_ids: torch.Tensor, targets: torch.Tensor, chunk_rows: int = 8192):
+    def loss(self, input_ids: torch.Tensor, targets: torch.Tensor, chunk_rows: int = 8192,
+             vocab_piece: Optional[int] = None):
         """:func:`lm_loss` of ``self(input_ids)`` without the ``[B*T, V]`` logits: the tied head and the cross
-        entropy run in row chunks on the gfx950 kernels (:func:`~llattn_amd.xent.lm_head_loss`)."""
-        from .xent import head_supported, lm_head_loss
+        entropy run in row chunks on the gfx950 kernels (:func:`~llattn_amd.xent.lm_head_loss`), or with
+        ``vocab_piece`` in pieces of that many columns of a vocabulary of any size (0: chosen from the sizes;
+        :func:`~llattn_amd.xent.piecewise_head_loss`)."""
+        from .xent import head_supported, lm_head_loss, piecewise_head_loss
+        if vocab_piece is not None:
+            loss, pred = piecewise_head_loss(self.hidden(input_ids), self.lm_head.weight, targets, return_pred=True,
+                                             piece=vocab_piece)
+            return loss, _metrics(loss, (pred == targets).float().mean())
         V, D = self.lm_head.weight.shape
         if not head_supported(V, D):  # vocabularies the chunked kernels do not take: full logits, as the reference
             return lm_loss(self.lm_head(self.hidden(input_ids)), targets)
@@ -239,9 +246,23 @@ def _metrics(loss: torch.Tensor, acc: torch.Tensor) -> dict:
             "eval_bpt": loss_det / math.log(2.0)}
 
 
-def make_optimizer(model: nn.Module, lr: float = 3e-4) -> torch.optim.Optimizer:
+def make_optimizer(model: nn.Module, lr: float = 3e-4, matrices: str = "adamw",
+                   muon_lr: float = 0.02) -> torch.optim.Optimizer:
     """AdamW with weight decay 0.1 on matrices and 0 on vectors, betas (0.9, 0.95), fused on GPU (reference
-    train.py:851-859; default lr of reference train.py:159)."""
+    train.py:851-859; default lr of reference train.py:159).  With ``matrices="muon"`` the blocks' weight matrices
+    are updated by :class:`~llattn_amd.muon.Muon` at ``muon_lr`` (weight decay 0.1) and the rest (embeddings, norms,
+    biases, gate vectors) by AdamW as before."""
+    if matrices not in ("adamw", "muon"):
+        raise ValueError(f"make_optimizer: matrices must be 'adamw' or 'muon', got {matrices!r}")
+    if matrices == "muon":
+        from .muon import MuonAdamW
+        hidden = [p for p in model.blocks.parameters() if p.ndim == 2 and min(p.shape) > 1]
+        taken = {id(p) for p in hidden}
+        rest = [p for p in model.parameters() if id(p) not in taken]
+        return MuonAdamW(hidden, [{"params": [p for p in rest if p.ndim >= 2], "weight_decay": 0.1},
+                                  {"params": [p for p in rest if p.ndim < 2], "weight_decay": 0.0}],
+                         dict(lr=muon_lr, weight_decay=0.1), lr=lr, betas=(0.9, 0.95),
+                         fused=next(model.parameters()).device.type == "cuda")
     decay = [p for p in model.parameters() if p.ndim >= 2]
     no_decay = [p for p in model.parameters() if p.ndim < 2]
     fused = next(model.parameters()).device.type == "cuda"
@@ -250,14 +271,14 @@ def make_optimizer(model: nn.Module, lr: float = 3e-4) -> torch.optim.Optimizer:
 
 
 def train_step(model: nn.Module, optimizer: torch.optim.Optimizer, inputs: torch.Tensor, targets: torch.Tensor,
-               grad_clip: float = 1.0, fused_loss: bool = True) -> torch.Tensor:
+               grad_clip: float = 1.0, fused_loss: bool = True, vocab_piece: Optional[int] = None) -> torch.Tensor:
     """One bf16-autocast optimiser step: forward, loss, backward, gradient clipping, AdamW update, gradients
     cleared (reference train.py:960-1037 with one micro-step).  ``fused_loss``: the chunked head + cross entropy
-    (:meth:`LocalLatentLM.loss`) instead of full logits and ``F.cross_entropy``.  Returns the detached loss (no
-    sync)."""
+    (:meth:`LocalLatentLM.loss`, which ``vocab_piece`` is passed to) instead of full logits and ``F.cross_entropy``.
+    Returns the detached loss (no sync)."""
     with torch.autocast(device_type="cuda", dtype=torch.bfloat16):
         if fused_loss:
-            loss, _ = model.loss(inputs, targets)
+            loss, _ = model.loss(inputs, targets, vocab_piece=vocab_piece)
         else:
             loss, _ = lm_loss(model(inputs), targets)
         loss.backward()

@@ -17,7 +17,11 @@ chunk only.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from . import gemm
@@ -124,3 +128,117 @@ def lm_head_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, i
     if not head_supported(V, D):
         raise ValueError(f"lm_head_loss: V={V} (multiple of 8, at most 65536) and D={D} (multiple of 8) unsupported")
     return _HeadLoss.apply(h, weight, targets, int(ignore_index), int(chunk_rows), torch.is_grad_enabled())
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+REDUCTIONS = ("mean", "sum", "none")
+
+
+def _bf16_rows(t: torch.Tensor, pad: int) -> torch.Tensor:
+    """``t [R, D]`` in bf16 with ``pad`` zero columns behind, rows 16-byte aligned (``t`` itself where it is that)."""
+    t = t.detach().to(torch.bfloat16)
+    if pad:
+        return F.pad(t, (0, pad))
+    if t.stride(1) != 1 or t.stride(0) < t.shape[1] or t.stride(0) % 8 or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+class _PieceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, weight, targets, ignore_index, reduction, want_pred, piece, grad_enabled):
+        D, V, dev = h.shape[-1], weight.shape[0], h.device
+        N, pad = targets.numel(), -D % 8
+        t = targets.reshape(-1).to(torch.int64).contiguous()
+        hb, wb = _bf16_rows(h.reshape(-1, D), pad), _bf16_rows(weight, pad)
+        loss = torch.empty((N,), dtype=torch.float32, device=dev)
+        lse2 = torch.empty((N,), dtype=torch.float32, device=dev)
+        pred = torch.empty((N,), dtype=torch.int32, device=dev) if want_pred else None
+        total = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
+        inv = torch.empty((), dtype=torch.float32, device=dev) if reduction == "mean" else None
+        cfg = L.LlattnHeadCfg(N, V, D + pad, piece, L.F32 if weight.dtype is torch.float32 else L.BF16)
+        if N == 0:
+            if total is not None:
+                total.fill_(0.0 if inv is None else float("nan"))  # the mean of nothing
+        else:
+            n = _head_bytes(cfg, 0)
+            ws = torch.empty((n,), dtype=torch.uint8, device=dev)
+            from .ops import _call
+            with L.on_device(dev):
+                _call("llattn_head_fwd", ctypes.byref(cfg), hb.data_ptr(), hb.stride(0), wb.data_ptr(), wb.stride(0),
+                      t.data_ptr(), ignore_index, loss.data_ptr(), lse2.data_ptr(),
+                      _ptr(pred), _ptr(total), _ptr(inv), ws.data_ptr(), n, L.stream_ptr(dev), work=2 * (N + V) * D)
+        if grad_enabled and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]):
+            ctx.save_for_backward(hb, wb, t, lse2, inv)
+            ctx.meta = (cfg, ignore_index, reduction, tuple(h.shape), h.dtype, tuple(weight.shape), weight.dtype)
+        out = loss.view(targets.shape) if total is None else total
+        if not want_pred:
+            return out
+        pred = pred.view(targets.shape)
+        ctx.mark_non_differentiable(pred)
+        return out, pred
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gl, *_):
+        hb, wb, t, lse2, inv = ctx.saved_tensors
+        cfg, ignore_index, reduction, h_shape, h_dtype, w_shape, w_dtype = ctx.meta
+        dev, N, V, D = hb.device, cfg.rows, cfg.V, w_shape[1]
+        want_h, want_w = ctx.needs_input_grad[:2]
+        if N == 0:
+            return (torch.zeros(h_shape, dtype=h_dtype, device=dev) if want_h else None,
+                    torch.zeros(w_shape, dtype=w_dtype, device=dev) if want_w else None, *[None] * 6)
+        g = gl.to(torch.float32).reshape(-1).contiguous()
+        dh = torch.empty((N, cfg.D), dtype=torch.bfloat16, device=dev) if want_h else None
+        # whole groups of 8 rows: the weight gradient of the last piece is written to the end of its group
+        dw = torch.empty((V + -V % 8, cfg.D), dtype=w_dtype, device=dev) if want_w else None
+        n = _head_bytes(cfg, 1)
+        ws = torch.empty((n,), dtype=torch.uint8, device=dev)
+        from .ops import _call
+        with L.on_device(dev):
+            _call("llattn_head_bwd", ctypes.byref(cfg), hb.data_ptr(), hb.stride(0), wb.data_ptr(), wb.stride(0),
+                  t.data_ptr(), ignore_index, lse2.data_ptr(), g.data_ptr(), int(reduction == "none"),
+                  _ptr(inv), _ptr(dh), _ptr(dw), ws.data_ptr(), n, L.stream_ptr(dev), work=4 * (N + V) * D)
+        return (dh[:, :D].to(h_dtype).reshape(h_shape) if want_h else None, dw[:V, :D] if want_w else None, *[None] * 6)
+
+
+def _head_bytes(cfg, which: int) -> int:
+    n = L.load().llattn_head_bytes(ctypes.byref(cfg), which)
+    if n == 0:
+        L.check(L.ERR_SHAPE, "llattn_head_bytes")
+    return n
+
+
+def piecewise_head_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = IGNORE_INDEX,
+                        reduction: str = "mean", return_pred: bool = False, piece: int = 0):
+    """Cross entropy of ``h [..., D] @ weight [V, D]^T`` against ``targets [...]`` for a vocabulary of any size, without
+    keeping logits: the forward keeps a sum per row, the backward computes the logits again in pieces of ``piece``
+    columns (a multiple of 256; 0: as many as keep a piece within 512 MB).
+
+    ``reduction``: ``"mean"`` over the rows whose target is not ``ignore_index`` (NaN when there are none, with zero
+    gradients), ``"sum"``, or ``"none"`` (fp32, ``targets``' shape, 0 in ignored rows).  A target outside ``[0, V)``
+    gives NaN.  With ``return_pred`` also the first argmax of every row (int32).  ``h`` and ``weight`` are bf16 or fp32,
+    fp32 ones rounded to bf16 as under autocast; logits, sums and losses are fp32 and gradients come in their input's
+    type, ``weight``'s accumulated in fp32.  Differentiable once.  GPU only."""
+    if h.dim() < 1 or weight.dim() != 2 or weight.shape[1] != h.shape[-1] or 0 in weight.shape:
+        raise ValueError(f"piecewise_head_loss: weight {tuple(weight.shape)} does not match hidden states {tuple(h.shape)}")
+    if targets.shape != h.shape[:-1]:
+        raise ValueError(f"piecewise_head_loss: targets {tuple(targets.shape)} for hidden states {tuple(h.shape)}")
+    if targets.is_floating_point() or targets.is_complex() or targets.dtype is torch.bool:
+        raise ValueError(f"piecewise_head_loss: targets must be integers, got {targets.dtype}")
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"piecewise_head_loss: reduction must be one of {REDUCTIONS}, got {reduction!r}")
+    for t in (h, weight):
+        L.dtype_code(t.dtype)
+    if piece < 0 or piece % 256:
+        raise ValueError(f"piecewise_head_loss: piece must be 0 or a multiple of 256, got {piece}")
+    L.require_gpu(h, weight, targets)
+    if not h.device == weight.device == targets.device:
+        raise ValueError(f"piecewise_head_loss: tensors on {h.device}, {weight.device} and {targets.device}")
+    return _PieceLoss.apply(h, weight, targets, int(ignore_index), reduction, bool(return_pred), int(piece),
+                            torch.is_grad_enabled())

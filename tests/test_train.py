@@ -1,0 +1,167 @@
+"""CPU tests of the head loss and the weight update: the C interface (include/llattn_train.h), and what is refused before
+anything is launched."""
+import ctypes
+import re
+import subprocess
+
+import pytest
+import torch
+
+from conftest import REPO
+from llattn_amd import _lib as L
+from llattn_amd import muon
+from llattn_amd.lm import build_model, make_optimizer
+from llattn_amd.xent import piecewise_head_loss
+
+BF16 = torch.bfloat16
+
+
+def test_header_matches_the_binding(tmp_path):
+    text = (REPO / "include" / "llattn_train.h").read_text()
+    names = set(re.findall(r"^\s*(?:int32_t|size_t)\s+(llattn_\w+)\s*\(", text, re.M))
+    assert names == set(L.TRAIN_SIGNATURES) and all(hasattr(L.load(), n) for n in names)
+    structs = {"llattn_head_cfg": L.LlattnHeadCfg, "llattn_muon_cfg": L.LlattnMuonCfg}
+    lines = ["#include <stddef.h>", "#include <stdio.h>", '#include "llattn_train.h"', "int main(void) {"]
+    for c, t in structs.items():
+        lines.append(f'printf("%zu\\n", sizeof({c}));')
+        lines += [f'printf("%zu\\n", offsetof({c}, {f[0]}));' for f in t._fields_]
+    lines += ['printf("%d\\n", LLATTN_MUON_BATCH);', "return 0; }"]
+    src = tmp_path / "l.c"
+    src.write_text("\n".join(lines))
+    subprocess.run(["gcc", f"-I{REPO / 'include'}", str(src), "-o", str(tmp_path / "l")], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "l")], capture_output=True, text=True, check=True).stdout.split()]
+    want = []
+    for t in structs.values():
+        want.append(ctypes.sizeof(t))
+        want += [getattr(t, f[0]).offset for f in t._fields_]
+    assert got == want + [L.MUON_BATCH]
+
+
+@pytest.mark.parametrize("cfg,which", [((0, 10, 8, 0, 0), 0), ((4, 0, 8, 0, 0), 0), ((4, 10, 0, 0, 0), 0), ((4, 10, 12, 0, 0), 1),
+                                       ((4, 10, 8, 100, 0), 1), ((4, 10, 8, -256, 0), 1), ((4, 10, 8, 0, 7), 1),
+                                       ((4, 10, 8, 0, 0), 2)])
+def test_head_sizes_refused(cfg, which):
+    assert L.load().llattn_head_bytes(ctypes.byref(L.LlattnHeadCfg(*cfg)), which) == 0
+    assert L.load().llattn_last_error()
+
+
+def test_head_workspace_stays_bounded():
+    """Row sums of a forward over any vocabulary within 512 MB or a few columns a row; a piece of the backward within
+    512 MB (or 256 columns), whatever the vocabulary."""
+    n = L.load().llattn_head_bytes
+    assert 0 < n(ctypes.byref(L.LlattnHeadCfg(8192, 2 ** 31 - 257, 64, 0, 0)), 0) < 512 << 20
+    # beside the piece: the sum of dh in fp32, and its product's partial sums (192 tiles of 256 x 256: four k splits)
+    assert n(ctypes.byref(L.LlattnHeadCfg(8192, 131072, 1536, 0, 1)), 1) <= (512 << 20) + 5 * 8192 * 1536 * 4 + 1024
+
+
+def _head_fwd(rows=4, V=10, D=8, h=1 << 20, ldh=8, w=1 << 20, ldw=8, t=1 << 20, loss=1 << 20, lse=1 << 20, total=None, inv=None,
+              ws=1 << 20, n=1 << 30):
+    p = lambda v: None if not v else ctypes.c_void_p(v)  # noqa: E731
+    cfg = L.LlattnHeadCfg(rows, V, D, 0, 0)
+    return L.load().llattn_head_fwd(ctypes.byref(cfg), p(h), ldh, p(w), ldw, p(t), -100, p(loss), p(lse), None, p(total), p(inv),
+                                    p(ws), n, None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(h=0), L.ERR_LAYOUT), (dict(w=0), L.ERR_LAYOUT), (dict(t=0), L.ERR_LAYOUT), (dict(loss=0), L.ERR_LAYOUT),
+    (dict(lse=0), L.ERR_LAYOUT), (dict(inv=1 << 20), L.ERR_LAYOUT), (dict(ldh=4), L.ERR_LAYOUT), (dict(ldw=12), L.ERR_LAYOUT),
+    (dict(h=(1 << 20) + 2), L.ERR_LAYOUT), (dict(ldw=1 << 23), L.ERR_LAYOUT), (dict(ws=0), L.ERR_WORKSPACE), (dict(n=1), L.ERR_WORKSPACE),
+    (dict(D=9), L.ERR_SHAPE)])
+def test_head_forward_refused(kw, code):
+    assert _head_fwd(**kw) == code
+
+
+def test_head_backward_refused():
+    lib, cfg = L.load(), L.LlattnHeadCfg(4, 10, 8, 0, 0)
+    p = ctypes.c_void_p
+    def call(lse=1 << 20, grad=1 << 20, stride=0, dh=1 << 20, ws=1 << 20):
+        return lib.llattn_head_bwd(ctypes.byref(cfg), p(1 << 20), 8, p(1 << 20), 8, p(1 << 20), -100, p(lse), p(grad), stride, None,
+                                   p(dh), None, p(ws), 1 << 30, None)
+    assert call(lse=0) == call(grad=0) == call(stride=2) == call(stride=-1) == call(dh=(1 << 20) + 4) == L.ERR_LAYOUT
+    assert call(ws=0) == L.ERR_WORKSPACE
+
+
+def test_piecewise_head_loss_refusals():
+    h, w, t = torch.zeros(4, 8, dtype=BF16), torch.zeros(10, 8, dtype=BF16), torch.zeros(4, dtype=torch.int64)
+    bad = [dict(h=torch.zeros(4, 16, dtype=BF16)), dict(weight=w[0]), dict(weight=torch.zeros(0, 8, dtype=BF16)), dict(targets=t[:3]),
+           dict(targets=t.float()), dict(targets=t.bool()), dict(reduction="avg"), dict(h=h.half()), dict(weight=w.double()),
+           dict(piece=100), dict(piece=-256)]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            piecewise_head_loss(**{**dict(h=h, weight=w, targets=t), **kw})
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        piecewise_head_loss(h, w, t)
+
+
+GOOD = dict(batch=1, rows=4, cols=8, g_dtype=0, w_dtype=0, steps=5, nesterov=1, a=3.4445, b=-4.775, c=2.0315, eps=1e-7, mu=0.95,
+            keep=1.0, step=0.1)
+
+
+@pytest.mark.parametrize("kw", [dict(batch=0), dict(batch=129), dict(rows=0), dict(cols=-1), dict(rows=32769), dict(g_dtype=2),
+                                dict(w_dtype=-1), dict(steps=0), dict(steps=101), dict(eps=-1.0), dict(eps=float("nan")),
+                                dict(a=5.0), dict(a=2.0, b=0.0, c=0.0), dict(b=-20.0), dict(c=float("nan"))])
+def test_muon_configurations_refused(kw):
+    lib = L.load()
+    assert lib.llattn_muon_bytes(ctypes.byref(L.LlattnMuonCfg(*GOOD.values()))) > 0
+    assert lib.llattn_muon_bytes(ctypes.byref(L.LlattnMuonCfg(*{**GOOD, **kw}.values()))) == 0
+    assert b"llattn_muon" in lib.llattn_last_error()
+
+
+def test_muon_calls_refused():
+    lib, cfg, p = L.load(), L.LlattnMuonCfg(*GOOD.values()), ctypes.c_void_p
+    one, odd, none = (muon._pointers([v]) for v in (1 << 20, (1 << 20) + 2, None))
+    ref = ctypes.byref(cfg)
+    assert lib.llattn_orthogonalize(ref, one, one, None, 1 << 30, None) == L.ERR_WORKSPACE
+    assert lib.llattn_orthogonalize(ref, one, one, p(1 << 20), 16, None) == L.ERR_WORKSPACE
+    for g, o in ((none, one), (one, none), (odd, one), (one, odd), (None, one), (one, None)):
+        assert lib.llattn_orthogonalize(ref, g, o, p(1 << 20), 1 << 40, None) == L.ERR_LAYOUT
+    for k in range(5):
+        for v in (none, odd, None):
+            args = [one] * 5
+            args[k] = v
+            assert lib.llattn_muon_update(ref, *args, p(1 << 20), 1 << 40, None) == L.ERR_LAYOUT
+    bad = L.LlattnMuonCfg(*{**GOOD, "mu": 1.0}.values())
+    assert lib.llattn_muon_update(ctypes.byref(bad), *[one] * 5, p(1 << 20), 1 << 40, None) == L.ERR_SHAPE
+
+
+def test_orthogonalize_refusals():
+    x = torch.zeros(3, 4)
+    for args, kw in (((x[0],), {}), ((x.half(),), {}), ((x,), dict(steps=0)), ((x,), dict(steps=2.5)), ((x,), dict(eps=-1.0)),
+                     ((x,), dict(coefficients=(1.0, 2.0))), ((x.clone().requires_grad_(True),), {})):
+        with pytest.raises(ValueError):
+            muon.orthogonalize(*args, **kw)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        muon.orthogonalize(x)
+
+
+def test_muon_update_refusals():
+    w, g, m = torch.zeros(4, 6), torch.zeros(4, 6), torch.zeros(4, 6)
+    other = torch.zeros(4, 6)
+    bad = [(([w], [g], []), {}), (([w[0]], [g[0]], [m[0]]), {}), (([w.half()], [g], [m]), {}), (([w], [g.t()], [m]), {}),
+           (([w], [g], [m.to(BF16)]), {}), (([w.t()], [g.t()], [m.t()]), {}), (([w, w], [g, g], [m, other]), {}),
+           (([w], [g], [w]), {}), (([w], [w], [m]), {}), (([w, other], [g, g], [m, other.clone()]), dict(out=([other, w], [m, g.clone()]))),
+           (([w], [g], [m]), dict(out=([other],))), (([w], [g], [m]), dict(out=([other.to(BF16)], [m]))),
+           (([w], [g], [m]), dict(lr=torch.tensor(0.1))), (([w], [g], [m]), dict(momentum=1.0)), (([w], [g], [m]), dict(scale="none")),
+           (([w], [g], [m]), dict(steps=-1)), ((torch.zeros(1, 0, 4), torch.zeros(1, 0, 4), torch.zeros(1, 0, 4)), {})]
+    for args, kw in bad:
+        with pytest.raises(ValueError):
+            muon.muon_update(*args, **{"lr": 0.1, **kw})
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        muon.muon_update([w], [g], [m], lr=0.1)
+    muon.muon_update([], [], [], lr=0.1)
+
+
+def test_optimisers_refuse_vectors_and_unknown_choices():
+    with pytest.raises(ValueError):
+        muon.Muon([torch.nn.Parameter(torch.zeros(3))])
+    with pytest.raises(ValueError):
+        muon.Muon([torch.nn.Parameter(torch.zeros(3, 4))], scale="max")
+    model = build_model(vocab_size=32, max_seq_len=16, d_model=16, n_heads=2, n_layers=2, d_ff=32, latent_d_model=8, latent_heads=2)
+    with pytest.raises(ValueError):
+        make_optimizer(model, matrices="sgd")
+    opt = make_optimizer(model, matrices="muon")
+    mats = {id(p) for p in opt.param_groups[0]["params"]}
+    names = {n for n, p in model.named_parameters() if id(p) in mats}
+    assert len(names) == 2 * 7 and not any("embedding" in n or "position" in n or "gate" in n for n in names)
+    assert sum(len(g["params"]) for g in opt.param_groups) == len(list(model.parameters()))
+    assert isinstance(make_optimizer(model), torch.optim.AdamW)
