@@ -59,35 +59,45 @@ int32_t llattn_head_bwd(const llattn_head_cfg* cfg, const void* h, int64_t ldh, 
  * halves with fp32 accumulation, so results are as near to the exact ones as
  * fp32 products' are.  Fixed order of every sum (no atomics).
  *
- * llattn_orthogonalize: out[i] = ns(g[i]) for i < batch, rows contiguous, type
- * g_dtype in, w_dtype out.
- * llattn_muon_update: one optimiser step of batch equally shaped weights,
+ * Matrices come in groups of one shape and type (at most LLATTN_MUON_GROUPS a
+ * call, LLATTN_MUON_BATCH matrices, of at most 32768 rows and columns); all of
+ * them share the launches of the call.  Rows are contiguous.
+ *
+ * llattn_orthogonalize: out[i] = ns(g[i]), g_dtype in, w_dtype out.
+ * llattn_muon_update: one optimiser step,
  *   m_out = mu m + (1 - mu) g,  U = nesterov ? (1 - mu) g + mu m_out : m_out,
  *   w_out = keep w - step ns(U)
  * with g in g_dtype, m fp32, w in w_dtype; m_out may be m and w_out may be w
  * (the same arrays), nothing else may overlap.
  *
- * g, m, w, ... are host arrays of `batch` device pointers, read during the
- * call.  At most LLATTN_MUON_BATCH matrices a call, of at most 32768 rows and
- * columns.  a, b, c must keep singular values in [0, 1] below 3.8 and |b s^2 +
- * c s^4| below 15 over the steps (what the halves hold). */
+ * g, m, w, ... are host arrays of device pointers, the groups' matrices in
+ * order, read during the call.  a, b, c must keep singular values in [0, 1]
+ * below 3.8 and |b s^2 + c s^4| below 15 over the steps (what the halves hold). */
 #define LLATTN_MUON_BATCH 128
+#define LLATTN_MUON_GROUPS 16
 
-typedef struct llattn_muon_cfg {
+typedef struct llattn_muon_group {
   int32_t batch, rows, cols;
   int32_t g_dtype, w_dtype; /* LLATTN_F32 or LLATTN_BF16 */
+  float keep, step;         /* llattn_muon_update */
+} llattn_muon_group;
+
+typedef struct llattn_muon_cfg {
+  int32_t n_groups;
   int32_t steps, nesterov;
+  int32_t tiles; /* of the products: 0: chosen from the sizes, 1: 64 x 64, 2: 64 x 64 in two k groups, 3: 128 x 128,
+                    4: 256 x 256 (small matrices in one workgroup each: with 0 only) */
   float a, b, c, eps;
-  float mu, keep, step; /* llattn_muon_update */
+  float mu; /* llattn_muon_update */
 } llattn_muon_cfg;
 
 /* Workspace bytes of either call; 0 with an error message on a bad configuration. */
-size_t llattn_muon_bytes(const llattn_muon_cfg* cfg);
-int32_t llattn_orthogonalize(const llattn_muon_cfg* cfg, const void* const* g, void* const* out, void* workspace,
-                             size_t workspace_bytes, void* stream);
-int32_t llattn_muon_update(const llattn_muon_cfg* cfg, const void* const* g, const float* const* m, const void* const* w,
-                           float* const* m_out, void* const* w_out, void* workspace, size_t workspace_bytes,
-                           void* stream);
+size_t llattn_muon_bytes(const llattn_muon_cfg* cfg, const llattn_muon_group* groups);
+int32_t llattn_orthogonalize(const llattn_muon_cfg* cfg, const llattn_muon_group* groups, const void* const* g,
+                             void* const* out, void* workspace, size_t workspace_bytes, void* stream);
+int32_t llattn_muon_update(const llattn_muon_cfg* cfg, const llattn_muon_group* groups, const void* const* g,
+                           const float* const* m, const void* const* w, float* const* m_out, void* const* w_out,
+                           void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -14,9 +14,12 @@
 //
 // Storage: a row holds, for each block of 32 columns, its 32 hi and then its 32 lo halves: 128 bytes, one cache line.
 // A k step of 32 is then laid out like a 64-k step of the bf16 products, and their loads and fragment reads serve.
-// Rows and columns are padded to whole tiles with zeros, which the iteration keeps, so the loops know no edges.
+// Rows and columns are padded to multiples of 64 with zeros, which the iteration keeps; rows of a tile past them are past
+// the operand's extent and read zero.
 //
-// A and B are symmetric: tiles on and above the diagonal are computed and written to both sides.
+// A and B are symmetric: blocks on and above the diagonal are computed and written to both sides.
+//
+// Matrices of several shapes share a launch: workgroups find their group, matrix and tile.
 #include <algorithm>
 #include <cmath>
 
@@ -33,6 +36,15 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kSA = 4096.f;  // scale of A and B
 
+// f(integral_constant 0), f(1), ..., f(N - 1)
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void unroll(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    unroll<N, I + 1>(f);
+  }
+}
+
 template <typename P>
 struct Table { P p[LLATTN_MUON_BATCH]; };
 
@@ -41,15 +53,36 @@ __device__ __forceinline__ float load_as(const void* p, int64_t i, int dtype) {
 }
 
 // ---- momentum and |U|^2 -----------------------------------------------------------
-struct PrepArgs {
+// A group's share of a launch over elements: workgroups [b0, b0 + batch blocks), `blocks` a matrix.
+struct ElemGroup {
+  int b0, blocks, first, rows, cols, flip, g_dtype, mp, np;
+  float scale;
+  int64_t x_off;   // of the group's first X
+  int part0;       // of its first partial sum
+  int parts;       // partial sums a matrix
+};
+struct ElemArgs {
   Table<const void*> g;
   Table<const float*> m;
-  Table<float*> m_out;
-  int64_t n;       // elements of a matrix
-  int g_dtype, momentum, nesterov, blocks;
-  float mu, one_mu;
-  double* part;    // [batch][blocks]
+  int n_groups, momentum, nesterov;
+  float mu, one_mu, eps;
+  double* part;
+  uint16_t* x;
+  ElemGroup grp[LLATTN_MUON_GROUPS];
 };
+struct PrepArgs {
+  ElemArgs e;
+  Table<float*> m_out;
+};
+
+static_assert(sizeof(PrepArgs) <= 4096, "kernel arguments");
+
+template <typename G>
+__device__ __forceinline__ const G& group_of(const G* g, int n, int block) {
+  int i = 0;
+  while (i + 1 < n && block >= g[i + 1].b0) ++i;
+  return g[i];
+}
 
 __device__ __forceinline__ float direction(float g, float m, float mu, float one_mu, int nesterov) {
   return nesterov ? fmaf(mu, m, one_mu * g) : m;
@@ -66,16 +99,43 @@ __device__ __forceinline__ double block_sum(double v, double* s) {
   return s[0];
 }
 
+__device__ __forceinline__ bool by4(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == LLATTN_F32 ? 15u : 7u)) == 0; }
+__device__ __forceinline__ void load4_as(const void* p, int64_t i, int dtype, float v[4]) {
+  if (dtype == LLATTN_F32) load4<float>(static_cast<const float*>(p) + i, v);
+  else load4<uint16_t>(static_cast<const uint16_t*>(p) + i, v);
+}
+
 // m_out = mu m + (1 - mu) g and the workgroup's share of |U|^2, in 64 bits (any fp32 values, squares included).
-__global__ __launch_bounds__(256) void muon_prep_kernel(const PrepArgs a) {
+__global__ __launch_bounds__(256) void muon_prep_kernel(const PrepArgs pa) {
   __shared__ double s[256];
-  const int b = blockIdx.y;
-  const void* g = a.g.p[b];
-  const float* m = a.m.p[b];
-  float* mo = a.m_out.p[b];
+  const ElemArgs& a = pa.e;
+  const ElemGroup& G = group_of(a.grp, a.n_groups, blockIdx.x);
+  const int at = blockIdx.x - G.b0, mat = at / G.blocks, blk = at % G.blocks, id = G.first + mat;
+  const void* g = a.g.p[id];
+  const float* m = a.m.p[id];
+  float* mo = pa.m_out.p[id];
+  const int64_t n = (int64_t)G.rows * G.cols, quads = n / 4;
+  const bool vec = by4(g, G.g_dtype) && (!a.momentum || (by4(m, LLATTN_F32) && by4(mo, LLATTN_F32)));
+  const int64_t q_end = vec ? quads : 0, stride = (int64_t)G.blocks * 256;
   double sum = 0.0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.n; i += (int64_t)a.blocks * 256) {
-    float u = load_as(g, i, a.g_dtype);
+  for (int64_t q = (int64_t)blk * 256 + threadIdx.x; q < q_end; q += stride) {
+    float u[4];
+    load4_as(g, 4 * q, G.g_dtype, u);
+    if (a.momentum) {
+      float v[4];
+      load4<float>(m + 4 * q, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = fmaf(a.mu, v[e], a.one_mu * u[e]);
+        u[e] = direction(u[e], v[e], a.mu, a.one_mu, a.nesterov);
+      }
+      store4<float>(mo + 4 * q, v);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum += (double)u[e] * (double)u[e];
+  }
+  for (int64_t i = 4 * q_end + (int64_t)blk * 256 + threadIdx.x; i < n; i += stride) {
+    float u = load_as(g, i, G.g_dtype);
     if (a.momentum) {
       const float v = fmaf(a.mu, m[i], a.one_mu * u);
       mo[i] = v;
@@ -84,20 +144,10 @@ __global__ __launch_bounds__(256) void muon_prep_kernel(const PrepArgs a) {
     sum += (double)u * (double)u;
   }
   sum = block_sum(sum, s);
-  if (threadIdx.x == 0) a.part[(int64_t)b * a.blocks + blockIdx.x] = sum;
+  if (threadIdx.x == 0) a.part[G.part0 + mat * G.parts + blk] = sum;
 }
 
 // ---- X = U / (|U| + eps) as halves, transposed if rows > cols -----------------------
-struct SplitArgs {
-  Table<const void*> g;
-  Table<const float*> m;   // the new momentum
-  int rows, cols, flip, g_dtype, momentum, nesterov, blocks;
-  float mu, one_mu, eps, scale;
-  const double* part;
-  uint16_t* x; int64_t ld, batch_stride;  // 16-bit elements
-  int mp, np;
-};
-
 __device__ __forceinline__ uint16_t h_bits(float v) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v)); }
 __device__ __forceinline__ float h_val(uint16_t v) { return static_cast<float>(__builtin_bit_cast(_Float16, v)); }
 
@@ -115,238 +165,720 @@ __device__ __forceinline__ void store_halves4(uint16_t* row, int c, const float 
   *reinterpret_cast<uint2*>(p) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
   *reinterpret_cast<uint2*>(p + 32) = make_uint2(l[0] | (uint32_t)l[1] << 16, l[2] | (uint32_t)l[3] << 16);
 }
-__device__ __forceinline__ void load_halves4(const uint16_t* row, int c, float v[4]) {
-  const uint16_t* p = row + hi_at(c);
-  const f16x4 h = *reinterpret_cast<const f16x4*>(p), l = *reinterpret_cast<const f16x4*>(p + 32);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = (float)h[e] + (float)l[e];
-}
-
-// One 64 x 64 tile of X per workgroup, through LDS (the reads run along U's rows either way).
-__global__ __launch_bounds__(256) void muon_split_kernel(const SplitArgs a) {
+// One 64 x 64 tile of X per workgroup, through LDS (the reads run along U's rows either way).  a.m: the new momentum.
+__global__ __launch_bounds__(256) void muon_split_kernel(const ElemArgs a) {
   __shared__ double s[256];
   __shared__ float tile[64][65];
-  const int b = blockIdx.y, tn = a.np / 64, r0 = blockIdx.x / tn * 64, c0 = blockIdx.x % tn * 64;
+  const ElemGroup& G = group_of(a.grp, a.n_groups, blockIdx.x);
+  const int at = blockIdx.x - G.b0, mat = at / G.blocks, blk = at % G.blocks, id = G.first + mat;
+  const int tn = G.np / 64, r0 = blk / tn * 64, c0 = blk % tn * 64;
   double sum = 0.0;
-  for (int i = threadIdx.x; i < a.blocks; i += 256) sum += a.part[(int64_t)b * a.blocks + i];
-  const double f = (double)a.scale / (sqrt(block_sum(sum, s)) + (double)a.eps);
-  const void* g = a.g.p[b];
-  const float* m = a.m.p[b];
-  const int u0 = a.flip ? c0 : r0, v0 = a.flip ? r0 : c0;  // the tile's origin in U
-  for (int q = threadIdx.x; q < 4096; q += 256) {
-    const int lr = q >> 6, lc = q & 63, r = u0 + lr, c = v0 + lc;
-    float u = 0.f;
-    if (r < a.rows && c < a.cols) {
-      const int64_t i = (int64_t)r * a.cols + c;
-      u = load_as(g, i, a.g_dtype);
-      if (a.momentum) u = direction(u, m[i], a.mu, a.one_mu, a.nesterov);
-      u = (float)((double)u * f);
+  for (int i = threadIdx.x; i < G.parts; i += 256) sum += a.part[G.part0 + mat * G.parts + i];
+  const double f = (double)G.scale / (sqrt(block_sum(sum, s)) + (double)a.eps);
+  const void* g = a.g.p[id];
+  const float* m = a.m.p[id];
+  const int u0 = G.flip ? c0 : r0, v0 = G.flip ? r0 : c0;  // the tile's origin in U
+  const bool vec = G.cols % 4 == 0 && by4(g, G.g_dtype) && (!a.momentum || by4(m, LLATTN_F32));
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int q = threadIdx.x + 256 * k, lr = q >> 4, lc = (q & 15) * 4, r = u0 + lr, c = v0 + lc;
+    float u[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
+    const int64_t i = (int64_t)r * G.cols + c;
+    if (r < G.rows && vec) {
+      if (c < G.cols) {
+        load4_as(g, i, G.g_dtype, u);
+        if (a.momentum) load4<float>(m + i, v);
+      }
+    } else if (r < G.rows) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (c + e >= G.cols) continue;
+        u[e] = load_as(g, i + e, G.g_dtype);
+        if (a.momentum) v[e] = m[i + e];
+      }
     }
-    tile[lr][lc] = u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (a.momentum) u[e] = direction(u[e], v[e], a.mu, a.one_mu, a.nesterov);
+      tile[lr][lc + e] = r < G.rows && c + e < G.cols ? (float)((double)u[e] * f) : 0.f;  // eps 0: f may be infinite
+    }
   }
   __syncthreads();
-  uint16_t* x = a.x + b * a.batch_stride;
-  for (int q = threadIdx.x; q < 1024; q += 256) {
-    const int lr = q >> 4, lc = (q & 15) * 4;
+  const int64_t ld = 2 * (int64_t)G.np;
+  uint16_t* x = a.x + G.x_off + mat * G.mp * ld;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int q = threadIdx.x + 256 * k, lr = q >> 4, lc = (q & 15) * 4;
     float v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = a.flip ? tile[lc + e][lr] : tile[lr][lc + e];
-    store_halves4(x + (int64_t)(r0 + lr) * a.ld, c0 + lc, v);
+    for (int e = 0; e < 4; ++e) v[e] = G.flip ? tile[lc + e][lr] : tile[lr][lc + e];
+    store_halves4(x + (r0 + lr) * ld, c0 + lc, v);
   }
 }
 
 // ---- the products -------------------------------------------------------------------
 enum NsMode { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3 };
 
+// A group's share of a launch over tiles: workgroups [b0, b0 + count), then padding to a multiple of 8 (the XCDs).
+struct TileGroup {
+  int b0, count, tiles, tiles_n;  // tiles a matrix, tile columns
+  int steps;                      // of 32 k
+  int mp, np, first, rows, cols, w_dtype;
+  int64_t x_off, a_off;           // of the group's first X and A
+  float alpha, beta;              // C = alpha D + beta (products), in stored scales
+  float keep, step;               // LAST
+};
 struct NsArgs {
-  const uint16_t* A; int64_t lda, a_stride;  // rows of the tile, k along them
-  const uint16_t* B; int64_t ldb, b_stride;  // GRAM, POLY: rows = columns of the tile; APPLY, LAST: rows = k
-  const uint16_t* D; int64_t ldd, d_stride;  // POLY: A; APPLY, LAST: X
-  uint16_t* C; int64_t ldc, c_stride;
-  int steps;                                 // of 32 k
-  int tiles, tiles_n;                        // of one matrix; GRAM, POLY: of the upper triangle, and its side
-  float alpha, beta;                         // C = alpha D + beta (products), in stored scales
-  // LAST
-  int rows, cols, flip, w_dtype, update;
-  float keep, step;
+  const uint16_t* x;   // X
+  uint16_t* y;         // the next X (APPLY)
+  uint16_t *a, *b;     // A, B
+  int n_groups, update;
+  TileGroup grp[LLATTN_MUON_GROUPS];
+};
+struct LastArgs {
+  NsArgs n;
   Table<const void*> w;
   Table<void*> out;
 };
 
-// k-major operand of a step: 32 k-rows of T columns (4 T bytes each); chunk c (16 bytes) of k-row k at c ^ 2 (k & 3).
-template <int T>
-struct ColOp {
-  static constexpr int BYTES = T * 128, NB = BYTES / 1024 / 4, PER = T / 4;
-  uint32_t off[NB];
-  __device__ __forceinline__ void init(int64_t ld, int w4, int lane) {
+static_assert(sizeof(LastArgs) <= 4096, "kernel arguments");
+
+// One wave's copy of 64 x 16 bytes into the 1 KB LDS block at byte address lds + AT (buffer_load ... lds, as dma_block).
+template <int AT>
+__device__ __forceinline__ void dma_at(const i32x4& rs, uint32_t off, uint32_t lds) {
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+               :
+               : "v"(off), "s"(rs), "s"(lds), "i"(AT)
+               : "memory", "m0", "scc");
+}
+
+// T rows of a step with k along them (128 bytes each: 32 hi, 32 lo), loaded by W waves.  Chunk c of row o at c ^ (o & 7).
+template <int T, int W>
+struct RowOp {
+  static constexpr int BYTES = T * 128, LOADS = BYTES / 1024 / W;
+  uint32_t off[LOADS], base[2];  // base: of this lane's fragments, hi and lo
+  __device__ __forceinline__ void init(int64_t ld, int w, int lane, int o0) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int q = (w4 * NB + i) * 64 + lane, k = q / PER, c = (q % PER) ^ (2 * (k & 3));
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = 8 * (w * LOADS + i) + (lane >> 3);
+      off[i] = (uint32_t)((int64_t)row * ld * 2 + 16 * ((lane & 7) ^ (row & 7)));
+    }
+    const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) base[h] = (o0 + r) * 128 + (((4 * h + g) ^ (r & 7)) << 4);
+  }
+  // rows o0 + 16 i + r, k 8 g .. 8 g + 7 of the stage at st
+  __device__ __forceinline__ f16x8 frag(const unsigned char* st, int i, int half) const {
+    return *reinterpret_cast<const f16x8*>(st + base[half] + i * 2048);
+  }
+};
+
+// 32 rows of a step, T columns of them (4 T bytes each).  Chunk c of k-row k at c ^ 2 (k & 3).
+template <int T, int W>
+struct ColOp {
+  static constexpr int BYTES = T * 128, LOADS = BYTES / 1024 / W, PER = T / 4;
+  uint32_t off[LOADS], base[4];  // base: by half and the parity of the 16-column block
+  __device__ __forceinline__ void init(int64_t ld, int w, int lane, int o0) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int q = (w * LOADS + i) * 64 + lane, k = q / PER, c = (q % PER) ^ (2 * (k & 3));
       off[i] = (uint32_t)((int64_t)k * ld * 2 + 16 * c);
     }
+    // transposing reads: the 16 lanes of group g supply k-rows 8 g + r / 4 (and 4 further), 8 bytes at column 4 (r % 4)
+    const int r = lane & 15, g = lane >> 4, k = 8 * g + (r >> 2);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int byte = (o0 >> 5) * 128 + (u >> 1) * 64 + (u & 1) * 32 + 8 * (r & 3);
+      base[u] = k * (4 * T) + (((byte >> 4) ^ (2 * (k & 3))) << 4) + (byte & 15);
+    }
   }
-  __device__ __forceinline__ void dma(const i32x4& rs, unsigned char* st, int w4, int i) const {
-    dma_block(rs, off[i], st + (w4 * NB + i) * 1024);
-  }
-  // columns o16 + r, k 8 g .. 8 g + 7; half 0: hi, 1: lo
-  static __device__ __forceinline__ f16x8 frag(const unsigned char* st, int o16, int r, int g, int half) {
-    const int byte = (o16 >> 5) * 128 + half * 64 + (o16 & 31) * 2 + 8 * (r & 3), chunk = byte >> 4, inner = byte & 15;
+  // columns o0 + 16 j + r (o0 a multiple of 32), k 8 g .. 8 g + 7
+  __device__ __forceinline__ f16x8 frag(const unsigned char* st, int j, int half) const {
+    const unsigned char* p = st + base[2 * half + (j & 1)] + (j >> 1) * 128;
     bf16x4 hv[2];
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int k = 8 * g + 4 * q + (r >> 2);
-      const unsigned char* p = st + k * (4 * T) + ((chunk ^ (2 * (k & 3))) << 4) + inner;
-      hv[q] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(p));
-    }
+    for (int q = 0; q < 2; ++q)
+      hv[q] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(p + q * 16 * T));
     return __builtin_bit_cast(f16x8, bf16x8{hv[0][0], hv[0][1], hv[0][2], hv[0][3], hv[1][0], hv[1][1], hv[1][2], hv[1][3]});
   }
 };
 
-// T x T tiles, four waves (2 x 2), NST stages of 32 k, loads NST - 1 steps ahead, one barrier a step (as in
-// llattn_gemm_tile.hip).
-template <int MODE, int T, int NST>
-__global__ __launch_bounds__(256) void ns_kernel(const NsArgs a) {
-  constexpr bool SYM = MODE == GRAM || MODE == POLY;
-  constexpr int NBK = T / 32;  // 16 x 16 blocks of a wave per side
-  typedef TileOp<true, false, T> OpA;
-  typedef std::conditional_t<SYM, OpA, ColOp<T>> OpB;
-  constexpr int STAGE = OpA::BYTES + OpB::BYTES, LOADS = OpA::NB + OpB::NB;
-  __shared__ __align__(1024) unsigned char smem[NST * STAGE];
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
-  const int v = xcd_remap(blockIdx.x, gridDim.x), b = v / a.tiles, t = v % a.tiles;
-  int tm, tn;
-  if constexpr (SYM) {  // t = tn (tn + 1) / 2 + tm, tm <= tn
-    tn = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-    while (tn * (tn + 1) / 2 > t) --tn;
-    while ((tn + 1) * (tn + 2) / 2 <= t) ++tn;
-    tm = t - tn * (tn + 1) / 2;
-  } else {  // groups of 8 tile rows
-    const int tiles_m = a.tiles / a.tiles_n, group = t / (8 * a.tiles_n), gm = min(tiles_m - group * 8, 8);
-    tm = group * 8 + t % (8 * a.tiles_n) % gm;
-    tn = t % (8 * a.tiles_n) / gm;
+// 4 x 4 transpose within each group of four lanes: lane l gives v[e] and receives lane e's v[l].
+__device__ __forceinline__ float quad_swap1(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0xB1, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float quad_swap2(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x4E, 0xf, 0xf, true));
+}
+__device__ __forceinline__ void quad_transpose(float v[4], int lane) {
+  const bool b0 = lane & 1, b1 = lane & 2;
+#pragma unroll
+  for (int e = 0; e < 4; e += 2) {
+    const float t = quad_swap1(b0 ? v[e] : v[e + 1]);
+    if (b0) v[e] = t;
+    else v[e + 1] = t;
   }
-  const int m0 = __builtin_amdgcn_readfirstlane(tm * T), n0 = __builtin_amdgcn_readfirstlane(tn * T);
-  const uint16_t* A = a.A + b * a.a_stride + m0 * a.lda;
-  const uint16_t* B = a.B + b * a.b_stride + (SYM ? n0 * a.ldb : (int64_t)n0 * 2);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const float t = quad_swap2(b1 ? v[e] : v[e + 2]);
+    if (b1) v[e] = t;
+    else v[e + 2] = t;
+  }
+}
+
+// A shape of workgroup: KG groups of WR x WC waves, each wave 16 MB x 16 NB of the tile, NST LDS stages of 32 k a group.
+template <int MB_, int NB_, int WR_, int WC_, int KG_, int NST_>
+struct Shape {
+  static constexpr int MB = MB_, NB = NB_, WR = WR_, WC = WC_, KG = KG_, NST = NST_;
+  static constexpr int W = WR * WC, THREADS = 64 * W * KG, TM = 16 * MB * WR, TN = 16 * NB * WC, STAGE = (TM + TN) * 128;
+};
+
+// One tile.  A step is three rounds of products, each beside the fragment reads of the next: lo hi (reads A hi), hi hi
+// (reads B lo), then a barrier, hi lo (reads B hi and A lo of the next step, and issues the loads of step kt + NST into
+// the stage just read).  One set of fragment registers serves, and no round waits for reads of its own.  Waves whose
+// part of the tile is not stored load and wait like the others but read and multiply nothing.  Each of the KG groups
+// takes a share of the steps; their sums are added through LDS in order.
+template <int MODE, typename S>
+__device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*>* wt, const Table<void*>* ot,
+                                        unsigned char* smem) {
+  constexpr bool SYM = MODE == GRAM || MODE == POLY;
+  constexpr int MB = S::MB, NB = S::NB, TM = S::TM, TN = S::TN, NST = S::NST, KG = S::KG, W = S::W, STAGE = S::STAGE;
+  typedef RowOp<TM, W> OpA;
+  typedef std::conditional_t<SYM, RowOp<TN, W>, ColOp<TN, W>> OpB;
+  constexpr int LOADS = OpA::LOADS + OpB::LOADS;
+  static_assert(LOADS <= MB + NB, "the third round's reads carry the loads");
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / W, w = wave % W;
+  // eight waves: those of one SIMD (w, w + 4) lie in opposite halves of both sides, so that a tile half outside the
+  // matrix takes half the time
+  static_assert(S::WC == 2 && (S::WR == 2 || S::WR == 4), "wave layouts");
+  const int wm = W == 8 ? (w & 3) ^ (w >> 2 << 1) : w >> 1, wn = W == 8 ? (w & 1) ^ (w >> 2) : w & 1;
+  const TileGroup& G = group_of(a.grp, a.n_groups, blockIdx.x);
+  if ((int)blockIdx.x - G.b0 >= G.count) return;
+  const int v = xcd_remap(blockIdx.x - G.b0, G.count), mat = v / G.tiles;
+  int t = v % G.tiles, tm = 0, tn;
+  if constexpr (SYM) {  // tile rows from the diagonal on
+    int skip = 0;
+    while (t >= G.tiles_n - skip) {
+      t -= G.tiles_n - skip;
+      ++tm;
+      skip = tm * TM / TN;
+    }
+    tn = skip + t;
+  } else {  // groups of 8 tile rows
+    const int tiles_m = G.tiles / G.tiles_n, group = t / (8 * G.tiles_n), gm = min(tiles_m - group * 8, 8);
+    tm = group * 8 + t % (8 * G.tiles_n) % gm;
+    tn = t % (8 * G.tiles_n) / gm;
+  }
+  const int m0 = __builtin_amdgcn_readfirstlane(tm * TM), n0 = __builtin_amdgcn_readfirstlane(tn * TN);
+  const int64_t lx = 2 * (int64_t)G.np, la = 2 * (int64_t)G.mp;
+  const uint16_t* X = a.x + G.x_off + mat * G.mp * lx;
+  uint16_t* Am = a.a + G.a_off + mat * G.mp * la;
+  uint16_t* Bm = a.b + G.a_off + mat * G.mp * la;
+  // operands: rows of the tile with k along them; SYM: the same for its columns, else X with k along its rows
+  const uint16_t* opa = MODE == GRAM ? X : MODE == POLY ? Am : Bm;
+  const int64_t lda = MODE == GRAM ? lx : la, end_a = G.mp * lda;
+  const int64_t beg_a = m0 * lda, beg_b = SYM ? n0 * lda : (int64_t)n0 * 2;
+  const uint16_t* opb = SYM ? opa : X;
+  const int64_t end_b = SYM ? end_a : G.mp * lx;
+  // first row and column of this wave's part
+  const int row0 = m0 + wm * 16 * MB, col0 = n0 + wn * 16 * NB, lim = SYM ? G.mp : G.np;
+  const int per = (G.steps + KG - 1) / KG;  // steps of a group: this one's are [kg per, kg per + own)
+  const int own = row0 < G.mp && col0 < lim && !(SYM && col0 + 16 * NB <= row0) ? min(max(G.steps - kg * per, 0), per) : 0;
   OpA oa;
   OpB ob;
-  oa.init(a.lda, 0, T, wave, lane);
-  if constexpr (SYM) ob.init(a.ldb, 0, T, wave, lane);
-  else ob.init(a.ldb, wave, lane);
-  auto rsrc = [](const uint16_t* p) {  // operands are padded to whole tiles and steps: every offset lies inside
-    const uint64_t addr = reinterpret_cast<uint64_t>(p);
-    return i32x4{(int)(uint32_t)addr, (int)((addr >> 32) & 0xffff), (int)kOffPastK, kRsrcWord3};
-  };
-  auto fetch = [&](int kt) {  // step kt (the last one again past the end: never read) into stage kt % NST
-    const int k = min(kt, a.steps - 1);
-    const i32x4 ra = rsrc(A + (int64_t)k * 64), rb = rsrc(SYM ? B + (int64_t)k * 64 : B + (int64_t)k * 32 * a.ldb);
-    unsigned char* st = smem + (kt % NST) * STAGE;
-#pragma unroll
-    for (int i = 0; i < OpA::NB; ++i) oa.dma(ra, st, wave, i, SK);
-#pragma unroll
-    for (int i = 0; i < OpB::NB; ++i) {
-      if constexpr (SYM) ob.dma(rb, st + OpA::BYTES, wave, i, SK);
-      else ob.dma(rb, st + OpA::BYTES, wave, i);
+  oa.init(lda, w, lane, wm * 16 * MB);
+  ob.init(SYM ? lda : lx, w, lane, wn * 16 * NB);
+  // An operand from the next step to load on; what lies past its end (rows of a ragged tile, steps past the last: never
+  // used) reads zero.  Columns past the end of a k-major row read the next row's: products that are never stored.
+  struct Src {
+    uint64_t addr;
+    int left;  // 128-byte blocks up to the operand's end
+    __device__ __forceinline__ i32x4 rsrc() const {
+      const uint32_t bytes = (uint32_t)min(max(left, 0), (1 << 25) - 1) << 7;
+      return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)addr), __builtin_amdgcn_readfirstlane((int)((addr >> 32) & 0xffff)),
+                   __builtin_amdgcn_readfirstlane((int)bytes), kRsrcWord3};
+    }
+    __device__ __forceinline__ void advance(int blocks) {
+      addr += (uint64_t)((int64_t)blocks * 128);
+      left -= blocks;
     }
   };
-  f32x4 acc[NBK][NBK];
+  Src sa{reinterpret_cast<uint64_t>(opa + beg_a), (int)((end_a - beg_a) >> 6)};
+  Src sb{reinterpret_cast<uint64_t>(opb + beg_b), (int)((end_b - beg_b) >> 6)};
+  const int inc_b = SYM ? 1 : (int)(lx >> 1) ;  // blocks a step: 32 k of a row, or 32 rows
+  if (KG > 1) {
+    sa.advance(kg * per);
+    sb.advance(kg * per * inc_b);
+  }
+  unsigned char* sm = smem + kg * NST * STAGE;
+  const uint32_t lds_a = __builtin_amdgcn_readfirstlane(lds_addr(sm) + w * OpA::LOADS * 1024);
+  const uint32_t lds_b = __builtin_amdgcn_readfirstlane(lds_addr(sm) + OpA::BYTES + w * OpB::LOADS * 1024);
+  auto load = [&](const i32x4& ra, const i32x4& rb, auto stage, auto q) {
+    constexpr int s = decltype(stage)::value, n = decltype(q)::value;
+    if constexpr (n < OpA::LOADS) dma_at<s * STAGE + n * 1024>(ra, oa.off[n], lds_a);
+    else dma_at<s * STAGE + (n - OpA::LOADS) * 1024>(rb, ob.off[n - OpA::LOADS], lds_b);
+  };
+  f16x8 ah[MB], al[MB], bh[NB], bl[NB];
+  f32x4 acc[MB][NB];
 #pragma unroll
-  for (int i = 0; i < NBK; ++i)
+  for (int i = 0; i < MB; ++i)
 #pragma unroll
-    for (int j = 0; j < NBK; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // MB NB products, B first: lane (r, g) accumulates C[r][4 g + e]; io(q) for q < N spread over them
+  auto round = [&](const f16x8 (&x)[MB], const f16x8 (&y)[NB], auto n_tag, auto io) {
+    constexpr int N = decltype(n_tag)::value, P = MB * NB;
+    unroll<N>([&](auto qt) {
+      constexpr int q = decltype(qt)::value;
+      io(qt);
 #pragma unroll
-  for (int s = 0; s < NST - 1; ++s) fetch(s);
-  for (int kt = 0; kt < a.steps; ++kt) {
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0((NST - 2) * LOADS));  // this wave's loads of step kt have landed
-    __builtin_amdgcn_s_barrier();  // every wave's; and every wave has read step kt - 1, whose stage is free
+      for (int n = q * P / N; n < (q + 1) * P / N; ++n)
+        acc[n / NB][n % NB] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y[n % NB], x[n / NB], acc[n / NB][n % NB], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  unroll<NST>([&](auto st) {
+    const i32x4 ra = sa.rsrc(), rb = sb.rsrc();
+    unroll<LOADS>([&](auto q) { load(ra, rb, st, q); });
+    sa.advance(1);
+    sb.advance(inc_b);
+  });
+  __builtin_amdgcn_s_waitcnt(wait_vm((NST - 1) * LOADS));  // loads complete in issue order: step 0 has landed
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  if (own > 0) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) bh[j] = ob.frag(sm + OpA::BYTES, j, 0);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) al[i] = oa.frag(sm, i, 1);
+  }
+  // step kt, in stage ST
+  auto step = [&](auto st, int kt) {
+    constexpr int ST = decltype(st)::value, NEXT = (ST + 1) % NST;
+    const unsigned char* cur = sm + ST * STAGE;
+    const unsigned char* nxt = sm + NEXT * STAGE;
+    __builtin_amdgcn_sched_barrier(0);
+    if (kt < own) {
+      round(al, bh, std::integral_constant<int, MB>{}, [&](auto q) { ah[q] = oa.frag(cur, q, 0); });
+      round(ah, bh, std::integral_constant<int, NB>{}, [&](auto q) { bl[q] = ob.frag(cur + OpA::BYTES, q, 1); });
+    }
+    // this wave's loads of step kt + 1 have landed and its fragments of step kt are read; then every wave's
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0((NST - 2) * LOADS));
+    __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    fetch(kt + NST - 1);
-    const unsigned char* st = smem + (kt % NST) * STAGE;
-    f16x8 fa[2][NBK], fb[2][NBK];  // hi, lo
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int j = 0; j < NBK; ++j) fb[h][j] = __builtin_bit_cast(f16x8, OpB::frag(st + OpA::BYTES, wn * 16 * NBK + 16 * j, r, g, h));
-#pragma unroll
-      for (int i = 0; i < NBK; ++i) fa[h][i] = __builtin_bit_cast(f16x8, OpA::frag(st, wm * 16 * NBK + 16 * i, r, g, h));
+    const i32x4 ra = sa.rsrc(), rb = sb.rsrc();
+    if (kt < own) {
+      round(ah, bl, std::integral_constant<int, MB + NB>{}, [&](auto qt) {
+        constexpr int q = decltype(qt)::value;
+        if constexpr (q < NB) bh[q] = ob.frag(nxt + OpA::BYTES, q, 0);
+        else al[q - NB] = oa.frag(nxt, q - NB, 1);
+        if constexpr (q < LOADS) load(ra, rb, st, qt);
+      });
+    } else {
+      unroll<LOADS>([&](auto q) { load(ra, rb, st, q); });
     }
-#pragma unroll
-    for (int p = 0; p < 3; ++p)  // hi hi, hi lo, lo hi; B first: lane (r, g) accumulates C[r][4 g + e]
-#pragma unroll
-      for (int i = 0; i < NBK; ++i)
-#pragma unroll
-        for (int j = 0; j < NBK; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[p == 1][j], fa[p == 2][i], acc[i][j], 0, 0, 0);
+    sa.advance(1);
+    sb.advance(inc_b);
+  };
+  int kt = 0;
+  while (kt < per) {
+    unroll<NST>([&](auto st) {
+      if (kt < per) step(st, kt++);
+    });
   }
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no DMA may land after the workgroup exits
 
-  const uint16_t* D = MODE == GRAM ? nullptr : a.D + b * a.d_stride;
-  uint16_t* C = MODE == LAST ? nullptr : a.C + b * a.c_stride;
-#pragma unroll
-  for (int i = 0; i < NBK; ++i) {
-    const int row = m0 + wm * 16 * NBK + 16 * i + r;
-#pragma unroll
-    for (int j = 0; j < NBK; ++j) {
-      const int col = n0 + wn * 16 * NBK + 16 * j + 4 * g;
-      float x[4] = {a.beta * acc[i][j][0], a.beta * acc[i][j][1], a.beta * acc[i][j][2], a.beta * acc[i][j][3]};
-      if constexpr (MODE != GRAM) {
-        float d[4];
-        load_halves4(D + row * a.ldd, col, d);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = fmaf(a.alpha, d[e], x[e]);
-      }
-      if constexpr (MODE != LAST) {
-        store_halves4(C + row * a.ldc, col, x);
-        if (SYM && tm != tn) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint16_t h = h_bits(x[e]);
-            uint16_t* p = C + (col + e) * a.ldc + hi_at(row);
-            p[0] = h;
-            p[32] = h_bits(x[e] - h_val(h));
-          }
-        }
+  const void* w_ptr = nullptr;
+  void* out = nullptr;
+  bool vec = false, flip = false;
+  if constexpr (MODE == LAST) {
+    w_ptr = wt->p[G.first + mat];
+    out = ot->p[G.first + mat];
+    flip = G.rows > G.cols;
+    vec = G.cols % 4 == 0 && by4(out, G.w_dtype) && (!a.update || by4(w_ptr, G.w_dtype));
+  }
+  // What the epilogue of a block reads: D, and the weight that LAST updates.  Loaded a row of blocks ahead of the stores:
+  // taken one by one behind them, each cost its latency (22 x 1408 x 1408, POLY: 34 of 139 us a tile).
+  struct Extra { uint2 h, l; uint4 w; };
+  auto at = [&](int i, int j, int& orow, int& ocol) {  // of LAST's output: first of this lane's four columns
+    const int row = row0 + 16 * i, col = col0 + 16 * j;
+    orow = flip ? col + 4 * g + (r & 3) : row + r;
+    ocol = flip ? row + (r & 12) : col + 4 * g;
+  };
+  auto fetch = [&](int i, int j, Extra& x) {
+    const int rb = row0 + 16 * i, cb = col0 + 16 * j, row = rb + r, col = cb + 4 * g;
+    if (MODE == GRAM || rb >= G.mp || cb >= lim || (SYM && cb < rb)) return;
+    const uint16_t* d = (MODE == POLY ? Am + row * la : X + row * lx) + hi_at(col);
+    x.h = *reinterpret_cast<const uint2*>(d);
+    x.l = *reinterpret_cast<const uint2*>(d + 32);
+    if constexpr (MODE == LAST) {
+      int orow, ocol;
+      at(i, j, orow, ocol);
+      if (!a.update || !vec || orow >= G.rows || ocol >= G.cols) return;
+      const int64_t o = (int64_t)orow * G.cols + ocol;
+      if (G.w_dtype == LLATTN_F32) {
+        x.w = *reinterpret_cast<const uint4*>(static_cast<const float*>(w_ptr) + o);
       } else {
-        const int M = a.flip ? a.cols : a.rows, N = a.flip ? a.rows : a.cols;
-        if (row >= M) continue;
+        const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(w_ptr) + o);
+        x.w = make_uint4(v.x << 16, v.x & 0xffff0000u, v.y << 16, v.y & 0xffff0000u);
+      }
+    }
+  };
+  auto store = [&](int i, int j, const f32x4& c, const Extra& xt) {
+    const int rb = row0 + 16 * i, cb = col0 + 16 * j, row = rb + r, col = cb + 4 * g;
+    if (rb >= G.mp || cb >= lim || (SYM && cb < rb)) return;
+    float x[4] = {G.beta * c[0], G.beta * c[1], G.beta * c[2], G.beta * c[3]};
+    if constexpr (MODE != GRAM) {
+      const f16x4 h = __builtin_bit_cast(f16x4, xt.h), l = __builtin_bit_cast(f16x4, xt.l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = fmaf(G.alpha, (float)h[e] + (float)l[e], x[e]);
+    }
+    if constexpr (MODE == APPLY) {
+      store_halves4(a.y + G.x_off + (mat * G.mp + row) * lx, col, x);
+    } else if constexpr (SYM) {
+      uint16_t* C = MODE == GRAM ? Am : Bm;
+      store_halves4(C + row * la, col, x);
+      if (cb > rb) {  // and below the diagonal: this lane's column 4 g + r % 4, rows 4 (r / 4) ..
+        quad_transpose(x, lane);
+        store_halves4(C + (col + (r & 3)) * la, rb + (r & 12), x);
+      }
+    } else {
+      int orow, ocol;
+      at(i, j, orow, ocol);
+      if (flip) quad_transpose(x, lane);
+      const int n = min(4, G.cols - ocol);
+      if (orow >= G.rows || n <= 0) return;
+      const int64_t o = (int64_t)orow * G.cols + ocol;
+      if (a.update) {
+        float c4[4] = {__uint_as_float(xt.w.x), __uint_as_float(xt.w.y), __uint_as_float(xt.w.z), __uint_as_float(xt.w.w)};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if (col + e >= N) continue;
-          const int64_t o = a.flip ? (int64_t)(col + e) * a.cols + row : (int64_t)row * a.cols + col + e;
-          float y = x[e];
-          if (a.update) y = fmaf(-a.step, y, a.keep * load_as(a.w.p[b], o, a.w_dtype));
-          if (a.w_dtype == LLATTN_F32) static_cast<float*>(a.out.p[b])[o] = y;
-          else static_cast<uint16_t*>(a.out.p[b])[o] = f2bf(y);
+          if (!vec) c4[e] = e < n ? load_as(w_ptr, o + e, G.w_dtype) : 0.f;
+          x[e] = fmaf(-G.step, x[e], G.keep * c4[e]);
+        }
+      }
+      const bool f32 = G.w_dtype == LLATTN_F32;
+      if (vec) {
+        if (f32) store4<float>(static_cast<float*>(out) + o, x);
+        else store4<uint16_t>(static_cast<uint16_t*>(out) + o, x);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (e >= n) continue;
+          if (f32) static_cast<float*>(out)[o + e] = x[e];
+          else static_cast<uint16_t*>(out)[o + e] = f2bf(x[e]);
         }
       }
     }
+  };
+  if constexpr (KG == 1) {
+    Extra xt[2][NB];
+    auto fetch_row = [&](int i) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) fetch(i, j, xt[i & 1][j]);
+    };
+    fetch_row(0);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+      if (i + 1 < MB) fetch_row(i + 1);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) store(i, j, acc[i][j], xt[i & 1][j]);
+    }
+  } else {
+    static_assert(KG * W * MB * NB * 1024 <= KG * NST * STAGE, "the groups' sums fit their stages");
+    __builtin_amdgcn_s_barrier();  // every wave has read its fragments and its loads have landed
+    asm volatile("" ::: "memory");
+    f32x4* sum = reinterpret_cast<f32x4*>(smem);  // [KG][W][MB NB][64]
+#pragma unroll
+    for (int u = 0; u < MB * NB; ++u) sum[(wave * MB * NB + u) * 64 + lane] = acc[u / NB][u % NB];
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < MB * NB; ++u) {  // blocks are shared out among the groups
+      if (u % KG != kg) continue;
+      Extra xt;
+      fetch(u / NB, u % NB, xt);
+      f32x4 c = sum[(w * MB * NB + u) * 64 + lane];
+#pragma unroll
+      for (int k = 1; k < KG; ++k) c += sum[((k * W + w) * MB * NB + u) * 64 + lane];
+      store(u / NB, u % NB, c, xt);
+    }
+  }
+}
+
+template <int MODE, typename S, int WGS>
+__global__ __launch_bounds__(S::THREADS, WGS * S::W * S::KG / 4) void ns_kernel(const NsArgs a) {
+  __shared__ __align__(1024) unsigned char smem[S::KG * S::NST * S::STAGE];
+  ns_tile<MODE, S>(a, nullptr, nullptr, smem);
+}
+template <typename S, int WGS>
+__global__ __launch_bounds__(S::THREADS, WGS * S::W * S::KG / 4) void ns_last_kernel(const LastArgs a) {
+  __shared__ __align__(1024) unsigned char smem[S::KG * S::NST * S::STAGE];
+  ns_tile<LAST, S>(a.n, &a.w, &a.out, smem);
+}
+
+// ---- small matrices: the whole call in one workgroup each ---------------------------------------------------------------
+// Up to 64 rows of X (the smaller side) and kSmallCols columns: X, A and B stay in LDS, as blocks of 32 columns (64 rows
+// of 128 bytes, chunk c of row o at c ^ (o & 7)).  The chain of 2 + 3 steps launches that it replaces waits for launches
+// and for its own tail 15 times: 4 x 64 x 128 in 81 us.
+constexpr int kSmall = 64;         // matrices a launch
+constexpr int kSmallCols = 448;    // X: 112 KB of LDS beside 32 KB for A and B
+
+struct SmallGroup {
+  int first, rows, cols, np, g_dtype, w_dtype;
+  float scale, keep, step;
+};
+struct SmallArgs {
+  const void* g[kSmall];
+  const float* m[kSmall];
+  float* m_out[kSmall];
+  const void* w[kSmall];
+  void* out[kSmall];
+  int n_groups, update, nesterov, steps;
+  float mu, one_mu, eps, a, b, c;
+  SmallGroup grp[LLATTN_MUON_GROUPS];
+};
+static_assert(sizeof(SmallArgs) <= 4096, "kernel arguments");
+
+__device__ __forceinline__ int small_at(int row, int col) {  // byte of the hi half
+  return (col >> 5) * 8192 + row * 128 + ((((col & 31) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2;
+}
+__device__ __forceinline__ int lo_of(int byte) { return byte ^ 64; }  // its lo half: four chunks further
+
+__global__ __launch_bounds__(256) void ns_small_kernel(const SmallArgs a) {
+  extern __shared__ __align__(1024) unsigned char lds[];  // A, B, X
+  __shared__ double red[256];
+  unsigned char *As = lds, *Bs = lds + 16384, *Xs = lds + 32768;
+  int gi = 0;
+  while (gi + 1 < a.n_groups && (int)blockIdx.x >= a.grp[gi + 1].first) ++gi;
+  const SmallGroup& G = a.grp[gi];
+  const int id = blockIdx.x, tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), r0 = (wave >> 1) * 32, c0 = (wave & 1) * 32;
+  const bool flip = G.rows > G.cols;
+  const int n = G.rows * G.cols, blocks = G.np / 32;
+  for (int i = tid; i < blocks * 512; i += 256) *reinterpret_cast<uint4*>(Xs + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+  const void* gp = a.g[id];
+  double sum = 0.0;
+  for (int i = tid; i < n; i += 256) {
+    float u = load_as(gp, i, G.g_dtype);
+    if (a.update) {
+      const float v = fmaf(a.mu, a.m[id][i], a.one_mu * u);
+      a.m_out[id][i] = v;
+      u = direction(u, v, a.mu, a.one_mu, a.nesterov);
+    }
+    sum += (double)u * (double)u;
+  }
+  const double f = (double)G.scale / (sqrt(block_sum(sum, red)) + (double)a.eps);
+  for (int i = tid; i < n; i += 256) {  // each thread reads back what it wrote itself
+    float u = load_as(gp, i, G.g_dtype);
+    if (a.update) u = direction(u, a.m_out[id][i], a.mu, a.one_mu, a.nesterov);
+    u = (float)((double)u * f);
+    const int ur = i / G.cols, uc = i - ur * G.cols;
+    const int at = small_at(flip ? uc : ur, flip ? ur : uc);
+    const uint16_t h = h_bits(u);
+    *reinterpret_cast<uint16_t*>(Xs + at) = h;
+    *reinterpret_cast<uint16_t*>(Xs + lo_of(at)) = h_bits(u - h_val(h));
+  }
+  __syncthreads();
+  // fragment of rows o16 + r of block kb (half 0: hi, 1: lo), k along the block's columns
+  auto row_frag = [&](const unsigned char* M, int kb, int o16, int half) {
+    const int row = o16 + r;
+    return *reinterpret_cast<const f16x8*>(M + kb * 8192 + row * 128 + (((4 * half + g) ^ (row & 7)) << 4));
+  };
+  // of columns o16 + r, k along X's rows k0 ..
+  auto col_frag = [&](int k0, int o16, int half) {
+    bf16x4 hv[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int k = k0 + 8 * g + 4 * q + (r >> 2), at = small_at(k, o16 + 4 * (r & 3));
+      hv[q] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(Xs + (half ? lo_of(at) : at)));
+    }
+    return __builtin_bit_cast(f16x8, bf16x8{hv[0][0], hv[0][1], hv[0][2], hv[0][3], hv[1][0], hv[1][1], hv[1][2], hv[1][3]});
+  };
+  f32x4 acc[2][2];
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  auto products = [&](const f16x8 (&x)[2][2], const f16x8 (&y)[2][2]) {  // [half][block]
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y[p == 1][j], x[p == 2][i], acc[i][j], 0, 0, 0);
+  };
+  auto get4 = [&](const unsigned char* M, int row, int col, float (&v)[4]) {
+    const int at = small_at(row, col);
+    const f16x4 h = *reinterpret_cast<const f16x4*>(M + at), l = *reinterpret_cast<const f16x4*>(M + lo_of(at));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)h[e] + (float)l[e];
+  };
+  auto put4 = [&](unsigned char* M, int row, int col, const float (&v)[4]) {
+    const int at = small_at(row, col);
+    f16x4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      h[e] = (_Float16)v[e];
+      l[e] = (_Float16)(v[e] - (float)h[e]);
+    }
+    *reinterpret_cast<f16x4*>(M + at) = h;
+    *reinterpret_cast<f16x4*>(M + lo_of(at)) = l;
+  };
+  const float ga = kSA / (G.scale * G.scale), pb = a.c / kSA;
+  for (int step = 0; step < a.steps; ++step) {
+    const bool last = step + 1 == a.steps;
+    clear();
+    for (int kb = 0; kb < blocks; ++kb) {
+      f16x8 x[2][2], y[2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          x[h][i] = row_frag(Xs, kb, r0 + 16 * i, h);
+          y[h][i] = row_frag(Xs, kb, c0 + 16 * i, h);
+        }
+      products(x, y);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float v[4] = {ga * acc[i][j][0], ga * acc[i][j][1], ga * acc[i][j][2], ga * acc[i][j][3]};
+        put4(As, r0 + 16 * i + r, c0 + 16 * j + 4 * g, v);
+      }
+    __syncthreads();
+    clear();
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      f16x8 x[2][2], y[2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          x[h][i] = row_frag(As, kb, r0 + 16 * i, h);
+          y[h][i] = row_frag(As, kb, c0 + 16 * i, h);
+        }
+      products(x, y);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = r0 + 16 * i + r, col = c0 + 16 * j + 4 * g;
+        float v[4];
+        get4(As, row, col, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(a.b, v[e], pb * acc[i][j][e]);
+        put4(Bs, row, col, v);
+      }
+    __syncthreads();
+    f16x8 bf[2][2][2];  // [k block][half][row block] of B
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) bf[kb][h][i] = row_frag(Bs, kb, r0 + 16 * i, h);
+    for (int cb = 0; cb < G.np; cb += 64) {
+      clear();
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        f16x8 y[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) y[h][j] = col_frag(32 * kb, cb + c0 + 16 * j, h);
+        products(bf[kb], y);
+      }
+      float v[2][2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          get4(Xs, r0 + 16 * i + r, cb + c0 + 16 * j + 4 * g, v[i][j]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[i][j][e] = fmaf(a.a, v[i][j][e], acc[i][j][e] / kSA);
+        }
+      if (!last) __syncthreads();  // every wave has read these columns
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int row = r0 + 16 * i + r, col = cb + c0 + 16 * j + 4 * g;
+          if (!last) {
+            put4(Xs, row, col, v[i][j]);
+            continue;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int ur = flip ? col + e : row, uc = flip ? row : col + e;
+            if (ur >= G.rows || uc >= G.cols) continue;
+            const int o = ur * G.cols + uc;
+            float y = v[i][j][e] / G.scale;
+            if (a.update) y = fmaf(-G.step, y, G.keep * load_as(a.w[id], o, G.w_dtype));
+            if (G.w_dtype == LLATTN_F32) static_cast<float*>(a.out[id])[o] = y;
+            else static_cast<uint16_t*>(a.out[id])[o] = f2bf(y);
+          }
+        }
+    }
+    __syncthreads();
   }
 }
 
 // ---- host -----------------------------------------------------------------------------
 constexpr size_t up(size_t n) { return (n + 255) & ~size_t(255); }
 
+// Workgroups of a launch.
+enum Kind { SMALL = 0, SPLIT = 1, SQUARE = 2, BIG = 3, KINDS = 4 };
+typedef Shape<2, 2, 2, 2, 1, 3> SmallShape;
+typedef Shape<2, 2, 2, 2, 2, 3> SplitShape;
+typedef Shape<4, 4, 2, 2, 1, 2> SquareShape;
+typedef Shape<4, 8, 4, 2, 1, 2> BigShape;
+constexpr int kTm[KINDS] = {SmallShape::TM, SplitShape::TM, SquareShape::TM, BigShape::TM};
+constexpr int kTn[KINDS] = {SmallShape::TN, SplitShape::TN, SquareShape::TN, BigShape::TN};
+constexpr int kPerCu[KINDS] = {3, 1, 2, 1};
+// us of a 32-k step of a workgroup with 1, 2, 3 of them on a CU, and of a tile beside its steps.
+constexpr double kStep[KINDS][3] = {{0.33, 0.50, 0.80}, {0.28, 0.28, 0.28}, {0.67, 1.37, 1.37}, {2.25, 2.25, 2.25}};
+constexpr double kTile[KINDS] = {3.5, 4.0, 7.0, 16.0};
+
+struct GroupPlan {
+  int m, n, mp, np, parts, first, part0;
+  size_t x_off, a_off;  // 16-bit elements
+};
 struct Plan {
-  int m, n, T, mp, np, blocks;
-  size_t x, a, part;  // bytes of one X, of one A (whole batch), of the partial sums
+  int matrices;
+  GroupPlan g[LLATTN_MUON_GROUPS];
+  size_t x, a, part;    // bytes of one X, of one A, of the partial sums
   size_t bytes() const { return 2 * x + 2 * a + part; }
 };
 
-// 128 x 128 tiles where X has at least one for every CU, else 64 x 64.
-Plan plan_of(const llattn_muon_cfg* c) {
+Plan plan_of(const llattn_muon_cfg* c, const llattn_muon_group* groups) {
   Plan p{};
-  p.m = std::min(c->rows, c->cols);
-  p.n = std::max(c->rows, c->cols);
-  const int64_t t128 = (int64_t)c->batch * ((p.m + 127) / 128) * ((p.n + 127) / 128);
-  p.T = t128 >= 256 ? 128 : 64;
-  p.mp = (p.m + p.T - 1) / p.T * p.T;
-  p.np = (p.n + p.T - 1) / p.T * p.T;
-  p.blocks = (int)std::min<int64_t>(256, ((int64_t)p.m * p.n + 4095) / 4096);
-  p.x = up((size_t)c->batch * p.mp * p.np * 4);
-  p.a = up((size_t)c->batch * p.mp * p.mp * 4);
-  p.part = up((size_t)c->batch * p.blocks * 8);
+  size_t x = 0, a = 0, part = 0;
+  for (int i = 0; i < c->n_groups; ++i) {
+    const llattn_muon_group& q = groups[i];
+    GroupPlan& g = p.g[i];
+    g.m = std::min(q.rows, q.cols);
+    g.n = std::max(q.rows, q.cols);
+    g.mp = (g.m + 63) / 64 * 64;
+    g.np = (g.n + 63) / 64 * 64;
+    g.parts = (int)std::min<int64_t>(256, ((int64_t)g.m * g.n + 4095) / 4096);
+    g.first = p.matrices;
+    g.part0 = (int)part;
+    g.x_off = x;
+    g.a_off = a;
+    p.matrices += q.batch;
+    part += (size_t)q.batch * g.parts;
+    x += (size_t)q.batch * g.mp * g.np * 2;
+    a += (size_t)q.batch * g.mp * g.mp * 2;
+  }
+  p.x = up(2 * x);
+  p.a = up(2 * a);
+  p.part = up(8 * part);
   return p;
 }
 
@@ -370,13 +902,22 @@ double grow(double a, double b, double c, double top, double* poly) {
   return best;
 }
 
-int32_t check(const llattn_muon_cfg* c) {
-  if (!c) return fail(LLATTN_ERR_SHAPE, "llattn_muon: null configuration");
-  if (c->batch <= 0 || c->batch > LLATTN_MUON_BATCH || c->rows <= 0 || c->cols <= 0 || c->rows > 32768 || c->cols > 32768)
-    return fail(LLATTN_ERR_SHAPE, "llattn_muon: batch %d (1 to %d), %d x %d matrices (1 to 32768)", c->batch,
-                LLATTN_MUON_BATCH, c->rows, c->cols);
-  for (const int d : {c->g_dtype, c->w_dtype})
-    if (d != LLATTN_F32 && d != LLATTN_BF16) return fail(LLATTN_ERR_DTYPE, "llattn_muon: unknown dtype %d", d);
+int32_t check(const llattn_muon_cfg* c, const llattn_muon_group* groups) {
+  if (!c || !groups) return fail(LLATTN_ERR_SHAPE, "llattn_muon: null configuration");
+  if (c->n_groups < 1 || c->n_groups > LLATTN_MUON_GROUPS)
+    return fail(LLATTN_ERR_SHAPE, "llattn_muon: %d groups (1 to %d)", c->n_groups, LLATTN_MUON_GROUPS);
+  int64_t total = 0;
+  for (int i = 0; i < c->n_groups; ++i) {
+    const llattn_muon_group& q = groups[i];
+    if (q.batch <= 0 || q.rows <= 0 || q.cols <= 0 || q.rows > 32768 || q.cols > 32768)
+      return fail(LLATTN_ERR_SHAPE, "llattn_muon: group %d: %d matrices of %d x %d (1 to 32768)", i, q.batch, q.rows, q.cols);
+    for (const int d : {q.g_dtype, q.w_dtype})
+      if (d != LLATTN_F32 && d != LLATTN_BF16) return fail(LLATTN_ERR_DTYPE, "llattn_muon: unknown dtype %d", d);
+    total += q.batch;
+  }
+  if (total > LLATTN_MUON_BATCH)
+    return fail(LLATTN_ERR_SHAPE, "llattn_muon: %lld matrices (at most %d a call)", (long long)total, LLATTN_MUON_BATCH);
+  if (c->tiles < 0 || c->tiles > KINDS) return fail(LLATTN_ERR_SHAPE, "llattn_muon: tiles %d (0 to 4)", c->tiles);
   if (c->steps < 1 || c->steps > 100) return fail(LLATTN_ERR_SHAPE, "llattn_muon: %d steps (1 to 100)", c->steps);
   if (!(c->eps >= 0.f) || !std::isfinite(c->eps)) return fail(LLATTN_ERR_SHAPE, "llattn_muon: eps %g must not be negative", c->eps);
   double s = 1.0, poly = 0.0;  // singular values start in [0, 1]: the Frobenius norm bounds the largest
@@ -389,88 +930,237 @@ int32_t check(const llattn_muon_cfg* c) {
   return LLATTN_OK;
 }
 
-template <int MODE>
-void launch_ns(NsArgs& a, const Plan& p, int batch, hipStream_t st) {
-  const int tm = p.mp / p.T, tn = p.np / p.T;
-  a.tiles_n = MODE == GRAM || MODE == POLY ? tm : tn;
-  a.tiles = MODE == GRAM || MODE == POLY ? tm * (tm + 1) / 2 : tm * tn;
-  const dim3 grid((unsigned)(a.tiles * batch)), block(256);
-  if (p.T == 128) hipLaunchKernelGGL((ns_kernel<MODE, 128, 2>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((ns_kernel<MODE, 64, 3>), grid, block, 0, st, a);
+// Tiles of a matrix: all of an m x n one, or those of a symmetric one that reach the diagonal.
+int tiles_of(bool sym, int kind, int m, int n) {
+  const int tm = (m + kTm[kind] - 1) / kTm[kind], tn = (n + kTn[kind] - 1) / kTn[kind];
+  if (!sym) return tm * tn;
+  int t = 0;
+  for (int i = 0; i < tm; ++i) t += tn - i * kTm[kind] / kTn[kind];
+  return t;
 }
 
-int32_t run(const char* who, const llattn_muon_cfg* c, const void* const* g, const float* const* m, const void* const* w,
-            float* const* m_out, void* const* out, void* workspace, size_t workspace_bytes, hipStream_t st) {
-  if (const int32_t rc = check(c)) return rc;
-  const Plan p = plan_of(c);
+struct Call {
+  const llattn_muon_cfg* c;
+  const llattn_muon_group* groups;
+  Plan p;
+  hipStream_t st;
+  uint16_t *X[2], *A, *B;
+  bool update;
+  int kind[3];  // workgroups of GRAM, POLY, APPLY and LAST
+};
+
+template <int MODE, typename S, int WGS>
+void launch_shape(const LastArgs& a, int blocks, hipStream_t st) {
+  if constexpr (MODE == LAST) hipLaunchKernelGGL((ns_last_kernel<S, WGS>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, a);
+  else hipLaunchKernelGGL((ns_kernel<MODE, S, WGS>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, a.n);
+}
+template <int MODE>
+void launch_kind(int kind, const LastArgs& a, int blocks, hipStream_t st) {
+  if (kind == SMALL) launch_shape<MODE, SmallShape, kPerCu[SMALL]>(a, blocks, st);
+  else if (kind == SPLIT) launch_shape<MODE, SplitShape, kPerCu[SPLIT]>(a, blocks, st);
+  else if (kind == SQUARE) launch_shape<MODE, SquareShape, kPerCu[SQUARE]>(a, blocks, st);
+  else launch_shape<MODE, BigShape, kPerCu[BIG]>(a, blocks, st);
+}
+
+float scale_of(const GroupPlan& g) { return std::exp2f((float)std::min(14, (int)(0.5 * std::log2((double)g.m * g.n)))); }
+
+// The workgroups that a launch takes: the least expected time.  A launch of one shape runs in rounds of whole tiles over
+// the 256 CUs, the last with fewer workgroups on each; of several, its work is shared out and ends with a part of the
+// longest tile.  Measured in us (G: X Xᵀ, P: A A, A: B X):
+//                                   64 x 64        64 x 64, 2 k groups   128 x 128       256 x 256
+//   3 of 333 x 1001     G P A     13   9  12         12   9  15          28  20  19      64  42  49
+//   1 of 512 x 1408     G P A     15  10  10         13   9  10          39  22  21      95  64  55
+//   1 of 1408 x 4096    G P A     44  20  70         39  18  89          87  43  64     218 109 102
+//   6 of 1000 x 1500    G P A     52  42  82          -                  46  38  81     109  96  88
+//   22 of 1408 x 1408   G P A    287 307 526          -                 236 249 399     232 254 427
+//   22 of 1408 x 4096   G P A    831 307 1526         -                 557 261 1106    549 263 1076
+//   8 of 4096 x 4096    G P A   3250 3397 4082        -                1633 1813 2947  1601 1607 2469
+// (128 x 256 tiles on eight waves lay between the last two throughout.)
+template <bool SYM>
+int choose(const llattn_muon_cfg* c, const llattn_muon_group* groups, const Plan& p, bool gram) {
+  if (c->tiles > 0) return c->tiles - 1;
+  int best = SMALL;
+  double best_t = 0.0;
+  for (int kind = 0; kind < KINDS; ++kind) {
+    const auto count = [&](int i) {
+      return (int64_t)groups[i].batch * tiles_of(SYM, kind, p.g[i].mp, SYM ? p.g[i].mp : p.g[i].np);
+    };
+    const auto tile_us = [&](int i, int64_t on) { return (gram ? p.g[i].np : p.g[i].mp) / 32 * kStep[kind][on - 1] + kTile[kind]; };
+    int64_t tiles = 0;
+    for (int i = 0; i < c->n_groups; ++i) tiles += count(i);
+    if (kind == SPLIT && tiles > 256) continue;
+    const int64_t slots = 256 * kPerCu[kind], on = std::min<int64_t>(kPerCu[kind], (tiles + 255) / 256);
+    double t;
+    if (c->n_groups == 1) {
+      const int64_t rest = tiles % slots;
+      t = (double)(tiles / slots) * tile_us(0, kPerCu[kind]) + (rest ? tile_us(0, (rest + 255) / 256) : 0.0);
+    } else {
+      double work = 0.0, longest = 0.0;
+      for (int i = 0; i < c->n_groups; ++i) {
+        work += tile_us(i, on) * (double)count(i);
+        longest = std::max(longest, tile_us(i, on));
+      }
+      const double rounds = work / (256.0 * (double)on) / longest;
+      t = longest * (rounds < 2.0 ? std::ceil(rounds) : rounds + 0.3);
+    }
+    if (kind == 0 || t < best_t) {
+      best = kind;
+      best_t = t;
+    }
+  }
+  return best;
+}
+
+template <int MODE>
+void launch_products(const Call& k, LastArgs& a) {
+  constexpr bool SYM = MODE == GRAM || MODE == POLY;
+  int order[LLATTN_MUON_GROUPS];  // long contractions first: the short ones fill up behind them
+  for (int i = 0; i < k.c->n_groups; ++i) order[i] = i;
+  std::stable_sort(order, order + k.c->n_groups, [&](int i, int j) {
+    return MODE == GRAM ? k.p.g[i].np > k.p.g[j].np : k.p.g[i].mp > k.p.g[j].mp;
+  });
+  const int kind = k.kind[MODE == LAST ? APPLY : MODE];
+  int blocks = 0;
+  for (int o = 0; o < k.c->n_groups; ++o) {
+    const int i = order[o];
+    const GroupPlan& g = k.p.g[i];
+    const llattn_muon_group& q = k.groups[i];
+    TileGroup& t = a.n.grp[o];
+    t = TileGroup{};
+    t.b0 = blocks;
+    t.tiles = tiles_of(SYM, kind, g.mp, SYM ? g.mp : g.np);
+    t.tiles_n = ((SYM ? g.mp : g.np) + kTn[kind] - 1) / kTn[kind];
+    t.count = t.tiles * q.batch;
+    t.steps = (MODE == GRAM ? g.np : g.mp) / 32;
+    t.mp = g.mp; t.np = g.np; t.first = g.first; t.rows = q.rows; t.cols = q.cols; t.w_dtype = q.w_dtype;
+    t.x_off = (int64_t)g.x_off; t.a_off = (int64_t)g.a_off;
+    t.keep = q.keep; t.step = q.step;
+    const float sx = scale_of(g);
+    t.alpha = MODE == POLY ? k.c->b : MODE == LAST ? k.c->a / sx : k.c->a;
+    t.beta = MODE == GRAM ? kSA / (sx * sx) : MODE == POLY ? k.c->c / kSA : MODE == LAST ? 1.f / (kSA * sx) : 1.f / kSA;
+    blocks += (t.count + 7) / 8 * 8;
+  }
+  a.n.n_groups = k.c->n_groups;
+  launch_kind<MODE>(kind, a, blocks, k.st);
+}
+
+// All of the call in one workgroup a matrix (ns_small_kernel), where every matrix fits.
+bool all_small(const llattn_muon_cfg* c, const Plan& p) {
+  if (c->tiles) return false;
+  for (int i = 0; i < c->n_groups; ++i)
+    if (p.g[i].mp > 64 || p.g[i].np > kSmallCols) return false;
+  return true;
+}
+
+int32_t run_small(const char* who, const llattn_muon_cfg* c, const llattn_muon_group* groups, const Plan& p, const void* const* g,
+                  const float* const* m, const void* const* w, float* const* m_out, void* const* out, bool update, hipStream_t st) {
+  SmallArgs a{};
+  a.update = update; a.nesterov = c->nesterov; a.steps = c->steps;
+  a.mu = c->mu; a.one_mu = (float)(1.0 - (double)c->mu); a.eps = c->eps;
+  a.a = c->a; a.b = c->b; a.c = c->c;
+  int np = 0, held = 0;
+  const auto launch = [&]() {
+    hipLaunchKernelGGL(ns_small_kernel, dim3(held), dim3(256), 32768 + (size_t)np * 256, st, a);
+    a.n_groups = held = np = 0;
+  };
+  for (int i = 0; i < c->n_groups; ++i) {
+    int b = p.g[i].first;
+    const int end = b + groups[i].batch;
+    while (b < end) {
+      SmallGroup& t = a.grp[a.n_groups++];
+      t = SmallGroup{held, groups[i].rows, groups[i].cols, p.g[i].np, groups[i].g_dtype, groups[i].w_dtype, scale_of(p.g[i]),
+                     groups[i].keep, groups[i].step};
+      np = std::max(np, t.np);
+      for (; b < end && held < kSmall; ++b, ++held) {
+        a.g[held] = g[b];
+        a.out[held] = out[b];
+        if (!update) continue;
+        a.m[held] = m[b];
+        a.m_out[held] = m_out[b];
+        a.w[held] = w[b];
+      }
+      if (held == kSmall) launch();
+    }
+  }
+  if (held) launch();
+  return check_launch(who);
+}
+
+int32_t run(const char* who, const llattn_muon_cfg* c, const llattn_muon_group* groups, const void* const* g,
+            const float* const* m, const void* const* w, float* const* m_out, void* const* out, void* workspace,
+            size_t workspace_bytes, hipStream_t st) {
+  if (const int32_t rc = check(c, groups)) return rc;
+  Call k{c, groups, plan_of(c, groups), st, {}, nullptr, nullptr, m != nullptr, {}};
+  const Plan& p = k.p;
   if (!workspace || workspace_bytes < p.bytes() || !aligned16(workspace))
     return fail(LLATTN_ERR_WORKSPACE, "%s: needs %zu workspace bytes (got %zu)", who, p.bytes(), workspace_bytes);
-  const bool update = m != nullptr;
-  if (!g || !out || (update && (!w || !m_out))) return fail(LLATTN_ERR_LAYOUT, "%s: null pointer array", who);
+  if (!g || !out || (k.update && (!w || !m_out))) return fail(LLATTN_ERR_LAYOUT, "%s: null pointer array", who);
   const auto misplaced = [](const void* q, int dtype) { return !q || (uintptr_t)q % (size_t)elem_size(dtype); };
-  for (int i = 0; i < c->batch; ++i)
-    if (misplaced(g[i], c->g_dtype) || misplaced(out[i], c->w_dtype) ||
-        (update && (misplaced(m[i], LLATTN_F32) || misplaced(m_out[i], LLATTN_F32) || misplaced(w[i], c->w_dtype))))
-      return fail(LLATTN_ERR_LAYOUT, "%s: matrix %d has a null or misaligned pointer", who, i);
   char* ws = static_cast<char*>(workspace);
-  uint16_t* X[2] = {reinterpret_cast<uint16_t*>(ws), reinterpret_cast<uint16_t*>(ws + p.x)};
-  uint16_t* A = reinterpret_cast<uint16_t*>(ws + 2 * p.x);
-  uint16_t* B = reinterpret_cast<uint16_t*>(ws + 2 * p.x + p.a);
-  double* part = reinterpret_cast<double*>(ws + 2 * p.x + 2 * p.a);
-  const float sx = std::exp2f((float)std::min(14, (int)(0.5 * std::log2((double)p.m * p.n))));
-  const float one_mu = (float)(1.0 - (double)c->mu);
+  k.X[0] = reinterpret_cast<uint16_t*>(ws);
+  k.X[1] = reinterpret_cast<uint16_t*>(ws + p.x);
+  k.A = reinterpret_cast<uint16_t*>(ws + 2 * p.x);
+  k.B = reinterpret_cast<uint16_t*>(ws + 2 * p.x + p.a);
 
   PrepArgs pa{};
-  SplitArgs sa{};
-  NsArgs na{};
-  for (int i = 0; i < c->batch; ++i) {
-    pa.g.p[i] = sa.g.p[i] = g[i];
-    na.out.p[i] = out[i];
-    if (!update) continue;
-    pa.m.p[i] = m[i];
-    pa.m_out.p[i] = m_out[i];
-    sa.m.p[i] = m_out[i];
-    na.w.p[i] = w[i];
-  }
-  pa.n = (int64_t)c->rows * c->cols;
-  pa.g_dtype = sa.g_dtype = c->g_dtype;
-  pa.momentum = sa.momentum = update;
-  pa.nesterov = sa.nesterov = c->nesterov;
-  pa.blocks = sa.blocks = p.blocks;
-  pa.mu = sa.mu = c->mu;
-  pa.one_mu = sa.one_mu = one_mu;
-  pa.part = part;
-  hipLaunchKernelGGL(muon_prep_kernel, dim3(p.blocks, c->batch), dim3(256), 0, st, pa);
-  sa.rows = c->rows; sa.cols = c->cols; sa.flip = c->rows > c->cols;
-  sa.eps = c->eps; sa.scale = sx; sa.part = part;
-  sa.x = X[0]; sa.ld = 2 * (int64_t)p.np; sa.batch_stride = (int64_t)p.mp * p.np * 2;
-  sa.mp = p.mp; sa.np = p.np;
-  hipLaunchKernelGGL(muon_split_kernel, dim3((p.mp / 64) * (p.np / 64), c->batch), dim3(256), 0, st, sa);
-
-  const int64_t lx = sa.ld, sx_stride = sa.batch_stride, la = 2 * (int64_t)p.mp, sa_stride = (int64_t)p.mp * p.mp * 2;
-  na.rows = c->rows; na.cols = c->cols; na.flip = sa.flip; na.w_dtype = c->w_dtype; na.update = update;
-  na.keep = c->keep; na.step = c->step;
-  for (int i = 0; i < c->steps; ++i) {
-    const uint16_t* x = X[i & 1];
-    na.A = na.B = x; na.lda = na.ldb = lx; na.a_stride = na.b_stride = sx_stride;
-    na.C = A; na.ldc = la; na.c_stride = sa_stride;
-    na.steps = p.np / 32; na.beta = kSA / (sx * sx);
-    launch_ns<GRAM>(na, p, c->batch, st);
-    na.A = na.B = na.D = A; na.lda = na.ldb = na.ldd = la; na.a_stride = na.b_stride = na.d_stride = sa_stride;
-    na.C = B;
-    na.steps = p.mp / 32; na.alpha = c->b; na.beta = c->c / kSA;
-    launch_ns<POLY>(na, p, c->batch, st);
-    na.A = B;
-    na.B = na.D = x; na.ldb = na.ldd = lx; na.b_stride = na.d_stride = sx_stride;
-    na.C = X[(i + 1) & 1]; na.ldc = lx; na.c_stride = sx_stride;
-    na.alpha = c->a; na.beta = 1.f / kSA;
-    if (i + 1 < c->steps) {
-      launch_ns<APPLY>(na, p, c->batch, st);
-    } else {
-      na.alpha /= sx;
-      na.beta /= sx;
-      launch_ns<LAST>(na, p, c->batch, st);
+  LastArgs na{};
+  ElemArgs& e = pa.e;
+  e.n_groups = c->n_groups;
+  e.momentum = k.update;
+  e.nesterov = c->nesterov;
+  e.mu = c->mu;
+  e.one_mu = (float)(1.0 - (double)c->mu);
+  e.eps = c->eps;
+  e.part = reinterpret_cast<double*>(ws + 2 * p.x + 2 * p.a);
+  e.x = k.X[0];
+  int blocks = 0;
+  for (int i = 0; i < c->n_groups; ++i) {
+    const GroupPlan& q = p.g[i];
+    for (int b = q.first; b < q.first + groups[i].batch; ++b) {
+      if (misplaced(g[b], groups[i].g_dtype) || misplaced(out[b], groups[i].w_dtype) ||
+          (k.update && (misplaced(m[b], LLATTN_F32) || misplaced(m_out[b], LLATTN_F32) || misplaced(w[b], groups[i].w_dtype))))
+        return fail(LLATTN_ERR_LAYOUT, "%s: matrix %d has a null or misaligned pointer", who, b);
+      e.g.p[b] = g[b];
+      na.out.p[b] = out[b];
+      if (!k.update) continue;
+      e.m.p[b] = m[b];
+      pa.m_out.p[b] = m_out[b];
+      na.w.p[b] = w[b];
     }
+    ElemGroup& t = e.grp[i];
+    t.b0 = blocks;
+    t.blocks = t.parts = q.parts;
+    t.first = q.first; t.rows = groups[i].rows; t.cols = groups[i].cols; t.flip = t.rows > t.cols;
+    t.g_dtype = groups[i].g_dtype; t.mp = q.mp; t.np = q.np;
+    t.scale = scale_of(q);
+    t.x_off = (int64_t)q.x_off;
+    t.part0 = q.part0;
+    blocks += groups[i].batch * q.parts;
+  }
+  if (all_small(c, p)) return run_small(who, c, groups, p, g, m, w, m_out, out, k.update, st);
+  k.kind[GRAM] = choose<true>(c, groups, p, true);
+  k.kind[POLY] = choose<true>(c, groups, p, false);
+  k.kind[APPLY] = choose<false>(c, groups, p, false);
+  hipLaunchKernelGGL(muon_prep_kernel, dim3(blocks), dim3(256), 0, st, pa);
+  blocks = 0;
+  for (int i = 0; i < c->n_groups; ++i) {  // one workgroup per 64 x 64 tile of X
+    e.grp[i].b0 = blocks;
+    e.grp[i].blocks = (p.g[i].mp / 64) * (p.g[i].np / 64);
+    blocks += groups[i].batch * e.grp[i].blocks;
+  }
+  for (int b = 0; b < p.matrices; ++b) e.m.p[b] = pa.m_out.p[b];
+  hipLaunchKernelGGL(muon_split_kernel, dim3(blocks), dim3(256), 0, st, e);
+
+  na.n.a = k.A;
+  na.n.b = k.B;
+  na.n.update = k.update;
+  for (int i = 0; i < c->steps; ++i) {
+    na.n.x = k.X[i & 1];
+    na.n.y = k.X[(i + 1) & 1];
+    launch_products<GRAM>(k, na);
+    launch_products<POLY>(k, na);
+    if (i + 1 < c->steps) launch_products<APPLY>(k, na);
+    else launch_products<LAST>(k, na);
   }
   return check_launch(who);
 }
@@ -480,18 +1170,21 @@ int32_t run(const char* who, const llattn_muon_cfg* c, const void* const* g, con
 
 using namespace llattn;
 
-extern "C" size_t llattn_muon_bytes(const llattn_muon_cfg* c) { return check(c) == LLATTN_OK ? plan_of(c).bytes() : 0; }
+extern "C" size_t llattn_muon_bytes(const llattn_muon_cfg* c, const llattn_muon_group* groups) {
+  return check(c, groups) == LLATTN_OK ? plan_of(c, groups).bytes() : 0;
+}
 
-extern "C" int32_t llattn_orthogonalize(const llattn_muon_cfg* c, const void* const* g, void* const* out, void* workspace,
-                                        size_t workspace_bytes, void* stream) {
-  return run("llattn_orthogonalize", c, g, nullptr, nullptr, nullptr, out, workspace, workspace_bytes,
+extern "C" int32_t llattn_orthogonalize(const llattn_muon_cfg* c, const llattn_muon_group* groups, const void* const* g,
+                                        void* const* out, void* workspace, size_t workspace_bytes, void* stream) {
+  return run("llattn_orthogonalize", c, groups, g, nullptr, nullptr, nullptr, out, workspace, workspace_bytes,
              static_cast<hipStream_t>(stream));
 }
 
-extern "C" int32_t llattn_muon_update(const llattn_muon_cfg* c, const void* const* g, const float* const* m,
-                                      const void* const* w, float* const* m_out, void* const* w_out, void* workspace,
-                                      size_t workspace_bytes, void* stream) {
+extern "C" int32_t llattn_muon_update(const llattn_muon_cfg* c, const llattn_muon_group* groups, const void* const* g,
+                                      const float* const* m, const void* const* w, float* const* m_out, void* const* w_out,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
   if (!m) return fail(LLATTN_ERR_LAYOUT, "llattn_muon_update: null momentum array");
   if (c && !(c->mu >= 0.f && c->mu < 1.f)) return fail(LLATTN_ERR_SHAPE, "llattn_muon_update: momentum %g outside [0, 1)", c->mu);
-  return run("llattn_muon_update", c, g, m, w, m_out, w_out, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+  return run("llattn_muon_update", c, groups, g, m, w, m_out, w_out, workspace, workspace_bytes,
+             static_cast<hipStream_t>(stream));
 }

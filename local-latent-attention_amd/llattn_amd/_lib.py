@@ -83,12 +83,17 @@ class LlattnHeadCfg(ctypes.Structure):  # include/llattn_train.h
     _fields_ = [(n, ctypes.c_int32) for n in ("rows", "V", "D", "piece", "dw_dtype")]
 
 
-MUON_BATCH = 128  # LLATTN_MUON_BATCH
+MUON_BATCH, MUON_GROUPS = 128, 16  # LLATTN_MUON_BATCH, LLATTN_MUON_GROUPS
+
+
+class LlattnMuonGroup(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("batch", "rows", "cols", "g_dtype", "w_dtype")] + \
+        [(n, ctypes.c_float) for n in ("keep", "step")]
 
 
 class LlattnMuonCfg(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_int32) for n in ("batch", "rows", "cols", "g_dtype", "w_dtype", "steps", "nesterov")] + \
-        [(n, ctypes.c_float) for n in ("a", "b", "c", "eps", "mu", "keep", "step")]
+    _fields_ = [(n, ctypes.c_int32) for n in ("n_groups", "steps", "nesterov", "tiles")] + \
+        [(n, ctypes.c_float) for n in ("a", "b", "c", "eps", "mu")]
 
 
 _P = ctypes.c_void_p
@@ -146,14 +151,14 @@ STEP_SIGNATURES = {
 }
 
 # the same for include/llattn_train.h
-_HC, _MC, _PP = ctypes.POINTER(LlattnHeadCfg), ctypes.POINTER(LlattnMuonCfg), ctypes.POINTER(ctypes.c_void_p)
+_HC, _MC, _MG, _PP = (ctypes.POINTER(t) for t in (LlattnHeadCfg, LlattnMuonCfg, LlattnMuonGroup, ctypes.c_void_p))
 TRAIN_SIGNATURES = {
     "llattn_head_bytes": (_SZ, [_HC, _I32]),
     "llattn_head_fwd": (_I32, [_HC, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "llattn_head_bwd": (_I32, [_HC, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I32, _P, _P, _P, _P, _SZ, _P]),
-    "llattn_muon_bytes": (_SZ, [_MC]),
-    "llattn_orthogonalize": (_I32, [_MC, _PP, _PP, _P, _SZ, _P]),
-    "llattn_muon_update": (_I32, [_MC, _PP, _PP, _PP, _PP, _PP, _P, _SZ, _P]),
+    "llattn_muon_bytes": (_SZ, [_MC, _MG]),
+    "llattn_orthogonalize": (_I32, [_MC, _MG, _PP, _PP, _P, _SZ, _P]),
+    "llattn_muon_update": (_I32, [_MC, _MG, _PP, _PP, _PP, _PP, _PP, _P, _SZ, _P]),
 }
 
 _lib = None

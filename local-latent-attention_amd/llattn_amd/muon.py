@@ -22,16 +22,18 @@ from . import _lib as L
 # coefficients that raise small singular values fastest while those near 1 stay within about 0.7 to 1.2
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 SCALES = ("aspect", "rms")
-WORKSPACE_BYTES = 4 << 30  # matrices of one shape are taken together up to this
+WORKSPACE_BYTES = 4 << 30  # matrices are taken together up to this
 
 
-def _config(batch, shape, g_dtype, w_dtype, steps, coefficients, eps, nesterov=False, mu=0.0, keep=0.0, step=0.0):
-    return L.LlattnMuonCfg(batch, *shape, L.dtype_code(g_dtype), L.dtype_code(w_dtype), steps, int(nesterov),
-                           *[float(v) for v in coefficients], float(eps), mu, keep, step)
+TILES = 0  # workgroups of the products: the library's choice (llattn_muon_cfg.tiles)
 
 
-def _bytes(cfg) -> int:
-    n = L.load().llattn_muon_bytes(ctypes.byref(cfg))
+def _config(steps, coefficients, eps, nesterov=False, mu=0.0):
+    return L.LlattnMuonCfg(0, steps, int(nesterov), TILES, *[float(v) for v in coefficients], float(eps), mu)
+
+
+def _bytes(cfg, groups) -> int:
+    n = L.load().llattn_muon_bytes(ctypes.byref(cfg), groups)
     if n == 0:
         L.check(L.ERR_SHAPE, "llattn_muon_bytes")
     return n
@@ -41,10 +43,39 @@ def _pointers(values):
     return (ctypes.c_void_p * len(values))(*values)
 
 
-def _chunk(cfg) -> int:
-    """Matrices of a call: what fits the workspace, at least one."""
-    cfg.batch = 1
-    return max(1, min(L.MUON_BATCH, WORKSPACE_BYTES // _bytes(cfg)))
+def _padded(shape) -> int:
+    """Bytes of workspace that a matrix takes."""
+    m, n = (v + -v % 64 for v in sorted(shape))
+    return 8 * m * (n + m)
+
+
+def _calls(kinds):
+    """``kinds``: a list of (shape, count) of alike matrices in a row.  Cuts it into calls: lists of (kind, first, count)
+    of at most 16 kinds, 128 matrices and the workspace's bytes (one matrix at least)."""
+    call, held, room = [], 0, WORKSPACE_BYTES
+    for k, (shape, count) in enumerate(kinds):
+        each, first = _padded(shape), 0
+        while first < count:
+            n = min(count - first, L.MUON_BATCH - held, max(room // each, 0 if call else 1))
+            if n == 0 or len(call) == L.MUON_GROUPS:
+                yield call
+                call, held, room = [], 0, WORKSPACE_BYTES
+                continue
+            call.append((k, first, n))
+            held, room, first = held + n, room - n * each, first + n
+    if call:
+        yield call
+
+
+def _launch(name, cfg, groups, device, *pointers, work):
+    """One call of ``name`` with its workspace."""
+    table = (L.LlattnMuonGroup * len(groups))(*groups)
+    cfg.n_groups = len(groups)
+    n = _bytes(cfg, table)
+    ws = torch.empty((n,), dtype=torch.uint8, device=device)
+    from .ops import _call
+    with L.on_device(device):
+        _call(name, ctypes.byref(cfg), table, *[_pointers(p) for p in pointers], ws.data_ptr(), n, L.stream_ptr(device), work=work)
 
 
 def _check_numbers(who, steps, eps, coefficients):
@@ -77,56 +108,60 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, eps: float = 1e-7, coefficien
     if x.numel() == 0:
         return out
     src = x.detach().contiguous()
-    count, dev = x.numel() // (m * n), x.device
-    cfg = _config(1, (m, n), x.dtype, x.dtype, steps, coefficients, eps)
-    most, each = _chunk(cfg), m * n * x.element_size()
-    from .ops import _call
-    with L.on_device(dev):
-        for i in range(0, count, most):
-            cfg.batch = k = min(most, count - i)
-            nws = _bytes(cfg)
-            ws = torch.empty((nws,), dtype=torch.uint8, device=dev)
-            _call("llattn_orthogonalize", ctypes.byref(cfg), _pointers([src.data_ptr() + (i + j) * each for j in range(k)]),
-                  _pointers([out.data_ptr() + (i + j) * each for j in range(k)]), ws.data_ptr(), nws, L.stream_ptr(dev),
-                  work=2 * k * each)
+    each, dt = m * n * x.element_size(), L.dtype_code(x.dtype)
+    cfg = _config(steps, coefficients, eps)
+    for call in _calls([((m, n), x.numel() // (m * n))]):
+        (_, first, k), = call
+        at = range(first * each, (first + k) * each, each)
+        _launch("llattn_orthogonalize", cfg, [L.LlattnMuonGroup(k, m, n, dt, dt, 0.0, 0.0)], x.device,
+                [src.data_ptr() + i for i in at], [out.data_ptr() + i for i in at], work=2 * k * each)
     _written([out])
     return out
 
 
 def _written(tensors) -> None:
     """Tensors that a kernel has written in place, for autograd's checks of what it saved."""
-    for t in tensors:
-        torch.autograd.graph.increment_version(t)
+    torch.autograd.graph.increment_version(tensors)
 
 
 def _update_scale(scale: str, rows: int, cols: int) -> float:
     return math.sqrt(max(1.0, rows / cols)) if scale == "aspect" else 0.2 * math.sqrt(max(rows, cols))
 
 
-def _check_update(weights, grads, momenta, out):
+def _rows(weights, grads, momenta, out):
+    """The checked matrices as rows of tensors and data pointers: (w, g, m, w_out, m_out, pointers of w, m, w_out, m_out, g),
+    gradients contiguous."""
     lists = [weights, grads, momenta, *out]
     if len({len(v) for v in lists}) != 1:
         raise ValueError(f"muon_update: lists of different lengths ({', '.join(str(len(v)) for v in lists)})")
+    f32, types = torch.float32, (torch.float32, torch.bfloat16)
+    rows = []
     for w, g, m, wo, mo in zip(*lists):
-        if w.dim() != 2 or 0 in w.shape:
-            raise ValueError(f"muon_update: weights must be non-empty matrices, got shape {tuple(w.shape)}")
-        L.dtype_code(w.dtype), L.dtype_code(g.dtype)
-        if any(t.shape != w.shape or t.device != w.device for t in (g, m, wo, mo)):
-            raise ValueError(f"muon_update: gradient, momentum and outputs must have their weight's shape "
-                             f"{tuple(w.shape)} and device")
-        if m.dtype is not torch.float32 or mo.dtype is not torch.float32 or wo.dtype is not w.dtype:
+        shape, dev = w.shape, w.get_device()
+        if len(shape) != 2 or 0 in shape:
+            raise ValueError(f"muon_update: weights must be non-empty matrices, got shape {tuple(shape)}")
+        if w.dtype not in types or g.dtype not in types:
+            raise ValueError(f"muon_update: weights and gradients must be fp32 or bf16, got {w.dtype} and {g.dtype}")
+        same = g.shape == shape and m.shape == shape and g.get_device() == dev and m.get_device() == dev
+        if wo is not w or mo is not m:
+            same = same and wo.shape == shape and mo.shape == shape and wo.get_device() == dev and mo.get_device() == dev
+        if not same:
+            raise ValueError(f"muon_update: gradient, momentum and outputs must have their weight's shape {tuple(shape)} "
+                             "and device")
+        if m.dtype is not f32 or mo.dtype is not f32 or wo.dtype is not w.dtype:
             raise ValueError("muon_update: momenta must be fp32 and new weights of their weight's type")
-        if not all(t.is_contiguous() for t in (w, m, wo, mo)):
+        if not (w.is_contiguous() and m.is_contiguous() and wo.is_contiguous() and mo.is_contiguous()):
             raise ValueError("muon_update: weights, momenta and outputs must be contiguous")
-    new = {}
-    for k, pair in enumerate(zip(*out)):
-        for t in pair:
-            if new.setdefault(t.data_ptr(), k) != k or pair[0].data_ptr() == pair[1].data_ptr():
-                raise ValueError("muon_update: a tensor is written twice")
-    for k, (w, g, m, wo, mo) in enumerate(zip(*lists)):
-        for t, own in ((w, wo), (m, mo), (g, None)):
-            if t.data_ptr() in new and (own is None or new[t.data_ptr()] != k or t.data_ptr() != own.data_ptr()):
-                raise ValueError("muon_update: an output is another tensor's input")
+        if not g.is_contiguous():
+            g = g.contiguous()
+        rows.append((w, g, m, wo, mo, w.data_ptr(), m.data_ptr(), wo.data_ptr(), mo.data_ptr(), g.data_ptr()))
+    new = {p for r in rows for p in r[7:9]}
+    if len(new) != 2 * len(rows):
+        raise ValueError("muon_update: a tensor is written twice")
+    for _, _, _, _, _, w, m, wo, mo, g in rows:
+        if (w != wo and w in new) or (m != mo and m in new) or g in new:
+            raise ValueError("muon_update: an output is another tensor's input")
+    return rows
 
 
 @torch.no_grad()
@@ -141,8 +176,8 @@ def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nest
         W <- (1 - lr weight_decay) W - lr s orthogonalize(U)
 
     with ``s = sqrt(max(1, m / n))`` (``scale="aspect"``) or ``0.2 sqrt(max(m, n))`` (``"rms"``: the size of an AdamW
-    update).  Weights and momenta change in place, or ``out = (new weights, new momenta)`` receives them.  Matrices of
-    one shape share launches.  ``lr`` is a number: a captured graph keeps it.  GPU only."""
+    update).  Weights and momenta change in place, or ``out = (new weights, new momenta)`` receives them.  The matrices
+    of a call share launches, whatever their shapes.  ``lr`` is a number: a captured graph keeps it.  GPU only."""
     weights, grads, momenta = list(weights), list(grads), list(momenta)
     out = (weights, momenta) if out is None else tuple(list(v) for v in out)
     if len(out) != 2:
@@ -155,26 +190,24 @@ def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nest
     if scale not in SCALES:
         raise ValueError(f"muon_update: scale must be one of {SCALES}, got {scale!r}")
     _check_numbers("muon_update", steps, eps, coefficients)
-    _check_update(weights, grads, momenta, out)
+    rows = _rows(weights, grads, momenta, out)
     L.require_gpu(*weights)
-    groups: dict = {}
-    for row in zip(weights, grads, momenta, *out):
-        groups.setdefault((tuple(row[0].shape), row[0].dtype, row[1].dtype, row[0].device), []).append(row)
-    from .ops import _call
-    for (shape, w_dtype, g_dtype, dev), rows in groups.items():
-        cfg = _config(1, shape, g_dtype, w_dtype, steps, coefficients, eps, nesterov, float(momentum),
-                      1.0 - lr * weight_decay, lr * _update_scale(scale, *shape))
-        most = _chunk(cfg)
-        with L.on_device(dev):
-            for i in range(0, len(rows), most):
-                part = rows[i:i + most]
-                cfg.batch = len(part)
-                n = _bytes(cfg)
-                ws = torch.empty((n,), dtype=torch.uint8, device=dev)
-                g = [r[1].contiguous() for r in part]
-                w, m, wo, mo = (_pointers([r[k].data_ptr() for r in part]) for k in (0, 2, 3, 4))
-                _call("llattn_muon_update", ctypes.byref(cfg), _pointers([t.data_ptr() for t in g]), m, w, mo, wo,
-                      ws.data_ptr(), n, L.stream_ptr(dev), work=12 * len(part) * shape[0] * shape[1])
+    devices: dict = {}
+    for row in rows:
+        devices.setdefault(row[0].get_device(), {}).setdefault((row[0].shape, row[0].dtype, row[1].dtype), []).append(row)
+    cfg = _config(steps, coefficients, eps, nesterov, float(momentum))
+    for kinds in devices.values():
+        keys = list(kinds)
+        dev = kinds[keys[0]][0][0].device
+        for call in _calls([(k[0], len(kinds[k])) for k in keys]):
+            groups, part = [], []
+            for k, first, n in call:
+                shape, w_dtype, g_dtype = keys[k]
+                groups.append(L.LlattnMuonGroup(n, *shape, L.dtype_code(g_dtype), L.dtype_code(w_dtype), 1.0 - lr * weight_decay,
+                                                lr * _update_scale(scale, *shape)))
+                part += kinds[keys[k]][first:first + n]
+            _launch("llattn_muon_update", cfg, groups, dev, *[[r[k] for r in part] for k in (9, 6, 5, 8, 7)],
+                    work=sum(12 * q.batch * q.rows * q.cols for q in groups))
     _written([t for v in out for t in v])
 
 

@@ -100,6 +100,26 @@ def test_orthogonalize(batch, m, n, kind):
     _near(_muon().orthogonalize(x), x, f"{batch}x{m}x{n} {kind}")
 
 
+@pytest.mark.parametrize("tiles", [1, 2, 3, 4])
+@pytest.mark.parametrize("batch,m,n", [(2, 33, 70), (1, 64, 64), (3, 130, 200), (2, 257, 130), (1, 333, 1001), (2, 390, 514),
+                                       (9, 450, 449), (1, 1408, 700)])
+def test_every_workgroup_of_the_products(tiles, batch, m, n, monkeypatch):
+    """Tiles inside the matrices, ragged, half outside and larger than them; an update of the same in place."""
+    mu = _muon()
+    monkeypatch.setattr(mu, "TILES", tiles)
+    x = _matrices(batch, m, n, "decay", seed=m + tiles)
+    _near(mu.orthogonalize(x), x, f"tiles {tiles}: {batch}x{m}x{n}")
+    ws, ms = [torch.zeros(m, n, device=DEV) for _ in x], [torch.zeros(m, n, device=DEV) for _ in x]
+    mu.muon_update(ws, list(x), ms, lr=1.0, momentum=0.0)  # W = -s ns(G)
+    _near(torch.stack(ws) / -math.sqrt(max(1.0, m / n)), x, f"tiles {tiles}: update")
+
+
+@pytest.mark.parametrize("batch,m,n", [(1, 1408, 4096), (6, 1000, 1500), (16, 640, 1300), (2, 2048, 640), (12, 1408, 1408)])
+def test_large_matrices(batch, m, n):
+    x = _matrices(batch, m, n, "flat")
+    _near(_muon().orthogonalize(x), x, f"{batch}x{m}x{n}")
+
+
 @pytest.mark.parametrize("m,n", [(70, 90), (90, 70), (256, 256)])
 def test_orthogonalize_bf16(m, n):
     x = _matrices(3, m, n, "decay").to(BF16)

@@ -20,12 +20,13 @@ def test_header_matches_the_binding(tmp_path):
     text = (REPO / "include" / "llattn_train.h").read_text()
     names = set(re.findall(r"^\s*(?:int32_t|size_t)\s+(llattn_\w+)\s*\(", text, re.M))
     assert names == set(L.TRAIN_SIGNATURES) and all(hasattr(L.load(), n) for n in names)
-    structs = {"llattn_head_cfg": L.LlattnHeadCfg, "llattn_muon_cfg": L.LlattnMuonCfg}
+    structs = {"llattn_head_cfg": L.LlattnHeadCfg, "llattn_muon_cfg": L.LlattnMuonCfg,
+               "llattn_muon_group": L.LlattnMuonGroup}
     lines = ["#include <stddef.h>", "#include <stdio.h>", '#include "llattn_train.h"', "int main(void) {"]
     for c, t in structs.items():
         lines.append(f'printf("%zu\\n", sizeof({c}));')
         lines += [f'printf("%zu\\n", offsetof({c}, {f[0]}));' for f in t._fields_]
-    lines += ['printf("%d\\n", LLATTN_MUON_BATCH);', "return 0; }"]
+    lines += ['printf("%d\\n%d\\n", LLATTN_MUON_BATCH, LLATTN_MUON_GROUPS);', "return 0; }"]
     src = tmp_path / "l.c"
     src.write_text("\n".join(lines))
     subprocess.run(["gcc", f"-I{REPO / 'include'}", str(src), "-o", str(tmp_path / "l")], check=True)
@@ -34,7 +35,7 @@ def test_header_matches_the_binding(tmp_path):
     for t in structs.values():
         want.append(ctypes.sizeof(t))
         want += [getattr(t, f[0]).offset for f in t._fields_]
-    assert got == want + [L.MUON_BATCH]
+    assert got == want + [L.MUON_BATCH, L.MUON_GROUPS]
 
 
 @pytest.mark.parametrize("cfg,which", [((0, 10, 8, 0, 0), 0), ((4, 0, 8, 0, 0), 0), ((4, 10, 0, 0, 0), 0), ((4, 10, 12, 0, 0), 1),
@@ -93,35 +94,60 @@ def test_piecewise_head_loss_refusals():
         piecewise_head_loss(h, w, t)
 
 
-GOOD = dict(batch=1, rows=4, cols=8, g_dtype=0, w_dtype=0, steps=5, nesterov=1, a=3.4445, b=-4.775, c=2.0315, eps=1e-7, mu=0.95,
-            keep=1.0, step=0.1)
+CFG = dict(n_groups=1, steps=5, nesterov=1, tiles=0, a=3.4445, b=-4.775, c=2.0315, eps=1e-7, mu=0.95)
+GROUP = dict(batch=1, rows=4, cols=8, g_dtype=0, w_dtype=0, keep=1.0, step=0.1)
+
+
+def _muon_cfg(**kw):
+    group = L.LlattnMuonGroup(*{**GROUP, **{k: v for k, v in kw.items() if k in GROUP}}.values())
+    return L.LlattnMuonCfg(*{**CFG, **{k: v for k, v in kw.items() if k in CFG}}.values()), (L.LlattnMuonGroup * 20)(*[group] * 20)
 
 
 @pytest.mark.parametrize("kw", [dict(batch=0), dict(batch=129), dict(rows=0), dict(cols=-1), dict(rows=32769), dict(g_dtype=2),
                                 dict(w_dtype=-1), dict(steps=0), dict(steps=101), dict(eps=-1.0), dict(eps=float("nan")),
-                                dict(a=5.0), dict(a=2.0, b=0.0, c=0.0), dict(b=-20.0), dict(c=float("nan"))])
+                                dict(a=5.0), dict(a=2.0, b=0.0, c=0.0), dict(b=-20.0), dict(c=float("nan")), dict(n_groups=0),
+                                dict(n_groups=17), dict(n_groups=2, batch=65), dict(tiles=-1), dict(tiles=5)])
 def test_muon_configurations_refused(kw):
     lib = L.load()
-    assert lib.llattn_muon_bytes(ctypes.byref(L.LlattnMuonCfg(*GOOD.values()))) > 0
-    assert lib.llattn_muon_bytes(ctypes.byref(L.LlattnMuonCfg(*{**GOOD, **kw}.values()))) == 0
+    cfg, groups = _muon_cfg()
+    assert lib.llattn_muon_bytes(ctypes.byref(cfg), groups) > 0
+    cfg, groups = _muon_cfg(**kw)
+    assert lib.llattn_muon_bytes(ctypes.byref(cfg), groups) == 0
     assert b"llattn_muon" in lib.llattn_last_error()
 
 
 def test_muon_calls_refused():
-    lib, cfg, p = L.load(), L.LlattnMuonCfg(*GOOD.values()), ctypes.c_void_p
+    lib, p = L.load(), ctypes.c_void_p
+    cfg, groups = _muon_cfg()
     one, odd, none = (muon._pointers([v]) for v in (1 << 20, (1 << 20) + 2, None))
-    ref = ctypes.byref(cfg)
-    assert lib.llattn_orthogonalize(ref, one, one, None, 1 << 30, None) == L.ERR_WORKSPACE
-    assert lib.llattn_orthogonalize(ref, one, one, p(1 << 20), 16, None) == L.ERR_WORKSPACE
+    ref = ctypes.byref(cfg), groups
+    assert lib.llattn_orthogonalize(*ref, one, one, None, 1 << 30, None) == L.ERR_WORKSPACE
+    assert lib.llattn_orthogonalize(*ref, one, one, p(1 << 20), 16, None) == L.ERR_WORKSPACE
     for g, o in ((none, one), (one, none), (odd, one), (one, odd), (None, one), (one, None)):
-        assert lib.llattn_orthogonalize(ref, g, o, p(1 << 20), 1 << 40, None) == L.ERR_LAYOUT
+        assert lib.llattn_orthogonalize(*ref, g, o, p(1 << 20), 1 << 40, None) == L.ERR_LAYOUT
     for k in range(5):
         for v in (none, odd, None):
             args = [one] * 5
             args[k] = v
-            assert lib.llattn_muon_update(ref, *args, p(1 << 20), 1 << 40, None) == L.ERR_LAYOUT
-    bad = L.LlattnMuonCfg(*{**GOOD, "mu": 1.0}.values())
-    assert lib.llattn_muon_update(ctypes.byref(bad), *[one] * 5, p(1 << 20), 1 << 40, None) == L.ERR_SHAPE
+            assert lib.llattn_muon_update(*ref, *args, p(1 << 20), 1 << 40, None) == L.ERR_LAYOUT
+    bad, groups = _muon_cfg(mu=1.0)
+    assert lib.llattn_muon_update(ctypes.byref(bad), groups, *[one] * 5, p(1 << 20), 1 << 40, None) == L.ERR_SHAPE
+
+
+def test_muon_calls_are_cut():
+    """Every matrix once, in order, within 16 kinds, 128 matrices and the workspace that the library asks for."""
+    for kinds in ([((64, 128), 300)], [((8 + i, 9), 1 + i) for i in range(40)], [((4096, 4096), 60), ((16, 16), 3)],
+                  [((32768, 32768), 2), ((8, 8), 1)], []):
+        seen = [[] for _ in kinds]
+        for call in muon._calls(kinds):
+            assert 0 < len(call) <= L.MUON_GROUPS and sum(n for _, _, n in call) <= L.MUON_BATCH
+            groups = [L.LlattnMuonGroup(n, *kinds[k][0], 0, 0, 1.0, 0.1) for k, _, n in call]
+            cfg, _ = _muon_cfg(n_groups=len(groups))
+            n = L.load().llattn_muon_bytes(ctypes.byref(cfg), (L.LlattnMuonGroup * len(groups))(*groups))
+            assert 0 < n <= muon.WORKSPACE_BYTES + (1 << 20) or len(groups) == groups[0].batch == 1
+            for k, first, n in call:
+                seen[k] += range(first, first + n)
+        assert seen == [list(range(c)) for _, c in kinds]
 
 
 def test_orthogonalize_refusals():
