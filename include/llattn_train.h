@@ -23,7 +23,8 @@ extern "C" {
  * logsumexp_v l[n] / ln 2 (what the backward reads, and nothing else does),
  * and, with pred non-null, pred[n] = first index of the row's maximum.  With
  * total non-null (one fp32 value): the sum of loss, or with inv non-null too
- * its mean over the rows that count, inv receiving 1 / their number.
+ * its mean over the rows that count, inv receiving 1 / their number (NaN and 0
+ * where there are none).
  *
  * Backward: dl[n][v] = (softmax(l[n])_v - [v == t_n]) * s_n with s_n =
  * grad[n * grad_stride] (grad_stride 0 or 1) * (inv ? *inv : 1), 0 in

@@ -227,6 +227,24 @@ __device__ __forceinline__ bf16x8 frag64(const unsigned char* tile, int o16, int
   }
 }
 
+// f(integral_constant 0), f(1), ..., f(N - 1)
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void unroll(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    unroll<N, I + 1>(f);
+  }
+}
+
+// One wave's copy of 64 x 16 bytes into the 1 KB LDS block at byte address lds + AT (buffer_load ... lds, as dma_block).
+template <int AT>
+__device__ __forceinline__ void dma_at(const i32x4& rs, uint32_t off, uint32_t lds) {
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+               :
+               : "v"(off), "s"(rs), "s"(lds), "i"(AT)
+               : "memory", "m0", "scc");
+}
+
 constexpr int SK = 64;  // k per stage
 
 // Tile operand of O rows / columns x 64 k.  k-contiguous: rows of 128 bytes, chunk c (8 k) of row o at slot
@@ -280,8 +298,6 @@ int resolve_split(const llattn_gemm_desc* d);
 // (llattn_gemm_tile.hip).
 struct TilePlan { int mb, nb, kg, splits; };
 TilePlan tile_plan(const llattn_gemm_desc* d, double* us = nullptr);  // us: the time it expects
-// llattn_gemm with `b_rows` <= K rows in an m/n-contiguous B: the rows past them read zero (A holds zeros there).
-int32_t product(const llattn_gemm_desc* d, int b_rows, void* workspace, size_t workspace_bytes, hipStream_t st);
 void launch_tile(const GemmArgs& a, const TilePlan& p, bool a_kmaj, bool b_kmaj, int c_dtype, hipStream_t st);
 // Two independent products in one launch: x Wᵀ or dy W into bf16, and then dyᵀ x into fp32 or (after x Wᵀ) another x Wᵀ.
 TilePlan pair_plan(const llattn_gemm_desc* d0, const llattn_gemm_desc* d1);

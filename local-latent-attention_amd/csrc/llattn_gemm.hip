@@ -946,12 +946,12 @@ extern "C" int32_t llattn_gemm_pair(const llattn_gemm_desc* d0, const llattn_gem
   return check_launch("llattn_gemm_pair");
 }
 
-int32_t gemm::product(const llattn_gemm_desc* d, int b_rows, void* workspace, size_t workspace_bytes, hipStream_t st) {
+extern "C" int32_t llattn_gemm(const llattn_gemm_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
   GemmArgs a;
   if (const int32_t rc = prepare(d, workspace, workspace_bytes, false, a)) return rc;
-  if (d->b_trans) a.b_bytes = ((int64_t)(b_rows - 1) * d->ldb + d->N) * 2;
   const int S = a.n_split, k_pairs = a.k_pairs;
   const HeadsMap ch = a.ch;
+  hipStream_t st = static_cast<hipStream_t>(stream);
   if (const TilePlan tp = tile_plan(d); tp.mb) {
     launch_tile(a, tp, !d->a_trans, !d->b_trans, d->c_dtype, st);
     if (tp.splits > 1) launch_reduce(a, tp.splits, d->c_dtype, st);
@@ -991,9 +991,4 @@ int32_t gemm::product(const llattn_gemm_desc* d, int b_rows, void* workspace, si
   else if (d->a_trans && d->b_trans) launch<false, false>(a, S, d->c_dtype, st);
   else launch<false, true>(a, S, d->c_dtype, st);
   return check_launch("llattn_gemm");
-}
-
-extern "C" int32_t llattn_gemm(const llattn_gemm_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!d) return fail(LLATTN_ERR_SHAPE, "llattn_gemm: null descriptor");
-  return product(d, d->K, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }

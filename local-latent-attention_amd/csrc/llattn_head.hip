@@ -10,9 +10,11 @@
 // given back to the joined sum, so its rounding cancels; loss = ((C - l_t log2 e) + log2 S) ln 2 takes the small
 // difference first.
 //
-// Backward: a piece of the vocabulary at a time, the same product again with dl (bf16) in its epilogue, then dh (+)=
-// dl W and dW = dlᵀ h on the GEMM kernels.  Rounding dl to bf16 is as far off as rounding the results to bf16 is (half
-// a step of 2^-8 each), and those errors average out over the contraction.
+// Backward: a piece of the vocabulary at a time, the same product again with q = softmax - onehot (bf16) in its epilogue,
+// then dh (+)= q W and dW = qᵀ h, times the scale that every row shares.  Rounding q to bf16 is as far off as rounding the
+// results to bf16 is (half a step of 2^-8 each), and those errors average out over the contraction.  The shared scale stays
+// out of q: within it, the entries near -1, which are one value in all rows, would round alike (1 / 4096 rows: 0.4% of
+// the whole gradient).  Only gradients that differ by row are multiplied in.
 //
 // What bounds it: 2 rows V D operations for each of the four products on the matrix cores; with few rows the reads of
 // W.
@@ -26,28 +28,31 @@ namespace {
 
 using namespace gemm;
 
+enum Epilogue { STATS = 0, STATS_PRED = 1, GRAD = 2, SUM = 3, OUT_BF16 = 4, OUT_F32 = 5 };
+
 struct HeadArgs {
-  int M, N, D;     // rows, columns of this piece, hidden size
-  int v0;          // first column of the piece in the vocabulary
-  int64_t V;       // vocabulary: targets outside [0, V) are errors
-  const uint16_t* h; int64_t ldh;
-  const uint16_t* w; int64_t ldw;  // at the piece's first row
+  int M, N, K;              // rows, columns, contraction
+  int steps, per;           // 64-wide k steps, of a split
   int tiles_m, tiles_n;
+  const uint16_t* A; int64_t lda; int64_t a_end;  // a_end: elements up to the operand's end
+  const uint16_t* B; int64_t ldb; int64_t b_end;
+  // logits
+  int v0;                   // first column of the piece in the vocabulary
+  int64_t V;                // targets outside [0, V) are errors
   const int64_t* targets;
   int64_t ignore_index;
-  // forward: parts [slots][M] and the target's logit [M]
-  float2* part;
+  float2* part;             // STATS: parts [slots][M] and the target's logit [M]
   int32_t* part_i;
   float* tgt;
-  // backward
-  const float* lse2;
-  const float* grad;
-  int grad_stride;
-  const float* inv;
+  const float* lse2;        // GRAD
   uint16_t* p; int64_t ldp;
+  // gradients: alpha = grad[0] * (inv ? *inv : 1), or grad[row] within q (per_row)
+  const float* grad;
+  const float* inv;
+  int per_row;
+  void* C;                  // SUM: fp32 [splits][M][N]
+  int accumulate;
 };
-
-enum Mode { STATS = 0, STATS_PRED = 1, GRAD = 2 };
 
 // (value, index) maximum with the smaller index on ties
 __device__ __forceinline__ void max_first(float& m, int& i, float m2, int i2) {
@@ -57,95 +62,266 @@ __device__ __forceinline__ void max_first(float& m, int& i, float m2, int i2) {
   }
 }
 
-// One (32 MB) x (32 NB) tile of l per workgroup, as tile_product of llattn_gemm_tile.hip: four waves, NST stages of
-// 64 k, loads NST - 1 steps ahead.  Offsets are taken from the tile's first row, so h and W may be of any size.
-template <int MODE, int MB, int NB, int NST>
-__global__ __launch_bounds__(256) void head_tile_kernel(const HeadArgs a) {
-  constexpr int TM = 32 * MB, TN = 32 * NB;
-  typedef TileOp<true, false, TM> OpA;
-  typedef TileOp<true, false, TN> OpB;
-  constexpr int STAGE = OpA::BYTES + OpB::BYTES, LOADS = OpA::NB + OpB::NB;
+// A shape of workgroup: WR x WC waves, each 16 MB x 16 NB of the tile, NST LDS stages of 64 k.
+template <int MB_, int NB_, int WR_, int WC_, int NST_>
+struct Shape {
+  static constexpr int MB = MB_, NB = NB_, WR = WR_, WC = WC_, NST = NST_;
+  static constexpr int W = WR * WC, THREADS = 64 * W, TM = 16 * MB * WR, TN = 16 * NB * WC, STAGE = (TM + TN) * 128;
+};
+
+// T rows of a step with its 64 k along them (128 bytes each), loaded by W waves.  Chunk c (8 k) of row o at c ^ swz(o).
+// PERM: lane r of fragment block j reads row 32 (j / 2) + 4 (j % 2) + 8 (r / 4) + r % 4, so that as the first operand a pair of
+// blocks gives each lane 8 consecutive columns of the product.
+template <int T, int W, bool PERM>
+struct RowOp {
+  static constexpr int BYTES = T * 128, LOADS = BYTES / 1024 / W;
+  uint32_t off[LOADS], base[2];  // base: of this lane's fragments, by 32-k half
+  int kc[LOADS];                 // first k of this lane's chunks
+  __device__ __forceinline__ void init(int64_t ld, int w, int lane, int o0) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = 8 * (w * LOADS + i) + (lane >> 3), c = (lane & 7) ^ pswz<PERM>(row);
+      off[i] = step_off((int64_t)row * ld * 2 + 16 * c);
+      kc[i] = 8 * c;
+    }
+    const int r = lane & 15, g = lane >> 4, row = PERM ? 8 * (r >> 2) + (r & 3) : r;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) base[h] = (o0 + row) * 128 + (((4 * h + g) ^ pswz<PERM>(row)) << 4);
+  }
+  // load i of a step with `left` k to the contraction's end: chunks past it read zero
+  __device__ __forceinline__ uint32_t at(int i, int left) const { return kmask(off[i], kc[i], left); }
+  // rows o0 + 16 i + r (PERM: as above), k 32 half + 8 g .. of the stage at st; o0 a multiple of 32
+  __device__ __forceinline__ bf16x8 frag(const unsigned char* st, int i, int half) const {
+    // PERM: the swizzle's third bit is bit 3 of the row and its low two those of r, so 4 and 32 rows on leave it alone
+    return *reinterpret_cast<const bf16x8*>(st + base[half] + (PERM ? (i >> 1) * 4096 + (i & 1) * 512 : i * 2048));
+  }
+};
+
+// 64 k-rows of a step, T columns of them (2 T bytes each).  Chunk c (8 columns) of k-row k at c ^ swz(k): the 32 lanes
+// that read at a time (eight k-rows of 16 columns) take 16 different chunks of 256 bytes.
+template <int T, int W>
+struct ColOp {
+  static constexpr int BYTES = T * 128, LOADS = BYTES / 1024 / W, PER = T / 8;
+  uint32_t off[LOADS], base[4];  // base: by the 16-column block's place in its four
+  static __device__ __forceinline__ int swz(int k) { return 2 * (k & 3) + 8 * ((k >> 3) & 1); }
+  __device__ __forceinline__ void init(int64_t ld, int w, int lane, int o0) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int q = (w * LOADS + i) * 64 + lane, k = q / PER;
+      off[i] = step_off((int64_t)k * ld * 2 + 16 * ((q % PER) ^ swz(k)));
+    }
+    // transposing reads: the 16 lanes of group g supply k-rows 8 g + r / 4 (and 4 further), 8 bytes at column 4 (r % 4)
+    const int r = lane & 15, g = lane >> 4, k = 8 * g + (r >> 2);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int byte = 2 * (o0 + 16 * u) + 8 * (r & 3);  // o0 is a multiple of 64: the swizzle stays within 128 columns
+      base[u] = k * (2 * T) + (((byte >> 4) ^ swz(k)) << 4) + (byte & 15);
+    }
+  }
+  __device__ __forceinline__ uint32_t at(int i, int) const { return off[i]; }  // k-rows past the end lie past the extent
+  // columns o0 + 16 j + r, k 32 half + 8 g ..
+  __device__ __forceinline__ bf16x8 frag(const unsigned char* st, int j, int half) const {
+    bf16x4 hv[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      // blocks j >= 4 lie 128 bytes further: bit 3 of their chunk is that of base's flipped
+      const unsigned char* p = st + (base[j & 3] ^ ((j >> 2) << 7)) + (32 * half + 4 * q) * (2 * T);
+      hv[q] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(p));
+    }
+    return bf16x8{hv[0][0], hv[0][1], hv[0][2], hv[0][3], hv[1][0], hv[1][1], hv[1][2], hv[1][3]};
+  }
+};
+
+// One tile of a product.  A 64-k step is two rounds of products, each beside the fragment reads of the next: k 0..31
+// (reads k 32..63), a barrier, k 32..63 (reads the next step's k 0..31 and issues the loads of step kt + NST into the
+// stage just read).  Waves whose part of the tile lies outside load and wait like the others and do nothing else.
+// Offsets are taken from the tile's first row and step, so operands may be of any size below 32 GiB.
+template <int EPI, bool AT, bool BT, typename S, int WGS>
+__global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const HeadArgs a) {
+  constexpr int MB = S::MB, NB = S::NB, TM = S::TM, TN = S::TN, NST = S::NST, STAGE = S::STAGE, W = S::W;
+  typedef std::conditional_t<AT, ColOp<TM, W>, RowOp<TM, W, false>> OpA;
+  typedef std::conditional_t<BT, ColOp<TN, W>, RowOp<TN, W, true>> OpB;
+  constexpr int LOADS = OpA::LOADS + OpB::LOADS;
+  static_assert(LOADS <= MB + NB, "the second round's reads carry the loads");
+  static_assert((!AT || (16 * MB) % 64 == 0) && (!BT || (16 * NB) % 64 == 0), "ColOp::base");
   __shared__ __align__(1024) unsigned char smem[NST * STAGE];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
-  const int t = xcd_remap(blockIdx.x, gridDim.x);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  static_assert(S::WC == 2 && (S::WR == 2 || S::WR == 4), "wave layouts");
+  // eight waves: those of one SIMD (w, w + 4) lie in opposite halves of both sides
+  const int wm = W == 8 ? (w & 3) ^ (w >> 2 << 1) : w >> 1, wn = W == 8 ? (w & 1) ^ (w >> 2) : w & 1;
+  int t = xcd_remap(blockIdx.x, gridDim.x);
+  const int tiles = a.tiles_m * a.tiles_n, split = t / tiles;
+  t -= split * tiles;
   constexpr int GM = 8;
   const int group = t / (GM * a.tiles_n), first_m = group * GM, gm = min(a.tiles_m - first_m, GM);
   const int tm = first_m + (t % (GM * a.tiles_n)) % gm, tn = t % (GM * a.tiles_n) / gm;
-  const int m0 = tm * TM, n0 = tn * TN;
-  const int rows = min(TM, a.M - m0), cols = min(TN, a.N - n0);
-  const uint16_t* hb = a.h + (int64_t)m0 * a.ldh;
-  const uint16_t* wb = a.w + (int64_t)n0 * a.ldw;
-  const int64_t hbytes = ((int64_t)(rows - 1) * a.ldh + a.D) * 2, wbytes = ((int64_t)(cols - 1) * a.ldw + a.D) * 2;
+  const int m0 = __builtin_amdgcn_readfirstlane(tm * TM), n0 = __builtin_amdgcn_readfirstlane(tn * TN);
+  const int row0 = m0 + wm * 16 * MB, col0 = n0 + wn * 16 * NB;
+  const int k0 = split * a.per, mine = min(a.steps - k0, a.per);  // steps of this split (none: zeros)
+  const int own = row0 < a.M && col0 < a.N ? mine : 0;
   OpA oa;
   OpB ob;
-  oa.init(a.ldh, 0, rows, wave, lane);
-  ob.init(a.ldw, 0, cols, wave, lane);
-  const int nk = (a.D + SK - 1) / SK;
-  auto fetch = [&](int kt) {
-    const int k0 = min(kt, nk - 1) * SK, klim = a.D - k0;
-    const i32x4 ra = step_rsrc<true>(hb, a.ldh, hbytes, k0), rb = step_rsrc<true>(wb, a.ldw, wbytes, k0);
-    unsigned char* st = smem + (kt % NST) * STAGE;
-#pragma unroll
-    for (int i = 0; i < OpA::NB; ++i) oa.dma(ra, st, wave, i, klim);
-#pragma unroll
-    for (int i = 0; i < OpB::NB; ++i) ob.dma(rb, st + OpA::BYTES, wave, i, klim);
+  oa.init(a.lda, w, lane, wm * 16 * MB);
+  ob.init(a.ldb, w, lane, wn * 16 * NB);
+  struct Src {  // an operand from the next step to load on; what lies past its end reads zero
+    uint64_t addr;
+    int64_t left;  // elements up to the end
+    __device__ __forceinline__ i32x4 rsrc() const {
+      const uint64_t n = left > 0 ? (uint64_t)left * 2 : 0;
+      const uint32_t bytes = (n >> 32) ? kOffPastK : (uint32_t)(n > kOffPastK ? kOffPastK : n);
+      return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)addr), __builtin_amdgcn_readfirstlane((int)((addr >> 32) & 0xffff)),
+                   __builtin_amdgcn_readfirstlane((int)bytes), kRsrcWord3};
+    }
+    __device__ __forceinline__ void advance(int64_t n) {
+      addr += (uint64_t)(n * 2);
+      left -= n;
+    }
   };
+  const int64_t beg_a = (AT ? (int64_t)m0 : m0 * a.lda) + (AT ? k0 * 64 * a.lda : (int64_t)k0 * 64);
+  const int64_t beg_b = (BT ? (int64_t)n0 : n0 * a.ldb) + (BT ? k0 * 64 * a.ldb : (int64_t)k0 * 64);
+  Src sa{reinterpret_cast<uint64_t>(a.A + beg_a), a.a_end - beg_a}, sb{reinterpret_cast<uint64_t>(a.B + beg_b), a.b_end - beg_b};
+  const int64_t inc_a = AT ? 64 * a.lda : 64, inc_b = BT ? 64 * a.ldb : 64;
+  int left = a.K - k0 * 64;  // k from the next step to load to the contraction's end
+  const uint32_t lds_a = __builtin_amdgcn_readfirstlane(lds_addr(smem) + w * OpA::LOADS * 1024);
+  const uint32_t lds_b = __builtin_amdgcn_readfirstlane(lds_addr(smem) + OpA::BYTES + w * OpB::LOADS * 1024);
+  auto load = [&](const i32x4& ra, const i32x4& rb, auto stage, auto q) {
+    constexpr int s = decltype(stage)::value, n = decltype(q)::value;
+    if constexpr (n < OpA::LOADS) dma_at<s * STAGE + n * 1024>(ra, oa.at(n, left), lds_a);
+    else dma_at<s * STAGE + (n - OpA::LOADS) * 1024>(rb, ob.at(n - OpA::LOADS, left), lds_b);
+  };
+  auto advance = [&]() {
+    sa.advance(inc_a);
+    sb.advance(inc_b);
+    left -= 64;
+  };
+  bf16x8 a0[MB], a1[MB], b0[NB], b1[NB];  // k 0..31 and 32..63
   f32x4 acc[MB][NB];
 #pragma unroll
   for (int i = 0; i < MB; ++i)
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // MB NB products, B first: lane (r, g) accumulates C[r][4 g + e]; io(q), q < MB + NB, spread over them
+  auto round = [&](const bf16x8 (&x)[MB], const bf16x8 (&y)[NB], auto io) {
+    constexpr int N = MB + NB, P = MB * NB;
+    unroll<N>([&](auto qt) {
+      constexpr int q = decltype(qt)::value;
+      io(qt);
 #pragma unroll
-  for (int s = 0; s < NST - 1; ++s) fetch(s);
-  for (int kt = 0; kt < nk; ++kt) {
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0((NST - 2) * LOADS));  // this wave's loads of step kt have landed
-    __builtin_amdgcn_s_barrier();  // every wave's; and every wave has read step kt - 1, whose stage is free
+      for (int n = q * P / N; n < (q + 1) * P / N; ++n)
+        acc[n / NB][n % NB] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[n % NB], x[n / NB], acc[n / NB][n % NB], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  unroll<NST>([&](auto st) {
+    const i32x4 ra = sa.rsrc(), rb = sb.rsrc();
+    unroll<LOADS>([&](auto q) { load(ra, rb, st, q); });
+    advance();
+  });
+  __builtin_amdgcn_s_waitcnt(wait_vm((NST - 1) * LOADS));  // loads complete in issue order: step 0 has landed
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  if (own > 0) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) b0[j] = ob.frag(smem + OpA::BYTES, j, 0);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) a0[i] = oa.frag(smem, i, 0);
+  }
+  auto step = [&](auto st) {
+    constexpr int ST = decltype(st)::value, NEXT = (ST + 1) % NST;
+    const unsigned char* cur = smem + ST * STAGE;
+    const unsigned char* nxt = smem + NEXT * STAGE;
+    __builtin_amdgcn_sched_barrier(0);
+    if (own > 0)
+      round(a0, b0, [&](auto qt) {
+        constexpr int q = decltype(qt)::value;
+        if constexpr (q < NB) b1[q] = ob.frag(cur + OpA::BYTES, q, 1);
+        else a1[q - NB] = oa.frag(cur, q - NB, 1);
+      });
+    // this wave's loads of step kt + 1 have landed and its fragments of step kt are read; then every wave's
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0((NST - 2) * LOADS));
+    __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    fetch(kt + NST - 1);
-    const unsigned char* st = smem + (kt % NST) * STAGE;
-    bf16x8 fa[2][MB], fb[2][NB];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int j = 0; j < NB; ++j) fb[h][j] = OpB::frag(st + OpA::BYTES, wn * 16 * NB + 16 * j, r, g, h);
-#pragma unroll
-      for (int i = 0; i < MB; ++i) fa[h][i] = OpA::frag(st, wm * 16 * MB + 16 * i, r, g, h);
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j)  // B first: lane (r, g) accumulates l[row r][column 4 g + e]
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[h][j], fa[h][i], acc[i][j], 0, 0, 0);
+    const i32x4 ra = sa.rsrc(), rb = sb.rsrc();
+    if (own > 0)
+      round(a1, b1, [&](auto qt) {
+        constexpr int q = decltype(qt)::value;
+        if constexpr (q < NB) b0[q] = ob.frag(nxt + OpA::BYTES, q, 0);
+        else a0[q - NB] = oa.frag(nxt, q - NB, 0);
+        if constexpr (q < LOADS) load(ra, rb, st, qt);
+      });
+    else unroll<LOADS>([&](auto q) { load(ra, rb, st, q); });
+    advance();
+  };
+  int kt = 0;
+  while (kt < mine) {
+    unroll<NST>([&](auto st) {
+      if (kt < mine) {
+        step(st);
+        ++kt;
+      }
+    });
   }
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no DMA may land after the workgroup exits
-  const int colw = n0 + wn * 16 * NB + 4 * g;    // first column of this lane within the piece
+
+  if constexpr (EPI == SUM || EPI == OUT_BF16 || EPI == OUT_F32) {
+    float alpha = 1.f;
+    if (EPI != SUM && !a.per_row) alpha = *a.grad * (a.inv ? *a.inv : 1.f);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+      const int row = row0 + 16 * i + r;
+      if (row >= a.M) continue;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const int col = col0 + 16 * j + 4 * g;
+        if (col >= a.N) continue;
+        const int64_t o = ((int64_t)(EPI == SUM ? split : 0) * a.M + row) * a.N + col;
+        float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        if constexpr (EPI == SUM) {
+          float* c = static_cast<float*>(a.C) + o;
+          if (a.accumulate) {
+            float x[4];
+            load4<float>(c, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += x[e];
+          }
+          store4<float>(c, v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] *= alpha;
+          if constexpr (EPI == OUT_F32) store4<float>(static_cast<float*>(a.C) + o, v);
+          else store4<uint16_t>(static_cast<uint16_t*>(a.C) + o, v);
+        }
+      }
+    }
+    return;
+  }
+  const auto column = [&](int j) { return col0 + 32 * (j >> 1) + 8 * g + 4 * (j & 1); };  // of block j's element 0, within the piece
 #pragma unroll
   for (int i = 0; i < MB; ++i) {
-    const int row = m0 + wm * 16 * MB + 16 * i + r;
+    const int row = row0 + 16 * i + r;
     const bool live = row < a.M;
     const int64_t tg = live ? a.targets[row] : a.ignore_index;
     const int64_t tc = tg - a.v0;  // the target's column within the piece
-    if constexpr (MODE == GRAD) {
+    if constexpr (EPI == GRAD) {
       const float l2 = live ? a.lse2[row] : 0.f;
       const bool ignored = tg == a.ignore_index;
       float s = 0.f;
-      if (live && !ignored)
-        s = tg < 0 || tg >= a.V ? __builtin_nanf("") : a.grad[(int64_t)row * a.grad_stride] * (a.inv ? *a.inv : 1.f);
+      if (live && !ignored) s = tg < 0 || tg >= a.V ? __builtin_nanf("") : a.per_row ? a.grad[row] : 1.f;
       uint16_t* out = a.p + (int64_t)row * a.ldp;
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
-        const int c = colw + 16 * j;
-        float d[4];
+        const int c = column(j);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float q = fast_exp2(fmaf(acc[i][j][e], kLog2e, -l2)) - (c + e == tc ? 1.f : 0.f);
-          d[e] = ignored || c + e >= a.N ? 0.f : q * s;  // columns past the piece are zero: the products contract over them
+          acc[i][j][e] = ignored || c + e >= a.N ? 0.f : q * s;  // columns past the piece are zero: the products contract over them
         }
-        if (live && c < a.ldp) store4<uint16_t>(out + c, d);
+        if (j % 2 == 1 && live && c < a.ldp) {  // 16 rows x 64 bytes a store (64 rows of 8 bytes took a tenth longer)
+          const f32x4 u = acc[i][j - 1], v = acc[i][j];
+          st16(out + column(j - 1), make_uint4(pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])));
+        }
       }
     } else {
       float m = kNegInf;
@@ -154,17 +330,17 @@ __global__ __launch_bounds__(256) void head_tile_kernel(const HeadArgs a) {
       for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int c = colw + 16 * j + e;
+          const int c = column(j) + e;
           const float v = c < a.N ? acc[i][j][e] : kNegInf;
           acc[i][j][e] = v;
-          if constexpr (MODE == STATS_PRED) {
+          if constexpr (EPI == STATS_PRED) {
             if (c < a.N) max_first(m, mi, v, a.v0 + c);
           } else {
             m = fmaxf(m, v);
           }
           if (c == tc && live && c < a.N) a.tgt[row] = v;
         }
-      if constexpr (MODE == STATS_PRED) {
+      if constexpr (EPI == STATS_PRED) {
         max_first(m, mi, __shfl_xor(m, 16), __shfl_xor(mi, 16));
         max_first(m, mi, __shfl_xor(m, 32), __shfl_xor(mi, 32));
       } else {
@@ -180,14 +356,16 @@ __global__ __launch_bounds__(256) void head_tile_kernel(const HeadArgs a) {
       if (live && g == 0) {
         const int64_t o = (int64_t)(2 * tn + wn) * a.M + row;
         a.part[o] = make_float2(m, s);
-        if constexpr (MODE == STATS_PRED) a.part_i[o] = mi;
+        if constexpr (EPI == STATS_PRED) a.part_i[o] = mi;
       }
     }
   }
 }
 
-// Joins the parts of 8 rows: 32 threads a row take every 32nd part, then the 32 in order, behind what the columns before
-// left (`run`, where `more`).  FINAL: the loss, else `run`.
+// Joins the parts of R rows: Q = 256 / R threads a row take every Q-th part, first the maxima, then the sums against the
+// row's maximum; the Q in a fixed order, behind what the columns before left (`run`, where `more`).  FINAL: the loss, else
+// `run`.  (16 rows a workgroup read whole cache lines, 4 fill the chip where rows are few: 8192 rows of 1024 parts 29 us
+// against 80, 333 rows of 786 parts 17 against 8.)
 struct JoinArgs {
   const float2* part; const int32_t* part_i;
   int slots, M, more;
@@ -197,46 +375,69 @@ struct JoinArgs {
   int32_t* pred;
 };
 
-__device__ __forceinline__ void join(float& m, float& s, int& i, float m2, float s2, int i2) {
-  const float M = fmaxf(m, m2);
-  const float C = M == kNegInf ? 0.f : __fmul_rn(M, kLog2e);
-  const float c1 = m == kNegInf ? C : __fmul_rn(m, kLog2e), c2 = m2 == kNegInf ? C : __fmul_rn(m2, kLog2e);
-  s = s * fast_exp2(c1 - C) + s2 * fast_exp2(c2 - C);
-  max_first(m, i, m2, i2);
-  m = M;
-}
-
-template <bool FINAL>
+template <bool FINAL, int R>
 __global__ __launch_bounds__(256) void head_join_kernel(const JoinArgs a) {
-  __shared__ float sm[32][8], ss[32][8];
-  __shared__ int si[32][8];
-  const int lr = threadIdx.x & 7, q = threadIdx.x >> 3, row = blockIdx.x * 8 + lr;
-  float m = kNegInf, s = 0.f;
+  constexpr int Q = 256 / R;
+  __shared__ float sm[Q][R], ss[Q][R];
+  __shared__ int si[Q][R];
+  const int lr = threadIdx.x % R, q = threadIdx.x / R, row = blockIdx.x * R + lr;
+  const bool live = row < a.M;
+  float m = kNegInf;
   int mi = 0x7fffffff;
-  if (row < a.M) {
-    if (a.more && q == 0) {
-      const float2 x = a.run[row];
-      m = x.x;
-      s = x.y;
+  float2 before = make_float2(kNegInf, 0.f);
+  if (live && a.more) {
+    before = a.run[row];
+    if (q == 0) {
+      m = before.x;
       if (a.part_i) mi = a.run_i[row];
     }
-    for (int k = q; k < a.slots; k += 32) {
-      const float2 x = a.part[(int64_t)k * a.M + row];
-      join(m, s, mi, x.x, x.y, a.part_i ? a.part_i[(int64_t)k * a.M + row] : 0);
+  }
+  if (live) {
+    if (a.part_i) {
+      for (int k = q; k < a.slots; k += Q) max_first(m, mi, a.part[(int64_t)k * a.M + row].x, a.part_i[(int64_t)k * a.M + row]);
+    } else {
+#pragma unroll 8
+      for (int k = q; k < a.slots; k += Q) m = fmaxf(m, a.part[(int64_t)k * a.M + row].x);
     }
   }
   sm[q][lr] = m;
-  ss[q][lr] = s;
   si[q][lr] = mi;
   __syncthreads();
-  if (threadIdx.x >= 8 || row >= a.M) return;
-  for (int k = 1; k < 32; ++k) join(m, s, mi, sm[k][lr], ss[k][lr], si[k][lr]);
+  for (int o = Q / 2; o > 0; o >>= 1) {
+    if (q < o) {
+      float m1 = sm[q][lr];
+      int i1 = si[q][lr];
+      if (a.part_i) max_first(m1, i1, sm[q + o][lr], si[q + o][lr]);
+      else m1 = fmaxf(m1, sm[q + o][lr]);
+      sm[q][lr] = m1;
+      si[q][lr] = i1;
+    }
+    __syncthreads();
+  }
+  m = sm[0][lr];
+  // a part's sum is in units of exp2(its maximum's rounded multiple of log2 e), as the tile took it
+  const float C = m == kNegInf ? 0.f : __fmul_rn(m, kLog2e);
+  const auto in_units = [&](float2 x) { return x.x == kNegInf ? (x.y == x.y ? 0.f : x.y) : x.y * fast_exp2(__fmul_rn(x.x, kLog2e) - C); };
+  float s = live && a.more && q == 0 ? in_units(before) : 0.f;
+  if (live) {
+#pragma unroll 8
+    for (int k = q; k < a.slots; k += Q) s += in_units(a.part[(int64_t)k * a.M + row]);
+  }
+  ss[q][lr] = s;
+  __syncthreads();
+  for (int o = Q / 2; o > 0; o >>= 1) {
+    if (q < o) ss[q][lr] += ss[q + o][lr];
+    __syncthreads();
+  }
+  if (q != 0 || !live) return;
+  s = ss[0][lr];
+  mi = si[0][lr];
   if constexpr (!FINAL) {
     a.run[row] = make_float2(m, s);
     if (a.part_i) a.run_i[row] = mi;
     return;
   }
-  const float C = m == kNegInf ? 0.f : __fmul_rn(m, kLog2e), lg = __builtin_amdgcn_logf(s);  // base 2
+  const float lg = __builtin_amdgcn_logf(s);  // base 2
   const int64_t t = a.targets[row];
   a.lse2[row] = C + lg;
   a.loss[row] = t == a.ignore_index ? 0.f
@@ -267,23 +468,63 @@ __global__ __launch_bounds__(1024) void head_total_kernel(const float* loss, con
   }
   if (threadIdx.x == 0) {
     *total = (float)(inv ? sl[0] / (double)sn[0] : sl[0]);  // the mean of no rows is NaN
-    if (inv) *inv = 1.f / (float)sn[0];
+    if (inv) *inv = sn[0] ? 1.f / (float)sn[0] : 0.f;  // and its gradients are zero
   }
 }
 
-__global__ __launch_bounds__(256) void head_cast_kernel(const float* x, uint16_t* y, int64_t quads) {
-  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < quads; q += (int64_t)gridDim.x * 256) {
+// out = alpha * sum over splits of the partial sums, in order
+template <typename T>
+__global__ __launch_bounds__(256) void head_reduce_kernel(const float* x, int splits, int64_t n, T* y, const float* grad,
+                                                          const float* inv, int per_row) {
+  const float alpha = per_row ? 1.f : *grad * (inv ? *inv : 1.f);
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
     float v[4];
-    load4<float>(x + 4 * q, v);
-    store4<uint16_t>(y + 4 * q, v);
+    load4<float>(x + i, v);
+    for (int s = 1; s < splits; ++s) {
+      float u[4];
+      load4<float>(x + s * n + i, u);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += u[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= alpha;
+    store4<T>(y + i, v);
   }
 }
 
 constexpr size_t up(size_t n) { return (n + 255) & ~size_t(255); }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-struct Tile { int tm, tn; };
-Tile tile_of(int rows) { return rows <= 64 ? Tile{64, 128} : Tile{128, 128}; }
+// Workgroups: tiles of 64 x 128, 128 x 128 and 256 x 256.
+enum Kind { THIN = 0, SQUARE = 1, BIG = 2, KINDS = 3 };
+typedef Shape<2, 4, 2, 2, 3> ThinShape;
+typedef Shape<4, 4, 2, 2, 2> SquareShape;
+typedef Shape<4, 8, 4, 2, 2> BigShape;
+constexpr int kTm[KINDS] = {64, 128, 256}, kTn[KINDS] = {128, 128, 256}, kPerCu[KINDS] = {2, 2, 1};
+// us of a 64-k step of a workgroup with 1 or 2 of them on a CU, and of a tile beside its steps
+constexpr double kStep[KINDS][2] = {{0.45, 0.60}, {0.60, 1.00}, {1.55, 1.55}};
+constexpr double kTile[KINDS] = {5.0, 6.0, 10.0};
+
+struct Tiling { int kind, splits; double us; };
+
+// The tiles of an M x N product over `steps` 64-wide k steps, and the splits of its contraction (at most `most`): the least
+// expected time, in rounds of whole tiles over the 256 CUs, the partial sums written and read at 4.5 TB/s.
+Tiling tiling(int64_t M, int64_t N, int steps, int most) {
+  Tiling best{SQUARE, 1, 1e30};
+  for (int kind = M <= 64 ? THIN : SQUARE; kind < KINDS; ++kind) {
+    if (most > 1 && kind == THIN) continue;  // gradients: 128 x 128 and larger
+    const int64_t tiles = ceil_div(M, kTm[kind]) * ceil_div(N, kTn[kind]), slots = 256 * kPerCu[kind];
+    for (int S = 1; S <= most && (S == 1 || steps / S >= 4); ++S) {
+      const int64_t n = tiles * S, rest = n % slots;
+      const double per = (double)ceil_div(steps, S);
+      double t = (double)(n / slots) * (per * kStep[kind][kPerCu[kind] - 1] + kTile[kind]);
+      if (rest) t += per * kStep[kind][rest > 256 ? 1 : 0] + kTile[kind];
+      if (S > 1) t += 6.0 + 8.0 * S * (double)M * (double)N / 4.5e6;
+      if (t < best.us) best = Tiling{kind, S, t};
+    }
+  }
+  return best;
+}
 
 int32_t check(const llattn_head_cfg* c) {
   if (!c) return fail(LLATTN_ERR_SHAPE, "llattn_head: null configuration");
@@ -298,13 +539,13 @@ int32_t check(const llattn_head_cfg* c) {
 }
 
 // forward: columns whose parts are joined at once, so that those stay within 256 MB
-struct FwdPlan { Tile t; int range; size_t slots, bytes; };
+struct FwdPlan { int kind, range; size_t slots, bytes; };
 FwdPlan fwd_plan(const llattn_head_cfg* c) {
   FwdPlan f;
-  f.t = tile_of(c->rows);
+  f.kind = tiling(c->rows, c->V, (c->D + 63) / 64, 1).kind;
   const int64_t most = std::max<int64_t>(1, (int64_t)(256 << 20) / (24 * (int64_t)c->rows));  // tile columns, two parts of 12 bytes each
-  const int64_t tiles = ceil_div(c->V, f.t.tn);
-  f.range = (int)(std::min(tiles, most) * f.t.tn);
+  const int64_t tiles = ceil_div(c->V, kTn[f.kind]);
+  f.range = (int)(std::min(tiles, most) * kTn[f.kind]);
   f.slots = 2 * (size_t)std::min(tiles, most);
   const size_t r = (size_t)c->rows;
   f.bytes = up(f.slots * r * 8) + up(f.slots * r * 4) + up(r * 8) + 2 * up(r * 4);
@@ -318,47 +559,55 @@ int piece_of(const llattn_head_cfg* c) {
   return (int)std::min<int64_t>(p, ceil_div(c->V, 256) * 256);
 }
 
-llattn_gemm_desc dh_desc(const llattn_head_cfg* c, const void* p, int64_t ldp, const void* w, int64_t ldw, int nv, void* out,
-                         bool f32, bool add) {
-  llattn_gemm_desc d{};
-  d.M = c->rows; d.N = c->D; d.K = (nv + 7) / 8 * 8;
-  d.A = p; d.lda = ldp;
-  d.B = w; d.ldb = ldw; d.b_trans = 1;
-  d.C = out; d.ldc = c->D; d.c_dtype = f32 ? LLATTN_F32 : LLATTN_BF16; d.accumulate = add;
-  return d;
-}
-llattn_gemm_desc dw_desc(const llattn_head_cfg* c, const void* p, int64_t ldp, const void* h, int64_t ldh, int nv, void* out) {
-  llattn_gemm_desc d{};
-  d.M = (nv + 7) / 8 * 8; d.N = c->D; d.K = c->rows;
-  d.A = p; d.lda = ldp; d.a_trans = 1;
-  d.B = h; d.ldb = ldh; d.b_trans = 1;
-  d.C = out; d.ldc = c->D; d.c_dtype = c->dw_dtype;
-  return d;
-}
-
-struct BwdPlan { int piece, pieces; size_t p, acc, gemm; size_t bytes() const { return p + acc + gemm; } };
+// q of a piece [rows][piece], the sums of dh over pieces and splits, the partial sums of dW
+struct BwdPlan {
+  int piece, pieces, ldp;
+  Tiling logits, dh, dw;
+  size_t p, dh_part, dw_part;
+  bool dh_direct() const { return pieces == 1 && dh.splits == 1; }
+  size_t bytes() const { return p + dh_part + dw_part; }
+};
 BwdPlan bwd_plan(const llattn_head_cfg* c) {
   BwdPlan b{};
   b.piece = piece_of(c);
   b.pieces = (int)ceil_div(c->V, b.piece);
-  b.p = up((size_t)c->rows * b.piece * 2);
-  b.acc = b.pieces > 1 ? up((size_t)c->rows * c->D * 4) : 0;
-  const int last = c->V - (b.pieces - 1) * b.piece;
-  for (int nv : {std::min(b.piece, c->V), last}) {
-    const llattn_gemm_desc d0 = dh_desc(c, nullptr, b.piece, nullptr, c->D, nv, nullptr, b.pieces > 1, false);
-    const llattn_gemm_desc d1 = dw_desc(c, nullptr, b.piece, nullptr, c->D, nv, nullptr);
-    b.gemm = std::max({b.gemm, up(llattn_gemm_workspace_size(&d0)), up(llattn_gemm_workspace_size(&d1))});
-  }
+  const int nv = std::min(b.piece, c->V);
+  b.logits = tiling(c->rows, nv, (c->D + 63) / 64, 1);
+  b.dh = tiling(c->rows, c->D, (nv + 63) / 64, 16);
+  b.dw = tiling(nv, c->D, (c->rows + 63) / 64, 16);
+  // rows a cache line apart from the next power of two: at 64 KB the 256 rows of a tile shared memory channels (8192 rows,
+  // pieces of 32768: q 1039 us, dh 826; so 823 and 771)
+  b.ldp = b.piece + 64;
+  b.p = up((size_t)c->rows * b.ldp * 2);
+  b.dh_part = b.dh_direct() ? 0 : up((size_t)b.dh.splits * c->rows * c->D * 4);
+  b.dw_part = b.dw.splits > 1 ? up((size_t)b.dw.splits * ((nv + 7) / 8 * 8) * c->D * 4) : 0;
   return b;
 }
 
-template <int MODE>
-void launch_tiles(HeadArgs& a, const Tile& t, hipStream_t st) {
-  a.tiles_m = (a.M + t.tm - 1) / t.tm;
-  a.tiles_n = (a.N + t.tn - 1) / t.tn;
-  const dim3 grid(a.tiles_m * a.tiles_n), block(256);
-  if (t.tm == 64) hipLaunchKernelGGL((head_tile_kernel<MODE, 2, 4, 3>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((head_tile_kernel<MODE, 4, 4, 2>), grid, block, 0, st, a);
+template <int EPI, bool AT, bool BT>
+void launch(HeadArgs& a, int kind, int splits, hipStream_t st) {
+  a.steps = (a.K + 63) / 64;
+  a.per = (a.steps + splits - 1) / splits;
+  a.tiles_m = (a.M + kTm[kind] - 1) / kTm[kind];
+  a.tiles_n = (a.N + kTn[kind] - 1) / kTn[kind];
+  const dim3 grid((unsigned)(a.tiles_m * a.tiles_n * splits));
+  if (kind == BIG) hipLaunchKernelGGL((head_kernel<EPI, AT, BT, BigShape, 1>), grid, dim3(BigShape::THREADS), 0, st, a);
+  else if (kind == SQUARE) hipLaunchKernelGGL((head_kernel<EPI, AT, BT, SquareShape, 2>), grid, dim3(SquareShape::THREADS), 0, st, a);
+  else if constexpr (!AT && !BT) hipLaunchKernelGGL((head_kernel<EPI, AT, BT, ThinShape, 2>), grid, dim3(ThinShape::THREADS), 0, st, a);
+}
+
+// l of `cols` columns from v0 on: h [rows][D] by W [cols][D]
+void logits_of(HeadArgs& a, const llattn_head_cfg* c, const void* h, int64_t ldh, const void* W, int64_t ldw, int v0, int cols) {
+  a.M = c->rows; a.N = cols; a.K = c->D;
+  a.A = static_cast<const uint16_t*>(h); a.lda = ldh; a.a_end = (c->rows - 1) * ldh + c->D;
+  a.B = static_cast<const uint16_t*>(W) + v0 * ldw; a.ldb = ldw; a.b_end = (cols - 1) * ldw + c->D;
+  a.v0 = v0; a.V = c->V;
+}
+
+template <typename T>
+void launch_reduce(const float* x, int splits, int64_t n, T* y, const HeadArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL(head_reduce_kernel<T>, dim3((unsigned)std::min<int64_t>(ceil_div(n, 1024), 8192)), dim3(256), 0, st, x, splits,
+                     n, y, a.grad, a.inv, a.per_row);
 }
 
 int32_t check_operands(const char* who, const llattn_head_cfg* c, const void* h, int64_t ldh, const void* W, int64_t ldw,
@@ -403,23 +652,23 @@ extern "C" int32_t llattn_head_fwd(const llattn_head_cfg* c, const void* h, int6
   j.run = reinterpret_cast<float2*>(p); p += up(r * 8);
   j.run_i = reinterpret_cast<int32_t*>(p); p += up(r * 4);
   a.tgt = reinterpret_cast<float*>(p);
-  a.M = c->rows; a.D = c->D; a.V = c->V;
-  a.h = static_cast<const uint16_t*>(h); a.ldh = ldh; a.ldw = ldw;
   a.targets = targets; a.ignore_index = ignore_index;
   j.M = c->rows; j.tgt = a.tgt; j.targets = targets; j.ignore_index = ignore_index; j.V = c->V;
   j.loss = loss; j.lse2 = lse2; j.pred = pred;
-  const dim3 jgrid((c->rows + 7) / 8), block(256);
+  const bool many = c->rows >= 2048;
+  const dim3 jgrid(many ? (c->rows + 15) / 16 : (c->rows + 3) / 4), block(256);
   j.part = a.part; j.part_i = pred ? a.part_i : nullptr;
   for (int64_t v0 = 0; v0 < c->V; v0 += f.range) {
-    a.v0 = (int)v0;
-    a.N = std::min(f.range, c->V - a.v0);
-    a.w = static_cast<const uint16_t*>(W) + (int64_t)a.v0 * ldw;
-    if (pred) launch_tiles<STATS_PRED>(a, f.t, st);
-    else launch_tiles<STATS>(a, f.t, st);
+    logits_of(a, c, h, ldh, W, ldw, (int)v0, (int)std::min<int64_t>(f.range, c->V - v0));
+    if (pred) launch<STATS_PRED, false, false>(a, f.kind, 1, st);
+    else launch<STATS, false, false>(a, f.kind, 1, st);
     j.slots = 2 * a.tiles_n;
     j.more = v0 > 0;
-    if (v0 + f.range < c->V) hipLaunchKernelGGL(head_join_kernel<false>, jgrid, block, 0, st, j);
-    else hipLaunchKernelGGL(head_join_kernel<true>, jgrid, block, 0, st, j);
+    const bool last = v0 + f.range >= c->V;
+    if (many && last) hipLaunchKernelGGL((head_join_kernel<true, 16>), jgrid, block, 0, st, j);
+    else if (many) hipLaunchKernelGGL((head_join_kernel<false, 16>), jgrid, block, 0, st, j);
+    else if (last) hipLaunchKernelGGL((head_join_kernel<true, 4>), jgrid, block, 0, st, j);
+    else hipLaunchKernelGGL((head_join_kernel<false, 4>), jgrid, block, 0, st, j);
   }
   if (total) hipLaunchKernelGGL(head_total_kernel, dim3(1), dim3(1024), 0, st, loss, targets, ignore_index, c->rows, total, inv);
   return check_launch("llattn_head_fwd");
@@ -438,36 +687,50 @@ extern "C" int32_t llattn_head_bwd(const llattn_head_cfg* c, const void* h, int6
   if ((dh && !aligned16(dh)) || (dW && !aligned16(dW)))
     return fail(LLATTN_ERR_LAYOUT, "llattn_head_bwd: dh and dW must be 16-byte aligned");
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  char* ws = static_cast<char*>(workspace);
-  HeadArgs a{};
-  a.p = reinterpret_cast<uint16_t*>(ws); a.ldp = b.piece;
-  float* acc = reinterpret_cast<float*>(ws + b.p);
-  void* gws = ws + b.p + b.acc;
-  a.M = c->rows; a.D = c->D; a.V = c->V;
-  a.h = static_cast<const uint16_t*>(h); a.ldh = ldh; a.ldw = ldw;
-  a.targets = targets; a.ignore_index = ignore_index;
-  a.lse2 = lse2; a.grad = grad; a.grad_stride = grad_stride; a.inv = inv;
-  const int64_t dwsz = c->dw_dtype == LLATTN_F32 ? 4 : 2;
   if (!dh && !dW) return LLATTN_OK;
+  char* ws = static_cast<char*>(workspace);
+  float* dh_part = reinterpret_cast<float*>(ws + b.p);
+  float* dw_part = reinterpret_cast<float*>(ws + b.p + b.dh_part);
+  HeadArgs a{};
+  a.p = reinterpret_cast<uint16_t*>(ws); a.ldp = b.ldp;
+  a.targets = targets; a.ignore_index = ignore_index;
+  a.lse2 = lse2; a.grad = grad; a.per_row = grad_stride; a.inv = inv;
+  const int64_t dw_size = c->dw_dtype == LLATTN_F32 ? 4 : 2;
   for (int q = 0; q < b.pieces; ++q) {
-    a.v0 = (int)((int64_t)q * b.piece);
-    a.N = std::min(b.piece, c->V - a.v0);
-    a.w = static_cast<const uint16_t*>(W) + (int64_t)a.v0 * ldw;
-    launch_tiles<GRAD>(a, tile_of(c->rows), st);
-    if (dh) {
-      const bool f32 = b.pieces > 1;
-      const llattn_gemm_desc d = dh_desc(c, a.p, a.ldp, a.w, ldw, a.N, f32 ? static_cast<void*>(acc) : dh, f32, q > 0);
-      if (const int32_t rc = gemm::product(&d, a.N, gws, b.gemm, st)) return rc;
+    const int v0 = (int)((int64_t)q * b.piece), cols = std::min(b.piece, c->V - v0);
+    logits_of(a, c, h, ldh, W, ldw, v0, cols);
+    launch<GRAD, false, false>(a, b.logits.kind, 1, st);
+    HeadArgs d = a;
+    d.A = a.p; d.lda = a.ldp;
+    d.N = c->D;
+    if (dh) {  // q W: q's columns past the piece are zero up to the next 128, and W's rows read zero there
+      d.M = c->rows; d.K = (cols + 63) / 64 * 64;
+      d.a_end = (c->rows - 1) * a.ldp + b.piece;
+      d.accumulate = q > 0;
+      d.C = b.dh_direct() ? dh : dh_part;
+      if (b.dh_direct()) launch<OUT_BF16, false, true>(d, b.dh.kind, 1, st);
+      else launch<SUM, false, true>(d, b.dh.kind, b.dh.splits, st);
     }
-    if (dW) {
-      const llattn_gemm_desc d = dw_desc(c, a.p, a.ldp, h, ldh, a.N, static_cast<char*>(dW) + (int64_t)a.v0 * c->D * dwsz);
-      if (const int32_t rc = gemm::product(&d, c->rows, gws, b.gemm, st)) return rc;
+    if (dW) {  // qᵀ h
+      d.M = (cols + 7) / 8 * 8; d.K = c->rows;
+      d.a_end = (c->rows - 1) * a.ldp + b.piece;
+      d.B = a.A; d.ldb = a.lda; d.b_end = a.a_end;
+      d.accumulate = 0;
+      void* out = static_cast<char*>(dW) + (int64_t)v0 * c->D * dw_size;
+      d.C = b.dw.splits > 1 ? static_cast<void*>(dw_part) : out;
+      if (b.dw.splits > 1) {
+        launch<SUM, true, true>(d, b.dw.kind, b.dw.splits, st);
+        const int64_t n = (int64_t)d.M * c->D;
+        if (c->dw_dtype == LLATTN_F32) launch_reduce(dw_part, b.dw.splits, n, static_cast<float*>(out), a, st);
+        else launch_reduce(dw_part, b.dw.splits, n, static_cast<uint16_t*>(out), a, st);
+      } else if (c->dw_dtype == LLATTN_F32) {
+        launch<OUT_F32, true, true>(d, b.dw.kind, 1, st);
+      } else {
+        launch<OUT_BF16, true, true>(d, b.dw.kind, 1, st);
+      }
     }
   }
-  if (dh && b.pieces > 1) {
-    const int64_t quads = (int64_t)c->rows * c->D / 4;
-    hipLaunchKernelGGL(head_cast_kernel, dim3((unsigned)std::min<int64_t>((quads + 255) / 256, 4096)), dim3(256), 0, st, acc,
-                       static_cast<uint16_t*>(dh), quads);
-  }
+  if (dh && !b.dh_direct())
+    launch_reduce(dh_part, b.dh.splits, (int64_t)c->rows * c->D, static_cast<uint16_t*>(dh), a, st);
   return check_launch("llattn_head_bwd");
 }

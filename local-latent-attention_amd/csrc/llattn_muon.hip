@@ -36,21 +36,16 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kSA = 4096.f;  // scale of A and B
 
-// f(integral_constant 0), f(1), ..., f(N - 1)
-template <int N, int I = 0, typename F>
-__device__ __forceinline__ void unroll(F&& f) {
-  if constexpr (I < N) {
-    f(std::integral_constant<int, I>{});
-    unroll<N, I + 1>(f);
-  }
-}
-
 template <typename P>
 struct Table { P p[LLATTN_MUON_BATCH]; };
 
 __device__ __forceinline__ float load_as(const void* p, int64_t i, int dtype) {
   return dtype == LLATTN_F32 ? static_cast<const float*>(p)[i] : bf2f(static_cast<const uint16_t*>(p)[i]);
 }
+
+// 16-bit elements from a row of n columns to the next: its halves and one cache line more, so that the rows of a tile are
+// never a power of two apart (they would share memory channels).
+__host__ __device__ constexpr int64_t row_elems(int n) { return 2 * ((int64_t)n + 32); }
 
 // ---- momentum and |U|^2 -----------------------------------------------------------
 // A group's share of a launch over elements: workgroups [b0, b0 + batch blocks), `blocks` a matrix.
@@ -204,7 +199,7 @@ __global__ __launch_bounds__(256) void muon_split_kernel(const ElemArgs a) {
     }
   }
   __syncthreads();
-  const int64_t ld = 2 * (int64_t)G.np;
+  const int64_t ld = row_elems(G.np);
   uint16_t* x = a.x + G.x_off + mat * G.mp * ld;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -242,15 +237,6 @@ struct LastArgs {
 };
 
 static_assert(sizeof(LastArgs) <= 4096, "kernel arguments");
-
-// One wave's copy of 64 x 16 bytes into the 1 KB LDS block at byte address lds + AT (buffer_load ... lds, as dma_block).
-template <int AT>
-__device__ __forceinline__ void dma_at(const i32x4& rs, uint32_t off, uint32_t lds) {
-  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
-               :
-               : "v"(off), "s"(rs), "s"(lds), "i"(AT)
-               : "memory", "m0", "scc");
-}
 
 // T rows of a step with k along them (128 bytes each: 32 hi, 32 lo), loaded by W waves.  Chunk c of row o at c ^ (o & 7).
 template <int T, int W>
@@ -371,7 +357,7 @@ __device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*
     tn = t % (8 * G.tiles_n) / gm;
   }
   const int m0 = __builtin_amdgcn_readfirstlane(tm * TM), n0 = __builtin_amdgcn_readfirstlane(tn * TN);
-  const int64_t lx = 2 * (int64_t)G.np, la = 2 * (int64_t)G.mp;
+  const int64_t lx = row_elems(G.np), la = row_elems(G.mp);
   const uint16_t* X = a.x + G.x_off + mat * G.mp * lx;
   uint16_t* Am = a.a + G.a_off + mat * G.mp * la;
   uint16_t* Bm = a.b + G.a_off + mat * G.mp * la;
@@ -842,7 +828,7 @@ constexpr int kTm[KINDS] = {SmallShape::TM, SplitShape::TM, SquareShape::TM, Big
 constexpr int kTn[KINDS] = {SmallShape::TN, SplitShape::TN, SquareShape::TN, BigShape::TN};
 constexpr int kPerCu[KINDS] = {3, 1, 2, 1};
 // us of a 32-k step of a workgroup with 1, 2, 3 of them on a CU, and of a tile beside its steps.
-constexpr double kStep[KINDS][3] = {{0.33, 0.50, 0.80}, {0.28, 0.28, 0.28}, {0.67, 1.37, 1.37}, {2.25, 2.25, 2.25}};
+constexpr double kStep[KINDS][3] = {{0.33, 0.50, 0.80}, {0.28, 0.28, 0.28}, {0.67, 1.37, 1.37}, {2.15, 2.15, 2.15}};
 constexpr double kTile[KINDS] = {3.5, 4.0, 7.0, 16.0};
 
 struct GroupPlan {
@@ -873,8 +859,8 @@ Plan plan_of(const llattn_muon_cfg* c, const llattn_muon_group* groups) {
     g.a_off = a;
     p.matrices += q.batch;
     part += (size_t)q.batch * g.parts;
-    x += (size_t)q.batch * g.mp * g.np * 2;
-    a += (size_t)q.batch * g.mp * g.mp * 2;
+    x += (size_t)q.batch * g.mp * row_elems(g.np);
+    a += (size_t)q.batch * g.mp * row_elems(g.mp);
   }
   p.x = up(2 * x);
   p.a = up(2 * a);

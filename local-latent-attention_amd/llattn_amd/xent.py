@@ -149,37 +149,42 @@ def _bf16_rows(t: torch.Tensor, pad: int) -> torch.Tensor:
     return t
 
 
+def _piece_forward(h, weight, targets, ignore_index, reduction, want_pred, piece):
+    """(loss, pred or None, what a backward reads)."""
+    D, V, dev = h.shape[-1], weight.shape[0], h.device
+    N, pad = targets.numel(), -D % 8
+    t = targets.reshape(-1).to(torch.int64).contiguous()
+    hb, wb = _bf16_rows(h.reshape(-1, D), pad), _bf16_rows(weight, pad)
+    loss = torch.empty((N,), dtype=torch.float32, device=dev)
+    lse2 = torch.empty((N,), dtype=torch.float32, device=dev)
+    pred = torch.empty((N,), dtype=torch.int32, device=dev) if want_pred else None
+    total = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
+    inv = torch.empty((), dtype=torch.float32, device=dev) if reduction == "mean" else None
+    cfg = L.LlattnHeadCfg(N, V, D + pad, piece, L.F32 if weight.dtype is torch.float32 else L.BF16)
+    if N == 0:
+        if total is not None:
+            total.fill_(0.0 if inv is None else float("nan"))  # the mean of nothing
+    else:
+        n = _head_bytes(cfg, 0)
+        ws = torch.empty((n,), dtype=torch.uint8, device=dev)
+        from .ops import _call
+        with L.on_device(dev):
+            _call("llattn_head_fwd", ctypes.byref(cfg), hb.data_ptr(), hb.stride(0), wb.data_ptr(), wb.stride(0),
+                  t.data_ptr(), ignore_index, loss.data_ptr(), lse2.data_ptr(),
+                  _ptr(pred), _ptr(total), _ptr(inv), ws.data_ptr(), n, L.stream_ptr(dev), work=2 * (N + V) * D)
+    out = loss.view(targets.shape) if total is None else total
+    return out, pred.view(targets.shape) if want_pred else None, (hb, wb, t, lse2, inv, cfg)
+
+
 class _PieceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, weight, targets, ignore_index, reduction, want_pred, piece, grad_enabled):
-        D, V, dev = h.shape[-1], weight.shape[0], h.device
-        N, pad = targets.numel(), -D % 8
-        t = targets.reshape(-1).to(torch.int64).contiguous()
-        hb, wb = _bf16_rows(h.reshape(-1, D), pad), _bf16_rows(weight, pad)
-        loss = torch.empty((N,), dtype=torch.float32, device=dev)
-        lse2 = torch.empty((N,), dtype=torch.float32, device=dev)
-        pred = torch.empty((N,), dtype=torch.int32, device=dev) if want_pred else None
-        total = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
-        inv = torch.empty((), dtype=torch.float32, device=dev) if reduction == "mean" else None
-        cfg = L.LlattnHeadCfg(N, V, D + pad, piece, L.F32 if weight.dtype is torch.float32 else L.BF16)
-        if N == 0:
-            if total is not None:
-                total.fill_(0.0 if inv is None else float("nan"))  # the mean of nothing
-        else:
-            n = _head_bytes(cfg, 0)
-            ws = torch.empty((n,), dtype=torch.uint8, device=dev)
-            from .ops import _call
-            with L.on_device(dev):
-                _call("llattn_head_fwd", ctypes.byref(cfg), hb.data_ptr(), hb.stride(0), wb.data_ptr(), wb.stride(0),
-                      t.data_ptr(), ignore_index, loss.data_ptr(), lse2.data_ptr(),
-                      _ptr(pred), _ptr(total), _ptr(inv), ws.data_ptr(), n, L.stream_ptr(dev), work=2 * (N + V) * D)
+        out, pred, (hb, wb, t, lse2, inv, cfg) = _piece_forward(h, weight, targets, ignore_index, reduction, want_pred, piece)
         if grad_enabled and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]):
             ctx.save_for_backward(hb, wb, t, lse2, inv)
             ctx.meta = (cfg, ignore_index, reduction, tuple(h.shape), h.dtype, tuple(weight.shape), weight.dtype)
-        out = loss.view(targets.shape) if total is None else total
         if not want_pred:
             return out
-        pred = pred.view(targets.shape)
         ctx.mark_non_differentiable(pred)
         return out, pred
 
@@ -240,5 +245,8 @@ def piecewise_head_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Te
     L.require_gpu(h, weight, targets)
     if not h.device == weight.device == targets.device:
         raise ValueError(f"piecewise_head_loss: tensors on {h.device}, {weight.device} and {targets.device}")
-    return _PieceLoss.apply(h, weight, targets, int(ignore_index), reduction, bool(return_pred), int(piece),
-                            torch.is_grad_enabled())
+    args = (h, weight, targets, int(ignore_index), reduction, bool(return_pred), int(piece))
+    if not (h.requires_grad or weight.requires_grad) and type(h) is torch.Tensor and type(weight) is torch.Tensor:
+        out, pred, _ = _piece_forward(*args)  # nothing to differentiate: evaluation
+        return (out, pred) if return_pred else out
+    return _PieceLoss.apply(*args, torch.is_grad_enabled())
