@@ -236,6 +236,24 @@ __device__ __forceinline__ void unroll(F&& f) {
   }
 }
 
+// An operand tile from the next k step to load on.  Loads past a step's extent read zero; the extent is `full` while whole
+// steps are left, `tail` in a shorter last one and nothing past it.  (Every step's descriptor is three scalar instructions,
+// issued among the products of the step before.)
+struct StepSrc {
+  uint64_t addr;
+  uint32_t full, tail, inc;  // bytes; inc: from a step to the next
+  __device__ __forceinline__ i32x4 rsrc(int left, int step) const {
+    const int n = left >= step ? (int)full : left > 0 ? (int)tail : 0;  // uniform, which the compiler does not always see
+    return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)addr), __builtin_amdgcn_readfirstlane((int)(uint32_t)(addr >> 32)),
+                 __builtin_amdgcn_readfirstlane(n), kRsrcWord3};
+  }
+};
+// (rows - 1) ld + cols elements in bytes, as an extent (rows, cols >= 1)
+__device__ __forceinline__ uint32_t extent_of(int rows, int64_t ld, int cols) {
+  const uint64_t n = (uint64_t)((int64_t)(rows - 1) * ld + cols) * 2;
+  return n > kOffPastK ? kOffPastK : (uint32_t)n;
+}
+
 // One wave's copy of 64 x 16 bytes into the 1 KB LDS block at byte address lds + AT (buffer_load ... lds, as dma_block).
 template <int AT>
 __device__ __forceinline__ void dma_at(const i32x4& rs, uint32_t off, uint32_t lds) {

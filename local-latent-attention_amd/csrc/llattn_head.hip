@@ -34,8 +34,8 @@ struct HeadArgs {
   int M, N, K;              // rows, columns, contraction
   int steps, per;           // 64-wide k steps, of a split
   int tiles_m, tiles_n;
-  const uint16_t* A; int64_t lda; int64_t a_end;  // a_end: elements up to the operand's end
-  const uint16_t* B; int64_t ldb; int64_t b_end;
+  const uint16_t* A; int64_t lda;
+  const uint16_t* B; int64_t ldb;
   // logits
   int v0;                   // first column of the piece in the vocabulary
   int64_t V;                // targets outside [0, V) are errors
@@ -159,41 +159,36 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
   const int m0 = __builtin_amdgcn_readfirstlane(tm * TM), n0 = __builtin_amdgcn_readfirstlane(tn * TN);
   const int row0 = m0 + wm * 16 * MB, col0 = n0 + wn * 16 * NB;
   const int k0 = split * a.per, mine = min(a.steps - k0, a.per);  // steps of this split (none: zeros)
-  const int own = row0 < a.M && col0 < a.N ? mine : 0;
+  const bool own = row0 < a.M && col0 < a.N && mine > 0;
   OpA oa;
   OpB ob;
   oa.init(a.lda, w, lane, wm * 16 * MB);
   ob.init(a.ldb, w, lane, wn * 16 * NB);
-  struct Src {  // an operand from the next step to load on; what lies past its end reads zero
-    uint64_t addr;
-    int64_t left;  // elements up to the end
-    __device__ __forceinline__ i32x4 rsrc() const {
-      const uint64_t n = left > 0 ? (uint64_t)left * 2 : 0;
-      const uint32_t bytes = (n >> 32) ? kOffPastK : (uint32_t)(n > kOffPastK ? kOffPastK : n);
-      return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)addr), __builtin_amdgcn_readfirstlane((int)((addr >> 32) & 0xffff)),
-                   __builtin_amdgcn_readfirstlane((int)bytes), kRsrcWord3};
-    }
-    __device__ __forceinline__ void advance(int64_t n) {
-      addr += (uint64_t)(n * 2);
-      left -= n;
-    }
-  };
-  const int64_t beg_a = (AT ? (int64_t)m0 : m0 * a.lda) + (AT ? k0 * 64 * a.lda : (int64_t)k0 * 64);
-  const int64_t beg_b = (BT ? (int64_t)n0 : n0 * a.ldb) + (BT ? k0 * 64 * a.ldb : (int64_t)k0 * 64);
-  Src sa{reinterpret_cast<uint64_t>(a.A + beg_a), a.a_end - beg_a}, sb{reinterpret_cast<uint64_t>(a.B + beg_b), a.b_end - beg_b};
-  const int64_t inc_a = AT ? 64 * a.lda : 64, inc_b = BT ? 64 * a.ldb : 64;
   int left = a.K - k0 * 64;  // k from the next step to load to the contraction's end
+  auto source = [&](const uint16_t* p, int64_t ld, bool t, int o, int n) {  // a tile of n of the operand's rows (t: columns) from o on
+    StepSrc s;
+    s.addr = reinterpret_cast<uint64_t>(p + (t ? o + (int64_t)k0 * 64 * ld : o * ld + (int64_t)k0 * 64));
+    s.full = t ? extent_of(64, ld, n) : extent_of(n, ld, 64);  // not t: chunks past the last k are masked (RowOp::at)
+    s.tail = t ? extent_of(a.K & 63 ? a.K & 63 : 64, ld, n) : s.full;
+    s.inc = t ? (uint32_t)(128 * ld) : 128u;
+    return s;
+  };
+  StepSrc sa = source(a.A, a.lda, AT, m0, min(TM, a.M - m0)), sb = source(a.B, a.ldb, BT, n0, min(TN, a.N - n0));
+  i32x4 ra = sa.rsrc(left, 64), rb = sb.rsrc(left, 64);
+  int ahead = left;  // of the step that ra and rb describe
+  auto next_step = [&]() {
+    sa.addr += sa.inc;
+    sb.addr += sb.inc;
+    ahead -= 64;
+    ra = sa.rsrc(ahead, 64);
+    rb = sb.rsrc(ahead, 64);
+  };
   const uint32_t lds_a = __builtin_amdgcn_readfirstlane(lds_addr(smem) + w * OpA::LOADS * 1024);
   const uint32_t lds_b = __builtin_amdgcn_readfirstlane(lds_addr(smem) + OpA::BYTES + w * OpB::LOADS * 1024);
-  auto load = [&](const i32x4& ra, const i32x4& rb, auto stage, auto q) {
+  auto load = [&](auto stage, auto q) {
     constexpr int s = decltype(stage)::value, n = decltype(q)::value;
-    if constexpr (n < OpA::LOADS) dma_at<s * STAGE + n * 1024>(ra, oa.at(n, left), lds_a);
-    else dma_at<s * STAGE + (n - OpA::LOADS) * 1024>(rb, ob.at(n - OpA::LOADS, left), lds_b);
-  };
-  auto advance = [&]() {
-    sa.advance(inc_a);
-    sb.advance(inc_b);
-    left -= 64;
+    if constexpr (n < OpA::LOADS) dma_at<s * STAGE + n * 1024>(ra, oa.at(n, ahead), lds_a);
+    else dma_at<s * STAGE + (n - OpA::LOADS) * 1024>(rb, ob.at(n - OpA::LOADS, ahead), lds_b);
   };
   bf16x8 a0[MB], a1[MB], b0[NB], b1[NB];  // k 0..31 and 32..63
   f32x4 acc[MB][NB];
@@ -214,55 +209,59 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
     });
   };
   unroll<NST>([&](auto st) {
-    const i32x4 ra = sa.rsrc(), rb = sb.rsrc();
-    unroll<LOADS>([&](auto q) { load(ra, rb, st, q); });
-    advance();
+    if constexpr (decltype(st)::value > 0) next_step();
+    unroll<LOADS>([&](auto q) { load(st, q); });
   });
   __builtin_amdgcn_s_waitcnt(wait_vm((NST - 1) * LOADS));  // loads complete in issue order: step 0 has landed
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  if (own > 0) {
+  if (own) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) b0[j] = ob.frag(smem + OpA::BYTES, j, 0);
 #pragma unroll
     for (int i = 0; i < MB; ++i) a0[i] = oa.frag(smem, i, 0);
   }
-  auto step = [&](auto st) {
+  auto step = [&](auto st, auto live_tag) {
     constexpr int ST = decltype(st)::value, NEXT = (ST + 1) % NST;
+    constexpr bool LIVE = decltype(live_tag)::value;
     const unsigned char* cur = smem + ST * STAGE;
     const unsigned char* nxt = smem + NEXT * STAGE;
     __builtin_amdgcn_sched_barrier(0);
-    if (own > 0)
+    if constexpr (LIVE)
       round(a0, b0, [&](auto qt) {
         constexpr int q = decltype(qt)::value;
         if constexpr (q < NB) b1[q] = ob.frag(cur + OpA::BYTES, q, 1);
         else a1[q - NB] = oa.frag(cur, q - NB, 1);
+        if constexpr (q == 0) next_step();
       });
+    else next_step();
     // this wave's loads of step kt + 1 have landed and its fragments of step kt are read; then every wave's
     __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0((NST - 2) * LOADS));
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    const i32x4 ra = sa.rsrc(), rb = sb.rsrc();
-    if (own > 0)
+    if constexpr (LIVE)
       round(a1, b1, [&](auto qt) {
         constexpr int q = decltype(qt)::value;
         if constexpr (q < NB) b0[q] = ob.frag(nxt + OpA::BYTES, q, 0);
         else a0[q - NB] = oa.frag(nxt, q - NB, 0);
-        if constexpr (q < LOADS) load(ra, rb, st, qt);
+        if constexpr (q < LOADS) load(st, qt);
       });
-    else unroll<LOADS>([&](auto q) { load(ra, rb, st, q); });
-    advance();
+    else unroll<LOADS>([&](auto q) { load(st, q); });
   };
-  int kt = 0;
-  while (kt < mine) {
-    unroll<NST>([&](auto st) {
-      if (kt < mine) {
-        step(st);
-        ++kt;
-      }
-    });
-  }
+  auto steps = [&](auto live_tag) {
+    int kt = 0;
+    while (kt < mine) {
+      unroll<NST>([&](auto st) {
+        if (kt < mine) {
+          step(st, live_tag);
+          ++kt;
+        }
+      });
+    }
+  };
+  if (own) steps(std::true_type{});
+  else steps(std::false_type{});
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no DMA may land after the workgroup exits
 
   if constexpr (EPI == SUM || EPI == OUT_BF16 || EPI == OUT_F32) {
@@ -599,8 +598,8 @@ void launch(HeadArgs& a, int kind, int splits, hipStream_t st) {
 // l of `cols` columns from v0 on: h [rows][D] by W [cols][D]
 void logits_of(HeadArgs& a, const llattn_head_cfg* c, const void* h, int64_t ldh, const void* W, int64_t ldw, int v0, int cols) {
   a.M = c->rows; a.N = cols; a.K = c->D;
-  a.A = static_cast<const uint16_t*>(h); a.lda = ldh; a.a_end = (c->rows - 1) * ldh + c->D;
-  a.B = static_cast<const uint16_t*>(W) + v0 * ldw; a.ldb = ldw; a.b_end = (cols - 1) * ldw + c->D;
+  a.A = static_cast<const uint16_t*>(h); a.lda = ldh;
+  a.B = static_cast<const uint16_t*>(W) + v0 * ldw; a.ldb = ldw;
   a.v0 = v0; a.V = c->V;
 }
 
@@ -703,9 +702,8 @@ extern "C" int32_t llattn_head_bwd(const llattn_head_cfg* c, const void* h, int6
     HeadArgs d = a;
     d.A = a.p; d.lda = a.ldp;
     d.N = c->D;
-    if (dh) {  // q W: q's columns past the piece are zero up to the next 128, and W's rows read zero there
-      d.M = c->rows; d.K = (cols + 63) / 64 * 64;
-      d.a_end = (c->rows - 1) * a.ldp + b.piece;
+    if (dh) {  // q W: q's chunk that reaches past the piece's columns holds zeros there, W's rows past them read zero
+      d.M = c->rows; d.K = cols;
       d.accumulate = q > 0;
       d.C = b.dh_direct() ? dh : dh_part;
       if (b.dh_direct()) launch<OUT_BF16, false, true>(d, b.dh.kind, 1, st);
@@ -713,8 +711,7 @@ extern "C" int32_t llattn_head_bwd(const llattn_head_cfg* c, const void* h, int6
     }
     if (dW) {  // qᵀ h
       d.M = (cols + 7) / 8 * 8; d.K = c->rows;
-      d.a_end = (c->rows - 1) * a.ldp + b.piece;
-      d.B = a.A; d.ldb = a.lda; d.b_end = a.a_end;
+      d.B = a.A; d.ldb = a.lda;
       d.accumulate = 0;
       void* out = static_cast<char*>(dW) + (int64_t)v0 * c->D * dw_size;
       d.C = b.dw.splits > 1 ? static_cast<void*>(dw_part) : out;

@@ -43,9 +43,8 @@ __device__ __forceinline__ float load_as(const void* p, int64_t i, int dtype) {
   return dtype == LLATTN_F32 ? static_cast<const float*>(p)[i] : bf2f(static_cast<const uint16_t*>(p)[i]);
 }
 
-// 16-bit elements from a row of n columns to the next: its halves and one cache line more, so that the rows of a tile are
-// never a power of two apart (they would share memory channels).
-__host__ __device__ constexpr int64_t row_elems(int n) { return 2 * ((int64_t)n + 32); }
+// 16-bit elements of a row of n columns.
+__host__ __device__ constexpr int64_t row_elems(int n) { return 2 * (int64_t)n; }
 
 // ---- momentum and |U|^2 -----------------------------------------------------------
 // A group's share of a launch over elements: workgroups [b0, b0 + batch blocks), `blocks` a matrix.
@@ -363,10 +362,8 @@ __device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*
   uint16_t* Bm = a.b + G.a_off + mat * G.mp * la;
   // operands: rows of the tile with k along them; SYM: the same for its columns, else X with k along its rows
   const uint16_t* opa = MODE == GRAM ? X : MODE == POLY ? Am : Bm;
-  const int64_t lda = MODE == GRAM ? lx : la, end_a = G.mp * lda;
-  const int64_t beg_a = m0 * lda, beg_b = SYM ? n0 * lda : (int64_t)n0 * 2;
   const uint16_t* opb = SYM ? opa : X;
-  const int64_t end_b = SYM ? end_a : G.mp * lx;
+  const int64_t lda = MODE == GRAM ? lx : la, ldb = SYM ? lda : lx;
   // first row and column of this wave's part
   const int row0 = m0 + wm * 16 * MB, col0 = n0 + wn * 16 * NB, lim = SYM ? G.mp : G.np;
   const int per = (G.steps + KG - 1) / KG;  // steps of a group: this one's are [kg per, kg per + own)
@@ -374,33 +371,37 @@ __device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*
   OpA oa;
   OpB ob;
   oa.init(lda, w, lane, wm * 16 * MB);
-  ob.init(SYM ? lda : lx, w, lane, wn * 16 * NB);
-  // An operand from the next step to load on; what lies past its end (rows of a ragged tile, steps past the last: never
-  // used) reads zero.  Columns past the end of a k-major row read the next row's: products that are never stored.
-  struct Src {
-    uint64_t addr;
-    int left;  // 128-byte blocks up to the operand's end
-    __device__ __forceinline__ i32x4 rsrc() const {
-      const uint32_t bytes = (uint32_t)min(max(left, 0), (1 << 25) - 1) << 7;
-      return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)addr), __builtin_amdgcn_readfirstlane((int)((addr >> 32) & 0xffff)),
-                   __builtin_amdgcn_readfirstlane((int)bytes), kRsrcWord3};
-    }
-    __device__ __forceinline__ void advance(int blocks) {
-      addr += (uint64_t)((int64_t)blocks * 128);
-      left -= blocks;
-    }
-  };
-  Src sa{reinterpret_cast<uint64_t>(opa + beg_a), (int)((end_a - beg_a) >> 6)};
-  Src sb{reinterpret_cast<uint64_t>(opb + beg_b), (int)((end_b - beg_b) >> 6)};
-  const int inc_b = SYM ? 1 : (int)(lx >> 1) ;  // blocks a step: 32 k of a row, or 32 rows
-  if (KG > 1) {
-    sa.advance(kg * per);
-    sb.advance(kg * per * inc_b);
+  ob.init(ldb, w, lane, wn * 16 * NB);
+  // Rows of a ragged tile and steps past the last read zero.  Columns past the end of a k-major row read the next row's:
+  // products that are never stored.
+  const int first = kg * per;
+  int left = G.steps - first;  // steps from the next one to load on
+  StepSrc sa, sb;
+  sa.addr = reinterpret_cast<uint64_t>(opa + m0 * lda + (int64_t)first * 64);
+  sa.full = extent_of(min(TM, G.mp - m0), lda, 64);
+  sa.inc = 128;
+  if constexpr (SYM) {
+    sb.addr = reinterpret_cast<uint64_t>(opb + n0 * ldb + (int64_t)first * 64);
+    sb.full = extent_of(min(TN, G.mp - n0), ldb, 64);
+    sb.inc = 128;
+  } else {
+    sb.addr = reinterpret_cast<uint64_t>(opb + (int64_t)n0 * 2 + first * 32 * ldb);
+    sb.full = extent_of(32, ldb, 2 * min(TN, G.np - n0));
+    sb.inc = (uint32_t)(64 * ldb);
   }
+  sa.tail = sb.tail = 0;
+  i32x4 ra = sa.rsrc(left, 1), rb = sb.rsrc(left, 1);
+  auto next_step = [&]() {
+    sa.addr += sa.inc;
+    sb.addr += sb.inc;
+    left -= 1;
+    ra = sa.rsrc(left, 1);
+    rb = sb.rsrc(left, 1);
+  };
   unsigned char* sm = smem + kg * NST * STAGE;
   const uint32_t lds_a = __builtin_amdgcn_readfirstlane(lds_addr(sm) + w * OpA::LOADS * 1024);
   const uint32_t lds_b = __builtin_amdgcn_readfirstlane(lds_addr(sm) + OpA::BYTES + w * OpB::LOADS * 1024);
-  auto load = [&](const i32x4& ra, const i32x4& rb, auto stage, auto q) {
+  auto load = [&](auto stage, auto q) {
     constexpr int s = decltype(stage)::value, n = decltype(q)::value;
     if constexpr (n < OpA::LOADS) dma_at<s * STAGE + n * 1024>(ra, oa.off[n], lds_a);
     else dma_at<s * STAGE + (n - OpA::LOADS) * 1024>(rb, ob.off[n - OpA::LOADS], lds_b);
@@ -424,10 +425,8 @@ __device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*
     });
   };
   unroll<NST>([&](auto st) {
-    const i32x4 ra = sa.rsrc(), rb = sb.rsrc();
-    unroll<LOADS>([&](auto q) { load(ra, rb, st, q); });
-    sa.advance(1);
-    sb.advance(inc_b);
+    if constexpr (decltype(st)::value > 0) next_step();
+    unroll<LOADS>([&](auto q) { load(st, q); });
   });
   __builtin_amdgcn_s_waitcnt(wait_vm((NST - 1) * LOADS));  // loads complete in issue order: step 0 has landed
   __builtin_amdgcn_s_barrier();
@@ -438,40 +437,59 @@ __device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*
 #pragma unroll
     for (int i = 0; i < MB; ++i) al[i] = oa.frag(sm, i, 1);
   }
-  // step kt, in stage ST
-  auto step = [&](auto st, int kt) {
+  // a step in stage ST; LIVE: this wave multiplies in it
+  auto step = [&](auto st, auto live_tag) {
     constexpr int ST = decltype(st)::value, NEXT = (ST + 1) % NST;
+    constexpr bool LIVE = decltype(live_tag)::value;
     const unsigned char* cur = sm + ST * STAGE;
     const unsigned char* nxt = sm + NEXT * STAGE;
     __builtin_amdgcn_sched_barrier(0);
-    if (kt < own) {
+    if constexpr (LIVE) {
       round(al, bh, std::integral_constant<int, MB>{}, [&](auto q) { ah[q] = oa.frag(cur, q, 0); });
-      round(ah, bh, std::integral_constant<int, NB>{}, [&](auto q) { bl[q] = ob.frag(cur + OpA::BYTES, q, 1); });
+      round(ah, bh, std::integral_constant<int, NB>{}, [&](auto q) {
+        bl[q] = ob.frag(cur + OpA::BYTES, q, 1);
+        if constexpr (decltype(q)::value == 0) next_step();
+      });
+    } else {
+      next_step();
     }
     // this wave's loads of step kt + 1 have landed and its fragments of step kt are read; then every wave's
     __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0((NST - 2) * LOADS));
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    const i32x4 ra = sa.rsrc(), rb = sb.rsrc();
-    if (kt < own) {
+    if constexpr (LIVE) {
       round(ah, bl, std::integral_constant<int, MB + NB>{}, [&](auto qt) {
         constexpr int q = decltype(qt)::value;
         if constexpr (q < NB) bh[q] = ob.frag(nxt + OpA::BYTES, q, 0);
         else al[q - NB] = oa.frag(nxt, q - NB, 1);
-        if constexpr (q < LOADS) load(ra, rb, st, qt);
+        if constexpr (q < LOADS) load(st, qt);
       });
     } else {
-      unroll<LOADS>([&](auto q) { load(ra, rb, st, q); });
+      unroll<LOADS>([&](auto q) { load(st, q); });
     }
-    sa.advance(1);
-    sb.advance(inc_b);
   };
-  int kt = 0;
-  while (kt < per) {
-    unroll<NST>([&](auto st) {
-      if (kt < per) step(st, kt++);
-    });
+  // a wave multiplies in all of the group's steps, in none, or (in the last k group) in all but the last ones
+  auto steps = [&](auto live_tag) {
+    for (int kt = 0; kt < per;) {
+      unroll<NST>([&](auto st) {
+        if (kt < per) step(st, live_tag);
+        ++kt;
+      });
+    }
+  };
+  if (own == 0) {
+    steps(std::false_type{});
+  } else if (KG == 1 || own == per) {
+    steps(std::true_type{});
+  } else {
+    for (int kt = 0; kt < per;) {
+      unroll<NST>([&](auto st) {
+        if (kt < own) step(st, std::true_type{});
+        else if (kt < per) step(st, std::false_type{});
+        ++kt;
+      });
+    }
   }
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no DMA may land after the workgroup exits
 

@@ -46,7 +46,7 @@ def _pointers(values):
 def _padded(shape) -> int:
     """Bytes of workspace that a matrix takes."""
     m, n = (v + -v % 64 for v in sorted(shape))
-    return 8 * m * (n + m + 64)
+    return 8 * m * (n + m)
 
 
 def _calls(kinds):

@@ -144,7 +144,7 @@ def test_muon_calls_are_cut():
             groups = [L.LlattnMuonGroup(n, *kinds[k][0], 0, 0, 1.0, 0.1) for k, _, n in call]
             cfg, _ = _muon_cfg(n_groups=len(groups))
             n = L.load().llattn_muon_bytes(ctypes.byref(cfg), (L.LlattnMuonGroup * len(groups))(*groups))
-            assert 0 < n <= muon.WORKSPACE_BYTES + (1 << 20) or len(groups) == groups[0].batch == 1
+            assert n > 0 and (n <= muon.WORKSPACE_BYTES + (1 << 20) or len(groups) == groups[0].batch == 1)
             for k, first, n in call:
                 seen[k] += range(first, first + n)
         assert seen == [list(range(c)) for _, c in kinds]
