@@ -297,47 +297,78 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
     return;
   }
   const auto column = [&](int j) { return col0 + 32 * (j >> 1) + 8 * g + 4 * (j & 1); };  // of block j's element 0, within the piece
+  // What few elements need stands behind branches that few waves take: the target's element and the columns past the
+  // piece.  (An exponential takes 16 cycles of its SIMD and any other instruction 4; 128 elements a lane, two waves.)
+  const bool ragged = n0 + TN > a.N;
 #pragma unroll
   for (int i = 0; i < MB; ++i) {
     const int row = row0 + 16 * i + r;
     const bool live = row < a.M;
     const int64_t tg = live ? a.targets[row] : a.ignore_index;
-    const int64_t tc = tg - a.v0;  // the target's column within the piece
+    const bool inside = live && tg >= a.v0 && tg < a.v0 + a.N;
+    const int tc = inside ? (int)(tg - a.v0) : -1;                                             // the target's column
+    const bool mine_too = inside && (unsigned)(tc - col0) < 16u * NB && ((tc - col0) >> 3 & 3) == g;  // among this lane's
     if constexpr (EPI == GRAD) {
-      const float l2 = live ? a.lse2[row] : 0.f;
+      float l2 = live ? a.lse2[row] : 0.f;
       const bool ignored = tg == a.ignore_index;
-      float s = 0.f;
-      if (live && !ignored) s = tg < 0 || tg >= a.V ? __builtin_nanf("") : a.per_row ? a.grad[row] : 1.f;
+      if (!ignored && (tg < 0 || tg >= a.V)) l2 = __builtin_nanf("");
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fast_exp2(fmaf(acc[i][j][e], kLog2e, -l2));
+      if (mine_too) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] -= column(j) + e == tc ? 1.f : 0.f;
+      }
+      if (a.per_row) {
+        const float s = live ? a.grad[row] : 0.f;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] *= s;
+      }
+      if (ragged) {  // columns past the piece are zero: the products contract over them
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = column(j) + e < a.N ? acc[i][j][e] : 0.f;
+      }
       uint16_t* out = a.p + (int64_t)row * a.ldp;
 #pragma unroll
-      for (int j = 0; j < NB; ++j) {
+      for (int j = 0; j < NB; j += 2) {
         const int c = column(j);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float q = fast_exp2(fmaf(acc[i][j][e], kLog2e, -l2)) - (c + e == tc ? 1.f : 0.f);
-          acc[i][j][e] = ignored || c + e >= a.N ? 0.f : q * s;  // columns past the piece are zero: the products contract over them
-        }
-        if (j % 2 == 1 && live && c < a.ldp) {  // 16 rows x 64 bytes a store (64 rows of 8 bytes took a tenth longer)
-          const f32x4 u = acc[i][j - 1], v = acc[i][j];
-          st16(out + column(j - 1), make_uint4(pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])));
-        }
+        const f32x4 u = acc[i][j], v = acc[i][j + 1];
+        uint4 q = make_uint4(pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        if (ignored) q = make_uint4(0, 0, 0, 0);
+        if (live && c < a.ldp) st16(out + c, q);  // 16 rows x 64 bytes a store (64 rows of 8 bytes took a tenth longer)
       }
     } else {
       float m = kNegInf;
       int mi = 0x7fffffff;
+      if (ragged) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = column(j) + e < a.N ? acc[i][j][e] : kNegInf;
+      }
+      if (mine_too) {
+        float v = 0.f;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v = column(j) + e == tc ? acc[i][j][e] : v;
+        a.tgt[row] = v;
+      }
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int c = column(j) + e;
-          const float v = c < a.N ? acc[i][j][e] : kNegInf;
-          acc[i][j][e] = v;
           if constexpr (EPI == STATS_PRED) {
-            if (c < a.N) max_first(m, mi, v, a.v0 + c);
+            const int c = column(j) + e;
+            if (c < a.N) max_first(m, mi, acc[i][j][e], a.v0 + c);
           } else {
-            m = fmaxf(m, v);
+            m = fmaxf(m, acc[i][j][e]);
           }
-          if (c == tc && live && c < a.N) a.tgt[row] = v;
         }
       if constexpr (EPI == STATS_PRED) {
         max_first(m, mi, __shfl_xor(m, 16), __shfl_xor(mi, 16));
