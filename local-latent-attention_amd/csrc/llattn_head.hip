@@ -208,6 +208,17 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
       __builtin_amdgcn_sched_barrier(0);
     });
   };
+  // What the epilogue reads of the wave's rows, a row a lane: read here, it costs no latency there.
+  constexpr bool LOSS = EPI == STATS || EPI == STATS_PRED || EPI == GRAD;
+  const int lane_row = row0 + lane % (16 * MB);
+  int64_t tg = a.ignore_index;
+  float lane_l2 = 0.f;
+  if constexpr (LOSS) {
+    if (lane_row < a.M) {
+      tg = a.targets[lane_row];
+      if constexpr (EPI == GRAD) lane_l2 = a.lse2[lane_row];
+    }
+  }
   unroll<NST>([&](auto st) {
     if constexpr (decltype(st)::value > 0) next_step();
     unroll<LOADS>([&](auto q) { load(st, q); });
@@ -215,6 +226,12 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
   __builtin_amdgcn_s_waitcnt(wait_vm((NST - 1) * LOADS));  // loads complete in issue order: step 0 has landed
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+  int lane_tc = -1;  // the target's column within the piece; -1: it has none, -2: an ignored row
+  if constexpr (LOSS) {
+    if (tg == a.ignore_index) lane_tc = -2;
+    else if (tg >= a.v0 && tg < a.v0 + a.N) lane_tc = (int)(tg - a.v0);
+    else if (tg < 0 || tg >= a.V) lane_l2 = __builtin_nanf("");
+  }
   if (own) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) b0[j] = ob.frag(smem + OpA::BYTES, j, 0);
@@ -304,19 +321,15 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
   for (int i = 0; i < MB; ++i) {
     const int row = row0 + 16 * i + r;
     const bool live = row < a.M;
-    const int64_t tg = live ? a.targets[row] : a.ignore_index;
-    const bool inside = live && tg >= a.v0 && tg < a.v0 + a.N;
-    const int tc = inside ? (int)(tg - a.v0) : -1;                                             // the target's column
-    const bool mine_too = inside && (unsigned)(tc - col0) < 16u * NB && ((tc - col0) >> 3 & 3) == g;  // among this lane's
+    const int tc = __shfl(lane_tc, 16 * i + r);
+    const bool has = tc >= col0 && tc < col0 + 16 * NB && ((tc - col0) >> 3 & 3) == g;  // among this lane's columns
     if constexpr (EPI == GRAD) {
-      float l2 = live ? a.lse2[row] : 0.f;
-      const bool ignored = tg == a.ignore_index;
-      if (!ignored && (tg < 0 || tg >= a.V)) l2 = __builtin_nanf("");
+      const float l2 = __shfl(lane_l2, 16 * i + r);
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][j][e] = fast_exp2(fmaf(acc[i][j][e], kLog2e, -l2));
-      if (mine_too) {
+      if (has) {
 #pragma unroll
         for (int j = 0; j < NB; ++j)
 #pragma unroll
@@ -339,7 +352,7 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
         const int c = column(j);
         const f32x4 u = acc[i][j], v = acc[i][j + 1];
         uint4 q = make_uint4(pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-        if (ignored) q = make_uint4(0, 0, 0, 0);
+        if (tc == -2) q = make_uint4(0, 0, 0, 0);
         if (live && c < a.ldp) st16(out + c, q);  // 16 rows x 64 bytes a store (64 rows of 8 bytes took a tenth longer)
       }
     } else {
@@ -351,7 +364,7 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i][j][e] = column(j) + e < a.N ? acc[i][j][e] : kNegInf;
       }
-      if (mine_too) {
+      if (has) {
         float v = 0.f;
 #pragma unroll
         for (int j = 0; j < NB; ++j)
