@@ -33,7 +33,7 @@ enum Epilogue { STATS = 0, STATS_PRED = 1, GRAD = 2, SUM = 3, OUT_BF16 = 4, OUT_
 struct HeadArgs {
   int M, N, K;              // rows, columns, contraction
   int steps, per;           // 64-wide k steps, of a split
-  int tiles_m, tiles_n;
+  int tiles_m, tiles_n, total;  // total: with the splits
   const uint16_t* A; int64_t lda;
   const uint16_t* B; int64_t ldb;
   // logits
@@ -150,22 +150,24 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
   static_assert(S::WC == 2 && (S::WR == 2 || S::WR == 4), "wave layouts");
   // eight waves: those of one SIMD (w, w + 4) lie in opposite halves of both sides
   const int wm = W == 8 ? (w & 3) ^ (w >> 2 << 1) : w >> 1, wn = W == 8 ? (w & 1) ^ (w >> 2) : w & 1;
-  int t = xcd_remap(blockIdx.x, gridDim.x);
-  const int tiles = a.tiles_m * a.tiles_n, split = t / tiles;
-  t -= split * tiles;
-  constexpr int GM = 8;
-  const int group = t / (GM * a.tiles_n), first_m = group * GM, gm = min(a.tiles_m - first_m, GM);
-  const int tm = first_m + (t % (GM * a.tiles_n)) % gm, tn = t % (GM * a.tiles_n) / gm;
-  const int m0 = __builtin_amdgcn_readfirstlane(tm * TM), n0 = __builtin_amdgcn_readfirstlane(tn * TN);
-  const int row0 = m0 + wm * 16 * MB, col0 = n0 + wn * 16 * NB;
-  const int k0 = split * a.per, mine = min(a.steps - k0, a.per);  // steps of this split (none: zeros)
-  const bool own = row0 < a.M && col0 < a.N && mine > 0;
+  // Workgroup b takes tiles b, b + gridDim.x, ... of the launch's order (its XCD's share of them, a run of the tiles).
+  struct Tile { int m0, n0, split, steps; };  // steps: of the split (none or less: zeros)
+  auto tile_at = [&](int v) {
+    int t = xcd_remap(v, a.total);
+    const int tiles = a.tiles_m * a.tiles_n, split = t / tiles;
+    t -= split * tiles;
+    constexpr int GM = 8;
+    const int group = t / (GM * a.tiles_n), first_m = group * GM, gm = min(a.tiles_m - first_m, GM);
+    const int tm = first_m + (t % (GM * a.tiles_n)) % gm, tn = t % (GM * a.tiles_n) / gm;
+    const int steps = min(a.steps - split * a.per, a.per);
+    return Tile{__builtin_amdgcn_readfirstlane(tm * TM), __builtin_amdgcn_readfirstlane(tn * TN),
+                __builtin_amdgcn_readfirstlane(split), __builtin_amdgcn_readfirstlane(steps)};
+  };
   OpA oa;
   OpB ob;
   oa.init(a.lda, w, lane, wm * 16 * MB);
   ob.init(a.ldb, w, lane, wn * 16 * NB);
-  int left = a.K - k0 * 64;  // k from the next step to load to the contraction's end
-  auto source = [&](const uint16_t* p, int64_t ld, bool t, int o, int n) {  // a tile of n of the operand's rows (t: columns) from o on
+  auto source = [&](const uint16_t* p, int64_t ld, bool t, int o, int n, int k0) {  // n of the operand's rows (t: columns) from o on
     StepSrc s;
     s.addr = reinterpret_cast<uint64_t>(p + (t ? o + (int64_t)k0 * 64 * ld : o * ld + (int64_t)k0 * 64));
     s.full = t ? extent_of(64, ld, n) : extent_of(n, ld, 64);  // not t: chunks past the last k are masked (RowOp::at)
@@ -173,10 +175,15 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
     s.inc = t ? (uint32_t)(128 * ld) : 128u;
     return s;
   };
-  StepSrc sa = source(a.A, a.lda, AT, m0, min(TM, a.M - m0)), sb = source(a.B, a.ldb, BT, n0, min(TN, a.N - n0));
-  i32x4 ra = sa.rsrc(left, 64), rb = sb.rsrc(left, 64);
-  int ahead = left;  // of the step that ra and rb describe
-  auto next_step = [&]() {
+  auto source_a = [&](const Tile& t) { return source(a.A, a.lda, AT, t.m0, min(TM, a.M - t.m0), t.split * a.per); };
+  auto source_b = [&](const Tile& t) { return source(a.B, a.ldb, BT, t.n0, min(TN, a.N - t.n0), t.split * a.per); };
+  auto k_of = [&](const Tile& t) { return min(a.K - t.split * a.per * 64, t.steps * 64); };
+  int v = blockIdx.x;
+  Tile tile = tile_at(v);
+  StepSrc sa = source_a(tile), sb = source_b(tile);
+  int ahead = k_of(tile);  // k from the step that ra and rb describe to the end of its tile's
+  i32x4 ra = sa.rsrc(ahead, 64), rb = sb.rsrc(ahead, 64);
+  auto advance = [&]() {
     sa.addr += sa.inc;
     sb.addr += sb.inc;
     ahead -= 64;
@@ -192,10 +199,6 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
   };
   bf16x8 a0[MB], a1[MB], b0[NB], b1[NB];  // k 0..31 and 32..63
   f32x4 acc[MB][NB];
-#pragma unroll
-  for (int i = 0; i < MB; ++i)
-#pragma unroll
-    for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   // MB NB products, B first: lane (r, g) accumulates C[r][4 g + e]; io(q), q < MB + NB, spread over them
   auto round = [&](const bf16x8 (&x)[MB], const bf16x8 (&y)[NB], auto io) {
     constexpr int N = MB + NB, P = MB * NB;
@@ -208,201 +211,244 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
       __builtin_amdgcn_sched_barrier(0);
     });
   };
-  // What the epilogue reads of the wave's rows, a row a lane: read here, it costs no latency there.
+  // What the epilogue of a tile reads of the wave's rows, a row a lane: read ahead of it, it costs no latency there.
   constexpr bool LOSS = EPI == STATS || EPI == STATS_PRED || EPI == GRAD;
-  const int lane_row = row0 + lane % (16 * MB);
-  int64_t tg = a.ignore_index;
-  float lane_l2 = 0.f;
-  if constexpr (LOSS) {
-    if (lane_row < a.M) {
-      tg = a.targets[lane_row];
-      if constexpr (EPI == GRAD) lane_l2 = a.lse2[lane_row];
+  int64_t read_tg = a.ignore_index;
+  float read_l2 = 0.f;
+  auto read_rows = [&](const Tile& t) {
+    if constexpr (LOSS) {
+      const int row = t.m0 + wm * 16 * MB + lane % (16 * MB);
+      read_tg = a.ignore_index;
+      read_l2 = 0.f;
+      if (row < a.M) {
+        read_tg = a.targets[row];
+        if constexpr (EPI == GRAD) read_l2 = a.lse2[row];
+      }
     }
-  }
+  };
+  float lane_l2 = 0.f;
+  int lane_tc = -1;  // the target's column within the piece; -1: it has none, -2: an ignored row
+  auto settle_rows = [&]() {
+    if constexpr (LOSS) {
+      const int64_t t = read_tg;
+      lane_tc = t == a.ignore_index ? -2 : t >= a.v0 && t < a.v0 + a.N ? (int)(t - a.v0) : -1;
+      lane_l2 = t != a.ignore_index && (t < 0 || t >= a.V) ? __builtin_nanf("") : read_l2;
+    }
+  };
+  read_rows(tile);
   unroll<NST>([&](auto st) {
-    if constexpr (decltype(st)::value > 0) next_step();
+    if constexpr (decltype(st)::value > 0) advance();
     unroll<LOADS>([&](auto q) { load(st, q); });
   });
   __builtin_amdgcn_s_waitcnt(wait_vm((NST - 1) * LOADS));  // loads complete in issue order: step 0 has landed
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  int lane_tc = -1;  // the target's column within the piece; -1: it has none, -2: an ignored row
-  if constexpr (LOSS) {
-    if (tg == a.ignore_index) lane_tc = -2;
-    else if (tg >= a.v0 && tg < a.v0 + a.N) lane_tc = (int)(tg - a.v0);
-    else if (tg < 0 || tg >= a.V) lane_l2 = __builtin_nanf("");
-  }
-  if (own) {
+  auto first_frags = [&]() {
 #pragma unroll
     for (int j = 0; j < NB; ++j) b0[j] = ob.frag(smem + OpA::BYTES, j, 0);
 #pragma unroll
     for (int i = 0; i < MB; ++i) a0[i] = oa.frag(smem, i, 0);
-  }
-  auto step = [&](auto st, auto live_tag) {
-    constexpr int ST = decltype(st)::value, NEXT = (ST + 1) % NST;
-    constexpr bool LIVE = decltype(live_tag)::value;
-    const unsigned char* cur = smem + ST * STAGE;
-    const unsigned char* nxt = smem + NEXT * STAGE;
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (LIVE)
-      round(a0, b0, [&](auto qt) {
-        constexpr int q = decltype(qt)::value;
-        if constexpr (q < NB) b1[q] = ob.frag(cur + OpA::BYTES, q, 1);
-        else a1[q - NB] = oa.frag(cur, q - NB, 1);
-        if constexpr (q == 0) next_step();
-      });
-    else next_step();
-    // this wave's loads of step kt + 1 have landed and its fragments of step kt are read; then every wave's
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0((NST - 2) * LOADS));
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (LIVE)
-      round(a1, b1, [&](auto qt) {
-        constexpr int q = decltype(qt)::value;
-        if constexpr (q < NB) b0[q] = ob.frag(nxt + OpA::BYTES, q, 0);
-        else a0[q - NB] = oa.frag(nxt, q - NB, 0);
-        if constexpr (q < LOADS) load(st, qt);
-      });
-    else unroll<LOADS>([&](auto q) { load(st, q); });
   };
-  auto steps = [&](auto live_tag) {
+  bool own = tile.m0 + wm * 16 * MB < a.M && tile.n0 + wn * 16 * NB < a.N;  // part of the tile is this wave's
+  if (own) first_frags();
+  for (;;) {
+    // The next tile's first steps are loaded, and its first fragments read, in this one's last steps: no step of the
+    // pipeline waits for the epilogue between them.  A tile before another takes whole turns of the stages.
+    const bool more = LOSS && v + (int)gridDim.x < a.total;
+    const Tile next = more ? tile_at(v + gridDim.x) : tile;
+    const StepSrc next_a = source_a(next), next_b = source_b(next);
+    const int next_k = more ? k_of(next) : 0;
+    const int steps = more ? (max(tile.steps, 1) + NST - 1) / NST * NST : tile.steps;
+    const int row0 = tile.m0 + wm * 16 * MB, n0 = tile.n0, col0 = n0 + wn * 16 * NB, tn = n0 / TN;
+    settle_rows();
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     int kt = 0;
-    while (kt < mine) {
-      unroll<NST>([&](auto st) {
-        if (kt < mine) {
-          step(st, live_tag);
-          ++kt;
-        }
-      });
-    }
-  };
-  if (own) steps(std::true_type{});
-  else steps(std::false_type{});
-  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no DMA may land after the workgroup exits
-
-  if constexpr (EPI == SUM || EPI == OUT_BF16 || EPI == OUT_F32) {
-    float alpha = 1.f;
-    if (EPI != SUM && !a.per_row) alpha = *a.grad * (a.inv ? *a.inv : 1.f);
-#pragma unroll
-    for (int i = 0; i < MB; ++i) {
-      const int row = row0 + 16 * i + r;
-      if (row >= a.M) continue;
-#pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        const int col = col0 + 16 * j + 4 * g;
-        if (col >= a.N) continue;
-        const int64_t o = ((int64_t)(EPI == SUM ? split : 0) * a.M + row) * a.N + col;
-        float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        if constexpr (EPI == SUM) {
-          float* c = static_cast<float*>(a.C) + o;
-          if (a.accumulate) {
-            float x[4];
-            load4<float>(c, x);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += x[e];
+    auto next_step = [&]() {
+      if (LOSS && kt + NST == steps) {
+        sa = next_a;
+        sb = next_b;
+        ahead = next_k;
+        ra = sa.rsrc(ahead, 64);
+        rb = sb.rsrc(ahead, 64);
+      } else {
+        advance();
+      }
+    };
+    auto step = [&](auto st, auto live_tag) {
+      constexpr int ST = decltype(st)::value, NEXT = (ST + 1) % NST;
+      constexpr bool LIVE = decltype(live_tag)::value;
+      const unsigned char* cur = smem + ST * STAGE;
+      const unsigned char* nxt = smem + NEXT * STAGE;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (LIVE)
+        round(a0, b0, [&](auto qt) {
+          constexpr int q = decltype(qt)::value;
+          if constexpr (q < NB) b1[q] = ob.frag(cur + OpA::BYTES, q, 1);
+          else a1[q - NB] = oa.frag(cur, q - NB, 1);
+          if constexpr (q == 0) next_step();
+        });
+      else next_step();
+      // this wave's loads of step kt + 1 have landed and its fragments of step kt are read; then every wave's
+      __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0((NST - 2) * LOADS));
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (LIVE)
+        round(a1, b1, [&](auto qt) {
+          constexpr int q = decltype(qt)::value;
+          if constexpr (q < NB) b0[q] = ob.frag(nxt + OpA::BYTES, q, 0);
+          else a0[q - NB] = oa.frag(nxt, q - NB, 0);
+          if constexpr (q < LOADS) load(st, qt);
+        });
+      else unroll<LOADS>([&](auto q) { load(st, q); });
+    };
+    auto all_steps = [&](auto live_tag) {
+      while (kt < steps) {
+        unroll<NST>([&](auto st) {
+          if (kt < steps) {
+            step(st, live_tag);
+            ++kt;
           }
-          store4<float>(c, v);
-        } else {
+        });
+      }
+    };
+    if (own) all_steps(std::true_type{});
+    else all_steps(std::false_type{});
+    const bool next_own = next.m0 + wm * 16 * MB < a.M && next.n0 + wn * 16 * NB < a.N;
+    if (more && next_own && !own) first_frags();
+    if (more) read_rows(next);
+
+    if constexpr (EPI == SUM || EPI == OUT_BF16 || EPI == OUT_F32) {
+      float alpha = 1.f;
+      if (EPI != SUM && !a.per_row) alpha = *a.grad * (a.inv ? *a.inv : 1.f);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] *= alpha;
-          if constexpr (EPI == OUT_F32) store4<float>(static_cast<float*>(a.C) + o, v);
-          else store4<uint16_t>(static_cast<uint16_t*>(a.C) + o, v);
+      for (int i = 0; i < MB; ++i) {
+        const int row = row0 + 16 * i + r;
+        if (row >= a.M) continue;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const int col = col0 + 16 * j + 4 * g;
+          if (col >= a.N) continue;
+          const int64_t o = ((int64_t)(EPI == SUM ? tile.split : 0) * a.M + row) * a.N + col;
+          float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+          if constexpr (EPI == SUM) {
+            float* c = static_cast<float*>(a.C) + o;
+            if (a.accumulate) {
+              float x[4];
+              load4<float>(c, x);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] += x[e];
+            }
+            store4<float>(c, v);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= alpha;
+            if constexpr (EPI == OUT_F32) store4<float>(static_cast<float*>(a.C) + o, v);
+            else store4<uint16_t>(static_cast<uint16_t*>(a.C) + o, v);
+          }
         }
-      }
-    }
-    return;
-  }
-  const auto column = [&](int j) { return col0 + 32 * (j >> 1) + 8 * g + 4 * (j & 1); };  // of block j's element 0, within the piece
-  // What few elements need stands behind branches that few waves take: the target's element and the columns past the
-  // piece.  (An exponential takes 16 cycles of its SIMD and any other instruction 4; 128 elements a lane, two waves.)
-  const bool ragged = n0 + TN > a.N;
-#pragma unroll
-  for (int i = 0; i < MB; ++i) {
-    const int row = row0 + 16 * i + r;
-    const bool live = row < a.M;
-    const int tc = __shfl(lane_tc, 16 * i + r);
-    const bool has = tc >= col0 && tc < col0 + 16 * NB && ((tc - col0) >> 3 & 3) == g;  // among this lane's columns
-    if constexpr (EPI == GRAD) {
-      const float l2 = __shfl(lane_l2, 16 * i + r);
-#pragma unroll
-      for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = fast_exp2(fmaf(acc[i][j][e], kLog2e, -l2));
-      if (has) {
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] -= column(j) + e == tc ? 1.f : 0.f;
-      }
-      if (a.per_row) {
-        const float s = live ? a.grad[row] : 0.f;
-#pragma unroll
-        for (int j = 0; j < NB; ++j) acc[i][j] *= s;
-      }
-      if (ragged) {  // columns past the piece are zero: the products contract over them
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] = column(j) + e < a.N ? acc[i][j][e] : 0.f;
-      }
-      uint16_t* out = a.p + (int64_t)row * a.ldp;
-#pragma unroll
-      for (int j = 0; j < NB; j += 2) {
-        const int c = column(j);
-        const f32x4 u = acc[i][j], v = acc[i][j + 1];
-        uint4 q = make_uint4(pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-        if (tc == -2) q = make_uint4(0, 0, 0, 0);
-        if (live && c < a.ldp) st16(out + c, q);  // 16 rows x 64 bytes a store (64 rows of 8 bytes took a tenth longer)
       }
     } else {
-      float m = kNegInf;
-      int mi = 0x7fffffff;
-      if (ragged) {
+      const auto column = [&](int j) { return col0 + 32 * (j >> 1) + 8 * g + 4 * (j & 1); };  // of block j's element 0, within the piece
+      // What few elements need stands behind branches that few waves take: the target's element and the columns past the
+      // piece.  (An exponential takes 16 cycles of its SIMD and any other instruction 4; 128 elements a lane, two waves.)
+      const bool ragged = n0 + TN > a.N;
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
+      for (int i = 0; i < MB; ++i) {
+        const int row = row0 + 16 * i + r;
+        const bool live = row < a.M;
+        const int tc = __shfl(lane_tc, 16 * i + r);
+        const bool has = tc >= col0 && tc < col0 + 16 * NB && ((tc - col0) >> 3 & 3) == g;  // among this lane's columns
+        if constexpr (EPI == GRAD) {
+          const float l2 = __shfl(lane_l2, 16 * i + r);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] = column(j) + e < a.N ? acc[i][j][e] : kNegInf;
-      }
-      if (has) {
-        float v = 0.f;
+          for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = fast_exp2(fmaf(acc[i][j][e], kLog2e, -l2));
+          if (has) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v = column(j) + e == tc ? acc[i][j][e] : v;
-        a.tgt[row] = v;
-      }
+            for (int j = 0; j < NB; ++j)
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
+              for (int e = 0; e < 4; ++e) acc[i][j][e] -= column(j) + e == tc ? 1.f : 0.f;
+          }
+          if (a.per_row) {
+            const float s = live ? a.grad[row] : 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+            for (int j = 0; j < NB; ++j) acc[i][j] *= s;
+          }
+          if (ragged) {  // columns past the piece are zero: the products contract over them
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[i][j][e] = column(j) + e < a.N ? acc[i][j][e] : 0.f;
+          }
+          uint16_t* out = a.p + (int64_t)row * a.ldp;
+#pragma unroll
+          for (int j = 0; j < NB; j += 2) {
+            const int c = column(j);
+            const f32x4 u = acc[i][j], v = acc[i][j + 1];
+            uint4 q = make_uint4(pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+            if (tc == -2) q = make_uint4(0, 0, 0, 0);
+            if (live && c < a.ldp) st16(out + c, q);  // 16 rows x 64 bytes a store (64 rows of 8 bytes took a tenth longer)
+          }
+        } else {
+          float m = kNegInf;
+          int mi = 0x7fffffff;
+          if (ragged) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[i][j][e] = column(j) + e < a.N ? acc[i][j][e] : kNegInf;
+          }
+          if (has) {
+            float v = 0.f;
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v = column(j) + e == tc ? acc[i][j][e] : v;
+            a.tgt[row] = v;
+          }
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (EPI == STATS_PRED) {
+                const int c = column(j) + e;
+                if (c < a.N) max_first(m, mi, acc[i][j][e], a.v0 + c);
+              } else {
+                m = fmaxf(m, acc[i][j][e]);
+              }
+            }
           if constexpr (EPI == STATS_PRED) {
-            const int c = column(j) + e;
-            if (c < a.N) max_first(m, mi, acc[i][j][e], a.v0 + c);
+            max_first(m, mi, __shfl_xor(m, 16), __shfl_xor(mi, 16));
+            max_first(m, mi, __shfl_xor(m, 32), __shfl_xor(mi, 32));
           } else {
-            m = fmaxf(m, acc[i][j][e]);
+            m = max_groups(m);
+          }
+          const float c0 = m == kNegInf ? 0.f : __fmul_rn(m, kLog2e);
+          float s = 0.f;
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s += fast_exp2(fmaf(acc[i][j][e], kLog2e, -c0));
+          s = sum_groups(s);
+          if (live && g == 0) {
+            const int64_t o = (int64_t)(2 * tn + wn) * a.M + row;
+            a.part[o] = make_float2(m, s);
+            if constexpr (EPI == STATS_PRED) a.part_i[o] = mi;
           }
         }
-      if constexpr (EPI == STATS_PRED) {
-        max_first(m, mi, __shfl_xor(m, 16), __shfl_xor(mi, 16));
-        max_first(m, mi, __shfl_xor(m, 32), __shfl_xor(mi, 32));
-      } else {
-        m = max_groups(m);
-      }
-      const float c0 = m == kNegInf ? 0.f : __fmul_rn(m, kLog2e);
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s += fast_exp2(fmaf(acc[i][j][e], kLog2e, -c0));
-      s = sum_groups(s);
-      if (live && g == 0) {
-        const int64_t o = (int64_t)(2 * tn + wn) * a.M + row;
-        a.part[o] = make_float2(m, s);
-        if constexpr (EPI == STATS_PRED) a.part_i[o] = mi;
       }
     }
+    if (!more) break;
+    v += gridDim.x;
+    tile = next;
+    own = next_own;
   }
+  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no DMA may land after the workgroup exits
 }
 
 // Joins the parts of R rows: Q = 256 / R threads a row take every Q-th part, first the maxima, then the sums against the
@@ -633,7 +679,9 @@ void launch(HeadArgs& a, int kind, int splits, hipStream_t st) {
   a.per = (a.steps + splits - 1) / splits;
   a.tiles_m = (a.M + kTm[kind] - 1) / kTm[kind];
   a.tiles_n = (a.N + kTn[kind] - 1) / kTn[kind];
-  const dim3 grid((unsigned)(a.tiles_m * a.tiles_n * splits));
+  a.total = a.tiles_m * a.tiles_n * splits;
+  const bool loss = EPI == STATS || EPI == STATS_PRED || EPI == GRAD;
+  const dim3 grid((unsigned)(loss ? std::min(a.total, 256 * kPerCu[kind]) : a.total));
   if (kind == BIG) hipLaunchKernelGGL((head_kernel<EPI, AT, BT, BigShape, 1>), grid, dim3(BigShape::THREADS), 0, st, a);
   else if (kind == SQUARE) hipLaunchKernelGGL((head_kernel<EPI, AT, BT, SquareShape, 2>), grid, dim3(SquareShape::THREADS), 0, st, a);
   else if constexpr (!AT && !BT) hipLaunchKernelGGL((head_kernel<EPI, AT, BT, ThinShape, 2>), grid, dim3(ThinShape::THREADS), 0, st, a);
