@@ -471,7 +471,8 @@ __device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*
   };
   // a wave multiplies in all of the group's steps, in none, or (in the last k group) in all but the last ones
   auto steps = [&](auto live_tag) {
-    for (int kt = 0; kt < per;) {
+    int kt = 0;
+    while (kt < per) {
       unroll<NST>([&](auto st) {
         if (kt < per) step(st, live_tag);
         ++kt;
@@ -483,7 +484,8 @@ __device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*
   } else if (KG == 1 || own == per) {
     steps(std::true_type{});
   } else {
-    for (int kt = 0; kt < per;) {
+    int kt = 0;
+    while (kt < per) {
       unroll<NST>([&](auto st) {
         if (kt < own) step(st, std::true_type{});
         else if (kt < per) step(st, std::false_type{});
@@ -972,13 +974,13 @@ float scale_of(const GroupPlan& g) { return std::exp2f((float)std::min(14, (int)
 // the 256 CUs, the last with fewer workgroups on each; of several, its work is shared out and ends with a part of the
 // longest tile.  Measured in us (G: X Xᵀ, P: A A, A: B X):
 //                                   64 x 64        64 x 64, 2 k groups   128 x 128       256 x 256
-//   3 of 333 x 1001     G P A     13   9  12         12   9  15          28  20  19      64  42  49
-//   1 of 512 x 1408     G P A     15  10  10         13   9  10          39  22  21      95  64  55
-//   1 of 1408 x 4096    G P A     44  20  70         39  18  89          87  43  64     218 109 102
-//   6 of 1000 x 1500    G P A     52  42  82          -                  46  38  81     109  96  88
-//   22 of 1408 x 1408   G P A    287 307 526          -                 236 249 399     232 254 427
-//   22 of 1408 x 4096   G P A    831 307 1526         -                 557 261 1106    549 263 1076
-//   8 of 4096 x 4096    G P A   3250 3397 4082        -                1633 1813 2947  1601 1607 2469
+//   3 of 333 x 1001     G P A     11   9  12         11   9  15          26  20  19      62  41  48
+//   1 of 512 x 1408     G P A     14   9  10         13   9  10          36  22  21      91  64  54
+//   1 of 1408 x 4096    G P A     37  18  63         32  16  73          80  41  62     208 107  98
+//   6 of 1000 x 1500    G P A     49  39  77          -                  43  36  75     105  95  87
+//   22 of 1408 x 1408   G P A    273 291 506          -                 225 235 376     215 239 405
+//   22 of 1408 x 4096   G P A    846 288 1442         -                 517 251 1051    492 244 993
+//   8 of 4096 x 4096    G P A   3255 3395 3914        -                1489 1635 2751  1416 1472 2334
 // (128 x 256 tiles on eight waves lay between the last two throughout.)
 template <bool SYM>
 int choose(const llattn_muon_cfg* c, const llattn_muon_group* groups, const Plan& p, bool gram) {

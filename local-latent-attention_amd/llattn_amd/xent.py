@@ -246,7 +246,7 @@ def piecewise_head_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Te
     if not h.device == weight.device == targets.device:
         raise ValueError(f"piecewise_head_loss: tensors on {h.device}, {weight.device} and {targets.device}")
     args = (h, weight, targets, int(ignore_index), reduction, bool(return_pred), int(piece))
-    if not (h.requires_grad or weight.requires_grad) and type(h) is torch.Tensor and type(weight) is torch.Tensor:
+    if not (torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad)):
         out, pred, _ = _piece_forward(*args)  # nothing to differentiate: evaluation
         return (out, pred) if return_pred else out
     return _PieceLoss.apply(*args, torch.is_grad_enabled())

@@ -93,6 +93,29 @@ def test_loss_and_gradients(N, D, V, piece):
     _near(gw, dw, ew, BF16, "dw")
 
 
+@pytest.mark.parametrize("N,D,V", [(40, 200, 200003), (300, 72, 70001), (777, 64, 33000), (2100, 192, 40001)])
+def test_many_tiles_a_workgroup(N, D, V):
+    """More tiles than workgroups: odd numbers of steps, rows and columns that end inside a tile, gradients row by row,
+    targets that count for nothing or lie outside."""
+    h, w, t = _inputs(N, D, V, seed=V)
+    g = torch.randn(N, generator=torch.Generator().manual_seed(2)).to(DEV)
+    t[N // 2], t[N - 1] = V - 1, -100
+    (l, el), (dh, eh), (dw, ew) = _exact(h, w, t, g, "none")
+    hg, wg = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    rows, pred = _loss(hg, wg, t, reduction="none", return_pred=True)
+    _near(rows.detach(), l, el, F32, "loss")
+    assert torch.equal(rows.detach(), _loss(h, w, t, reduction="none"))
+    gh, gw = torch.autograd.grad(rows, (hg, wg), g)
+    _near(gh, dh, eh, BF16, "dh")
+    _near(gw, dw, ew, BF16, "dw")
+    logits = h.double() @ w.double().t()
+    top = logits.gather(1, pred.long()[:, None]).squeeze(1)
+    assert bool((logits.amax(1) - top <= 2 * D * U * (h.double().abs() @ w.double().abs().t()).amax(1)).all())
+    t[1] = V
+    rows = _loss(h, w, t, reduction="none")
+    assert torch.isnan(rows).nonzero().flatten().tolist() == [1]
+
+
 @pytest.mark.parametrize("reduction", ["sum", "none", "mean"])
 @pytest.mark.parametrize("which", ["h", "w", "both"])
 def test_reductions_and_upstream_gradients(reduction, which):
