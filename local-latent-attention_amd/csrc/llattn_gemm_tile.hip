@@ -23,6 +23,52 @@ namespace gemm {
 
 namespace {
 
+constexpr int SK = 64;  // k per stage
+
+// Tile operand of O rows / columns x 64 k.  k-contiguous: rows of 128 bytes, chunk c (8 k) of row o at slot
+// c ^ pswz<PERM>(o).  m/n-contiguous: 64 k-rows of 2 O bytes, chunk c (8 columns) of k-row k at c ^ 2 (k & 3).
+template <bool KC, bool PERM, int O>
+struct TileOp {
+  static constexpr int BYTES = O * 128, NB = BYTES / 1024 / 4;  // NB: 1 KB DMA blocks per wave
+  uint32_t off[NB];
+  int kc[NB];
+  __device__ __forceinline__ void init(int64_t ld, int o0, int omax, int w4, int lane) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int bi = w4 * NB + i;
+      if constexpr (KC) {  // rows past omax are clamped to a valid row (their outputs are never stored)
+        const int row = 8 * bi + (lane >> 3), c = (lane & 7) ^ pswz<PERM>(row);
+        off[i] = (uint32_t)(((int64_t)min(o0 + row, omax - 1) * ld + 8 * c) * 2);
+        kc[i] = 8 * c;
+      } else {
+        constexpr int PER = O / 8;
+        const int q = bi * 64 + lane, k = q / PER, c = (q % PER) ^ (2 * (k & 3));
+        off[i] = step_off(((int64_t)k * ld + min(o0 + 8 * c, omax - 8)) * 2);
+        kc[i] = 0;
+      }
+    }
+  }
+  // block i of this wave; klim = K - k0 of the step: k-contiguous chunks at or past K read zero
+  __device__ __forceinline__ void dma(const i32x4& rs, unsigned char* st, int w4, int i, int klim) const {
+    dma_block(rs, KC ? kmask(off[i], kc[i], klim) : off[i], st + (w4 * NB + i) * 1024);
+  }
+  static __device__ __forceinline__ bf16x8 frag(const unsigned char* st, int o16, int r, int g, int h) {
+    if constexpr (KC) {
+      return frag64<true, PERM>(st, o16, r, g, h);
+    } else {
+      const int kb = 32 * h + 8 * g, col = o16 + 4 * (r & 3), chunk = col >> 3, inner = (col & 7) << 1;
+      bf16x4 hv[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int k = kb + 4 * half + (r >> 2);
+        const unsigned char* p = st + k * (2 * O) + ((chunk ^ (2 * (k & 3))) << 4) + inner;
+        hv[half] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(p));
+      }
+      return bf16x8{hv[0][0], hv[0][1], hv[0][2], hv[0][3], hv[1][0], hv[1][1], hv[1][2], hv[1][3]};
+    }
+  }
+};
+
 // C[row][col .. col + 4) = v with the epilogue of the 256 x 256 kernels: bias, accumulation or row addends in fp32,
 // one rounding, then the activation on the rounded value.
 // EPI_PART: the plain sums into the partials of split `split`.
