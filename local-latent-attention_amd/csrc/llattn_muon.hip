@@ -159,6 +159,18 @@ __device__ __forceinline__ void store_halves4(uint16_t* row, int c, const float 
   *reinterpret_cast<uint2*>(p) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
   *reinterpret_cast<uint2*>(p + 32) = make_uint2(l[0] | (uint32_t)l[1] << 16, l[2] | (uint32_t)l[3] << 16);
 }
+__device__ __forceinline__ void store_halves8(uint16_t* row, int c, const float v[8]) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint16_t h0 = h_bits(v[2 * e]), h1 = h_bits(v[2 * e + 1]);
+    h[e] = h0 | (uint32_t)h1 << 16;
+    l[e] = h_bits(v[2 * e] - h_val(h0)) | (uint32_t)h_bits(v[2 * e + 1] - h_val(h1)) << 16;
+  }
+  uint16_t* p = row + hi_at(c);
+  st16(p, make_uint4(h[0], h[1], h[2], h[3]));
+  st16(p + 32, make_uint4(l[0], l[1], l[2], l[3]));
+}
 // One 64 x 64 tile of X per workgroup, through LDS (the reads run along U's rows either way).  a.m: the new momentum.
 __global__ __launch_bounds__(256) void muon_split_kernel(const ElemArgs a) {
   __shared__ double s[256];
@@ -504,92 +516,120 @@ __device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*
     flip = G.rows > G.cols;
     vec = G.cols % 4 == 0 && by4(out, G.w_dtype) && (!a.update || by4(w_ptr, G.w_dtype));
   }
-  // What the epilogue of a block reads: D, and the weight that LAST updates.  Loaded a row of blocks ahead of the stores:
-  // taken one by one behind them, each cost its latency (22 x 1408 x 1408, POLY: 34 of 139 us a tile).
-  struct Extra { uint2 h, l; uint4 w; };
-  auto at = [&](int i, int j, int& orow, int& ocol) {  // of LAST's output: first of this lane's four columns
-    const int row = row0 + 16 * i, col = col0 + 16 * j;
-    orow = flip ? col + 4 * g + (r & 3) : row + r;
-    ocol = flip ? row + (r & 12) : col + 4 * g;
+  // The epilogue takes two neighbouring blocks at a time and swaps halves between their lanes, so that a lane holds 8
+  // consecutive columns of one of them (g even: the left, g odd: the right) and moves 16 bytes at a time.
+  // What it reads, D and the weight that LAST updates (as it is stored), is loaded DEPTH pairs ahead of the stores: taken
+  // one by one behind them, each cost its latency (22 x 1408 x 1408, POLY: 34 of 139 us a tile).
+  constexpr int PAIRS = MB * NB / 2, DEPTH = KG > 1 ? 1 : PAIRS < 4 ? PAIRS : 4;
+  struct Extra { uint4 h, l, w[2]; };
+  struct Spot { int rb, cb, row, col; };  // the lane's block, and its row and first column
+  auto spot = [&](int p) {
+    const int rb = row0 + 16 * (p / (NB / 2)), cb = col0 + 32 * (p % (NB / 2)) + 16 * (g & 1);
+    return Spot{rb, cb, rb + r, cb + 4 * (g & 2)};
   };
-  auto fetch = [&](int i, int j, Extra& x) {
-    const int rb = row0 + 16 * i, cb = col0 + 16 * j, row = rb + r, col = cb + 4 * g;
-    if (MODE == GRAM || rb >= G.mp || cb >= lim || (SYM && cb < rb)) return;
-    const uint16_t* d = (MODE == POLY ? Am + row * la : X + row * lx) + hi_at(col);
-    x.h = *reinterpret_cast<const uint2*>(d);
-    x.l = *reinterpret_cast<const uint2*>(d + 32);
+  auto outside = [&](const Spot& s) { return s.rb >= G.mp || s.cb >= lim || (SYM && s.cb < s.rb); };
+  auto at = [&](const Spot& s, int q, int& orow, int& ocol) {  // of LAST's output: first of this lane's q-th four columns
+    orow = flip ? s.col + 4 * q + (r & 3) : s.row;
+    ocol = flip ? s.rb + (r & 12) : s.col + 4 * q;
+  };
+  auto fetch = [&](int p, Extra& x) {
+    const Spot s = spot(p);
+    if (MODE == GRAM || outside(s)) return;
+    const uint16_t* d = (MODE == POLY ? Am + s.row * la : X + s.row * lx) + hi_at(s.col);
+    x.h = *reinterpret_cast<const uint4*>(d);
+    x.l = *reinterpret_cast<const uint4*>(d + 32);
     if constexpr (MODE == LAST) {
-      int orow, ocol;
-      at(i, j, orow, ocol);
-      if (!a.update || !vec || orow >= G.rows || ocol >= G.cols) return;
-      const int64_t o = (int64_t)orow * G.cols + ocol;
-      if (G.w_dtype == LLATTN_F32) {
-        x.w = *reinterpret_cast<const uint4*>(static_cast<const float*>(w_ptr) + o);
-      } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(w_ptr) + o);
-        x.w = make_uint4(v.x << 16, v.x & 0xffff0000u, v.y << 16, v.y & 0xffff0000u);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        int orow, ocol;
+        at(s, q, orow, ocol);
+        if (!a.update || !vec || orow >= G.rows || ocol >= G.cols) continue;
+        const int64_t o = (int64_t)orow * G.cols + ocol;
+        if (G.w_dtype == LLATTN_F32) {
+          x.w[q] = *reinterpret_cast<const uint4*>(static_cast<const float*>(w_ptr) + o);
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(w_ptr) + o);
+          x.w[q].x = v.x;
+          x.w[q].y = v.y;
+        }
       }
     }
   };
-  auto store = [&](int i, int j, const f32x4& c, const Extra& xt) {
-    const int rb = row0 + 16 * i, cb = col0 + 16 * j, row = rb + r, col = cb + 4 * g;
-    if (rb >= G.mp || cb >= lim || (SYM && cb < rb)) return;
-    float x[4] = {G.beta * c[0], G.beta * c[1], G.beta * c[2], G.beta * c[3]};
-    if constexpr (MODE != GRAM) {
-      const f16x4 h = __builtin_bit_cast(f16x4, xt.h), l = __builtin_bit_cast(f16x4, xt.l);
+  // pair p, its sums in left and right; then(): once x is read
+  auto finish = [&](int p, const f32x4& left, const f32x4& right, const Extra& xt, auto then) {
+    const Spot s = spot(p);
+    float x[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = fmaf(G.alpha, (float)h[e] + (float)l[e], x[e]);
+    for (int e = 0; e < 4; ++e) {
+      const auto v = __builtin_amdgcn_permlane16_swap(__float_as_uint(left[e]), __float_as_uint(right[e]), false, false);
+      x[e] = G.beta * __uint_as_float(v[0]);
+      x[4 + e] = G.beta * __uint_as_float(v[1]);
     }
+    if constexpr (MODE != GRAM) {
+      const f16x8 h = __builtin_bit_cast(f16x8, xt.h), l = __builtin_bit_cast(f16x8, xt.l);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = fmaf(G.alpha, (float)h[e] + (float)l[e], x[e]);
+    }
+    const uint4 w0 = xt.w[0], w1 = xt.w[1];
+    then();
+    if (outside(s)) return;
     if constexpr (MODE == APPLY) {
-      store_halves4(a.y + G.x_off + (mat * G.mp + row) * lx, col, x);
+      store_halves8(a.y + G.x_off + (mat * G.mp + s.row) * lx, s.col, x);
     } else if constexpr (SYM) {
       uint16_t* C = MODE == GRAM ? Am : Bm;
-      store_halves4(C + row * la, col, x);
-      if (cb > rb) {  // and below the diagonal: this lane's column 4 g + r % 4, rows 4 (r / 4) ..
-        quad_transpose(x, lane);
-        store_halves4(C + (col + (r & 3)) * la, rb + (r & 12), x);
-      }
-    } else {
-      int orow, ocol;
-      at(i, j, orow, ocol);
-      if (flip) quad_transpose(x, lane);
-      const int n = min(4, G.cols - ocol);
-      if (orow >= G.rows || n <= 0) return;
-      const int64_t o = (int64_t)orow * G.cols + ocol;
-      if (a.update) {
-        float c4[4] = {__uint_as_float(xt.w.x), __uint_as_float(xt.w.y), __uint_as_float(xt.w.z), __uint_as_float(xt.w.w)};
+      store_halves8(C + s.row * la, s.col, x);
+      if (s.cb > s.rb) {  // and below the diagonal: this lane's columns col + 4 q + r % 4, rows 4 (r / 4) ..
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (!vec) c4[e] = e < n ? load_as(w_ptr, o + e, G.w_dtype) : 0.f;
-          x[e] = fmaf(-G.step, x[e], G.keep * c4[e]);
+        for (int q = 0; q < 2; ++q) {
+          quad_transpose(x + 4 * q, lane);
+          store_halves4(C + (s.col + 4 * q + (r & 3)) * la, s.rb + (r & 12), x + 4 * q);
         }
       }
-      const bool f32 = G.w_dtype == LLATTN_F32;
-      if (vec) {
-        if (f32) store4<float>(static_cast<float*>(out) + o, x);
-        else store4<uint16_t>(static_cast<uint16_t*>(out) + o, x);
-      } else {
+    } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (e >= n) continue;
-          if (f32) static_cast<float*>(out)[o + e] = x[e];
-          else static_cast<uint16_t*>(out)[o + e] = f2bf(x[e]);
+      for (int q = 0; q < 2; ++q) {
+        float* y = x + 4 * q;
+        int orow, ocol;
+        at(s, q, orow, ocol);
+        if (flip) quad_transpose(y, lane);
+        const int n = min(4, G.cols - ocol);
+        if (orow >= G.rows || n <= 0) continue;
+        const int64_t o = (int64_t)orow * G.cols + ocol;
+        const bool f32 = G.w_dtype == LLATTN_F32;
+        if (a.update) {
+          uint4 u = q ? w1 : w0;
+          if (!f32) u = make_uint4(u.x << 16, u.x & 0xffff0000u, u.y << 16, u.y & 0xffff0000u);
+          float c4[4] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w)};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (!vec) c4[e] = e < n ? load_as(w_ptr, o + e, G.w_dtype) : 0.f;
+            y[e] = fmaf(-G.step, y[e], G.keep * c4[e]);
+          }
+        }
+        if (vec) {
+          if (f32) store4<float>(static_cast<float*>(out) + o, y);
+          else store4<uint16_t>(static_cast<uint16_t*>(out) + o, y);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (e >= n) continue;
+            if (f32) static_cast<float*>(out)[o + e] = y[e];
+            else static_cast<uint16_t*>(out)[o + e] = f2bf(y[e]);
+          }
         }
       }
     }
   };
+  Extra xt[DEPTH];
   if constexpr (KG == 1) {
-    Extra xt[2][NB];
-    auto fetch_row = [&](int i) {
 #pragma unroll
-      for (int j = 0; j < NB; ++j) fetch(i, j, xt[i & 1][j]);
-    };
-    fetch_row(0);
+    for (int p = 0; p < DEPTH; ++p) fetch(p, xt[p]);
 #pragma unroll
-    for (int i = 0; i < MB; ++i) {
-      if (i + 1 < MB) fetch_row(i + 1);
-#pragma unroll
-      for (int j = 0; j < NB; ++j) store(i, j, acc[i][j], xt[i & 1][j]);
+    for (int p = 0; p < PAIRS; ++p) {
+      const int i = p / (NB / 2), j = 2 * (p % (NB / 2));
+      finish(p, acc[i][j], acc[i][j + 1], xt[p % DEPTH], [&]() {
+        if (p + DEPTH < PAIRS) fetch(p + DEPTH, xt[p % DEPTH]);
+      });
     }
   } else {
     static_assert(KG * W * MB * NB * 1024 <= KG * NST * STAGE, "the groups' sums fit their stages");
@@ -600,14 +640,18 @@ __device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*
     for (int u = 0; u < MB * NB; ++u) sum[(wave * MB * NB + u) * 64 + lane] = acc[u / NB][u % NB];
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < MB * NB; ++u) {  // blocks are shared out among the groups
-      if (u % KG != kg) continue;
-      Extra xt;
-      fetch(u / NB, u % NB, xt);
-      f32x4 c = sum[(w * MB * NB + u) * 64 + lane];
+    for (int p = 0; p < PAIRS; ++p) {  // pairs are shared out among the groups
+      if (p % KG != kg) continue;
+      fetch(p, xt[0]);
+      f32x4 c[2];
 #pragma unroll
-      for (int k = 1; k < KG; ++k) c += sum[((k * W + w) * MB * NB + u) * 64 + lane];
-      store(u / NB, u % NB, c, xt);
+      for (int k = 0; k < KG; ++k)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const f32x4 v = sum[((k * W + w) * MB * NB + 2 * p + u) * 64 + lane];
+          c[u] = k ? c[u] + v : v;
+        }
+      finish(p, c[0], c[1], xt[0], []() {});
     }
   }
 }
