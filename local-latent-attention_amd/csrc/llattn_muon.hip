@@ -148,25 +148,24 @@ __device__ __forceinline__ float h_val(uint16_t v) { return static_cast<float>(_
 // position of column c within a row
 __device__ __forceinline__ int hi_at(int c) { return (c >> 5) * 64 + (c & 31); }
 
+// two values' hi and lo halves
+__device__ __forceinline__ void halves2(float v0, float v1, uint32_t& h, uint32_t& l) {
+  const uint16_t h0 = h_bits(v0), h1 = h_bits(v1);
+  h = h0 | (uint32_t)h1 << 16;
+  l = h_bits(v0 - h_val(h0)) | (uint32_t)h_bits(v1 - h_val(h1)) << 16;
+}
 __device__ __forceinline__ void store_halves4(uint16_t* row, int c, const float v[4]) {
-  uint16_t h[4], l[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    h[e] = h_bits(v[e]);
-    l[e] = h_bits(v[e] - h_val(h[e]));
-  }
+  uint2 h, l;
+  halves2(v[0], v[1], h.x, l.x);
+  halves2(v[2], v[3], h.y, l.y);
   uint16_t* p = row + hi_at(c);
-  *reinterpret_cast<uint2*>(p) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
-  *reinterpret_cast<uint2*>(p + 32) = make_uint2(l[0] | (uint32_t)l[1] << 16, l[2] | (uint32_t)l[3] << 16);
+  *reinterpret_cast<uint2*>(p) = h;
+  *reinterpret_cast<uint2*>(p + 32) = l;
 }
 __device__ __forceinline__ void store_halves8(uint16_t* row, int c, const float v[8]) {
   uint32_t h[4], l[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint16_t h0 = h_bits(v[2 * e]), h1 = h_bits(v[2 * e + 1]);
-    h[e] = h0 | (uint32_t)h1 << 16;
-    l[e] = h_bits(v[2 * e] - h_val(h0)) | (uint32_t)h_bits(v[2 * e + 1] - h_val(h1)) << 16;
-  }
+  for (int e = 0; e < 4; ++e) halves2(v[2 * e], v[2 * e + 1], h[e], l[e]);
   uint16_t* p = row + hi_at(c);
   st16(p, make_uint4(h[0], h[1], h[2], h[3]));
   st16(p + 32, make_uint4(l[0], l[1], l[2], l[3]));
@@ -321,6 +320,15 @@ __device__ __forceinline__ void quad_transpose(float v[4], int lane) {
     if (b1) v[e] = t;
     else v[e + 2] = t;
   }
+}
+
+// Lanes r and r ^ 4 of each eight: those with bit 2 set give x and receive y, the others give y and receive x.
+__device__ __forceinline__ void swap4(uint32_t& x, uint32_t& y, int lane) {
+  const bool odd = lane & 4;
+  const int t = __builtin_amdgcn_update_dpp(0, (int)(odd ? x : y), 0x141, 0xf, 0xf, true);        // lane 7 - r of the eight
+  const uint32_t u = (uint32_t)__builtin_amdgcn_update_dpp(0, t, 0x1B, 0xf, 0xf, true);           // and 3 - r of the four
+  if (odd) x = u;
+  else y = u;
 }
 
 // A shape of workgroup: KG groups of WR x WC waves, each wave 16 MB x 16 NB of the tile, NST LDS stages of 32 k a group.
@@ -523,8 +531,11 @@ __device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*
   constexpr int PAIRS = MB * NB / 2, DEPTH = KG > 1 ? 1 : PAIRS < 4 ? PAIRS : 4;
   struct Extra { uint4 h, l, w[2]; };
   struct Spot { int rb, cb, row, col; };  // the lane's block, and its row and first column
+  // Pairs run down two rows of blocks before the next columns, where one group of waves has both.
+  auto block_row = [](int p) { return KG > 1 ? p / (NB / 2) : 2 * (p / NB) + (p & 1); };
+  auto block_col = [](int p) { return 2 * (KG > 1 ? p % (NB / 2) : (p / 2) % (NB / 2)); };
   auto spot = [&](int p) {
-    const int rb = row0 + 16 * (p / (NB / 2)), cb = col0 + 32 * (p % (NB / 2)) + 16 * (g & 1);
+    const int rb = row0 + 16 * block_row(p), cb = col0 + 16 * block_col(p) + 16 * (g & 1);
     return Spot{rb, cb, rb + r, cb + 4 * (g & 2)};
   };
   auto outside = [&](const Spot& s) { return s.rb >= G.mp || s.cb >= lim || (SYM && s.cb < s.rb); };
@@ -555,6 +566,7 @@ __device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*
       }
     }
   };
+  uint2 below_h[2][2], below_l[2][2];  // two rows of blocks' halves for below the diagonal
   // pair p, its sums in left and right; then(): once x is read
   auto finish = [&](int p, const f32x4& left, const f32x4& right, const Extra& xt, auto then) {
     const Spot s = spot(p);
@@ -578,11 +590,18 @@ __device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*
     } else if constexpr (SYM) {
       uint16_t* C = MODE == GRAM ? Am : Bm;
       store_halves8(C + s.row * la, s.col, x);
-      if (s.cb > s.rb) {  // and below the diagonal: this lane's columns col + 4 q + r % 4, rows 4 (r / 4) ..
+      if (s.cb <= s.rb) return;
+      // and below the diagonal: this lane's columns col + 4 q + r % 4, rows 4 (r / 4) ..
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          quad_transpose(x + 4 * q, lane);
-          store_halves4(C + (s.col + 4 * q + (r & 3)) * la, s.rb + (r & 12), x + 4 * q);
+      for (int q = 0; q < 2; ++q) {
+        float* y = x + 4 * q;
+        quad_transpose(y, lane);
+        uint16_t* c = C + (s.col + 4 * q + (r & 3)) * la;
+        if constexpr (KG > 1) {
+          store_halves4(c, s.rb + (r & 12), y);
+        } else {
+          halves2(y[0], y[1], below_h[p & 1][q].x, below_l[p & 1][q].x);
+          halves2(y[2], y[3], below_h[p & 1][q].y, below_l[p & 1][q].y);
         }
       }
     } else {
@@ -626,10 +645,29 @@ __device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*
     for (int p = 0; p < DEPTH; ++p) fetch(p, xt[p]);
 #pragma unroll
     for (int p = 0; p < PAIRS; ++p) {
-      const int i = p / (NB / 2), j = 2 * (p % (NB / 2));
+      const int i = block_row(p), j = block_col(p);
       finish(p, acc[i][j], acc[i][j + 1], xt[p % DEPTH], [&]() {
         if (p + DEPTH < PAIRS) fetch(p + DEPTH, xt[p % DEPTH]);
       });
+      if constexpr (SYM) {
+        // Both blocks' halves for below the diagonal: lanes of r / 4 even take 8 rows of the upper one, the odd of the lower.
+        const Spot s = spot(p - 1);
+        if (p % 2 == 0 || outside(s) || s.cb <= s.rb) continue;
+        uint16_t* C = MODE == GRAM ? Am : Bm;
+        const int rb = s.rb + 4 * (r & 4);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint2 *h0 = &below_h[0][q], *h1 = &below_h[1][q], *l0 = &below_l[0][q], *l1 = &below_l[1][q];
+          swap4(h0->x, h1->x, lane);
+          swap4(h0->y, h1->y, lane);
+          swap4(l0->x, l1->x, lane);
+          swap4(l0->y, l1->y, lane);
+          uint16_t* c = C + (s.col + 4 * q + (r & 3)) * la + hi_at(rb + (r & 8));
+          if (s.cb <= rb) continue;
+          st16(c, make_uint4(h0->x, h0->y, h1->x, h1->y));
+          st16(c + 32, make_uint4(l0->x, l0->y, l1->x, l1->y));
+        }
+      }
     }
   } else {
     static_assert(KG * W * MB * NB * 1024 <= KG * NST * STAGE, "the groups' sums fit their stages");
@@ -648,7 +686,7 @@ __device__ __forceinline__ void ns_tile(const NsArgs& a, const Table<const void*
       for (int k = 0; k < KG; ++k)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const f32x4 v = sum[((k * W + w) * MB * NB + 2 * p + u) * 64 + lane];
+          const f32x4 v = sum[((k * W + w) * MB * NB + block_row(p) * NB + block_col(p) + u) * 64 + lane];
           c[u] = k ? c[u] + v : v;
         }
       finish(p, c[0], c[1], xt[0], []() {});
