@@ -322,32 +322,59 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
     if (more) read_rows(next);
 
     if constexpr (EPI == SUM || EPI == OUT_BF16 || EPI == OUT_F32) {
-      float alpha = 1.f;
-      if (EPI != SUM && !a.per_row) alpha = *a.grad * (a.inv ? *a.inv : 1.f);
+      if constexpr (EPI == SUM) {
+        // What is added to is read a row of blocks ahead of the stores (read one by one behind them: 34 us a tile).
+        float* const c = static_cast<float*>(a.C) + (int64_t)tile.split * a.M * a.N;
+        const auto at = [&](int i, int j, int64_t& o) {
+          const int row = row0 + 16 * i + r, col = col0 + 16 * j + 4 * g;
+          o = (int64_t)row * a.N + col;
+          return row < a.M && col < a.N;
+        };
+        f32x4 before[2][NB];
+        auto fetch = [&](int i) {
 #pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        const int row = row0 + 16 * i + r;
-        if (row >= a.M) continue;
+          for (int j = 0; j < NB; ++j) {
+            int64_t o;
+            before[i & 1][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (at(i, j, o) && a.accumulate) before[i & 1][j] = *reinterpret_cast<const f32x4*>(c + o);
+          }
+        };
+        fetch(0);
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          const int col = col0 + 16 * j + 4 * g;
-          if (col >= a.N) continue;
-          const int64_t o = ((int64_t)(EPI == SUM ? tile.split : 0) * a.M + row) * a.N + col;
-          float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-          if constexpr (EPI == SUM) {
-            float* c = static_cast<float*>(a.C) + o;
-            if (a.accumulate) {
-              float x[4];
-              load4<float>(c, x);
+        for (int i = 0; i < MB; ++i) {
+          if (i + 1 < MB) fetch(i + 1);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] += x[e];
+          for (int j = 0; j < NB; ++j) {
+            int64_t o;
+            if (at(i, j, o)) *reinterpret_cast<f32x4*>(c + o) = acc[i][j] + before[i & 1][j];
+          }
+        }
+      } else {
+        const float alpha = a.per_row ? 1.f : *a.grad * (a.inv ? *a.inv : 1.f);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          const int row = row0 + 16 * i + r;
+#pragma unroll
+          for (int j = 0; j < NB; j += 2) {
+            f32x4 u = acc[i][j] * alpha, v = acc[i][j + 1] * alpha;
+            if constexpr (EPI == OUT_F32) {
+              const int col = col0 + 16 * j + 4 * g;
+              float* c = static_cast<float*>(a.C) + (int64_t)row * a.N + col;
+              if (row < a.M && col < a.N) *reinterpret_cast<f32x4*>(c) = u;
+              if (row < a.M && col + 16 < a.N) *reinterpret_cast<f32x4*>(c + 16) = v;
+            } else {
+              // Neighbouring blocks swap halves between their lanes: 8 consecutive columns of one of them each, 16 bytes.
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(u[e]), __float_as_uint(v[e]), false, false);
+                u[e] = __uint_as_float(x[0]);
+                v[e] = __uint_as_float(x[1]);
+              }
+              const int col = col0 + 16 * (j + (g & 1)) + 4 * (g & 2);
+              if (row < a.M && col < a.N)
+                st16(static_cast<uint16_t*>(a.C) + (int64_t)row * a.N + col,
+                     make_uint4(pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])));
             }
-            store4<float>(c, v);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= alpha;
-            if constexpr (EPI == OUT_F32) store4<float>(static_cast<float*>(a.C) + o, v);
-            else store4<uint16_t>(static_cast<uint16_t*>(a.C) + o, v);
           }
         }
       }
