@@ -16,7 +16,7 @@ extern "C" {
 /* ---- softmax cross entropy of h W^T, no logits kept ------------------------
  * l[n][v] = sum_d h[n][d] W[v][d] in fp32 from bf16 h [rows][D], W [V][D] (row
  * strides ldh, ldw in elements, multiples of 8; bases 16-byte aligned; D a
- * multiple of 8, any V and rows).
+ * multiple of 8, any V, below 2^23 rows).
  *
  * Forward: loss[n] = logsumexp_v l[n] - l[n][t_n] (0 where t_n ==
  * ignore_index, NaN where t_n lies outside [0, V) otherwise), lse2[n] =

@@ -45,7 +45,7 @@ struct HeadArgs {
   int32_t* part_i;
   float* tgt;
   const float* lse2;        // GRAD
-  uint16_t* p; int64_t ldp;
+  uint16_t* p; int64_t p_block; int p_cols;  // q, its columns and the elements of 64 of them
   // gradients: alpha = grad[0] * (inv ? *inv : 1), or grad[row] within q (per_row)
   const float* grad;
   const float* inv;
@@ -132,6 +132,23 @@ struct ColOp {
   }
 };
 
+// The same for q: 64 k-rows of T columns, whose blocks of 64 lie ld elements apart, a row of one in 128 bytes.
+template <int T, int W>
+struct BlockOp : ColOp<T, W> {
+  using ColOp<T, W>::LOADS, ColOp<T, W>::PER, ColOp<T, W>::off;
+  int k_of[LOADS];
+  __device__ __forceinline__ void init(int64_t ld, int w, int lane, int o0) {
+    ColOp<T, W>::init(0, w, lane, o0);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int q = (w * LOADS + i) * 64 + lane, k = q / PER, c = (q % PER) ^ this->swz(k);
+      off[i] = (uint32_t)((c >> 3) * ld * 2 + k * 128 + 16 * (c & 7));
+      k_of[i] = k;
+    }
+  }
+  __device__ __forceinline__ uint32_t at(int i, int left) const { return kmask(off[i], k_of[i], left); }
+};
+
 // One tile of a product.  A 64-k step is two rounds of products, each beside the fragment reads of the next: k 0..31
 // (reads k 32..63), a barrier, k 32..63 (reads the next step's k 0..31 and issues the loads of step kt + NST into the
 // stage just read).  Waves whose part of the tile lies outside load and wait like the others and do nothing else.
@@ -139,7 +156,8 @@ struct ColOp {
 template <int EPI, bool AT, bool BT, typename S, int WGS>
 __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const HeadArgs a) {
   constexpr int MB = S::MB, NB = S::NB, TM = S::TM, TN = S::TN, NST = S::NST, STAGE = S::STAGE, W = S::W;
-  typedef std::conditional_t<AT, ColOp<TM, W>, RowOp<TM, W, false>> OpA;
+  constexpr bool LOSS = EPI == STATS || EPI == STATS_PRED || EPI == GRAD;  // else A is q, in blocks of 64 columns
+  typedef std::conditional_t<AT, BlockOp<TM, W>, RowOp<TM, W, false>> OpA;
   typedef std::conditional_t<BT, ColOp<TN, W>, RowOp<TN, W, true>> OpB;
   constexpr int LOADS = OpA::LOADS + OpB::LOADS;
   static_assert(LOADS <= MB + NB, "the second round's reads carry the loads");
@@ -165,7 +183,7 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
   };
   OpA oa;
   OpB ob;
-  oa.init(a.lda, w, lane, wm * 16 * MB);
+  oa.init(LOSS || AT ? a.lda : 64, w, lane, wm * 16 * MB);
   ob.init(a.ldb, w, lane, wn * 16 * NB);
   auto source = [&](const uint16_t* p, int64_t ld, bool t, int o, int n, int k0) {  // n of the operand's rows (t: columns) from o on
     StepSrc s;
@@ -175,7 +193,17 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
     s.inc = t ? (uint32_t)(128 * ld) : 128u;
     return s;
   };
-  auto source_a = [&](const Tile& t) { return source(a.A, a.lda, AT, t.m0, min(TM, a.M - t.m0), t.split * a.per); };
+  auto source_a = [&](const Tile& t) {
+    const int n = min(TM, a.M - t.m0), k0 = t.split * a.per;
+    if constexpr (LOSS) return source(a.A, a.lda, false, t.m0, n, k0);
+    StepSrc s;
+    s.addr = reinterpret_cast<uint64_t>(a.A + (AT ? t.m0 / 64 : k0) * a.lda + (AT ? (int64_t)k0 * 64 : t.m0) * 64);
+    const uint32_t blocks = AT ? (uint32_t)((n - 1) / 64 * a.lda * 2) : 0;  // up to the last block's
+    s.full = blocks + (AT ? 64 : n) * 128;
+    s.tail = AT && a.K & 63 ? blocks + (a.K & 63) * 128 : s.full;
+    s.inc = AT ? 64 * 128 : (uint32_t)(a.lda * 2);
+    return s;
+  };
   auto source_b = [&](const Tile& t) { return source(a.B, a.ldb, BT, t.n0, min(TN, a.N - t.n0), t.split * a.per); };
   auto k_of = [&](const Tile& t) { return min(a.K - t.split * a.per * 64, t.steps * 64); };
   int v = blockIdx.x;
@@ -212,7 +240,6 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
     });
   };
   // What the epilogue of a tile reads of the wave's rows, a row a lane: read ahead of it, it costs no latency there.
-  constexpr bool LOSS = EPI == STATS || EPI == STATS_PRED || EPI == GRAD;
   int64_t read_tg = a.ignore_index;
   float read_l2 = 0.f;
   auto read_rows = [&](const Tile& t) {
@@ -412,14 +439,13 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[i][j][e] = column(j) + e < a.N ? acc[i][j][e] : 0.f;
           }
-          uint16_t* out = a.p + (int64_t)row * a.ldp;
 #pragma unroll
           for (int j = 0; j < NB; j += 2) {
             const int c = column(j);
             const f32x4 u = acc[i][j], v = acc[i][j + 1];
             uint4 q = make_uint4(pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
             if (tc == -2) q = make_uint4(0, 0, 0, 0);
-            if (live && c < a.ldp) st16(out + c, q);  // 16 rows x 64 bytes a store (64 rows of 8 bytes took a tenth longer)
+            if (live && c < a.p_cols) st16(a.p + (c >> 6) * a.p_block + (int64_t)row * 64 + (c & 63), q);  // 16 rows x 64 bytes a store
           }
         } else {
           float m = kNegInf;
@@ -644,9 +670,9 @@ Tiling tiling(int64_t M, int64_t N, int steps, int most) {
 
 int32_t check(const llattn_head_cfg* c) {
   if (!c) return fail(LLATTN_ERR_SHAPE, "llattn_head: null configuration");
-  if (c->rows <= 0 || c->V <= 0 || c->D <= 0 || c->D % 8 || c->V > 0x7fffff00)
-    return fail(LLATTN_ERR_SHAPE, "llattn_head: rows %d, V %d, D %d: must be positive, D a multiple of 8", c->rows, c->V,
-                c->D);
+  if (c->rows <= 0 || c->rows >= (1 << 23) || c->V <= 0 || c->D <= 0 || c->D % 8 || c->V > 0x7fffff00)
+    return fail(LLATTN_ERR_SHAPE, "llattn_head: rows %d, V %d, D %d: must be positive, rows below 2^23, D a multiple of 8",
+                c->rows, c->V, c->D);
   if (c->piece < 0 || c->piece % 256)
     return fail(LLATTN_ERR_SHAPE, "llattn_head: piece %d must be 0 or a multiple of 256", c->piece);
   if (c->dw_dtype != LLATTN_F32 && c->dw_dtype != LLATTN_BF16)
@@ -677,7 +703,7 @@ int piece_of(const llattn_head_cfg* c) {
 
 // q of a piece [rows][piece], the sums of dh over pieces and splits, the partial sums of dW
 struct BwdPlan {
-  int piece, pieces, ldp;
+  int piece, pieces;
   Tiling logits, dh, dw;
   size_t p, dh_part, dw_part;
   bool dh_direct() const { return pieces == 1 && dh.splits == 1; }
@@ -691,10 +717,7 @@ BwdPlan bwd_plan(const llattn_head_cfg* c) {
   b.logits = tiling(c->rows, nv, (c->D + 63) / 64, 1);
   b.dh = tiling(c->rows, c->D, (nv + 63) / 64, 16);
   b.dw = tiling(nv, c->D, (c->rows + 63) / 64, 16);
-  // rows a cache line apart from the next power of two: at 64 KB the 256 rows of a tile shared memory channels (8192 rows,
-  // pieces of 32768: q 1039 us, dh 826; so 823 and 771)
-  b.ldp = b.piece + 64;
-  b.p = up((size_t)c->rows * b.ldp * 2);
+  b.p = up((size_t)c->rows * b.piece * 2);
   b.dh_part = b.dh_direct() ? 0 : up((size_t)b.dh.splits * c->rows * c->D * 4);
   b.dw_part = b.dw.splits > 1 ? up((size_t)b.dw.splits * ((nv + 7) / 8 * 8) * c->D * 4) : 0;
   return b;
@@ -810,7 +833,7 @@ extern "C" int32_t llattn_head_bwd(const llattn_head_cfg* c, const void* h, int6
   float* dh_part = reinterpret_cast<float*>(ws + b.p);
   float* dw_part = reinterpret_cast<float*>(ws + b.p + b.dh_part);
   HeadArgs a{};
-  a.p = reinterpret_cast<uint16_t*>(ws); a.ldp = b.ldp;
+  a.p = reinterpret_cast<uint16_t*>(ws); a.p_block = (int64_t)c->rows * 64; a.p_cols = b.piece;
   a.targets = targets; a.ignore_index = ignore_index;
   a.lse2 = lse2; a.grad = grad; a.per_row = grad_stride; a.inv = inv;
   const int64_t dw_size = c->dw_dtype == LLATTN_F32 ? 4 : 2;
@@ -819,7 +842,7 @@ extern "C" int32_t llattn_head_bwd(const llattn_head_cfg* c, const void* h, int6
     logits_of(a, c, h, ldh, W, ldw, v0, cols);
     launch<GRAD, false, false>(a, b.logits.kind, 1, st);
     HeadArgs d = a;
-    d.A = a.p; d.lda = a.ldp;
+    d.A = a.p; d.lda = a.p_block;
     d.N = c->D;
     if (dh) {  // q W: q's chunk that reaches past the piece's columns holds zeros there, W's rows past them read zero
       d.M = c->rows; d.K = cols;

@@ -67,7 +67,7 @@ def _head_fwd(rows=4, V=10, D=8, h=1 << 20, ldh=8, w=1 << 20, ldw=8, t=1 << 20, 
     (dict(h=0), L.ERR_LAYOUT), (dict(w=0), L.ERR_LAYOUT), (dict(t=0), L.ERR_LAYOUT), (dict(loss=0), L.ERR_LAYOUT),
     (dict(lse=0), L.ERR_LAYOUT), (dict(inv=1 << 20), L.ERR_LAYOUT), (dict(ldh=4), L.ERR_LAYOUT), (dict(ldw=12), L.ERR_LAYOUT),
     (dict(h=(1 << 20) + 2), L.ERR_LAYOUT), (dict(ldw=1 << 23), L.ERR_LAYOUT), (dict(ws=0), L.ERR_WORKSPACE), (dict(n=1), L.ERR_WORKSPACE),
-    (dict(D=9), L.ERR_SHAPE)])
+    (dict(D=9), L.ERR_SHAPE), (dict(rows=1 << 23), L.ERR_SHAPE)])
 def test_head_forward_refused(kw, code):
     assert _head_fwd(**kw) == code
 
