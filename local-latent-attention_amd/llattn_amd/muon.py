@@ -251,14 +251,14 @@ def _muon_group(group, state) -> None:
 
 class MuonAdamW(torch.optim.Optimizer):
     """Muon for ``matrices``, AdamW for the other parameter groups, as one optimiser: one list of groups, one state.
-    The matrices are the first group."""
+    The matrices are the first group; groups added later are AdamW's."""
 
     def __init__(self, matrices, others, muon: dict | None = None, **adamw) -> None:
         matrices, others = list(matrices), list(others)
         self._muon = Muon(matrices, **(muon or {}))
         self._adamw = torch.optim.AdamW(others, **adamw)
         groups = [dict(g) for g in self._muon.param_groups + self._adamw.param_groups]
-        super().__init__(groups, {})
+        super().__init__(groups, dict(self._adamw.defaults))
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -229,7 +229,7 @@ def piecewise_head_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Te
     gradients), ``"sum"``, or ``"none"`` (fp32, ``targets``' shape, 0 in ignored rows).  A target outside ``[0, V)``
     gives NaN.  With ``return_pred`` also the first argmax of every row (int32).  ``h`` and ``weight`` are bf16 or fp32,
     fp32 ones rounded to bf16 as under autocast; logits, sums and losses are fp32 and gradients come in their input's
-    type, ``weight``'s accumulated in fp32.  Differentiable once.  GPU only."""
+    type, ``weight``'s accumulated in fp32.  Fewer than 2^23 rows.  Differentiable once.  GPU only."""
     if h.dim() < 1 or weight.dim() != 2 or weight.shape[1] != h.shape[-1] or 0 in weight.shape:
         raise ValueError(f"piecewise_head_loss: weight {tuple(weight.shape)} does not match hidden states {tuple(h.shape)}")
     if targets.shape != h.shape[:-1]:

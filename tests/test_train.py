@@ -191,3 +191,16 @@ def test_optimisers_refuse_vectors_and_unknown_choices():
     assert len(names) == 2 * 7 and not any("embedding" in n or "position" in n or "gate" in n for n in names)
     assert sum(len(g["params"]) for g in opt.param_groups) == len(list(model.parameters()))
     assert isinstance(make_optimizer(model), torch.optim.AdamW)
+
+
+def test_groups_added_to_the_joint_optimiser_are_adamws():
+    w, b, e = (torch.nn.Parameter(torch.zeros(s)) for s in ((4, 8), (4,), (3, 4)))
+    opt = muon.MuonAdamW([w], [b], dict(lr=0.1), lr=1e-3, betas=(0.9, 0.95))
+    opt.add_param_group({"params": [e], "weight_decay": 0.0})
+    b.grad, e.grad = torch.ones(4), torch.ones(3, 4)
+    opt.step()
+    assert not w.detach().any()
+    assert torch.allclose(e.detach(), torch.full((3, 4), -1e-3)) and torch.allclose(b.detach(), torch.full((4,), -1e-3))
+    again = muon.MuonAdamW([w], [{"params": [b]}, {"params": [e], "weight_decay": 0.0}], dict(lr=0.1), lr=1e-3)
+    again.load_state_dict(opt.state_dict())
+    assert again.param_groups[2]["betas"] == (0.9, 0.95) and again.param_groups[0]["momentum"] == 0.95
