@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 from numbers import Real
 
 import torch
@@ -40,7 +41,8 @@ def _bytes(cfg, groups) -> int:
 
 
 def _pointers(values):
-    return (ctypes.c_void_p * len(values))(*values)
+    """An array of pointers from data pointers (by way of an array of numbers, a tenth of ctypes' own time)."""
+    return (ctypes.c_void_p * len(values)).from_buffer(array("Q", [v or 0 for v in values]))
 
 
 def _padded(shape) -> int:
@@ -129,39 +131,60 @@ def _update_scale(scale: str, rows: int, cols: int) -> float:
 
 
 def _rows(weights, grads, momenta, out):
-    """The checked matrices as rows of tensors and data pointers: (w, g, m, w_out, m_out, pointers of w, m, w_out, m_out, g),
-    gradients contiguous."""
+    """The checked matrices by device and kind (shape, weight's type, gradient's type), each as data pointers (g, m, w, m_out,
+    w_out); and what has to live until the launch."""
     lists = [weights, grads, momenta, *out]
     if len({len(v) for v in lists}) != 1:
         raise ValueError(f"muon_update: lists of different lengths ({', '.join(str(len(v)) for v in lists)})")
     f32, types = torch.float32, (torch.float32, torch.bfloat16)
-    rows = []
+    devices, kept, inputs, new = {}, [], [], []
     for w, g, m, wo, mo in zip(*lists):
-        shape, dev = w.shape, w.get_device()
+        shape, dev, w_dtype, g_dtype = w.shape, w.get_device(), w.dtype, g.dtype
         if len(shape) != 2 or 0 in shape:
             raise ValueError(f"muon_update: weights must be non-empty matrices, got shape {tuple(shape)}")
-        if w.dtype not in types or g.dtype not in types:
-            raise ValueError(f"muon_update: weights and gradients must be fp32 or bf16, got {w.dtype} and {g.dtype}")
+        if w_dtype not in types or g_dtype not in types:
+            raise ValueError(f"muon_update: weights and gradients must be fp32 or bf16, got {w_dtype} and {g_dtype}")
         same = g.shape == shape and m.shape == shape and g.get_device() == dev and m.get_device() == dev
-        if wo is not w or mo is not m:
-            same = same and wo.shape == shape and mo.shape == shape and wo.get_device() == dev and mo.get_device() == dev
+        typed = m.dtype is f32
+        plain = w.is_contiguous() and m.is_contiguous()
+        pw, pm = w.data_ptr(), m.data_ptr()
+        pwo, pmo = pw, pm
+        if wo is not w:
+            same = same and wo.shape == shape and wo.get_device() == dev
+            typed, plain, pwo = typed and wo.dtype is w_dtype, plain and wo.is_contiguous(), wo.data_ptr()
+        if mo is not m:
+            same = same and mo.shape == shape and mo.get_device() == dev
+            typed, plain, pmo = typed and mo.dtype is f32, plain and mo.is_contiguous(), mo.data_ptr()
         if not same:
             raise ValueError(f"muon_update: gradient, momentum and outputs must have their weight's shape {tuple(shape)} "
                              "and device")
-        if m.dtype is not f32 or mo.dtype is not f32 or wo.dtype is not w.dtype:
+        if not typed:
             raise ValueError("muon_update: momenta must be fp32 and new weights of their weight's type")
-        if not (w.is_contiguous() and m.is_contiguous() and wo.is_contiguous() and mo.is_contiguous()):
+        if not plain:
             raise ValueError("muon_update: weights, momenta and outputs must be contiguous")
         if not g.is_contiguous():
             g = g.contiguous()
-        rows.append((w, g, m, wo, mo, w.data_ptr(), m.data_ptr(), wo.data_ptr(), mo.data_ptr(), g.data_ptr()))
-    new = {p for r in rows for p in r[7:9]}
-    if len(new) != 2 * len(rows):
+            kept.append(g)
+        pg = g.data_ptr()
+        inputs.append(pg)
+        if pwo != pw:
+            inputs.append(pw)
+        if pmo != pm:
+            inputs.append(pm)
+        new += (pwo, pmo)
+        if dev not in devices:
+            devices[dev] = w.device, {}
+        kinds, key = devices[dev][1], (shape, w_dtype, g_dtype)
+        if key in kinds:
+            kinds[key].append((pg, pm, pw, pmo, pwo))
+        else:
+            kinds[key] = [(pg, pm, pw, pmo, pwo)]
+    written = set(new)
+    if len(written) != len(new):
         raise ValueError("muon_update: a tensor is written twice")
-    for _, _, _, _, _, w, m, wo, mo, g in rows:
-        if (w != wo and w in new) or (m != mo and m in new) or g in new:
-            raise ValueError("muon_update: an output is another tensor's input")
-    return rows
+    if not written.isdisjoint(inputs):
+        raise ValueError("muon_update: an output is another tensor's input")
+    return list(devices.values()), kept
 
 
 @torch.no_grad()
@@ -190,23 +213,20 @@ def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nest
     if scale not in SCALES:
         raise ValueError(f"muon_update: scale must be one of {SCALES}, got {scale!r}")
     _check_numbers("muon_update", steps, eps, coefficients)
-    rows = _rows(weights, grads, momenta, out)
+    devices, kept = _rows(weights, grads, momenta, out)
     L.require_gpu(*weights)
-    devices: dict = {}
-    for row in rows:
-        devices.setdefault(row[0].get_device(), {}).setdefault((row[0].shape, row[0].dtype, row[1].dtype), []).append(row)
     cfg = _config(steps, coefficients, eps, nesterov, float(momentum))
-    for kinds in devices.values():
+    keep = 1.0 - lr * weight_decay
+    for device, kinds in devices:
         keys = list(kinds)
-        dev = kinds[keys[0]][0][0].device
         for call in _calls([(k[0], len(kinds[k])) for k in keys]):
             groups, part = [], []
             for k, first, n in call:
-                shape, w_dtype, g_dtype = keys[k]
-                groups.append(L.LlattnMuonGroup(n, *shape, L.dtype_code(g_dtype), L.dtype_code(w_dtype), 1.0 - lr * weight_decay,
+                shape, w_dtype, g_dtype = key = keys[k]
+                groups.append(L.LlattnMuonGroup(n, *shape, L.dtype_code(g_dtype), L.dtype_code(w_dtype), keep,
                                                 lr * _update_scale(scale, *shape)))
-                part += kinds[keys[k]][first:first + n]
-            _launch("llattn_muon_update", cfg, groups, dev, *[[r[k] for r in part] for k in (9, 6, 5, 8, 7)],
+                part += kinds[key][first:first + n]
+            _launch("llattn_muon_update", cfg, groups, device, *zip(*part),
                     work=sum(12 * q.batch * q.rows * q.cols for q in groups))
     _written([t for v in out for t in v])
 
