@@ -149,10 +149,17 @@ struct BlockOp : ColOp<T, W> {
   __device__ __forceinline__ uint32_t at(int i, int left) const { return kmask(off[i], k_of[i], left); }
 };
 
-// One tile of a product.  A 64-k step is two rounds of products, each beside the fragment reads of the next: k 0..31
+// Tiles of a product.  A 64-k step is two rounds of products, each beside the fragment reads of the next: k 0..31
 // (reads k 32..63), a barrier, k 32..63 (reads the next step's k 0..31 and issues the loads of step kt + NST into the
 // stage just read).  Waves whose part of the tile lies outside load and wait like the others and do nothing else.
-// Offsets are taken from the tile's first row and step, so operands may be of any size below 32 GiB.
+// Offsets are taken from the tile's first row and step, so operands may be of any size.
+//
+// The logits' products take tile after tile (2048 x 1408 x 131072: 614 us, so 583); the gradients' one tile a workgroup
+// (131 steps a tile: the longer loop cost 586 -> 636 us a piece of 8192 x 1536 x 32768).
+//
+// Measured, 8192 rows, D 1536: l of 131072 columns 2420 us (1360 TFLOP/s), a piece of 32768 of them: q 683 us (1210; it
+// writes 537 MB), dh 630 us (1310) and 680 where it adds to the piece's before, dW 604 us (1370).  256 x 256 tiles: matrix
+// cores 59-68% busy at a clock of 1.9 GHz that these products themselves bring down.
 template <int EPI, bool AT, bool BT, typename S, int WGS>
 __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const HeadArgs a) {
   constexpr int MB = S::MB, NB = S::NB, TM = S::TM, TN = S::TN, NST = S::NST, STAGE = S::STAGE, W = S::W;
@@ -506,8 +513,8 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
 
 // Joins the parts of R rows: Q = 256 / R threads a row take every Q-th part, first the maxima, then the sums against the
 // row's maximum; the Q in a fixed order, behind what the columns before left (`run`, where `more`).  FINAL: the loss, else
-// `run`.  (16 rows a workgroup read whole cache lines, 4 fill the chip where rows are few: 8192 rows of 1024 parts 29 us
-// against 80, 333 rows of 786 parts 17 against 8.)
+// `run`.  (16 rows a workgroup read whole cache lines, 4 fill the chip where rows are few: 8192 rows of 1024 parts 34 us
+// against 80, 333 rows of 786 parts 17 against 8.  Latency and 2 TB/s: the parts are read twice, 134 MB.)
 struct JoinArgs {
   const float2* part; const int32_t* part_i;
   int slots, M, more;
@@ -614,7 +621,7 @@ __global__ __launch_bounds__(1024) void head_total_kernel(const float* loss, con
   }
 }
 
-// out = alpha * sum over splits of the partial sums, in order
+// out = alpha * sum over splits of the partial sums, in order (bandwidth: 8192 x 1536 from 4 splits in 40 us, 5.6 TB/s)
 template <typename T>
 __global__ __launch_bounds__(256) void head_reduce_kernel(const float* x, int splits, int64_t n, T* y, const float* grad,
                                                           const float* inv, int per_row) {
