@@ -1062,13 +1062,13 @@ float scale_of(const GroupPlan& g) { return std::exp2f((float)std::min(14, (int)
 // the 256 CUs, the last with fewer workgroups on each; of several, its work is shared out and ends with a part of the
 // longest tile.  Measured in us (G: X Xᵀ, P: A A, A: B X):
 //                                   64 x 64        64 x 64, 2 k groups   128 x 128       256 x 256
-//   3 of 333 x 1001     G P A     11   9  12         11   9  15          26  20  19      62  41  48
-//   1 of 512 x 1408     G P A     14   9  10         13   9  10          36  22  21      91  64  54
-//   1 of 1408 x 4096    G P A     37  18  63         32  16  73          80  41  62     208 107  98
-//   6 of 1000 x 1500    G P A     49  39  77          -                  43  36  75     105  95  87
-//   22 of 1408 x 1408   G P A    273 291 506          -                 225 235 376     215 239 405
-//   22 of 1408 x 4096   G P A    846 288 1442         -                 517 251 1051    492 244 993
-//   8 of 4096 x 4096    G P A   3255 3395 3914        -                1489 1635 2751  1416 1472 2334
+//   3 of 333 x 1001     G P A     11   8  10         10   8  13          23  15  15      57  34  34
+//   1 of 512 x 1408     G P A     14   9   9         12   9   9          33  17  17      78  44  41
+//   1 of 1408 x 4096    G P A     37  17  60         32  15  70          76  36  55     191  86  85
+//   6 of 1000 x 1500    G P A     47  35  73          -                  38  30  65      87  72  71
+//   22 of 1408 x 1408   G P A    252 259 475          -                 204 209 343     188 201 365
+//   22 of 1408 x 4096   G P A    833 257 1353         -                 495 218 934     479 215 897
+//   8 of 4096 x 4096    G P A   3212 3217 3808        -                1393 1469 2636  1387 1391 2194
 // (128 x 256 tiles on eight waves lay between the last two throughout.)
 template <bool SYM>
 int choose(const llattn_muon_cfg* c, const llattn_muon_group* groups, const Plan& p, bool gram) {
