@@ -475,13 +475,16 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
           for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              if constexpr (EPI == STATS_PRED) {
-                const int c = column(j) + e;
-                if (c < a.N) max_first(m, mi, acc[i][j][e], a.v0 + c);
+              if constexpr (EPI == STATS_PRED) {  // a lane's columns ascend: the first of equal ones stays
+                if (acc[i][j][e] > m) {
+                  m = acc[i][j][e];
+                  mi = 32 * (j >> 1) + 4 * (j & 1) + e;
+                }
               } else {
                 m = fmaxf(m, acc[i][j][e]);
               }
             }
+          if (EPI == STATS_PRED && mi != 0x7fffffff) mi += a.v0 + col0 + 8 * g;
           if constexpr (EPI == STATS_PRED) {
             max_first(m, mi, __shfl_xor(m, 16), __shfl_xor(mi, 16));
             max_first(m, mi, __shfl_xor(m, 32), __shfl_xor(mi, 32));

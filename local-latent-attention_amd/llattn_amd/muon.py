@@ -93,7 +93,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, eps: float = 1e-7, coefficien
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """Newton-Schulz iteration on every matrix of ``x [..., m, n]`` (fp32 or bf16; any strides), from ``X = x / (|x|_F +
     eps)``: towards the orthogonal factor of ``x``'s polar decomposition.  Returns ``x``'s type and shape; ``out``
-    (contiguous, may be ``x``) receives the result.  A zero matrix stays zero; one that holds an infinity or NaN gives
+    (contiguous, may be ``x``) receives the result.  A zero matrix stays zero (``eps`` > 0); one that holds an infinity or NaN gives
     NaN throughout.  Not differentiable.  GPU only."""
     if x.dim() < 2:
         raise ValueError(f"orthogonalize: expected [..., m, n], got shape {tuple(x.shape)}")
