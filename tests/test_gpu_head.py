@@ -327,3 +327,14 @@ def test_forward_in_several_ranges():
     logits = h[at].double() @ w.double().t()
     top = logits.gather(1, pred[at].long()[:, None]).squeeze(1)
     assert bool((logits.amax(1) - top <= 2 * D * U * (h[at].double().abs() @ w.double().abs().t()).amax(1)).all())
+
+
+def test_evaluation_of_parameters():
+    """Under no_grad leaves that require gradients take the same path as plain tensors: the same bits, no graph."""
+    h, w, t = _inputs(90, 64, 700, seed=21)
+    want, pred = _loss(h, w, t, return_pred=True)
+    with torch.no_grad():
+        got, p = _loss(h.clone().requires_grad_(True), torch.nn.Parameter(w), t, return_pred=True)
+    assert not got.requires_grad and torch.equal(got, want) and torch.equal(p, pred)
+    live = _loss(h, torch.nn.Parameter(w), t)
+    assert live.requires_grad and torch.equal(live.detach(), want)
