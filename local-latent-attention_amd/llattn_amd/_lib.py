@@ -15,6 +15,7 @@ from dataclasses import dataclass
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "libllattn_gfx950.so"
 ABI_VERSION = 8
@@ -206,6 +207,16 @@ def require_gpu(*tensors: torch.Tensor) -> None:
         if t is not None and t.device.type != "cuda":
             raise RuntimeError("llattn runs on MI355X (gfx950) GPUs only; got a tensor on "
                                f"{t.device} (there is no CPU path)")
+
+
+def refuse_tangents(who: str, tensors) -> None:
+    """Raises where one of ``tensors`` carries a forward-mode tangent, for calls that no autograd function stands around:
+    their results would have none, which reads as a derivative of zero."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no dual level is open
+        return
+    for t in tensors:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{who} has no forward-mode derivative")
 
 
 def on_device(device: torch.device):

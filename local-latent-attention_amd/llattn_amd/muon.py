@@ -101,6 +101,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, eps: float = 1e-7, coefficien
     L.dtype_code(x.dtype)
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("orthogonalize has no gradient: call it under torch.no_grad() or on a detached tensor")
+    L.refuse_tangents("orthogonalize", (x,))
     L.require_gpu(x)
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -214,6 +215,7 @@ def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nest
         raise ValueError(f"muon_update: scale must be one of {SCALES}, got {scale!r}")
     _check_numbers("muon_update", steps, eps, coefficients)
     devices, kept = _rows(weights, grads, momenta, out)
+    L.refuse_tangents("muon_update", weights + grads + momenta)
     L.require_gpu(*weights)
     cfg = _config(steps, coefficients, eps, nesterov, float(momentum))
     keep = 1.0 - lr * weight_decay

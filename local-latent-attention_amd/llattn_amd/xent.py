@@ -229,7 +229,8 @@ def piecewise_head_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Te
     gradients), ``"sum"``, or ``"none"`` (fp32, ``targets``' shape, 0 in ignored rows).  A target outside ``[0, V)``
     gives NaN.  With ``return_pred`` also the first argmax of every row (int32).  ``h`` and ``weight`` are bf16 or fp32,
     fp32 ones rounded to bf16 as under autocast; logits, sums and losses are fp32 and gradients come in their input's
-    type, ``weight``'s accumulated in fp32.  Fewer than 2^23 rows.  Differentiable once.  GPU only."""
+    type, ``weight``'s accumulated in fp32.  Fewer than 2^23 rows.  Differentiable once, in
+    reverse mode.  GPU only."""
     if h.dim() < 1 or weight.dim() != 2 or weight.shape[1] != h.shape[-1] or 0 in weight.shape:
         raise ValueError(f"piecewise_head_loss: weight {tuple(weight.shape)} does not match hidden states {tuple(h.shape)}")
     if targets.shape != h.shape[:-1]:
@@ -242,6 +243,7 @@ def piecewise_head_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Te
         L.dtype_code(t.dtype)
     if piece < 0 or piece % 256:
         raise ValueError(f"piecewise_head_loss: piece must be 0 or a multiple of 256, got {piece}")
+    L.refuse_tangents("piecewise_head_loss", (h, weight))
     L.require_gpu(h, weight, targets)
     if not h.device == weight.device == targets.device:
         raise ValueError(f"piecewise_head_loss: tensors on {h.device}, {weight.device} and {targets.device}")

@@ -204,3 +204,22 @@ def test_groups_added_to_the_joint_optimiser_are_adamws():
     again = muon.MuonAdamW([w], [{"params": [b]}, {"params": [e], "weight_decay": 0.0}], dict(lr=0.1), lr=1e-3)
     again.load_state_dict(opt.state_dict())
     assert again.param_groups[2]["betas"] == (0.9, 0.95) and again.param_groups[0]["momentum"] == 0.95
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_forward_mode_tangents_are_refused(which):
+    """A dual tensor whose primal needs no gradient: an answer without a tangent would read as a derivative of zero."""
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        def dual(*shape, dtype=torch.float32):
+            return fw.make_dual(torch.zeros(*shape, dtype=dtype), torch.ones(*shape, dtype=dtype))
+        h, w, t = torch.zeros(4, 8, dtype=BF16), torch.zeros(10, 8, dtype=BF16), torch.zeros(4, dtype=torch.int64)
+        x = [torch.zeros(4, 6) for _ in range(3)]
+        calls = [lambda: piecewise_head_loss(dual(4, 8, dtype=BF16), w, t),
+                 lambda: piecewise_head_loss(h, dual(10, 8, dtype=BF16), t, reduction="none"),
+                 lambda: muon.orthogonalize(dual(3, 4)),
+                 *[lambda k=k: muon.muon_update(*[[dual(4, 6) if i == k else v] for i, v in enumerate(x)], lr=0.1) for k in range(3)]]
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            calls[which]()
+        with pytest.raises(RuntimeError, match="no CPU path"):  # plain tensors beside an open level
+            piecewise_head_loss(h, w, t)
