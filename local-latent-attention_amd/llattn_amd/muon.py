@@ -258,6 +258,20 @@ class Muon(torch.optim.Optimizer):
             _muon_group(group, self.state)
         return loss
 
+    def load_state_dict(self, state_dict) -> None:
+        super().load_state_dict(state_dict)
+        _restore_momenta(self, state_dict)
+
+
+def _restore_momenta(optimizer, state_dict) -> None:
+    """fp32 momenta from ``state_dict``: Optimizer.load_state_dict gives a state its parameter's type, and bf16 parameters'
+    momenta would lose 16 bits."""
+    ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+    for i, p in zip(ids, [p for g in optimizer.param_groups for p in g["params"]]):
+        buf = state_dict["state"].get(i, {}).get("momentum_buffer")
+        if buf is not None:
+            optimizer.state[p]["momentum_buffer"] = buf.detach().to(device=p.device, dtype=torch.float32, copy=True)
+
 
 def _muon_group(group, state) -> None:
     params = [p for p in group["params"] if p.grad is not None]
@@ -265,8 +279,6 @@ def _muon_group(group, state) -> None:
         buf = state[p].get("momentum_buffer")
         if buf is None:
             state[p]["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-        elif buf.dtype is not torch.float32:  # load_state_dict gives a state its parameter's type
-            state[p]["momentum_buffer"] = buf.float()
     muon_update(params, [p.grad for p in params], [state[p]["momentum_buffer"] for p in params],
                 **{k: group[k] for k in ("lr", "momentum", "nesterov", "weight_decay", "steps", "eps", "coefficients", "scale")})
 
@@ -293,3 +305,7 @@ class MuonAdamW(torch.optim.Optimizer):
         self._adamw.param_groups, self._adamw.state = self.param_groups[1:], self.state
         self._adamw.step()
         return loss
+
+    def load_state_dict(self, state_dict) -> None:
+        super().load_state_dict(state_dict)
+        _restore_momenta(self, state_dict)

@@ -223,3 +223,27 @@ def test_forward_mode_tangents_are_refused(which):
             calls[which]()
         with pytest.raises(RuntimeError, match="no CPU path"):  # plain tensors beside an open level
             piecewise_head_loss(h, w, t)
+
+
+def _optimiser(kind, mats, vecs):
+    return muon.Muon(mats, lr=0.1) if kind == "muon" else muon.MuonAdamW(mats, vecs, dict(lr=0.1), lr=1e-3)
+
+
+@pytest.mark.parametrize("kind", ["muon", "joint"])
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+def test_momenta_are_loaded_in_fp32(kind, dtype):
+    """A state saved and loaded has the same bits, bf16 parameters' momenta too, and shares no memory with the dict."""
+    def build():
+        return _optimiser(kind, [torch.nn.Parameter(torch.zeros(3, 5, dtype=dtype)) for _ in range(3)], [torch.nn.Parameter(torch.zeros(4))])
+    a, b = build(), build()
+    want = {i: torch.randn(3, 5, generator=torch.Generator().manual_seed(i)) for i in (0, 2)}  # the second has not been updated yet
+    for i, m in want.items():
+        a.state[a.param_groups[0]["params"][i]]["momentum_buffer"] = m.clone()
+    saved = a.state_dict()
+    b.load_state_dict(saved)
+    for i, p in enumerate(b.param_groups[0]["params"]):
+        assert (i in want) == ("momentum_buffer" in b.state.get(p, {}))
+        if i in want:
+            got = b.state[p]["momentum_buffer"]
+            assert got.dtype is torch.float32 and torch.equal(got, want[i])
+            assert got.data_ptr() != saved["state"][i]["momentum_buffer"].data_ptr()
