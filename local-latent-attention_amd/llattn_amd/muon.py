@@ -11,6 +11,7 @@ multiplied on the fp16 matrix cores.
 """
 from __future__ import annotations
 
+import copy
 import ctypes
 import math
 from array import array
@@ -289,9 +290,9 @@ class MuonAdamW(torch.optim.Optimizer):
 
     def __init__(self, matrices, others, muon: dict | None = None, **adamw) -> None:
         matrices, others = list(matrices), list(others)
-        self._muon = Muon(matrices, **(muon or {}))
+        matrix_groups = Muon(matrices, **(muon or {})).param_groups
         self._adamw = torch.optim.AdamW(others, **adamw)
-        groups = [dict(g) for g in self._muon.param_groups + self._adamw.param_groups]
+        groups = [dict(g) for g in matrix_groups + self._adamw.param_groups]
         super().__init__(groups, dict(self._adamw.defaults))
 
     @torch.no_grad()
@@ -305,6 +306,13 @@ class MuonAdamW(torch.optim.Optimizer):
         self._adamw.param_groups, self._adamw.state = self.param_groups[1:], self.state
         self._adamw.step()
         return loss
+
+    def __getstate__(self) -> dict:
+        # Optimizer's own keeps groups, state and defaults, for copies and pickles.  The AdamW inside goes along without
+        # parameters or state: step() hands it this optimiser's.
+        inner = copy.copy(self._adamw)
+        inner.param_groups, inner.state = [], {}
+        return {**super().__getstate__(), "_adamw": inner}
 
     def load_state_dict(self, state_dict) -> None:
         super().load_state_dict(state_dict)

@@ -1,6 +1,8 @@
 """CPU tests of the head loss and the weight update: the C interface (include/llattn_train.h), and what is refused before
 anything is launched."""
+import copy
 import ctypes
+import pickle
 import re
 import subprocess
 
@@ -247,3 +249,31 @@ def test_momenta_are_loaded_in_fp32(kind, dtype):
             got = b.state[p]["momentum_buffer"]
             assert got.dtype is torch.float32 and torch.equal(got, want[i])
             assert got.data_ptr() != saved["state"][i]["momentum_buffer"].data_ptr()
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle"])
+def test_copies_of_the_optimisers_go_on(how):
+    """A copy has its own parameters and state and steps like the original (vectors; matrices need a GPU)."""
+    w, b = torch.nn.Parameter(torch.zeros(4, 8)), torch.nn.Parameter(torch.zeros(4))
+    opt = muon.MuonAdamW([w], [b], dict(lr=0.1), lr=1e-3, betas=(0.9, 0.95))
+    b.grad = torch.ones(4)
+    opt.step()
+    opt.state[w]["momentum_buffer"] = torch.ones(4, 8)
+    twin = copy.deepcopy(opt) if how == "deepcopy" else pickle.loads(pickle.dumps(opt))
+    (w2,), (b2,) = (g["params"] for g in twin.param_groups)
+    assert b2 is not b and torch.equal(b2, b) and torch.equal(twin.state[w2]["momentum_buffer"], torch.ones(4, 8))
+    assert twin.param_groups[0]["momentum"] == 0.95 and twin.param_groups[1]["betas"] == (0.9, 0.95)
+    b.grad, b2.grad = torch.full((4,), -2.0), torch.full((4,), -2.0)
+    opt.step()
+    before = b.detach().clone()
+    assert not torch.equal(b2, b)
+    twin.step()
+    assert torch.equal(b2, b) and torch.equal(b, before)
+    twin.add_param_group({"params": [torch.nn.Parameter(torch.zeros(2))]})
+    assert twin.param_groups[2]["betas"] == (0.9, 0.95) and len(opt.param_groups) == 2
+    twin.zero_grad()
+    twin.step()
+    only = muon.Muon([w], lr=0.1)
+    again = copy.deepcopy(only) if how == "deepcopy" else pickle.loads(pickle.dumps(only))
+    again.step()  # no gradients
+    assert again.param_groups[0]["lr"] == 0.1
