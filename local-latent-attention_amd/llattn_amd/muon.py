@@ -285,8 +285,8 @@ def _muon_group(group, state) -> None:
 
 
 class MuonAdamW(torch.optim.Optimizer):
-    """Muon for ``matrices``, AdamW for the other parameter groups, as one optimiser: one list of groups, one state.
-    The matrices are the first group; groups added later are AdamW's."""
+    """Muon for ``matrices`` (parameters or groups of them), AdamW for the other parameter groups, as one optimiser: one
+    list of groups, the matrices' first, and one state.  Groups added later are AdamW's."""
 
     def __init__(self, matrices, others, muon: dict | None = None, **adamw) -> None:
         matrices, others = list(matrices), list(others)
@@ -301,9 +301,12 @@ class MuonAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        _muon_group(self.param_groups[0], self.state)
         # the groups and the state are this optimiser's own (schedulers and load_state_dict act on them)
-        self._adamw.param_groups, self._adamw.state = self.param_groups[1:], self.state
+        for group in self.param_groups:
+            if "coefficients" in group:  # Muon's, as no group of AdamW's has them
+                _muon_group(group, self.state)
+        self._adamw.param_groups = [g for g in self.param_groups if "coefficients" not in g]
+        self._adamw.state = self.state
         self._adamw.step()
         return loss
 

@@ -277,3 +277,17 @@ def test_copies_of_the_optimisers_go_on(how):
     again = copy.deepcopy(only) if how == "deepcopy" else pickle.loads(pickle.dumps(only))
     again.step()  # no gradients
     assert again.param_groups[0]["lr"] == 0.1
+
+
+def test_groups_of_matrices_are_all_muons(monkeypatch):
+    """Matrices in several groups, each with options of its own: none is left to AdamW."""
+    seen = []
+    monkeypatch.setattr(muon, "muon_update", lambda w, g, m, **kw: seen.append((list(w), kw["lr"], kw["momentum"])))
+    u, v, w = (torch.nn.Parameter(torch.zeros(4, 8)) for _ in range(3))
+    b = torch.nn.Parameter(torch.zeros(4))
+    opt = muon.MuonAdamW([{"params": [u]}, {"params": [v, w], "lr": 0.5}], [b], dict(lr=0.1, momentum=0.9), lr=1e-3)
+    for p in (u, v, b):
+        p.grad = torch.ones_like(p)
+    opt.step()
+    assert [([id(p) for p in ps], lr, mu) for ps, lr, mu in seen] == [([id(u)], 0.1, 0.9), ([id(v)], 0.5, 0.9)]
+    assert not any(p.detach().any() for p in (u, v, w)) and torch.allclose(b.detach(), torch.full((4,), -1e-3))
