@@ -135,17 +135,17 @@ def _ptr(t):
 
 
 REDUCTIONS = ("mean", "sum", "none")
+MAX_STRIDE = 1 << 23  # elements from a row to the next, for llattn_head_fwd and _bwd
 
 
 def _bf16_rows(t: torch.Tensor, pad: int) -> torch.Tensor:
-    """``t [R, D]`` in bf16 with ``pad`` zero columns behind, rows 16-byte aligned (``t`` itself where it is that)."""
+    """``t [R, D]`` in bf16 with ``pad`` zero columns behind, rows 16-byte aligned and less than 2^23 elements apart
+    (``t`` itself where it is that)."""
     t = t.detach().to(torch.bfloat16)
     if pad:
         return F.pad(t, (0, pad))
-    if t.stride(1) != 1 or t.stride(0) < t.shape[1] or t.stride(0) % 8 or t.data_ptr() % 16:
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
+    if t.stride(1) != 1 or not t.shape[1] <= t.stride(0) < MAX_STRIDE or t.stride(0) % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)  # also of one row, whose stride may be anything
     return t
 
 

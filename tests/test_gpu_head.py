@@ -338,3 +338,26 @@ def test_evaluation_of_parameters():
     assert not got.requires_grad and torch.equal(got, want) and torch.equal(p, pred)
     live = _loss(h, torch.nn.Parameter(w), t)
     assert live.requires_grad and torch.equal(live.detach(), want)
+
+
+@pytest.mark.parametrize("B", [1, 3])
+def test_last_position_of_long_sequences(B):
+    """hidden[:, -1] of sequences so long that its rows lie 2^23 elements and more apart, and a weight of one far row."""
+    T, D, V = 8192, 1024, 300
+    g = torch.Generator().manual_seed(22)
+    hidden = torch.zeros(B, T, D, dtype=BF16, device=DEV)
+    hidden[:, -1] = torch.randn(B, D, generator=g).to(BF16).to(DEV)
+    w = (torch.randn(V, D, generator=g) * 0.06).to(BF16).to(DEV)
+    t = torch.randint(0, V, (B,), generator=g).to(DEV)
+    leaf = hidden.clone().requires_grad_(True)
+    weight = w.clone().requires_grad_(True)
+    want = hidden[:, -1].clone().requires_grad_(True)
+    rows = _loss(leaf[:, -1], weight, t, reduction="none")
+    ref = _loss(want, weight, t, reduction="none")
+    assert torch.equal(rows, ref)
+    rows.sum().backward()
+    gh, = torch.autograd.grad(ref.sum(), want)
+    assert torch.equal(leaf.grad[:, -1], gh) and not leaf.grad[:, :-1].any()
+    one = torch.zeros_like(t)  # a vocabulary of one, a row far along
+    (l, el), _, _ = _exact(want.detach(), hidden[0, -1:], one)
+    _near(_loss(want.detach(), hidden[:1, -1], one, reduction="none"), l, el, F32, "one column")

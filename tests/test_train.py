@@ -13,7 +13,7 @@ from conftest import REPO
 from llattn_amd import _lib as L
 from llattn_amd import muon
 from llattn_amd.lm import build_model, make_optimizer
-from llattn_amd.xent import piecewise_head_loss
+from llattn_amd.xent import _bf16_rows, piecewise_head_loss
 
 BF16 = torch.bfloat16
 
@@ -291,3 +291,27 @@ def test_groups_of_matrices_are_all_muons(monkeypatch):
     opt.step()
     assert [([id(p) for p in ps], lr, mu) for ps, lr, mu in seen] == [([id(u)], 0.1, 0.9), ([id(v)], 0.5, 0.9)]
     assert not any(p.detach().any() for p in (u, v, w)) and torch.allclose(b.detach(), torch.full((4,), -1e-3))
+
+
+def _row_views():
+    """[R, 64] bf16 views whose rows the kernels do not read as they are."""
+    x = torch.randn(2 * (1 << 23) + 64, generator=torch.Generator().manual_seed(0)).to(BF16)
+    return [("far apart", x.as_strided((2, 64), (1 << 23, 1))), ("farther", x.as_strided((2, 64), ((1 << 23) + 8, 1))),
+            ("one row, far stride", x.as_strided((1, 64), (1 << 25, 1))), ("one row, stride 1", x.as_strided((1, 64), (1, 1))),
+            ("one row, stride 0", x[:64].expand(1, 64).as_strided((1, 64), (0, 1))), ("overlapping", x.as_strided((3, 64), (8, 1))),
+            ("odd stride", x.as_strided((3, 64), (65, 1))), ("shifted", x[1:129].view(2, 64)), ("columns", x[:128].view(64, 2).t())]
+
+
+@pytest.mark.parametrize("k", range(9))
+def test_rows_come_in_a_layout_that_the_kernels_take(k):
+    name, t = _row_views()[k]
+    got = _bf16_rows(t, 0)
+    assert got.stride(1) == 1 and 64 <= got.stride(0) < 1 << 23 and got.stride(0) % 8 == 0 and got.data_ptr() % 16 == 0, name
+    assert torch.equal(got, t)
+    L.check(L.OK if _head_fwd(rows=len(got), D=64, ldh=got.stride(0), ldw=64, n=1) == L.ERR_WORKSPACE else L.ERR_LAYOUT, name)
+
+
+def test_rows_that_the_kernels_take_are_not_copied():
+    x = torch.zeros(6, 128, dtype=BF16)
+    for t in (x, x[:, :64], x[1:, 64:], x[::2]):
+        assert _bf16_rows(t, 0).data_ptr() == t.data_ptr() and _bf16_rows(t, 0).stride() == t.stride()
