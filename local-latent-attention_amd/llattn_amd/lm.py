@@ -278,7 +278,8 @@ def train_step(model: nn.Module, optimizer: torch.optim.Optimizer, inputs: torch
     Returns the detached loss (no sync)."""
     with torch.autocast(device_type="cuda", dtype=torch.bfloat16):
         if fused_loss:
-            loss, _ = model.loss(inputs, targets, vocab_piece=vocab_piece)
+            # models with a loss of their own need not know vocab_piece
+            loss, _ = model.loss(inputs, targets, **({} if vocab_piece is None else {"vocab_piece": vocab_piece}))
         else:
             loss, _ = lm_loss(model(inputs), targets)
         loss.backward()

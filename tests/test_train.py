@@ -12,7 +12,7 @@ import torch
 from conftest import REPO
 from llattn_amd import _lib as L
 from llattn_amd import muon
-from llattn_amd.lm import build_model, make_optimizer
+from llattn_amd.lm import build_model, make_optimizer, train_step
 from llattn_amd.xent import _bf16_rows, piecewise_head_loss
 
 BF16 = torch.bfloat16
@@ -315,3 +315,23 @@ def test_rows_that_the_kernels_take_are_not_copied():
     x = torch.zeros(6, 128, dtype=BF16)
     for t in (x, x[:, :64], x[1:, 64:], x[::2]):
         assert _bf16_rows(t, 0).data_ptr() == t.data_ptr() and _bf16_rows(t, 0).stride() == t.stride()
+
+
+class _OwnLoss(torch.nn.Module):
+    """A model whose loss takes inputs and targets alone."""
+
+    def __init__(self):
+        super().__init__()
+        self.w = torch.nn.Parameter(torch.ones(3))
+
+    def loss(self, inputs, targets):
+        return (self.w * inputs).sum() - targets.sum(), {}
+
+
+def test_train_step_asks_for_pieces_only_where_told():
+    model = _OwnLoss()
+    opt = torch.optim.SGD(model.parameters(), lr=0.5)
+    loss = train_step(model, opt, torch.tensor([1.0, 0.0, 2.0]), torch.zeros(1), grad_clip=0.0)
+    assert float(loss) == 3.0 and model.w.tolist() == [0.5, 1.0, 0.0]
+    with pytest.raises(TypeError):
+        train_step(model, opt, torch.ones(3), torch.zeros(1), vocab_piece=256)
