@@ -276,6 +276,8 @@ def train_step(model: nn.Module, optimizer: torch.optim.Optimizer, inputs: torch
     cleared (reference train.py:960-1037 with one micro-step).  ``fused_loss``: the chunked head + cross entropy
     (:meth:`LocalLatentLM.loss`, which ``vocab_piece`` is passed to) instead of full logits and ``F.cross_entropy``.
     Returns the detached loss (no sync)."""
+    if vocab_piece is not None and not fused_loss:
+        raise ValueError("train_step: vocab_piece belongs to the fused loss, and fused_loss=False asks for full logits")
     with torch.autocast(device_type="cuda", dtype=torch.bfloat16):
         if fused_loss:
             # models with a loss of their own need not know vocab_piece

@@ -335,3 +335,9 @@ def test_train_step_asks_for_pieces_only_where_told():
     assert float(loss) == 3.0 and model.w.tolist() == [0.5, 1.0, 0.0]
     with pytest.raises(TypeError):
         train_step(model, opt, torch.ones(3), torch.zeros(1), vocab_piece=256)
+
+
+def test_train_step_refuses_pieces_of_full_logits():
+    model = _OwnLoss()
+    with pytest.raises(ValueError, match="vocab_piece"):
+        train_step(model, torch.optim.SGD(model.parameters(), lr=0.5), torch.ones(3), torch.zeros(1), fused_loss=False, vocab_piece=0)
