@@ -25,6 +25,7 @@ from . import _lib as L
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 SCALES = ("aspect", "rms")
 WORKSPACE_BYTES = 4 << 30  # matrices are taken together up to this
+MOST = 32768  # rows and columns of a matrix
 
 
 TILES = 0  # workgroups of the products: the library's choice (llattn_muon_cfg.tiles)
@@ -180,6 +181,8 @@ def _rows(weights, grads, momenta, out):
         if key in kinds:
             kinds[key].append((pg, pm, pw, pmo, pwo))
         else:
+            if max(shape) > MOST:  # before any launch: a list may take several calls, and those before would have updated
+                raise ValueError(f"muon_update: at most {MOST} rows and columns, got shape {tuple(shape)}")
             kinds[key] = [(pg, pm, pw, pmo, pwo)]
     written = set(new)
     if len(written) != len(new):

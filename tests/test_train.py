@@ -341,3 +341,14 @@ def test_train_step_refuses_pieces_of_full_logits():
     model = _OwnLoss()
     with pytest.raises(ValueError, match="vocab_piece"):
         train_step(model, torch.optim.SGD(model.parameters(), lr=0.5), torch.ones(3), torch.zeros(1), fused_loss=False, vocab_piece=0)
+
+
+def test_a_list_is_refused_before_any_of_it_is_updated():
+    """A matrix that the library refuses, in a place that a later call of several would reach."""
+    small, wide = [torch.zeros(4, 6) for _ in range(3)], [torch.zeros(1, 32769) for _ in range(3)]
+    for order in ((small, wide), (wide, small)):
+        with pytest.raises(ValueError, match="32768"):
+            muon.muon_update(*([v[i] for v in order] for i in range(3)), lr=0.1)
+    fits = [torch.zeros(32768, 1) for _ in range(3)]
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        muon.muon_update(*([v] for v in fits), lr=0.1)
