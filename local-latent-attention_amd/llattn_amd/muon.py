@@ -91,11 +91,18 @@ def _check_numbers(who, steps, eps, coefficients):
         raise ValueError(f"{who}: three coefficients expected, got {coefficients}")
 
 
+def _apart(src: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+    """``src`` (contiguous, as large as ``out``), as a copy where it lies across ``out``: a matrix is written while others are
+    still read, and only its own place is safe."""
+    off = src.data_ptr() - out.data_ptr()
+    return src.clone() if 0 < abs(off) < out.numel() * out.element_size() else src
+
+
 def orthogonalize(x: torch.Tensor, steps: int = 5, eps: float = 1e-7, coefficients=COEFFICIENTS,
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """Newton-Schulz iteration on every matrix of ``x [..., m, n]`` (fp32 or bf16; any strides), from ``X = x / (|x|_F +
     eps)``: towards the orthogonal factor of ``x``'s polar decomposition.  Returns ``x``'s type and shape; ``out``
-    (contiguous, may be ``x``) receives the result.  A zero matrix stays zero (``eps`` > 0); one that holds an infinity or NaN gives
+    (contiguous, may be ``x`` or overlap it) receives the result.  A zero matrix stays zero (``eps`` > 0); one that holds an infinity or NaN gives
     NaN throughout.  Not differentiable.  GPU only."""
     if x.dim() < 2:
         raise ValueError(f"orthogonalize: expected [..., m, n], got shape {tuple(x.shape)}")
@@ -112,7 +119,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, eps: float = 1e-7, coefficien
     m, n = x.shape[-2:]
     if x.numel() == 0:
         return out
-    src = x.detach().contiguous()
+    src = _apart(x.detach().contiguous(), out)
     each, dt = m * n * x.element_size(), L.dtype_code(x.dtype)
     cfg = _config(steps, coefficients, eps)
     for call in _calls([((m, n), x.numel() // (m * n))]):

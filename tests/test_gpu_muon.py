@@ -300,3 +300,13 @@ def test_optimisers():
     only = mu.Muon([p for p in d.parameters() if p.dim() == 2])
     d(x).sum().backward()
     assert float(only.step(lambda: torch.tensor(3.0))) == 3.0
+
+
+@pytest.mark.parametrize("m,n", [(20, 30), (100, 140)])
+@pytest.mark.parametrize("shift", [1, -1])
+def test_an_output_across_its_input(m, n, shift):
+    """One matrix of a batch along, for matrices of one workgroup each and of many."""
+    x = _matrices(6, m, n, "flat")
+    want = _muon().orthogonalize(x[:5] if shift > 0 else x[1:])
+    src, out = (x[:5], x[1:]) if shift > 0 else (x[1:], x[:5])
+    assert _muon().orthogonalize(src, out=out) is out and torch.equal(out, want)

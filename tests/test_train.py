@@ -352,3 +352,12 @@ def test_a_list_is_refused_before_any_of_it_is_updated():
     fits = [torch.zeros(32768, 1) for _ in range(3)]
     with pytest.raises(RuntimeError, match="no CPU path"):
         muon.muon_update(*([v] for v in fits), lr=0.1)
+
+
+@pytest.mark.parametrize("src,out,copied", [((0, 4), (0, 4), False), ((1, 5), (0, 4), True), ((0, 4), (1, 5), True), ((0, 4), (4, 8), False),
+                                            ((4, 8), (0, 4), False), ((0, 4), (3, 7), True)])
+def test_an_output_across_its_input_gets_a_copy(src, out, copied):
+    x = torch.arange(8 * 6, dtype=torch.float32).view(8, 2, 3)
+    a, b = x[src[0]:src[1]], x[out[0]:out[1]]
+    got = muon._apart(a, b)
+    assert torch.equal(got, a) and (got.data_ptr() != a.data_ptr()) == copied
