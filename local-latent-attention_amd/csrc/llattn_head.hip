@@ -46,7 +46,7 @@ struct HeadArgs {
   float* tgt;
   const float* lse2;        // GRAD
   uint16_t* p; int64_t p_block; int p_cols;  // q, its columns and the elements of 64 of them
-  // gradients: alpha = grad[0] * (inv ? *inv : 1), or grad[row] within q (per_row)
+  // gradients: alpha = (grad[0], or per_row 1 and grad[row] within q) * (inv ? *inv : 1)
   const float* grad;
   const float* inv;
   int per_row;
@@ -384,7 +384,7 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
           }
         }
       } else {
-        const float alpha = a.per_row ? 1.f : *a.grad * (a.inv ? *a.inv : 1.f);
+        const float alpha = (a.per_row ? 1.f : *a.grad) * (a.inv ? *a.inv : 1.f);
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
           const int row = row0 + 16 * i + r;
@@ -628,7 +628,7 @@ __global__ __launch_bounds__(1024) void head_total_kernel(const float* loss, con
 template <typename T>
 __global__ __launch_bounds__(256) void head_reduce_kernel(const float* x, int splits, int64_t n, T* y, const float* grad,
                                                           const float* inv, int per_row) {
-  const float alpha = per_row ? 1.f : *grad * (inv ? *inv : 1.f);
+  const float alpha = (per_row ? 1.f : *grad) * (inv ? *inv : 1.f);
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
     float v[4];
     load4<float>(x + i, v);

@@ -361,3 +361,31 @@ def test_last_position_of_long_sequences(B):
     one = torch.zeros_like(t)  # a vocabulary of one, a row far along
     (l, el), _, _ = _exact(want.detach(), hidden[0, -1:], one)
     _near(_loss(want.detach(), hidden[:1, -1], one, reduction="none"), l, el, F32, "one column")
+
+
+def _backward(h, w, t, lse2, grad, stride, inv):
+    """llattn_head_bwd itself: (dh, dW)."""
+    import ctypes
+    from llattn_amd import _lib as L
+    (N, D), V = h.shape, w.shape[0]
+    cfg = L.LlattnHeadCfg(N, V, D, 256, L.BF16)
+    n = L.load().llattn_head_bytes(ctypes.byref(cfg), 1)
+    ws = torch.empty(n, dtype=torch.uint8, device=DEV)
+    dh, dw = torch.empty_like(h), torch.empty(V + -V % 8, D, dtype=BF16, device=DEV)
+    p = lambda x: None if x is None else x.data_ptr()  # noqa: E731
+    L.check(L.load().llattn_head_bwd(ctypes.byref(cfg), p(h), D, p(w), D, p(t), -100, p(lse2), p(grad), stride, p(inv), p(dh), p(dw),
+                                     p(ws), n, L.stream_ptr(DEV)), "llattn_head_bwd")
+    return dh, dw[:V]
+
+
+@pytest.mark.parametrize("N,D,V", [(70, 64, 500), (300, 264, 1001)])
+def test_the_rows_share_of_a_gradient_per_row(N, D, V):
+    """s_n = grad[n * grad_stride] * inv: with gradients row by row as with one, and the power of two changes no bit."""
+    h, w, t = _inputs(N, D, V, seed=23)
+    lse2 = torch.logsumexp(h.float() @ w.float().t(), 1) / torch.log(torch.tensor(2.0))
+    g = torch.randn(N, generator=torch.Generator().manual_seed(24)).to(DEV)
+    inv = torch.tensor(0.125, device=DEV)
+    for grad, stride in ((g, 1), (g[:1].clone(), 0)):
+        want = _backward(h, w, t, lse2, grad / 8, stride, None)
+        got = _backward(h, w, t, lse2, grad, stride, inv)
+        assert any(x.any() for x in want) and all(torch.equal(a, b) for a, b in zip(got, want))
