@@ -14,7 +14,8 @@
 // then dh (+)= q W and dW = qᵀ h, times the scale that every row shares.  Rounding q to bf16 is as far off as rounding the
 // results to bf16 is (half a step of 2^-8 each), and those errors average out over the contraction.  The shared scale stays
 // out of q: within it, the entries near -1, which are one value in all rows, would round alike (1 / 4096 rows: 0.4% of
-// the whole gradient).  Only gradients that differ by row are multiplied in.
+// the whole gradient).  Gradients row by row are divided by the largest of them, which is shared in the same way: rows
+// of one gradient (a mean taken outside) then round as if there were none.  Their ratios to it are multiplied in.
 //
 // What bounds it: 2 rows V D operations for each of the four products on the matrix cores; with few rows the reads of
 // W.
@@ -46,10 +47,10 @@ struct HeadArgs {
   float* tgt;
   const float* lse2;        // GRAD
   uint16_t* p; int64_t p_block; int p_cols;  // q, its columns and the elements of 64 of them
-  // gradients: alpha = (grad[0], or per_row 1 and grad[row] within q) * (inv ? *inv : 1)
+  // gradients: alpha = *scale * (inv ? *inv : 1) of the products, and grad[row] / *scale within q (grad null: 1)
   const float* grad;
+  const float* scale;
   const float* inv;
-  int per_row;
   void* C;                  // SUM: fp32 [splits][M][N]
   int accumulate;
 };
@@ -384,7 +385,7 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
           }
         }
       } else {
-        const float alpha = (a.per_row ? 1.f : *a.grad) * (a.inv ? *a.inv : 1.f);
+        const float alpha = *a.scale * (a.inv ? *a.inv : 1.f);
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
           const int row = row0 + 16 * i + r;
@@ -435,8 +436,8 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[i][j][e] -= column(j) + e == tc ? 1.f : 0.f;
           }
-          if (a.per_row) {
-            const float s = live ? a.grad[row] : 0.f;
+          if (a.grad) {
+            const float s = live ? a.grad[row] / *a.scale : 0.f;  // the largest gives exactly 1
 #pragma unroll
             for (int j = 0; j < NB; ++j) acc[i][j] *= s;
           }
@@ -624,11 +625,36 @@ __global__ __launch_bounds__(1024) void head_total_kernel(const float* loss, con
   }
 }
 
+// What q leaves to the products' scale: the first of the largest gradients by size among the finite ones of rows that count
+// (1 where all are zero), with its sign, so that rows of one gradient have q = softmax - onehot exactly.
+__global__ __launch_bounds__(1024) void head_scale_kernel(const float* grad, const int64_t* targets, int64_t ignore_index, int M,
+                                                          float* scale) {
+  __shared__ float sm[1024];
+  __shared__ int si[1024];
+  float m = 0.f;
+  int mi = 0x7fffffff;
+  for (int i = threadIdx.x; i < M; i += 1024) {
+    const float g = fabsf(grad[i]);
+    if (targets[i] != ignore_index && g > m && g < __builtin_inff()) {
+      m = g;
+      mi = i;
+    }
+  }
+  sm[threadIdx.x] = m;
+  si[threadIdx.x] = mi;
+  __syncthreads();
+  for (int o = 512; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) max_first(sm[threadIdx.x], si[threadIdx.x], sm[threadIdx.x + o], si[threadIdx.x + o]);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *scale = sm[0] > 0.f ? grad[si[0]] : 1.f;
+}
+
 // out = alpha * sum over splits of the partial sums, in order (bandwidth: 8192 x 1536 from 4 splits in 40 us, 5.6 TB/s)
 template <typename T>
-__global__ __launch_bounds__(256) void head_reduce_kernel(const float* x, int splits, int64_t n, T* y, const float* grad,
-                                                          const float* inv, int per_row) {
-  const float alpha = (per_row ? 1.f : *grad) * (inv ? *inv : 1.f);
+__global__ __launch_bounds__(256) void head_reduce_kernel(const float* x, int splits, int64_t n, T* y, const float* scale,
+                                                          const float* inv) {
+  const float alpha = *scale * (inv ? *inv : 1.f);
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
     float v[4];
     load4<float>(x + i, v);
@@ -711,13 +737,13 @@ int piece_of(const llattn_head_cfg* c) {
   return (int)std::min<int64_t>(p, ceil_div(c->V, 256) * 256);
 }
 
-// q of a piece [rows][piece], the sums of dh over pieces and splits, the partial sums of dW
+// q of a piece [rows][piece], the sums of dh over pieces and splits, the partial sums of dW, the shared scale
 struct BwdPlan {
   int piece, pieces;
   Tiling logits, dh, dw;
   size_t p, dh_part, dw_part;
   bool dh_direct() const { return pieces == 1 && dh.splits == 1; }
-  size_t bytes() const { return p + dh_part + dw_part; }
+  size_t bytes() const { return p + dh_part + dw_part + up(4); }
 };
 BwdPlan bwd_plan(const llattn_head_cfg* c) {
   BwdPlan b{};
@@ -758,7 +784,7 @@ void logits_of(HeadArgs& a, const llattn_head_cfg* c, const void* h, int64_t ldh
 template <typename T>
 void launch_reduce(const float* x, int splits, int64_t n, T* y, const HeadArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(head_reduce_kernel<T>, dim3((unsigned)std::min<int64_t>(ceil_div(n, 1024), 8192)), dim3(256), 0, st, x, splits,
-                     n, y, a.grad, a.inv, a.per_row);
+                     n, y, a.scale, a.inv);
 }
 
 int32_t check_operands(const char* who, const llattn_head_cfg* c, const void* h, int64_t ldh, const void* W, int64_t ldw,
@@ -842,10 +868,14 @@ extern "C" int32_t llattn_head_bwd(const llattn_head_cfg* c, const void* h, int6
   char* ws = static_cast<char*>(workspace);
   float* dh_part = reinterpret_cast<float*>(ws + b.p);
   float* dw_part = reinterpret_cast<float*>(ws + b.p + b.dh_part);
+  float* scale = reinterpret_cast<float*>(ws + b.p + b.dh_part + b.dw_part);
   HeadArgs a{};
   a.p = reinterpret_cast<uint16_t*>(ws); a.p_block = (int64_t)c->rows * 64; a.p_cols = b.piece;
   a.targets = targets; a.ignore_index = ignore_index;
-  a.lse2 = lse2; a.grad = grad; a.per_row = grad_stride; a.inv = inv;
+  a.lse2 = lse2; a.inv = inv;
+  a.grad = grad_stride ? grad : nullptr;
+  a.scale = grad_stride ? scale : grad;
+  if (grad_stride) hipLaunchKernelGGL(head_scale_kernel, dim3(1), dim3(1024), 0, st, grad, targets, ignore_index, c->rows, scale);
   const int64_t dw_size = c->dw_dtype == LLATTN_F32 ? 4 : 2;
   for (int q = 0; q < b.pieces; ++q) {
     const int v0 = (int)((int64_t)q * b.piece), cols = std::min(b.piece, c->V - v0);

@@ -389,3 +389,45 @@ def test_the_rows_share_of_a_gradient_per_row(N, D, V):
         want = _backward(h, w, t, lse2, grad / 8, stride, None)
         got = _backward(h, w, t, lse2, grad, stride, inv)
         assert any(x.any() for x in want) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_one_gradient_for_all_rows_is_the_means(dtype):
+    """reduction="none" with the same gradient in every row that counts, whatever stands in the others: the bits of the
+    mean, whose scale is never rounded into the logits' gradient (1 / n would be, alike in every row's entry near -1)."""
+    h, w, t = _inputs(333, 72, 1003, seed=25, dtype=dtype)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    want = torch.autograd.grad(_loss(h, w, t, piece=256), (h, w))
+    keep = t != -100
+    n = int(keep.sum())
+    for other in (0.0, 1.0 / n, 5.0, float("nan")):
+        g = torch.where(keep, torch.tensor(1.0 / n, device=DEV), torch.tensor(other, device=DEV))
+        got = torch.autograd.grad(_loss(h, w, t, reduction="none", piece=256), (h, w), g)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), other
+    g = torch.where(keep, torch.tensor(-1.0 / n, device=DEV), 0.0)
+    got = torch.autograd.grad(_loss(h, w, t, reduction="none", piece=256), (h, w), g)
+    assert all(torch.equal(a, -b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("size", [1e-36, 1e-3, 1e30])
+def test_gradients_of_any_size_row_by_row(size):
+    """Some of them zero; none but zeros gives zeros."""
+    h, w, t = _inputs(150, 64, 700, seed=26, ignore=0.1)
+    g = torch.randn(150, generator=torch.Generator().manual_seed(27)).to(DEV) * size
+    g[::3] = 0.0
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    rows = _loss(h, w, t, reduction="none")
+    gh, gw = torch.autograd.grad(rows, (h, w), g, retain_graph=True)
+    _, (dh, eh), (dw, ew) = _exact(h.detach(), w.detach(), t, g, "none")
+    for got, want, err, name in ((gh, dh, eh, "dh"), (gw, dw, ew, "dw")):
+        # rounded once more here; below 2^-126 half a step of bf16 is 2^-134
+        _near((got.double() / size).to(BF16), want / size, err / size + B16 * want.abs() / size + 2.0 ** -134 / size, BF16, name)
+    gh, gw = torch.autograd.grad(rows, (h, w), torch.zeros_like(g))
+    assert not gh.any() and not gw.any()
+    g[1] = float("inf")  # its own row alone
+    t1 = t.clone()
+    t1[1] = 5
+    gh, = torch.autograd.grad(_loss(h, w, t1, reduction="none"), h, g)
+    assert not torch.isfinite(gh[1]).any() and torch.isfinite(gh[2:]).all() and torch.isfinite(gh[0]).all()
