@@ -289,6 +289,9 @@ def _muon_group(group, state) -> None:
     for p in params:
         buf = state[p].get("momentum_buffer")
         if buf is None:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("Muon: momenta must exist before a step is captured (a replay would begin them at zero each "
+                                   "time): take one step first, or load a state")
             state[p]["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
     muon_update(params, [p.grad for p in params], [state[p]["momentum_buffer"] for p in params],
                 **{k: group[k] for k in ("lr", "momentum", "nesterov", "weight_decay", "steps", "eps", "coefficients", "scale")})

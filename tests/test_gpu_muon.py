@@ -310,3 +310,24 @@ def test_an_output_across_its_input(m, n, shift):
     want = _muon().orthogonalize(x[:5] if shift > 0 else x[1:])
     src, out = (x[:5], x[1:]) if shift > 0 else (x[1:], x[:5])
     assert _muon().orthogonalize(src, out=out) is out and torch.equal(out, want)
+
+
+def test_first_step_is_not_captured():
+    """Momenta made during a capture would begin at zero in every replay; made before it, replays go on like eager steps."""
+    mu = _muon()
+    p, q = (torch.nn.Parameter(_matrices(1, 40, 70, "flat")[0]) for _ in range(2))
+    p.grad = q.grad = _matrices(1, 40, 70, "lowrank")[0]
+    a, b = mu.Muon([p], lr=0.01), mu.Muon([q], lr=0.01)
+    with pytest.raises(RuntimeError, match="before a step is captured"), torch.cuda.graph(torch.cuda.CUDAGraph()):
+        a.step()
+    assert "momentum_buffer" not in a.state[p]
+    a.step()
+    b.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        b.step()
+        assert torch.equal(p, q) and torch.equal(a.state[p]["momentum_buffer"], b.state[q]["momentum_buffer"])
