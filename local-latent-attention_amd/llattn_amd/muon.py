@@ -32,7 +32,8 @@ TILES = 0  # workgroups of the products: the library's choice (llattn_muon_cfg.t
 
 
 def _config(steps, coefficients, eps, nesterov=False, mu=0.0):
-    return L.LlattnMuonCfg(0, steps, int(nesterov), TILES, *[float(v) for v in coefficients], float(eps), mu)
+    # the library takes eps in fp32, where one below 2^-149 would be none at all
+    return L.LlattnMuonCfg(0, steps, int(nesterov), TILES, *[float(v) for v in coefficients], eps and max(float(eps), 2.0 ** -149), mu)
 
 
 def _bytes(cfg, groups) -> int:

@@ -361,3 +361,10 @@ def test_an_output_across_its_input_gets_a_copy(src, out, copied):
     a, b = x[src[0]:src[1]], x[out[0]:out[1]]
     got = muon._apart(a, b)
     assert torch.equal(got, a) and (got.data_ptr() != a.data_ptr()) == copied
+
+
+@pytest.mark.parametrize("eps", [1e-46, 1e-300, 2.0 ** -149, 1e-7, 0.0])
+def test_an_eps_above_zero_stays_above_zero(eps):
+    """Rounded to fp32, in which the library takes it, it would be 0, and a zero matrix NaN instead of zero."""
+    got = muon._config(5, muon.COEFFICIENTS, eps).eps
+    assert (got > 0) == (eps > 0) and got == pytest.approx(max(eps, 2.0 ** -149) if eps else 0.0)
