@@ -33,7 +33,7 @@ TILES = 0  # workgroups of the products: the library's choice (llattn_muon_cfg.t
 
 def _config(steps, coefficients, eps, nesterov=False, mu=0.0):
     # the library takes eps in fp32, where one below 2^-149 would be none at all
-    return L.LlattnMuonCfg(0, steps, int(nesterov), TILES, *[float(v) for v in coefficients], eps and max(float(eps), 2.0 ** -149), mu)
+    return L.LlattnMuonCfg(0, int(steps), int(nesterov), TILES, *[float(v) for v in coefficients], eps and max(float(eps), 2.0 ** -149), mu)
 
 
 def _bytes(cfg, groups) -> int:
@@ -84,7 +84,7 @@ def _launch(name, cfg, groups, device, *pointers, work):
 
 
 def _check_numbers(who, steps, eps, coefficients):
-    if int(steps) != steps or steps < 1:
+    if not isinstance(steps, Real) or not 1 <= steps < 2 ** 31 or int(steps) != steps:
         raise ValueError(f"{who}: steps must be a positive whole number, got {steps}")
     if not eps >= 0:
         raise ValueError(f"{who}: eps must not be negative, got {eps}")

@@ -368,3 +368,15 @@ def test_an_eps_above_zero_stays_above_zero(eps):
     """Rounded to fp32, in which the library takes it, it would be 0, and a zero matrix NaN instead of zero."""
     got = muon._config(5, muon.COEFFICIENTS, eps).eps
     assert (got > 0) == (eps > 0) and got == pytest.approx(max(eps, 2.0 ** -149) if eps else 0.0)
+
+
+def test_whole_numbers_of_steps():
+    """A whole number of any type counts; what is none is refused as such."""
+    x = torch.zeros(3, 4)
+    assert muon._config(5.0, muon.COEFFICIENTS, 1e-7).steps == 5
+    for steps in (5, 5.0):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            muon.orthogonalize(x, steps=steps)
+    for steps in (float("inf"), float("nan"), 2 ** 32 + 5, None, "5"):
+        with pytest.raises(ValueError, match="steps"):
+            muon.orthogonalize(x, steps=steps)
