@@ -331,3 +331,96 @@ def test_first_step_is_not_captured():
         torch.cuda.synchronize()
         b.step()
         assert torch.equal(p, q) and torch.equal(a.state[p]["momentum_buffer"], b.state[q]["momentum_buffer"])
+
+
+# ---- to fp32's own error ----------------------------------------------------------------------------------------------
+# The bound above adds worst cases and lets pass what loses half of the bits at small sizes.  Here the result is held to
+# twice the sum of the errors that fp32 products have and that the scheme of two halves has (emulated below with exact
+# sums), with a floor: a step rounds X, A and B to fp32 (2^-24 each) whatever its sums, and the steps behind multiply a
+# relative error of a singular value s by |s p'(s) / p(s)| each; over all s in [0, 1] and five steps the products of those
+# factors add up to 27.2 at most, so 3 * 27.2 * 2^-24 of the result.
+FLOOR = 82 * 2.0 ** -24
+
+
+def _emulated(x, lo=True, steps=5, eps=1e-7, coef=COEF):
+    """The iteration on two fp16 halves of X, A and B (lo False: on the upper ones alone), sums in 64 bits."""
+    a, b, c = coef
+    flip = x.shape[-2] > x.shape[-1]
+    x = (x.mT if flip else x).double()
+    m, n = x.shape[-2:]
+    s = 2.0 ** min(14, int(0.5 * math.log2(m * n)))
+
+    def halves(v):
+        h = v.float().half().double()
+        return h, (v.float().double() - h).half().double() if lo else torch.zeros_like(h)
+
+    def times(p, q):
+        return p[0] @ q[0] + p[0] @ q[1] + p[1] @ q[0]
+
+    def flipped(p):
+        return [v.mT.contiguous() for v in p]
+
+    x = halves(s * x / (torch.linalg.matrix_norm(x)[..., None, None] + eps))
+    for _ in range(steps):
+        g = halves(4096.0 / s ** 2 * times(x, flipped(x)))
+        q = halves(b * (g[0] + g[1]) + c / 4096.0 * times(g, flipped(g)))
+        new = a * (x[0] + x[1]) + times(q, x) / 4096.0
+        x = halves(new)
+    out = (new / s).float()
+    return out.mT.contiguous() if flip else out
+
+
+def _errors(u32, want):
+    """|error| against ``want`` (float64) allowed to the iteration on ``u32``."""
+    norm = torch.linalg.matrix_norm
+    return 2 * (norm(_emulated(u32).double() - want) + norm(_ns(u32).double() - want)) + FLOOR * norm(want)
+
+
+@pytest.mark.parametrize("batch,m,n", [(4, 64, 128), (3, 65, 63), (3, 128, 64), (2, 100, 300), (2, 129, 1000), (2, 40, 70), (1, 64, 448),
+                                       (2, 448, 64), (2, 64, 449), (2, 449, 64), (1, 65, 448), (3, 20, 448), (1, 33, 4100), (2, 250, 255)])
+@pytest.mark.parametrize("kind", ["flat", "decay", "lowrank"])
+def test_as_exact_as_fp32(batch, m, n, kind):
+    """At small sizes too, and at both sides of where one workgroup takes a matrix (64 rows, 448 columns)."""
+    x = _matrices(batch, m, n, kind, seed=m * n)
+    want = _ns(x.double())
+    got, most = torch.linalg.matrix_norm(_muon().orthogonalize(x).double() - want), _errors(x, want)
+    print(f"{batch}x{m}x{n} {kind}: {float((got / most).max()):.3f} of the bound", flush=True)
+    assert bool((got <= most).all())
+    if kind == "flat":  # what the upper halves alone give is outside
+        assert bool((torch.linalg.matrix_norm(_emulated(x, lo=False).double() - want) > 10 * most).all())
+
+
+TILED = [(130, 200), (200, 130), (333, 70), (257, 514), (96, 450), (130, 200), (65, 64), (451, 33)]
+
+
+@pytest.mark.parametrize("tiles", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("wt,gt", [(F32, F32), (BF16, BF16), (F32, BF16), (BF16, F32)])
+def test_updates_of_matrices_over_many_workgroups(tiles, nesterov, wt, gt, monkeypatch):
+    """Shapes mixed in one call, none of which one workgroup takes alone: weights, momenta and decay by value, into buffers
+    of their own and in place."""
+    mu = _muon()
+    monkeypatch.setattr(mu, "TILES", tiles)
+    lr, beta, wd = 0.03, 0.9, 2.0
+    ws = [_matrices(1, *s, "flat", i)[0].mul(0.05).to(wt) for i, s in enumerate(TILED)]
+    gs = [_matrices(1, *s, "lowrank", i + 50)[0].to(gt) for i, s in enumerate(TILED)]
+    ms = [_matrices(1, *s, "decay", i + 90)[0] for i, s in enumerate(TILED)]
+    out = ([torch.full_like(w, 9.0) for w in ws], [torch.full_like(m, 9.0) for m in ms])
+    kw = dict(lr=lr, momentum=beta, nesterov=nesterov, weight_decay=wd)
+    mu.muon_update(ws, gs, ms, out=out, **kw)
+    for w, g, m, nw, nm in zip(ws, gs, ms, *out):
+        m32 = beta * m + (1 - beta) * g.float()
+        m64 = beta * m.double() + (1 - beta) * g.double()
+        u32 = (1 - beta) * g.float() + beta * m32 if nesterov else m32
+        u64 = (1 - beta) * g.double() + beta * m64 if nesterov else m64
+        assert bool(((nm.double() - m64).abs() <= 2.0 ** -22 * (m.abs() + g.abs()).double()).all())
+        o, s = _ns(u64), math.sqrt(max(1.0, w.shape[0] / w.shape[1]))
+        want = (1 - lr * wd) * w.double() - lr * s * o
+        # the products' and the sum's roundings in fp32, and the one to the weight's type
+        most = lr * s * float(_errors(u32, o)) + 2.0 ** -22 * float(w.double().norm() + lr * s * o.norm()) \
+            + torch.finfo(wt).eps / 2 * float(want.norm())
+        off = float((nw.double() - want).norm())
+        assert off <= most, (tuple(w.shape), off, most)
+        assert lr * wd * float(w.double().norm()) > 5 * most  # a decay or a weight that is not this one's would show
+    mu.muon_update(ws, gs, ms, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(ws + ms, out[0] + out[1]))
