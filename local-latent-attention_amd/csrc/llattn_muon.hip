@@ -7,8 +7,9 @@
 // roundings of X, A and B leave there: bf16 matrices (half a step of 2^-8) leave order-1 errors in directions that a
 // gradient hardly has, fp32 ones nothing.  Matrices are held as hi + lo, two fp16 halves (22 bits), and a product as
 // hi hi + hi lo + lo hi on the fp16 matrix cores with fp32 accumulation: what is left out, lo lo, is 2^-22 of it.
-// Against float64 that is as exact as fp32 products are (64 x 64 to 1408 x 1408, flat, decaying and low-rank spectra:
-// within 2% of fp32's own error; two bf16 halves: 10 to 20 times that), at a third of the 16-bit rate, five times the
+// Against float64 that is as exact as fp32 products are from 64 rows on (64 x 64 to 1408 x 1408, flat, decaying and low-rank
+// spectra: within 2% of fp32's own error, below it from 100 on; two bf16 halves: 10 to 20 times that) and 1.2 times
+// as far off down to 17 rows (fewer: ns_thin_kernel), at a third of the 16-bit rate, five times the
 // fp32 one.  Scales are powers of two: X is held times S_X ~ sqrt(m n) (its entries average 1 / sqrt(m n)), A and B times
 // 2^12 (their entries are at most a few).
 //
@@ -923,6 +924,120 @@ __global__ __launch_bounds__(256) void ns_small_kernel(const SmallArgs a) {
   }
 }
 
+// ---- thin matrices: the iteration on the smaller side's Gram matrix, in 64 bits -----------------------------------------
+// Up to kThin rows of X (the smaller side), any number of columns.  Sums over so few rows are short, and what fp32 products
+// round is then less than what the halves do: 82 x 1 was off by 2.3e-6 and fp32 by 3.3e-7, sides of 1 to 10 by 1.5 to 3
+// times fp32's; from 17 to 32 by 1.2 times (500 matrices: 1.6 at most), from 33 on 1.1.  X after the steps is Q X0 with
+//   A = X0 X0ᵀ,  P = a + b A + c A A,  Q <- P Q,  A <- P A P        (steps times)
+// so X is read twice and written once, and all else is a 16 x 16 matrix: with fp64 products what is left is one rounding.
+// One workgroup a matrix, 16 waves: bound by the latency of their loads.  Against the products on halves, a call: 16 x 448 at
+// most 20 us (the host's) and 72, 16 x 4096 58 and 164, 16 x 32768 409 and 799, 128 of 16 x 4096 128 and 557.
+constexpr int kThin = 16;
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+__global__ __launch_bounds__(1024) void ns_thin_kernel(const SmallArgs a) {
+  __shared__ double part[16][256];
+  __shared__ double A[16][17], P[16][17], Q[16][17], T[16][17];
+  int gi = 0;
+  while (gi + 1 < a.n_groups && (int)blockIdx.x >= a.grp[gi + 1].first) ++gi;
+  const SmallGroup& G = a.grp[gi];
+  const int id = blockIdx.x, tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4, wave = tid >> 6;
+  const bool flip = G.rows > G.cols;
+  const int m = flip ? G.cols : G.rows, n = flip ? G.rows : G.cols;
+  const auto at = [&](int row, int col) { return flip ? col * m + row : row * n + col; };  // of X: at most 16 x 32768
+  const void* gp = a.g[id];
+  // A lane gives row r, columns k0 + 4 e + g: as both operands, X Xᵀ.  Each element is one lane's, which updates its momentum.
+  f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+  for (int k0 = 16 * wave; k0 < n; k0 += 256) {
+    double u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int k = k0 + 4 * e + g;
+      float v = 0.f;
+      if (r < m && k < n) {
+        const int i = at(r, k);
+        v = load_as(gp, i, G.g_dtype);
+        if (a.update) {
+          const float mo = fmaf(a.mu, a.m[id][i], a.one_mu * v);
+          a.m_out[id][i] = mo;
+          v = direction(v, mo, a.mu, a.one_mu, a.nesterov);
+        }
+      }
+      u[e] = (double)v;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(u[e], u[e], acc, 0, 0, 0);
+  }
+#pragma unroll
+  for (int v = 0; v < 4; ++v) part[wave][(4 * v + g) * 16 + r] = acc[v];  // lane (r, g): rows 4 v + g of column r
+  __syncthreads();
+  const int i = tid >> 4 & 15, j = tid & 15;
+  const bool mine = tid < 256;
+  if (mine) {
+    double s = 0.0;
+    for (int w = 0; w < 16; ++w) s += part[w][tid];
+    T[i][j] = s;
+  }
+  __syncthreads();
+  double f = 0.0;
+  if (mine) {
+    double s = 0.0;
+    for (int d = 0; d < 16; ++d) s += T[d][d];  // |U|^2
+    f = 1.0 / (sqrt(s) + (double)a.eps);
+    A[i][j] = T[i][j] * f * f;
+    Q[i][j] = i == j ? f : 0.0;
+  }
+  __syncthreads();
+  const auto dot = [&](const double (&x)[16][17], const double (&y)[16][17]) {
+    double s = 0.0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s = fma(x[i][k], y[k][j], s);
+    return s;
+  };
+  for (int step = 0; step < a.steps; ++step) {
+    if (mine) P[i][j] = fma((double)a.c, dot(A, A), (double)a.b * A[i][j]) + (i == j ? (double)a.a : 0.0);
+    __syncthreads();
+    double q = 0.0;
+    if (mine) {
+      q = dot(P, Q);
+      T[i][j] = dot(P, A);
+    }
+    __syncthreads();
+    if (mine) {
+      Q[i][j] = q;
+      A[i][j] = dot(T, P);
+    }
+    __syncthreads();
+  }
+  double qf[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) qf[s] = Q[r][4 * s + g];
+  // 16 columns at a time, all read before any is written
+  for (int c0 = 16 * wave; c0 < n; c0 += 256) {
+    const int k = c0 + r;
+    f64x4 y = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      float v = 0.f;
+      if (4 * s + g < m && k < n) {
+        const int e = at(4 * s + g, k);
+        v = load_as(gp, e, G.g_dtype);
+        if (a.update) v = direction(v, a.m_out[id][e], a.mu, a.one_mu, a.nesterov);
+      }
+      y = __builtin_amdgcn_mfma_f64_16x16x4f64(qf[s], (double)v, y, 0, 0, 0);
+    }
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      if (4 * v + g >= m || k >= n) continue;
+      const int e = at(4 * v + g, k);
+      float x = (float)y[v];
+      if (a.update) x = fmaf(-G.step, x, G.keep * load_as(a.w[id], e, G.w_dtype));
+      if (G.w_dtype == LLATTN_F32) static_cast<float*>(a.out[id])[e] = x;
+      else static_cast<uint16_t*>(a.out[id])[e] = f2bf(x);
+    }
+  }
+}
+
 // ---- host -----------------------------------------------------------------------------
 constexpr size_t up(size_t n) { return (n + 255) & ~size_t(255); }
 
@@ -1138,6 +1253,8 @@ void launch_products(const Call& k, LastArgs& a) {
   launch_kind<MODE>(kind, a, blocks, k.st);
 }
 
+bool thin(const llattn_muon_group& g) { return std::min(g.rows, g.cols) <= kThin; }
+
 // All of the call in one workgroup a matrix (ns_small_kernel), where every matrix fits.
 bool all_small(const llattn_muon_cfg* c, const Plan& p) {
   if (c->tiles) return false;
@@ -1146,15 +1263,18 @@ bool all_small(const llattn_muon_cfg* c, const Plan& p) {
   return true;
 }
 
-int32_t run_small(const char* who, const llattn_muon_cfg* c, const llattn_muon_group* groups, const Plan& p, const void* const* g,
-                  const float* const* m, const void* const* w, float* const* m_out, void* const* out, bool update, hipStream_t st) {
+// One workgroup a matrix: ns_small_kernel or ns_thin_kernel.
+int32_t run_single(const char* who, const llattn_muon_cfg* c, const llattn_muon_group* groups, const Plan& p, const void* const* g,
+                   const float* const* m, const void* const* w, float* const* m_out, void* const* out, bool update, bool thin,
+                   hipStream_t st) {
   SmallArgs a{};
   a.update = update; a.nesterov = c->nesterov; a.steps = c->steps;
   a.mu = c->mu; a.one_mu = (float)(1.0 - (double)c->mu); a.eps = c->eps;
   a.a = c->a; a.b = c->b; a.c = c->c;
   int np = 0, held = 0;
   const auto launch = [&]() {
-    hipLaunchKernelGGL(ns_small_kernel, dim3(held), dim3(256), 32768 + (size_t)np * 256, st, a);
+    if (thin) hipLaunchKernelGGL(ns_thin_kernel, dim3(held), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL(ns_small_kernel, dim3(held), dim3(256), 32768 + (size_t)np * 256, st, a);
     a.n_groups = held = np = 0;
   };
   for (int i = 0; i < c->n_groups; ++i) {
@@ -1180,16 +1300,14 @@ int32_t run_small(const char* who, const llattn_muon_cfg* c, const llattn_muon_g
   return check_launch(who);
 }
 
-int32_t run(const char* who, const llattn_muon_cfg* c, const llattn_muon_group* groups, const void* const* g,
-            const float* const* m, const void* const* w, float* const* m_out, void* const* out, void* workspace,
-            size_t workspace_bytes, hipStream_t st) {
-  if (const int32_t rc = check(c, groups)) return rc;
-  Call k{c, groups, plan_of(c, groups), st, {}, nullptr, nullptr, m != nullptr, {}};
+// The launches of matrices that need not be thin; k.p is their plan.
+int32_t run_chain(const char* who, Call& k, const void* const* g, const float* const* m, const void* const* w, float* const* m_out,
+                  void* const* out, void* workspace) {
+  const llattn_muon_cfg* c = k.c;
+  const llattn_muon_group* groups = k.groups;
   const Plan& p = k.p;
-  if (!workspace || workspace_bytes < p.bytes() || !aligned16(workspace))
-    return fail(LLATTN_ERR_WORKSPACE, "%s: needs %zu workspace bytes (got %zu)", who, p.bytes(), workspace_bytes);
-  if (!g || !out || (k.update && (!w || !m_out))) return fail(LLATTN_ERR_LAYOUT, "%s: null pointer array", who);
-  const auto misplaced = [](const void* q, int dtype) { return !q || (uintptr_t)q % (size_t)elem_size(dtype); };
+  const hipStream_t st = k.st;
+  if (all_small(c, p)) return run_single(who, c, groups, p, g, m, w, m_out, out, k.update, false, st);
   char* ws = static_cast<char*>(workspace);
   k.X[0] = reinterpret_cast<uint16_t*>(ws);
   k.X[1] = reinterpret_cast<uint16_t*>(ws + p.x);
@@ -1211,9 +1329,6 @@ int32_t run(const char* who, const llattn_muon_cfg* c, const llattn_muon_group* 
   for (int i = 0; i < c->n_groups; ++i) {
     const GroupPlan& q = p.g[i];
     for (int b = q.first; b < q.first + groups[i].batch; ++b) {
-      if (misplaced(g[b], groups[i].g_dtype) || misplaced(out[b], groups[i].w_dtype) ||
-          (k.update && (misplaced(m[b], LLATTN_F32) || misplaced(m_out[b], LLATTN_F32) || misplaced(w[b], groups[i].w_dtype))))
-        return fail(LLATTN_ERR_LAYOUT, "%s: matrix %d has a null or misaligned pointer", who, b);
       e.g.p[b] = g[b];
       na.out.p[b] = out[b];
       if (!k.update) continue;
@@ -1231,7 +1346,6 @@ int32_t run(const char* who, const llattn_muon_cfg* c, const llattn_muon_group* 
     t.part0 = q.part0;
     blocks += groups[i].batch * q.parts;
   }
-  if (all_small(c, p)) return run_small(who, c, groups, p, g, m, w, m_out, out, k.update, st);
   k.kind[GRAM] = choose<true>(c, groups, p, true);
   k.kind[POLY] = choose<true>(c, groups, p, false);
   k.kind[APPLY] = choose<false>(c, groups, p, false);
@@ -1257,6 +1371,62 @@ int32_t run(const char* who, const llattn_muon_cfg* c, const llattn_muon_group* 
     else launch_products<LAST>(k, na);
   }
   return check_launch(who);
+}
+
+// A part of a call's matrices.
+struct Part {
+  llattn_muon_cfg c;
+  llattn_muon_group groups[LLATTN_MUON_GROUPS];
+  const void* g[LLATTN_MUON_BATCH];
+  const float* m[LLATTN_MUON_BATCH];
+  const void* w[LLATTN_MUON_BATCH];
+  float* m_out[LLATTN_MUON_BATCH];
+  void* out[LLATTN_MUON_BATCH];
+};
+
+int32_t run(const char* who, const llattn_muon_cfg* c, const llattn_muon_group* groups, const void* const* g,
+            const float* const* m, const void* const* w, float* const* m_out, void* const* out, void* workspace,
+            size_t workspace_bytes, hipStream_t st) {
+  if (const int32_t rc = check(c, groups)) return rc;
+  Call k{c, groups, plan_of(c, groups), st, {}, nullptr, nullptr, m != nullptr, {}};
+  if (!workspace || workspace_bytes < k.p.bytes() || !aligned16(workspace))
+    return fail(LLATTN_ERR_WORKSPACE, "%s: needs %zu workspace bytes (got %zu)", who, k.p.bytes(), workspace_bytes);
+  if (!g || !out || (k.update && (!w || !m_out))) return fail(LLATTN_ERR_LAYOUT, "%s: null pointer array", who);
+  const auto misplaced = [](const void* q, int dtype) { return !q || (uintptr_t)q % (size_t)elem_size(dtype); };
+  int thin_groups = 0;
+  for (int i = 0; i < c->n_groups; ++i) {
+    thin_groups += thin(groups[i]);
+    for (int b = k.p.g[i].first; b < k.p.g[i].first + groups[i].batch; ++b)
+      if (misplaced(g[b], groups[i].g_dtype) || misplaced(out[b], groups[i].w_dtype) ||
+          (k.update && (misplaced(m[b], LLATTN_F32) || misplaced(m_out[b], LLATTN_F32) || misplaced(w[b], groups[i].w_dtype))))
+        return fail(LLATTN_ERR_LAYOUT, "%s: matrix %d has a null or misaligned pointer", who, b);
+  }
+  if (c->tiles || !thin_groups) return run_chain(who, k, g, m, w, m_out, out, workspace);
+  if (thin_groups == c->n_groups) return run_single(who, c, groups, k.p, g, m, w, m_out, out, k.update, true, st);
+  // both: each with its own launches
+  for (const bool want : {true, false}) {
+    Part q{};
+    q.c = *c;
+    q.c.n_groups = 0;
+    int held = 0;
+    for (int i = 0; i < c->n_groups; ++i) {
+      if (thin(groups[i]) != want) continue;
+      q.groups[q.c.n_groups++] = groups[i];
+      for (int b = k.p.g[i].first; b < k.p.g[i].first + groups[i].batch; ++b, ++held) {
+        q.g[held] = g[b];
+        q.out[held] = out[b];
+        if (!k.update) continue;
+        q.m[held] = m[b];
+        q.w[held] = w[b];
+        q.m_out[held] = m_out[b];
+      }
+    }
+    Call part{&q.c, q.groups, plan_of(&q.c, q.groups), st, {}, nullptr, nullptr, k.update, {}};
+    const int32_t rc = want ? run_single(who, &q.c, q.groups, part.p, q.g, q.m, q.w, q.m_out, q.out, k.update, true, st)
+                            : run_chain(who, part, q.g, q.m, q.w, q.m_out, q.out, workspace);
+    if (rc) return rc;
+  }
+  return LLATTN_OK;
 }
 
 }  // namespace

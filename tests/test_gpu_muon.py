@@ -424,3 +424,71 @@ def test_updates_of_matrices_over_many_workgroups(tiles, nesterov, wt, gt, monke
         assert lr * wd * float(w.double().norm()) > 5 * most  # a decay or a weight that is not this one's would show
     mu.muon_update(ws, gs, ms, **kw)
     assert all(torch.equal(a, b) for a, b in zip(ws + ms, out[0] + out[1]))
+
+
+# The library takes the coefficients in fp32.  Off by up to 2^-25 of themselves, they move a singular value by up to 27.2
+# times that over the steps (see FLOOR), more than the one rounding that the results below are held to.
+COEF32 = tuple(float(torch.tensor(c)) for c in COEF)
+
+THIN = [(5, 1, 1), (3, 1, 29), (1, 82, 1), (2, 2, 3), (9, 3079, 1), (4, 5, 448), (2, 5, 4096), (70, 6, 262), (1, 9, 17), (2, 15, 16),
+        (3, 16, 16), (2, 16, 1000), (1, 16, 32768), (1, 32768, 13), (2, 255, 16), (2, 257, 7)]
+
+
+@pytest.mark.parametrize("batch,m,n", THIN)
+@pytest.mark.parametrize("kind", ["flat", "decay", "lowrank"])
+def test_thin_matrices_are_rounded_once(batch, m, n, kind):
+    """A smaller side of up to 16 is taken in 64 bits: half a step of the result's type, and next to nothing besides."""
+    x = _matrices(batch, m, n, kind, seed=m + 3 * n)
+    for v in (x, x.to(BF16)):
+        want = _ns(v.double(), coef=COEF32)
+        norm = torch.linalg.matrix_norm(want)
+        off = torch.linalg.matrix_norm(_muon().orthogonalize(v).double() - want)
+        assert bool((off <= 1.01 * torch.finfo(v.dtype).eps / 2 * norm).all()), (off / norm).max()
+
+
+def test_thin_matrices_beside_others():
+    """Small, thin and large ones in one call, weights by value and in place; each has the bits that it has by itself."""
+    mu = _muon()
+    shapes = [(130, 200), (7, 300), (40, 70), (300, 7), (1, 9), (130, 200), (7, 300), (16, 17), (20, 17)]
+    for types in ((F32, F32), (BF16, F32), (F32, BF16)):
+        ws = [_matrices(1, *s, "flat", i)[0].mul(0.05).to(types[0]) for i, s in enumerate(shapes)]
+        gs = [_matrices(1, *s, "flat", i + 50)[0].to(types[1]) for i, s in enumerate(shapes)]
+        ms = [_matrices(1, *s, "flat", i + 90)[0] for i, s in enumerate(shapes)]
+        out = ([torch.full_like(w, 9.0) for w in ws], [torch.full_like(m, 9.0) for m in ms])
+        kw = dict(lr=0.03, momentum=0.9, weight_decay=2.0)
+        mu.muon_update(ws, gs, ms, out=out, **kw)
+        for w, g, m, nw, nm in zip(ws, gs, ms, *out):
+            w64, m64 = _plain_update(w, g, m, 0.03, 0.9, True, 2.0, "aspect", torch.float64)
+            assert bool(((nm.double() - m64).abs() <= 2.0 ** -22 * (m.abs() + g.abs()).double()).all())
+            u = 0.1 * g.float() + 0.9 * (0.9 * m + 0.1 * g.float())
+            o = _ns(0.1 * g.double() + 0.9 * m64)
+            s = math.sqrt(max(1.0, w.shape[0] / w.shape[1]))
+            most = 0.03 * s * float(_errors(u, o)) + 2.0 ** -22 * float(w.double().norm() + 0.03 * s * o.norm())
+            assert float((nw.double() - w64).norm()) <= most + torch.finfo(types[0]).eps / 2 * float(w64.norm()), tuple(w.shape)
+            if min(w.shape) <= 16:
+                one = [w.clone()], [m.clone()]
+                mu.muon_update(one[0], [g], one[1], **kw)
+                assert torch.equal(one[0][0], nw) and torch.equal(one[1][0], nm)
+        mu.muon_update(ws, gs, ms, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(ws + ms, out[0] + out[1]))
+
+
+def test_thin_matrices_of_any_values_and_places():
+    mu = _muon()
+    x = _matrices(5, 6, 50, "flat")
+    x[0] = 0.0
+    x[2, 3, 4] = float("inf")
+    x[3, 1, 1] = float("nan")
+    want = _ns(x[[1, 4]].double(), coef=COEF32)
+    got = mu.orthogonalize(x)
+    assert not got[0].any() and torch.isnan(got[2]).all() and torch.isnan(got[3]).all()
+    assert bool((torch.linalg.matrix_norm(got[[1, 4]].double() - want) <= 1.01 * 2.0 ** -24 * torch.linalg.matrix_norm(want)).all())
+    y = x[[1, 4]]
+    got = got[[1, 4]]
+    shifted = torch.zeros(y.numel() + 1, device=DEV)[1:].view_as(y).copy_(y)
+    assert torch.equal(mu.orthogonalize(shifted), got) and torch.equal(mu.orthogonalize(y.mT).mT, got)
+    assert mu.orthogonalize(shifted, out=shifted) is shifted and torch.equal(shifted, got)
+    big, small = (y.double() * 1e30).float(), (y.double() * 1e-30).float()
+    assert float((mu.orthogonalize(big).double() - _ns(big.double(), coef=COEF32)).norm()) <= 1.01 * 2.0 ** -24 * float(want.norm())
+    far = _ns(small.double(), coef=COEF32)
+    assert float((mu.orthogonalize(small).double() - far).norm()) <= 1.01 * 2.0 ** -24 * float(far.norm())
