@@ -83,3 +83,23 @@ def test_training_steps_with_both():
             # the bound of the orthogonalisation at these sizes (5 steps, at most 96 columns) is below 0.1 of the step
             assert float((p.detach().double() - want).norm()) <= 0.1 * float(step.norm()) + 2.0 ** -22 * float(w.norm())
     assert all(opt.state[p]["momentum_buffer"].dtype is torch.float32 for p in mats)
+
+
+@pytest.mark.parametrize("transform", ["jvp", "vmap", "dual"])
+def test_what_no_autograd_function_stands_around_refuses_transforms(transform):
+    """Batched inputs and forward-mode tangents raise instead of being dropped, also where nothing needs a gradient."""
+    from llattn_amd import muon_update, orthogonalize, piecewise_head_loss
+    fw = torch.autograd.forward_ad
+    h, w = torch.randn(5, 16, device=DEV).bfloat16(), torch.randn(50, 16, device=DEV).bfloat16()
+    t, x = torch.zeros(5, dtype=torch.int64, device=DEV), torch.randn(6, 9, device=DEV)
+    for fn, arg in ((lambda v: piecewise_head_loss(v, w, t, reduction="sum"), h), (lambda v: piecewise_head_loss(h, v, t), w),
+                    (orthogonalize, x), (lambda v: muon_update([x.clone()], [v], [x.clone()], lr=0.1), x)):
+        fn(arg)
+        with pytest.raises((RuntimeError, ValueError, NotImplementedError)):
+            if transform == "jvp":
+                torch.func.jvp(fn, (arg,), (torch.ones_like(arg),))
+            elif transform == "vmap":
+                torch.func.vmap(fn)(arg[None])
+            else:
+                with fw.dual_level():
+                    fn(fw.make_dual(arg, torch.ones_like(arg)))
