@@ -715,9 +715,12 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W * S::KG / 4) void ns_last_ke
 // ---- small matrices: the whole call in one workgroup each ---------------------------------------------------------------
 // Up to 64 rows of X (the smaller side) and kSmallCols columns: X, A and B stay in LDS, as blocks of 32 columns (64 rows
 // of 128 bytes, chunk c of row o at c ^ (o & 7)).  The chain of 2 + 3 steps launches that it replaces waits for launches
-// and for its own tail 15 times: 4 x 64 x 128 in 79 us, here 40: latency of LDS reads and barriers, 15 dependent products.
+// and for its own tail 15 times; here it is the latency of LDS reads and barriers of 15 dependent products, which grows
+// with the columns and with launches one behind the other.  A call in us, here and by the chain's best tiles:
+//   4 of 64 x 64: 24, 70   x 128: 40, 73   x 256: 70, 78   x 448: 115, 84     128 of 64 x 128: 82, 86   x 448: 234, 120
+// so up to kSmallCols columns times launches.
 constexpr int kSmall = 64;         // matrices a launch
-constexpr int kSmallCols = 448;    // X: 112 KB of LDS beside 32 KB for A and B
+constexpr int kSmallCols = 256;    // X: 64 KB of LDS beside 32 KB for A and B
 
 struct SmallGroup {
   int first, rows, cols, np, g_dtype, w_dtype;
@@ -1255,11 +1258,12 @@ void launch_products(const Call& k, LastArgs& a) {
 
 bool thin(const llattn_muon_group& g) { return std::min(g.rows, g.cols) <= kThin; }
 
-// All of the call in one workgroup a matrix (ns_small_kernel), where every matrix fits.
+// All of the call in one workgroup a matrix (ns_small_kernel), where every matrix fits and its launches are the quicker ones.
 bool all_small(const llattn_muon_cfg* c, const Plan& p) {
   if (c->tiles) return false;
+  const int launches = (p.matrices + kSmall - 1) / kSmall;
   for (int i = 0; i < c->n_groups; ++i)
-    if (p.g[i].mp > 64 || p.g[i].np > kSmallCols) return false;
+    if (p.g[i].mp > 64 || p.g[i].np * launches > kSmallCols) return false;
   return true;
 }
 

@@ -492,3 +492,12 @@ def test_thin_matrices_of_any_values_and_places():
     assert float((mu.orthogonalize(big).double() - _ns(big.double(), coef=COEF32)).norm()) <= 1.01 * 2.0 ** -24 * float(want.norm())
     far = _ns(small.double(), coef=COEF32)
     assert float((mu.orthogonalize(small).double() - far).norm()) <= 1.01 * 2.0 ** -24 * float(far.norm())
+
+
+@pytest.mark.parametrize("batch,m,n", [(4, 64, 256), (4, 64, 257), (64, 33, 256), (65, 33, 128), (65, 33, 129), (128, 128, 64), (129, 64, 65)])
+def test_where_matrices_go_to_one_workgroup_each(batch, m, n):
+    """Both sides of the limits: 64 rows, 256 columns, 64 matrices a launch."""
+    x = _matrices(batch, m, n, "decay", seed=batch)
+    want = _ns(x.double())
+    off = torch.linalg.matrix_norm(_muon().orthogonalize(x).double() - want)
+    assert bool((off <= _errors(x, want)).all())
