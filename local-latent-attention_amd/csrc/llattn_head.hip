@@ -11,8 +11,10 @@
 // difference first.
 //
 // Backward: a piece of the vocabulary at a time, the same product again with q = softmax - onehot (bf16) in its epilogue,
-// then dh (+)= q W and dW = qᵀ h, times the scale that every row shares.  Rounding q to bf16 is as far off as rounding the
-// results to bf16 is (half a step of 2^-8 each), and those errors average out over the contraction.  The shared scale stays
+// then dh (+)= q W and dW = qᵀ h, times the scale that every row shares.  q is bf16 because the matrix cores take 16 bits: off
+// by half a step of 2^-8 of each entry, which averages out over the contraction.  What it leaves, with dW in fp32: 5e-5 of dW at
+// 333 x 1408 x 50256, 1.7e-4 at 4096 x 256 x 8000, 1.5e-3 where single entries make up a row (333 x 128 x 512); results in
+// bf16 are off by 1.7e-3 from their own rounding (2.2e-3 in the last case).  The shared scale stays
 // out of q: within it, the entries near -1, which are one value in all rows, would round alike (1 / 4096 rows: 0.4% of
 // the whole gradient).  Gradients row by row are divided by the largest of them, which is shared in the same way: rows
 // of one gradient (a mean taken outside) then round as if there were none.  Their ratios to it are multiplied in.
@@ -156,7 +158,7 @@ struct BlockOp : ColOp<T, W> {
 // Offsets are taken from the tile's first row and step, so operands may be of any size.
 //
 // The logits' products take tile after tile (2048 x 1408 x 131072: 614 us, so 583); the gradients' one tile a workgroup
-// (131 steps a tile: the longer loop cost 586 -> 636 us a piece of 8192 x 1536 x 32768).
+// (128 steps a tile of dW: the longer loop cost 586 -> 636 us a piece of 8192 x 1536 x 32768).
 //
 // Measured, 8192 rows, D 1536: l of 131072 columns 2420 us (1360 TFLOP/s), a piece of 32768 of them: q 683 us (1210; it
 // writes 537 MB), dh 630 us (1310) and 680 where it adds to the piece's before, dW 604 us (1370).  256 x 256 tiles: matrix
@@ -679,7 +681,26 @@ typedef Shape<2, 4, 2, 2, 3> ThinShape;
 typedef Shape<4, 4, 2, 2, 2> SquareShape;
 typedef Shape<4, 8, 4, 2, 2> BigShape;
 constexpr int kTm[KINDS] = {64, 128, 256}, kTn[KINDS] = {128, 128, 256}, kPerCu[KINDS] = {2, 2, 1};
-// us of a 64-k step of a workgroup with 1 or 2 of them on a CU, and of a tile beside its steps
+// us of a 64-k step of a workgroup with 1 or 2 of them on a CU, and of a tile beside its steps.  Products alone, us (taken: *;
+// S: splits):
+//                            64 x 128   128 x 128                256 x 256
+//   64 x 128 x 509       l     5.2 *      6.2                      9.4
+//   512 x 256 x 4000     l     6.0        7.2 *                   12.5     (64 x 128 is for up to 64 rows)
+//                        dh               35 S 1, 13 S 4           71 S 1  (* 128, S 13)
+//                        dW               7.4 *                   15.0
+//   333 x 1408 x 50257   l    71.8       55.4 *                   65.4
+//                        dh              118 S 4, 68 S 8, 50 S 15 * 222 S 4, 120 S 8
+//                        dW              75.4                     76.2 *
+//   2048 x 1408 x 131072 l               753                      583 *
+//   4096 x 1408 x 32000  l               331                      293 *
+//                        q               416                      306 *
+//                        dh              413 S 1                  605 S 1, 334 S 2, 488 S 3, 355 S 5 *
+//                        dW              342                      317 *
+//   8192 x 1536 x 32768  l               719                      622 *
+//                        q               844                      654 *
+//                        dh              878 S 1                  698 S 1, 749 S 2, 620 S 4 *
+//                        dW              739                      623 *
+// The model misses the best by 6% in dh of 4096 x 1408 x 32000 and by 1 us at 512 rows.
 constexpr double kStep[KINDS][2] = {{0.45, 0.60}, {0.60, 1.00}, {1.55, 1.55}};
 constexpr double kTile[KINDS] = {5.0, 6.0, 10.0};
 

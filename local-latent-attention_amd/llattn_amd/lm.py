@@ -210,7 +210,10 @@ class LocalLatentLM(nn.Module):
         """:func:`lm_loss` of ``self(input_ids)`` without the ``[B*T, V]`` logits: the tied head and the cross
         entropy run in row chunks on the gfx950 kernels (:func:`~llattn_amd.xent.lm_head_loss`), or with
         ``vocab_piece`` in pieces of that many columns of a vocabulary of any size (0: chosen from the sizes;
-        :func:`~llattn_amd.xent.piecewise_head_loss`)."""
+        :func:`~llattn_amd.xent.piecewise_head_loss`).  Without it vocabularies above 65536 or not a multiple of 8 form the
+        full logits, as the reference does.  Up to 65536 the chunks keep the logits and save a product: 2.4 ms a step at
+        8192 x 1408 x 32000 against 2.5; pieces are quicker for few rows (333: 0.26 against 0.36 ms) and forward alone
+        (0.62 against 0.80 ms at 8192), and their gradients nearer to the exact ones."""
         from .xent import head_supported, lm_head_loss, piecewise_head_loss
         if vocab_piece is not None:
             loss, pred = piecewise_head_loss(self.hidden(input_ids), self.lm_head.weight, targets, return_pred=True,

@@ -6,8 +6,8 @@ of matrices; :func:`muon_update` is one step of the Muon optimiser on a list of 
 decay and update), and :class:`Muon` / :class:`MuonAdamW` are the optimisers made of it
 (:func:`llattn_amd.lm.make_optimizer` builds the second for the language model).
 
-The iteration runs at fp32's precision whatever the tensors' type: its matrices are held as two fp16 halves and
-multiplied on the fp16 matrix cores.
+The iteration runs at about fp32's precision whatever the tensors' type: its matrices are held as two fp16 halves and
+multiplied on the fp16 matrix cores; those of at most 16 rows or columns are taken in 64 bits.
 """
 from __future__ import annotations
 
@@ -212,8 +212,10 @@ def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nest
         W <- (1 - lr weight_decay) W - lr s orthogonalize(U)
 
     with ``s = sqrt(max(1, m / n))`` (``scale="aspect"``) or ``0.2 sqrt(max(m, n))`` (``"rms"``: the size of an AdamW
-    update).  Weights and momenta change in place, or ``out = (new weights, new momenta)`` receives them.  The matrices
-    of a call share launches, whatever their shapes.  ``lr`` is a number: a captured graph keeps it.  GPU only."""
+    update).  Weights and momenta change in place, or ``out = (new weights, new momenta)`` receives them; tensors that are
+    not the same must not overlap.  ``momentum``, ``eps`` and the coefficients count as fp32 holds them (1 - momentum is
+    that of the fp32 value).  The matrices of a call share launches, whatever their shapes.  ``lr`` is a number: a captured
+    graph keeps it.  GPU only."""
     weights, grads, momenta = list(weights), list(grads), list(momenta)
     out = (weights, momenta) if out is None else tuple(list(v) for v in out)
     if len(out) != 2:
@@ -246,7 +248,8 @@ def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nest
 
 
 class Muon(torch.optim.Optimizer):
-    """Muon on matrices: :func:`muon_update` of every parameter that has a gradient, momenta kept in fp32."""
+    """Muon on matrices: :func:`muon_update` of every parameter that has a gradient, momenta kept in fp32 (and loaded in
+    fp32).  A step can be captured into a graph once the momenta exist."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
                  steps: int = 5, eps: float = 1e-7, coefficients=COEFFICIENTS, scale: str = "aspect") -> None:

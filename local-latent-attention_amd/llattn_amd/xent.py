@@ -227,9 +227,12 @@ def piecewise_head_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Te
 
     ``reduction``: ``"mean"`` over the rows whose target is not ``ignore_index`` (NaN when there are none, with zero
     gradients), ``"sum"``, or ``"none"`` (fp32, ``targets``' shape, 0 in ignored rows).  A target outside ``[0, V)``
-    gives NaN.  With ``return_pred`` also the first argmax of every row (int32).  ``h`` and ``weight`` are bf16 or fp32,
-    fp32 ones rounded to bf16 as under autocast; logits, sums and losses are fp32 and gradients come in their input's
-    type, ``weight``'s accumulated in fp32.  Fewer than 2^23 rows.  Differentiable once, in
+    gives NaN.  With ``return_pred`` also the first argmax of every row (int32; NaN logits are passed over).  ``h`` and
+    ``weight`` are bf16 or fp32, fp32 ones rounded to bf16 as under autocast; logits, sums and losses are fp32.  The logits'
+    gradient is rounded to bf16 (as under autocast) but for the scale that the rows share; gradients come in their input's
+    type, ``weight``'s accumulated in fp32, ``h``'s rounded to bf16 before they are widened.  What is not finite in an
+    ignored row of ``h`` reaches ``weight``'s gradient (0 times infinity), as in any product of the two.  Fewer than 2^23
+    rows.  Differentiable once, in
     reverse mode.  GPU only."""
     if h.dim() < 1 or weight.dim() != 2 or weight.shape[1] != h.shape[-1] or 0 in weight.shape:
         raise ValueError(f"piecewise_head_loss: weight {tuple(weight.shape)} does not match hidden states {tuple(h.shape)}")
