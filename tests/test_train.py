@@ -380,3 +380,9 @@ def test_whole_numbers_of_steps():
     for steps in (float("inf"), float("nan"), 2 ** 32 + 5, None, "5"):
         with pytest.raises(ValueError, match="steps"):
             muon.orthogonalize(x, steps=steps)
+
+
+def test_head_workspace_of_the_present_plan():
+    """q of a piece, the sums of dh over splits (4 for 192 tiles of 256 x 256 on 256 CUs), the shared scale: nothing besides."""
+    n = L.load().llattn_head_bytes
+    assert n(ctypes.byref(L.LlattnHeadCfg(8192, 131072, 1536, 0, 1)), 1) == (512 << 20) + 4 * 8192 * 1536 * 4 + 256
