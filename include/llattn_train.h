@@ -63,8 +63,8 @@ int32_t llattn_head_bwd(const llattn_head_cfg* cfg, const void* h, int64_t ldh, 
  * order of every sum (no atomics).
  *
  * Matrices come in groups of one shape and type (at most LLATTN_MUON_GROUPS a
- * call, LLATTN_MUON_BATCH matrices, of at most 32768 rows and columns); all of
- * them share the launches of the call.  Rows are contiguous.
+ * call, LLATTN_MUON_BATCH matrices, of at most 32768 rows and columns), which
+ * share launches whatever their shapes.  Rows are contiguous.
  *
  * llattn_orthogonalize: out[i] = ns(g[i]), g_dtype in, w_dtype out.
  * llattn_muon_update: one optimiser step,
