@@ -59,7 +59,7 @@ int32_t llattn_head_bwd(const llattn_head_cfg* cfg, const void* h, int64_t ldh, 
  * halves (22 bits of significand) and every product as three products of
  * halves with fp32 accumulation, so results are about as near to the exact ones
  * as fp32 products' are; matrices of at most 16 rows or columns are taken in 64
- * bits (with tiles 0).  a, b, c, eps and mu count as fp32 holds them.  Fixed
+ * bits (with tiles 0, while |a|^(2 steps) is up to 1e10).  a, b, c, eps and mu count as fp32 holds them.  Fixed
  * order of every sum (no atomics).
  *
  * Matrices come in groups of one shape and type (at most LLATTN_MUON_GROUPS a

@@ -1258,7 +1258,13 @@ void launch_products(const Call& k, LastArgs& a) {
   launch_kind<MODE>(kind, a, blocks, k.st);
 }
 
-bool thin(const llattn_muon_group& g) { return std::min(g.rows, g.cols) <= kThin; }
+// ns_thin_kernel's matrices.  A singular value of zero is an eigenvalue of 1e-17 or so of A, of either sign, which every step
+// multiplies by a^2: a negative one that has grown to order 1 runs away (rank 4 of 10 x 40: five steps differ from the
+// iteration on X by 2e-16, 15 steps by 1e-9, 20 overflow).  Up to 1e10 of growth, 9 steps of a = 3.4445, it stays below 1e-4
+// beside sums of any length here.
+bool thin(const llattn_muon_cfg* c, const llattn_muon_group& g) {
+  return std::min(g.rows, g.cols) <= kThin && std::pow(std::fabs((double)c->a), 2.0 * c->steps) <= 1e10;
+}
 
 // All of the call in one workgroup a matrix (ns_small_kernel), where every matrix fits and its launches are the quicker ones.
 bool all_small(const llattn_muon_cfg* c, const Plan& p) {
@@ -1401,7 +1407,7 @@ int32_t run(const char* who, const llattn_muon_cfg* c, const llattn_muon_group* 
   const auto misplaced = [](const void* q, int dtype) { return !q || (uintptr_t)q % (size_t)elem_size(dtype); };
   int thin_groups = 0;
   for (int i = 0; i < c->n_groups; ++i) {
-    thin_groups += thin(groups[i]);
+    thin_groups += thin(c, groups[i]);
     for (int b = k.p.g[i].first; b < k.p.g[i].first + groups[i].batch; ++b)
       if (misplaced(g[b], groups[i].g_dtype) || misplaced(out[b], groups[i].w_dtype) ||
           (k.update && (misplaced(m[b], LLATTN_F32) || misplaced(m_out[b], LLATTN_F32) || misplaced(w[b], groups[i].w_dtype))))
@@ -1416,7 +1422,7 @@ int32_t run(const char* who, const llattn_muon_cfg* c, const llattn_muon_group* 
     q.c.n_groups = 0;
     int held = 0;
     for (int i = 0; i < c->n_groups; ++i) {
-      if (thin(groups[i]) != want) continue;
+      if (thin(c, groups[i]) != want) continue;
       q.groups[q.c.n_groups++] = groups[i];
       for (int b = k.p.g[i].first; b < k.p.g[i].first + groups[i].batch; ++b, ++held) {
         q.g[held] = g[b];

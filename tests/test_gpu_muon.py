@@ -501,3 +501,21 @@ def test_where_matrices_go_to_one_workgroup_each(batch, m, n):
     want = _ns(x.double())
     off = torch.linalg.matrix_norm(_muon().orthogonalize(x).double() - want)
     assert bool((off <= _errors(x, want)).all())
+
+
+@pytest.mark.parametrize("steps", [5, 9, 10, 16, 20, 40])
+@pytest.mark.parametrize("m,n", [(10, 40), (40, 10), (16, 3000), (3, 5)])
+def test_thin_matrices_of_low_rank_over_many_steps(m, n, steps):
+    """Rows of which some are others' copies: directions without a singular value stay as small as they are, whatever the
+    number of steps, and the others stay in their band (the iteration maps [0, 1.21] into itself)."""
+    k = min(m, n)
+    x = _matrices(2, max(1, k // 3), max(m, n), "flat", seed=steps)
+    x = x.repeat(1, 4, 1)[:, :k]
+    x = x.mT.contiguous() if m > n else x
+    got = _muon().orthogonalize(x, steps=steps)
+    assert torch.isfinite(got).all()
+    s = torch.linalg.svdvals(got.double())
+    assert bool((s <= 1.21).all()) and bool((s[:, :max(1, k // 3)] >= 0.6).all())
+    if steps <= 9:
+        want = _ns(x.double(), steps=steps, coef=COEF32)
+        assert bool((torch.linalg.matrix_norm(got.double() - want) <= 1.01 * 2.0 ** -24 * torch.linalg.matrix_norm(want)).all())
