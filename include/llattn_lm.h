@@ -1,0 +1,73 @@
+/* The ends and the feed-forward of the language model around the block: token
+ * and position rows with their gradients, the gated feed-forward, the norm of
+ * all gradients and their clipping.  Same conventions as llattn.h (status
+ * codes, llattn_last_error, explicit stream, caller-supplied memory, nothing
+ * allocated, no state kept between calls).  In the reference: nn.Embedding
+ * twice and their sum (within models.py:505-580), clip_grad_norm_
+ * (train.py:1021); its feed-forward (models.py:50-58) has no gate. */
+#ifndef LLATTN_LM_H
+#define LLATTN_LM_H
+
+#include "llattn.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* ---- token rows, scaled, plus position rows ---------------------------------
+ *   out[n] = scale W[id_n] + Pos[pos_n]      in fp32, rounded once
+ * for rows n < rows: W [V][D], Pos [P][D] (P = 0: none), out [rows][D], all of
+ * `dtype`, row strides ldw and ldp in elements, any alignment of whole
+ * elements.  ids and pos hold integers of index_bytes (4 or 8); pos NULL: pos_n
+ * = n % T.  A row whose id lies outside [0, V), or whose position lies outside
+ * [0, P), is NaN.
+ *
+ * Backward, from dout [rows][D] contiguous:
+ *   dW[v] = scale sum of dout[n] over id_n = v (v != padding), dPos[p] = sum of
+ *   dout[n] over pos_n = p,
+ * whole tables [V][D] and [P][D], contiguous (rows that no token names are
+ * zero), either NULL.  Rows of no valid id (position) leave dW (dPos) alone.
+ * The rows of one token are summed in fp32 in their order, in a tree that the
+ * number of them alone decides: no atomics, and the same bits whatever the
+ * other tokens are. */
+typedef struct llattn_embed_cfg {
+  int64_t rows;         /* below 2^31 */
+  int32_t T, V, P, D;   /* V and P at most 2^22 */
+  int32_t dtype;        /* LLATTN_F32 or LLATTN_BF16 */
+  int32_t index_bytes;
+  int64_t padding;      /* a token without gradient, or -1 */
+  float scale;
+} llattn_embed_cfg;
+
+int32_t llattn_embed_fwd(const llattn_embed_cfg* cfg, const void* ids, const void* pos, const void* W, int64_t ldw,
+                         const void* Pos, int64_t ldp, void* out, void* stream);
+/* Workspace bytes of llattn_embed_bwd for a configuration; has_pos: pos is not NULL.  0 with an error message on a bad one. */
+size_t llattn_embed_bytes(const llattn_embed_cfg* cfg, int32_t has_pos);
+int32_t llattn_embed_bwd(const llattn_embed_cfg* cfg, const void* ids, const void* pos, const void* dout, void* dW,
+                         void* dPos, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- the norm over a list of gradients, and clipping -------------------------
+ *   norm = sqrt(sum over all elements of g^2),  c = min(1, max_norm / (norm + 1e-6)),  out = c g
+ * with squares, sums and products in 64 bits and one rounding to each output's
+ * type.  g, out, numel and dtype are host arrays of n entries, read during the
+ * call: tensors of numel[i] contiguous elements of dtype[i] at any alignment of
+ * whole elements (0 elements: skipped).  A norm that is not finite reaches the
+ * gradients: infinity makes c zero (and infinite gradients NaN), NaN makes them
+ * all NaN.
+ *
+ * llattn_grad_norm writes the norm (fp32).  llattn_clip_grads also writes out[i]
+ * (out NULL: in place; where c is 1 nothing is written in place); out[i] may be
+ * g[i] itself and overlaps nothing else.  With norm_in (a device fp32 value)
+ * that is the norm and none is computed (norm NULL then). */
+size_t llattn_grad_norm_bytes(int32_t n, const int64_t* numel);
+int32_t llattn_grad_norm(int32_t n, const void* const* g, const int64_t* numel, const int32_t* dtype, float* norm,
+                         void* workspace, size_t workspace_bytes, void* stream);
+int32_t llattn_clip_grads(int32_t n, const void* const* g, void* const* out, const int64_t* numel, const int32_t* dtype,
+                          double max_norm, const float* norm_in, float* norm, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* LLATTN_LM_H */

@@ -97,6 +97,11 @@ class LlattnMuonCfg(ctypes.Structure):
         [(n, ctypes.c_float) for n in ("a", "b", "c", "eps", "mu")]
 
 
+class LlattnEmbedCfg(ctypes.Structure):  # include/llattn_lm.h
+    _fields_ = [("rows", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("T", "V", "P", "D", "dtype", "index_bytes")] + \
+        [("padding", ctypes.c_int64), ("scale", ctypes.c_float)]
+
+
 _P = ctypes.c_void_p
 _T = ctypes.POINTER(LlattnTensor)
 _G = ctypes.POINTER(LlattnGemmDesc)
@@ -162,6 +167,17 @@ TRAIN_SIGNATURES = {
     "llattn_muon_update": (_I32, [_MC, _MG, _PP, _PP, _PP, _PP, _PP, _P, _SZ, _P]),
 }
 
+# the same for include/llattn_lm.h
+_EC = ctypes.POINTER(LlattnEmbedCfg)
+LM_SIGNATURES = {
+    "llattn_embed_fwd": (_I32, [_EC, _P, _P, _P, _I64, _P, _I64, _P, _P]),
+    "llattn_embed_bytes": (_SZ, [_EC, _I32]),
+    "llattn_embed_bwd": (_I32, [_EC, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "llattn_grad_norm_bytes": (_SZ, [_I32, _P]),
+    "llattn_grad_norm": (_I32, [_I32, _P, _P, _P, _P, _P, _SZ, _P]),
+    "llattn_clip_grads": (_I32, [_I32, _P, _P, _P, _P, ctypes.c_double, _P, _P, _P, _SZ, _P]),
+}
+
 _lib = None
 
 
@@ -174,7 +190,7 @@ def load() -> ctypes.CDLL:
         raise RuntimeError(f"llattn HIP library not built ({LIB_PATH} missing); run __graft_entry__.build() "
                            "or `python -m llattn_amd._build` on a machine with ROCm hipcc")
     lib = ctypes.CDLL(str(LIB_PATH))
-    for name, (res, args) in (SIGNATURES | STEP_SIGNATURES | TRAIN_SIGNATURES).items():
+    for name, (res, args) in (SIGNATURES | STEP_SIGNATURES | TRAIN_SIGNATURES | LM_SIGNATURES).items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

@@ -1,0 +1,186 @@
+"""The norm over all gradients and their clipping on the gfx950 kernels (``llattn_grad_norm`` and ``llattn_clip_grads`` of
+``include/llattn_lm.h``).
+
+:func:`grad_norm` and :func:`clip_grad_norm` take lists of tensors; :func:`clip_grad_norm_` and
+:func:`clip_grads_with_norm_` take parameters, as the trainer's ``clip_grad_norm_`` does (reference train.py:1021).  A list
+of any length takes one launch per 128 tensors and pass; squares and sums are 64-bit whatever the tensors' type.
+"""
+from __future__ import annotations
+
+import math
+from array import array
+from ctypes import c_void_p
+from numbers import Real
+
+import torch
+
+from . import _lib as L
+
+_CODE = {torch.float32: L.F32, torch.bfloat16: L.BF16}
+
+
+def _flat(t: torch.Tensor):
+    """``t`` as a contiguous tensor on the same memory where its elements fill one stretch of it (in any order of its axes), else
+    None."""
+    if t.is_contiguous():
+        return t
+    order = sorted(range(t.dim()), key=t.stride, reverse=True)
+    t = t.permute(order)
+    return t if t.is_contiguous() else None
+
+
+def _lists(who: str, tensors):
+    """Checks that every call needs: the tensors' device."""
+    for t in tensors:
+        if t.dtype not in _CODE:
+            raise ValueError(f"{who}: gradients must be fp32 or bf16, got {t.dtype}")
+        if t.layout is not torch.strided:
+            raise ValueError(f"{who}: gradients must be dense tensors, got {t.layout}")
+    L.refuse_tangents(who, tensors)
+    L.require_gpu(*tensors)
+    devices = {t.get_device() for t in tensors}
+    if len(devices) > 1:
+        raise ValueError(f"{who}: gradients on {len(devices)} devices")
+    return tensors[0].device
+
+
+class _Arrays:
+    """The host arrays of a call."""
+
+    def __init__(self, tensors):
+        self.n = len(tensors)
+        self.g = array("Q", [t.data_ptr() for t in tensors])
+        self.numel = array("q", [t.numel() for t in tensors])
+        self.dtype = array("i", [_CODE[t.dtype] for t in tensors])
+
+    def workspace(self, device):
+        n = L.load().llattn_grad_norm_bytes(self.n, _at(self.numel))
+        if n == 0:
+            L.check(L.ERR_SHAPE, "llattn_grad_norm_bytes")
+        return torch.empty((n,), dtype=torch.uint8, device=device), n
+
+    def bytes(self) -> int:
+        return sum(n * (2 if d else 4) for n, d in zip(self.numel, self.dtype))
+
+
+def _at(a):
+    return c_void_p(a.buffer_info()[0])
+
+
+def _most(who: str, max_norm) -> float:
+    if not isinstance(max_norm, Real) or not max_norm >= 0:
+        raise ValueError(f"{who}: max_norm must be a number that is not negative, got {max_norm!r}")
+    return float(max_norm)
+
+
+@torch.no_grad()
+def grad_norm(tensors) -> torch.Tensor:
+    """The 2-norm of all elements of ``tensors`` (fp32 or bf16, any shapes and strides, one device) as an fp32 scalar on
+    their device; 0 on the CPU for an empty list.  GPU only."""
+    tensors = [t.detach() for t in tensors]
+    if not tensors:
+        return torch.zeros(())
+    device = _lists("grad_norm", tensors)
+    flat = [_flat(t) for t in tensors]
+    flat = [t.contiguous() if f is None else f for t, f in zip(tensors, flat)]
+    a = _Arrays(flat)
+    ws, n = a.workspace(device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    from .ops import _call
+    with L.on_device(device):
+        _call("llattn_grad_norm", a.n, _at(a.g), _at(a.numel), _at(a.dtype), norm.data_ptr(), ws.data_ptr(), n,
+              L.stream_ptr(device), work=a.bytes())
+    return norm
+
+
+def _clip(who: str, tensors, out, max_norm: float, norm_in) -> torch.Tensor | None:
+    """Scales ``tensors`` into ``out`` (or in place); the norm where none is given."""
+    device = _lists(who, tensors)
+    if norm_in is not None and (norm_in.numel() != 1 or norm_in.dtype is not torch.float32 or norm_in.device != device):
+        raise ValueError(f"{who}: the norm must be one fp32 value on {device}, got {tuple(norm_in.shape)} {norm_in.dtype} on {norm_in.device}")
+    src, dst, back = [], [], []
+    for i, g in enumerate(tensors):
+        o = g if out is None else out[i]
+        f = _flat(g)
+        if o is not g:
+            if o.shape != g.shape or o.dtype is not g.dtype or o.get_device() != g.get_device():
+                raise ValueError(f"{who}: outputs must have their gradient's shape {tuple(g.shape)}, type and device")
+            # both in one order of the axes: that of memory
+            if not (f is not None and o.stride() == g.stride()):
+                f = g.contiguous()
+        if o.is_contiguous() or (f is not None and o.stride() == g.stride()):
+            d = o if o.is_contiguous() else _flat(o)
+        else:  # not in one stretch: scaled in a copy
+            if torch._debug_has_internal_overlap(o) == 1:
+                raise ValueError(f"{who}: a tensor that is written holds one element in several places (strides {o.stride()})")
+            d = f = g.contiguous() if o is not g else g.clone(memory_format=torch.contiguous_format)
+            if o is not g:
+                d = torch.empty_like(f)
+            back.append((o, d))
+        src.append(f)
+        dst.append(d)
+    a = _Arrays(src)
+    o = array("Q", [t.data_ptr() for t in dst])
+    ws = norm = None
+    n = 0
+    if norm_in is None:
+        ws, n = a.workspace(device)
+        norm = torch.empty((), dtype=torch.float32, device=device)
+    from .ops import _call
+    with L.on_device(device):
+        _call("llattn_clip_grads", a.n, _at(a.g), _at(o), _at(a.numel), _at(a.dtype), max_norm,
+              None if norm_in is None else norm_in.data_ptr(), None if norm is None else norm.data_ptr(),
+              None if ws is None else ws.data_ptr(), n, L.stream_ptr(device), work=(3 if norm_in is None else 2) * a.bytes())
+    for to, d in back:
+        to.copy_(d)
+    torch.autograd.graph.increment_version(list(tensors) if out is None else out)
+    return norm
+
+
+@torch.no_grad()
+def clip_grad_norm(grads, max_norm: float, out=None) -> torch.Tensor:
+    """Scales ``grads`` (tensors, fp32 or bf16) by ``min(1, max_norm / (norm + 1e-6))``, ``norm`` being their
+    :func:`grad_norm`, which is returned.  In place, or into ``out`` (a list of as many tensors of the same shapes and types;
+    each may be its gradient itself and overlaps nothing else).  Nothing waits for the GPU.  GPU only."""
+    grads = [g.detach() for g in grads]
+    most = _most("clip_grad_norm", max_norm)
+    if out is not None:
+        out = list(out)
+        if len(out) != len(grads):
+            raise ValueError(f"clip_grad_norm: {len(out)} outputs for {len(grads)} gradients")
+        if any(o.requires_grad and o.is_leaf for o in out):
+            raise ValueError("clip_grad_norm: out holds leaves that require gradients")
+    return torch.zeros(()) if not grads else _clip("clip_grad_norm", grads, out, most, None)
+
+
+def _grads(parameters):
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    return [p.grad.detach() for p in parameters if p.grad is not None]
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Clips the gradients of ``parameters`` in place to a 2-norm of ``max_norm`` over all of them, as
+    ``torch.nn.utils.clip_grad_norm_``, and returns the norm (fp32).  ``error_if_nonfinite`` waits for the norm and raises
+    before anything is scaled.  Gradients are fp32 or bf16 (each once), on one GPU."""
+    if float(norm_type) != 2.0:
+        raise ValueError(f"clip_grad_norm_: the 2-norm only, got norm_type={norm_type}")
+    most, grads = _most("clip_grad_norm_", max_norm), _grads(parameters)
+    if not grads:
+        return torch.zeros(())
+    if not error_if_nonfinite:
+        return _clip("clip_grad_norm_", grads, None, most, None)
+    norm = grad_norm(grads)
+    if not math.isfinite(norm.item()):
+        raise RuntimeError(f"clip_grad_norm_: the gradients' norm is {norm.item()}; error_if_nonfinite=False scales them all the same")
+    _clip("clip_grad_norm_", grads, None, most, norm)
+    return norm
+
+
+@torch.no_grad()
+def clip_grads_with_norm_(parameters, max_norm: float, total_norm: torch.Tensor) -> None:
+    """Clips the gradients of ``parameters`` in place by a norm that the caller has (one fp32 value on their device: say, one
+    joined over the shards of a model)."""
+    most, grads = _most("clip_grads_with_norm_", max_norm), _grads(parameters)
+    if grads:
+        _clip("clip_grads_with_norm_", grads, None, most, total_norm.detach())

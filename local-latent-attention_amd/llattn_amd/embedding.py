@@ -1,0 +1,130 @@
+"""Token rows plus position rows on the gfx950 kernels (``llattn_embed_fwd/bwd`` of ``include/llattn_lm.h``).
+
+:func:`embed` is the beginning of the language model (reference models.py:505-580: the token embedding plus the learned
+position embedding) as one pass over its output; its backward sums the gradients of both tables in the order of the
+sorted tokens, without atomics: the same bits in every call.
+"""
+from __future__ import annotations
+
+import ctypes
+from numbers import Integral, Real
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+
+MOST = 1 << 22  # rows of a table
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """A table whose rows are whole, any distance apart."""
+    t = t.detach()
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def _index(t: torch.Tensor) -> torch.Tensor:
+    return t.reshape(-1).contiguous() if t.dtype in (torch.int64, torch.int32) else t.reshape(-1).to(torch.int64)
+
+
+def _forward(ids, weight, position, positions, scale, padding):
+    """(out, the indices and the configuration that a backward reads)."""
+    D = weight.shape[1]
+    i, p = _index(ids), None if positions is None else _index(positions)
+    if p is not None and p.dtype is not i.dtype:
+        i, p = i.to(torch.int64), p.to(torch.int64)
+    T = ids.shape[-1] if ids.dim() else 1
+    cfg = L.LlattnEmbedCfg(i.numel(), max(T, 1), weight.shape[0], 0 if position is None else position.shape[0], D,
+                           L.dtype_code(weight.dtype), i.element_size(), padding, scale)
+    out = torch.empty((*ids.shape, D), dtype=weight.dtype, device=weight.device)
+    if out.numel():
+        w, q = _rows(weight), None if position is None else _rows(position)
+        from .ops import _call
+        with L.on_device(weight.device):
+            _call("llattn_embed_fwd", ctypes.byref(cfg), i.data_ptr(), None if p is None else p.data_ptr(), w.data_ptr(), w.stride(0),
+                  None if q is None else q.data_ptr(), 0 if q is None else q.stride(0), out.data_ptr(),
+                  L.stream_ptr(weight.device), work=(2 + (q is not None)) * out.numel() * out.element_size())
+    return out, i, p, cfg
+
+
+class _Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, position, positions, scale, padding, grad_enabled):
+        out, i, p, cfg = _forward(ids, weight, position, positions, scale, padding)
+        if grad_enabled:
+            ctx.save_for_backward(i, p)
+            ctx.meta = (cfg, weight.shape, None if position is None else position.shape)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        i, p = ctx.saved_tensors
+        cfg, w_shape, p_shape = ctx.meta
+        dev = dout.device
+        dw = torch.empty(w_shape, dtype=dout.dtype, device=dev) if ctx.needs_input_grad[1] else None
+        dp = torch.empty(p_shape, dtype=dout.dtype, device=dev) if p_shape is not None and ctx.needs_input_grad[2] else None
+        d = dout.contiguous()
+        n = L.load().llattn_embed_bytes(ctypes.byref(cfg), int(p is not None))
+        if n == 0:
+            L.check(L.ERR_SHAPE, "llattn_embed_bytes")
+        ws = torch.empty((n,), dtype=torch.uint8, device=dev)
+        written = sum(t.numel() for t in (dw, dp) if t is not None)
+        from .ops import _call
+        with L.on_device(dev):
+            _call("llattn_embed_bwd", ctypes.byref(cfg), i.data_ptr(), None if p is None else p.data_ptr(), d.data_ptr(),
+                  None if dw is None else dw.data_ptr(), None if dp is None else dp.data_ptr(), ws.data_ptr(), n,
+                  L.stream_ptr(dev), work=(d.numel() + written) * d.element_size())
+        return None, dw, dp, None, None, None, None
+
+
+def _check_integers(name: str, t: torch.Tensor) -> None:
+    if t.is_floating_point() or t.is_complex() or t.dtype is torch.bool:
+        raise ValueError(f"embed: {name} must be integers, got {t.dtype}")
+
+
+def embed(ids: torch.Tensor, weight: torch.Tensor, position: torch.Tensor | None = None,
+          positions: torch.Tensor | None = None, scale: float = 1.0, padding_idx: int | None = None) -> torch.Tensor:
+    """``scale * weight[ids] + position[positions]`` for ``ids [..., T]``, ``weight [V, D]`` and ``position [P, D]``
+    (fp32 or bf16, one type; any strides), computed in fp32 and rounded once to that type.
+
+    Without ``positions`` (integers of ``ids``' shape, for packed documents or single tokens at their places) the tokens
+    of the last axis stand at positions 0, 1, ...; without ``position`` nothing is added.  An id outside ``[0, V)`` or a
+    position outside ``[0, P)`` gives a row of NaN and no gradient to the table that has no such row.  Gradients are
+    whole tables in their table's type, summed in fp32 in a fixed order (no atomics); the row ``padding_idx`` of
+    ``weight`` gets none.  V and P at most 2^22.  Differentiable once, in reverse mode.  GPU only."""
+    if weight.dim() != 2 or 0 in weight.shape:
+        raise ValueError(f"embed: weight must be a non-empty matrix, got shape {tuple(weight.shape)}")
+    V, D = weight.shape
+    _check_integers("ids", ids)
+    L.dtype_code(weight.dtype)
+    if position is not None and (position.dim() != 2 or position.shape[1] != D or not len(position)
+                                 or position.dtype is not weight.dtype):
+        raise ValueError(f"embed: position {tuple(position.shape)} ({position.dtype}) does not match weight {tuple(weight.shape)} "
+                         f"({weight.dtype})")
+    if max(V, 0 if position is None else len(position)) > MOST:
+        raise ValueError(f"embed: at most {MOST} rows in a table")
+    if positions is not None:
+        if position is None:
+            raise ValueError("embed: positions without position rows")
+        _check_integers("positions", positions)
+        if positions.shape != ids.shape:
+            raise ValueError(f"embed: positions {tuple(positions.shape)} for ids {tuple(ids.shape)}")
+    elif position is not None and ids.dim() and ids.shape[-1] > len(position):
+        raise ValueError(f"embed: {ids.shape[-1]} tokens in a row and {len(position)} positions")
+    if not isinstance(scale, Real):
+        raise ValueError(f"embed: scale must be a number, got {type(scale).__name__}")
+    if padding_idx is not None and (not isinstance(padding_idx, Integral) or not -V <= padding_idx < V):
+        raise ValueError(f"embed: padding_idx {padding_idx} outside the {V} rows")
+    if ids.numel() >= 1 << 31:
+        raise ValueError(f"embed: {ids.numel()} tokens, fewer than 2^31 expected")
+    tensors = [t for t in (ids, weight, position, positions) if t is not None]
+    L.refuse_tangents("embed", [t for t in (weight, position) if t is not None])
+    L.require_gpu(*tensors)
+    if len({t.device for t in tensors}) > 1:
+        raise ValueError(f"embed: tensors on {', '.join(str(t.device) for t in tensors)}")
+    padding = -1 if padding_idx is None else int(padding_idx) % V
+    args = (ids, weight, position, positions, float(scale), padding)
+    if not (torch.is_grad_enabled() and (weight.requires_grad or position is not None and position.requires_grad)):
+        return _forward(*args)[0]
+    return _Embed.apply(*args, True)

@@ -1,0 +1,179 @@
+"""CPU tests of the language model's operators: the C interface (include/llattn_lm.h), and what is refused before anything
+is launched."""
+import ctypes
+import re
+import subprocess
+from array import array
+
+import pytest
+import torch
+
+from conftest import REPO
+from llattn_amd import _lib as L
+from llattn_amd import clip, clip_grad_norm, clip_grad_norm_, clip_grads_with_norm_, embed, grad_norm
+
+BF16 = torch.bfloat16
+AT = 1 << 20  # a pointer that nothing reads
+
+
+def test_header_matches_the_binding(tmp_path):
+    text = (REPO / "include" / "llattn_lm.h").read_text()
+    names = set(re.findall(r"^\s*(?:int32_t|size_t)\s+(llattn_\w+)\s*\(", text, re.M))
+    assert names == set(L.LM_SIGNATURES) and all(hasattr(L.load(), n) for n in names)
+    structs = {"llattn_embed_cfg": L.LlattnEmbedCfg}
+    lines = ["#include <stddef.h>", "#include <stdio.h>", '#include "llattn_lm.h"', "int main(void) {"]
+    for c, t in structs.items():
+        lines.append(f'printf("%zu\\n", sizeof({c}));')
+        lines += [f'printf("%zu\\n", offsetof({c}, {f[0]}));' for f in t._fields_]
+    src = tmp_path / "l.c"
+    src.write_text("\n".join([*lines, "return 0; }"]))
+    subprocess.run(["gcc", f"-I{REPO / 'include'}", str(src), "-o", str(tmp_path / "l")], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "l")], capture_output=True, text=True, check=True).stdout.split()]
+    want = []
+    for t in structs.values():
+        want.append(ctypes.sizeof(t))
+        want += [getattr(t, f[0]).offset for f in t._fields_]
+    assert got == want
+
+
+# ---------------------------------------------------------------------------
+# token and position rows
+# ---------------------------------------------------------------------------
+
+def _cfg(rows=6, T=3, V=10, P=4, D=8, dtype=0, index_bytes=8, padding=-1, scale=1.0):
+    return L.LlattnEmbedCfg(rows, T, V, P, D, dtype, index_bytes, padding, scale)
+
+
+@pytest.mark.parametrize("kw", [dict(rows=-1), dict(rows=1 << 31), dict(V=0), dict(V=(1 << 22) + 1), dict(P=-1), dict(P=(1 << 22) + 1),
+                                dict(D=0), dict(D=(1 << 20) + 1), dict(T=0), dict(T=5), dict(rows=7), dict(dtype=2),
+                                dict(index_bytes=2), dict(padding=10), dict(padding=-2)], ids=str)
+def test_embed_sizes_refused(kw):
+    assert L.load().llattn_embed_bytes(ctypes.byref(_cfg(**kw)), 0) == 0 and L.load().llattn_last_error()
+
+
+def test_embed_sizes_taken():
+    n = L.load().llattn_embed_bytes
+    assert n(ctypes.byref(_cfg()), 0) > 0 and n(ctypes.byref(_cfg(rows=0)), 0) > 0
+    assert n(ctypes.byref(_cfg(T=9, rows=7)), 1) > 0 and n(ctypes.byref(_cfg(T=0, P=0)), 0) > 0
+    # sums of 32 rows, two tables; rows in order twice
+    assert n(ctypes.byref(_cfg(rows=32768, T=2048, V=32000, P=2048, D=1408)), 0) < 2 * 32768 * 1408 * 4 // 31 + 32768 * 12 + 32000 * 8 + 4096
+
+
+@pytest.mark.parametrize("kw,code", [(dict(ids=None), 3), (dict(W=None), 3), (dict(out=None), 3), (dict(Pos=None), 3), (dict(ids=AT + 4), 3),
+                                     (dict(W=AT + 2), 3), (dict(out=AT + 1), 3), (dict(ldw=7), 3), (dict(ldp=7), 3)], ids=str)
+def test_embed_forward_refused(kw, code):
+    a = dict(ids=AT, pos=None, W=AT, ldw=8, Pos=AT, ldp=8, out=AT) | kw
+    assert L.load().llattn_embed_fwd(ctypes.byref(_cfg()), *a.values(), None) == code
+
+
+@pytest.mark.parametrize("kw,code", [(dict(ids=None), 3), (dict(dout=None), 3), (dict(dW=AT + 2), 3), (dict(ws=None), 5), (dict(ws=AT + 8), 5),
+                                     (dict(n=100), 5)], ids=str)
+def test_embed_backward_refused(kw, code):
+    lib = L.load()
+    cfg = _cfg()
+    a = dict(ids=AT, pos=None, dout=AT, dW=AT, dPos=AT, ws=AT, n=lib.llattn_embed_bytes(ctypes.byref(cfg), 0)) | kw
+    assert lib.llattn_embed_bwd(ctypes.byref(cfg), *a.values(), None) == code
+    assert lib.llattn_embed_bwd(ctypes.byref(_cfg(P=0)), *(a | dict(n=1 << 20)).values(), None) in (1, code)
+
+
+def test_embed_refusals():
+    ids, w, p = torch.zeros(2, 3, dtype=torch.int64), torch.zeros(5, 4), torch.zeros(3, 4)
+    for args, kw, msg in [((ids, w[0]), {}, "matrix"), ((ids, w[:0]), {}, "matrix"), ((ids.float(), w), {}, "integers"),
+                          ((ids.bool(), w), {}, "integers"), ((ids, w.double()), {}, "float32"), ((ids, w, p[:, :2]), {}, "match"),
+                          ((ids, w, p[0]), {}, "match"), ((ids, w, p.to(BF16)), {}, "match"), ((ids, w, p[:2]), {}, "positions"),
+                          ((ids, w), dict(positions=ids), "without"), ((ids, w, p), dict(positions=ids[:1]), "positions"),
+                          ((ids, w, p), dict(positions=ids.float()), "integers"), ((ids, w), dict(scale="2"), "number"),
+                          ((ids, w), dict(scale=torch.ones(())), "number"), ((ids, w), dict(padding_idx=5), "padding_idx"),
+                          ((ids, w), dict(padding_idx=-6), "padding_idx"), ((ids, torch.zeros((1 << 22) + 1, 1)), {}, "at most")]:
+        with pytest.raises(ValueError, match=msg):
+            embed(*args, **kw)
+    with pytest.raises(RuntimeError, match="MI355X"):
+        embed(ids, w, p)
+
+
+# ---------------------------------------------------------------------------
+# the norm over gradients, and clipping
+# ---------------------------------------------------------------------------
+
+def _list(*values, code="Q"):
+    a = array(code, values)
+    return a, clip._at(a)
+
+
+def test_grad_norm_sizes():
+    lib = L.load()
+
+    def size(*n):
+        keep = array("q", n)
+        return lib.llattn_grad_norm_bytes(len(n), clip._at(keep))
+    assert size() == 8 and size(0, 0) == 8 and size(1) == 8 and size(16384) == 8 and size(16385) == 16 and size(1, 1) == 16
+    assert size(1 << 30) == 8 * 2048 and size(*[1] * 129) == 8 * 129
+    assert size(-1) == 0 and size(1 << 45) == 0 and lib.llattn_grad_norm_bytes(-1, None) == 0 and lib.llattn_grad_norm_bytes(1, None) == 0
+
+
+def _clip_call(g=(AT,), out=None, numel=(10,), dtype=(0,), norm_in=None, norm=AT, ws=AT, n=1 << 20):
+    keep = [_list(*g), None if out is None else _list(*out), _list(*numel, code="q"), _list(*dtype, code="i")]
+    p = [k and k[1] for k in keep]
+    return L.load().llattn_clip_grads(len(g), p[0], p[1], p[2], p[3], 1.0, norm_in, norm, ws, n, None)
+
+
+@pytest.mark.parametrize("kw,code", [(dict(g=(0,)), 3), (dict(g=(AT + 2,)), 3), (dict(out=(0,)), 3), (dict(out=(AT + 4002,)), 3),
+                                     (dict(dtype=(2,)), 2), (dict(numel=(-1,)), 1), (dict(norm=None), 3), (dict(norm_in=AT), 3),
+                                     (dict(ws=None), 5), (dict(ws=AT + 4), 5), (dict(n=7), 5),
+                                     (dict(g=(AT, AT), numel=(10, 10), dtype=(0, 0)), 3),
+                                     (dict(g=(AT, AT + 36), numel=(10, 10), dtype=(0, 0)), 3),
+                                     (dict(out=(AT + 36,)), 3), (dict(out=(AT - 36,)), 3),
+                                     (dict(g=(AT, AT + 400), out=(AT + 400, AT), numel=(10, 10), dtype=(0, 0)), 3),
+                                     (dict(g=(AT, AT + 400), out=(AT, AT + 20), numel=(10, 10), dtype=(0, 0)), 3),
+                                     (dict(g=(AT, AT + 400), out=(AT + 800, AT + 820), numel=(10, 10), dtype=(1, 1)), 5)], ids=str)
+def test_clip_calls_refused(kw, code):
+    if code == 5 and "ws" not in kw and "n" not in kw:
+        kw = kw | dict(n=0)  # side by side: what is refused is the workspace
+    assert _clip_call(**kw) == code and L.load().llattn_last_error()
+
+
+def test_clip_refusals():
+    g = torch.ones(3)
+    for f, msg in [(lambda: clip_grad_norm([g], -1.0), "max_norm"), (lambda: clip_grad_norm([g], float("nan")), "max_norm"),
+                   (lambda: clip_grad_norm([g], g[0]), "max_norm"), (lambda: clip_grad_norm([g], 1.0, out=[]), "outputs"),
+                   (lambda: clip_grad_norm([g.half()], 1.0), "fp32 or bf16"), (lambda: grad_norm([g.long()]), "fp32 or bf16"),
+                   (lambda: grad_norm([g.to_sparse()]), "dense"),
+                   (lambda: clip_grad_norm([g], 1.0, out=[torch.ones(3, requires_grad=True)]), "leaves"),
+                   (lambda: clip_grad_norm_([], 1.0, norm_type=1.0), "2-norm"),
+                   (lambda: clip_grad_norm_([], -1.0), "max_norm")]:
+        with pytest.raises(ValueError, match=msg):
+            f()
+    p = torch.nn.Parameter(g)
+    p.grad = g
+    for f in (lambda: grad_norm([g]), lambda: clip_grad_norm([g], 1.0), lambda: clip_grad_norm_(p, 1.0),
+              lambda: clip_grads_with_norm_([p], 1.0, torch.ones(()))):
+        with pytest.raises(RuntimeError, match="MI355X"):
+            f()
+
+
+def test_nothing_to_clip():
+    assert float(grad_norm([])) == 0.0 and float(clip_grad_norm([], 1.0)) == 0.0
+    assert float(clip_grad_norm_([torch.nn.Parameter(torch.ones(2))], 1.0)) == 0.0
+    clip_grads_with_norm_([], 1.0, torch.ones(()))
+
+
+@pytest.mark.parametrize("which", ["embed", "clip"])
+def test_forward_mode_tangents_are_refused(which):
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        t = fwd.make_dual(torch.ones(4, 3), torch.ones(4, 3))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            if which == "embed":
+                embed(torch.zeros(2, dtype=torch.int64), t)
+            else:
+                grad_norm([t])
+
+
+def test_flat_views():
+    """Tensors in one stretch of memory, whatever the order of their axes, are taken as they lie."""
+    x = torch.arange(24.0).reshape(2, 3, 4)
+    for t in (x, x.permute(2, 0, 1), x.transpose(0, 1), x[0].t()):
+        f = clip._flat(t)
+        assert f.is_contiguous() and f.data_ptr() == t.data_ptr() and f.numel() == t.numel()
+    for t in (x[:, :, ::2], x[:, :2], torch.ones(3).expand(4, 3)):
+        assert clip._flat(t) is None
