@@ -9,6 +9,7 @@ Public surface:
 * :func:`pool` -- segment pooling op;
 * :func:`piecewise_head_loss` -- LM head and cross entropy over a vocabulary of any size, no logits kept;
 * :func:`embed` -- token rows, scaled, plus position rows;
+* :func:`gated_feed_forward` -- ``w2(act(w1 x) * w3 x)``;
 * :func:`grad_norm`, :func:`clip_grad_norm`, :func:`clip_grad_norm_`, :func:`clip_grads_with_norm_` -- the norm over all
   gradients, and clipping;
 * :func:`orthogonalize`, :func:`muon_update`, :class:`Muon`, :class:`MuonAdamW` -- orthogonalised weight updates.
@@ -17,6 +18,7 @@ from ._lib import DIV_COUNT, DIV_ONE, DIV_SEG, Layout, resolve_layout
 from .clip import clip_grad_norm, clip_grad_norm_, clip_grads_with_norm_, grad_norm
 from .config import ModelConfig, build_attention
 from .embedding import embed
+from .gated import gated_feed_forward
 from .module import LocalLatentAttentionHIP, LocalLatentAttentionTriton
 from .muon import Muon, MuonAdamW, muon_update, orthogonalize
 from .ops import LLAttnCore, LLAttnFunction, pool
@@ -26,5 +28,5 @@ __all__ = [
     "DIV_COUNT", "DIV_ONE", "DIV_SEG", "Layout", "resolve_layout", "ModelConfig", "build_attention",
     "LocalLatentAttentionHIP", "LocalLatentAttentionTriton", "LLAttnCore", "LLAttnFunction", "pool",
     "piecewise_head_loss", "orthogonalize", "muon_update", "Muon", "MuonAdamW",
-    "embed", "grad_norm", "clip_grad_norm", "clip_grad_norm_", "clip_grads_with_norm_",
+    "embed", "gated_feed_forward", "grad_norm", "clip_grad_norm", "clip_grad_norm_", "clip_grads_with_norm_",
 ]

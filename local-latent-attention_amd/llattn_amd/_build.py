@@ -20,7 +20,7 @@ SOURCES = ("llattn_abi.cpp", "llattn_steps.cpp", "llattn_pool.hip", "llattn_late
            "llattn_gemm.hip", "llattn_gemm_tile.hip", "llattn_gemm_f32.hip",
            "llattn_colsum.hip", "llattn_cast.hip", "llattn_norm.hip",
            "llattn_xent.hip", "llattn_head.hip", "llattn_muon.hip",
-           "llattn_embed.hip", "llattn_clip.hip")
+           "llattn_embed.hip", "llattn_clip.hip", "llattn_gated.hip")
 ARCH = "gfx950"
 
 # -packed-fp32-ops off: hipcc must not emit packed fp32 arithmetic for this target.

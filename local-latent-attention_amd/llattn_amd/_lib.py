@@ -102,6 +102,18 @@ class LlattnEmbedCfg(ctypes.Structure):  # include/llattn_lm.h
         [("padding", ctypes.c_int64), ("scale", ctypes.c_float)]
 
 
+class LlattnGatedCfg(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("rows", "D", "F", "D_out", "act", "dw_dtype", "dw2_dtype")]
+
+
+class LlattnGatedWeights(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("W1", "W3", "W2", "b1", "b3", "b2")]
+
+
+class LlattnGatedGrads(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dx", "dW1", "dW3", "dW2", "db1", "db3", "db2")]
+
+
 _P = ctypes.c_void_p
 _T = ctypes.POINTER(LlattnTensor)
 _G = ctypes.POINTER(LlattnGemmDesc)
@@ -168,7 +180,7 @@ TRAIN_SIGNATURES = {
 }
 
 # the same for include/llattn_lm.h
-_EC = ctypes.POINTER(LlattnEmbedCfg)
+_EC, _GC, _GW, _GG = (ctypes.POINTER(t) for t in (LlattnEmbedCfg, LlattnGatedCfg, LlattnGatedWeights, LlattnGatedGrads))
 LM_SIGNATURES = {
     "llattn_embed_fwd": (_I32, [_EC, _P, _P, _P, _I64, _P, _I64, _P, _P]),
     "llattn_embed_bytes": (_SZ, [_EC, _I32]),
@@ -176,6 +188,9 @@ LM_SIGNATURES = {
     "llattn_grad_norm_bytes": (_SZ, [_I32, _P]),
     "llattn_grad_norm": (_I32, [_I32, _P, _P, _P, _P, _P, _SZ, _P]),
     "llattn_clip_grads": (_I32, [_I32, _P, _P, _P, _P, ctypes.c_double, _P, _P, _P, _SZ, _P]),
+    "llattn_gated_bytes": (_SZ, [_GC, _I32]),
+    "llattn_gated_fwd": (_I32, [_GC, _P, _I64, _GW, _P, _P, _P, _P, _P, _SZ, _P]),
+    "llattn_gated_bwd": (_I32, [_GC, _P, _I64, _GW, _P, _P, _P, _P, _GG, _P, _SZ, _P]),
 }
 
 _lib = None

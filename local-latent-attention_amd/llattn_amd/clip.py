@@ -36,7 +36,6 @@ def _lists(who: str, tensors):
             raise ValueError(f"{who}: gradients must be fp32 or bf16, got {t.dtype}")
         if t.layout is not torch.strided:
             raise ValueError(f"{who}: gradients must be dense tensors, got {t.layout}")
-    L.refuse_tangents(who, tensors)
     L.require_gpu(*tensors)
     devices = {t.get_device() for t in tensors}
     if len(devices) > 1:
@@ -77,9 +76,11 @@ def _most(who: str, max_norm) -> float:
 def grad_norm(tensors) -> torch.Tensor:
     """The 2-norm of all elements of ``tensors`` (fp32 or bf16, any shapes and strides, one device) as an fp32 scalar on
     their device; 0 on the CPU for an empty list.  GPU only."""
-    tensors = [t.detach() for t in tensors]
+    tensors = list(tensors)
     if not tensors:
         return torch.zeros(())
+    L.refuse_tangents("grad_norm", tensors)
+    tensors = [t.detach() for t in tensors]
     device = _lists("grad_norm", tensors)
     flat = [_flat(t) for t in tensors]
     flat = [t.contiguous() if f is None else f for t, f in zip(tensors, flat)]
@@ -142,8 +143,9 @@ def clip_grad_norm(grads, max_norm: float, out=None) -> torch.Tensor:
     """Scales ``grads`` (tensors, fp32 or bf16) by ``min(1, max_norm / (norm + 1e-6))``, ``norm`` being their
     :func:`grad_norm`, which is returned.  In place, or into ``out`` (a list of as many tensors of the same shapes and types;
     each may be its gradient itself and overlaps nothing else).  Nothing waits for the GPU.  GPU only."""
+    grads, most = list(grads), _most("clip_grad_norm", max_norm)
+    L.refuse_tangents("clip_grad_norm", grads)
     grads = [g.detach() for g in grads]
-    most = _most("clip_grad_norm", max_norm)
     if out is not None:
         out = list(out)
         if len(out) != len(grads):

@@ -1,7 +1,8 @@
 """Block configuration and the attention dispatcher.
 
 ``ModelConfig`` carries the fields of the reference dataclass that shape the
-attention block (reference models.py:21-37); ``build_attention`` is the
+attention block (reference models.py:21-37), and choices of the model around it that
+have no counterpart there (``ffn``, ``fused_embeddings``); ``build_attention`` is the
 counterpart of the reference ``_build_attention`` (reference models.py:465-488)
 but forwards every block field, including ``local_block_size`` and
 ``latent_query_block_size`` that the reference dispatcher drops.
@@ -28,6 +29,8 @@ class ModelConfig:
     latent_query_block_size: int = 0
     checkpoint_blocks: bool = False
     use_triton_kernel: bool = True
+    ffn: str = "gelu"  # the reference's w2(gelu(w1 x)); "swiglu" or "geglu": gated, w2(act(w1 x) * w3 x)
+    fused_embeddings: bool = False  # both lookups in one pass in training too: their gradients by sorted tokens
 
 
 # architecture presets of the reference trainer (reference train.py:71-93); the

@@ -27,9 +27,12 @@ from typing import Callable, Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.nn.modules.module import _has_any_global_hook
 from torch.utils.checkpoint import checkpoint
 
+from .clip import clip_grad_norm_
 from .config import MODEL_PRESETS, ModelConfig, build_attention
+from .embedding import MOST as MOST_EMBEDDINGS, embed
 from .norm import add_rms_norm, rms_norm
 
 
@@ -65,6 +68,42 @@ class FeedForward(nn.Module):
         return self.dropout(self.w2(F.gelu(self.w1(x))))
 
 
+GATES = {"swiglu": "silu", "geglu": "gelu"}
+
+
+class GatedFeedForward(nn.Module):
+    """``w2(act(w1 x) * w3 x)``, the gated kind of :class:`FeedForward` (``config.ffn``: ``"swiglu"`` or ``"geglu"``).  On the GPU
+    under bf16 autocast, or in bf16 throughout, it runs as :func:`llattn_amd.gated.gated_feed_forward`."""
+
+    def __init__(self, config: ModelConfig) -> None:
+        super().__init__()
+        self.act = GATES[config.ffn]
+        self.w1 = nn.Linear(config.d_model, config.d_ff)
+        self.w3 = nn.Linear(config.d_model, config.d_ff)
+        self.w2 = nn.Linear(config.d_ff, config.d_model)
+        self.dropout = nn.Dropout(config.dropout)
+        self.fused = True  # False: separate torch ops (a comparison model sets it)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        autocast = torch.is_autocast_enabled("cuda")
+        bf16 = torch.get_autocast_dtype("cuda") == torch.bfloat16 if autocast else \
+            x.dtype == torch.bfloat16 == self.w1.weight.dtype == self.w3.weight.dtype == self.w2.weight.dtype
+        if self.fused and x.is_cuda and bf16 and (self.dropout.p == 0.0 or not self.training):
+            from .gated import gated_feed_forward
+            return gated_feed_forward(x, self.w1, self.w3, self.w2, self.act)
+        act = F.silu if self.act == "silu" else F.gelu
+        return self.dropout(self.w2(act(self.w1(x)) * self.w3(x)))
+
+
+def build_feed_forward(config: ModelConfig) -> nn.Module:
+    """The feed-forward that ``config.ffn`` names."""
+    if config.ffn == "gelu":
+        return FeedForward(config)
+    if config.ffn not in GATES:
+        raise ValueError(f"ffn must be one of {('gelu', *GATES)}, got {config.ffn!r}")
+    return GatedFeedForward(config)
+
+
 class TransformerBlock(nn.Module):
     """Pre-norm residual block (reference models.py:490-502)."""
 
@@ -74,7 +113,7 @@ class TransformerBlock(nn.Module):
         self.norm1 = norm_factory(config.d_model)
         self.norm2 = norm_factory(config.d_model)
         self.attn = attention_factory(config)
-        self.ff = FeedForward(config)
+        self.ff = build_feed_forward(config)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         x = x + self.attn(self.norm1(x))
@@ -91,6 +130,9 @@ class LocalLatentLM(nn.Module):
         self.config = config
         self.checkpoint_blocks = config.checkpoint_blocks
         self.fuse_residual_norms = True  # residual adds inside the next norm (same values, fewer passes)
+        # both lookups and their sum in one pass: always where no gradient is asked for (same values), in training if the
+        # configuration says so (the tables' gradients are then summed by sorted tokens, in another order than torch's)
+        self.fuse_embeddings = config.fused_embeddings
         factory = attention_factory or build_attention
         norm = norm_factory or RMSNorm
         self.embedding = nn.Embedding(config.vocab_size, config.d_model)
@@ -138,8 +180,11 @@ class LocalLatentLM(nn.Module):
     def hidden(self, input_ids: torch.Tensor) -> torch.Tensor:
         """The final-norm hidden states ``[B, T, D]`` that the tied head maps to logits."""
         _, seq_len = input_ids.shape
-        pos = torch.arange(seq_len, device=input_ids.device)
-        x = self.embedding(input_ids) + self.position(pos).unsqueeze(0)
+        if self._fused_embeddings(input_ids):
+            x = embed(input_ids, self.embedding.weight, self.position.weight, padding_idx=self.embedding.padding_idx)
+        else:
+            pos = torch.arange(seq_len, device=input_ids.device)
+            x = self.embedding(input_ids) + self.position(pos).unsqueeze(0)
         if self._fused_norms(x):
             return self._hidden_fused(x)
         for block in self.blocks:
@@ -185,6 +230,22 @@ class LocalLatentLM(nn.Module):
             if eos_token_id is not None and int(nxt) == eos_token_id:
                 break
         return ids
+
+    def _fused_embeddings(self, input_ids: torch.Tensor) -> bool:
+        """Whether the lookups run as :func:`~llattn_amd.embedding.embed`: the model is this module's own (its norms too), both
+        tables are plain embeddings of one type on the GPU, and nothing is hooked to them that wants to see their calls."""
+        tables = (self.embedding, self.position)
+        if not input_ids.is_cuda or not self.fuse_embeddings and torch.is_grad_enabled() and any(
+                m.weight.requires_grad for m in tables):
+            return False
+        if type(self.norm) is not RMSNorm or _has_any_global_hook() or any(
+                type(m) is not nn.Embedding or m.max_norm is not None or m.sparse or m.scale_grad_by_freq or not m.weight.is_cuda
+                or m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in tables):
+            return False
+        types = {m.weight.dtype for m in tables}
+        return len(types) == 1 and types <= {torch.float32, torch.bfloat16} and self.position.padding_idx is None \
+            and input_ids.dtype in (torch.int64, torch.int32) and input_ids.shape[-1] <= len(self.position.weight) \
+            and max(len(m.weight) for m in tables) <= MOST_EMBEDDINGS
 
     def _fused_norms(self, x: torch.Tensor) -> bool:
         """Whether each residual add runs inside the following norm (:func:`~llattn_amd.norm.add_rms_norm`): all
@@ -274,11 +335,13 @@ def make_optimizer(model: nn.Module, lr: float = 3e-4, matrices: str = "adamw",
 
 
 def train_step(model: nn.Module, optimizer: torch.optim.Optimizer, inputs: torch.Tensor, targets: torch.Tensor,
-               grad_clip: float = 1.0, fused_loss: bool = True, vocab_piece: Optional[int] = None) -> torch.Tensor:
+               grad_clip: float = 1.0, fused_loss: bool = True, vocab_piece: Optional[int] = None,
+               fused_clip: bool = False) -> torch.Tensor:
     """One bf16-autocast optimiser step: forward, loss, backward, gradient clipping, AdamW update, gradients
     cleared (reference train.py:960-1037 with one micro-step).  ``fused_loss``: the chunked head + cross entropy
     (:meth:`LocalLatentLM.loss`, which ``vocab_piece`` is passed to) instead of full logits and ``F.cross_entropy``.
-    Returns the detached loss (no sync)."""
+    ``fused_clip``: clipping by :func:`~llattn_amd.clip.clip_grad_norm_` (two launches per 128 gradients, the norm summed in 64 bits)
+    instead of torch's.  Returns the detached loss (no sync)."""
     if vocab_piece is not None and not fused_loss:
         raise ValueError("train_step: vocab_piece belongs to the fused loss, and fused_loss=False asks for full logits")
     with torch.autocast(device_type="cuda", dtype=torch.bfloat16):
@@ -289,7 +352,8 @@ def train_step(model: nn.Module, optimizer: torch.optim.Optimizer, inputs: torch
             loss, _ = lm_loss(model(inputs), targets)
         loss.backward()
     if grad_clip > 0:
-        torch.nn.utils.clip_grad_norm_(model.parameters(), grad_clip)
+        clip = clip_grad_norm_ if fused_clip else torch.nn.utils.clip_grad_norm_
+        clip(model.parameters(), grad_clip)
     optimizer.step()
     optimizer.zero_grad(set_to_none=True)
     return loss.detach()

@@ -10,7 +10,8 @@ import torch
 
 from conftest import REPO
 from llattn_amd import _lib as L
-from llattn_amd import clip, clip_grad_norm, clip_grad_norm_, clip_grads_with_norm_, embed, grad_norm
+from llattn_amd import clip, clip_grad_norm, clip_grad_norm_, clip_grads_with_norm_, embed, gated_feed_forward, grad_norm
+from llattn_amd.lm import FeedForward, GatedFeedForward, build_model, train_step
 
 BF16 = torch.bfloat16
 AT = 1 << 20  # a pointer that nothing reads
@@ -20,7 +21,8 @@ def test_header_matches_the_binding(tmp_path):
     text = (REPO / "include" / "llattn_lm.h").read_text()
     names = set(re.findall(r"^\s*(?:int32_t|size_t)\s+(llattn_\w+)\s*\(", text, re.M))
     assert names == set(L.LM_SIGNATURES) and all(hasattr(L.load(), n) for n in names)
-    structs = {"llattn_embed_cfg": L.LlattnEmbedCfg}
+    structs = {"llattn_embed_cfg": L.LlattnEmbedCfg, "llattn_gated_cfg": L.LlattnGatedCfg,
+               "llattn_gated_weights": L.LlattnGatedWeights, "llattn_gated_grads": L.LlattnGatedGrads}
     lines = ["#include <stddef.h>", "#include <stdio.h>", '#include "llattn_lm.h"', "int main(void) {"]
     for c, t in structs.items():
         lines.append(f'printf("%zu\\n", sizeof({c}));')
@@ -157,16 +159,15 @@ def test_nothing_to_clip():
     clip_grads_with_norm_([], 1.0, torch.ones(()))
 
 
-@pytest.mark.parametrize("which", ["embed", "clip"])
+@pytest.mark.parametrize("which", ["embed", "gated", "norm", "clip"])
 def test_forward_mode_tangents_are_refused(which):
     import torch.autograd.forward_ad as fwd
     with fwd.dual_level():
         t = fwd.make_dual(torch.ones(4, 3), torch.ones(4, 3))
+        call = {"embed": lambda: embed(torch.zeros(2, dtype=torch.int64), t), "gated": lambda: gated_feed_forward(t, *_layers(3, 5, 2)),
+                "norm": lambda: grad_norm([t]), "clip": lambda: clip_grad_norm([t], 1.0)}[which]
         with pytest.raises(NotImplementedError, match="forward-mode"):
-            if which == "embed":
-                embed(torch.zeros(2, dtype=torch.int64), t)
-            else:
-                grad_norm([t])
+            call()
 
 
 def test_flat_views():
@@ -177,3 +178,105 @@ def test_flat_views():
         assert f.is_contiguous() and f.data_ptr() == t.data_ptr() and f.numel() == t.numel()
     for t in (x[:, :, ::2], x[:, :2], torch.ones(3).expand(4, 3)):
         assert clip._flat(t) is None
+
+
+# ---------------------------------------------------------------------------
+# gated feed-forward
+# ---------------------------------------------------------------------------
+
+def _layers(D, F, Do, bias=True, dtype=torch.float32):
+    return [torch.nn.Linear(i, o, bias=bias).to(dtype) for i, o in ((D, F), (D, F), (F, Do))]
+
+
+def _gated_cfg(rows=10, D=16, F=24, D_out=8, act=0, dw=0, dw2=1):
+    return L.LlattnGatedCfg(rows, D, F, D_out, act, dw, dw2)
+
+
+@pytest.mark.parametrize("kw", [dict(rows=0), dict(rows=1 << 23), dict(D=0), dict(D=12), dict(F=4), dict(D_out=-8), dict(F=1 << 22), dict(act=2),
+                                dict(dw=2), dict(dw2=-1)], ids=str)
+def test_gated_sizes_refused(kw):
+    for which in (0, 1):
+        assert L.load().llattn_gated_bytes(ctypes.byref(_gated_cfg(**kw)), which) == 0 and L.load().llattn_last_error()
+    assert L.load().llattn_gated_bytes(ctypes.byref(_gated_cfg()), 2) == 0
+
+
+@pytest.mark.parametrize("kw,code", [(dict(x=None), 3), (dict(x=AT + 8), 3), (dict(ldx=8), 3), (dict(ldx=20), 3), (dict(ldx=1 << 23), 3), (dict(W1=None), 3),
+                                     (dict(W3=AT + 2), 3), (dict(b1=AT + 4), 3), (dict(y=None), 3), (dict(p=None), 3), (dict(s=None), 3),
+                                     (dict(h=None), 3), (dict(h=AT + 8), 3), (dict(ws=None), 5), (dict(ws=AT + 8), 5), (dict(n=100), 5)], ids=str)
+def test_gated_forward_refused(kw, code):
+    lib, cfg = L.load(), _gated_cfg()
+    a = dict(x=AT, ldx=16, W1=AT, W3=AT, W2=AT, b1=None, h=AT, p=AT, s=AT, y=AT, ws=AT, n=lib.llattn_gated_bytes(ctypes.byref(cfg), 0)) | kw
+    w = L.LlattnGatedWeights(a["W1"], a["W3"], a["W2"], a["b1"], None, None)
+    assert lib.llattn_gated_fwd(ctypes.byref(cfg), a["x"], a["ldx"], ctypes.byref(w), a["h"], a["p"], a["s"], a["y"], a["ws"], a["n"], None) == code
+
+
+@pytest.mark.parametrize("kw,code", [(dict(x=None), 3), (dict(h=None), 3), (dict(dy=None), 3), (dict(p=AT + 8), 3), (dict(dx=AT + 8), 3),
+                                     (dict(dW1=None), 3), (dict(dW3=None), 3), (dict(ws=None), 5), (dict(n=100), 5)], ids=str)
+def test_gated_backward_refused(kw, code):
+    lib, cfg = L.load(), _gated_cfg()
+    a = dict(x=AT, h=AT, p=AT, s=AT, dy=AT, dx=AT, dW1=AT, dW3=AT, dW2=AT, ws=AT, n=lib.llattn_gated_bytes(ctypes.byref(cfg), 1)) | kw
+    w = L.LlattnGatedWeights(AT, AT, AT, None, None, None)
+    g = L.LlattnGatedGrads(a["dx"], a["dW1"], a["dW3"], a["dW2"], None, None, None)
+    assert lib.llattn_gated_bwd(ctypes.byref(cfg), a["x"], 16, ctypes.byref(w), a["h"], a["p"], a["s"], a["dy"], ctypes.byref(g), a["ws"],
+                                a["n"], None) == code
+
+
+def test_gated_refusals():
+    x, ls = torch.zeros(2, 3), _layers(3, 5, 2)
+    for args, kw, msg in [((x, *ls), dict(act="relu"), "act"), ((x[:, :2], *ls), {}, "match"), ((x, ls[0], ls[2], ls[2]), {}, "match"),
+                          ((x, ls[0], ls[1], ls[0]), {}, "match"), ((torch.zeros(()), *ls), {}, "match"), ((x.double(), *ls), {}, "float32"),
+                          ((x, ls[0], ls[1].half(), ls[2]), {}, "float32")]:
+        with pytest.raises(ValueError, match=msg):
+            gated_feed_forward(*args, **kw)
+    bad = _layers(3, 5, 2)
+    bad[0].bias = torch.nn.Parameter(torch.zeros(4))
+    with pytest.raises(ValueError, match="bias"):
+        gated_feed_forward(x, *bad)
+    with pytest.raises(RuntimeError, match="MI355X"):
+        gated_feed_forward(x, *_layers(3, 5, 2))
+
+
+# ---------------------------------------------------------------------------
+# the model
+# ---------------------------------------------------------------------------
+
+def _model(**kw):
+    return build_model(vocab_size=40, max_seq_len=16, d_model=16, n_heads=2, n_layers=2, d_ff=24, latent_d_model=8, latent_heads=1, **kw)
+
+
+def test_models_with_a_gate():
+    m = _model()
+    assert type(m.blocks[0].ff) is FeedForward and m.config.ffn == "gelu"
+    for name, act in (("swiglu", "silu"), ("geglu", "gelu")):
+        m = _model(ffn=name)
+        ff = m.blocks[1].ff
+        assert type(ff) is GatedFeedForward and ff.act == act and ff.w3.weight.shape == (24, 16)
+        assert float(ff.w2.weight.std()) < 0.8 * float(ff.w3.weight.std())  # scaled as an output projection
+        x = torch.randn(3, 16)
+        f = torch.nn.functional.silu if act == "silu" else torch.nn.functional.gelu
+        assert torch.equal(ff(x), ff.w2(f(ff.w1(x)) * ff.w3(x)))  # on the CPU: torch's own
+    with pytest.raises(ValueError, match="ffn"):
+        _model(ffn="relu")
+
+
+def test_lookups_on_the_cpu_are_torchs():
+    m = _model()
+    ids = torch.zeros(2, 5, dtype=torch.int64)
+    assert not m._fused_embeddings(ids) and not m.config.fused_embeddings
+    m = _model(fused_embeddings=True)
+    assert m.fuse_embeddings and not m._fused_embeddings(ids)
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_the_training_step_clips_as_asked(fused, monkeypatch):
+    from llattn_amd import lm
+    calls = []
+    monkeypatch.setattr(lm, "clip_grad_norm_", lambda p, most: calls.append(("own", most)))
+    monkeypatch.setattr(torch.nn.utils, "clip_grad_norm_", lambda p, most: calls.append(("torch", most)))
+
+    class Linear(torch.nn.Linear):
+        def loss(self, x, t):
+            return (self(x) - t).square().mean(), {}
+    m = Linear(3, 2)
+    train_step(m, torch.optim.SGD(m.parameters(), 0.1), torch.ones(4, 3), torch.ones(4, 2), grad_clip=0.5, fused_clip=fused)
+    assert calls == [("own" if fused else "torch", 0.5)]
