@@ -35,11 +35,15 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_f __attribute__((aligned(4)));
 typedef u32x4 u32x4_h __attribute__((aligned(2)));
 
-// 16 bytes of a row at any alignment of whole elements; `left` elements remain in the row
-template <typename T>
+// Pieces of a lane, all held at the same time (1 to 4 tried: embedding rows of 5632 bytes 40 us with 1 and 2)
+constexpr int kTurns = 2;
+
+// 16 bytes of a row at any alignment of whole elements; `left` elements remain in the row.  RAGGED: rows of not a whole
+// number of pieces
+template <typename T, bool RAGGED>
 __device__ __forceinline__ u32x4 load_piece(const T* p, int left) {
   constexpr int N = Vec16<T>::N;
-  if (left >= N) {
+  if (!RAGGED || left >= N) {
     if constexpr (N == 4) return *reinterpret_cast<const u32x4_f*>(p);
     else return *reinterpret_cast<const u32x4_h*>(p);
   }
@@ -50,12 +54,14 @@ __device__ __forceinline__ u32x4 load_piece(const T* p, int left) {
   }
   return v;
 }
-template <typename T>
+// Non-temporal: what is written does not push out of the caches what is read (the tables' rows, dout: 32768 x 1408 forward 71 us
+// otherwise against 40, the last launch backward 137 against 83).
+template <typename T, bool RAGGED>
 __device__ __forceinline__ void store_piece(T* p, u32x4 v, int left) {
   constexpr int N = Vec16<T>::N;
-  if (left >= N) {
-    if constexpr (N == 4) *reinterpret_cast<u32x4_f*>(p) = v;
-    else *reinterpret_cast<u32x4_h*>(p) = v;
+  if (!RAGGED || left >= N) {
+    if constexpr (N == 4) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_f*>(p));
+    else __builtin_nontemporal_store(v, reinterpret_cast<u32x4_h*>(p));
     return;
   }
   for (int e = 0; e < left; ++e) {
@@ -87,14 +93,17 @@ __device__ __forceinline__ u32x4 pack(const float (&o)[Vec16<T>::N]) {
   return v;
 }
 
-// A row's 16-byte pieces are shared by `width` lanes (8 to 64) of a wave, in `parts` tasks of `per` pieces each.
-struct Split { int pieces, width, parts, per; };
-// Threads of a launch whose workgroups may pass 2^32 threads in one dimension
-__device__ __forceinline__ int64_t thread_of() { return ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; }
-struct Task { int row, from, to, lane; };
-__device__ __forceinline__ Task task_of(const Split& s, int64_t task, int lane) {
-  const int row = (int)(task / s.parts), part = (int)(task - (int64_t)row * s.parts);
-  return Task{row, part * s.per, min((part + 1) * s.per, s.pieces), lane};
+// A row's 16-byte pieces are shared by 2^shift lanes (8 to 64) of a wave, in `parts` tasks of `per` pieces each, up to kTurns a
+// lane.  A workgroup takes one part of 256 / 2^shift rows; workgroups of neighbouring parts follow one another, all those of one
+// set of rows (`blocks`) before the next set's.  (Divisions by workgroup, in scalar registers: by thread they took longer than the
+// memory.)
+struct Split { int pieces, shift, parts, per; };
+struct Task { int row, from, to, lane, width; };
+__device__ __forceinline__ int64_t block_of() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+__device__ __forceinline__ Task task_of(const Split& s, int64_t block) {
+  const uint32_t group = (uint32_t)block / (uint32_t)s.parts, part = (uint32_t)block - group * s.parts;
+  const int lw = s.shift, from = (int)part * s.per;
+  return Task{(int)((group << (8 - lw)) + (threadIdx.x >> lw)), from, min(from + s.per, s.pieces), (int)threadIdx.x & ((1 << lw) - 1), 1 << lw};
 }
 
 __device__ __forceinline__ int64_t index_at(const void* p, int bytes, int64_t n) {
@@ -111,51 +120,60 @@ struct FwdArgs {
   Split split;
 };
 
-template <typename T>
+template <typename T, bool RAGGED>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const FwdArgs a) {
   constexpr int N = Vec16<T>::N;
-  const int64_t t = thread_of() / a.split.width;
-  if (t >= (int64_t)a.rows * a.split.parts) return;
-  const Task k = task_of(a.split, t, threadIdx.x % a.split.width);
+  const Task k = task_of(a.split, block_of());
+  if ((uint32_t)k.row >= (uint32_t)a.rows) return;
   const int64_t id = index_at(a.ids, a.index_bytes, k.row);
-  const int64_t p = a.P ? a.pos ? index_at(a.pos, a.index_bytes, k.row) : k.row % a.T : 0;
+  const int64_t p = a.P ? a.pos ? index_at(a.pos, a.index_bytes, k.row) : (uint32_t)k.row % (uint32_t)a.T : 0;
   const bool ok = id >= 0 && id < a.V && (!a.P || (p >= 0 && p < a.P));
   const T* w = static_cast<const T*>(a.W) + (ok ? id : 0) * a.ldw;
   const T* q = static_cast<const T*>(a.Pos) + (ok ? p : 0) * a.ldp;
   T* o = static_cast<T*>(a.out) + (int64_t)k.row * a.D;
-  for (int c = k.from + k.lane; c < k.to; c += a.split.width) {
-    const int d = c * N, left = a.D - d;
-    float x[N], y[N];
-    unpack<T>(load_piece(w + d, left), x);
-    if (a.P) unpack<T>(load_piece(q + d, left), y);
+  u32x4 x[kTurns], y[kTurns];  // every load before the first store
+#pragma unroll
+  for (int u = 0; u < kTurns; ++u) {
+    const int c = k.from + k.lane + u * k.width, d = c * N;
+    if (c < k.to) {
+      x[u] = load_piece<T, RAGGED>(w + d, a.D - d);
+      if (a.P) y[u] = load_piece<T, RAGGED>(q + d, a.D - d);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kTurns; ++u) {
+    const int c = k.from + k.lane + u * k.width, d = c * N;
+    if (c >= k.to) continue;
+    float f[N], g[N];
+    unpack<T>(x[u], f);
+    unpack<T>(y[u], g);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      x[e] = a.P ? fmaf(a.scale, x[e], y[e]) : a.scale * x[e];
-      if (!ok) x[e] = __builtin_nanf("");
+      f[e] = a.P ? fmaf(a.scale, f[e], g[e]) : a.scale * f[e];
+      if (!ok) f[e] = __builtin_nanf("");
     }
-    store_piece(o + d, pack<T>(x), left);
+    store_piece<T, RAGGED>(o + d, pack<T>(f), a.D - d);
   }
 }
 
-// Rows by key.  order: rows, the runs of a bucket one after another; runs[key]: first and one past the last position of its run.
+// Rows by key.  order: rows, the runs of a bucket one after another; runs: first and one past the last position of each key's run.
 struct Keys {
   const void* keys;       // null: row n has key n % T, and nothing is written (runs of `alike` rows)
   int index_bytes;
   int T, alike;
   int R;                  // keys outside [0, R) and `padding` have no run
   int64_t padding;
-  int buckets;            // a power of two, R <= kKeys buckets
+  int buckets, per;       // buckets: a power of two, of `per` keys at most (R <= per buckets, per <= kKeys)
   int32_t* order;
-  int2* runs;
+  int2* runs;             // by bucket, then by key
   int2* list;             // scratch [rows]
 };
-__device__ __forceinline__ int row_at(const Keys& s, int i) {
-  return s.keys ? s.order[i] : (i % s.alike) * s.T + i / s.alike;
-}
+// The run of a key, and the row that stands j-th in it
 __device__ __forceinline__ int2 run_of(const Keys& s, int key) {
-  if (s.keys) return s.runs[key];
+  if (s.keys) return s.runs[(key & (s.buckets - 1)) * s.per + (key >> (31 - __builtin_clz(s.buckets)))];
   return key < s.T ? make_int2(key * s.alike, (key + 1) * s.alike) : make_int2(0, 0);
 }
+__device__ __forceinline__ int row_at(const Keys& s, int2 run, int key, int j) { return s.keys ? s.order[run.x + j] : j * s.T + key; }
 __device__ __forceinline__ int key_at(const Keys& s, int i) {  // of position i < the number of rows that have runs
   return s.keys ? (int)index_at(s.keys, s.index_bytes, s.order[i]) : i / s.alike;
 }
@@ -167,7 +185,9 @@ struct SortArgs {
   int32_t* counted;  // rows that have runs, of each set
 };
 
-// What a workgroup reads of 16 waves x 64 keys at a time: latency-bound, so several such pieces are in flight.
+// The keys of a workgroup's waves, 64 at a time, stay in registers between the counting and the collecting where they are no
+// more than kSteps times 64 a wave (32768 rows); others are read again.
+constexpr int kSteps = 32;
 __global__ __launch_bounds__(64 * kWaves) void embed_sort_kernel(const SortArgs a) {
   __shared__ int2 list[kList];
   __shared__ int count[kWaves][kKeys];
@@ -175,39 +195,55 @@ __global__ __launch_bounds__(64 * kWaves) void embed_sort_kernel(const SortArgs 
   const int which = (int)blockIdx.x >= a.first[1];
   const Keys& s = a.set[which];
   const int b = blockIdx.x - a.first[which], mask = s.buckets - 1, shift = 31 - __builtin_clz(s.buckets);
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int64_t seg = ((a.rows + kWaves - 1) / kWaves + 63) / 64 * 64;
   const int64_t lo = min((int64_t)a.rows, w * seg), hi = min((int64_t)a.rows, lo + seg);
-  const auto key_of = [&](int64_t n) -> int {  // or -1
-    if (n >= hi) return -1;
-    const int64_t k = index_at(s.keys, s.index_bytes, n);
-    return k >= 0 && k < s.R && k != s.padding ? (int)k : -1;
-  };
-  constexpr int U = 8;
-  int eq = 0, lt = 0, all = 0;
-  for (int64_t n = lo; n < hi; n += 64 * U) {
-    int k[U];
+  constexpr uint32_t kNone = 0xffffffffu;
+  const uint32_t padding = s.padding < 0 ? kNone : (uint32_t)s.padding;
+  uint32_t key[kSteps];
+  const auto read = [&](int64_t n0) {  // the keys n0 + 64 u + lane; kNone: none that has a run
 #pragma unroll
-    for (int u = 0; u < U; ++u) k[u] = key_of(n + 64 * u + lane);
+    for (int u0 = 0; u0 < kSteps; u0 += 16) {
+      if (n0 + 64 * u0 >= hi) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      eq += k[u] >= 0 && (k[u] & mask) == b;
-      lt += k[u] >= 0 && (k[u] & mask) < b;
-      all += k[u] >= 0;
+        for (int u = 0; u < 16; ++u) key[u0 + u] = kNone;
+        continue;
+      }
+      uint2 raw[16];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        const int64_t n = n0 + 64 * (u0 + u) + lane;
+        raw[u] = make_uint2(kNone, 0);
+        if (n < hi) {
+          if (s.index_bytes == 8) raw[u] = static_cast<const uint2*>(s.keys)[n];
+          else raw[u].x = static_cast<const uint32_t*>(s.keys)[n];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 16; ++u)
+        key[u0 + u] = raw[u].y == 0 && raw[u].x < (uint32_t)s.R && raw[u].x != padding ? raw[u].x : kNone;
     }
-  }
+  };
+  // a key's residue class; past every one for none
+  const auto bucket = [&](uint32_t k) { return k == kNone ? kNone : k & (uint32_t)mask; };
+  int eq = 0, lt = 0, all = 0;
+  for (int64_t n = lo; n < hi; n += 64 * kSteps) {
+    read(n);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    eq += __shfl_xor(eq, o);
-    lt += __shfl_xor(lt, o);
-    all += __shfl_xor(all, o);
+    for (int u = 0; u < kSteps; ++u) {
+      if (n + 64 * u >= hi) continue;
+      const uint32_t k = bucket(key[u]);
+      eq += __popcll(__ballot(k == (uint32_t)b));
+      lt += __popcll(__ballot(k < (uint32_t)b));
+      if (b == 0) all += __popcll(__ballot(k != kNone));
+    }
   }
   if (lane == 0) {
     eq_of[w] = eq;
     lt_of[w] = lt;
     all_of[w] = all;
   }
-  for (int i = threadIdx.x; i < kWaves * kKeys; i += 64 * kWaves) (&count[0][0])[i] = 0;
+  for (int i = lane; i < s.per; i += 64) count[w][i] = 0;
   __syncthreads();
   int base = 0, n_list = 0, at = 0, total = 0;
 #pragma unroll
@@ -221,15 +257,14 @@ __global__ __launch_bounds__(64 * kWaves) void embed_sort_kernel(const SortArgs 
   // this bucket's rows in their order
   int2* const kept = n_list <= kList ? list : s.list + base;
   if (eq) {
-    for (int64_t n = lo; n < hi; n += 64 * U) {
-      int k[U];
+    for (int64_t n = lo; n < hi; n += 64 * kSteps) {
+      if (seg > 64 * kSteps) read(n);
 #pragma unroll
-      for (int u = 0; u < U; ++u) k[u] = key_of(n + 64 * u + lane);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool mine = k[u] >= 0 && (k[u] & mask) == b;
+      for (int u = 0; u < kSteps; ++u) {
+        const bool mine = bucket(key[u]) == (uint32_t)b;
         const uint64_t m = __ballot(mine);
-        if (mine) kept[at + __popcll(m & ((1ull << lane) - 1))] = make_int2((int)(n + 64 * u + lane), k[u] >> shift);
+        if (!m) continue;
+        if (mine) kept[at + __popcll(m & ((1ull << lane) - 1))] = make_int2((int)(n + 64 * u + lane), (int)(key[u] >> shift));
         at += __popcll(m);
       }
     }
@@ -240,13 +275,13 @@ __global__ __launch_bounds__(64 * kWaves) void embed_sort_kernel(const SortArgs 
   const int from = min(n_list, w * step), to = min(n_list, from + step);
   for (int i = from + lane; i < to; i += 64) atomicAdd(&count[w][kept[i].y], 1);
   __syncthreads();
-  if (threadIdx.x < kKeys) {
-    const int k = threadIdx.x;
+  const int k = threadIdx.x;
+  if (w * 64 < s.per) {
     int c[kWaves], mine = 0;
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) {
       c[v] = mine;
-      mine += count[v][k];
+      mine += k < s.per ? count[v][k] : 0;
     }
     int before = mine;  // inclusive scan over the 64 keys of this wave
 #pragma unroll
@@ -255,21 +290,23 @@ __global__ __launch_bounds__(64 * kWaves) void embed_sort_kernel(const SortArgs 
       if (lane >= o) before += x;
     }
     if (lane == 63) sums[w] = before;
-    before -= mine;
-#pragma unroll
-    for (int v = 0; v < kWaves; ++v) count[v][k] = before + c[v];
-    // waves of the keys before are added below, once their sums are there
+    lt = before - mine;
     eq = mine;
-    lt = before;
+    if (k < s.per) {
+#pragma unroll
+      for (int v = 0; v < kWaves; ++v) count[v][k] = lt + c[v];
+    }
   }
   __syncthreads();
-  if (threadIdx.x < kKeys) {
-    int more = 0;
+  if (k < s.per) {
+    int more = 0;  // the keys of the waves before
     for (int v = 0; v < w; ++v) more += sums[v];
+    if (more) {
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) count[v][threadIdx.x] += more;
-    const int64_t key = b + ((int64_t)threadIdx.x << shift);
-    if (key < s.R) s.runs[key] = eq ? make_int2(base + more + lt, base + more + lt + eq) : make_int2(0, 0);
+      for (int v = 0; v < kWaves; ++v) count[v][k] += more;
+    }
+    const int first = base + more + lt;
+    s.runs[b * s.per + k] = eq ? make_int2(first, first + eq) : make_int2(0, 0);
   }
   __syncthreads();
   for (int i = from; i < to; i += 64) {
@@ -295,7 +332,8 @@ static_assert(kKeys == 1 << 9, "bits of a key within its bucket");
 
 struct BwdArgs {
   Keys set[2];
-  int64_t tasks[3];        // first task of each set
+  int64_t blocks, total;   // workgroups of the first set, and of both
+  int n_rows[2];           // rows of this launch's results, of each set
   int rows, D;
   const int32_t* counted;  // rows that have runs, of the sorted sets
   const void* dout;
@@ -307,134 +345,303 @@ struct BwdArgs {
   int Dp;
 };
 
-// acc += the rows at `get(i)`, i < n, in order
-template <typename T, typename F>
-__device__ __forceinline__ void add_rows(float (&acc)[Vec16<T>::N], int n, int left, F&& get) {
-  constexpr int N = Vec16<T>::N, U = 8;
-  int i = 0;
-  for (; i + U <= n; i += U) {
-    u32x4 v[U];
+// The pieces of one lane of a row of sums
+template <typename T>
+struct Sum {
+  static constexpr int N = Vec16<T>::N;
+  float v[kTurns][N];
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = load_piece(get(i + u), left);
+    for (int u = 0; u < kTurns; ++u)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float x[N];
-      unpack<T>(v[u], x);
-#pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] += x[e];
-    }
+      for (int e = 0; e < N; ++e) v[u][e] = 0.f;
   }
-  for (; i < n; ++i) {
-    float x[N];
-    unpack<T>(load_piece(get(i), left), x);
+  __device__ __forceinline__ void add(const Sum& x) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] += x[e];
+    for (int u = 0; u < kTurns; ++u)
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[u][e] += x.v[u][e];
+  }
+};
+
+// sum += the rows of T that start at get(i), i < n, in order, U at a time
+template <typename T, bool RAGGED, int U, typename F>
+__device__ __forceinline__ void add_rows(Sum<T>& sum, int n, const Task& k, int D, F&& get) {
+  constexpr int N = Vec16<T>::N;
+  for (int i = 0; i < n; i += U) {
+    u32x4 v[U][kTurns];
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      const T* p = i + q < n ? get(i + q) : nullptr;
+#pragma unroll
+      for (int u = 0; u < kTurns; ++u) {
+        const int c = k.from + k.lane + u * k.width;
+        v[q][u] = u32x4{0, 0, 0, 0};
+        if (p && c < k.to) v[q][u] = load_piece<T, RAGGED>(p + c * N, D - c * N);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      if (i + q >= n) break;
+#pragma unroll
+      for (int u = 0; u < kTurns; ++u) {
+        float x[N];
+        unpack<T>(v[q][u], x);
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum.v[u][e] += x[e];
+      }
+    }
   }
 }
 
-// The first position of the block of `size` positions that starts in [c size, (c + 1) size), or -1
-__device__ __forceinline__ int block_start(const Keys& s, int counted, int c, int size) {
+// sum += the rows of fp32 sums that start at get(i), i < n, in order
+template <typename T, typename F>
+__device__ __forceinline__ void add_sums(Sum<T>& sum, int n, const Task& k, F&& get) {
+  constexpr int N = Vec16<T>::N, U = 4;
+  for (int i = 0; i < n; i += U) {
+    float4 v[U][kTurns][N / 4];
+#pragma unroll
+    for (int q = 0; q < U; ++q)
+#pragma unroll
+      for (int u = 0; u < kTurns; ++u)
+#pragma unroll
+        for (int e = 0; e < N / 4; ++e) {
+          const int c = k.from + k.lane + u * k.width;
+          v[q][u][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i + q < n && c < k.to) v[q][u][e] = *reinterpret_cast<const float4*>(get(i + q) + c * N + 4 * e);
+        }
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      if (i + q >= n) break;
+#pragma unroll
+      for (int u = 0; u < kTurns; ++u)
+#pragma unroll
+        for (int e = 0; e < N / 4; ++e) {
+          sum.v[u][4 * e] += v[q][u][e].x;
+          sum.v[u][4 * e + 1] += v[q][u][e].y;
+          sum.v[u][4 * e + 2] += v[q][u][e].z;
+          sum.v[u][4 * e + 3] += v[q][u][e].w;
+        }
+    }
+  }
+}
+
+// The block of `size` positions that starts in [c size, (c + 1) size): its run and key, and where in the run it starts (-1: there
+// is none)
+struct Block { int2 run; int key, at; };
+__device__ __forceinline__ Block block_at(const Keys& s, int counted, int c, int size) {
   const int64_t last = (int64_t)c * size + size - 1;
-  if (last >= counted) return -1;
-  const int2 r = run_of(s, key_at(s, (int)last));
-  const int at = r.x + ((int)last - r.x) / size * size;
-  return at + size <= r.y ? at : -1;
+  if (last >= counted) return Block{make_int2(0, 0), 0, -1};
+  const int key = key_at(s, (int)last);
+  const int2 run = run_of(s, key);
+  const int at = ((int)last - run.x) / size * size;
+  return Block{run, key, at + size <= run.y - run.x ? at : -1};
+}
+
+// This workgroup's set and task
+__device__ __forceinline__ Task task_in(const BwdArgs& a, const Split& split, int& set) {
+  int64_t b = block_of();
+  set = b >= a.blocks;
+  if (set) b -= a.blocks;
+  Task k = task_of(split, b);
+  if ((uint32_t)k.row >= (uint32_t)a.n_rows[set]) k.row = -1;
+  return k;
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void embed_leaf_kernel(const BwdArgs a) {
+__device__ __forceinline__ void store_sums(float* o, const Sum<T>& x, const Task& k) {
   constexpr int N = Vec16<T>::N;
-  const int64_t t = thread_of() / a.split.width;
-  const int set = t >= a.tasks[1];
-  if (t >= a.tasks[2]) return;
-  const Keys& s = a.set[set];
-  const Task k = task_of(a.split, t - a.tasks[set], threadIdx.x % a.split.width);
-  const int at = block_start(s, s.keys ? a.counted[set] : a.rows, k.row, kLeaf);
-  if (at < 0) return;
-  float* const o = a.leaf[set] + (int64_t)k.row * a.Dp;
-  for (int c = k.from + k.lane; c < k.to; c += a.split.width) {
-    const int d = c * N, left = a.D - d;
-    float acc[N] = {};
-    add_rows<T>(acc, kLeaf, left, [&](int i) { return static_cast<const T*>(a.dout) + (int64_t)row_at(s, at + i) * a.D + d; });
 #pragma unroll
-    for (int e = 0; e < N; e += 4) *reinterpret_cast<float4*>(o + d + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+  for (int u = 0; u < kTurns; ++u) {
+    const int c = k.from + k.lane + u * k.width;
+    if (c >= k.to) continue;
+#pragma unroll
+    for (int e = 0; e < N; e += 4)
+      *reinterpret_cast<float4*>(o + c * N + e) = make_float4(x.v[u][e], x.v[u][e + 1], x.v[u][e + 2], x.v[u][e + 3]);
   }
+}
+
+template <typename T, bool RAGGED>
+__global__ __launch_bounds__(256) void embed_leaf_kernel(const BwdArgs a) {
+  int set;
+  const Task k = task_in(a, a.split, set);
+  if (k.row < 0 || block_of() >= a.total) return;
+  const Keys& s = a.set[set];
+  const Block b = block_at(s, s.keys ? a.counted[set] : a.rows, k.row, kLeaf);
+  if (b.at < 0) return;
+  Sum<T> sum;
+  sum.zero();
+  add_rows<T, RAGGED, 8>(sum, kLeaf, k, a.D,
+                         [&](int i) { return static_cast<const T*>(a.dout) + (int64_t)row_at(s, b.run, b.key, b.at + i) * a.D; });
+  store_sums(a.leaf[set] + (int64_t)k.row * a.Dp, sum, k);
 }
 
 __global__ __launch_bounds__(256) void embed_node_kernel(const BwdArgs a) {
-  const int64_t t = thread_of() / a.fsplit.width;
-  const int set = t >= a.tasks[1];
-  if (t >= a.tasks[2]) return;
+  int set;
+  const Task k = task_in(a, a.fsplit, set);
+  if (k.row < 0 || block_of() >= a.total) return;
   const Keys& s = a.set[set];
-  const Task k = task_of(a.fsplit, t - a.tasks[set], threadIdx.x % a.fsplit.width);
-  const int at = block_start(s, s.keys ? a.counted[set] : a.rows, k.row, kLeaf * kLeaf);
-  if (at < 0) return;
+  const Block b = block_at(s, s.keys ? a.counted[set] : a.rows, k.row, kLeaf * kLeaf);
+  if (b.at < 0) return;
+  const float* const leaf = a.leaf[set] + (int64_t)((b.run.x + b.at) / kLeaf) * a.Dp;
   float* const o = a.node[set] + (int64_t)k.row * a.Dp;
-  for (int c = k.from + k.lane; c < k.to; c += a.fsplit.width) {
-    float acc[4] = {};
-    add_rows<float>(acc, kLeaf, 4, [&](int i) { return a.leaf[set] + (int64_t)(at / kLeaf + i) * a.Dp + 4 * c; });
-    *reinterpret_cast<float4*>(o + 4 * c) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  for (int c = k.from + k.lane; c < k.to; c += k.width) {
+    float4 v[kLeaf];
+#pragma unroll
+    for (int i = 0; i < kLeaf; ++i) v[i] = *reinterpret_cast<const float4*>(leaf + (int64_t)i * a.Dp + 4 * c);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kLeaf; ++i) x = make_float4(x.x + v[i].x, x.y + v[i].y, x.z + v[i].z, x.w + v[i].w);
+    *reinterpret_cast<float4*>(o + 4 * c) = x;
   }
 }
 
-// Rows of sums, of a whole run: the blocks of 1024, those of 32 behind them, the rows behind those
-template <typename T>
-__global__ __launch_bounds__(256) void embed_bwd_kernel(const BwdArgs a) {
+template <typename T, bool RAGGED>
+__device__ __forceinline__ void store_row(const BwdArgs& a, int set, const Task& k, const Sum<T>& sum) {
   constexpr int N = Vec16<T>::N;
-  const int64_t t = thread_of() / a.split.width;
-  const int set = t >= a.tasks[1];
-  if (t >= a.tasks[2]) return;
+  T* const o = static_cast<T*>(a.out[set]) + (int64_t)k.row * a.D;
+#pragma unroll
+  for (int u = 0; u < kTurns; ++u) {
+    const int c = k.from + k.lane + u * k.width;
+    if (c >= k.to) continue;
+    float x[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = sum.v[u][e] * a.scale[set];
+    store_piece<T, RAGGED>(o + c * N, pack<T>(x), a.D - c * N);
+  }
+}
+
+// Rows of the tables' gradients, of a whole run each: the blocks of 1024, those of 32 behind them, the rows behind those
+template <typename T, bool RAGGED>
+__global__ __launch_bounds__(256) void embed_bwd_kernel(const BwdArgs a) {
+  int set;
+  const Task k = task_in(a, a.split, set);
+  if (k.row < 0 || block_of() >= a.total) return;
   const Keys& s = a.set[set];
-  const Task k = task_of(a.split, t - a.tasks[set], threadIdx.x % a.split.width);
   const int2 run = run_of(s, k.row);
   const int L = run.y - run.x, nodes = L / (kLeaf * kLeaf), leaves = L / kLeaf - nodes * kLeaf, rest = L % kLeaf;
-  T* const o = static_cast<T*>(a.out[set]) + (int64_t)k.row * a.D;
-  const int leaf0 = run.x + nodes * kLeaf * kLeaf, row0 = run.y - rest;
-  for (int c = k.from + k.lane; c < k.to; c += a.split.width) {
-    const int d = c * N, left = a.D - d;
-    float acc[N] = {};
-    for (int e = 0; e < N && nodes; e += 4) {
-      float x[4] = {};
-      add_rows<float>(x, nodes, 4, [&](int i) { return a.node[set] + (int64_t)(run.x / (kLeaf * kLeaf) + i) * a.Dp + d + e; });
-#pragma unroll
-      for (int q = 0; q < 4; ++q) acc[e + q] += x[q];
-    }
-    for (int e = 0; e < N && leaves; e += 4) {
-      float x[4] = {};
-      add_rows<float>(x, leaves, 4, [&](int i) { return a.leaf[set] + (int64_t)(leaf0 / kLeaf + i) * a.Dp + d + e; });
-#pragma unroll
-      for (int q = 0; q < 4; ++q) acc[e + q] += x[q];
-    }
-    if (rest) {
-      float x[N] = {};
-      add_rows<T>(x, rest, left, [&](int i) { return static_cast<const T*>(a.dout) + (int64_t)row_at(s, row0 + i) * a.D + d; });
-#pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] += x[e];
-    }
-#pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] *= a.scale[set];
-    store_piece(o + d, pack<T>(acc), left);
+  Sum<T> sum;
+  sum.zero();
+  if (nodes) add_sums<T>(sum, nodes, k, [&](int i) { return a.node[set] + (int64_t)(run.x / (kLeaf * kLeaf) + i) * a.Dp; });
+  if (leaves) {
+    Sum<T> x;
+    x.zero();
+    const int leaf0 = (run.x + nodes * kLeaf * kLeaf) / kLeaf;
+    add_sums<T>(x, leaves, k, [&](int i) { return a.leaf[set] + (int64_t)(leaf0 + i) * a.Dp; });
+    sum.add(x);
   }
+  if (rest) {
+    Sum<T> x;
+    x.zero();
+    add_rows<T, RAGGED, 4>(x, rest, k, a.D,
+                           [&](int i) { return static_cast<const T*>(a.dout) + (int64_t)row_at(s, run, k.row, L - rest + i) * a.D; });
+    sum.add(x);
+  }
+  store_row<T, RAGGED>(a, set, k, sum);
+}
+
+// Few tokens: a wave for every row of the tables looks through the keys itself and adds up what it finds, in the same tree; no
+// other launch and no workspace.
+template <typename T, bool RAGGED>
+__global__ __launch_bounds__(256) void embed_scan_kernel(const BwdArgs a) {
+  constexpr int N = Vec16<T>::N, U = 8;
+  int set;
+  const Task k = task_in(a, a.split, set);
+  if (k.row < 0 || block_of() >= a.total) return;
+  const Keys& s = a.set[set];
+  const int lane = k.lane;
+  const int c = k.from + lane, d = c * N;
+  const bool live = c < k.to;
+  float rest[N] = {}, leaf[N] = {}, node[N] = {};
+  int n = 0;
+  const auto add = [&](const u32x4& v) {
+    float x[N];
+    unpack<T>(v, x);
+#pragma unroll
+    for (int e = 0; e < N; ++e) rest[e] += x[e];
+    ++n;
+    if (n % kLeaf == 0) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        leaf[e] += rest[e];
+        rest[e] = 0.f;
+      }
+      if (n % (kLeaf * kLeaf) == 0) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          node[e] += leaf[e];
+          leaf[e] = 0.f;
+        }
+      }
+    }
+  };
+  const auto load = [&](int row) {
+    u32x4 v = {0, 0, 0, 0};
+    if (live) v = load_piece<T, RAGGED>(static_cast<const T*>(a.dout) + (int64_t)row * a.D + d, a.D - d);
+    return v;
+  };
+  if (s.keys) {
+    for (int n0 = 0; n0 < a.rows; n0 += 64) {
+      const int i = n0 + lane;
+      bool mine = false;
+      if (i < a.rows) {
+        const int64_t key = index_at(s.keys, s.index_bytes, i);
+        mine = key == k.row && key != s.padding;
+      }
+      uint64_t m = __ballot(mine);
+      while (m) {
+        u32x4 v[U];
+        int found = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (!m) break;
+          v[u] = load(n0 + __builtin_ctzll(m));
+          m &= m - 1;
+          ++found;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u < found) add(v[u]);
+      }
+    }
+  } else {
+    const int2 run = run_of(s, k.row);
+    for (int i = run.x; i < run.y; i += U) {
+      u32x4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u < run.y) v[u] = load(row_at(s, run, k.row, i + u - run.x));
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u < run.y) add(v[u]);
+    }
+  }
+  if (!live) return;
+#pragma unroll
+  for (int e = 0; e < N; ++e) rest[e] = ((node[e] + leaf[e]) + rest[e]) * a.scale[set];
+  store_piece<T, RAGGED>(static_cast<T*>(a.out[set]) + (int64_t)k.row * a.D + d, pack<T>(rest), a.D - d);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr size_t up(size_t n) { return (n + 255) & ~size_t(255); }
 
-// Lanes and tasks of a row of D elements: up to four pieces a lane, fewer where there are too few rows to fill the chip.
+// Lanes and tasks of a row of D elements: up to kTurns pieces a lane, fewer where there are too few rows to fill the chip.
 Split split_of(int D, int n, int64_t rows) {
   Split s;
   s.pieces = (int)ceil_div(D, n);
-  s.width = s.pieces > 32 ? 64 : s.pieces > 16 ? 32 : s.pieces > 8 ? 16 : 8;
-  const int turns = (int)ceil_div(s.pieces, s.width), most = rows * s.width >= 64 * 4096 ? 4 : 1;
+  s.shift = s.pieces > 32 ? 6 : s.pieces > 16 ? 5 : s.pieces > 8 ? 4 : 3;
+  const int width = 1 << s.shift, turns = (int)ceil_div(s.pieces, width), most = rows * width >= 64 * 4096 ? kTurns : 1;
   s.parts = (int)ceil_div(turns, most);
-  s.per = (int)ceil_div(turns, s.parts) * s.width;
+  s.per = (int)ceil_div(turns, s.parts) * width;
   s.parts = (int)ceil_div(s.pieces, s.per);
   return s;
 }
 
-dim3 grid_of(int64_t tasks, const Split& s) {
-  const int64_t n = ceil_div(tasks * s.width, 256), x = std::min<int64_t>(n, 1 << 20);
-  return dim3((unsigned)x, (unsigned)ceil_div(n, x));
+// Workgroups of `rows` rows; their grid (a launch holds fewer than 2^32 threads in a dimension)
+int64_t blocks_of(const Split& s, int64_t rows) { return ceil_div(rows, 256 >> s.shift) * s.parts; }
+dim3 grid_of(int64_t blocks) {
+  const int64_t x = std::min<int64_t>(blocks, 1 << 20);
+  return dim3((unsigned)x, (unsigned)ceil_div(blocks, x));
 }
 
 int32_t check(const char* who, const llattn_embed_cfg* c, bool has_pos) {
@@ -457,6 +664,19 @@ int buckets_of(int R) {
   return b;
 }
 
+// Few tokens: pieces shared by whole waves, one a lane
+Split scan_split(int D, int n) {
+  Split s;
+  s.pieces = (int)ceil_div(D, n);
+  s.shift = 6;
+  s.per = 64;
+  s.parts = (int)ceil_div(s.pieces, 64);
+  return s;
+}
+bool scans(const llattn_embed_cfg* c) {
+  return c->rows <= 1024 && ((int64_t)c->V + c->P) * ceil_div(c->D, 256) * c->rows <= 1 << 24;
+}
+
 // Workspace: for a sorted set order, runs and list; for every set the sums of 32 and of 1024 rows; counted
 struct Plan {
   int64_t rows, leaves, nodes;
@@ -467,40 +687,49 @@ struct Plan {
 };
 Plan plan_of(const llattn_embed_cfg* c, bool has_pos) {
   Plan p{};
+  if (scans(c)) return p;
   p.rows = c->rows;
   p.leaves = c->rows / kLeaf;
   p.nodes = c->rows / (kLeaf * kLeaf);
   p.Dp = (c->D + 7) / 8 * 8;
   p.trees = c->P ? 2 : 1;
-  const auto sorted = [&](int R) { return up((size_t)c->rows * 4) + up((size_t)R * 8) + up((size_t)c->rows * 8); };
+  const auto sorted = [&](int R) {
+    const size_t b = buckets_of(R);
+    return up((size_t)c->rows * 4) + up(b * ceil_div(R, b) * 8) + up((size_t)c->rows * 8);
+  };
   p.set_bytes[0] = sorted(c->V);
   p.set_bytes[1] = c->P && has_pos ? sorted(c->P) : 0;
   p.tree_bytes = up((size_t)p.leaves * p.Dp * 4) + up((size_t)p.nodes * p.Dp * 4);
   return p;
 }
 
-template <typename T>
+// The workgroups of n0 rows of one set and n1 of the other
+dim3 blocks_for(BwdArgs& a, const Split& s, int64_t n0, int64_t n1) {
+  a.blocks = blocks_of(s, n0);
+  a.total = a.blocks + blocks_of(s, n1);
+  a.n_rows[0] = (int)n0;
+  a.n_rows[1] = (int)n1;
+  return grid_of(a.total);
+}
+
+template <typename T, bool RAGGED>
 void launch_bwd(BwdArgs& a, const Plan& p, const int64_t (&table)[2], hipStream_t st) {
-  const auto tasks = [&](const Split& s, int64_t n0, int64_t n1) {
-    a.tasks[0] = 0;
-    a.tasks[1] = n0 * s.parts;
-    a.tasks[2] = (n0 + n1) * s.parts;
-    return a.tasks[2];
-  };
   const int64_t on0 = table[0] > 0, on1 = table[1] > 0;
   if (p.leaves) {
     a.split = split_of(a.D, Vec16<T>::N, p.leaves);
-    const int64_t n = tasks(a.split, on0 * p.leaves, on1 * p.leaves);
-    hipLaunchKernelGGL(embed_leaf_kernel<T>, grid_of(n, a.split), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((embed_leaf_kernel<T, RAGGED>), blocks_for(a, a.split, on0 * p.leaves, on1 * p.leaves), dim3(256), 0, st, a);
   }
   if (p.nodes) {
     a.fsplit = split_of(a.Dp, 4, p.nodes);
-    const int64_t n = tasks(a.fsplit, on0 * p.nodes, on1 * p.nodes);
-    hipLaunchKernelGGL(embed_node_kernel, grid_of(n, a.fsplit), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(embed_node_kernel, blocks_for(a, a.fsplit, on0 * p.nodes, on1 * p.nodes), dim3(256), 0, st, a);
   }
   a.split = split_of(a.D, Vec16<T>::N, table[0] + table[1]);
-  const int64_t n = tasks(a.split, table[0], table[1]);
-  hipLaunchKernelGGL(embed_bwd_kernel<T>, grid_of(n, a.split), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((embed_bwd_kernel<T, RAGGED>), blocks_for(a, a.split, table[0], table[1]), dim3(256), 0, st, a);
+}
+template <typename T, bool RAGGED>
+void launch_scan(BwdArgs& a, const int64_t (&table)[2], hipStream_t st) {
+  a.split = scan_split(a.D, Vec16<T>::N);
+  hipLaunchKernelGGL((embed_scan_kernel<T, RAGGED>), blocks_for(a, a.split, table[0], table[1]), dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -520,9 +749,13 @@ extern "C" int32_t llattn_embed_fwd(const llattn_embed_cfg* c, const void* ids, 
     return fail(LLATTN_ERR_LAYOUT, "llattn_embed_fwd: row strides %lld, %lld under D %d, or past 2^40", (long long)ldw, (long long)ldp, c->D);
   FwdArgs a{(int)c->rows, c->T, c->V, c->P, c->D, c->index_bytes, ids, c->P ? pos : nullptr, W, Pos, ldw, ldp, out, c->scale, {}};
   a.split = split_of(c->D, (int)(16 / size), c->rows);
-  const dim3 grid = grid_of(c->rows * a.split.parts, a.split);
-  if (c->dtype == LLATTN_F32) hipLaunchKernelGGL(embed_fwd_kernel<float>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
-  else hipLaunchKernelGGL(embed_fwd_kernel<uint16_t>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  const dim3 grid = grid_of(blocks_of(a.split, c->rows));
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool ragged = c->D % (16 / size) != 0;
+  if (c->dtype == LLATTN_F32 && ragged) hipLaunchKernelGGL((embed_fwd_kernel<float, true>), grid, dim3(256), 0, st, a);
+  else if (c->dtype == LLATTN_F32) hipLaunchKernelGGL((embed_fwd_kernel<float, false>), grid, dim3(256), 0, st, a);
+  else if (ragged) hipLaunchKernelGGL((embed_fwd_kernel<uint16_t, true>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((embed_fwd_kernel<uint16_t, false>), grid, dim3(256), 0, st, a);
   return check_launch("llattn_embed_fwd");
 }
 
@@ -544,23 +777,37 @@ extern "C" int32_t llattn_embed_bwd(const llattn_embed_cfg* c, const void* ids, 
   if (!workspace || workspace_bytes < p.bytes() || !aligned16(workspace))
     return fail(LLATTN_ERR_WORKSPACE, "llattn_embed_bwd: needs %zu workspace bytes (got %zu)", p.bytes(), workspace_bytes);
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t table[2] = {dW ? c->V : 0, dPos ? c->P : 0};
+  const bool f32 = c->dtype == LLATTN_F32, ragged = c->D % (16 / size) != 0, scan = scans(c);
   char* at = static_cast<char*>(workspace);
   const auto take = [&](size_t n) { char* x = at; at += up(n); return x; };
   const size_t r = (size_t)c->rows;
   SortArgs s{};
   s.rows = (int)c->rows;
   s.counted = reinterpret_cast<int32_t*>(take(256));
-  const auto sorted = [&](Keys& k, const void* keys, int R, int64_t padding) {
-    k.keys = keys; k.index_bytes = c->index_bytes; k.R = R; k.padding = padding; k.buckets = buckets_of(R);
+  const auto keyed = [&](Keys& k, const void* keys, int R, int64_t padding) {
+    k.keys = keys; k.index_bytes = c->index_bytes; k.R = R; k.padding = padding; k.buckets = buckets_of(R); k.per = (int)ceil_div(R, k.buckets);
+    if (scan) return;
     k.order = reinterpret_cast<int32_t*>(take(4 * r));
-    k.runs = reinterpret_cast<int2*>(take(8 * (size_t)R));
+    k.runs = reinterpret_cast<int2*>(take(8 * (size_t)k.per * k.buckets));
     k.list = reinterpret_cast<int2*>(take(8 * r));
   };
-  sorted(s.set[0], ids, c->V, c->padding);
-  if (c->P && pos) sorted(s.set[1], pos, c->P, -1);
+  keyed(s.set[0], ids, c->V, c->padding);
+  if (c->P && pos) keyed(s.set[1], pos, c->P, -1);
   else if (c->P) { s.set[1].T = c->T; s.set[1].alike = (int)(c->rows / c->T); }
   BwdArgs a{};
+  a.set[0] = s.set[0]; a.set[1] = s.set[1];
   a.rows = s.rows; a.D = c->D; a.Dp = p.Dp; a.dout = dout;
+  a.counted = s.counted;
+  a.out[0] = dW; a.out[1] = dPos;
+  a.scale[0] = c->scale; a.scale[1] = 1.f;
+  if (scan) {
+    if (f32 && ragged) launch_scan<float, true>(a, table, st);
+    else if (f32) launch_scan<float, false>(a, table, st);
+    else if (ragged) launch_scan<uint16_t, true>(a, table, st);
+    else launch_scan<uint16_t, false>(a, table, st);
+    return check_launch("llattn_embed_bwd");
+  }
   for (int k = 0; k < p.trees; ++k) {
     a.leaf[k] = reinterpret_cast<float*>(take((size_t)p.leaves * p.Dp * 4));
     a.node[k] = reinterpret_cast<float*>(take((size_t)p.nodes * p.Dp * 4));
@@ -568,12 +815,9 @@ extern "C" int32_t llattn_embed_bwd(const llattn_embed_cfg* c, const void* ids, 
   s.first[1] = dW ? s.set[0].buckets : 0;
   s.first[2] = s.first[1] + (dPos && pos ? s.set[1].buckets : 0);
   if (s.first[2]) hipLaunchKernelGGL(embed_sort_kernel, dim3(s.first[2]), dim3(64 * kWaves), 0, st, s);
-  a.set[0] = s.set[0]; a.set[1] = s.set[1];
-  a.counted = s.counted;
-  a.out[0] = dW; a.out[1] = dPos;
-  a.scale[0] = c->scale; a.scale[1] = 1.f;
-  const int64_t table[2] = {dW ? c->V : 0, dPos ? c->P : 0};
-  if (c->dtype == LLATTN_F32) launch_bwd<float>(a, p, table, st);
-  else launch_bwd<uint16_t>(a, p, table, st);
+  if (f32 && ragged) launch_bwd<float, true>(a, p, table, st);
+  else if (f32) launch_bwd<float, false>(a, p, table, st);
+  else if (ragged) launch_bwd<uint16_t, true>(a, p, table, st);
+  else launch_bwd<uint16_t, false>(a, p, table, st);
   return check_launch("llattn_embed_bwd");
 }

@@ -19,41 +19,46 @@ MOST = 1 << 22  # rows of a table
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """A table whose rows are whole, any distance apart."""
-    t = t.detach()
-    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.detach().contiguous()
 
 
 def _index(t: torch.Tensor) -> torch.Tensor:
-    return t.reshape(-1).contiguous() if t.dtype in (torch.int64, torch.int32) else t.reshape(-1).to(torch.int64)
+    """The indices in order, of 32 or 64 bits (their shape is of no matter to a kernel)."""
+    t = t if t.dtype in (torch.int64, torch.int32) else t.to(torch.int64)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _forward(ids, weight, position, positions, scale, padding):
     """(out, the indices and the configuration that a backward reads)."""
-    D = weight.shape[1]
+    V, D = weight.shape
+    dev, dtype = weight.device, weight.dtype
     i, p = _index(ids), None if positions is None else _index(positions)
     if p is not None and p.dtype is not i.dtype:
         i, p = i.to(torch.int64), p.to(torch.int64)
-    T = ids.shape[-1] if ids.dim() else 1
-    cfg = L.LlattnEmbedCfg(i.numel(), max(T, 1), weight.shape[0], 0 if position is None else position.shape[0], D,
-                           L.dtype_code(weight.dtype), i.element_size(), padding, scale)
-    out = torch.empty((*ids.shape, D), dtype=weight.dtype, device=weight.device)
-    if out.numel():
+    shape = ids.shape
+    cfg = L.LlattnEmbedCfg(i.numel(), max(shape[-1] if shape else 1, 1), V, 0 if position is None else position.shape[0], D,
+                           L.dtype_code(dtype), i.element_size(), padding, scale)
+    out = torch.empty((*shape, D), dtype=dtype, device=dev)
+    if cfg.rows:
         w, q = _rows(weight), None if position is None else _rows(position)
         from .ops import _call
-        with L.on_device(weight.device):
-            _call("llattn_embed_fwd", ctypes.byref(cfg), i.data_ptr(), None if p is None else p.data_ptr(), w.data_ptr(), w.stride(0),
-                  None if q is None else q.data_ptr(), 0 if q is None else q.stride(0), out.data_ptr(),
-                  L.stream_ptr(weight.device), work=(2 + (q is not None)) * out.numel() * out.element_size())
+        with L.on_device(dev):
+            _call("llattn_embed_fwd", ctypes.byref(cfg), i.data_ptr(), _ptr(p), w.data_ptr(), w.stride(0), _ptr(q),
+                  0 if q is None else q.stride(0), out.data_ptr(), L.stream_ptr(dev),
+                  work=(2 + (q is not None)) * cfg.rows * D * out.element_size())
     return out, i, p, cfg
 
 
 class _Embed(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, weight, position, positions, scale, padding, grad_enabled):
+    def forward(ctx, ids, weight, position, positions, scale, padding):
         out, i, p, cfg = _forward(ids, weight, position, positions, scale, padding)
-        if grad_enabled:
-            ctx.save_for_backward(i, p)
-            ctx.meta = (cfg, weight.shape, None if position is None else position.shape)
+        ctx.save_for_backward(i, p)
+        ctx.meta = (cfg, weight.shape, None if position is None else position.shape)
         return out
 
     @staticmethod
@@ -61,21 +66,21 @@ class _Embed(torch.autograd.Function):
     def backward(ctx, dout):
         i, p = ctx.saved_tensors
         cfg, w_shape, p_shape = ctx.meta
-        dev = dout.device
-        dw = torch.empty(w_shape, dtype=dout.dtype, device=dev) if ctx.needs_input_grad[1] else None
-        dp = torch.empty(p_shape, dtype=dout.dtype, device=dev) if p_shape is not None and ctx.needs_input_grad[2] else None
-        d = dout.contiguous()
-        n = L.load().llattn_embed_bytes(ctypes.byref(cfg), int(p is not None))
+        dev, dtype = dout.device, dout.dtype
+        need = ctx.needs_input_grad
+        dw = torch.empty(w_shape, dtype=dtype, device=dev) if need[1] else None
+        dp = torch.empty(p_shape, dtype=dtype, device=dev) if p_shape is not None and need[2] else None
+        d = dout if dout.is_contiguous() else dout.contiguous()
+        ref = ctypes.byref(cfg)
+        n = L.load().llattn_embed_bytes(ref, int(p is not None))
         if n == 0:
             L.check(L.ERR_SHAPE, "llattn_embed_bytes")
         ws = torch.empty((n,), dtype=torch.uint8, device=dev)
-        written = sum(t.numel() for t in (dw, dp) if t is not None)
         from .ops import _call
         with L.on_device(dev):
-            _call("llattn_embed_bwd", ctypes.byref(cfg), i.data_ptr(), None if p is None else p.data_ptr(), d.data_ptr(),
-                  None if dw is None else dw.data_ptr(), None if dp is None else dp.data_ptr(), ws.data_ptr(), n,
-                  L.stream_ptr(dev), work=(d.numel() + written) * d.element_size())
-        return None, dw, dp, None, None, None, None
+            _call("llattn_embed_bwd", ref, i.data_ptr(), _ptr(p), d.data_ptr(), _ptr(dw), _ptr(dp), ws.data_ptr(), n,
+                  L.stream_ptr(dev), work=(cfg.rows + cfg.V + cfg.P) * cfg.D * d.element_size())
+        return None, dw, dp, None, None, None
 
 
 def _check_integers(name: str, t: torch.Tensor) -> None:
@@ -127,4 +132,4 @@ def embed(ids: torch.Tensor, weight: torch.Tensor, position: torch.Tensor | None
     args = (ids, weight, position, positions, float(scale), padding)
     if not (torch.is_grad_enabled() and (weight.requires_grad or position is not None and position.requires_grad)):
         return _forward(*args)[0]
-    return _Embed.apply(*args, True)
+    return _Embed.apply(*args)
