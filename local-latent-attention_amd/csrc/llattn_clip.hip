@@ -7,7 +7,10 @@
 // squares, a workgroup over its share of all tensors' chunks; the scaling launch adds the workgroups' sums up again
 // in every workgroup, in one order, so that no launch stands between them.
 //
-// What bounds it: memory.  Gradients are read twice (a norm has to be known before anything is scaled) and written once.
+// What bounds it: memory.  Gradients are read twice (a norm has to be known before anything is scaled) and written once, past the
+// caches (non-temporal), which are left to what the norm has read last.  The 463 M fp32 gradients of the 0.55b model: squares
+// 0.34 ms (5.4 TB/s), scaling 0.79 ms (4.7 TB/s).  Eight loads ahead instead of four took 7% off the squares; chunks of
+// 65536, 1024 to 4096 workgroups and one workgroup a chunk were no quicker (the last 50% slower, as each adds up the parts).
 #include <algorithm>
 #include <vector>
 
@@ -20,7 +23,8 @@ namespace {
 
 constexpr int kGroup = 128;        // tensors of a launch: their table travels in the kernel's arguments
 constexpr int kChunk = 16384;      // elements of a chunk; a workgroup takes chunk after chunk
-constexpr int kWgs = 2048;         // 8 workgroups of 256 on each of 256 CUs
+constexpr int kWgs = 2048;       // 8 workgroups of 256 on each of 256 CUs
+constexpr int kAhead = 8;          // 16-byte loads a thread has in flight
 constexpr double kEps = 1e-6;
 
 struct Table {
@@ -42,7 +46,7 @@ template <typename T> struct Piece;
 template <> struct Piece<float> {
   static constexpr int N = 4;
   static __device__ __forceinline__ u32x4 load(const float* p) { return *reinterpret_cast<const u32x4_f*>(p); }
-  static __device__ __forceinline__ void store(float* p, u32x4 v) { *reinterpret_cast<u32x4_f*>(p) = v; }
+  static __device__ __forceinline__ void store(float* p, u32x4 v) { __builtin_nontemporal_store(v, reinterpret_cast<u32x4_f*>(p)); }
   static __device__ __forceinline__ double square(u32x4 v, double s) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -60,7 +64,7 @@ template <> struct Piece<float> {
 template <> struct Piece<uint16_t> {
   static constexpr int N = 8;
   static __device__ __forceinline__ u32x4 load(const uint16_t* p) { return *reinterpret_cast<const u32x4_h*>(p); }
-  static __device__ __forceinline__ void store(uint16_t* p, u32x4 v) { *reinterpret_cast<u32x4_h*>(p) = v; }
+  static __device__ __forceinline__ void store(uint16_t* p, u32x4 v) { __builtin_nontemporal_store(v, reinterpret_cast<u32x4_h*>(p)); }
   static __device__ __forceinline__ double square(u32x4 v, double s) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -108,12 +112,12 @@ __device__ __forceinline__ double chunk_square(const T* g, int64_t n, double s) 
   constexpr int N = Piece<T>::N, STEP = 256 * N;
   const int full = (int)(n / N) * N;
   int i = threadIdx.x * N;
-  for (; i + 3 * STEP < full; i += 4 * STEP) {
-    u32x4 v[4];
+  for (; i + (kAhead - 1) * STEP < full; i += kAhead * STEP) {
+    u32x4 v[kAhead];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = Piece<T>::load(g + i + k * STEP);
+    for (int k = 0; k < kAhead; ++k) v[k] = Piece<T>::load(g + i + k * STEP);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s = Piece<T>::square(v[k], s);
+    for (int k = 0; k < kAhead; ++k) s = Piece<T>::square(v[k], s);
   }
   for (; i < full; i += STEP) s = Piece<T>::square(Piece<T>::load(g + i), s);
   if (full + (int)threadIdx.x < n) {
@@ -151,12 +155,12 @@ __device__ __forceinline__ void chunk_scale(const T* g, T* out, int64_t n, doubl
   constexpr int N = Piece<T>::N, STEP = 256 * N;
   const int full = (int)(n / N) * N;
   int i = threadIdx.x * N;
-  for (; i + 3 * STEP < full; i += 4 * STEP) {
-    u32x4 v[4];
+  for (; i + (kAhead - 1) * STEP < full; i += kAhead * STEP) {
+    u32x4 v[kAhead];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = Piece<T>::load(g + i + k * STEP);
+    for (int k = 0; k < kAhead; ++k) v[k] = Piece<T>::load(g + i + k * STEP);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) Piece<T>::store(out + i + k * STEP, Piece<T>::times(v[k], c));
+    for (int k = 0; k < kAhead; ++k) Piece<T>::store(out + i + k * STEP, Piece<T>::times(v[k], c));
   }
   for (; i < full; i += STEP) Piece<T>::store(out + i, Piece<T>::times(Piece<T>::load(g + i), c));
   if (full + (int)threadIdx.x < n) out[full + threadIdx.x] = from_f<T>((float)((double)to_f<T>(g[full + threadIdx.x]) * c));

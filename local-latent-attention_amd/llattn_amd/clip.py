@@ -29,22 +29,24 @@ def _flat(t: torch.Tensor):
     return t if t.is_contiguous() else None
 
 
-def _lists(who: str, tensors):
-    """Checks that every call needs: the tensors' device."""
+def _check(who: str, tensors) -> torch.device:
+    """The device of ``tensors`` (one at least), which are what the kernels take."""
+    devices = {t.get_device() for t in tensors}
     for t in tensors:
         if t.dtype not in _CODE:
             raise ValueError(f"{who}: gradients must be fp32 or bf16, got {t.dtype}")
         if t.layout is not torch.strided:
             raise ValueError(f"{who}: gradients must be dense tensors, got {t.layout}")
-    L.require_gpu(*tensors)
-    devices = {t.get_device() for t in tensors}
+    L.refuse_tangents(who, tensors)
+    if min(devices) < 0:
+        L.require_gpu(*tensors)
     if len(devices) > 1:
         raise ValueError(f"{who}: gradients on {len(devices)} devices")
     return tensors[0].device
 
 
 class _Arrays:
-    """The host arrays of a call."""
+    """The host arrays of a call on contiguous tensors."""
 
     def __init__(self, tensors):
         self.n = len(tensors)
@@ -59,7 +61,8 @@ class _Arrays:
         return torch.empty((n,), dtype=torch.uint8, device=device), n
 
     def bytes(self) -> int:
-        return sum(n * (2 if d else 4) for n, d in zip(self.numel, self.dtype))
+        from .ops import EVENT_LOG
+        return 0 if EVENT_LOG is None else sum(n * (2 if d else 4) for n, d in zip(self.numel, self.dtype))
 
 
 def _at(a):
@@ -72,6 +75,11 @@ def _most(who: str, max_norm) -> float:
     return float(max_norm)
 
 
+def _whole(t: torch.Tensor) -> torch.Tensor:
+    f = _flat(t.detach())
+    return t.detach().contiguous() if f is None else f
+
+
 @torch.no_grad()
 def grad_norm(tensors) -> torch.Tensor:
     """The 2-norm of all elements of ``tensors`` (fp32 or bf16, any shapes and strides, one device) as an fp32 scalar on
@@ -79,12 +87,10 @@ def grad_norm(tensors) -> torch.Tensor:
     tensors = list(tensors)
     if not tensors:
         return torch.zeros(())
-    L.refuse_tangents("grad_norm", tensors)
-    tensors = [t.detach() for t in tensors]
-    device = _lists("grad_norm", tensors)
-    flat = [_flat(t) for t in tensors]
-    flat = [t.contiguous() if f is None else f for t, f in zip(tensors, flat)]
-    a = _Arrays(flat)
+    device = _check("grad_norm", tensors)
+    if not all([t.is_contiguous() for t in tensors]):
+        tensors = [_whole(t) for t in tensors]
+    a = _Arrays(tensors)
     ws, n = a.workspace(device)
     norm = torch.empty((), dtype=torch.float32, device=device)
     from .ops import _call
@@ -94,34 +100,43 @@ def grad_norm(tensors) -> torch.Tensor:
     return norm
 
 
-def _clip(who: str, tensors, out, max_norm: float, norm_in) -> torch.Tensor | None:
-    """Scales ``tensors`` into ``out`` (or in place); the norm where none is given."""
-    device = _lists(who, tensors)
-    if norm_in is not None and (norm_in.numel() != 1 or norm_in.dtype is not torch.float32 or norm_in.device != device):
-        raise ValueError(f"{who}: the norm must be one fp32 value on {device}, got {tuple(norm_in.shape)} {norm_in.dtype} on {norm_in.device}")
+def _pairs(who: str, tensors, out):
+    """Contiguous (sources, destinations) for gradients that are not all so; and (tensor, destination) pairs to be copied back."""
     src, dst, back = [], [], []
     for i, g in enumerate(tensors):
-        o = g if out is None else out[i]
-        f = _flat(g)
-        if o is not g:
-            if o.shape != g.shape or o.dtype is not g.dtype or o.get_device() != g.get_device():
-                raise ValueError(f"{who}: outputs must have their gradient's shape {tuple(g.shape)}, type and device")
-            # both in one order of the axes: that of memory
-            if not (f is not None and o.stride() == g.stride()):
-                f = g.contiguous()
-        if o.is_contiguous() or (f is not None and o.stride() == g.stride()):
-            d = o if o.is_contiguous() else _flat(o)
-        else:  # not in one stretch: scaled in a copy
-            if torch._debug_has_internal_overlap(o) == 1:
-                raise ValueError(f"{who}: a tensor that is written holds one element in several places (strides {o.stride()})")
-            d = f = g.contiguous() if o is not g else g.clone(memory_format=torch.contiguous_format)
-            if o is not g:
+        g = g.detach()
+        o = g if out is None else out[i].detach()
+        same = o.stride() == g.stride()
+        f = _flat(g) if same else None  # both in one order of the axes: that of memory
+        d = _flat(o) if same else o if o.is_contiguous() else None
+        if f is None or d is None:
+            f = g.contiguous()
+            if not o.is_contiguous():  # not in one stretch: scaled apart
+                if torch._debug_has_internal_overlap(o) == 1:
+                    raise ValueError(f"{who}: a tensor that is written holds one element in several places (strides {o.stride()})")
                 d = torch.empty_like(f)
-            back.append((o, d))
+                back.append((o, d))
+            else:
+                d = o
         src.append(f)
         dst.append(d)
+    return src, dst, back
+
+
+def _clip(who: str, tensors, out, max_norm: float, norm_in) -> torch.Tensor | None:
+    """Scales ``tensors`` (one at least) into ``out`` (or in place); the norm where none is given."""
+    device = _check(who, tensors)
+    if norm_in is not None and (norm_in.numel() != 1 or norm_in.dtype is not torch.float32 or norm_in.device != device):
+        raise ValueError(f"{who}: the norm must be one fp32 value on {device}, got {tuple(norm_in.shape)} {norm_in.dtype} on {norm_in.device}")
+    written = tensors if out is None else out
+    if out is not None and ([t.shape for t in out] != [t.shape for t in tensors] or [t.dtype for t in out] != [t.dtype for t in tensors]
+                            or {t.get_device() for t in out} != {device.index}):
+        raise ValueError(f"{who}: outputs must have their gradients' shapes, types and device")
+    src, dst, back = tensors, out, ()
+    if not all([t.is_contiguous() for t in tensors]) or out is not None and not all([t.is_contiguous() for t in out]):
+        src, dst, back = _pairs(who, tensors, out)
     a = _Arrays(src)
-    o = array("Q", [t.data_ptr() for t in dst])
+    o = None if dst is None else array("Q", [t.data_ptr() for t in dst])
     ws = norm = None
     n = 0
     if norm_in is None:
@@ -129,12 +144,12 @@ def _clip(who: str, tensors, out, max_norm: float, norm_in) -> torch.Tensor | No
         norm = torch.empty((), dtype=torch.float32, device=device)
     from .ops import _call
     with L.on_device(device):
-        _call("llattn_clip_grads", a.n, _at(a.g), _at(o), _at(a.numel), _at(a.dtype), max_norm,
+        _call("llattn_clip_grads", a.n, _at(a.g), None if o is None else _at(o), _at(a.numel), _at(a.dtype), max_norm,
               None if norm_in is None else norm_in.data_ptr(), None if norm is None else norm.data_ptr(),
               None if ws is None else ws.data_ptr(), n, L.stream_ptr(device), work=(3 if norm_in is None else 2) * a.bytes())
     for to, d in back:
         to.copy_(d)
-    torch.autograd.graph.increment_version(list(tensors) if out is None else out)
+    torch.autograd.graph.increment_version(written)
     return norm
 
 
@@ -144,8 +159,6 @@ def clip_grad_norm(grads, max_norm: float, out=None) -> torch.Tensor:
     :func:`grad_norm`, which is returned.  In place, or into ``out`` (a list of as many tensors of the same shapes and types;
     each may be its gradient itself and overlaps nothing else).  Nothing waits for the GPU.  GPU only."""
     grads, most = list(grads), _most("clip_grad_norm", max_norm)
-    L.refuse_tangents("clip_grad_norm", grads)
-    grads = [g.detach() for g in grads]
     if out is not None:
         out = list(out)
         if len(out) != len(grads):
@@ -157,7 +170,7 @@ def clip_grad_norm(grads, max_norm: float, out=None) -> torch.Tensor:
 
 def _grads(parameters):
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    return [p.grad.detach() for p in parameters if p.grad is not None]
+    return [g for p in parameters if (g := p.grad) is not None]
 
 
 @torch.no_grad()
