@@ -70,20 +70,19 @@ int32_t llattn_clip_grads(int32_t n, const void* const* g, void* const* out, con
  *   a = x W1^T + b1,  u = x W3^T + b3,  h = act(a) u,  y = h W2^T + b2
  * with x [rows][D], W1 and W3 [F][D], W2 [D_out][F], y [rows][D_out], all bf16,
  * biases fp32 or NULL; products summed in fp32, a and u not rounded, h rounded
- * to bf16 (what the last product reads).  act: LLATTN_GATE_SILU a / (1 +
- * exp(-a)) or LLATTN_GATE_GELU a Phi(a).  D, F and D_out are multiples of 8,
- * weights, y, h, p and s contiguous, x of row stride ldx (a multiple of 8, below
- * 2^23); everything 16-byte aligned.
+ * to bf16 (what the last product reads; forward alone over at most 64 rows it
+ * stays in fp32).  act: LLATTN_GATE_SILU a / (1 + exp(-a)) or LLATTN_GATE_GELU
+ * a Phi(a).  D, F and D_out are multiples of 8, weights and y contiguous, x of
+ * row stride ldx (a multiple of 8, below 2^23); everything 16-byte aligned.
  *
- * Forward: y; h (NULL: in the workspace) and, for a backward, p = act(a) and s =
- * act'(a) u (both or neither; [rows][F] of three bytes each, the upper 24 bits of
- * fp32 in a layout of the library's own).  Backward of it, given dy [rows][D_out]
- * contiguous:
- *   dh = dy W2,  da = dh s,  du = dh p  (da and du bf16),
+ * Forward: y; with `kept` not NULL (llattn_gated_bytes(cfg, LLATTN_GATED_KEPT)
+ * bytes of the caller's) also what the backward reads.  Backward of it, given dy
+ * [rows][D_out] contiguous, with p = act(a) and s = act'(a) u:
+ *   dh = dy W2,  da = dh s,  du = dh p  (da and du rounded to bf16),
  *   dx = da W1 + du W3,  dW1 = da^T x,  dW3 = du^T x,  dW2 = dy^T h,
  *   db1, db3, db2: sums of da, du, dy over the rows (fp32)
- * (any of them NULL), dx bf16, dW1 and dW3 of dw_dtype, dW2 of dw2_dtype.  Sums
- * run in a fixed order (no atomics). */
+ * (any of them NULL; dW1 and dW3 together), dx bf16, dW1 and dW3 of dw_dtype, dW2
+ * of dw2_dtype.  Sums run in a fixed order (no atomics). */
 #define LLATTN_GATE_SILU 0
 #define LLATTN_GATE_GELU 1
 
@@ -103,14 +102,18 @@ typedef struct llattn_gated_grads {
   float *db1, *db3, *db2;
 } llattn_gated_grads;
 
-/* Workspace bytes of llattn_gated_fwd (which = 0) and llattn_gated_bwd (which = 1); 0 with an error message on a bad
- * configuration. */
+/* Bytes of a buffer; 0 with an error message on a bad configuration: workspace of a forward with `kept`, of one without, of the
+ * backward; what is kept between them. */
+#define LLATTN_GATED_FORWARD 0
+#define LLATTN_GATED_ALONE 1
+#define LLATTN_GATED_BACKWARD 2
+#define LLATTN_GATED_KEPT 3
 size_t llattn_gated_bytes(const llattn_gated_cfg* cfg, int32_t which);
-int32_t llattn_gated_fwd(const llattn_gated_cfg* cfg, const void* x, int64_t ldx, const llattn_gated_weights* w, void* h,
-                         void* p, void* s, void* y, void* workspace, size_t workspace_bytes, void* stream);
+int32_t llattn_gated_fwd(const llattn_gated_cfg* cfg, const void* x, int64_t ldx, const llattn_gated_weights* w, void* kept,
+                         void* y, void* workspace, size_t workspace_bytes, void* stream);
 int32_t llattn_gated_bwd(const llattn_gated_cfg* cfg, const void* x, int64_t ldx, const llattn_gated_weights* w,
-                         const void* h, const void* p, const void* s, const void* dy, const llattn_gated_grads* grads,
-                         void* workspace, size_t workspace_bytes, void* stream);
+                         const void* kept, const void* dy, const llattn_gated_grads* grads, void* workspace,
+                         size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -13,6 +13,10 @@
 // leaves them.  p and s are kept in 24 bits (16 of the significand: their rounding in bf16 would make that sqrt 3, at 8192 x 1536
 // x 4096 for 2% of the time), the upper two bytes and the third in planes of their own.
 //
+// Backward, two products share a launch where both take 128 x 128 tiles (the gate's gradients with dW2, dx with dW1 and dW3): small
+// ones fill the chip together.  Forward alone with few rows, two kernels of their own read every weight once, along k, and
+// h stays in fp32 between them.
+//
 // What bounds it: the matrix cores (2 rows D F operations for each of the three products, twice that backward); with few
 // rows the reads of the weights.
 #include <algorithm>
@@ -25,8 +29,8 @@ namespace {
 
 using namespace tiles;
 
-// OUT: C (bf16 or fp32); SUM: fp32 parts of it
-enum Epilogue { GATE = 0, DGATE = 1, OUT_BF16 = 2, OUT_F32 = 3, SUM = 4 };
+// OUT: C, or fp32 parts of it
+enum Epilogue { GATE = 0, DGATE = 1, OUT = 2 };
 
 struct GatedArgs {
   int M, N, K;                  // GATE: N columns of h
@@ -42,7 +46,8 @@ struct GatedArgs {
   uint16_t* d; int64_t ldd;     // DGATE: [M][ldd], da in its columns, du from column ldd / 2 on
   void *C, *C2; int64_t ldc;    // rows [0, m_live) of each of the two halves of m_half rows (one half: m_half = M)
   int m_half, m_live;
-  float* part;                  // SUM: [splits][M][N]
+  int f32;                      // C is fp32 (else bf16)
+  float* part;                  // OUT in splits: [splits][M][N]
 };
 
 // act(a) and act'(a).  SiLU: a g and g (1 + a (1 - g)), g = 1 / (1 + exp(-a)).  GELU: a Phi and Phi + a phi with
@@ -117,24 +122,82 @@ struct GateOp : RowOp<T, W, true> {
   }
 };
 
+// Column blocks of a tile that is not a power of two wide: V columns in rows of T (2 T bytes in LDS, as ColOp<T, W> lays them out;
+// chunks past V are not loaded), NB blocks from o0 on, a multiple of 16.
+template <int T, int V, int W, int NB>
+struct ColsOp {
+  static constexpr int BYTES = T * 128, LOADS = BYTES / 1024 / W, PER = T / 8;
+  uint32_t off[LOADS], base[NB];
+  static __device__ __forceinline__ int swz(int k) { return ColOp<T, W>::swz(k); }
+  __device__ __forceinline__ void init(int64_t ld, int w, int lane, int o0) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int q = (w * LOADS + i) * 64 + lane, k = q / PER, c = (q % PER) ^ swz(k);
+      off[i] = 8 * c < V ? step_off((int64_t)k * ld * 2 + 16 * c) : kOffPastK;
+    }
+    const int r = lane & 15, g = lane >> 4, k = 8 * g + (r >> 2);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int byte = 2 * (o0 + 16 * j) + 8 * (r & 3);
+      base[j] = k * (2 * T) + (((byte >> 4) ^ swz(k)) << 4) + (byte & 15);
+    }
+  }
+  __device__ __forceinline__ uint32_t at(int i, int) const { return off[i]; }
+  __device__ __forceinline__ bf16x8 frag(const unsigned char* st, int j, int half) const {
+    bf16x4 hv[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const unsigned char* p = st + base[j] + (32 * half + 4 * q) * (2 * T);
+      hv[q] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(p));
+    }
+    return bf16x8{hv[0][0], hv[0][1], hv[0][2], hv[0][3], hv[1][0], hv[1][1], hv[1][2], hv[1][3]};
+  }
+};
+
+// T columns along k: the operand that holds them
+template <int T, int W, int NB> struct Cols { typedef ColOp<T, W> Op; };
+template <int W, int NB> struct Cols<192, W, NB> { typedef ColsOp<256, 192, W, NB> Op; };
+
 // Tiles of a product, as those of the head loss: a 64-k step is two rounds of products, each beside the fragment reads of the
 // next: k 0..31 (reads k 32..63), a barrier, k 32..63 (reads the next step's k 0..31 and issues the loads of step
 // kt + NST into the stage just read).  Waves whose part of the tile lies outside load and wait like the others and do
-// nothing else.  PERSIST: a workgroup takes tile after tile, the next one's first steps loaded in the last ones of this.
+// nothing else.  The gate's workgroups take tile after tile, the next one's first steps loaded in the last ones of this.
 // AT: A stored with its rows along k.  BT: B likewise.  TWO: a second matrix B from step `half` on.
-template <int EPI, bool AT, bool BT, bool TWO, bool PERSIST, typename S, int WGS>
-__global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void gated_kernel(const GatedArgs a) {
-  constexpr int MB = S::MB, NB = S::NB, TM = S::TM, TN = S::TN, NST = S::NST, STAGE = S::STAGE, W = S::W;
+// What a product is made of: EPI, AT, BT and TWO as above
+template <int EPI_, bool AT_, bool BT_, bool TWO_>
+struct Product {
+  static constexpr int EPI = EPI_;
+  static constexpr bool AT = AT_, BT = BT_, TWO = TWO_;
+};
+typedef Product<GATE, false, false, false> GateProduct;
+typedef Product<OUT, false, false, false> OutProduct;   // y
+typedef Product<DGATE, false, true, false> DGateProduct;
+typedef Product<OUT, false, true, true> DxProduct;
+typedef Product<OUT, true, true, false> DwProduct;
+
+template <typename P, typename S>
+struct Operands {
+  static constexpr int W = S::W;
+  typedef std::conditional_t<P::AT, typename Cols<S::TM, W, S::MB>::Op, RowOp<S::TM, W, false>> A;
+  typedef std::conditional_t<P::EPI == GATE, GateOp<S::TN, W, S::NB>, std::conditional_t<P::BT, typename Cols<S::TN, W, S::NB>::Op, RowOp<S::TN, W, true>>> B;
+  static constexpr int STAGE = A::BYTES + B::BYTES, LDS = S::NST * STAGE;
+};
+
+// The tiles v, v + stride, ... of a product (one tile where it does not persist)
+template <typename P, typename S>
+__device__ __forceinline__ void gated_tiles(const GatedArgs& a, unsigned char* smem, int v, int stride) {
+  constexpr int EPI = P::EPI;
+  constexpr bool AT = P::AT, BT = P::BT, TWO = P::TWO, PERSIST = EPI == GATE;
+  constexpr int MB = S::MB, NB = S::NB, TM = S::TM, TN = S::TN, NST = S::NST, W = S::W;
   constexpr int TC = EPI == GATE ? TN / 2 : TN;      // columns of the result in a tile,
   constexpr int WCOLS = EPI == GATE ? 8 * NB : 16 * NB;  // and of a wave
-  typedef std::conditional_t<AT, ColOp<TM, W>, RowOp<TM, W, false>> OpA;
-  typedef std::conditional_t<EPI == GATE, GateOp<TN, W, NB>, std::conditional_t<BT, ColOp<TN, W>, RowOp<TN, W, true>>> OpB;
-  constexpr int LOADS = OpA::LOADS + OpB::LOADS;
+  typedef typename Operands<P, S>::A OpA;
+  typedef typename Operands<P, S>::B OpB;
+  constexpr int LOADS = OpA::LOADS + OpB::LOADS, STAGE = OpA::BYTES + OpB::BYTES;
   static_assert(LOADS <= MB + NB, "the second round's reads carry the loads");
-  static_assert((!AT || (16 * MB) % 64 == 0) && (!BT || (16 * NB) % 64 == 0), "ColOp::base");
+  static_assert((!AT || TM == 192 || (16 * MB) % 64 == 0) && (!BT || TN == 192 || (16 * NB) % 64 == 0), "ColOp::base");
   static_assert(S::WC == 2 && (S::WR == 2 || S::WR == 4), "wave layouts");
   static_assert(EPI != GATE || (TN / 2) % (8 * OpB::LOADS) == 0, "a wave loads rows of one of the two matrices");
-  __shared__ __align__(1024) unsigned char smem[NST * STAGE];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // eight waves: those of one SIMD (w, w + 4) lie in opposite halves of both sides
@@ -171,7 +234,6 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void gated_kernel(const
     return source(EPI == GATE && 2 * w >= W ? a.B2 : a.B, a.ldb, BT, t.n0, n, k, a.K);
   };
   auto k_of = [&](const Tile& t) { return min(a.K - t.split * a.per * 64, t.steps * 64); };
-  int v = blockIdx.x;
   Tile tile = tile_at(v);
   StepSrc sa = source_a(tile), sb = source_b(tile, tile.split * a.per);
   int ahead = k_of(tile);  // k from the step that ra and rb describe to the end of its tile's
@@ -201,12 +263,12 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void gated_kernel(const
   f32x4 acc[MB][NB];
   // MB NB products, B first: lane (r, g) accumulates C[r][4 g + e]; io(q), q < MB + NB, spread over them
   auto round = [&](const bf16x8 (&x)[MB], const bf16x8 (&y)[NB], auto io) {
-    constexpr int N = MB + NB, P = MB * NB;
+    constexpr int N = MB + NB, ALL = MB * NB;
     unroll<N>([&](auto qt) {
       constexpr int q = decltype(qt)::value;
       io(qt);
 #pragma unroll
-      for (int n = q * P / N; n < (q + 1) * P / N; ++n)
+      for (int n = q * ALL / N; n < (q + 1) * ALL / N; ++n)
         acc[n / NB][n % NB] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[n % NB], x[n / NB], acc[n / NB][n % NB], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -228,8 +290,8 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void gated_kernel(const
   if (own) first_frags();
   for (;;) {
     // A tile before another takes whole turns of the stages.
-    const bool more = PERSIST && v + (int)gridDim.x < a.total;
-    const Tile next = more ? tile_at(v + gridDim.x) : tile;
+    const bool more = PERSIST && v + stride < a.total;
+    const Tile next = more ? tile_at(v + stride) : tile;
     const StepSrc next_a = source_a(next), next_b = source_b(next, next.split * a.per);
     const int next_k = more ? k_of(next) : 0;
     const int steps = more ? (max(tile.steps, 1) + NST - 1) / NST * NST : tile.steps;
@@ -346,35 +408,42 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void gated_kernel(const
         }
       }
     } else if constexpr (EPI == DGATE) {
-#pragma unroll
-      for (int i = 0; i < MB; ++i) {
+      // p and s of a row of blocks are read a row ahead: left to the compiler, each pair of blocks waited for its own
+      const int64_t plane = 2 * (int64_t)a.M * a.N;
+      Float24 p[2][NB / 2], s[2][NB / 2];
+      const auto fetch = [&](auto it) {
+        constexpr int i = decltype(it)::value;
         const int row = row0 + 16 * i + r;
 #pragma unroll
         for (int j = 0; j < NB; j += 2) {
-          f32x4 x = acc[i][j], y = acc[i][j + 1];
+          const int c = pair(j);
+          const int64_t at = (int64_t)row * a.N + c;
+          p[i & 1][j / 2] = s[i & 1][j / 2] = Float24{make_uint4(0, 0, 0, 0), make_uint2(0, 0)};
+          if (row < a.M && c < a.N) {
+            p[i & 1][j / 2].load(a.p, plane, at);
+            s[i & 1][j / 2].load(a.s, plane, at);
+          }
+        }
+      };
+      fetch(std::integral_constant<int, 0>{});
+      unroll<MB>([&](auto it) {
+        constexpr int i = decltype(it)::value;
+        if constexpr (i + 1 < MB) fetch(std::integral_constant<int, i + 1>{});
+        const int row = row0 + 16 * i + r;
+#pragma unroll
+        for (int j = 0; j < NB; j += 2) {
+          f32x4 x = acc[i][j], y = acc[i][j + 1], m, n;
           swap(x, y);
           const int c = pair(j);
-          if (row >= a.M || 2 * c >= a.ldd) continue;
+          if (row >= a.M || 2 * c >= a.ldd) continue;  // columns from the last on: zeros, which the products contract over
           uint16_t* o = a.d + (int64_t)row * a.ldd + c;
-          uint4 da = make_uint4(0, 0, 0, 0), du = da;  // past the last column: zeros, which the products contract over
-          if (c < a.N) {
-            const int64_t plane = 2 * (int64_t)a.M * a.N, at = (int64_t)row * a.N + c;
-            Float24 p, s;
-            p.load(a.p, plane, at);
-            s.load(a.s, plane, at);
-            const auto times = [&](const Float24& q) {
-              f32x4 m, n;
-              q.get(m, n);
-              return bf16s(x * m, y * n);
-            };
-            da = times(s);
-            du = times(p);
-          }
-          st16(o, da);
-          st16(o + a.ldd / 2, du);
+          s[i & 1][j / 2].get(m, n);
+          st16(o, bf16s(x * m, y * n));
+          p[i & 1][j / 2].get(m, n);
+          st16(o + a.ldd / 2, bf16s(x * m, y * n));
         }
-      }
-    } else if constexpr (EPI == SUM) {
+      });
+    } else if (a.part) {
       float* const c = a.part + (int64_t)tile.split * a.M * a.N;
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
@@ -392,7 +461,7 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void gated_kernel(const
 #pragma unroll
         for (int j = 0; j < NB; j += 2) {
           f32x4 x = acc[i][j], y = acc[i][j + 1];
-          if constexpr (EPI == OUT_F32) {
+          if (AT && a.f32) {
             float* c = static_cast<float*>(C) + (int64_t)f * a.ldc;
             if (live && column(j) < a.N) *reinterpret_cast<f32x4*>(c + column(j)) = x;
             if (live && column(j + 1) < a.N) *reinterpret_cast<f32x4*>(c + column(j + 1)) = y;
@@ -400,80 +469,252 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void gated_kernel(const
             swap(x, y);
             const int c = pair(j);
             if (!live || c >= a.N) continue;
-            if (a.bias) add_bias(x, y, a.bias, c);
+            if (!BT && a.bias) add_bias(x, y, a.bias, c);
             st16(static_cast<uint16_t*>(C) + (int64_t)f * a.ldc + c, bf16s(x, y));
           }
         }
       }
     }
     if (!more) break;
-    v += gridDim.x;
+    v += stride;
     tile = next;
     own = next_own;
   }
-  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no DMA may land after the workgroup exits
+  // No DMA may land after the workgroup exits.  (Waiting for the loads before the epilogue, so that the next workgroup begins beside
+  // its stores, took longer: the gate's gradients of 8192 x 4096 161 -> 177 us.)
+  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
 }
 
-// C = the sum over splits of the parts [splits][M][N], in order, plus the bias; rows as GatedArgs has them
-template <typename T>
-__global__ __launch_bounds__(256) void gated_reduce_kernel(const GatedArgs a, int splits) {
-  const int64_t n = (int64_t)a.M * a.N;
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
-    const int row = (int)(i / a.N), col = (int)(i - (int64_t)row * a.N), f = row < a.m_half ? row : row - a.m_half;
-    if (f >= a.m_live) continue;
-    float x[4];
-    load4<float>(a.part + i, x);
-    for (int s = 1; s < splits; ++s) {
-      float y[4];
-      load4<float>(a.part + s * n + i, y);
+template <typename P, typename S, int WGS>
+__global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void gated_kernel(const GatedArgs a) {
+  __shared__ __align__(1024) unsigned char smem[Operands<P, S>::LDS];
+  gated_tiles<P, S>(a, smem, blockIdx.x, gridDim.x);
+}
+// Two products in one launch: the workgroups of the first, a multiple of 8 (so that the second's are dealt to the XCDs as alone), then
+// the other's
+template <typename P0, typename P1>
+__global__ __launch_bounds__(SquareShape::THREADS, SquareShape::W / 2) void gated_pair_kernel(const GatedArgs a, const GatedArgs b, int first) {
+  __shared__ __align__(1024) unsigned char smem[std::max(Operands<P0, SquareShape>::LDS, Operands<P1, SquareShape>::LDS)];
+  const int v = blockIdx.x;
+  if (v >= first) gated_tiles<P1, SquareShape>(b, smem, v - first, 0);
+  else if (v < a.total) gated_tiles<P0, SquareShape>(a, smem, v, 0);
+}
+
+// C = the sum over splits of the parts [splits][M][N], in order, plus the bias; rows as GatedArgs has them.  Up to three products
+// in a launch.
+struct ReduceArgs {
+  GatedArgs a[3];
+  int splits[3], first[4];  // first workgroup of each
+};
+__global__ __launch_bounds__(256) void gated_reduce_kernel(const ReduceArgs q) {
+  const int k = ((int)blockIdx.x >= q.first[1]) + ((int)blockIdx.x >= q.first[2]);
+  const GatedArgs& a = q.a[k];
+  const int64_t n = (int64_t)a.M * a.N, i = ((int64_t)(blockIdx.x - q.first[k]) * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const int row = (int)(i / a.N), col = (int)(i - (int64_t)row * a.N), f = row < a.m_half ? row : row - a.m_half;
+  if (f >= a.m_live) return;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  constexpr int U = 8;
+  for (int s = 0; s < q.splits[k]; s += U) {
+    float y[U][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] += y[e];
-    }
-    if (a.bias) {
+    for (int u = 0; u < U; ++u)
+      if (s + u < q.splits[k]) load4<float>(a.part + (s + u) * n + i, y[u]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] += a.bias[col + e];
+    for (int u = 0; u < U; ++u)
+      if (s + u < q.splits[k]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += y[u][e];
+      }
+  }
+  if (a.bias) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += a.bias[col + e];
+  }
+  void* const C = row < a.m_half ? a.C : a.C2;
+  if (a.f32) store4<float>(static_cast<float*>(C) + (int64_t)f * a.ldc + col, x);
+  else store4<uint16_t>(static_cast<uint16_t*>(C) + (int64_t)f * a.ldc + col, x);
+}
+
+// ---- few rows, forward alone ------------------------------------------------------------
+//
+// A workgroup takes 16 rows of the weights (of both, GATE) and all of x, its W waves the 32-k steps w, w + W, ... : every weight
+// is read once, straight into the operand of the matrix cores (lane (r, g): k 8 g .. of row r), W x 64 bytes of a row at a
+// time.  The waves' sums are added in LDS.  The last projection reads h in fp32 as two bf16 operands (16 bits of its significand):
+// y then carries its own rounding alone.  What bounds it: latency, and the reads of the weights.
+struct ThinArgs {
+  int M, N, K;                     // rows (up to 16 NT); rows of the weights, their length
+  const uint16_t* x; int64_t ldx;  // GATE
+  float* h;                        // [M][N] (GATE), [M][K]
+  const uint16_t *W, *W3;
+  const float *bias, *bias3;
+  int act;
+  uint16_t* y;
+};
+template <bool GATED, int NT, int W>
+__global__ __launch_bounds__(64 * W) void gated_thin_kernel(const ThinArgs a) {
+  constexpr int MATS = GATED ? 2 : 1, U = NT == 1 ? 4 : 2;
+  __shared__ f32x4 sums[W][MATS][NT][64];
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, w = threadIdx.x >> 6;
+  const int f0 = blockIdx.x * 16, steps = (a.K + 31) / 32;
+  const bool row_ok = f0 + r < a.N;
+  const uint16_t* p[2] = {a.W + (int64_t)(f0 + r) * a.K + 8 * g, GATED ? a.W3 + (int64_t)(f0 + r) * a.K + 8 * g : nullptr};
+  f32x4 acc[MATS][NT];
+#pragma unroll
+  for (int m = 0; m < MATS; ++m)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s0 = w; s0 < steps; s0 += U * W) {
+    bf16x8 v[U][MATS], x[U][NT];
+    f32x4 h[U][NT][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * W, k = 32 * s + 8 * g;
+      const bool ok = s < steps && k < a.K;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int m = 0; m < MATS; ++m) v[u][m] = __builtin_bit_cast(bf16x8, ok && row_ok ? ld16(p[m] + 32 * s) : zero);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int n = 16 * t + r;
+        const bool live = ok && n < a.M;
+        if constexpr (GATED) {
+          x[u][t] = __builtin_bit_cast(bf16x8, live ? ld16(a.x + n * a.ldx + k) : zero);
+        } else {
+          const float* q = a.h + (int64_t)n * a.K + k;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) h[u][t][e] = live ? *reinterpret_cast<const f32x4*>(q + 4 * e) : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+      }
     }
-    store4<T>(static_cast<T*>(row < a.m_half ? a.C : a.C2) + (int64_t)f * a.ldc + col, x);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if constexpr (GATED) {
+#pragma unroll
+          for (int m = 0; m < MATS; ++m) acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u][m], x[u][t], acc[m][t], 0, 0, 0);
+        } else {
+          bf16x8 hi, lo;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float f = h[u][t][e >> 2][e & 3];
+            hi[e] = (__bf16)f;
+            const float rest = f - (float)hi[e];
+            lo[e] = (__bf16)(fabsf(rest) < __builtin_inff() ? rest : 0.f);  // an infinity has no rest
+          }
+          acc[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u][0], hi, acc[0][t], 0, 0, 0);
+          acc[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u][0], lo, acc[0][t], 0, 0, 0);
+        }
+      }
+  }
+#pragma unroll
+  for (int m = 0; m < MATS; ++m)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) sums[w][m][t][lane] = acc[m][t];
+  __syncthreads();
+  if (w >= NT) return;
+  // wave t: rows 16 t + r of x, weights' rows f0 + 4 g + e
+  const int t = w, n = 16 * t + r, f = f0 + 4 * g;
+  f32x4 out[MATS];
+#pragma unroll
+  for (int m = 0; m < MATS; ++m) {
+    out[m] = sums[0][m][t][lane];
+    for (int q = 1; q < W; ++q) out[m] += sums[q][m][t][lane];
+  }
+  if (n >= a.M || f >= a.N) return;
+  if (a.bias) out[0] += *reinterpret_cast<const f32x4*>(a.bias + f);
+  if constexpr (GATED) {
+    if (a.bias3) out[1] += *reinterpret_cast<const f32x4*>(a.bias3 + f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float v, dv;
+      activation(a.act, out[0][e], v, dv);
+      out[0][e] = v * out[1][e];
+    }
+    *reinterpret_cast<f32x4*>(a.h + (int64_t)n * a.N + f) = out[0];
+  } else {
+    *reinterpret_cast<uint2*>(a.y + (int64_t)n * a.N + f) =
+        make_uint2(pack_bf16x2(out[0][0], out[0][1]), pack_bf16x2(out[0][2], out[0][3]));
   }
 }
+template <int NT>
+void launch_thin(const ThinArgs& gate, const ThinArgs& out, hipStream_t st) {
+  hipLaunchKernelGGL((gated_thin_kernel<true, NT, 8>), dim3((gate.N + 15) / 16), dim3(512), 0, st, gate);
+  hipLaunchKernelGGL((gated_thin_kernel<false, NT, 16>), dim3((out.N + 15) / 16), dim3(1024), 0, st, out);
+}
 
+// ---- launches ------------------------------------------------------------------------------
 constexpr size_t up(size_t n) { return (n + 255) & ~size_t(255); }
 
-template <int EPI, bool AT, bool BT, bool TWO, bool PERSIST>
-void launch(GatedArgs& a, const Tiling& t, hipStream_t st) {
+// 256 x 192 beside the shapes of the head's products: 1536 and 1408 columns are 8 tiles of it, and 8192 rows with them 256, one a CU
+// (8192 x 1536 over 4096 k 99 us with 192 tiles of 256 x 256, so 89; over 8192 k 193 and 185, 180 and 173)
+constexpr int WIDE = KINDS;
+typedef Shape<4, 6, 4, 2, 2> WideShape;
+constexpr double kWideStep = 1.38, kWideTile = 9.0;
+constexpr int tile_m(int kind) { return kind == WIDE ? 256 : kTm[kind]; }
+constexpr int tile_n(int kind) { return kind == WIDE ? 192 : kTn[kind]; }
+
+// As tiling(), without thin tiles and with wide ones
+Tiling choose(int64_t M, int64_t N, int steps, int most, bool wide) {
+  Tiling best = tiling(std::max<int64_t>(M, 65), N, steps, most);
+  for (int S = 1; wide && S <= most && (S == 1 || steps / S >= 4); ++S) {
+    const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 192) * S;
+    double t = (double)ceil_div(tiles, 256) * ((double)ceil_div(steps, S) * kWideStep + kWideTile);
+    if (S > 1) t += 6.0 + 8.0 * S * (double)M * (double)N / 4.5e6;
+    if (t < best.us) best = Tiling{WIDE, S, t};
+  }
+  return best;
+}
+
+// Sizes that follow from the tiling; the number of workgroups
+template <typename P>
+int prepare(GatedArgs& a, const Tiling& t) {
   a.steps = (a.K + 63) / 64;
   a.per = (a.steps + t.splits - 1) / t.splits;
-  a.tiles_m = (a.M + kTm[t.kind] - 1) / kTm[t.kind];
-  const int tn = EPI == GATE ? kTn[t.kind] / 2 : kTn[t.kind];
+  a.tiles_m = (a.M + tile_m(t.kind) - 1) / tile_m(t.kind);
+  const int tn = P::EPI == GATE ? tile_n(t.kind) / 2 : tile_n(t.kind);
   a.tiles_n = (a.N + tn - 1) / tn;
   a.total = a.tiles_m * a.tiles_n * t.splits;
-  const dim3 grid((unsigned)(PERSIST ? std::min(a.total, 256 * kPerCu[t.kind]) : a.total));
-  if (t.kind == BIG) hipLaunchKernelGGL((gated_kernel<EPI, AT, BT, TWO, PERSIST, BigShape, 1>), grid, dim3(BigShape::THREADS), 0, st, a);
-  else if (t.kind == SQUARE) hipLaunchKernelGGL((gated_kernel<EPI, AT, BT, TWO, PERSIST, SquareShape, 2>), grid, dim3(SquareShape::THREADS), 0, st, a);
-  else if constexpr (EPI == GATE || EPI == DGATE) hipLaunchKernelGGL((gated_kernel<EPI, AT, BT, TWO, PERSIST, ThinShape, 2>), grid, dim3(ThinShape::THREADS), 0, st, a);
+  return a.total;
 }
-
-// A product into C, whole or in splits
-template <bool AT, bool BT, bool TWO>
-void product(GatedArgs& a, const Tiling& t, int dtype, float* part, hipStream_t st) {
-  if (t.splits > 1) {
-    a.part = part;
-    launch<SUM, AT, BT, TWO, false>(a, t, st);
-    const dim3 grid((unsigned)std::min<int64_t>(ceil_div((int64_t)a.M * a.N, 1024), 8192));
-    if (dtype == LLATTN_F32) hipLaunchKernelGGL(gated_reduce_kernel<float>, grid, dim3(256), 0, st, a, t.splits);
-    else hipLaunchKernelGGL(gated_reduce_kernel<uint16_t>, grid, dim3(256), 0, st, a, t.splits);
-  } else if (dtype == LLATTN_F32) {
-    if constexpr (AT) launch<OUT_F32, AT, BT, TWO, false>(a, t, st);
-  } else {
-    launch<OUT_BF16, AT, BT, TWO, false>(a, t, st);
+template <typename P>
+void launch(GatedArgs& a, const Tiling& t, hipStream_t st) {
+  int n = prepare<P>(a, t);
+  if (P::EPI == GATE) n = std::min(n, 256 * (t.kind == SQUARE ? kPerCu[SQUARE] : 1));
+  const dim3 grid((unsigned)n);
+  if (t.kind == BIG) hipLaunchKernelGGL((gated_kernel<P, BigShape, 1>), grid, dim3(BigShape::THREADS), 0, st, a);
+  else if (t.kind == SQUARE) hipLaunchKernelGGL((gated_kernel<P, SquareShape, 2>), grid, dim3(SquareShape::THREADS), 0, st, a);
+  else if constexpr (P::EPI == OUT) hipLaunchKernelGGL((gated_kernel<P, WideShape, 1>), grid, dim3(WideShape::THREADS), 0, st, a);
+}
+template <typename P0, typename P1>
+void launch_pair(GatedArgs& a, const Tiling& ta, GatedArgs& b, const Tiling& tb, hipStream_t st) {
+  const int first = (prepare<P0>(a, ta) + 7) / 8 * 8, n = first + prepare<P1>(b, tb);
+  hipLaunchKernelGGL((gated_pair_kernel<P0, P1>), dim3((unsigned)n), dim3(SquareShape::THREADS), 0, st, a, b, first);
+}
+// Adds up the parts of those products that have some
+void launch_reduce(const GatedArgs* const* a, const Tiling* const* t, int n, hipStream_t st) {
+  ReduceArgs q{};
+  int k = 0;
+  int64_t blocks = 0;
+  for (int i = 0; i < n; ++i) {
+    if (!a[i]->part) continue;
+    q.a[k] = *a[i];
+    q.splits[k] = t[i]->splits;
+    blocks += ceil_div((int64_t)a[i]->M * a[i]->N, 1024);
+    q.first[++k] = (int)blocks;
   }
+  if (!k) return;
+  for (int i = k; i < 3; ++i) q.first[i + 1] = q.first[i];
+  hipLaunchKernelGGL(gated_reduce_kernel, dim3((unsigned)blocks), dim3(256), 0, st, q);
 }
 
-constexpr int kSplits = 16;
+constexpr int kSplits = 16, kThinRows = 64;
 struct Plan {
   int half;                 // columns of da (and of du): F rounded up to 64
   Tiling gate, out, dgate, dx, dw, dw2;
-  size_t h, d, part[2];     // forward: h, parts; backward: da and du, parts
+  size_t h, d, part[4];     // h; da and du; parts of out, dx, dw, dw2
+  size_t plane;             // p and s, of three bytes
   size_t colsum;
 };
 Plan plan_of(const llattn_gated_cfg* c) {
@@ -481,20 +722,32 @@ Plan plan_of(const llattn_gated_cfg* c) {
   const auto steps = [](int k) { return (k + 63) / 64; };
   const auto part = [](const Tiling& t, int64_t m, int64_t n) { return t.splits > 1 ? up((size_t)t.splits * m * n * 4) : 0; };
   p.half = (c->F + 63) / 64 * 64;
-  p.gate = tiling(c->rows, 2 * (int64_t)c->F, steps(c->D), 1);
-  p.out = tiling(c->rows, c->D_out, steps(c->F), kSplits);
-  p.dgate = tiling(c->rows, c->F, steps(c->D_out), 1);
-  p.dx = tiling(c->rows, c->D, 2 * steps(c->F), kSplits);
-  p.dw = tiling(2 * (int64_t)p.half, c->D, steps(c->rows), kSplits);
-  p.dw2 = tiling(c->D_out, c->F, steps(c->rows), kSplits);
+  p.gate = choose(c->rows, 2 * (int64_t)c->F, steps(c->D), 1, false);
+  p.out = choose(c->rows, c->D_out, steps(c->F), kSplits, true);
+  p.dgate = choose(c->rows, c->F, steps(c->D_out), 1, false);
+  p.dx = choose(c->rows, c->D, 2 * steps(c->F), kSplits, true);
+  p.dw = choose(2 * (int64_t)p.half, c->D, steps(c->rows), kSplits, true);
+  p.dw2 = choose(c->D_out, c->F, steps(c->rows), kSplits, true);
   p.h = up((size_t)c->rows * c->F * 2);
+  p.plane = up((size_t)c->rows * c->F * 3);
   p.d = up((size_t)c->rows * 2 * p.half * 2);
   p.part[0] = part(p.out, c->rows, c->D_out);
-  p.part[1] = std::max({part(p.dx, c->rows, c->D), part(p.dw, 2 * (int64_t)p.half, c->D), part(p.dw2, c->D_out, c->F)});
+  p.part[1] = part(p.dx, c->rows, c->D);
+  p.part[2] = part(p.dw, 2 * (int64_t)p.half, c->D);
+  p.part[3] = part(p.dw2, c->D_out, c->F);
   p.colsum = up(std::max(llattn_colsum_workspace_size(c->rows, c->F), llattn_colsum_workspace_size(c->rows, c->D_out)));
   return p;
 }
-size_t bytes_of(const Plan& p, int which) { return which == 0 ? p.h + p.part[0] : p.d + p.part[1] + p.colsum; }
+// Forward with a backward to follow, forward alone (h in it, in fp32 where rows are few), backward, what is kept between them
+enum Space { FORWARD = LLATTN_GATED_FORWARD, ALONE = LLATTN_GATED_ALONE, BACKWARD = LLATTN_GATED_BACKWARD, KEPT = LLATTN_GATED_KEPT };
+size_t bytes_of(const llattn_gated_cfg* c, const Plan& p, int which) {
+  switch (which) {
+    case FORWARD: return std::max<size_t>(p.part[0], 256);
+    case ALONE: return c->rows <= kThinRows ? up((size_t)c->rows * c->F * 4) : p.h + p.part[0];
+    case BACKWARD: return p.d + p.part[1] + p.part[2] + p.part[3] + p.colsum;
+    default: return p.h + 2 * p.plane;
+  }
+}
 
 int32_t check(const char* who, const llattn_gated_cfg* c) {
   if (!c) return fail(LLATTN_ERR_SHAPE, "%s: null configuration", who);
@@ -518,7 +771,7 @@ int32_t check_operands(const char* who, const llattn_gated_cfg* c, const void* x
   return LLATTN_OK;
 }
 
-const uint16_t* half_floats(const void* p) { return static_cast<const uint16_t*>(p); }
+const uint16_t* bf16(const void* p) { return static_cast<const uint16_t*>(p); }
 
 }  // namespace
 }  // namespace llattn
@@ -527,96 +780,137 @@ using namespace llattn;
 
 extern "C" size_t llattn_gated_bytes(const llattn_gated_cfg* c, int32_t which) {
   if (check("llattn_gated_bytes", c) != LLATTN_OK) return 0;
-  if (which != 0 && which != 1) {
-    fail(LLATTN_ERR_SHAPE, "llattn_gated_bytes: unknown workspace %d", which);
+  if (which < FORWARD || which > KEPT) {
+    fail(LLATTN_ERR_SHAPE, "llattn_gated_bytes: unknown buffer %d", which);
     return 0;
   }
-  return bytes_of(plan_of(c), which);
+  return bytes_of(c, plan_of(c), which);
 }
 
-extern "C" int32_t llattn_gated_fwd(const llattn_gated_cfg* c, const void* x, int64_t ldx, const llattn_gated_weights* w, void* h,
-                                    void* p, void* s, void* y, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int32_t llattn_gated_fwd(const llattn_gated_cfg* c, const void* x, int64_t ldx, const llattn_gated_weights* w, void* kept,
+                                    void* y, void* workspace, size_t workspace_bytes, void* stream) {
   if (const int32_t rc = check("llattn_gated_fwd", c)) return rc;
   const Plan plan = plan_of(c);
-  if (const int32_t rc = check_operands("llattn_gated_fwd", c, x, ldx, w, workspace, workspace_bytes, bytes_of(plan, 0))) return rc;
-  if (!y || !p != !s || (p && !h)) return fail(LLATTN_ERR_LAYOUT, "llattn_gated_fwd: y, and for a backward h, p and s");
-  for (const void* q : {h, p, s, y})
-    if (!aligned16(q)) return fail(LLATTN_ERR_LAYOUT, "llattn_gated_fwd: h, p, s and y must be 16-byte aligned");
+  const size_t need = bytes_of(c, plan, kept ? FORWARD : ALONE);
+  if (const int32_t rc = check_operands("llattn_gated_fwd", c, x, ldx, w, workspace, workspace_bytes, need)) return rc;
+  if (!y || !aligned16(y) || !aligned16(kept)) return fail(LLATTN_ERR_LAYOUT, "llattn_gated_fwd: null y, or y or kept not 16-byte aligned");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
+  if (!kept && c->rows <= kThinRows) {
+    ThinArgs gate{}, out{};
+    gate.M = out.M = c->rows;
+    gate.N = out.K = c->F; gate.K = c->D; out.N = c->D_out;
+    gate.x = bf16(x); gate.ldx = ldx;
+    gate.W = bf16(w->W1); gate.W3 = bf16(w->W3); out.W = bf16(w->W2);
+    gate.bias = w->b1; gate.bias3 = w->b3; out.bias = w->b2;
+    gate.act = c->act;
+    gate.h = out.h = reinterpret_cast<float*>(ws);
+    out.y = static_cast<uint16_t*>(y);
+    if (c->rows <= 16) launch_thin<1>(gate, out, st);
+    else if (c->rows <= 32) launch_thin<2>(gate, out, st);
+    else launch_thin<4>(gate, out, st);
+    return check_launch("llattn_gated_fwd");
+  }
   GatedArgs a{};
   a.M = c->rows; a.N = c->F; a.K = c->D;
-  a.A = half_floats(x); a.lda = ldx;
-  a.B = half_floats(w->W1); a.B2 = half_floats(w->W3); a.ldb = c->D;
+  a.A = bf16(x); a.lda = ldx;
+  a.B = bf16(w->W1); a.B2 = bf16(w->W3); a.ldb = c->D;
   a.bias = w->b1; a.bias2 = w->b3;
   a.act = c->act;
-  a.h = static_cast<uint16_t*>(h ? h : ws); a.p = static_cast<unsigned char*>(p); a.s = static_cast<unsigned char*>(s);
-  launch<GATE, false, false, false, true>(a, plan.gate, st);
+  a.h = reinterpret_cast<uint16_t*>(kept ? static_cast<char*>(kept) : ws);
+  if (kept) {
+    a.p = static_cast<unsigned char*>(kept) + plan.h;
+    a.s = a.p + plan.plane;
+  } else {
+    ws += plan.h;
+  }
+  launch<GateProduct>(a, plan.gate, st);
   GatedArgs o{};
   o.M = c->rows; o.N = c->D_out; o.K = c->F;
   o.A = a.h; o.lda = c->F;
-  o.B = half_floats(w->W2); o.ldb = c->F;
+  o.B = bf16(w->W2); o.ldb = c->F;
   o.bias = w->b2;
   o.C = y; o.ldc = c->D_out; o.m_half = o.m_live = c->rows;
-  product<false, false, false>(o, plan.out, LLATTN_BF16, reinterpret_cast<float*>(ws + plan.h), st);
+  o.part = plan.part[0] ? reinterpret_cast<float*>(ws) : nullptr;
+  launch<OutProduct>(o, plan.out, st);
+  const GatedArgs* args[] = {&o};
+  const Tiling* tilings[] = {&plan.out};
+  launch_reduce(args, tilings, 1, st);
   return check_launch("llattn_gated_fwd");
 }
 
 extern "C" int32_t llattn_gated_bwd(const llattn_gated_cfg* c, const void* x, int64_t ldx, const llattn_gated_weights* w,
-                                    const void* h, const void* p, const void* s, const void* dy, const llattn_gated_grads* g,
-                                    void* workspace, size_t workspace_bytes, void* stream) {
+                                    const void* kept, const void* dy, const llattn_gated_grads* g, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
   if (const int32_t rc = check("llattn_gated_bwd", c)) return rc;
   const Plan plan = plan_of(c);
-  if (const int32_t rc = check_operands("llattn_gated_bwd", c, x, ldx, w, workspace, workspace_bytes, bytes_of(plan, 1))) return rc;
-  if (!h || !p || !s || !dy || !g) return fail(LLATTN_ERR_LAYOUT, "llattn_gated_bwd: null h, p, s, dy or gradients");
-  for (const void* q : {h, p, s, dy, (const void*)g->dx, (const void*)g->dW1, (const void*)g->dW3, (const void*)g->dW2})
-    if (!aligned16(q)) return fail(LLATTN_ERR_LAYOUT, "llattn_gated_bwd: h, p, s, dy and the gradients must be 16-byte aligned");
+  if (const int32_t rc = check_operands("llattn_gated_bwd", c, x, ldx, w, workspace, workspace_bytes, bytes_of(c, plan, BACKWARD))) return rc;
+  if (!kept || !dy || !g) return fail(LLATTN_ERR_LAYOUT, "llattn_gated_bwd: null kept, dy or gradients");
+  for (const void* q : {kept, dy, (const void*)g->dx, (const void*)g->dW1, (const void*)g->dW3, (const void*)g->dW2})
+    if (!aligned16(q)) return fail(LLATTN_ERR_LAYOUT, "llattn_gated_bwd: kept, dy and the gradients must be 16-byte aligned");
   if (!g->dW1 != !g->dW3) return fail(LLATTN_ERR_LAYOUT, "llattn_gated_bwd: dW1 and dW3 come together");
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  char* ws = static_cast<char*>(workspace);
-  uint16_t* const d = reinterpret_cast<uint16_t*>(ws);
-  float* const part = reinterpret_cast<float*>(ws + plan.d);
-  void* const sums = ws + plan.d + plan.part[1];
+  char* at = static_cast<char*>(workspace);
+  const auto take = [&](size_t n) { char* q = at; at += n; return q; };
+  uint16_t* const d = reinterpret_cast<uint16_t*>(take(plan.d));
+  float* part[4] = {};
+  for (int k = 1; k < 4; ++k) {
+    char* q = take(plan.part[k]);
+    if (plan.part[k]) part[k] = reinterpret_cast<float*>(q);
+  }
   const int ldd = 2 * plan.half;
-  if (g->dx || g->dW1 || g->db1 || g->db3) {
-    GatedArgs a{};
-    a.M = c->rows; a.N = c->F; a.K = c->D_out;
-    a.A = half_floats(dy); a.lda = c->D_out;
-    a.B = half_floats(w->W2); a.ldb = c->F;
-    a.p = static_cast<unsigned char*>(const_cast<void*>(p)); a.s = static_cast<unsigned char*>(const_cast<void*>(s));
-    a.d = d; a.ldd = ldd;
-    launch<DGATE, false, true, false, true>(a, plan.dgate, st);
+  unsigned char* const p = static_cast<unsigned char*>(const_cast<void*>(kept)) + plan.h;
+
+  GatedArgs gate{}, dx{}, dw{}, dw2{};
+  const bool on_gate = g->dx || g->dW1 || g->db1 || g->db3, on_dx = g->dx, on_dw = g->dW1, on_dw2 = g->dW2;
+  gate.M = c->rows; gate.N = c->F; gate.K = c->D_out;
+  gate.A = bf16(dy); gate.lda = c->D_out;
+  gate.B = bf16(w->W2); gate.ldb = c->F;
+  gate.p = p; gate.s = p + plan.plane;
+  gate.d = d; gate.ldd = ldd;
+
+  dw2.M = c->D_out; dw2.N = c->F; dw2.K = c->rows;
+  dw2.A = bf16(dy); dw2.lda = c->D_out;
+  dw2.B = bf16(kept); dw2.ldb = c->F;
+  dw2.C = g->dW2; dw2.ldc = c->F; dw2.m_half = dw2.m_live = c->D_out;
+  dw2.f32 = c->dw2_dtype == LLATTN_F32;
+  dw2.part = on_dw2 ? part[3] : nullptr;
+
+  dx.M = c->rows; dx.N = c->D; dx.K = ldd;
+  dx.A = d; dx.lda = ldd;
+  dx.B = bf16(w->W1); dx.B2 = bf16(w->W3); dx.ldb = c->D;
+  dx.half = plan.half / 64; dx.k_half = c->F;
+  dx.C = g->dx; dx.ldc = c->D; dx.m_half = dx.m_live = c->rows;
+  dx.part = on_dx ? part[1] : nullptr;
+
+  dw.M = ldd; dw.N = c->D; dw.K = c->rows;
+  dw.A = d; dw.lda = ldd;
+  dw.B = bf16(x); dw.ldb = ldx;
+  dw.C = g->dW1; dw.C2 = g->dW3; dw.ldc = c->D; dw.m_half = plan.half; dw.m_live = c->F;
+  dw.f32 = c->dw_dtype == LLATTN_F32;
+  dw.part = on_dw ? part[2] : nullptr;
+
+  // independent products of 128 x 128 tiles share a launch
+  if (on_gate && on_dw2 && plan.dgate.kind == SQUARE && plan.dw2.kind == SQUARE) {
+    launch_pair<DGateProduct, DwProduct>(gate, plan.dgate, dw2, plan.dw2, st);
+  } else {
+    if (on_gate) launch<DGateProduct>(gate, plan.dgate, st);
+    if (on_dw2) launch<DwProduct>(dw2, plan.dw2, st);
   }
-  if (g->dx) {
-    GatedArgs a{};
-    a.M = c->rows; a.N = c->D; a.K = ldd;
-    a.A = d; a.lda = ldd;
-    a.B = half_floats(w->W1); a.B2 = half_floats(w->W3); a.ldb = c->D;
-    a.half = plan.half / 64; a.k_half = c->F;
-    a.C = g->dx; a.ldc = c->D; a.m_half = a.m_live = c->rows;
-    product<false, true, true>(a, plan.dx, LLATTN_BF16, part, st);
+  if (on_dx && on_dw && plan.dx.kind == SQUARE && plan.dw.kind == SQUARE) {
+    launch_pair<DxProduct, DwProduct>(dx, plan.dx, dw, plan.dw, st);
+  } else {
+    if (on_dx) launch<DxProduct>(dx, plan.dx, st);
+    if (on_dw) launch<DwProduct>(dw, plan.dw, st);
   }
-  if (g->dW1) {
-    GatedArgs a{};
-    a.M = ldd; a.N = c->D; a.K = c->rows;
-    a.A = d; a.lda = ldd;
-    a.B = half_floats(x); a.ldb = ldx;
-    a.C = g->dW1; a.C2 = g->dW3; a.ldc = c->D; a.m_half = plan.half; a.m_live = c->F;
-    product<true, true, false>(a, plan.dw, c->dw_dtype, part, st);
-  }
-  if (g->dW2) {
-    GatedArgs a{};
-    a.M = c->D_out; a.N = c->F; a.K = c->rows;
-    a.A = half_floats(dy); a.lda = c->D_out;
-    a.B = half_floats(h); a.ldb = c->F;
-    a.C = g->dW2; a.ldc = c->F; a.m_half = a.m_live = c->D_out;
-    product<true, true, false>(a, plan.dw2, c->dw2_dtype, part, st);
-  }
+  const GatedArgs* args[] = {&dx, &dw, &dw2};
+  const Tiling* tilings[] = {&plan.dx, &plan.dw, &plan.dw2};
+  launch_reduce(args, tilings, 3, st);
   const auto bias = [&](float* out, const uint16_t* from, int64_t ld, int n) -> int32_t {
-    return out ? llattn_colsum(from, ld, c->rows, n, out, sums, plan.colsum, stream) : LLATTN_OK;
+    return out ? llattn_colsum(from, ld, c->rows, n, out, at, plan.colsum, stream) : LLATTN_OK;
   };
   if (const int32_t rc = bias(g->db1, d, ldd, c->F)) return rc;
   if (const int32_t rc = bias(g->db3, d + plan.half, ldd, c->F)) return rc;
-  if (const int32_t rc = bias(g->db2, half_floats(dy), c->D_out, c->D_out)) return rc;
+  if (const int32_t rc = bias(g->db2, bf16(dy), c->D_out, c->D_out)) return rc;
   return check_launch("llattn_gated_bwd");
 }

@@ -84,6 +84,7 @@ class LlattnHeadCfg(ctypes.Structure):  # include/llattn_train.h
     _fields_ = [(n, ctypes.c_int32) for n in ("rows", "V", "D", "piece", "dw_dtype")]
 
 
+GATED_FORWARD, GATED_ALONE, GATED_BACKWARD, GATED_KEPT = range(4)  # LLATTN_GATED_*
 MUON_BATCH, MUON_GROUPS = 128, 16  # LLATTN_MUON_BATCH, LLATTN_MUON_GROUPS
 
 
@@ -189,8 +190,8 @@ LM_SIGNATURES = {
     "llattn_grad_norm": (_I32, [_I32, _P, _P, _P, _P, _P, _SZ, _P]),
     "llattn_clip_grads": (_I32, [_I32, _P, _P, _P, _P, ctypes.c_double, _P, _P, _P, _SZ, _P]),
     "llattn_gated_bytes": (_SZ, [_GC, _I32]),
-    "llattn_gated_fwd": (_I32, [_GC, _P, _I64, _GW, _P, _P, _P, _P, _P, _SZ, _P]),
-    "llattn_gated_bwd": (_I32, [_GC, _P, _I64, _GW, _P, _P, _P, _P, _GG, _P, _SZ, _P]),
+    "llattn_gated_fwd": (_I32, [_GC, _P, _I64, _GW, _P, _P, _P, _SZ, _P]),
+    "llattn_gated_bwd": (_I32, [_GC, _P, _I64, _GW, _P, _P, _GG, _P, _SZ, _P]),
 }
 
 _lib = None

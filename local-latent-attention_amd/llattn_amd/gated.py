@@ -2,9 +2,9 @@
 the counterpart with a gate of :func:`llattn_amd.ffn.feed_forward`.
 
 Both projections, the activation and the product are one kernel; the backward's first product leaves the gradients of both
-projections, and every weight gradient comes out of one more.  Numerics: bf16 operands, fp32 sums, ``w1 x`` and ``w3 x`` not
-rounded, their gated product rounded to bf16 for the last projection; the backward keeps ``act(w1 x)`` and
-``act'(w1 x) w3 x`` in 24 bits.
+projections, and both weight gradients come out of one more.  Numerics: bf16 operands, fp32 sums, ``w1 x`` and ``w3 x`` not
+rounded, their gated product rounded to bf16 for the last projection (kept in fp32 where up to 64 rows are evaluated); the
+backward keeps ``act(w1 x)`` and ``act'(w1 x) w3 x`` in 24 bits.
 """
 from __future__ import annotations
 
@@ -18,7 +18,8 @@ from . import _lib as L
 from .linear import pack_params
 from .xent import _bf16_rows
 
-BF16 = torch.bfloat16
+BF16, F32 = torch.bfloat16, torch.float32
+TYPES = (F32, BF16)  # by LLATTN_F32, LLATTN_BF16
 ACTS = {"silu": 0, "gelu": 1}  # LLATTN_GATE_*
 MOST_ROWS, MOST_WIDTH = 1 << 23, 1 << 22
 
@@ -29,7 +30,10 @@ def _ptr(t):
 
 def _weights(ws, pads):
     """The weights in bf16, whole and aligned, with ``pads`` zero rows and columns behind; fp32 ones in one launch."""
-    cast = [w for w in ws if w.dtype is torch.float32]
+    if ws[0].dtype is ws[1].dtype is ws[2].dtype is BF16 and not any(map(any, pads)):
+        ws = [w if w.is_contiguous() else w.detach().contiguous() for w in ws]
+        return [w.detach().clone() if w.data_ptr() & 15 else w for w in ws]
+    cast = [w for w in ws if w.dtype is F32]
     done = dict(zip(map(id, cast), pack_params([([w], BF16) for w in cast]))) if cast else {}
     out = []
     for w, (rows, cols) in zip(ws, pads):
@@ -44,47 +48,44 @@ def _weights(ws, pads):
 def _bias(b, pad):
     if b is None:
         return None
-    b = b.detach().to(torch.float32).contiguous()
+    b = b.detach().to(F32).contiguous()
     if pad:
         return F.pad(b, (0, pad))
     return b.clone() if b.data_ptr() & 15 else b
 
 
-def _bytes(cfg, which):
+def _buffer(cfg, which, device):
     n = L.load().llattn_gated_bytes(ctypes.byref(cfg), which)
     if n == 0:
         L.check(L.ERR_SHAPE, "llattn_gated_bytes")
-    return n
+    return torch.empty((n,), dtype=torch.uint8, device=device), n
 
 
 def _forward(x, act, ps, saved):
-    """(y, what a backward reads)."""
+    """(y, configuration, what a backward reads)."""
     (w1, b1, w3, b3, w2, b2), dev = ps, x.device
     (Fd, D), Do = w1.shape, w2.shape[0]
     pd, pf, po = -D % 8, -Fd % 8, -Do % 8
-    xb = _bf16_rows(x.reshape(-1, D), pd)
+    xb = _bf16_rows(x if x.dim() == 2 else x.reshape(-1, D), pd)
     N = xb.shape[0]
     ws = _weights((w1, w3, w2), ((pf, pd), (pf, pd), (po, pf)))
-    bs = [_bias(b, p) for b, p in ((b1, pf), (b3, pf), (b2, po))]
-    f32 = torch.float32
-    cfg = L.LlattnGatedCfg(N, D + pd, Fd + pf, Do + po, act, L.F32 if w1.dtype is f32 or w3.dtype is f32 else L.BF16,
-                           L.F32 if w2.dtype is f32 else L.BF16)
+    cfg = L.LlattnGatedCfg(N, D + pd, Fd + pf, Do + po, act, L.F32 if w1.dtype is F32 or w3.dtype is F32 else L.BF16,
+                           L.F32 if w2.dtype is F32 else L.BF16)
     y = torch.empty((N, Do + po), dtype=BF16, device=dev)
-    h = p = s = None
-    if saved:
-        h = torch.empty((N, Fd + pf), dtype=BF16, device=dev)
-        p, s = (torch.empty((3 * N * (Fd + pf),), dtype=torch.uint8, device=dev) for _ in range(2))
+    kept = None
     if N:
-        n = _bytes(cfg, 0)
-        work = torch.empty((n,), dtype=torch.uint8, device=dev)
+        bs = (_bias(b1, pf), _bias(b3, pf), _bias(b2, po))
+        if saved:
+            kept, _ = _buffer(cfg, L.GATED_KEPT, dev)
+        work, n = _buffer(cfg, L.GATED_FORWARD if saved else L.GATED_ALONE, dev)
         from .ops import _call
         with L.on_device(dev):
             _call("llattn_gated_fwd", ctypes.byref(cfg), xb.data_ptr(), xb.stride(0),
-                  ctypes.byref(L.LlattnGatedWeights(*map(_ptr, ws), *map(_ptr, bs))), _ptr(h), _ptr(p), _ptr(s), y.data_ptr(),
-                  work.data_ptr(), n, L.stream_ptr(dev), work=6 * N * D * Fd)
+                  ctypes.byref(L.LlattnGatedWeights(*map(_ptr, ws), *map(_ptr, bs))), _ptr(kept), y.data_ptr(), work.data_ptr(), n,
+                  L.stream_ptr(dev), work=6 * N * D * Fd)
     if po:
         y = y[:, :Do]
-    return y.reshape(*x.shape[:-1], Do), cfg, (xb, *ws, h, p, s)
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], Do), cfg, (xb, *ws, kept)
 
 
 class _Gated(torch.autograd.Function):
@@ -98,43 +99,50 @@ class _Gated(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        xb, w1, w3, w2, h, p, s = ctx.saved_tensors
+        xb, w1, w3, w2, kept = ctx.saved_tensors
         cfg, x_shape, x_dtype, params = ctx.meta
         N, dev = cfg.rows, xb.device
-        want = [ctx.needs_input_grad[0], *ctx.needs_input_grad[2:]]
+        need = ctx.needs_input_grad
+        want = (need[0], *need[2:])
         if N == 0:
             grads = [torch.zeros(m[0], dtype=m[1], device=dev) if on else None
                      for m, on in zip([(x_shape, x_dtype), *params], want)]
             return grads[0], None, *grads[1:]
         Do = params[4][0][0]
-        d = dy.reshape(N, Do).to(BF16)
+        d = dy if dy.dim() == 2 else dy.reshape(N, Do)
+        if d.dtype is not BF16:
+            d = d.to(BF16)
         d = F.pad(d, (0, cfg.D_out - Do)) if cfg.D_out > Do else d.contiguous()
         if d.data_ptr() & 15:
             d = d.clone()
-        types = (torch.float32, BF16)
-        new = lambda on, *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=dev) if on else None  # noqa: E731
+        D, Fd, dt = cfg.D, cfg.F, TYPES[cfg.dw_dtype]
         both = want[1] or want[3]
-        dx = new(want[0], N, cfg.D, dtype=BF16)
-        dw1, dw3 = (new(both, cfg.F, cfg.D, dtype=types[cfg.dw_dtype]) for _ in range(2))
-        dw2 = new(want[5], cfg.D_out, cfg.F, dtype=types[cfg.dw2_dtype])
-        db1, db3, db2 = (new(want[i], n) for i, n in ((2, cfg.F), (4, cfg.F), (6, cfg.D_out)))
-        n = _bytes(cfg, 1)
-        work = torch.empty((n,), dtype=torch.uint8, device=dev)
+        dx = torch.empty((N, D), dtype=BF16, device=dev) if want[0] else None
+        dw1 = torch.empty((Fd, D), dtype=dt, device=dev) if both else None
+        dw3 = torch.empty((Fd, D), dtype=dt, device=dev) if both else None
+        dw2 = torch.empty((cfg.D_out, Fd), dtype=TYPES[cfg.dw2_dtype], device=dev) if want[5] else None
+        db1, db3, db2 = (torch.empty((n,), dtype=F32, device=dev) if want[i] else None
+                         for i, n in ((2, Fd), (4, Fd), (6, cfg.D_out)))
+        grads = (dx, dw1, dw3, dw2, db1, db3, db2)
+        work, n = _buffer(cfg, L.GATED_BACKWARD, dev)
         from .ops import _call
         with L.on_device(dev):
             _call("llattn_gated_bwd", ctypes.byref(cfg), xb.data_ptr(), xb.stride(0),
-                  ctypes.byref(L.LlattnGatedWeights(_ptr(w1), _ptr(w3), _ptr(w2), None, None, None)), h.data_ptr(), p.data_ptr(),
-                  s.data_ptr(), d.data_ptr(), ctypes.byref(L.LlattnGatedGrads(*map(_ptr, (dx, dw1, dw3, dw2, db1, db3, db2)))),
-                  work.data_ptr(), n, L.stream_ptr(dev), work=12 * N * cfg.D * cfg.F)
-        D = x_shape[-1]
-        out = [dx[:, :D].to(x_dtype).reshape(x_shape) if want[0] else None, None]
+                  ctypes.byref(L.LlattnGatedWeights(w1.data_ptr(), w3.data_ptr(), w2.data_ptr(), None, None, None)), kept.data_ptr(),
+                  d.data_ptr(), ctypes.byref(L.LlattnGatedGrads(*map(_ptr, grads))), work.data_ptr(), n, L.stream_ptr(dev),
+                  work=12 * N * D * Fd)
+        if dx is not None:
+            if D > x_shape[-1]:
+                dx = dx[:, :x_shape[-1]]
+            dx = dx.to(x_dtype) if len(x_shape) == 2 else dx.to(x_dtype).reshape(x_shape)
+        out = [dx, None]
         for g, m, on in zip((dw1, db1, dw3, db3, dw2, db2), params, want[1:]):
-            if not on:
+            if on:
+                if g.shape != m[0]:
+                    g = g[tuple(slice(k) for k in m[0])]
+                out.append(g if g.dtype is m[1] else g.to(m[1]))
+            else:
                 out.append(None)
-                continue
-            for axis, k in enumerate(m[0]):
-                g = g.narrow(axis, 0, k) if g.shape[axis] > k else g
-            out.append(g.to(m[1]))
         return tuple(out)
 
 
@@ -144,29 +152,30 @@ def gated_feed_forward(x: torch.Tensor, w1: torch.nn.Linear, w3: torch.nn.Linear
 
     ``w1`` and ``w3`` map D to F, ``w2`` F to any width, each with a bias or without.  ``x`` and the weights are bf16 or fp32,
     fp32 ones rounded to bf16 as under autocast; sums are fp32, gradients come in their input's type, those of weights and
-    biases from fp32 sums, ``x``'s rounded to bf16 before it is widened.  Widths that are not multiples of 8 are padded in copies.  Fewer than 2^23 rows.  Differentiable
-    once, in reverse mode.  GPU only."""
+    biases from fp32 sums, ``x``'s rounded to bf16 before it is widened.  Widths that are not multiples of 8 are padded in copies.
+    Fewer than 2^23 rows.  Differentiable once, in reverse mode.  GPU only."""
     from .ffn import _param
     if act not in ACTS:
         raise ValueError(f"gated_feed_forward: act must be one of {tuple(ACTS)}, got {act!r}")
     ps = [_param(m, n) for m in (w1, w3, w2) for n in ("weight", "bias")]
-    a, b, c = ps[0], ps[2], ps[4]
-    if x.dim() < 1 or a.dim() != 2 or a.shape[1] != x.shape[-1] or b.shape != a.shape or c.dim() != 2 or c.shape[1] != a.shape[0] \
-            or 0 in a.shape or 0 in c.shape:
-        raise ValueError(f"gated_feed_forward: weights {tuple(a.shape)}, {tuple(b.shape)} and {tuple(c.shape)} do not match "
-                         f"x {tuple(x.shape)}")
-    for w, bias in zip(ps[::2], ps[1::2]):
-        if bias is not None and bias.shape != w.shape[:1]:
-            raise ValueError(f"gated_feed_forward: bias {tuple(bias.shape)} for weight {tuple(w.shape)}")
-    tensors = [x, *(p for p in ps if p is not None)]
+    a, b, c, shape = ps[0].shape, ps[2].shape, ps[4].shape, x.shape
+    if not shape or len(a) != 2 or a[1] != shape[-1] or b != a or len(c) != 2 or c[1] != a[0] or 0 in a or 0 in c:
+        raise ValueError(f"gated_feed_forward: weights {tuple(a)}, {tuple(b)} and {tuple(c)} do not match x {tuple(shape)}")
+    tensors = [x, ps[0], ps[2], ps[4]]
+    for rows, bias in ((a[0], ps[1]), (a[0], ps[3]), (c[0], ps[5])):
+        if bias is not None:
+            if bias.shape != (rows,):
+                raise ValueError(f"gated_feed_forward: bias {tuple(bias.shape)} for {rows} outputs")
+            tensors.append(bias)
+    index = x.get_device()
     for t in tensors:
         L.dtype_code(t.dtype)
-    if max(*a.shape, *c.shape) >= MOST_WIDTH - 8 or x.numel() // x.shape[-1] >= MOST_ROWS:
-        raise ValueError(f"gated_feed_forward: fewer than 2^23 rows and widths below 2^22 expected, got x {tuple(x.shape)}, weights "
-                         f"{tuple(a.shape)} and {tuple(c.shape)}")
+    if max(*a, *c) >= MOST_WIDTH - 8 or x.numel() // a[1] >= MOST_ROWS:
+        raise ValueError(f"gated_feed_forward: fewer than 2^23 rows and widths below 2^22 expected, got x {tuple(shape)}, weights "
+                         f"{tuple(a)} and {tuple(c)}")
     L.refuse_tangents("gated_feed_forward", tensors)
-    L.require_gpu(*tensors)
-    if any(t.device != x.device for t in tensors):
+    if any(t.get_device() != index for t in tensors) or index < 0:
+        L.require_gpu(*tensors)
         raise ValueError(f"gated_feed_forward: tensors on {', '.join(sorted({str(t.device) for t in tensors}))}")
     if not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)):
         return _forward(x, ACTS[act], ps, False)[0]

@@ -49,8 +49,9 @@ def _act(name, a):
     return a * cdf, cdf + a * torch.exp(-0.5 * a * a) * 0.3989422804014327
 
 
-def _exact(x, layers, act, dy):
-    """Pairs (value, bound of the error before the last rounding) in 64 bits, in the order of NAMES."""
+def _exact(x, layers, act, dy, h_rounded=True):
+    """Pairs (value, bound of the error before the last rounding) in 64 bits, in the order of NAMES.  h not rounded: two bf16
+    halves of it, 2^-16 of itself."""
     x, dy = x.detach().to(BF16).double(), dy.to(BF16).double()
     w1, w3, w2 = (m.weight.detach().to(BF16).double() for m in layers)
     b1, b3, b2 = (torch.zeros((), dtype=torch.float64, device=DEV) if m.bias is None else m.bias.detach().double() for m in layers)
@@ -63,7 +64,7 @@ def _exact(x, layers, act, dy):
     ef, edf = 1.13 * ea + 2e-5 * f.abs(), 0.8 * ea + 2e-5
     h = f * u
     eh = f.abs() * eu + u.abs() * ef + ef * eu
-    eh = eh + B16 * (h.abs() + eh)
+    eh = eh + (B16 if h_rounded else 2.0 ** -16) * (h.abs() + eh)
     y = h @ w2.t() + b2
     ey = eh @ w2.abs().t() + c(Fd) * ((h.abs() + eh) @ w2.abs().t() + b2.abs())
     p, ep = f, ef + 2.0 ** -15 * (f.abs() + ef)
@@ -126,8 +127,11 @@ def test_values_and_gradients(case):
     for name, t, (want, err) in zip(NAMES, got, _exact(x, layers, act, dy)):
         if t is not None:
             _near(t, want, err, name)
-    with torch.no_grad():  # nothing kept: the same values
-        assert torch.equal(_ffn(x, *layers, act=act), got[0])
+    with torch.no_grad():  # nothing kept: the same values, up to 64 rows without the rounding of h
+        y = _ffn(x, *layers, act=act)
+    if N > 64:
+        assert torch.equal(y, got[0])
+    _near(y, *_exact(x, layers, act, dy, h_rounded=N > 64)[0], "y alone")
     again = _grads(x, layers, act, dy)
     assert all(a is None or torch.equal(a, b) for a, b in zip(got, again))
 
@@ -211,9 +215,10 @@ def test_strides_and_alignment():
     layers = _layers(64, 96, 64, bias=False)
     big = torch.randn(50, 3, 67, generator=torch.Generator().manual_seed(3)).to(BF16).to(DEV)
     x = big[:, 1, 2:66]
-    want = _ffn(x.contiguous(), *layers)
-    assert torch.equal(_ffn(x, *layers), want)
-    assert torch.equal(_ffn(x.t().contiguous().t(), *layers), want)
+    with torch.no_grad():
+        want = _ffn(x.contiguous(), *layers)
+        assert torch.equal(_ffn(x, *layers), want)
+        assert torch.equal(_ffn(x.t().contiguous().t(), *layers), want)
     other = []
     for m in layers:
         n = torch.nn.Linear(1, 1, bias=False)
@@ -221,7 +226,8 @@ def test_strides_and_alignment():
         flat[1:] = m.weight.detach().t().reshape(-1)
         n.weight = torch.nn.Parameter(flat[1:].view(m.weight.shape[1], m.weight.shape[0]).t())
         other.append(n)
-    assert torch.equal(_ffn(x, *other), want)
+    with torch.no_grad():
+        assert torch.equal(_ffn(x, *other), want)
     dy = torch.randn(64, generator=torch.Generator().manual_seed(4)).to(BF16).to(DEV)
     x0 = x.detach().requires_grad_()
     a = _grads(x0, layers, "silu", dy.expand(50, 64))
@@ -258,6 +264,47 @@ def test_rows_stay_apart():
     keep[77] = keep[150] = False
     for i in (0, 1):
         assert torch.equal(got[i][keep], clean[i][keep]) and bool(got[i][77].isnan().all())
+    with torch.no_grad():  # the kernels for few rows
+        a, b = _ffn(x[60:100].detach(), *layers), _ffn(x[140:170].detach(), *layers)
+        c = _ffn(torch.where(x.isfinite(), x, 0.0)[60:100].detach(), *layers)
+    keep = torch.arange(40, device=DEV) != 17
+    assert torch.equal(a[keep], c[keep]) and bool(a[17].isnan().all())
+    assert bool(b[10].isnan().any()) and bool(b[:10].isfinite().all()) and bool(b[11:].isfinite().all())
+
+
+@pytest.mark.parametrize("N", [1, 2, 15, 16, 17, 31, 32, 33, 48, 63, 64])
+def test_few_rows_forward_alone(N):
+    """The kernels for up to 64 rows: exact on whole numbers, each row's bits whatever the others are."""
+    for D, F, Do in ((8, 8, 8), (24, 40, 8), (264, 520, 72), (1408, 4096, 1408)):
+        x, w1, w3, w2, _ = _whole(N, D, F, Do)
+        layers = []
+        for w in (w1, w3, w2):
+            m = torch.nn.Linear(*reversed(w.shape), bias=False, device="meta")
+            m.weight = torch.nn.Parameter(w.to(BF16))
+            layers.append(m)
+        with torch.no_grad():
+            y = _ffn(x.to(BF16), *layers)
+        assert torch.equal(y, (((x @ w1.t()) * (x @ w3.t())) @ w2.t()).to(BF16)), (D, F, Do)
+    layers = _layers(136, 264, 136)
+    x = torch.randn(N, 136, generator=torch.Generator().manual_seed(N)).to(BF16).to(DEV)
+    with torch.no_grad():
+        y = _ffn(x, *layers, act="gelu")
+        for i in {0, N // 2, N - 1}:
+            assert torch.equal(_ffn(x[i:i + 1], *layers, act="gelu")[0], y[i])
+
+
+def test_a_large_h_of_few_rows():
+    """h past bf16's range, which its two halves cannot hold: infinite, as where it is rounded."""
+    layers = _layers(8, 8, 8, bias=False)
+    with torch.no_grad():
+        for m in layers:
+            m.weight.zero_()
+        layers[0].weight[0, 0] = layers[1].weight[0, 1] = layers[2].weight[0, 0] = 1.0
+        x = torch.zeros(2, 8, dtype=BF16, device=DEV)
+        x[0, 0], x[0, 1] = 2.0 ** 64, 2.0 ** 63
+        x[1, 0], x[1, 1] = 2.0 ** 100, 2.0 ** 100
+        y = _ffn(x, *layers)
+    assert float(y[0, 0]) == 2.0 ** 127 and float(y[1, 0]) == float("inf")
 
 
 def test_streams_and_replays():

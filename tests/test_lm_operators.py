@@ -195,29 +195,32 @@ def _gated_cfg(rows=10, D=16, F=24, D_out=8, act=0, dw=0, dw2=1):
 @pytest.mark.parametrize("kw", [dict(rows=0), dict(rows=1 << 23), dict(D=0), dict(D=12), dict(F=4), dict(D_out=-8), dict(F=1 << 22), dict(act=2),
                                 dict(dw=2), dict(dw2=-1)], ids=str)
 def test_gated_sizes_refused(kw):
-    for which in (0, 1):
+    for which in range(4):
         assert L.load().llattn_gated_bytes(ctypes.byref(_gated_cfg(**kw)), which) == 0 and L.load().llattn_last_error()
-    assert L.load().llattn_gated_bytes(ctypes.byref(_gated_cfg()), 2) == 0
+        assert L.load().llattn_gated_bytes(ctypes.byref(_gated_cfg()), which) > 0
+    for which in (-1, 4):
+        assert L.load().llattn_gated_bytes(ctypes.byref(_gated_cfg()), which) == 0
 
 
+@pytest.mark.parametrize("kept", [AT, None])
 @pytest.mark.parametrize("kw,code", [(dict(x=None), 3), (dict(x=AT + 8), 3), (dict(ldx=8), 3), (dict(ldx=20), 3), (dict(ldx=1 << 23), 3), (dict(W1=None), 3),
-                                     (dict(W3=AT + 2), 3), (dict(b1=AT + 4), 3), (dict(y=None), 3), (dict(p=None), 3), (dict(s=None), 3),
-                                     (dict(h=None), 3), (dict(h=AT + 8), 3), (dict(ws=None), 5), (dict(ws=AT + 8), 5), (dict(n=100), 5)], ids=str)
-def test_gated_forward_refused(kw, code):
+                                     (dict(W3=AT + 2), 3), (dict(b1=AT + 4), 3), (dict(y=None), 3), (dict(y=AT + 8), 3), (dict(kept=AT + 8), 3),
+                                     (dict(ws=None), 5), (dict(ws=AT + 8), 5), (dict(n=100), 5)], ids=str)
+def test_gated_forward_refused(kw, code, kept):
     lib, cfg = L.load(), _gated_cfg()
-    a = dict(x=AT, ldx=16, W1=AT, W3=AT, W2=AT, b1=None, h=AT, p=AT, s=AT, y=AT, ws=AT, n=lib.llattn_gated_bytes(ctypes.byref(cfg), 0)) | kw
+    a = dict(x=AT, ldx=16, W1=AT, W3=AT, W2=AT, b1=None, kept=kept, y=AT, ws=AT, n=1 << 20) | kw
     w = L.LlattnGatedWeights(a["W1"], a["W3"], a["W2"], a["b1"], None, None)
-    assert lib.llattn_gated_fwd(ctypes.byref(cfg), a["x"], a["ldx"], ctypes.byref(w), a["h"], a["p"], a["s"], a["y"], a["ws"], a["n"], None) == code
+    assert lib.llattn_gated_fwd(ctypes.byref(cfg), a["x"], a["ldx"], ctypes.byref(w), a["kept"], a["y"], a["ws"], a["n"], None) == code
 
 
-@pytest.mark.parametrize("kw,code", [(dict(x=None), 3), (dict(h=None), 3), (dict(dy=None), 3), (dict(p=AT + 8), 3), (dict(dx=AT + 8), 3),
+@pytest.mark.parametrize("kw,code", [(dict(x=None), 3), (dict(kept=None), 3), (dict(dy=None), 3), (dict(kept=AT + 8), 3), (dict(dx=AT + 8), 3),
                                      (dict(dW1=None), 3), (dict(dW3=None), 3), (dict(ws=None), 5), (dict(n=100), 5)], ids=str)
 def test_gated_backward_refused(kw, code):
     lib, cfg = L.load(), _gated_cfg()
-    a = dict(x=AT, h=AT, p=AT, s=AT, dy=AT, dx=AT, dW1=AT, dW3=AT, dW2=AT, ws=AT, n=lib.llattn_gated_bytes(ctypes.byref(cfg), 1)) | kw
+    a = dict(x=AT, kept=AT, dy=AT, dx=AT, dW1=AT, dW3=AT, dW2=AT, ws=AT, n=lib.llattn_gated_bytes(ctypes.byref(cfg), L.GATED_BACKWARD)) | kw
     w = L.LlattnGatedWeights(AT, AT, AT, None, None, None)
     g = L.LlattnGatedGrads(a["dx"], a["dW1"], a["dW3"], a["dW2"], None, None, None)
-    assert lib.llattn_gated_bwd(ctypes.byref(cfg), a["x"], 16, ctypes.byref(w), a["h"], a["p"], a["s"], a["dy"], ctypes.byref(g), a["ws"],
+    assert lib.llattn_gated_bwd(ctypes.byref(cfg), a["x"], 16, ctypes.byref(w), a["kept"], a["dy"], ctypes.byref(g), a["ws"],
                                 a["n"], None) == code
 
 
