@@ -490,14 +490,19 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void gated_kernel(const
   __shared__ __align__(1024) unsigned char smem[Operands<P, S>::LDS];
   gated_tiles<P, S>(a, smem, blockIdx.x, gridDim.x);
 }
-// Two products in one launch: the workgroups of the first, a multiple of 8 (so that the second's are dealt to the XCDs as alone), then
-// the other's
+// Two products in one launch, of 128 x 128 tiles: the `first` workgroups of the one with the longer contraction (P0 where `lead`), a
+// multiple of 8 (so that the other's are dealt to the XCDs as alone), then the other's.
 template <typename P0, typename P1>
-__global__ __launch_bounds__(SquareShape::THREADS, SquareShape::W / 2) void gated_pair_kernel(const GatedArgs a, const GatedArgs b, int first) {
+__global__ __launch_bounds__(SquareShape::THREADS, SquareShape::W / 2) void gated_pair_kernel(const GatedArgs a, const GatedArgs b, int first,
+                                                                                             int lead) {
   __shared__ __align__(1024) unsigned char smem[std::max(Operands<P0, SquareShape>::LDS, Operands<P1, SquareShape>::LDS)];
-  const int v = blockIdx.x;
-  if (v >= first) gated_tiles<P1, SquareShape>(b, smem, v - first, 0);
-  else if (v < a.total) gated_tiles<P0, SquareShape>(a, smem, v, 0);
+  const bool ahead = (int)blockIdx.x < first;
+  const int v = ahead ? blockIdx.x : blockIdx.x - first;
+  if (ahead == (lead != 0)) {
+    if (v < a.total) gated_tiles<P0, SquareShape>(a, smem, v, 0);
+  } else {
+    if (v < b.total) gated_tiles<P1, SquareShape>(b, smem, v, 0);
+  }
 }
 
 // C = the sum over splits of the parts [splits][M][N], in order, plus the bias; rows as GatedArgs has them.  Up to three products
@@ -553,7 +558,7 @@ struct ThinArgs {
 };
 template <bool GATED, int NT, int W>
 __global__ __launch_bounds__(64 * W) void gated_thin_kernel(const ThinArgs a) {
-  constexpr int MATS = GATED ? 2 : 1, U = NT == 1 ? 4 : 2;
+  constexpr int MATS = GATED ? 2 : 1, U = NT == 1 ? (GATED ? 6 : 8) : NT == 2 ? 4 : 2;
   __shared__ f32x4 sums[W][MATS][NT][64];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, w = threadIdx.x >> 6;
   const int f0 = blockIdx.x * 16, steps = (a.K + 31) / 32;
@@ -689,8 +694,9 @@ void launch(GatedArgs& a, const Tiling& t, hipStream_t st) {
 }
 template <typename P0, typename P1>
 void launch_pair(GatedArgs& a, const Tiling& ta, GatedArgs& b, const Tiling& tb, hipStream_t st) {
-  const int first = (prepare<P0>(a, ta) + 7) / 8 * 8, n = first + prepare<P1>(b, tb);
-  hipLaunchKernelGGL((gated_pair_kernel<P0, P1>), dim3((unsigned)n), dim3(SquareShape::THREADS), 0, st, a, b, first);
+  const int na = prepare<P0>(a, ta), nb = prepare<P1>(b, tb), lead = a.per >= b.per, first = ((lead ? na : nb) + 7) / 8 * 8;
+  hipLaunchKernelGGL((gated_pair_kernel<P0, P1>), dim3((unsigned)(first + (lead ? nb : na))), dim3(SquareShape::THREADS), 0, st, a, b, first,
+                     lead);
 }
 // Adds up the parts of those products that have some
 void launch_reduce(const GatedArgs* const* a, const Tiling* const* t, int n, hipStream_t st) {
@@ -728,6 +734,9 @@ Plan plan_of(const llattn_gated_cfg* c) {
   p.dx = choose(c->rows, c->D, 2 * steps(c->F), kSplits, true);
   p.dw = choose(2 * (int64_t)p.half, c->D, steps(c->rows), kSplits, true);
   p.dw2 = choose(c->D_out, c->F, steps(c->rows), kSplits, true);
+  // The gate's gradients wait for memory at the end of a tile, dW2 hardly: side by side on a CU they take less (8192 x 1536 x 4096 277 us
+  // in a launch of 128 x 128 tiles; apart 121 and 184, or 183 with 128 x 128)
+  if (p.dw2.kind == SQUARE) p.dgate.kind = SQUARE;
   p.h = up((size_t)c->rows * c->F * 2);
   p.plane = up((size_t)c->rows * c->F * 3);
   p.d = up((size_t)c->rows * 2 * p.half * 2);
