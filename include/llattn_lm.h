@@ -70,8 +70,8 @@ int32_t llattn_clip_grads(int32_t n, const void* const* g, void* const* out, con
  *   a = x W1^T + b1,  u = x W3^T + b3,  h = act(a) u,  y = h W2^T + b2
  * with x [rows][D], W1 and W3 [F][D], W2 [D_out][F], y [rows][D_out], all bf16,
  * biases fp32 or NULL; products summed in fp32, a and u not rounded, h rounded
- * to bf16 (what the last product reads; forward alone over at most 64 rows it
- * stays in fp32).  act: LLATTN_GATE_SILU a / (1 + exp(-a)) or LLATTN_GATE_GELU
+ * to bf16 (what the last product reads; forward alone over at most 24 rows it
+ * keeps 16 bits).  act: LLATTN_GATE_SILU a / (1 + exp(-a)) or LLATTN_GATE_GELU
  * a Phi(a).  D, F and D_out are multiples of 8, weights and y contiguous, x of
  * row stride ldx (a multiple of 8, below 2^23); everything 16-byte aligned.
  *

@@ -543,110 +543,119 @@ __global__ __launch_bounds__(256) void gated_reduce_kernel(const ReduceArgs q) {
 
 // ---- few rows, forward alone ------------------------------------------------------------
 //
-// A workgroup takes 16 rows of the weights (of both, GATE) and all of x, its W waves the 32-k steps w, w + W, ... : every weight
-// is read once, straight into the operand of the matrix cores (lane (r, g): k 8 g .. of row r), W x 64 bytes of a row at a
-// time.  The waves' sums are added in LDS.  The last projection reads h in fp32 as two bf16 operands (16 bits of its significand):
-// y then carries its own rounding alone.  What bounds it: latency, and the reads of the weights.
+// A workgroup takes ROWS = 16 / SEG rows of the weights (of both, GATED) and all of x; its W waves take the 32-k steps w,
+// w + W, ...: every weight is read once, straight into the operand of the matrix cores (lane (r, g): k 8 g .. of a row).  With
+// SEG > 1 the operand's 16 rows are SEG segments of k of each row; a product with x's segment s counts in the rows of segment s
+// alone, so that few rows of weights still take whole loads, and there are enough workgroups for the chip's bandwidth.  The waves'
+// sums are added in LDS.  (Whole rows for both projections, halves for the last: D 1408, F 4096, one row 6.2 and 6.7 us; the last one
+// 10.4 by whole rows, 8.7 by quarters.)  h goes from one launch to the next as two bf16 values (16 bits of its significand), so y carries its own
+// rounding alone.  What bounds it: latency, and the reads of the weights.
 struct ThinArgs {
   int M, N, K;                     // rows (up to 16 NT); rows of the weights, their length
-  const uint16_t* x; int64_t ldx;  // GATE
-  float* h;                        // [M][N] (GATE), [M][K]
+  const uint16_t* x; int64_t ldx;  // [M][K]; the other kernel: h
+  uint16_t* h;                     // [2][M][F]: upper and lower part
   const uint16_t *W, *W3;
   const float *bias, *bias3;
   int act;
   uint16_t* y;
 };
-template <bool GATED, int NT, int W>
+template <bool GATED, int NT, int SEG, int W, int U>
 __global__ __launch_bounds__(64 * W) void gated_thin_kernel(const ThinArgs a) {
-  constexpr int MATS = GATED ? 2 : 1, U = NT == 1 ? (GATED ? 6 : 8) : NT == 2 ? 4 : 2;
+  constexpr int MATS = GATED ? 2 : 1, PARTS = GATED ? 1 : 2, ROWS = 16 / SEG;
   __shared__ f32x4 sums[W][MATS][NT][64];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, w = threadIdx.x >> 6;
-  const int f0 = blockIdx.x * 16, steps = (a.K + 31) / 32;
-  const bool row_ok = f0 + r < a.N;
-  const uint16_t* p[2] = {a.W + (int64_t)(f0 + r) * a.K + 8 * g, GATED ? a.W3 + (int64_t)(f0 + r) * a.K + 8 * g : nullptr};
-  f32x4 acc[MATS][NT];
+  const int f0 = blockIdx.x * ROWS, row = f0 + r % ROWS, seg = (a.K + 32 * SEG - 1) / (32 * SEG), k0 = 32 * seg * (r / ROWS);  // steps of a segment
+  const uint16_t* p[2] = {a.W + (int64_t)row * a.K + k0 + 8 * g, GATED ? a.W3 + (int64_t)row * a.K + k0 + 8 * g : nullptr};
+  const int64_t low = (int64_t)a.M * a.K;  // from h's upper part to its lower one
+  f32x4 acc[MATS][NT][SEG];
 #pragma unroll
   for (int m = 0; m < MATS; ++m)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s0 = w; s0 < steps; s0 += U * W) {
-    bf16x8 v[U][MATS], x[U][NT];
-    f32x4 h[U][NT][2];
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int q = 0; q < SEG; ++q) acc[m][t][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s0 = w; s0 < seg; s0 += U * W) {
+    bf16x8 v[U][MATS], x[U][NT][SEG][PARTS];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int s = s0 + u * W, k = 32 * s + 8 * g;
-      const bool ok = s < steps && k < a.K;
+      const int s = s0 + u * W;
       const uint4 zero = make_uint4(0, 0, 0, 0);
+      const bool ok = s < seg && row < a.N && k0 + 32 * s + 8 * g < a.K;
 #pragma unroll
-      for (int m = 0; m < MATS; ++m) v[u][m] = __builtin_bit_cast(bf16x8, ok && row_ok ? ld16(p[m] + 32 * s) : zero);
+      for (int m = 0; m < MATS; ++m) v[u][m] = __builtin_bit_cast(bf16x8, ok ? ld16(p[m] + 32 * s) : zero);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int n = 16 * t + r;
-        const bool live = ok && n < a.M;
-        if constexpr (GATED) {
-          x[u][t] = __builtin_bit_cast(bf16x8, live ? ld16(a.x + n * a.ldx + k) : zero);
-        } else {
-          const float* q = a.h + (int64_t)n * a.K + k;
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) h[u][t][e] = live ? *reinterpret_cast<const f32x4*>(q + 4 * e) : f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < SEG; ++q) {
+          const int n = 16 * t + r, k = 32 * (q * seg + s) + 8 * g;
+          const bool live = s < seg && n < a.M && k < a.K;
+#pragma unroll
+          for (int e = 0; e < PARTS; ++e) x[u][t][q][e] = __builtin_bit_cast(bf16x8, live ? ld16(a.x + e * low + n * a.ldx + k) : zero);
         }
-      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if constexpr (GATED) {
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int m = 0; m < MATS; ++m) acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u][m], x[u][t], acc[m][t], 0, 0, 0);
-        } else {
-          bf16x8 hi, lo;
+        for (int q = 0; q < SEG; ++q)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float f = h[u][t][e >> 2][e & 3];
-            hi[e] = (__bf16)f;
-            const float rest = f - (float)hi[e];
-            lo[e] = (__bf16)(fabsf(rest) < __builtin_inff() ? rest : 0.f);  // an infinity has no rest
-          }
-          acc[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u][0], hi, acc[0][t], 0, 0, 0);
-          acc[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u][0], lo, acc[0][t], 0, 0, 0);
-        }
-      }
+          for (int e = 0; e < PARTS; ++e)
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) acc[m][t][q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u][m], x[u][t][q][e], acc[m][t][q], 0, 0, 0);
   }
+  // lane (r, g) holds the operand's rows 4 g + e: segment (4 g) / ROWS counts
 #pragma unroll
   for (int m = 0; m < MATS; ++m)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) sums[w][m][t][lane] = acc[m][t];
+    for (int t = 0; t < NT; ++t) {
+      f32x4 x = acc[m][t][0];
+#pragma unroll
+      for (int q = 1; q < SEG; ++q)
+        if (4 * g / ROWS == q) x = acc[m][t][q];
+      sums[w][m][t][lane] = x;
+    }
   __syncthreads();
   if (w >= NT) return;
-  // wave t: rows 16 t + r of x, weights' rows f0 + 4 g + e
-  const int t = w, n = 16 * t + r, f = f0 + 4 * g;
+  // wave t: rows 16 t + r of x, weights' rows f0 + (4 g + e) % ROWS
+  const int t = w, n = 16 * t + r, f = f0 + 4 * g % ROWS;
   f32x4 out[MATS];
 #pragma unroll
   for (int m = 0; m < MATS; ++m) {
     out[m] = sums[0][m][t][lane];
     for (int q = 1; q < W; ++q) out[m] += sums[q][m][t][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {  // the segments
+      if (SEG == 4) out[m][e] += __shfl_xor(out[m][e], 16);
+      if (SEG >= 2) out[m][e] += __shfl_xor(out[m][e], 32);
+    }
   }
-  if (n >= a.M || f >= a.N) return;
+  if (n >= a.M || f >= a.N || 4 * g >= ROWS) return;
   if (a.bias) out[0] += *reinterpret_cast<const f32x4*>(a.bias + f);
   if constexpr (GATED) {
     if (a.bias3) out[1] += *reinterpret_cast<const f32x4*>(a.bias3 + f);
+    f32x4 rest;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float v, dv;
       activation(a.act, out[0][e], v, dv);
       out[0][e] = v * out[1][e];
+      const float d = out[0][e] - bf2f(f2bf(out[0][e]));
+      rest[e] = fabsf(d) < __builtin_inff() ? d : 0.f;  // an infinity has no rest
     }
-    *reinterpret_cast<f32x4*>(a.h + (int64_t)n * a.N + f) = out[0];
+    uint16_t* const h = a.h + (int64_t)n * a.N + f;
+    *reinterpret_cast<uint2*>(h) = make_uint2(pack_bf16x2(out[0][0], out[0][1]), pack_bf16x2(out[0][2], out[0][3]));
+    *reinterpret_cast<uint2*>(h + (int64_t)a.M * a.N) = make_uint2(pack_bf16x2(rest[0], rest[1]), pack_bf16x2(rest[2], rest[3]));
   } else {
     *reinterpret_cast<uint2*>(a.y + (int64_t)n * a.N + f) =
         make_uint2(pack_bf16x2(out[0][0], out[0][1]), pack_bf16x2(out[0][2], out[0][3]));
   }
 }
-template <int NT>
+template <int NT, int S0, int U0, int S1, int W1, int U1>
 void launch_thin(const ThinArgs& gate, const ThinArgs& out, hipStream_t st) {
-  hipLaunchKernelGGL((gated_thin_kernel<true, NT, 8>), dim3((gate.N + 15) / 16), dim3(512), 0, st, gate);
-  hipLaunchKernelGGL((gated_thin_kernel<false, NT, 16>), dim3((out.N + 15) / 16), dim3(1024), 0, st, out);
+  constexpr int R0 = 16 / S0, R1 = 16 / S1;
+  hipLaunchKernelGGL((gated_thin_kernel<true, NT, S0, 8, U0>), dim3((gate.N + R0 - 1) / R0), dim3(512), 0, st, gate);
+  hipLaunchKernelGGL((gated_thin_kernel<false, NT, S1, W1, U1>), dim3((out.N + R1 - 1) / R1), dim3(64 * W1), 0, st, out);
 }
 
 // ---- launches ------------------------------------------------------------------------------
@@ -715,7 +724,10 @@ void launch_reduce(const GatedArgs* const* a, const Tiling* const* t, int n, hip
   hipLaunchKernelGGL(gated_reduce_kernel, dim3((unsigned)blocks), dim3(256), 0, st, q);
 }
 
-constexpr int kSplits = 16, kThinRows = 64;
+constexpr int kSplits = 16;
+// Rows of a forward alone that the kernels for few of them take.  us in a graph, these and the tiles, D 1408, F 4096: 1 row 11.7 and 23.6,
+// 16 rows 17.8 and 24.7, 24 rows 24.1 and 25.4, 32 rows 27.1 and 25.8 (F 256: 6.4 and 8.8)
+constexpr int kThinRows = 24;
 struct Plan {
   int half;                 // columns of da (and of du): F rounded up to 64
   Tiling gate, out, dgate, dx, dw, dw2;
@@ -747,7 +759,7 @@ Plan plan_of(const llattn_gated_cfg* c) {
   p.colsum = up(std::max(llattn_colsum_workspace_size(c->rows, c->F), llattn_colsum_workspace_size(c->rows, c->D_out)));
   return p;
 }
-// Forward with a backward to follow, forward alone (h in it, in fp32 where rows are few), backward, what is kept between them
+// Forward with a backward to follow, forward alone (h in it, as two bf16 values where rows are few), backward, what is kept between them
 enum Space { FORWARD = LLATTN_GATED_FORWARD, ALONE = LLATTN_GATED_ALONE, BACKWARD = LLATTN_GATED_BACKWARD, KEPT = LLATTN_GATED_KEPT };
 size_t bytes_of(const llattn_gated_cfg* c, const Plan& p, int which) {
   switch (which) {
@@ -813,11 +825,11 @@ extern "C" int32_t llattn_gated_fwd(const llattn_gated_cfg* c, const void* x, in
     gate.W = bf16(w->W1); gate.W3 = bf16(w->W3); out.W = bf16(w->W2);
     gate.bias = w->b1; gate.bias3 = w->b3; out.bias = w->b2;
     gate.act = c->act;
-    gate.h = out.h = reinterpret_cast<float*>(ws);
+    gate.h = reinterpret_cast<uint16_t*>(ws);
+    out.x = gate.h; out.ldx = c->F;
     out.y = static_cast<uint16_t*>(y);
-    if (c->rows <= 16) launch_thin<1>(gate, out, st);
-    else if (c->rows <= 32) launch_thin<2>(gate, out, st);
-    else launch_thin<4>(gate, out, st);
+    if (c->rows <= 16) launch_thin<1, 1, 6, 2, 8, 8>(gate, out, st);
+    else launch_thin<2, 1, 4, 2, 8, 2>(gate, out, st);
     return check_launch("llattn_gated_fwd");
   }
   GatedArgs a{};

@@ -127,11 +127,11 @@ def test_values_and_gradients(case):
     for name, t, (want, err) in zip(NAMES, got, _exact(x, layers, act, dy)):
         if t is not None:
             _near(t, want, err, name)
-    with torch.no_grad():  # nothing kept: the same values, up to 64 rows without the rounding of h
+    with torch.no_grad():  # nothing kept: the same values, up to 24 rows without the rounding of h
         y = _ffn(x, *layers, act=act)
-    if N > 64:
+    if N > 24:
         assert torch.equal(y, got[0])
-    _near(y, *_exact(x, layers, act, dy, h_rounded=N > 64)[0], "y alone")
+    _near(y, *_exact(x, layers, act, dy, h_rounded=N > 24)[0], "y alone")
     again = _grads(x, layers, act, dy)
     assert all(a is None or torch.equal(a, b) for a, b in zip(got, again))
 
@@ -265,16 +265,16 @@ def test_rows_stay_apart():
     for i in (0, 1):
         assert torch.equal(got[i][keep], clean[i][keep]) and bool(got[i][77].isnan().all())
     with torch.no_grad():  # the kernels for few rows
-        a, b = _ffn(x[60:100].detach(), *layers), _ffn(x[140:170].detach(), *layers)
-        c = _ffn(torch.where(x.isfinite(), x, 0.0)[60:100].detach(), *layers)
-    keep = torch.arange(40, device=DEV) != 17
+        a, b = _ffn(x[60:84].detach(), *layers), _ffn(x[140:160].detach(), *layers)
+        c = _ffn(torch.where(x.isfinite(), x, 0.0)[60:84].detach(), *layers)
+    keep = torch.arange(24, device=DEV) != 17
     assert torch.equal(a[keep], c[keep]) and bool(a[17].isnan().all())
     assert bool(b[10].isnan().any()) and bool(b[:10].isfinite().all()) and bool(b[11:].isfinite().all())
 
 
-@pytest.mark.parametrize("N", [1, 2, 15, 16, 17, 31, 32, 33, 48, 63, 64])
+@pytest.mark.parametrize("N", [1, 2, 15, 16, 17, 23, 24])
 def test_few_rows_forward_alone(N):
-    """The kernels for up to 64 rows: exact on whole numbers, each row's bits whatever the others are."""
+    """The kernels for up to 24 rows: exact on whole numbers, each row's bits whatever the others are."""
     for D, F, Do in ((8, 8, 8), (24, 40, 8), (264, 520, 72), (1408, 4096, 1408)):
         x, w1, w3, w2, _ = _whole(N, D, F, Do)
         layers = []
