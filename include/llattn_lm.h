@@ -41,7 +41,8 @@ typedef struct llattn_embed_cfg {
 
 int32_t llattn_embed_fwd(const llattn_embed_cfg* cfg, const void* ids, const void* pos, const void* W, int64_t ldw,
                          const void* Pos, int64_t ldp, void* out, void* stream);
-/* Workspace bytes of llattn_embed_bwd for a configuration; has_pos: pos is not NULL.  0 with an error message on a bad one. */
+/* Workspace bytes of llattn_embed_bwd for a configuration (1: it needs none, and takes NULL); has_pos: pos is not NULL.  0 with
+ * an error message on a bad one. */
 size_t llattn_embed_bytes(const llattn_embed_cfg* cfg, int32_t has_pos);
 int32_t llattn_embed_bwd(const llattn_embed_cfg* cfg, const void* ids, const void* pos, const void* dout, void* dW,
                          void* dPos, void* workspace, size_t workspace_bytes, void* stream);

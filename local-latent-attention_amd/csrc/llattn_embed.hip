@@ -683,7 +683,7 @@ struct Plan {
   int Dp;
   int trees;
   size_t set_bytes[2], tree_bytes;
-  size_t bytes() const { return 256 + set_bytes[0] + set_bytes[1] + trees * tree_bytes; }
+  size_t bytes() const { return set_bytes[0] ? 256 + set_bytes[0] + set_bytes[1] + trees * tree_bytes : 1; }
 };
 Plan plan_of(const llattn_embed_cfg* c, bool has_pos) {
   Plan p{};
@@ -774,7 +774,7 @@ extern "C" int32_t llattn_embed_bwd(const llattn_embed_cfg* c, const void* ids, 
   if (!whole(ids, c->index_bytes) || !whole(pos, c->index_bytes) || !whole(dout, size) || !whole(dW, size) || !whole(dPos, size))
     return fail(LLATTN_ERR_LAYOUT, "llattn_embed_bwd: a tensor is not aligned to its elements");
   const Plan p = plan_of(c, pos != nullptr);
-  if (!workspace || workspace_bytes < p.bytes() || !aligned16(workspace))
+  if (p.bytes() > 1 && (!workspace || workspace_bytes < p.bytes() || !aligned16(workspace)))
     return fail(LLATTN_ERR_WORKSPACE, "llattn_embed_bwd: needs %zu workspace bytes (got %zu)", p.bytes(), workspace_bytes);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t table[2] = {dW ? c->V : 0, dPos ? c->P : 0};
@@ -784,7 +784,7 @@ extern "C" int32_t llattn_embed_bwd(const llattn_embed_cfg* c, const void* ids, 
   const size_t r = (size_t)c->rows;
   SortArgs s{};
   s.rows = (int)c->rows;
-  s.counted = reinterpret_cast<int32_t*>(take(256));
+  if (!scan) s.counted = reinterpret_cast<int32_t*>(take(256));
   const auto keyed = [&](Keys& k, const void* keys, int R, int64_t padding) {
     k.keys = keys; k.index_bytes = c->index_bytes; k.R = R; k.padding = padding; k.buckets = buckets_of(R); k.per = (int)ceil_div(R, k.buckets);
     if (scan) return;

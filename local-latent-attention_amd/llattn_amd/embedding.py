@@ -13,8 +13,10 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
+from . import ops
 
 MOST = 1 << 22  # rows of a table
+_INDEX = (torch.int64, torch.int32)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -24,7 +26,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def _index(t: torch.Tensor) -> torch.Tensor:
     """The indices in order, of 32 or 64 bits (their shape is of no matter to a kernel)."""
-    t = t if t.dtype in (torch.int64, torch.int32) else t.to(torch.int64)
+    t = t if t.dtype in _INDEX else t.to(torch.int64)
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -45,12 +47,32 @@ def _forward(ids, weight, position, positions, scale, padding):
     out = torch.empty((*shape, D), dtype=dtype, device=dev)
     if cfg.rows:
         w, q = _rows(weight), None if position is None else _rows(position)
-        from .ops import _call
         with L.on_device(dev):
-            _call("llattn_embed_fwd", ctypes.byref(cfg), i.data_ptr(), _ptr(p), w.data_ptr(), w.stride(0), _ptr(q),
-                  0 if q is None else q.stride(0), out.data_ptr(), L.stream_ptr(dev),
-                  work=(2 + (q is not None)) * cfg.rows * D * out.element_size())
+            ops._call("llattn_embed_fwd", ctypes.byref(cfg), i.data_ptr(), _ptr(p), w.data_ptr(), w.stride(0), _ptr(q),
+                      0 if q is None else q.stride(0), out.data_ptr(), L.stream_ptr(dev),
+                      work=(2 + (q is not None)) * cfg.rows * D * out.element_size())
     return out, i, p, cfg
+
+
+def _backward(ctx, dout):
+    i, p = ctx.saved_tensors
+    cfg, w_shape, p_shape = ctx.meta
+    _, want_w, want_p, *_ = ctx.needs_input_grad
+    dw = dout.new_empty(w_shape) if want_w else None
+    dp = dout.new_empty(p_shape) if want_p else None
+    d = dout if dout.is_contiguous() else dout.contiguous()
+    dev, ref = d.device, ctypes.byref(cfg)
+    n = L.load().llattn_embed_bytes(ref, int(p is not None))
+    if n == 0:
+        L.check(L.ERR_SHAPE, "llattn_embed_bytes")
+    ws = torch.empty((n,), dtype=torch.uint8, device=dev) if n > 1 else None
+    with L.on_device(dev):
+        ops._call("llattn_embed_bwd", ref, i.data_ptr(), _ptr(p), d.data_ptr(), _ptr(dw), _ptr(dp), _ptr(ws), n,
+                  L.stream_ptr(dev), work=(cfg.rows + cfg.V + cfg.P) * cfg.D * d.element_size())
+    return None, dw, dp, None, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class _Embed(torch.autograd.Function):
@@ -62,25 +84,9 @@ class _Embed(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        i, p = ctx.saved_tensors
-        cfg, w_shape, p_shape = ctx.meta
-        dev, dtype = dout.device, dout.dtype
-        need = ctx.needs_input_grad
-        dw = torch.empty(w_shape, dtype=dtype, device=dev) if need[1] else None
-        dp = torch.empty(p_shape, dtype=dtype, device=dev) if p_shape is not None and need[2] else None
-        d = dout if dout.is_contiguous() else dout.contiguous()
-        ref = ctypes.byref(cfg)
-        n = L.load().llattn_embed_bytes(ref, int(p is not None))
-        if n == 0:
-            L.check(L.ERR_SHAPE, "llattn_embed_bytes")
-        ws = torch.empty((n,), dtype=torch.uint8, device=dev)
-        from .ops import _call
-        with L.on_device(dev):
-            _call("llattn_embed_bwd", ref, i.data_ptr(), _ptr(p), d.data_ptr(), _ptr(dw), _ptr(dp), ws.data_ptr(), n,
-                  L.stream_ptr(dev), work=(cfg.rows + cfg.V + cfg.P) * cfg.D * d.element_size())
-        return None, dw, dp, None, None, None
+        # a graph of the gradients is recorded: it refuses to go on; without one the wrapper has nothing to do
+        return _backward_once(ctx, dout) if torch.is_grad_enabled() else _backward(ctx, dout)
 
 
 def _check_integers(name: str, t: torch.Tensor) -> None:
@@ -98,38 +104,47 @@ def embed(ids: torch.Tensor, weight: torch.Tensor, position: torch.Tensor | None
     position outside ``[0, P)`` gives a row of NaN and no gradient to the table that has no such row.  Gradients are
     whole tables in their table's type, summed in fp32 in a fixed order (no atomics); the row ``padding_idx`` of
     ``weight`` gets none.  V and P at most 2^22.  Differentiable once, in reverse mode.  GPU only."""
-    if weight.dim() != 2 or 0 in weight.shape:
-        raise ValueError(f"embed: weight must be a non-empty matrix, got shape {tuple(weight.shape)}")
-    V, D = weight.shape
-    _check_integers("ids", ids)
-    L.dtype_code(weight.dtype)
-    if position is not None and (position.dim() != 2 or position.shape[1] != D or not len(position)
-                                 or position.dtype is not weight.dtype):
-        raise ValueError(f"embed: position {tuple(position.shape)} ({position.dtype}) does not match weight {tuple(weight.shape)} "
-                         f"({weight.dtype})")
-    if max(V, 0 if position is None else len(position)) > MOST:
+    w_shape, dtype = weight.shape, weight.dtype
+    if len(w_shape) != 2 or 0 in w_shape:
+        raise ValueError(f"embed: weight must be a non-empty matrix, got shape {tuple(w_shape)}")
+    V, D = w_shape
+    if ids.dtype not in _INDEX:
+        _check_integers("ids", ids)
+    L.dtype_code(dtype)
+    tensors = [ids, weight]
+    P = 0
+    if position is not None:
+        p_shape = position.shape
+        if len(p_shape) != 2 or p_shape[1] != D or not p_shape[0] or position.dtype is not dtype:
+            raise ValueError(f"embed: position {tuple(p_shape)} ({position.dtype}) does not match weight {tuple(w_shape)} ({dtype})")
+        P = p_shape[0]
+        tensors.append(position)
+    if V > MOST or P > MOST:
         raise ValueError(f"embed: at most {MOST} rows in a table")
     if positions is not None:
         if position is None:
             raise ValueError("embed: positions without position rows")
-        _check_integers("positions", positions)
+        if positions.dtype not in _INDEX:
+            _check_integers("positions", positions)
         if positions.shape != ids.shape:
             raise ValueError(f"embed: positions {tuple(positions.shape)} for ids {tuple(ids.shape)}")
-    elif position is not None and ids.dim() and ids.shape[-1] > len(position):
-        raise ValueError(f"embed: {ids.shape[-1]} tokens in a row and {len(position)} positions")
-    if not isinstance(scale, Real):
+        tensors.append(positions)
+    elif P and ids.dim() and ids.shape[-1] > P:
+        raise ValueError(f"embed: {ids.shape[-1]} tokens in a row and {P} positions")
+    if type(scale) is not float and not isinstance(scale, Real):
         raise ValueError(f"embed: scale must be a number, got {type(scale).__name__}")
-    if padding_idx is not None and (not isinstance(padding_idx, Integral) or not -V <= padding_idx < V):
-        raise ValueError(f"embed: padding_idx {padding_idx} outside the {V} rows")
+    padding = -1
+    if padding_idx is not None:
+        if not isinstance(padding_idx, Integral) or not -V <= padding_idx < V:
+            raise ValueError(f"embed: padding_idx {padding_idx} outside the {V} rows")
+        padding = int(padding_idx) % V
     if ids.numel() >= 1 << 31:
         raise ValueError(f"embed: {ids.numel()} tokens, fewer than 2^31 expected")
-    tensors = [t for t in (ids, weight, position, positions) if t is not None]
-    L.refuse_tangents("embed", [t for t in (weight, position) if t is not None])
-    L.require_gpu(*tensors)
-    if len({t.device for t in tensors}) > 1:
+    L.refuse_tangents("embed", tensors)
+    index = weight.get_device()
+    if index < 0 or any([t.get_device() != index for t in tensors]):
+        L.require_gpu(*tensors)
         raise ValueError(f"embed: tensors on {', '.join(str(t.device) for t in tensors)}")
-    padding = -1 if padding_idx is None else int(padding_idx) % V
-    args = (ids, weight, position, positions, float(scale), padding)
-    if not (torch.is_grad_enabled() and (weight.requires_grad or position is not None and position.requires_grad)):
-        return _forward(*args)[0]
-    return _Embed.apply(*args)
+    if torch.is_grad_enabled() and (weight.requires_grad or P and position.requires_grad):
+        return _Embed.apply(ids, weight, position, positions, float(scale), padding)
+    return _forward(ids, weight, position, positions, float(scale), padding)[0]

@@ -15,6 +15,8 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
+from . import ops
+from .ffn import _param
 from .linear import pack_params
 from .xent import _bf16_rows
 
@@ -78,14 +80,63 @@ def _forward(x, act, ps, saved):
         if saved:
             kept, _ = _buffer(cfg, L.GATED_KEPT, dev)
         work, n = _buffer(cfg, L.GATED_FORWARD if saved else L.GATED_ALONE, dev)
-        from .ops import _call
         with L.on_device(dev):
-            _call("llattn_gated_fwd", ctypes.byref(cfg), xb.data_ptr(), xb.stride(0),
+            ops._call("llattn_gated_fwd", ctypes.byref(cfg), xb.data_ptr(), xb.stride(0),
                   ctypes.byref(L.LlattnGatedWeights(*map(_ptr, ws), *map(_ptr, bs))), _ptr(kept), y.data_ptr(), work.data_ptr(), n,
                   L.stream_ptr(dev), work=6 * N * D * Fd)
     if po:
         y = y[:, :Do]
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], Do), cfg, (xb, *ws, kept)
+
+
+def _backward(ctx, dy):
+    xb, w1, w3, w2, kept = ctx.saved_tensors
+    cfg, x_shape, x_dtype, params = ctx.meta
+    N, dev = cfg.rows, xb.device
+    need = ctx.needs_input_grad
+    want = (need[0], *need[2:])
+    if N == 0:
+        grads = [torch.zeros(m[0], dtype=m[1], device=dev) if on else None
+                 for m, on in zip([(x_shape, x_dtype), *params], want)]
+        return grads[0], None, *grads[1:]
+    Do = params[4][0][0]
+    d = dy if dy.dim() == 2 else dy.reshape(N, Do)
+    if d.dtype is not BF16:
+        d = d.to(BF16)
+    d = F.pad(d, (0, cfg.D_out - Do)) if cfg.D_out > Do else d.contiguous()
+    if d.data_ptr() & 15:
+        d = d.clone()
+    D, Fd, dt = cfg.D, cfg.F, TYPES[cfg.dw_dtype]
+    both = want[1] or want[3]
+    dx = torch.empty((N, D), dtype=BF16, device=dev) if want[0] else None
+    dw1 = torch.empty((Fd, D), dtype=dt, device=dev) if both else None
+    dw3 = torch.empty((Fd, D), dtype=dt, device=dev) if both else None
+    dw2 = torch.empty((cfg.D_out, Fd), dtype=TYPES[cfg.dw2_dtype], device=dev) if want[5] else None
+    db1, db3, db2 = (torch.empty((n,), dtype=F32, device=dev) if want[i] else None
+                     for i, n in ((2, Fd), (4, Fd), (6, cfg.D_out)))
+    grads = (dx, dw1, dw3, dw2, db1, db3, db2)
+    work, n = _buffer(cfg, L.GATED_BACKWARD, dev)
+    with L.on_device(dev):
+        ops._call("llattn_gated_bwd", ctypes.byref(cfg), xb.data_ptr(), xb.stride(0),
+              ctypes.byref(L.LlattnGatedWeights(w1.data_ptr(), w3.data_ptr(), w2.data_ptr(), None, None, None)), kept.data_ptr(),
+              d.data_ptr(), ctypes.byref(L.LlattnGatedGrads(*map(_ptr, grads))), work.data_ptr(), n, L.stream_ptr(dev),
+              work=12 * N * D * Fd)
+    if dx is not None:
+        if D > x_shape[-1]:
+            dx = dx[:, :x_shape[-1]]
+        dx = dx.to(x_dtype) if len(x_shape) == 2 else dx.to(x_dtype).reshape(x_shape)
+    out = [dx, None]
+    for g, m, on in zip((dw1, db1, dw3, db3, dw2, db2), params, want[1:]):
+        if on:
+            if g.shape != m[0]:
+                g = g[tuple(slice(k) for k in m[0])]
+            out.append(g if g.dtype is m[1] else g.to(m[1]))
+        else:
+            out.append(None)
+    return tuple(out)
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class _Gated(torch.autograd.Function):
@@ -97,53 +148,9 @@ class _Gated(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        xb, w1, w3, w2, kept = ctx.saved_tensors
-        cfg, x_shape, x_dtype, params = ctx.meta
-        N, dev = cfg.rows, xb.device
-        need = ctx.needs_input_grad
-        want = (need[0], *need[2:])
-        if N == 0:
-            grads = [torch.zeros(m[0], dtype=m[1], device=dev) if on else None
-                     for m, on in zip([(x_shape, x_dtype), *params], want)]
-            return grads[0], None, *grads[1:]
-        Do = params[4][0][0]
-        d = dy if dy.dim() == 2 else dy.reshape(N, Do)
-        if d.dtype is not BF16:
-            d = d.to(BF16)
-        d = F.pad(d, (0, cfg.D_out - Do)) if cfg.D_out > Do else d.contiguous()
-        if d.data_ptr() & 15:
-            d = d.clone()
-        D, Fd, dt = cfg.D, cfg.F, TYPES[cfg.dw_dtype]
-        both = want[1] or want[3]
-        dx = torch.empty((N, D), dtype=BF16, device=dev) if want[0] else None
-        dw1 = torch.empty((Fd, D), dtype=dt, device=dev) if both else None
-        dw3 = torch.empty((Fd, D), dtype=dt, device=dev) if both else None
-        dw2 = torch.empty((cfg.D_out, Fd), dtype=TYPES[cfg.dw2_dtype], device=dev) if want[5] else None
-        db1, db3, db2 = (torch.empty((n,), dtype=F32, device=dev) if want[i] else None
-                         for i, n in ((2, Fd), (4, Fd), (6, cfg.D_out)))
-        grads = (dx, dw1, dw3, dw2, db1, db3, db2)
-        work, n = _buffer(cfg, L.GATED_BACKWARD, dev)
-        from .ops import _call
-        with L.on_device(dev):
-            _call("llattn_gated_bwd", ctypes.byref(cfg), xb.data_ptr(), xb.stride(0),
-                  ctypes.byref(L.LlattnGatedWeights(w1.data_ptr(), w3.data_ptr(), w2.data_ptr(), None, None, None)), kept.data_ptr(),
-                  d.data_ptr(), ctypes.byref(L.LlattnGatedGrads(*map(_ptr, grads))), work.data_ptr(), n, L.stream_ptr(dev),
-                  work=12 * N * D * Fd)
-        if dx is not None:
-            if D > x_shape[-1]:
-                dx = dx[:, :x_shape[-1]]
-            dx = dx.to(x_dtype) if len(x_shape) == 2 else dx.to(x_dtype).reshape(x_shape)
-        out = [dx, None]
-        for g, m, on in zip((dw1, db1, dw3, db3, dw2, db2), params, want[1:]):
-            if on:
-                if g.shape != m[0]:
-                    g = g[tuple(slice(k) for k in m[0])]
-                out.append(g if g.dtype is m[1] else g.to(m[1]))
-            else:
-                out.append(None)
-        return tuple(out)
+        # a graph of the gradients is recorded: it refuses to go on; without one the wrapper has nothing to do
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
 
 
 def gated_feed_forward(x: torch.Tensor, w1: torch.nn.Linear, w3: torch.nn.Linear, w2: torch.nn.Linear,
@@ -154,7 +161,6 @@ def gated_feed_forward(x: torch.Tensor, w1: torch.nn.Linear, w3: torch.nn.Linear
     fp32 ones rounded to bf16 as under autocast; sums are fp32, gradients come in their input's type, those of weights and
     biases from fp32 sums, ``x``'s rounded to bf16 before it is widened.  Widths that are not multiples of 8 are padded in copies.
     Fewer than 2^23 rows.  Differentiable once, in reverse mode.  GPU only."""
-    from .ffn import _param
     if act not in ACTS:
         raise ValueError(f"gated_feed_forward: act must be one of {tuple(ACTS)}, got {act!r}")
     ps = [_param(m, n) for m in (w1, w3, w2) for n in ("weight", "bias")]
@@ -174,9 +180,9 @@ def gated_feed_forward(x: torch.Tensor, w1: torch.nn.Linear, w3: torch.nn.Linear
         raise ValueError(f"gated_feed_forward: fewer than 2^23 rows and widths below 2^22 expected, got x {tuple(shape)}, weights "
                          f"{tuple(a)} and {tuple(c)}")
     L.refuse_tangents("gated_feed_forward", tensors)
-    if any(t.get_device() != index for t in tensors) or index < 0:
+    if index < 0 or any([t.get_device() != index for t in tensors]):
         L.require_gpu(*tensors)
         raise ValueError(f"gated_feed_forward: tensors on {', '.join(sorted({str(t.device) for t in tensors}))}")
-    if not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)):
+    if not (torch.is_grad_enabled() and any([t.requires_grad for t in tensors])):
         return _forward(x, ACTS[act], ps, False)[0]
     return _Gated.apply(x, ACTS[act], *ps)
