@@ -17,6 +17,7 @@ import torch
 from . import _lib as L
 
 _CODE = {torch.float32: L.F32, torch.bfloat16: L.BF16}
+_TYPES, _STRIDED = set(_CODE), {torch.strided}
 
 
 def _flat(t: torch.Tensor):
@@ -29,30 +30,31 @@ def _flat(t: torch.Tensor):
     return t if t.is_contiguous() else None
 
 
-def _check(who: str, tensors) -> torch.device:
-    """The device of ``tensors`` (one at least), which are what the kernels take."""
-    devices = {t.get_device() for t in tensors}
-    for t in tensors:
-        if t.dtype not in _CODE:
-            raise ValueError(f"{who}: gradients must be fp32 or bf16, got {t.dtype}")
-        if t.layout is not torch.strided:
-            raise ValueError(f"{who}: gradients must be dense tensors, got {t.layout}")
+def _check(who: str, tensors) -> list:
+    """The types of ``tensors`` (one at least), which are what the kernels take: dense, fp32 or bf16, on one GPU."""
+    types = [t.dtype for t in tensors]
+    if not _TYPES.issuperset(types):
+        raise ValueError(f"{who}: gradients must be fp32 or bf16, got {(set(types) - _TYPES).pop()}")
+    layouts = {t.layout for t in tensors}
+    if layouts != _STRIDED:
+        raise ValueError(f"{who}: gradients must be dense tensors, got {(layouts - _STRIDED).pop()}")
     L.refuse_tangents(who, tensors)
+    devices = {t.get_device() for t in tensors}
     if min(devices) < 0:
         L.require_gpu(*tensors)
     if len(devices) > 1:
         raise ValueError(f"{who}: gradients on {len(devices)} devices")
-    return tensors[0].device
+    return types
 
 
 class _Arrays:
     """The host arrays of a call on contiguous tensors."""
 
-    def __init__(self, tensors):
+    def __init__(self, tensors, types):
         self.n = len(tensors)
         self.g = array("Q", [t.data_ptr() for t in tensors])
         self.numel = array("q", [t.numel() for t in tensors])
-        self.dtype = array("i", [_CODE[t.dtype] for t in tensors])
+        self.dtype = array("i", [_CODE[t] for t in types])
 
     def workspace(self, device):
         n = L.load().llattn_grad_norm_bytes(self.n, _at(self.numel))
@@ -87,10 +89,10 @@ def grad_norm(tensors) -> torch.Tensor:
     tensors = list(tensors)
     if not tensors:
         return torch.zeros(())
-    device = _check("grad_norm", tensors)
+    types, device = _check("grad_norm", tensors), tensors[0].device
     if not all([t.is_contiguous() for t in tensors]):
         tensors = [_whole(t) for t in tensors]
-    a = _Arrays(tensors)
+    a = _Arrays(tensors, types)
     ws, n = a.workspace(device)
     norm = torch.empty((), dtype=torch.float32, device=device)
     from .ops import _call
@@ -125,17 +127,16 @@ def _pairs(who: str, tensors, out):
 
 def _clip(who: str, tensors, out, max_norm: float, norm_in) -> torch.Tensor | None:
     """Scales ``tensors`` (one at least) into ``out`` (or in place); the norm where none is given."""
-    device = _check(who, tensors)
+    types, device = _check(who, tensors), tensors[0].device
     if norm_in is not None and (norm_in.numel() != 1 or norm_in.dtype is not torch.float32 or norm_in.device != device):
         raise ValueError(f"{who}: the norm must be one fp32 value on {device}, got {tuple(norm_in.shape)} {norm_in.dtype} on {norm_in.device}")
     written = tensors if out is None else out
-    if out is not None and ([t.shape for t in out] != [t.shape for t in tensors] or [t.dtype for t in out] != [t.dtype for t in tensors]
-                            or {t.get_device() for t in out} != {device.index}):
+    if out is not None and ([t.shape for t in out] != [t.shape for t in tensors] or [t.dtype for t in out] != types or {t.get_device() for t in out} != {device.index}):
         raise ValueError(f"{who}: outputs must have their gradients' shapes, types and device")
     src, dst, back = tensors, out, ()
     if not all([t.is_contiguous() for t in tensors]) or out is not None and not all([t.is_contiguous() for t in out]):
         src, dst, back = _pairs(who, tensors, out)
-    a = _Arrays(src)
+    a = _Arrays(src, types)
     o = None if dst is None else array("Q", [t.data_ptr() for t in dst])
     ws = norm = None
     n = 0
