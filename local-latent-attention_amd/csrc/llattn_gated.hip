@@ -42,7 +42,7 @@ struct GatedArgs {
   const float *bias, *bias2;
   uint16_t* h;                  // GATE: [M][N]
   int act;
-  unsigned char *p, *s;         // [M][N] of three bytes (Float24), or null (GATE)
+  unsigned char *p, *s;         // [M][N] as Float24 lays them out, or null (GATE)
   uint16_t* d; int64_t ldd;     // DGATE: [M][ldd], da in its columns, du from column ldd / 2 on
   void *C, *C2; int64_t ldc;    // rows [0, m_live) of each of the two halves of m_half rows (one half: m_half = M)
   int m_half, m_live;
@@ -74,8 +74,14 @@ __device__ __forceinline__ void activation(int act, float a, float& f, float& df
 }
 
 // Eight values in 24 bits, cut off: the upper halves in one plane, the next bytes in the plane behind it.  (Cut off, not rounded: no
-// NaN turns into another value.)
+// NaN turns into another value.)  Pieces of eight columns lie by blocks of 16 rows, then by column, then by row: what a wave writes
+// or reads at a time (four pieces of 16 rows) is one run of memory, in the gate's tiles and in those of its gradients
+// (row by row instead, training passes of 8192 x 1536 x 4096 took 897 us for 872, of 333 rows 195 for 174).
 struct Float24 {
+  static __host__ __device__ __forceinline__ int64_t elements(int64_t rows, int cols) { return (rows + 15) / 16 * 16 * cols; }
+  static __device__ __forceinline__ int64_t place(int row, int col, int cols) {
+    return (((int64_t)(row >> 4) * (cols >> 3) + (col >> 3)) * 16 + (row & 15)) * 8;
+  }
   uint4 hi;
   uint2 lo;
   static __device__ __forceinline__ uint32_t lows(const f32x4& x) {  // byte 1 of each
@@ -401,15 +407,15 @@ __device__ __forceinline__ void gated_tiles(const GatedArgs& a, unsigned char* s
           const int64_t o = (int64_t)row * a.N + c;
           st16(a.h + o, bf16s(fx * u, fy * t));
           if (a.p) {
-            const int64_t plane = 2 * (int64_t)a.M * a.N;
-            Float24::store(a.p, plane, o, fx, fy);
-            Float24::store(a.s, plane, o, x * u, y * t);
+            const int64_t plane = 2 * Float24::elements(a.M, a.N), at = Float24::place(row, c, a.N);
+            Float24::store(a.p, plane, at, fx, fy);
+            Float24::store(a.s, plane, at, x * u, y * t);
           }
         }
       }
     } else if constexpr (EPI == DGATE) {
       // p and s of a row of blocks are read a row ahead: left to the compiler, each pair of blocks waited for its own
-      const int64_t plane = 2 * (int64_t)a.M * a.N;
+      const int64_t plane = 2 * Float24::elements(a.M, a.N);
       Float24 p[2][NB / 2], s[2][NB / 2];
       const auto fetch = [&](auto it) {
         constexpr int i = decltype(it)::value;
@@ -417,7 +423,7 @@ __device__ __forceinline__ void gated_tiles(const GatedArgs& a, unsigned char* s
 #pragma unroll
         for (int j = 0; j < NB; j += 2) {
           const int c = pair(j);
-          const int64_t at = (int64_t)row * a.N + c;
+          const int64_t at = Float24::place(row, c, a.N);
           p[i & 1][j / 2] = s[i & 1][j / 2] = Float24{make_uint4(0, 0, 0, 0), make_uint2(0, 0)};
           if (row < a.M && c < a.N) {
             p[i & 1][j / 2].load(a.p, plane, at);
@@ -750,7 +756,7 @@ Plan plan_of(const llattn_gated_cfg* c) {
   // in a launch of 128 x 128 tiles; apart 121 and 184, or 183 with 128 x 128)
   if (p.dw2.kind == SQUARE) p.dgate.kind = SQUARE;
   p.h = up((size_t)c->rows * c->F * 2);
-  p.plane = up((size_t)c->rows * c->F * 3);
+  p.plane = up((size_t)Float24::elements(c->rows, c->F) * 3);
   p.d = up((size_t)c->rows * 2 * p.half * 2);
   p.part[0] = part(p.out, c->rows, c->D_out);
   p.part[1] = part(p.dx, c->rows, c->D);
