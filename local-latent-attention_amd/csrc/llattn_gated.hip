@@ -29,6 +29,9 @@ namespace {
 
 using namespace tiles;
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 // OUT: C, or fp32 parts of it
 enum Epilogue { GATE = 0, DGATE = 1, OUT = 2 };
 
@@ -76,14 +79,16 @@ __device__ __forceinline__ void activation(int act, float a, float& f, float& df
 // Eight values in 24 bits, cut off: the upper halves in one plane, the next bytes in the plane behind it.  (Cut off, not rounded: no
 // NaN turns into another value.)  Pieces of eight columns lie by blocks of 16 rows, then by column, then by row: what a wave writes
 // or reads at a time (four pieces of 16 rows) is one run of memory, in the gate's tiles and in those of its gradients
-// (row by row instead, training passes of 8192 x 1536 x 4096 took 897 us for 872, of 333 rows 195 for 174).
+// (row by row instead, training passes of 8192 x 1536 x 4096 took 897 us for 872, of 333 rows 195 for 174), and past the caches,
+// which it would empty of the operands: the gate's product 220 -> 209 us there, its gradients' beside dW2 258 -> 240, the next
+// products, which read h and d, 98 -> 92 and 198 -> 182.
 struct Float24 {
   static __host__ __device__ __forceinline__ int64_t elements(int64_t rows, int cols) { return (rows + 15) / 16 * 16 * cols; }
   static __device__ __forceinline__ int64_t place(int row, int col, int cols) {
     return (((int64_t)(row >> 4) * (cols >> 3) + (col >> 3)) * 16 + (row & 15)) * 8;
   }
-  uint4 hi;
-  uint2 lo;
+  u32x4 hi;
+  u32x2 lo;
   static __device__ __forceinline__ uint32_t lows(const f32x4& x) {  // byte 1 of each
     const uint32_t a = __builtin_amdgcn_perm(__float_as_uint(x[1]), __float_as_uint(x[0]), 0x0c0c0501);
     const uint32_t b = __builtin_amdgcn_perm(__float_as_uint(x[3]), __float_as_uint(x[2]), 0x05010c0c);
@@ -91,12 +96,12 @@ struct Float24 {
   }
   static __device__ __forceinline__ void store(unsigned char* plane, int64_t plane_bytes, int64_t at, const f32x4& x, const f32x4& y) {
     const auto hi2 = [](float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302); };
-    st16(plane + 2 * at, make_uint4(hi2(x[0], x[1]), hi2(x[2], x[3]), hi2(y[0], y[1]), hi2(y[2], y[3])));
-    *reinterpret_cast<uint2*>(plane + plane_bytes + at) = make_uint2(lows(x), lows(y));
+    __builtin_nontemporal_store(u32x4{hi2(x[0], x[1]), hi2(x[2], x[3]), hi2(y[0], y[1]), hi2(y[2], y[3])}, reinterpret_cast<u32x4*>(plane + 2 * at));
+    __builtin_nontemporal_store(u32x2{lows(x), lows(y)}, reinterpret_cast<u32x2*>(plane + plane_bytes + at));
   }
   __device__ __forceinline__ void load(const unsigned char* plane, int64_t plane_bytes, int64_t at) {
-    hi = ld16(plane + 2 * at);
-    lo = *reinterpret_cast<const uint2*>(plane + plane_bytes + at);
+    hi = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(plane + 2 * at));
+    lo = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(plane + plane_bytes + at));
   }
   __device__ __forceinline__ void get(f32x4& x, f32x4& y) const {
     const auto four = [](uint32_t h0, uint32_t h1, uint32_t l) {  // (upper half, byte) -> the upper three bytes
@@ -424,7 +429,7 @@ __device__ __forceinline__ void gated_tiles(const GatedArgs& a, unsigned char* s
         for (int j = 0; j < NB; j += 2) {
           const int c = pair(j);
           const int64_t at = Float24::place(row, c, a.N);
-          p[i & 1][j / 2] = s[i & 1][j / 2] = Float24{make_uint4(0, 0, 0, 0), make_uint2(0, 0)};
+          p[i & 1][j / 2] = s[i & 1][j / 2] = Float24{u32x4{0, 0, 0, 0}, u32x2{0, 0}};
           if (row < a.M && c < a.N) {
             p[i & 1][j / 2].load(a.p, plane, at);
             s[i & 1][j / 2].load(a.s, plane, at);
