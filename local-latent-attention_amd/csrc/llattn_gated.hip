@@ -446,7 +446,8 @@ __device__ __forceinline__ void gated_tiles(const GatedArgs& a, unsigned char* s
           f32x4 x = acc[i][j], y = acc[i][j + 1], m, n;
           swap(x, y);
           const int c = pair(j);
-          if (row >= a.M || 2 * c >= a.ldd) continue;  // columns from the last on: zeros, which the products contract over
+          if (row >= a.M || 2 * c >= a.ldd) continue;
+          if (c >= a.N) x = y = f32x4{0.f, 0.f, 0.f, 0.f};  // the next product contracts over these columns too
           uint16_t* o = a.d + (int64_t)row * a.ldd + c;
           s[i & 1][j / 2].get(m, n);
           st16(o, bf16s(x * m, y * n));

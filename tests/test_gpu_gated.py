@@ -343,3 +343,68 @@ def test_streams_and_replays():
         torch.cuda.synchronize()
         assert all(torch.equal(s, t) and torch.equal(s, e) for s, t, e in zip(out, want[i], eager))
     assert len(ps) == 6
+
+
+def test_an_infinite_gradient_stays_infinite():
+    # positive weights and values: every gradient of row 0 is infinite, none is 0 times infinity.  F is no whole step of the
+    # products over F, and W2 has zeros in the rows that dy's row 0 does not read
+    layers = _layers(8, 8, 16, bias=False)
+    with torch.no_grad():
+        for m in layers:
+            m.weight.fill_(0.5)
+        layers[2].weight[1:] = 0.0
+    x = torch.ones(3, 8, dtype=BF16, device=DEV, requires_grad=True)
+    dy = torch.zeros(3, 16, dtype=BF16, device=DEV)
+    dy[0, 0], dy[1:] = float("inf"), 1.0
+    y = _ffn(x, *layers)
+    dx, dw1, dw3, dw2 = torch.autograd.grad(y, [x] + [m.weight for m in layers], dy)
+    assert bool((dx[0] == float("inf")).all()) and bool(dx[1:].isfinite().all())
+    assert bool((dw1 == float("inf")).all()) and bool((dw3 == float("inf")).all())
+    assert bool((dw2[0] == float("inf")).all()) and bool(dw2[1:].isfinite().all())
+
+
+def test_no_second_derivatives():
+    layers = _layers(16, 24, 16)
+    x = torch.randn(5, 16, device=DEV, dtype=BF16, requires_grad=True)
+    dx, = torch.autograd.grad(_ffn(x, *layers).float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.float().sum().backward()
+
+
+def test_two_graphs_at_once():
+    # each has its own memory: replayed side by side on two streams they give what each gives alone
+    g = torch.Generator().manual_seed(11)
+    runs = []
+
+    def call(x, layers, dy):
+        out = _grads(x, layers, "gelu", dy)
+        with torch.no_grad():  # forward alone
+            return out + [_ffn(x, *layers, act="gelu")]
+    for n, seed in ((300, 0), (5, 1)):
+        layers = _layers(128, 320, 128, seed=seed)
+        x = torch.randn(n, 128, generator=g).to(BF16).to(DEV).requires_grad_()
+        dy = torch.randn(n, 128, generator=g).to(BF16).to(DEV)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = [t.clone() for t in call(x, layers, dy)]
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(x, layers, dy)
+        runs.append((graph, out, want, side, layers, x, dy))
+    for _ in range(3):
+        torch.cuda.synchronize()
+        for graph, *_, side, _, _, _ in runs:
+            with torch.cuda.stream(side):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, out, want, *_ in runs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_vectorised_calls_are_refused():
+    layers = _layers(16, 24, 16)
+    x = torch.randn(2, 5, 16, device=DEV, dtype=BF16)
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda v: _ffn(v, *layers))(x)
