@@ -58,8 +58,9 @@ int32_t llattn_embed_bwd(const llattn_embed_cfg* cfg, const void* ids, const voi
  *
  * llattn_grad_norm writes the norm (fp32).  llattn_clip_grads also writes out[i]
  * (out NULL: in place; where c is 1 nothing is written in place); out[i] may be
- * g[i] itself and overlaps nothing else.  With norm_in (a device fp32 value)
- * that is the norm and none is computed (norm NULL then). */
+ * g[i] itself and overlaps nothing else.  With norm_in (a device fp32 value
+ * outside of what is written) that is the norm and none is computed (norm NULL
+ * then). */
 size_t llattn_grad_norm_bytes(int32_t n, const int64_t* numel);
 int32_t llattn_grad_norm(int32_t n, const void* const* g, const int64_t* numel, const int32_t* dtype, float* norm,
                          void* workspace, size_t workspace_bytes, void* stream);
@@ -72,7 +73,8 @@ int32_t llattn_clip_grads(int32_t n, const void* const* g, void* const* out, con
  * with x [rows][D], W1 and W3 [F][D], W2 [D_out][F], y [rows][D_out], all bf16,
  * biases fp32 or NULL; products summed in fp32, a and u not rounded, h rounded
  * to bf16 (what the last product reads; forward alone over at most 24 rows it
- * keeps 16 bits).  act: LLATTN_GATE_SILU a / (1 + exp(-a)) or LLATTN_GATE_GELU
+ * keeps 16 bits, as the sum of two bf16 values: infinite weights of W2, which
+ * must be finite otherwise, give NaN there).  act: LLATTN_GATE_SILU a / (1 + exp(-a)) or LLATTN_GATE_GELU
  * a Phi(a).  D, F and D_out are multiples of 8, weights and y contiguous, x of
  * row stride ldx (a multiple of 8, below 2^23); everything 16-byte aligned.
  *

@@ -12,6 +12,7 @@
 // 0.34 ms (5.4 TB/s), scaling 0.79 ms (4.7 TB/s).  Eight loads ahead instead of four took 7% off the squares; chunks of
 // 65536, 1024 to 4096 workgroups and one workgroup a chunk were no quicker (the last 50% slower, as each adds up the parts).
 #include <algorithm>
+#include <new>
 #include <vector>
 
 #include "llattn_abi.h"
@@ -241,8 +242,9 @@ int32_t check_lists(const char* who, int32_t n, const void* const* g, void* cons
   return LLATTN_OK;
 }
 
-// What is written overlaps nothing else: neither another output nor an input but its own in place.
-int32_t check_apart(const char* who, int32_t n, const void* const* g, void* const* out, const int64_t* numel, const int32_t* dtype) {
+// What is written overlaps nothing else: neither another output nor an input but its own in place, nor the norm that is read.
+int32_t check_apart(const char* who, int32_t n, const void* const* g, void* const* out, const int64_t* numel, const int32_t* dtype,
+                    const float* norm_in) {
   struct Span { uintptr_t at, end; int i; };
   std::vector<Span> w;
   w.reserve(n);
@@ -253,12 +255,17 @@ int32_t check_apart(const char* who, int32_t n, const void* const* g, void* cons
   std::sort(w.begin(), w.end(), [](const Span& a, const Span& b) { return a.at < b.at; });
   for (size_t k = 1; k < w.size(); ++k)
     if (w[k].at < w[k - 1].end) return fail(LLATTN_ERR_LAYOUT, "%s: tensors %d and %d, which are written, overlap", who, w[k - 1].i, w[k].i);
+  const auto first = [&](uintptr_t at) {  // the first that ends past it
+    return std::upper_bound(w.begin(), w.end(), at, [](uintptr_t v, const Span& s) { return v < s.end; });
+  };
+  const uintptr_t norm = reinterpret_cast<uintptr_t>(norm_in);
+  if (const auto k = first(norm); norm && k != w.end() && k->at < norm + sizeof(float))
+    return fail(LLATTN_ERR_LAYOUT, "%s: tensor %d, which is written, holds the norm", who, k->i);
   if (!out) return LLATTN_OK;
   for (int i = 0; i < n; ++i) {
     if (!numel[i]) continue;
     const uintptr_t at = reinterpret_cast<uintptr_t>(g[i]), end = at + (uintptr_t)numel[i] * elem_size(dtype[i]);
-    auto k = std::upper_bound(w.begin(), w.end(), at, [](uintptr_t v, const Span& s) { return v < s.end; });  // first that ends past it
-    for (; k != w.end() && k->at < end; ++k)
+    for (auto k = first(at); k != w.end() && k->at < end; ++k)
       if (k->i != i || k->at != at) return fail(LLATTN_ERR_LAYOUT, "%s: output %d overlaps gradient %d", who, k->i, i);
   }
   return LLATTN_OK;
@@ -313,8 +320,14 @@ extern "C" int32_t llattn_clip_grads(int32_t n, const void* const* g, void* cons
                                      double max_norm, const float* norm_in, float* norm, void* workspace, size_t workspace_bytes,
                                      void* stream) {
   if (const int32_t rc = check_lists("llattn_clip_grads", n, g, out, numel, dtype)) return rc;
-  if (const int32_t rc = check_apart("llattn_clip_grads", n, g, out, numel, dtype)) return rc;
   if (!norm_in == !norm) return fail(LLATTN_ERR_LAYOUT, "llattn_clip_grads: one of norm_in and norm");
+  std::vector<Table> all;
+  try {  // both need memory of the host's, before anything is launched
+    if (const int32_t rc = check_apart("llattn_clip_grads", n, g, out, numel, dtype, norm_in)) return rc;
+    tables(n, g, out, numel, dtype, [&](const Table& t) { all.push_back(t); });
+  } catch (const std::bad_alloc&) {
+    return fail(LLATTN_ERR_SHAPE, "llattn_clip_grads: no memory for the tables of %d tensors", n);
+  }
   const hipStream_t st = static_cast<hipStream_t>(stream);
   double* part = static_cast<double*>(workspace);
   int parts = 0;
@@ -326,8 +339,6 @@ extern "C" int32_t llattn_clip_grads(int32_t n, const void* const* g, void* cons
     if (parts == 0) hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(256), 0, st, part, 0, norm);
   }
   // the last table first, as its gradients were read last
-  std::vector<Table> all;
-  tables(n, g, out, numel, dtype, [&](const Table& t) { all.push_back(t); });
   for (size_t k = all.size(); k-- > 0;)
     hipLaunchKernelGGL(grad_scale_kernel, dim3(grid_of(all[k])), dim3(256), 0, st, all[k], part, parts, norm_in,
                        k == 0 ? norm : nullptr, max_norm);

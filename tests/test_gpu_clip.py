@@ -233,3 +233,12 @@ def test_a_tensor_past_32_bit_offsets():
     g[0], g[-1], g[n // 2] = 3.0, 4.0, 12.0
     assert float(clip_grad_norm([g], 6.5)) == 13.0
     assert [float(g[i]) for i in (0, n // 2, n - 1)] == [1.5, 6.0, 2.0] and int((g != 0).sum()) == 3
+
+
+def test_a_given_norm_within_a_gradient_is_refused():
+    from llattn_amd import clip_grads_with_norm_
+    p = torch.nn.Parameter(torch.ones(8, device=DEV))
+    p.grad = torch.ones(8, device=DEV)
+    with pytest.raises(ValueError, match="holds the norm"):
+        clip_grads_with_norm_([p], 1.0, p.grad[3])
+    assert bool((p.grad == 1).all())

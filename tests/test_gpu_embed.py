@@ -308,3 +308,46 @@ def test_offsets_past_32_bits():
     dw, = torch.autograd.grad(out, w, dy)
     last = [v for v, at in ((1.0, N - 1), (2.0, N - 2), (4.0, 3)) if int(ids[at]) == V - 1]
     assert bool((dw[V - 1] == sum(last)).all()) and bool((dw[3:V - 1] == 0).all())
+
+
+def test_no_second_derivatives():
+    w, p = (t.requires_grad_() for t in _tables(11, 6, 8, F32))
+    y = _embed(_ids((2, 6), 11), w, p)
+    dw, = torch.autograd.grad(y.square().sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dw.sum().backward()
+
+
+def test_vectorised_calls_are_refused():
+    w, _ = _tables(11, 0, 8, F32)
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda i: _embed(i, w))(_ids((2, 6), 11))
+
+
+def test_two_graphs_at_once():
+    # each has its own memory: replayed side by side on two streams they give what each gives alone
+    runs = []
+    for shape, V, P in (((4, 700), 5000, 700), ((3, 900), 300, 1000)):
+        w, p = (t.requires_grad_() for t in _tables(V, P, 136, F32))
+        ids, dy = _ids(shape, V), torch.randn(*shape, 136, device=DEV)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+
+        def call(ids=ids, w=w, p=p, dy=dy):
+            y = _embed(ids, w, p)
+            return [y.detach(), *torch.autograd.grad(y, (w, p), dy)]
+        with torch.cuda.stream(side):
+            want = [t.clone() for t in call()]
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        runs.append((graph, out, want, side, call))  # a graph reads its inputs where they are
+    for _ in range(3):
+        torch.cuda.synchronize()
+        for graph, _, _, side, _ in runs:
+            with torch.cuda.stream(side):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, out, want, _, _ in runs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))

@@ -122,6 +122,8 @@ def _clip_call(g=(AT,), out=None, numel=(10,), dtype=(0,), norm_in=None, norm=AT
 
 @pytest.mark.parametrize("kw,code", [(dict(g=(0,)), 3), (dict(g=(AT + 2,)), 3), (dict(out=(0,)), 3), (dict(out=(AT + 4002,)), 3),
                                      (dict(dtype=(2,)), 2), (dict(numel=(-1,)), 1), (dict(norm=None), 3), (dict(norm_in=AT), 3),
+                                     (dict(norm=None, norm_in=AT), 3), (dict(norm=None, norm_in=AT + 36), 3),
+                                     (dict(norm=None, norm_in=AT + 400, out=(AT + 400,)), 3),
                                      (dict(ws=None), 5), (dict(ws=AT + 4), 5), (dict(n=7), 5),
                                      (dict(g=(AT, AT), numel=(10, 10), dtype=(0, 0)), 3),
                                      (dict(g=(AT, AT + 36), numel=(10, 10), dtype=(0, 0)), 3),
@@ -158,6 +160,12 @@ def test_nothing_to_clip():
     assert float(grad_norm([])) == 0.0 and float(clip_grad_norm([], 1.0)) == 0.0
     assert float(clip_grad_norm_([torch.nn.Parameter(torch.ones(2))], 1.0)) == 0.0
     clip_grads_with_norm_([], 1.0, torch.ones(()))
+
+
+def test_a_given_norm_beside_the_gradients():
+    # right before and right behind what is written: what is refused is the output within the gradient
+    for norm in (AT + 16, AT + 60):
+        assert _clip_call(norm=None, norm_in=norm, out=(AT + 20,)) == 3 and b"output 0 overlaps" in L.load().llattn_last_error()
 
 
 @pytest.mark.parametrize("which", ["embed", "gated", "norm", "clip"])
