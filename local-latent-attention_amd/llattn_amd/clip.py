@@ -17,7 +17,7 @@ import torch
 from . import _lib as L
 
 _CODE = {torch.float32: L.F32, torch.bfloat16: L.BF16}
-_TYPES, _STRIDED = set(_CODE), {torch.strided}
+_TYPES = set(_CODE)
 
 
 def _flat(t: torch.Tensor):
@@ -30,31 +30,55 @@ def _flat(t: torch.Tensor):
     return t if t.is_contiguous() else None
 
 
+def _refuse_sparse(who: str, tensors) -> None:
+    layouts = {t.layout for t in tensors} - {torch.strided}
+    if layouts:
+        raise ValueError(f"{who}: gradients must be dense tensors, got {layouts.pop()}")
+
+
 def _check(who: str, tensors) -> list:
-    """The types of ``tensors`` (one at least), which are what the kernels take: dense, fp32 or bf16, on one GPU."""
+    """The types of ``tensors`` (one at least), which are what the kernels take: dense (those that are not have no address, which
+    :class:`_Arrays` meets), fp32 or bf16, on one GPU."""
     types = [t.dtype for t in tensors]
     if not _TYPES.issuperset(types):
         raise ValueError(f"{who}: gradients must be fp32 or bf16, got {(set(types) - _TYPES).pop()}")
-    layouts = {t.layout for t in tensors}
-    if layouts != _STRIDED:
-        raise ValueError(f"{who}: gradients must be dense tensors, got {(layouts - _STRIDED).pop()}")
     L.refuse_tangents(who, tensors)
     devices = {t.get_device() for t in tensors}
     if min(devices) < 0:
+        _refuse_sparse(who, tensors)
         L.require_gpu(*tensors)
     if len(devices) > 1:
         raise ValueError(f"{who}: gradients on {len(devices)} devices")
     return types
 
 
+def _whole_all(who: str, tensors) -> bool:
+    """Whether all are contiguous; asked of every tensor before its layout, which only those that are not can have."""
+    try:
+        whole = all([t.is_contiguous() for t in tensors])
+    except RuntimeError:
+        whole = False
+    if not whole:
+        _refuse_sparse(who, tensors)
+    return whole
+
+
+def _addresses(who: str, tensors) -> array:
+    try:
+        return array("Q", [t.data_ptr() for t in tensors])
+    except RuntimeError:
+        _refuse_sparse(who, tensors)
+        raise
+
+
 class _Arrays:
     """The host arrays of a call on contiguous tensors."""
 
-    def __init__(self, tensors, types):
+    def __init__(self, who, tensors, types):
         self.n = len(tensors)
-        self.g = array("Q", [t.data_ptr() for t in tensors])
+        self.g = _addresses(who, tensors)
         self.numel = array("q", [t.numel() for t in tensors])
-        self.dtype = array("i", [_CODE[t] for t in types])
+        self.dtype = array("i", [_CODE[types[0]]]) * self.n if types.count(types[0]) == self.n else array("i", [_CODE[t] for t in types])
 
     def workspace(self, device):
         n = L.load().llattn_grad_norm_bytes(self.n, _at(self.numel))
@@ -90,9 +114,9 @@ def grad_norm(tensors) -> torch.Tensor:
     if not tensors:
         return torch.zeros(())
     types, device = _check("grad_norm", tensors), tensors[0].device
-    if not all([t.is_contiguous() for t in tensors]):
+    if not _whole_all("grad_norm", tensors):
         tensors = [_whole(t) for t in tensors]
-    a = _Arrays(tensors, types)
+    a = _Arrays("grad_norm", tensors, types)
     ws, n = a.workspace(device)
     norm = torch.empty((), dtype=torch.float32, device=device)
     from .ops import _call
@@ -131,13 +155,14 @@ def _clip(who: str, tensors, out, max_norm: float, norm_in) -> torch.Tensor | No
     if norm_in is not None and (norm_in.numel() != 1 or norm_in.dtype is not torch.float32 or norm_in.device != device):
         raise ValueError(f"{who}: the norm must be one fp32 value on {device}, got {tuple(norm_in.shape)} {norm_in.dtype} on {norm_in.device}")
     written = tensors if out is None else out
-    if out is not None and ([t.shape for t in out] != [t.shape for t in tensors] or [t.dtype for t in out] != types or {t.get_device() for t in out} != {device.index}):
+    if out is not None and ([t.shape for t in out] != [t.shape for t in tensors] or [t.dtype for t in out] != types
+                            or {t.get_device() for t in out} != {device.index}):
         raise ValueError(f"{who}: outputs must have their gradients' shapes, types and device")
     src, dst, back = tensors, out, ()
-    if not all([t.is_contiguous() for t in tensors]) or out is not None and not all([t.is_contiguous() for t in out]):
+    if not _whole_all(who, tensors) or out is not None and not _whole_all(who, out):
         src, dst, back = _pairs(who, tensors, out)
-    a = _Arrays(src, types)
-    o = None if dst is None else array("Q", [t.data_ptr() for t in dst])
+    a = _Arrays(who, src, types)
+    o = None if dst is None else _addresses(who, dst)
     ws = norm = None
     n = 0
     if norm_in is None:
@@ -164,7 +189,7 @@ def clip_grad_norm(grads, max_norm: float, out=None) -> torch.Tensor:
         out = list(out)
         if len(out) != len(grads):
             raise ValueError(f"clip_grad_norm: {len(out)} outputs for {len(grads)} gradients")
-        if any(o.requires_grad and o.is_leaf for o in out):
+        if any([o.requires_grad for o in out]) and any(o.requires_grad and o.is_leaf for o in out):
             raise ValueError("clip_grad_norm: out holds leaves that require gradients")
     return torch.zeros(()) if not grads else _clip("clip_grad_norm", grads, out, most, None)
 

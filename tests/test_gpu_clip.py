@@ -242,3 +242,17 @@ def test_a_given_norm_within_a_gradient_is_refused():
     with pytest.raises(ValueError, match="holds the norm"):
         clip_grads_with_norm_([p], 1.0, p.grad[3])
     assert bool((p.grad == 1).all())
+
+
+@pytest.mark.parametrize("where", ["grad_norm", "gradients", "out"])
+def test_sparse_tensors_are_refused(where):
+    from llattn_amd import clip_grad_norm, grad_norm
+    g = torch.eye(4, device=DEV)
+    for t in (g.to_sparse(), g.to_sparse_csr()):
+        with pytest.raises(ValueError, match="dense"):
+            if where == "grad_norm":
+                grad_norm([g, t])
+            elif where == "gradients":
+                clip_grad_norm([t], 1.0)
+            else:
+                clip_grad_norm([g], 1.0, out=[t])
