@@ -29,7 +29,10 @@ extern "C" {
  * zero), either NULL.  Rows of no valid id (position) leave dW (dPos) alone.
  * The rows of one token are summed in fp32 in their order, in a tree that the
  * number of them alone decides: no atomics, and the same bits whatever the
- * other tokens are. */
+ * other tokens are.  It reads the order of the rows that llattn_embed_order has
+ * written for the same configuration and indices, at any time before: by token
+ * (`tokens`, where dW is wanted) and by position (`positions`, where pos is
+ * given and dPos wanted). */
 typedef struct llattn_embed_cfg {
   int64_t rows;         /* below 2^31 */
   int32_t T, V, P, D;   /* V and P at most 2^22 */
@@ -41,11 +44,15 @@ typedef struct llattn_embed_cfg {
 
 int32_t llattn_embed_fwd(const llattn_embed_cfg* cfg, const void* ids, const void* pos, const void* W, int64_t ldw,
                          const void* Pos, int64_t ldp, void* out, void* stream);
-/* Workspace bytes of llattn_embed_bwd for a configuration (1: it needs none, and takes NULL); has_pos: pos is not NULL.  0 with
- * an error message on a bad one. */
-size_t llattn_embed_bytes(const llattn_embed_cfg* cfg, int32_t has_pos);
-int32_t llattn_embed_bwd(const llattn_embed_cfg* cfg, const void* ids, const void* pos, const void* dout, void* dW,
-                         void* dPos, void* workspace, size_t workspace_bytes, void* stream);
+/* Bytes of a buffer (1: none is needed, NULL is taken), or 0 with an error message on a bad configuration: the order, the
+ * backward's workspace.  has_pos: pos is not NULL. */
+#define LLATTN_EMBED_ORDER 0
+#define LLATTN_EMBED_BACKWARD 1
+size_t llattn_embed_bytes(const llattn_embed_cfg* cfg, int32_t has_pos, int32_t which);
+int32_t llattn_embed_order(const llattn_embed_cfg* cfg, const void* ids, const void* pos, int32_t tokens, int32_t positions,
+                           void* order, size_t order_bytes, void* stream);
+int32_t llattn_embed_bwd(const llattn_embed_cfg* cfg, const void* ids, const void* pos, const void* order, const void* dout,
+                         void* dW, void* dPos, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- the norm over a list of gradients, and clipping -------------------------
  *   norm = sqrt(sum over all elements of g^2),  c = min(1, max_norm / (norm + 1e-6)),  out = c g

@@ -2,10 +2,12 @@
 //
 //   out[n] = s W[id_n] + Pos[pos_n],   dW[v] = s sum_{id_n = v} dout[n],   dPos[p] = sum_{pos_n = p} dout[n]
 //
-// The gradients are sums over the rows of one key (a token or a position), so the rows are ordered by key first: one
-// launch, a workgroup for each residue class of keys (key mod buckets), which reads all keys, keeps its own in their
-// order and counts them out by key.  The order of the keys among themselves is of no use here; the residues spread a
-// text's frequent tokens, whose numbers are close, over the workgroups.  Where positions are n % T the order is known.
+// The gradients are sums over the rows of one key (a token or a position), so the rows are ordered by key first.  That waits for no
+// gradient, so a training pass does it behind the forward, where the chip is idle until the host has come to the backward (packed
+// rows, 8192 x 1536: 143 us with it in the backward, 128; the sort is 19 us).  One launch, a workgroup for each residue class of keys
+// (key mod buckets), which reads all keys, keeps its own in their order and counts them out by key.  The order of the keys among
+// themselves is of no use here; the residues spread a text's frequent tokens, whose numbers are close, over the workgroups.  Where
+// positions are n % T the order is known.
 //
 // A run (the rows of one key, of length L) is summed in a tree of its own: blocks of 32 rows from its first row on, 32 of
 // these blocks to one of 1024 rows, then the blocks of 1024, the blocks of 32 behind them and the rows behind those in
@@ -15,7 +17,9 @@
 // (it covers position 32 c + 31), which makes c its number.
 //
 // What bounds it: memory.  Forward: a table row read and a row written per token; backward: dout read once for each
-// table, the tables' gradients written whole.
+// table, the tables' gradients written whole.  us in training passes of 32768 rows x 1408 fp32, 32000 tokens, 2048 positions: forward
+// 57 (250 MB), order 21 (latency: half of it the reading of the keys by 256 workgroups), sums of 32 rows 20, of 1024 5, the tables
+// 71 (380 MB); a copy runs at 5.0 TB/s.  Few tokens take none but the last of these launches (embed_scan_kernel).
 #include <algorithm>
 
 #include "llattn_abi.h"
@@ -35,7 +39,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_f __attribute__((aligned(4)));
 typedef u32x4 u32x4_h __attribute__((aligned(2)));
 
-// Pieces of a lane, all held at the same time (1 to 4 tried: embedding rows of 5632 bytes 40 us with 1 and 2)
+// Pieces of a lane, all held at the same time (1 and 4 were no quicker, rows of 5632 bytes)
 constexpr int kTurns = 2;
 
 // 16 bytes of a row at any alignment of whole elements; `left` elements remain in the row.  RAGGED: rows of not a whole
@@ -54,8 +58,9 @@ __device__ __forceinline__ u32x4 load_piece(const T* p, int left) {
   }
   return v;
 }
-// Non-temporal: what is written does not push out of the caches what is read (the tables' rows, dout: 32768 x 1408 forward 71 us
-// otherwise against 40, the last launch backward 137 against 83).
+// Non-temporal: what is written does not push out of the caches what is read (the tables' rows, dout: in training passes of 32768 x
+// 1408 the forward took 71 us otherwise against 57, the last launch backward 137 against 83; a norm that reads the rows right
+// behind takes as long either way, within 2%).
 template <typename T, bool RAGGED>
 __device__ __forceinline__ void store_piece(T* p, u32x4 v, int left) {
   constexpr int N = Vec16<T>::N;
@@ -673,34 +678,53 @@ Split scan_split(int D, int n) {
   s.parts = (int)ceil_div(s.pieces, 64);
   return s;
 }
+// What the scan takes grows with the keys that its waves read, (V + P) ceil(D / 256) rows.  us in a graph, lookup and gradients, by the scan
+// and by the order, at 2^20 of them 7.8 and 16.0, at 2^21.6 9.1 and 18.3, 2^23.3 11.4 and 20.0, 2^24.1 16.9 and 18.1, 2^24.6 44.5 and 45.0
 bool scans(const llattn_embed_cfg* c) {
   return c->rows <= 1024 && ((int64_t)c->V + c->P) * ceil_div(c->D, 256) * c->rows <= 1 << 24;
 }
 
-// Workspace: for a sorted set order, runs and list; for every set the sums of 32 and of 1024 rows; counted
+// What a backward reads besides dout (the order): counted; for each sorted set the rows in order, the runs and the list.  Its
+// workspace: for each table the sums of 32 and of 1024 rows.
 struct Plan {
-  int64_t rows, leaves, nodes;
+  int64_t leaves, nodes;
   int Dp;
-  int trees;
-  size_t set_bytes[2], tree_bytes;
-  size_t bytes() const { return set_bytes[0] ? 256 + set_bytes[0] + set_bytes[1] + trees * tree_bytes : 1; }
+  size_t order, trees;  // bytes; 1: none needed
 };
 Plan plan_of(const llattn_embed_cfg* c, bool has_pos) {
   Plan p{};
+  p.order = p.trees = 1;
   if (scans(c)) return p;
-  p.rows = c->rows;
   p.leaves = c->rows / kLeaf;
   p.nodes = c->rows / (kLeaf * kLeaf);
   p.Dp = (c->D + 7) / 8 * 8;
-  p.trees = c->P ? 2 : 1;
   const auto sorted = [&](int R) {
     const size_t b = buckets_of(R);
     return up((size_t)c->rows * 4) + up(b * ceil_div(R, b) * 8) + up((size_t)c->rows * 8);
   };
-  p.set_bytes[0] = sorted(c->V);
-  p.set_bytes[1] = c->P && has_pos ? sorted(c->P) : 0;
-  p.tree_bytes = up((size_t)p.leaves * p.Dp * 4) + up((size_t)p.nodes * p.Dp * 4);
+  p.order = 256 + sorted(c->V) + (c->P && has_pos ? sorted(c->P) : 0);
+  p.trees = std::max<size_t>((c->P ? 2 : 1) * (up((size_t)p.leaves * p.Dp * 4) + up((size_t)p.nodes * p.Dp * 4)), 1);
   return p;
+}
+// The sets of tokens and of positions, and where in the order they lie (it is null: nowhere)
+SortArgs sets_of(const llattn_embed_cfg* c, const void* ids, const void* pos, void* order) {
+  SortArgs s{};
+  s.rows = (int)c->rows;
+  char* at = static_cast<char*>(order);
+  const auto take = [&](size_t n) { char* x = at; at += up(n); return x; };
+  if (order) s.counted = reinterpret_cast<int32_t*>(take(256));
+  const size_t r = (size_t)c->rows;
+  const auto keyed = [&](Keys& k, const void* keys, int R, int64_t padding) {
+    k.keys = keys; k.index_bytes = c->index_bytes; k.R = R; k.padding = padding; k.buckets = buckets_of(R); k.per = (int)ceil_div(R, k.buckets);
+    if (!order) return;
+    k.order = reinterpret_cast<int32_t*>(take(4 * r));
+    k.runs = reinterpret_cast<int2*>(take(8 * (size_t)k.per * k.buckets));
+    k.list = reinterpret_cast<int2*>(take(8 * r));
+  };
+  keyed(s.set[0], ids, c->V, c->padding);
+  if (c->P && pos) keyed(s.set[1], pos, c->P, -1);
+  else if (c->P) { s.set[1].T = c->T; s.set[1].alike = (int)(c->rows / c->T); }
+  return s;
 }
 
 // The workgroups of n0 rows of one set and n1 of the other
@@ -759,13 +783,35 @@ extern "C" int32_t llattn_embed_fwd(const llattn_embed_cfg* c, const void* ids, 
   return check_launch("llattn_embed_fwd");
 }
 
-extern "C" size_t llattn_embed_bytes(const llattn_embed_cfg* c, int32_t has_pos) {
+extern "C" size_t llattn_embed_bytes(const llattn_embed_cfg* c, int32_t has_pos, int32_t which) {
   if (check("llattn_embed_bytes", c, has_pos != 0) != LLATTN_OK) return 0;
-  return plan_of(c, has_pos != 0).bytes();
+  if (which != LLATTN_EMBED_ORDER && which != LLATTN_EMBED_BACKWARD) {
+    fail(LLATTN_ERR_SHAPE, "llattn_embed_bytes: unknown buffer %d", which);
+    return 0;
+  }
+  const Plan p = plan_of(c, has_pos != 0);
+  return which == LLATTN_EMBED_ORDER ? p.order : p.trees;
 }
 
-extern "C" int32_t llattn_embed_bwd(const llattn_embed_cfg* c, const void* ids, const void* pos, const void* dout, void* dW,
-                                    void* dPos, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int32_t llattn_embed_order(const llattn_embed_cfg* c, const void* ids, const void* pos, int32_t tokens, int32_t positions,
+                                      void* order, size_t order_bytes, void* stream) {
+  if (const int32_t rc = check("llattn_embed_order", c, pos != nullptr)) return rc;
+  if ((c->rows && tokens && !ids) || (positions && c->P && !pos)) return fail(LLATTN_ERR_LAYOUT, "llattn_embed_order: null ids or positions");
+  if (!whole(ids, c->index_bytes) || !whole(pos, c->index_bytes))
+    return fail(LLATTN_ERR_LAYOUT, "llattn_embed_order: a tensor is not aligned to its elements");
+  const Plan p = plan_of(c, pos != nullptr);
+  if (p.order == 1) return LLATTN_OK;
+  if (!order || order_bytes < p.order || !aligned16(order))
+    return fail(LLATTN_ERR_WORKSPACE, "llattn_embed_order: needs %zu bytes (got %zu)", p.order, order_bytes);
+  SortArgs s = sets_of(c, ids, pos, order);
+  s.first[1] = tokens ? s.set[0].buckets : 0;
+  s.first[2] = s.first[1] + (positions && c->P ? s.set[1].buckets : 0);
+  if (s.first[2]) hipLaunchKernelGGL(embed_sort_kernel, dim3(s.first[2]), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream), s);
+  return check_launch("llattn_embed_order");
+}
+
+extern "C" int32_t llattn_embed_bwd(const llattn_embed_cfg* c, const void* ids, const void* pos, const void* order, const void* dout,
+                                    void* dW, void* dPos, void* workspace, size_t workspace_bytes, void* stream) {
   if (const int32_t rc = check("llattn_embed_bwd", c, pos != nullptr)) return rc;
   if (dPos && !c->P) return fail(LLATTN_ERR_SHAPE, "llattn_embed_bwd: a gradient of no position rows");
   if (!dW && !dPos) return LLATTN_OK;
@@ -774,47 +820,34 @@ extern "C" int32_t llattn_embed_bwd(const llattn_embed_cfg* c, const void* ids, 
   if (!whole(ids, c->index_bytes) || !whole(pos, c->index_bytes) || !whole(dout, size) || !whole(dW, size) || !whole(dPos, size))
     return fail(LLATTN_ERR_LAYOUT, "llattn_embed_bwd: a tensor is not aligned to its elements");
   const Plan p = plan_of(c, pos != nullptr);
-  if (p.bytes() > 1 && (!workspace || workspace_bytes < p.bytes() || !aligned16(workspace)))
-    return fail(LLATTN_ERR_WORKSPACE, "llattn_embed_bwd: needs %zu workspace bytes (got %zu)", p.bytes(), workspace_bytes);
+  if (p.order > 1 && (dW || pos) && (!order || !aligned16(order)))
+    return fail(LLATTN_ERR_LAYOUT, "llattn_embed_bwd: null order, or one not 16-byte aligned");
+  if (p.trees > 1 && (!workspace || workspace_bytes < p.trees || !aligned16(workspace)))
+    return fail(LLATTN_ERR_WORKSPACE, "llattn_embed_bwd: needs %zu workspace bytes (got %zu)", p.trees, workspace_bytes);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t table[2] = {dW ? c->V : 0, dPos ? c->P : 0};
-  const bool f32 = c->dtype == LLATTN_F32, ragged = c->D % (16 / size) != 0, scan = scans(c);
-  char* at = static_cast<char*>(workspace);
-  const auto take = [&](size_t n) { char* x = at; at += up(n); return x; };
-  const size_t r = (size_t)c->rows;
-  SortArgs s{};
-  s.rows = (int)c->rows;
-  if (!scan) s.counted = reinterpret_cast<int32_t*>(take(256));
-  const auto keyed = [&](Keys& k, const void* keys, int R, int64_t padding) {
-    k.keys = keys; k.index_bytes = c->index_bytes; k.R = R; k.padding = padding; k.buckets = buckets_of(R); k.per = (int)ceil_div(R, k.buckets);
-    if (scan) return;
-    k.order = reinterpret_cast<int32_t*>(take(4 * r));
-    k.runs = reinterpret_cast<int2*>(take(8 * (size_t)k.per * k.buckets));
-    k.list = reinterpret_cast<int2*>(take(8 * r));
-  };
-  keyed(s.set[0], ids, c->V, c->padding);
-  if (c->P && pos) keyed(s.set[1], pos, c->P, -1);
-  else if (c->P) { s.set[1].T = c->T; s.set[1].alike = (int)(c->rows / c->T); }
+  const bool f32 = c->dtype == LLATTN_F32, ragged = c->D % (16 / size) != 0;
+  const SortArgs s = sets_of(c, ids, pos, p.order > 1 ? const_cast<void*>(order) : nullptr);
   BwdArgs a{};
   a.set[0] = s.set[0]; a.set[1] = s.set[1];
   a.rows = s.rows; a.D = c->D; a.Dp = p.Dp; a.dout = dout;
   a.counted = s.counted;
   a.out[0] = dW; a.out[1] = dPos;
   a.scale[0] = c->scale; a.scale[1] = 1.f;
-  if (scan) {
+  if (p.order == 1) {
     if (f32 && ragged) launch_scan<float, true>(a, table, st);
     else if (f32) launch_scan<float, false>(a, table, st);
     else if (ragged) launch_scan<uint16_t, true>(a, table, st);
     else launch_scan<uint16_t, false>(a, table, st);
     return check_launch("llattn_embed_bwd");
   }
-  for (int k = 0; k < p.trees; ++k) {
-    a.leaf[k] = reinterpret_cast<float*>(take((size_t)p.leaves * p.Dp * 4));
-    a.node[k] = reinterpret_cast<float*>(take((size_t)p.nodes * p.Dp * 4));
+  char* at = static_cast<char*>(workspace);
+  for (int k = 0; k < (c->P ? 2 : 1); ++k) {
+    a.leaf[k] = reinterpret_cast<float*>(at);
+    at += up((size_t)p.leaves * p.Dp * 4);
+    a.node[k] = reinterpret_cast<float*>(at);
+    at += up((size_t)p.nodes * p.Dp * 4);
   }
-  s.first[1] = dW ? s.set[0].buckets : 0;
-  s.first[2] = s.first[1] + (dPos && pos ? s.set[1].buckets : 0);
-  if (s.first[2]) hipLaunchKernelGGL(embed_sort_kernel, dim3(s.first[2]), dim3(64 * kWaves), 0, st, s);
   if (f32 && ragged) launch_bwd<float, true>(a, p, table, st);
   else if (f32) launch_bwd<float, false>(a, p, table, st);
   else if (ragged) launch_bwd<uint16_t, true>(a, p, table, st);

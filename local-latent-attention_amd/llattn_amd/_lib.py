@@ -84,6 +84,7 @@ class LlattnHeadCfg(ctypes.Structure):  # include/llattn_train.h
     _fields_ = [(n, ctypes.c_int32) for n in ("rows", "V", "D", "piece", "dw_dtype")]
 
 
+EMBED_ORDER, EMBED_BACKWARD = 0, 1  # LLATTN_EMBED_*
 GATED_FORWARD, GATED_ALONE, GATED_BACKWARD, GATED_KEPT = range(4)  # LLATTN_GATED_*
 MUON_BATCH, MUON_GROUPS = 128, 16  # LLATTN_MUON_BATCH, LLATTN_MUON_GROUPS
 
@@ -184,8 +185,9 @@ TRAIN_SIGNATURES = {
 _EC, _GC, _GW, _GG = (ctypes.POINTER(t) for t in (LlattnEmbedCfg, LlattnGatedCfg, LlattnGatedWeights, LlattnGatedGrads))
 LM_SIGNATURES = {
     "llattn_embed_fwd": (_I32, [_EC, _P, _P, _P, _I64, _P, _I64, _P, _P]),
-    "llattn_embed_bytes": (_SZ, [_EC, _I32]),
-    "llattn_embed_bwd": (_I32, [_EC, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "llattn_embed_bytes": (_SZ, [_EC, _I32, _I32]),
+    "llattn_embed_order": (_I32, [_EC, _P, _P, _I32, _I32, _P, _SZ, _P]),
+    "llattn_embed_bwd": (_I32, [_EC, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "llattn_grad_norm_bytes": (_SZ, [_I32, _P]),
     "llattn_grad_norm": (_I32, [_I32, _P, _P, _P, _P, _P, _SZ, _P]),
     "llattn_clip_grads": (_I32, [_I32, _P, _P, _P, _P, ctypes.c_double, _P, _P, _P, _SZ, _P]),

@@ -54,20 +54,36 @@ def _forward(ids, weight, position, positions, scale, padding):
     return out, i, p, cfg
 
 
+def _buffer(ref, has_pos, which, device):
+    """(a buffer of the call's, its bytes), or (None, 1) where it needs none."""
+    n = L.load().llattn_embed_bytes(ref, has_pos, which)
+    if n == 0:
+        L.check(L.ERR_SHAPE, "llattn_embed_bytes")
+    return torch.empty((n,), dtype=torch.uint8, device=device) if n > 1 else None, n
+
+
+def _order(i, p, cfg, tokens, positions):
+    """The order of the rows that a backward reads, None where it needs none."""
+    ref, dev = ctypes.byref(cfg), i.device
+    order, n = _buffer(ref, int(p is not None), L.EMBED_ORDER, dev)
+    if order is not None:
+        with L.on_device(dev):
+            ops._call("llattn_embed_order", ref, i.data_ptr(), _ptr(p), int(tokens), int(positions), order.data_ptr(), n,
+                      L.stream_ptr(dev), work=cfg.rows * cfg.index_bytes)
+    return order
+
+
 def _backward(ctx, dout):
-    i, p = ctx.saved_tensors
+    i, p, order = ctx.saved_tensors
     cfg, w_shape, p_shape = ctx.meta
     _, want_w, want_p, *_ = ctx.needs_input_grad
     dw = dout.new_empty(w_shape) if want_w else None
     dp = dout.new_empty(p_shape) if want_p else None
     d = dout if dout.is_contiguous() else dout.contiguous()
     dev, ref = d.device, ctypes.byref(cfg)
-    n = L.load().llattn_embed_bytes(ref, int(p is not None))
-    if n == 0:
-        L.check(L.ERR_SHAPE, "llattn_embed_bytes")
-    ws = torch.empty((n,), dtype=torch.uint8, device=dev) if n > 1 else None
+    ws, n = _buffer(ref, int(p is not None), L.EMBED_BACKWARD, dev)
     with L.on_device(dev):
-        ops._call("llattn_embed_bwd", ref, i.data_ptr(), _ptr(p), d.data_ptr(), _ptr(dw), _ptr(dp), _ptr(ws), n,
+        ops._call("llattn_embed_bwd", ref, i.data_ptr(), _ptr(p), _ptr(order), d.data_ptr(), _ptr(dw), _ptr(dp), _ptr(ws), n,
                   L.stream_ptr(dev), work=(cfg.rows + cfg.V + cfg.P) * cfg.D * d.element_size())
     return None, dw, dp, None, None, None
 
@@ -79,7 +95,10 @@ class _Embed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, position, positions, scale, padding):
         out, i, p, cfg = _forward(ids, weight, position, positions, scale, padding)
-        ctx.save_for_backward(i, p)
+        _, tokens, places, *_ = ctx.needs_input_grad
+        places = places and p is not None
+        # here and not in the backward: nothing of it waits for a gradient
+        ctx.save_for_backward(i, p, _order(i, p, cfg, tokens, places) if tokens or places else None)
         ctx.meta = (cfg, weight.shape, None if position is None else position.shape)
         return out
 

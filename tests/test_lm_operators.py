@@ -50,16 +50,21 @@ def _cfg(rows=6, T=3, V=10, P=4, D=8, dtype=0, index_bytes=8, padding=-1, scale=
                                 dict(D=0), dict(D=(1 << 20) + 1), dict(T=0), dict(T=5), dict(rows=7), dict(dtype=2),
                                 dict(index_bytes=2), dict(padding=10), dict(padding=-2)], ids=str)
 def test_embed_sizes_refused(kw):
-    assert L.load().llattn_embed_bytes(ctypes.byref(_cfg(**kw)), 0) == 0 and L.load().llattn_last_error()
+    for which in (L.EMBED_ORDER, L.EMBED_BACKWARD):
+        assert L.load().llattn_embed_bytes(ctypes.byref(_cfg(**kw)), 0, which) == 0 and L.load().llattn_last_error()
 
 
 def test_embed_sizes_taken():
-    n = L.load().llattn_embed_bytes
-    assert n(ctypes.byref(_cfg()), 0) == 1 and n(ctypes.byref(_cfg(rows=0)), 0) == 1  # none for few tokens
-    assert n(ctypes.byref(_cfg(T=9, rows=7)), 1) == 1 and n(ctypes.byref(_cfg(T=0, P=0)), 0) == 1
-    assert n(ctypes.byref(_cfg(rows=1026)), 0) > 1026 * 12
-    # sums of 32 rows, two tables; rows in order twice
-    assert n(ctypes.byref(_cfg(rows=32768, T=2048, V=32000, P=2048, D=1408)), 0) < 2 * 32768 * 1408 * 4 // 31 + 32768 * 12 + 32000 * 8 + 4096
+    def n(cfg, has_pos):
+        return tuple(L.load().llattn_embed_bytes(ctypes.byref(cfg), has_pos, k) for k in (L.EMBED_ORDER, L.EMBED_BACKWARD))
+    assert n(_cfg(), 0) == n(_cfg(rows=0), 0) == (1, 1)  # none for few tokens
+    assert n(_cfg(T=9, rows=7), 1) == n(_cfg(T=0, P=0), 0) == (1, 1)
+    order, trees = n(_cfg(rows=32768, T=2048, V=32000, P=2048, D=1408), 0)
+    assert 32768 * 12 + 32000 * 8 <= order < 32768 * 12 + 32000 * 8 + 4096
+    assert n(_cfg(rows=32768, T=2048, V=32000, P=2048, D=1408), 1)[0] > order + 32768 * 12
+    assert 2 * 32768 // 32 * 1408 * 4 <= trees < 2 * 32768 * 1408 * 4 // 31 + 4096  # sums of 32 rows and of 1024, two tables
+    assert n(_cfg(rows=21, V=1 << 22), 0)[1] == 1  # too few for sums of 32
+    assert L.load().llattn_embed_bytes(ctypes.byref(_cfg()), 0, 2) == 0
 
 
 @pytest.mark.parametrize("kw,code", [(dict(ids=None), 3), (dict(W=None), 3), (dict(out=None), 3), (dict(Pos=None), 3), (dict(ids=AT + 4), 3),
@@ -69,14 +74,26 @@ def test_embed_forward_refused(kw, code):
     assert L.load().llattn_embed_fwd(ctypes.byref(_cfg()), *a.values(), None) == code
 
 
-@pytest.mark.parametrize("kw,code", [(dict(ids=None), 3), (dict(dout=None), 3), (dict(dW=AT + 2), 3), (dict(ws=None), 5), (dict(ws=AT + 8), 5),
-                                     (dict(n=100), 5)], ids=str)
+@pytest.mark.parametrize("kw,code", [(dict(ids=None), 3), (dict(ids=AT + 4), 3), (dict(positions=1), 3), (dict(pos=AT + 4), 3),
+                                     (dict(order=None), 5), (dict(order=AT + 8), 5), (dict(n=100), 5)], ids=str)
+def test_embed_order_refused(kw, code):
+    a = dict(ids=AT, pos=None, tokens=1, positions=0, order=AT, n=1 << 20) | kw
+    assert L.load().llattn_embed_order(ctypes.byref(_cfg(rows=1200)), *a.values(), None) == code
+
+
+def test_no_order_of_few_tokens():
+    assert L.load().llattn_embed_order(ctypes.byref(_cfg()), AT, None, 1, 0, None, 0, None) == 0
+
+
+@pytest.mark.parametrize("kw,code", [(dict(ids=None), 3), (dict(dout=None), 3), (dict(dW=AT + 2), 3), (dict(order=None), 3),
+                                     (dict(order=AT + 8), 3), (dict(dW=None, pos=AT, order=None), 3), (dict(ws=None), 5),
+                                     (dict(ws=AT + 8), 5), (dict(n=100), 5), (dict(dW=None, order=None, ws=None), 5)], ids=str)
 def test_embed_backward_refused(kw, code):
     lib = L.load()
-    cfg = _cfg(rows=1200)  # (few tokens take no workspace)
-    a = dict(ids=AT, pos=None, dout=AT, dW=AT, dPos=AT, ws=AT, n=lib.llattn_embed_bytes(ctypes.byref(cfg), 0)) | kw
+    cfg = _cfg(rows=1200)  # (few tokens take no order and no workspace)
+    a = dict(ids=AT, pos=None, order=AT, dout=AT, dW=AT, dPos=AT, ws=AT, n=1 << 20) | kw
     assert lib.llattn_embed_bwd(ctypes.byref(cfg), *a.values(), None) == code
-    assert lib.llattn_embed_bwd(ctypes.byref(_cfg(rows=1200, P=0)), *(a | dict(n=1 << 20)).values(), None) in (1, code)
+    assert lib.llattn_embed_bwd(ctypes.byref(_cfg(rows=1200, P=0)), *a.values(), None) == 1
 
 
 def test_embed_refusals():
