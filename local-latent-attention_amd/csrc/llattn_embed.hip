@@ -19,7 +19,7 @@
 // What bounds it: memory.  Forward: a table row read and a row written per token; backward: dout read once for each
 // table, the tables' gradients written whole.  us in training passes of 32768 rows x 1408 fp32, 32000 tokens, 2048 positions: forward
 // 57 (250 MB), order 21 (latency: half of it the reading of the keys by 256 workgroups), sums of 32 rows 20, of 1024 5, the tables
-// 71 (380 MB); a copy runs at 5.0 TB/s.  Few tokens take none but the last of these launches (embed_scan_kernel).
+// 68 (380 MB); a copy runs at 5.0 TB/s.  Few tokens take none but the last of these launches (embed_scan_kernel).
 #include <algorithm>
 
 #include "llattn_abi.h"
@@ -402,7 +402,7 @@ __device__ __forceinline__ void add_rows(Sum<T>& sum, int n, const Task& k, int 
 // sum += the rows of fp32 sums that start at get(i), i < n, in order
 template <typename T, typename F>
 __device__ __forceinline__ void add_sums(Sum<T>& sum, int n, const Task& k, F&& get) {
-  constexpr int N = Vec16<T>::N, U = 4;
+  constexpr int N = Vec16<T>::N, U = 2;
   for (int i = 0; i < n; i += U) {
     float4 v[U][kTurns][N / 4];
 #pragma unroll
@@ -516,9 +516,13 @@ __device__ __forceinline__ void store_row(const BwdArgs& a, int set, const Task&
   }
 }
 
-// Rows of the tables' gradients, of a whole run each: the blocks of 1024, those of 32 behind them, the rows behind those
+// Rows of the tables' gradients, of a whole run each: the blocks of 1024, those of 32 behind them, the rows behind those.  Most runs are
+// empty or short, so what counts is the number of waves at work and not what each has in flight: with 8 (bf16: 6) on a SIMD
+// instead of 6 (4), two sums and two rows (bf16: four) ahead instead of four, 52305 rows x 1536 bf16 take 43 us for 49, 34048 x 1408
+// fp32 68 for 71.
+template <typename T> constexpr bool kWide = std::is_same_v<T, float>;
 template <typename T, bool RAGGED>
-__global__ __launch_bounds__(256) void embed_bwd_kernel(const BwdArgs a) {
+__global__ __launch_bounds__(256, kWide<T> ? 8 : 6) void embed_bwd_kernel(const BwdArgs a) {
   int set;
   const Task k = task_in(a, a.split, set);
   if (k.row < 0 || block_of() >= a.total) return;
@@ -538,7 +542,7 @@ __global__ __launch_bounds__(256) void embed_bwd_kernel(const BwdArgs a) {
   if (rest) {
     Sum<T> x;
     x.zero();
-    add_rows<T, RAGGED, 4>(x, rest, k, a.D,
+    add_rows<T, RAGGED, kWide<T> ? 2 : 4>(x, rest, k, a.D,
                            [&](int i) { return static_cast<const T*>(a.dout) + (int64_t)row_at(s, run, k.row, L - rest + i) * a.D; });
     sum.add(x);
   }
