@@ -79,16 +79,16 @@ int32_t llattn_clip_grads(int32_t n, const void* const* g, void* const* out, con
  *   a = x W1^T + b1,  u = x W3^T + b3,  h = act(a) u,  y = h W2^T + b2
  * with x [rows][D], W1 and W3 [F][D], W2 [D_out][F], y [rows][D_out], all bf16,
  * biases fp32 or NULL; products summed in fp32, a and u not rounded, h rounded
- * to bf16 (what the last product reads; forward alone over at most 24 rows it
- * keeps 16 bits, as the sum of two bf16 values: infinite weights of W2, which
- * must be finite otherwise, give NaN there).  act: LLATTN_GATE_SILU a / (1 + exp(-a)) or LLATTN_GATE_GELU
+ * to bf16, which the last product reads; up to 64 rows it is the sum of two bf16
+ * values (16 bits), and so are da and du below: infinities of W2 and dy can give
+ * NaN there.  act: LLATTN_GATE_SILU a / (1 + exp(-a)) or LLATTN_GATE_GELU
  * a Phi(a).  D, F and D_out are multiples of 8, weights and y contiguous, x of
  * row stride ldx (a multiple of 8, below 2^23); everything 16-byte aligned.
  *
  * Forward: y; with `kept` not NULL (llattn_gated_bytes(cfg, LLATTN_GATED_KEPT)
  * bytes of the caller's) also what the backward reads.  Backward of it, given dy
  * [rows][D_out] contiguous, with p = act(a) and s = act'(a) u:
- *   dh = dy W2,  da = dh s,  du = dh p  (da and du rounded to bf16),
+ *   dh = dy W2,  da = dh s,  du = dh p  (da and du rounded as h is),
  *   dx = da W1 + du W3,  dW1 = da^T x,  dW3 = du^T x,  dW2 = dy^T h,
  *   db1, db3, db2: sums of da, du, dy over the rows (fp32)
  * (any of them NULL; dW1 and dW3 together), dx bf16, dW1 and dW3 of dw_dtype, dW2

@@ -10,12 +10,12 @@
 //
 // Rounded to bf16 besides the results: h, da and du, which the matrix cores take in 16 bits.  They are off by half a step
 // of each value at most, independently, so results are about sqrt 2 times as far from the exact ones as their own rounding
-// leaves them.  p and s are kept in 24 bits (16 of the significand: their rounding in bf16 would make that sqrt 3, at 8192 x 1536
-// x 4096 for 2% of the time), the upper two bytes and the third in planes of their own.
+// leaves them.  Up to 64 rows, where single results stray further and there is room in the tiles, they are held as the sums of two bf16
+// values.  p and s are kept in 24 bits (16 of the significand: their rounding in bf16 would make that sqrt 3, at 8192 x 1536 x 4096
+// for 2% of the time), the upper two bytes and the third in planes of their own.
 //
 // Backward, two products share a launch where both take 128 x 128 tiles (the gate's gradients with dW2, dx with dW1 and dW3): small
-// ones fill the chip together.  Forward alone with few rows, two kernels of their own read every weight once, along k, and
-// h stays in fp32 between them.
+// ones fill the chip together.  Forward alone with few rows, two kernels of their own read every weight once, along k.
 //
 // What bounds it: the matrix cores (2 rows D F operations for each of the three products, twice that backward); with few
 // rows the reads of the weights.
@@ -39,9 +39,11 @@ struct GatedArgs {
   int M, N, K;                  // GATE: N columns of h
   int steps, per;               // 64-wide k steps, of a split
   int tiles_m, tiles_n, total;  // total: with the splits
-  const uint16_t* A; int64_t lda;
+  const uint16_t *A, *A2; int64_t lda;  // A2: the matrix from step `half` on, where A lies along k and there are two
   const uint16_t *B, *B2; int64_t ldb;  // B2: the other matrix of a gate, or the one from step `half` on
   int half, k_half;             // two matrices along k: steps and k of the first, k of either
+  int low;                      // few rows: the lower halves of h (GATE), da and du (DGATE) lie that many rows on; or 0
+  int fold;                     // OUT in parts: rows [fold, 2 fold) of the product are added to the first; or 0
   const float *bias, *bias2;
   uint16_t* h;                  // GATE: [M][N]
   int act;
@@ -173,7 +175,7 @@ template <int W, int NB> struct Cols<192, W, NB> { typedef ColsOp<256, 192, W, N
 // next: k 0..31 (reads k 32..63), a barrier, k 32..63 (reads the next step's k 0..31 and issues the loads of step
 // kt + NST into the stage just read).  Waves whose part of the tile lies outside load and wait like the others and do
 // nothing else.  The gate's workgroups take tile after tile, the next one's first steps loaded in the last ones of this.
-// AT: A stored with its rows along k.  BT: B likewise.  TWO: a second matrix B from step `half` on.
+// AT: A stored with its rows along k.  BT: B likewise.  TWO: a second matrix B from step `half` on, and with AT a second A.
 // What a product is made of: EPI, AT, BT and TWO as above
 template <int EPI_, bool AT_, bool BT_, bool TWO_>
 struct Product {
@@ -185,6 +187,7 @@ typedef Product<OUT, false, false, false> OutProduct;   // y
 typedef Product<DGATE, false, true, false> DGateProduct;
 typedef Product<OUT, false, true, true> DxProduct;
 typedef Product<OUT, true, true, false> DwProduct;
+typedef Product<OUT, true, true, true> DwHalvesProduct;  // of few rows
 
 template <typename P, typename S>
 struct Operands {
@@ -238,7 +241,11 @@ __device__ __forceinline__ void gated_tiles(const GatedArgs& a, unsigned char* s
     s.inc = t ? (uint32_t)(128 * ld) : 128u;
     return s;
   };
-  auto source_a = [&](const Tile& t) { return source(a.A, a.lda, AT, t.m0, min(TM, a.M - t.m0), t.split * a.per, a.K); };
+  auto source_a = [&](const Tile& t, int k) {
+    const int n = min(TM, a.M - t.m0);
+    if constexpr (TWO && AT) return k < a.half ? source(a.A, a.lda, AT, t.m0, n, k, a.k_half) : source(a.A2, a.lda, AT, t.m0, n, k - a.half, a.k_half);
+    return source(a.A, a.lda, AT, t.m0, n, k, a.K);
+  };
   auto source_b = [&](const Tile& t, int k) {  // from step k on
     const int n = min(TC, a.N - t.n0);
     if constexpr (TWO) return k < a.half ? source(a.B, a.ldb, BT, t.n0, n, k, a.k_half) : source(a.B2, a.ldb, BT, t.n0, n, k - a.half, a.k_half);
@@ -246,21 +253,25 @@ __device__ __forceinline__ void gated_tiles(const GatedArgs& a, unsigned char* s
   };
   auto k_of = [&](const Tile& t) { return min(a.K - t.split * a.per * 64, t.steps * 64); };
   Tile tile = tile_at(v);
-  StepSrc sa = source_a(tile), sb = source_b(tile, tile.split * a.per);
+  StepSrc sa = source_a(tile, tile.split * a.per), sb = source_b(tile, tile.split * a.per);
   int ahead = k_of(tile);  // k from the step that ra and rb describe to the end of its tile's
   int kb = tile.split * a.per;  // that step, among all
   const auto left_b = [&]() { return TWO ? min(ahead, a.k_half - 64 * (kb < a.half ? kb : kb - a.half)) : ahead; };
   int bleft = left_b();
-  i32x4 ra = sa.rsrc(ahead, 64), rb = sb.rsrc(bleft, 64);
+  const auto left_a = [&]() { return TWO && AT ? bleft : ahead; };
+  i32x4 ra = sa.rsrc(left_a(), 64), rb = sb.rsrc(bleft, 64);
   auto advance = [&]() {
     sa.addr += sa.inc;
     sb.addr += sb.inc;
     ahead -= 64;
     if constexpr (TWO) {
-      if (++kb == a.half) sb = source_b(tile, kb);
+      if (++kb == a.half) {
+        sb = source_b(tile, kb);
+        if constexpr (AT) sa = source_a(tile, kb);
+      }
     }
     bleft = left_b();
-    ra = sa.rsrc(ahead, 64);
+    ra = sa.rsrc(left_a(), 64);
     rb = sb.rsrc(bleft, 64);
   };
   const uint32_t lds_a = __builtin_amdgcn_readfirstlane(lds_addr(smem) + w * OpA::LOADS * 1024);
@@ -303,7 +314,7 @@ __device__ __forceinline__ void gated_tiles(const GatedArgs& a, unsigned char* s
     // A tile before another takes whole turns of the stages.
     const bool more = PERSIST && v + stride < a.total;
     const Tile next = more ? tile_at(v + stride) : tile;
-    const StepSrc next_a = source_a(next), next_b = source_b(next, next.split * a.per);
+    const StepSrc next_a = source_a(next, next.split * a.per), next_b = source_b(next, next.split * a.per);
     const int next_k = more ? k_of(next) : 0;
     const int steps = more ? (max(tile.steps, 1) + NST - 1) / NST * NST : tile.steps;
     const int row0 = tile.m0 + wm * 16 * MB, col0 = tile.n0 + wn * WCOLS;
@@ -383,6 +394,17 @@ __device__ __forceinline__ void gated_tiles(const GatedArgs& a, unsigned char* s
     const auto bf16s = [](const f32x4& x, const f32x4& y) {
       return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
     };
+    // what bf16s leaves of finite values
+    const auto rests = [&](const f32x4& x, const f32x4& y, uint4 h) {
+      const uint32_t v[4] = {h.x, h.y, h.z, h.w};
+      f32x4 q[2] = {x, y};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = q[e >> 2][e & 3] - __uint_as_float(e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16);
+        q[e >> 2][e & 3] = fabsf(d) < __builtin_inff() ? d : 0.f;
+      }
+      return bf16s(q[0], q[1]);
+    };
     const auto add_bias = [&](f32x4& x, f32x4& y, const float* bias, int c) {
       const float4 u = *reinterpret_cast<const float4*>(bias + c), t = *reinterpret_cast<const float4*>(bias + c + 4);
       x += f32x4{u.x, u.y, u.z, u.w};
@@ -410,7 +432,9 @@ __device__ __forceinline__ void gated_tiles(const GatedArgs& a, unsigned char* s
             y[e] = df;
           }
           const int64_t o = (int64_t)row * a.N + c;
-          st16(a.h + o, bf16s(fx * u, fy * t));
+          const uint4 h = bf16s(fx * u, fy * t);
+          st16(a.h + o, h);
+          if (a.low) st16(a.h + o + (int64_t)a.low * a.N, rests(fx * u, fy * t, h));
           if (a.p) {
             const int64_t plane = 2 * Float24::elements(a.M, a.N), at = Float24::place(row, c, a.N);
             Float24::store(a.p, plane, at, fx, fy);
@@ -446,13 +470,17 @@ __device__ __forceinline__ void gated_tiles(const GatedArgs& a, unsigned char* s
           f32x4 x = acc[i][j], y = acc[i][j + 1], m, n;
           swap(x, y);
           const int c = pair(j);
-          if (row >= a.M || 2 * c >= a.ldd) continue;
+          if (row >= (a.low ? a.low : a.M) || 2 * c >= a.ldd) continue;  // few rows: zeros behind the last, for the bias gradients' sums
           if (c >= a.N) x = y = f32x4{0.f, 0.f, 0.f, 0.f};  // the next product contracts over these columns too
           uint16_t* o = a.d + (int64_t)row * a.ldd + c;
-          s[i & 1][j / 2].get(m, n);
-          st16(o, bf16s(x * m, y * n));
-          p[i & 1][j / 2].get(m, n);
-          st16(o + a.ldd / 2, bf16s(x * m, y * n));
+          const auto put = [&](uint16_t* o, const Float24& f) {
+            f.get(m, n);
+            const uint4 v = bf16s(x * m, y * n);
+            st16(o, v);
+            if (a.low) st16(o + a.low * a.ldd, rests(x * m, y * n, v));
+          };
+          put(o, s[i & 1][j / 2]);
+          put(o + a.ldd / 2, p[i & 1][j / 2]);
         }
       });
     } else if (a.part) {
@@ -527,7 +555,7 @@ __global__ __launch_bounds__(256) void gated_reduce_kernel(const ReduceArgs q) {
   const int k = ((int)blockIdx.x >= q.first[1]) + ((int)blockIdx.x >= q.first[2]);
   const GatedArgs& a = q.a[k];
   const int64_t n = (int64_t)a.M * a.N, i = ((int64_t)(blockIdx.x - q.first[k]) * 256 + threadIdx.x) * 4;
-  if (i >= n) return;
+  if (i >= (a.fold ? (int64_t)a.fold * a.N : n)) return;
   const int row = (int)(i / a.N), col = (int)(i - (int64_t)row * a.N), f = row < a.m_half ? row : row - a.m_half;
   if (f >= a.m_live) return;
   float x[4] = {0.f, 0.f, 0.f, 0.f};
@@ -543,6 +571,12 @@ __global__ __launch_bounds__(256) void gated_reduce_kernel(const ReduceArgs q) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] += y[u][e];
       }
+  }
+  for (int s = 0; a.fold && s < q.splits[k]; ++s) {
+    float y[4];
+    load4<float>(a.part + s * n + (int64_t)a.fold * a.N + i, y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += y[e];
   }
   if (a.bias) {
 #pragma unroll
@@ -713,6 +747,10 @@ void launch(GatedArgs& a, const Tiling& t, hipStream_t st) {
   else if (t.kind == SQUARE) hipLaunchKernelGGL((gated_kernel<P, SquareShape, 2>), grid, dim3(SquareShape::THREADS), 0, st, a);
   else if constexpr (P::EPI == OUT) hipLaunchKernelGGL((gated_kernel<P, WideShape, 1>), grid, dim3(WideShape::THREADS), 0, st, a);
 }
+template <typename P>
+void launch_square(GatedArgs& a, const Tiling& t, hipStream_t st) {
+  hipLaunchKernelGGL((gated_kernel<P, SquareShape, 2>), dim3((unsigned)prepare<P>(a, t)), dim3(SquareShape::THREADS), 0, st, a);
+}
 template <typename P0, typename P1>
 void launch_pair(GatedArgs& a, const Tiling& ta, GatedArgs& b, const Tiling& tb, hipStream_t st) {
   const int na = prepare<P0>(a, ta), nb = prepare<P1>(b, tb), lead = a.per >= b.per, first = ((lead ? na : nb) + 7) / 8 * 8;
@@ -728,7 +766,7 @@ void launch_reduce(const GatedArgs* const* a, const Tiling* const* t, int n, hip
     if (!a[i]->part) continue;
     q.a[k] = *a[i];
     q.splits[k] = t[i]->splits;
-    blocks += ceil_div((int64_t)a[i]->M * a[i]->N, 1024);
+    blocks += ceil_div((int64_t)(a[i]->fold ? a[i]->fold : a[i]->M) * a[i]->N, 1024);
     q.first[++k] = (int)blocks;
   }
   if (!k) return;
@@ -740,7 +778,12 @@ constexpr int kSplits = 16;
 // Rows of a forward alone that the kernels for few of them take.  us in a graph, these and the tiles, D 1408, F 4096: 1 row 11.7 and 23.6,
 // 16 rows 17.8 and 24.7, 24 rows 24.1 and 25.4, 32 rows 27.1 and 25.8 (F 256: 6.4 and 8.8)
 constexpr int kThinRows = 24;
+// Rows up to which h, da and du are held as two bf16 values (16 bits of significand), the lower ones kLow rows behind the upper: as more
+// rows of the products with the weights, whose 128 x 128 tiles have room for them, and as a second step of those over the rows.  With
+// few values their rounding shows: rms errors of single results then lie up to 1.55 times as far out as their own rounding puts them.
+constexpr int kLow = 64;
 struct Plan {
+  int low, rows;            // kLow or 0; rows of h and d
   int half;                 // columns of da (and of du): F rounded up to 64
   Tiling gate, out, dgate, dx, dw, dw2;
   size_t h, d, part[4];     // h; da and du; parts of out, dx, dw, dw2
@@ -750,25 +793,28 @@ struct Plan {
 Plan plan_of(const llattn_gated_cfg* c) {
   Plan p{};
   const auto steps = [](int k) { return (k + 63) / 64; };
-  const auto part = [](const Tiling& t, int64_t m, int64_t n) { return t.splits > 1 ? up((size_t)t.splits * m * n * 4) : 0; };
+  const auto part = [](const Tiling& t, int64_t m, int64_t n, bool folded) { return t.splits > 1 || folded ? up((size_t)t.splits * m * n * 4) : 0; };
+  p.low = c->rows <= kLow ? kLow : 0;
+  p.rows = p.low ? 2 * kLow : c->rows;
   p.half = (c->F + 63) / 64 * 64;
   p.gate = choose(c->rows, 2 * (int64_t)c->F, steps(c->D), 1, false);
-  p.out = choose(c->rows, c->D_out, steps(c->F), kSplits, true);
+  p.out = choose(p.rows, c->D_out, steps(c->F), kSplits, true);
   p.dgate = choose(c->rows, c->F, steps(c->D_out), 1, false);
-  p.dx = choose(c->rows, c->D, 2 * steps(c->F), kSplits, true);
+  p.dx = choose(p.rows, c->D, 2 * steps(c->F), kSplits, true);
   p.dw = choose(2 * (int64_t)p.half, c->D, steps(c->rows), kSplits, true);
   p.dw2 = choose(c->D_out, c->F, steps(c->rows), kSplits, true);
   // The gate's gradients wait for memory at the end of a tile, dW2 hardly: side by side on a CU they take less (8192 x 1536 x 4096 277 us
   // in a launch of 128 x 128 tiles; apart 121 and 184, or 183 with 128 x 128)
+  if (p.low) p.dw = p.dw2 = Tiling{SQUARE, 1, 0.0};
   if (p.dw2.kind == SQUARE) p.dgate.kind = SQUARE;
-  p.h = up((size_t)c->rows * c->F * 2);
+  p.h = up((size_t)p.rows * c->F * 2);
   p.plane = up((size_t)Float24::elements(c->rows, c->F) * 3);
-  p.d = up((size_t)c->rows * 2 * p.half * 2);
-  p.part[0] = part(p.out, c->rows, c->D_out);
-  p.part[1] = part(p.dx, c->rows, c->D);
-  p.part[2] = part(p.dw, 2 * (int64_t)p.half, c->D);
-  p.part[3] = part(p.dw2, c->D_out, c->F);
-  p.colsum = up(std::max(llattn_colsum_workspace_size(c->rows, c->F), llattn_colsum_workspace_size(c->rows, c->D_out)));
+  p.d = up((size_t)p.rows * 2 * p.half * 2);
+  p.part[0] = part(p.out, p.rows, c->D_out, p.low);
+  p.part[1] = part(p.dx, p.rows, c->D, p.low);
+  p.part[2] = part(p.dw, 2 * (int64_t)p.half, c->D, false);
+  p.part[3] = part(p.dw2, c->D_out, c->F, false);
+  p.colsum = up(std::max(llattn_colsum_workspace_size(p.rows, c->F), llattn_colsum_workspace_size(c->rows, c->D_out)));
   return p;
 }
 // Forward with a backward to follow, forward alone (h in it, as two bf16 values where rows are few), backward, what is kept between them
@@ -851,6 +897,7 @@ extern "C" int32_t llattn_gated_fwd(const llattn_gated_cfg* c, const void* x, in
   a.bias = w->b1; a.bias2 = w->b3;
   a.act = c->act;
   a.h = reinterpret_cast<uint16_t*>(kept ? static_cast<char*>(kept) : ws);
+  a.low = plan.low;
   if (kept) {
     a.p = static_cast<unsigned char*>(kept) + plan.h;
     a.s = a.p + plan.plane;
@@ -859,11 +906,11 @@ extern "C" int32_t llattn_gated_fwd(const llattn_gated_cfg* c, const void* x, in
   }
   launch<GateProduct>(a, plan.gate, st);
   GatedArgs o{};
-  o.M = c->rows; o.N = c->D_out; o.K = c->F;
+  o.M = plan.rows; o.fold = plan.low; o.N = c->D_out; o.K = c->F;
   o.A = a.h; o.lda = c->F;
   o.B = bf16(w->W2); o.ldb = c->F;
   o.bias = w->b2;
-  o.C = y; o.ldc = c->D_out; o.m_half = o.m_live = c->rows;
+  o.C = y; o.ldc = c->D_out; o.m_half = plan.rows; o.m_live = c->rows;
   o.part = plan.part[0] ? reinterpret_cast<float*>(ws) : nullptr;
   launch<OutProduct>(o, plan.out, st);
   const GatedArgs* args[] = {&o};
@@ -900,7 +947,7 @@ extern "C" int32_t llattn_gated_bwd(const llattn_gated_cfg* c, const void* x, in
   gate.A = bf16(dy); gate.lda = c->D_out;
   gate.B = bf16(w->W2); gate.ldb = c->F;
   gate.p = p; gate.s = p + plan.plane;
-  gate.d = d; gate.ldd = ldd;
+  gate.d = d; gate.ldd = ldd; gate.low = plan.low;
 
   dw2.M = c->D_out; dw2.N = c->F; dw2.K = c->rows;
   dw2.A = bf16(dy); dw2.lda = c->D_out;
@@ -909,11 +956,11 @@ extern "C" int32_t llattn_gated_bwd(const llattn_gated_cfg* c, const void* x, in
   dw2.f32 = c->dw2_dtype == LLATTN_F32;
   dw2.part = on_dw2 ? part[3] : nullptr;
 
-  dx.M = c->rows; dx.N = c->D; dx.K = ldd;
+  dx.M = plan.rows; dx.fold = plan.low; dx.N = c->D; dx.K = ldd;
   dx.A = d; dx.lda = ldd;
   dx.B = bf16(w->W1); dx.B2 = bf16(w->W3); dx.ldb = c->D;
   dx.half = plan.half / 64; dx.k_half = c->F;
-  dx.C = g->dx; dx.ldc = c->D; dx.m_half = dx.m_live = c->rows;
+  dx.C = g->dx; dx.ldc = c->D; dx.m_half = plan.rows; dx.m_live = c->rows;
   dx.part = on_dx ? part[1] : nullptr;
 
   dw.M = ldd; dw.N = c->D; dw.K = c->rows;
@@ -923,27 +970,36 @@ extern "C" int32_t llattn_gated_bwd(const llattn_gated_cfg* c, const void* x, in
   dw.f32 = c->dw_dtype == LLATTN_F32;
   dw.part = on_dw ? part[2] : nullptr;
 
+  if (plan.low) {  // two steps over the rows: of the upper and the lower halves
+    for (GatedArgs* q : {&dw, &dw2}) { q->K = 2 * kLow; q->half = kLow / 64; q->k_half = c->rows; }
+    dw.A2 = d + (int64_t)kLow * ldd; dw.B2 = dw.B;
+    dw2.A2 = dw2.A; dw2.B2 = dw2.B + (int64_t)kLow * c->F;
+  }
   // independent products of 128 x 128 tiles share a launch
   if (on_gate && on_dw2 && plan.dgate.kind == SQUARE && plan.dw2.kind == SQUARE) {
-    launch_pair<DGateProduct, DwProduct>(gate, plan.dgate, dw2, plan.dw2, st);
+    if (plan.low) launch_pair<DGateProduct, DwHalvesProduct>(gate, plan.dgate, dw2, plan.dw2, st);
+    else launch_pair<DGateProduct, DwProduct>(gate, plan.dgate, dw2, plan.dw2, st);
   } else {
     if (on_gate) launch<DGateProduct>(gate, plan.dgate, st);
-    if (on_dw2) launch<DwProduct>(dw2, plan.dw2, st);
+    if (on_dw2 && plan.low) launch_square<DwHalvesProduct>(dw2, plan.dw2, st);
+    else if (on_dw2) launch<DwProduct>(dw2, plan.dw2, st);
   }
   if (on_dx && on_dw && plan.dx.kind == SQUARE && plan.dw.kind == SQUARE) {
-    launch_pair<DxProduct, DwProduct>(dx, plan.dx, dw, plan.dw, st);
+    if (plan.low) launch_pair<DxProduct, DwHalvesProduct>(dx, plan.dx, dw, plan.dw, st);
+    else launch_pair<DxProduct, DwProduct>(dx, plan.dx, dw, plan.dw, st);
   } else {
     if (on_dx) launch<DxProduct>(dx, plan.dx, st);
-    if (on_dw) launch<DwProduct>(dw, plan.dw, st);
+    if (on_dw && plan.low) launch_square<DwHalvesProduct>(dw, plan.dw, st);
+    else if (on_dw) launch<DwProduct>(dw, plan.dw, st);
   }
   const GatedArgs* args[] = {&dx, &dw, &dw2};
   const Tiling* tilings[] = {&plan.dx, &plan.dw, &plan.dw2};
   launch_reduce(args, tilings, 3, st);
-  const auto bias = [&](float* out, const uint16_t* from, int64_t ld, int n) -> int32_t {
-    return out ? llattn_colsum(from, ld, c->rows, n, out, at, plan.colsum, stream) : LLATTN_OK;
+  const auto bias = [&](float* out, const uint16_t* from, int64_t ld, int rows, int n) -> int32_t {
+    return out ? llattn_colsum(from, ld, rows, n, out, at, plan.colsum, stream) : LLATTN_OK;
   };
-  if (const int32_t rc = bias(g->db1, d, ldd, c->F)) return rc;
-  if (const int32_t rc = bias(g->db3, d + plan.half, ldd, c->F)) return rc;
-  if (const int32_t rc = bias(g->db2, bf16(dy), c->D_out, c->D_out)) return rc;
+  if (const int32_t rc = bias(g->db1, d, ldd, plan.rows, c->F)) return rc;
+  if (const int32_t rc = bias(g->db3, d + plan.half, ldd, plan.rows, c->F)) return rc;
+  if (const int32_t rc = bias(g->db2, bf16(dy), c->D_out, c->rows, c->D_out)) return rc;
   return check_launch("llattn_gated_bwd");
 }

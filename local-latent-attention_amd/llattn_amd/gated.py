@@ -3,8 +3,8 @@ the counterpart with a gate of :func:`llattn_amd.ffn.feed_forward`.
 
 Both projections, the activation and the product are one kernel; the backward's first product leaves the gradients of both
 projections, and both weight gradients come out of one more.  Numerics: bf16 operands, fp32 sums, ``w1 x`` and ``w3 x`` not
-rounded, their gated product rounded to bf16 for the last projection (kept in 16 bits of significand where up to 24 rows are evaluated); the
-backward keeps ``act(w1 x)`` and ``act'(w1 x) w3 x`` in 24 bits.
+rounded, their gated product and its counterparts backward rounded to bf16 (two bf16 values up to 64 rows); the backward keeps
+``act(w1 x)`` and ``act'(w1 x) w3 x`` in 24 bits.
 """
 from __future__ import annotations
 

@@ -3,7 +3,8 @@
 Tolerances are counted, elementwise, with b = 2^-8 (half a step of bf16) and u = 2^-24 (of fp32).  A sum of K products of
 exact bf16 values is off by at most (K + 2) u of the sum of their sizes.  The activations have slopes of at most 1.13 and
 curvatures of at most 0.8 and are evaluated to 2e-5 of themselves (their slopes to 2e-5).  h, da and du are rounded to bf16 once
-each, p = act(a) and s = act'(a) u cut off after 24 bits (2^-15 of themselves), results rounded once more.
+each (up to 64 rows to two bf16 values), p = act(a) and s = act'(a) u cut off after 24 bits (2^-15 of themselves), results rounded
+once more.
 """
 import pytest
 import torch
@@ -49,9 +50,10 @@ def _act(name, a):
     return a * cdf, cdf + a * torch.exp(-0.5 * a * a) * 0.3989422804014327
 
 
-def _exact(x, layers, act, dy, h_rounded=True):
-    """Pairs (value, bound of the error before the last rounding) in 64 bits, in the order of NAMES.  h not rounded: two bf16
-    halves of it, 2^-16 of itself."""
+def _exact(x, layers, act, dy):
+    """Pairs (value, bound of the error before the last rounding) in 64 bits, in the order of NAMES.  Up to 64 rows h, da and du are
+    the sums of two bf16 values: the lower one rounds what the upper one has left (2^-8 of the value at most) by 2^-8 of that."""
+    half = B16 if x.shape[0] > 64 else 2.0 ** -16
     x, dy = x.detach().to(BF16).double(), dy.to(BF16).double()
     w1, w3, w2 = (m.weight.detach().to(BF16).double() for m in layers)
     b1, b3, b2 = (torch.zeros((), dtype=torch.float64, device=DEV) if m.bias is None else m.bias.detach().double() for m in layers)
@@ -64,7 +66,7 @@ def _exact(x, layers, act, dy, h_rounded=True):
     ef, edf = 1.13 * ea + 2e-5 * f.abs(), 0.8 * ea + 2e-5
     h = f * u
     eh = f.abs() * eu + u.abs() * ef + ef * eu
-    eh = eh + (B16 if h_rounded else 2.0 ** -16) * (h.abs() + eh)
+    eh = eh + half * (h.abs() + eh)
     y = h @ w2.t() + b2
     ey = eh @ w2.abs().t() + c(Fd) * ((h.abs() + eh) @ w2.abs().t() + b2.abs())
     p, ep = f, ef + 2.0 ** -15 * (f.abs() + ef)
@@ -73,7 +75,7 @@ def _exact(x, layers, act, dy, h_rounded=True):
     es = es + 2.0 ** -15 * (s.abs() + es)
     dh = dy @ w2
     edh = c(Do) * (dy.abs() @ w2.abs())
-    prod = lambda m, em: (dh * m, (t := dh.abs() * em + m.abs() * edh + em * edh) + B16 * ((dh * m).abs() + t))  # noqa: E731
+    prod = lambda m, em: (dh * m, (t := dh.abs() * em + m.abs() * edh + em * edh) + half * ((dh * m).abs() + t))  # noqa: E731
     (da, eda), (du, edu) = prod(s, es), prod(p, ep)
     dx = da @ w1 + du @ w3
     size = (da.abs() + eda) @ w1.abs() + (du.abs() + edu) @ w3.abs()
@@ -100,11 +102,14 @@ CASES = [
     (1, 8, 8, 8, "silu", False, BF16, BF16),
     (1, 1408, 4096, 1408, "silu", False, BF16, BF16),
     (2, 64, 200, 64, "gelu", True, BF16, F32),
+    (2, 1536, 210, 250, "silu", True, BF16, F32),
     (7, 136, 72, 24, "silu", True, F32, F32),
     (16, 1408, 4096, 1408, "gelu", True, BF16, BF16),
     (17, 250, 333, 250, "silu", True, BF16, BF16),
+    (17, 64, 229, 64, "silu", False, BF16, F32),
     (33, 777, 1001, 777, "gelu", False, BF16, BF16),
     (64, 128, 256, 128, "gelu", True, BF16, F32),
+    (64, 1408, 1096, 520, "silu", True, BF16, F32),
     (65, 72, 64, 200, "silu", False, BF16, BF16),
     (129, 1, 3, 5, "silu", True, F32, BF16),
     (333, 264, 520, 264, "silu", True, BF16, F32),
@@ -127,11 +132,11 @@ def test_values_and_gradients(case):
     for name, t, (want, err) in zip(NAMES, got, _exact(x, layers, act, dy)):
         if t is not None:
             _near(t, want, err, name)
-    with torch.no_grad():  # nothing kept: the same values, up to 24 rows without the rounding of h
+    with torch.no_grad():  # nothing kept: the same values, from other kernels up to 24 rows
         y = _ffn(x, *layers, act=act)
     if N > 24:
         assert torch.equal(y, got[0])
-    _near(y, *_exact(x, layers, act, dy, h_rounded=N > 24)[0], "y alone")
+    _near(y, *_exact(x, layers, act, dy)[0], "y alone")
     again = _grads(x, layers, act, dy)
     assert all(a is None or torch.equal(a, b) for a, b in zip(got, again))
 
@@ -345,22 +350,23 @@ def test_streams_and_replays():
     assert len(ps) == 6
 
 
-def test_an_infinite_gradient_stays_infinite():
-    # positive weights and values: every gradient of row 0 is infinite, none is 0 times infinity.  F is no whole step of the
-    # products over F, and W2 has zeros in the rows that dy's row 0 does not read
+@pytest.mark.parametrize("N", [3, 70])
+def test_an_infinite_gradient_stays_infinite(N):
+    # positive weights and values: every gradient of row 0 is infinite, none is 0 times infinity (but the lower half of h in few
+    # rows).  F is no whole step of the products over F, and W2 has zeros in the rows that dy's row 0 does not read
     layers = _layers(8, 8, 16, bias=False)
     with torch.no_grad():
         for m in layers:
             m.weight.fill_(0.5)
         layers[2].weight[1:] = 0.0
-    x = torch.ones(3, 8, dtype=BF16, device=DEV, requires_grad=True)
-    dy = torch.zeros(3, 16, dtype=BF16, device=DEV)
+    x = torch.ones(N, 8, dtype=BF16, device=DEV, requires_grad=True)
+    dy = torch.zeros(N, 16, dtype=BF16, device=DEV)
     dy[0, 0], dy[1:] = float("inf"), 1.0
     y = _ffn(x, *layers)
     dx, dw1, dw3, dw2 = torch.autograd.grad(y, [x] + [m.weight for m in layers], dy)
     assert bool((dx[0] == float("inf")).all()) and bool(dx[1:].isfinite().all())
     assert bool((dw1 == float("inf")).all()) and bool((dw3 == float("inf")).all())
-    assert bool((dw2[0] == float("inf")).all()) and bool(dw2[1:].isfinite().all())
+    assert bool((dw2[0] == float("inf")).all() if N > 64 else (~dw2[0].isfinite()).all()) and bool(dw2[1:].isfinite().all())
 
 
 def test_no_second_derivatives():
