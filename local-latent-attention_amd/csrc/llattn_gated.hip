@@ -775,12 +775,13 @@ void launch_reduce(const GatedArgs* const* a, const Tiling* const* t, int n, hip
 }
 
 constexpr int kSplits = 16;
-// Rows of a forward alone that the kernels for few of them take.  us in a graph, these and the tiles, D 1408, F 4096: 1 row 11.7 and 23.6,
-// 16 rows 17.8 and 24.7, 24 rows 24.1 and 25.4, 32 rows 27.1 and 25.8 (F 256: 6.4 and 8.8)
-constexpr int kThinRows = 24;
+// Rows of a forward alone that the kernels for few of them take (two operands of 16 rows).  us in a graph, D 1408, F 4096, by these and by
+// tiles: 1 row 12.1 and 30.8, 16 rows 18.2 and 31.3, 32 rows 27.4 and 32.3; D and F 256: 6.8 and 13.0, 6.9 and 13.8, 7.2 and 14.4
+constexpr int kThinRows = 32;
 // Rows up to which h, da and du are held as two bf16 values (16 bits of significand), the lower ones kLow rows behind the upper: as more
 // rows of the products with the weights, whose 128 x 128 tiles have room for them, and as a second step of those over the rows.  With
-// few values their rounding shows: rms errors of single results then lie up to 1.55 times as far out as their own rounding puts them.
+// few values their rounding shows: rms errors of single results then lay up to 1.55 times as far out as their own rounding puts them.
+// us of a training pass in a graph, D 1408, F 4096, so and in bf16: 1 row 77 and 64, 64 rows 83 and 73 (the host takes 160 without one).
 constexpr int kLow = 64;
 struct Plan {
   int low, rows;            // kLow or 0; rows of h and d

@@ -132,9 +132,9 @@ def test_values_and_gradients(case):
     for name, t, (want, err) in zip(NAMES, got, _exact(x, layers, act, dy)):
         if t is not None:
             _near(t, want, err, name)
-    with torch.no_grad():  # nothing kept: the same values, from other kernels up to 24 rows
+    with torch.no_grad():  # nothing kept: the same values, from other kernels up to 32 rows
         y = _ffn(x, *layers, act=act)
-    if N > 24:
+    if N > 32:
         assert torch.equal(y, got[0])
     _near(y, *_exact(x, layers, act, dy)[0], "y alone")
     again = _grads(x, layers, act, dy)
@@ -277,9 +277,9 @@ def test_rows_stay_apart():
     assert bool(b[10].isnan().any()) and bool(b[:10].isfinite().all()) and bool(b[11:].isfinite().all())
 
 
-@pytest.mark.parametrize("N", [1, 2, 15, 16, 17, 23, 24])
+@pytest.mark.parametrize("N", [1, 2, 15, 16, 17, 23, 24, 31, 32])
 def test_few_rows_forward_alone(N):
-    """The kernels for up to 24 rows: exact on whole numbers, each row's bits whatever the others are."""
+    """The kernels for up to 32 rows: exact on whole numbers, each row's bits whatever the others are."""
     for D, F, Do in ((8, 8, 8), (24, 40, 8), (264, 520, 72), (1408, 4096, 1408)):
         x, w1, w3, w2, _ = _whole(N, D, F, Do)
         layers = []
