@@ -8,8 +8,8 @@
 // in every workgroup, in one order, so that no launch stands between them.
 //
 // What bounds it: memory.  Gradients are read twice (a norm has to be known before anything is scaled) and written once, past the
-// caches (non-temporal), which are left to what the norm has read last.  The 463 M fp32 gradients of the 0.55b model: squares
-// 0.34 ms (5.4 TB/s), scaling 0.79 ms (4.7 TB/s).  Eight loads ahead instead of four took 7% off the squares; chunks of
+// caches (non-temporal), which are left to what the norm has read last.  The 540 M fp32 gradients of the 0.55b model: squares
+// 0.36 ms (6.0 TB/s), scaling 0.85 ms (5.1 TB/s; a copy 5.0).  Eight loads ahead instead of four took 7% off the squares; chunks of
 // 65536, 1024 to 4096 workgroups and one workgroup a chunk were no quicker (the last 50% slower, as each adds up the parts).
 #include <algorithm>
 #include <new>

@@ -17,8 +17,9 @@
 // Backward, two products share a launch where both take 128 x 128 tiles (the gate's gradients with dW2, dx with dW1 and dW3): small
 // ones fill the chip together.  Forward alone with few rows, two kernels of their own read every weight once, along k.
 //
-// What bounds it: the matrix cores (2 rows D F operations for each of the three products, twice that backward); with few
-// rows the reads of the weights.
+// What bounds it: the matrix cores (2 rows D F operations for each of the three products, twice that backward) and epilogues that no
+// other tile's products cover; with few rows the reads of the weights.  8192 x 1536 x 4096: gate 206 us (1.0 PFLOP/s), y 89 (1.16),
+// the gate's gradients and dW2 237 (0.87), dx 178 (1.16), dW1 and dW3 174 (1.18); 8192 cubed runs at 1.32 in this library's plain product.
 #include <algorithm>
 
 #include "llattn_lm.h"
@@ -804,8 +805,8 @@ Plan plan_of(const llattn_gated_cfg* c) {
   p.dx = choose(p.rows, c->D, 2 * steps(c->F), kSplits, true);
   p.dw = choose(2 * (int64_t)p.half, c->D, steps(c->rows), kSplits, true);
   p.dw2 = choose(c->D_out, c->F, steps(c->rows), kSplits, true);
-  // The gate's gradients wait for memory at the end of a tile, dW2 hardly: side by side on a CU they take less (8192 x 1536 x 4096 277 us
-  // in a launch of 128 x 128 tiles; apart 121 and 184, or 183 with 128 x 128)
+  // The gate's gradients wait for memory at the end of a tile, dW2 hardly: side by side on a CU they take less (8192 x 1536 x 4096, before p
+  // and s went past the caches: 277 us in a launch of 128 x 128 tiles, apart 121 and 184, or 183 with 128 x 128; 237 since)
   if (p.low) p.dw = p.dw2 = Tiling{SQUARE, 1, 0.0};
   if (p.dw2.kind == SQUARE) p.dgate.kind = SQUARE;
   p.h = up((size_t)p.rows * c->F * 2);
