@@ -112,8 +112,8 @@ typedef struct llattn_gated_grads {
   float *db1, *db3, *db2;
 } llattn_gated_grads;
 
-/* Bytes of a buffer; 0 with an error message on a bad configuration: workspace of a forward with `kept`, of one without, of the
- * backward; what is kept between them. */
+/* Bytes of a buffer (1: none is needed, NULL is taken); 0 with an error message on a bad configuration: workspace of a forward with
+ * `kept`, of one without, of the backward; what is kept between them. */
 #define LLATTN_GATED_FORWARD 0
 #define LLATTN_GATED_ALONE 1
 #define LLATTN_GATED_BACKWARD 2

@@ -792,38 +792,46 @@ struct Plan {
   size_t plane;             // p and s, of three bytes
   size_t colsum;
 };
-Plan plan_of(const llattn_gated_cfg* c) {
+// The sizes, and the tilings of a direction's products and what follows from them (a microsecond or two of the host's for each)
+enum { SIZES = 0, OF_FORWARD = 1, OF_BACKWARD = 2 };
+Plan plan_of(const llattn_gated_cfg* c, int which) {
   Plan p{};
   const auto steps = [](int k) { return (k + 63) / 64; };
   const auto part = [](const Tiling& t, int64_t m, int64_t n, bool folded) { return t.splits > 1 || folded ? up((size_t)t.splits * m * n * 4) : 0; };
   p.low = c->rows <= kLow ? kLow : 0;
   p.rows = p.low ? 2 * kLow : c->rows;
   p.half = (c->F + 63) / 64 * 64;
-  p.gate = choose(c->rows, 2 * (int64_t)c->F, steps(c->D), 1, false);
-  p.out = choose(p.rows, c->D_out, steps(c->F), kSplits, true);
-  p.dgate = choose(c->rows, c->F, steps(c->D_out), 1, false);
-  p.dx = choose(p.rows, c->D, 2 * steps(c->F), kSplits, true);
-  p.dw = choose(2 * (int64_t)p.half, c->D, steps(c->rows), kSplits, true);
-  p.dw2 = choose(c->D_out, c->F, steps(c->rows), kSplits, true);
-  // The gate's gradients wait for memory at the end of a tile, dW2 hardly: side by side on a CU they take less (8192 x 1536 x 4096, before p
-  // and s went past the caches: 277 us in a launch of 128 x 128 tiles, apart 121 and 184, or 183 with 128 x 128; 237 since)
-  if (p.low) p.dw = p.dw2 = Tiling{SQUARE, 1, 0.0};
-  if (p.dw2.kind == SQUARE) p.dgate.kind = SQUARE;
   p.h = up((size_t)p.rows * c->F * 2);
   p.plane = up((size_t)Float24::elements(c->rows, c->F) * 3);
   p.d = up((size_t)p.rows * 2 * p.half * 2);
-  p.part[0] = part(p.out, p.rows, c->D_out, p.low);
-  p.part[1] = part(p.dx, p.rows, c->D, p.low);
-  p.part[2] = part(p.dw, 2 * (int64_t)p.half, c->D, false);
-  p.part[3] = part(p.dw2, c->D_out, c->F, false);
-  p.colsum = up(std::max(llattn_colsum_workspace_size(p.rows, c->F), llattn_colsum_workspace_size(c->rows, c->D_out)));
+  if (which == OF_FORWARD) {
+    p.gate = choose(c->rows, 2 * (int64_t)c->F, steps(c->D), 1, false);
+    p.out = choose(p.rows, c->D_out, steps(c->F), kSplits, true);
+    p.part[0] = part(p.out, p.rows, c->D_out, p.low);
+  } else if (which == OF_BACKWARD) {
+    p.dgate = choose(c->rows, c->F, steps(c->D_out), 1, false);
+    p.dx = choose(p.rows, c->D, 2 * steps(c->F), kSplits, true);
+    if (p.low) {
+      p.dw = p.dw2 = Tiling{SQUARE, 1, 0.0};
+    } else {
+      p.dw = choose(2 * (int64_t)p.half, c->D, steps(c->rows), kSplits, true);
+      p.dw2 = choose(c->D_out, c->F, steps(c->rows), kSplits, true);
+    }
+    // The gate's gradients wait for memory at the end of a tile, dW2 hardly: side by side on a CU they take less (8192 x 1536 x 4096, before
+    // p and s went past the caches: 277 us in a launch of 128 x 128 tiles, apart 121 and 184, or 183 with 128 x 128; 237 since)
+    if (p.dw2.kind == SQUARE) p.dgate.kind = SQUARE;
+    p.part[1] = part(p.dx, p.rows, c->D, p.low);
+    p.part[2] = part(p.dw, 2 * (int64_t)p.half, c->D, false);
+    p.part[3] = part(p.dw2, c->D_out, c->F, false);
+    p.colsum = up(std::max(llattn_colsum_workspace_size(p.rows, c->F), llattn_colsum_workspace_size(c->rows, c->D_out)));
+  }
   return p;
 }
 // Forward with a backward to follow, forward alone (h in it, as two bf16 values where rows are few), backward, what is kept between them
 enum Space { FORWARD = LLATTN_GATED_FORWARD, ALONE = LLATTN_GATED_ALONE, BACKWARD = LLATTN_GATED_BACKWARD, KEPT = LLATTN_GATED_KEPT };
 size_t bytes_of(const llattn_gated_cfg* c, const Plan& p, int which) {
   switch (which) {
-    case FORWARD: return std::max<size_t>(p.part[0], 256);
+    case FORWARD: return std::max<size_t>(p.part[0], 1);
     case ALONE: return c->rows <= kThinRows ? up((size_t)c->rows * c->F * 4) : p.h + p.part[0];
     case BACKWARD: return p.d + p.part[1] + p.part[2] + p.part[3] + p.colsum;
     default: return p.h + 2 * p.plane;
@@ -847,8 +855,10 @@ int32_t check_operands(const char* who, const llattn_gated_cfg* c, const void* x
   if (!x || !w || !w->W1 || !w->W3 || !w->W2) return fail(LLATTN_ERR_LAYOUT, "%s: null x or weights", who);
   for (const void* p : {x, w->W1, w->W3, w->W2, (const void*)w->b1, (const void*)w->b3, (const void*)w->b2})
     if (!aligned16(p)) return fail(LLATTN_ERR_LAYOUT, "%s: x, weights and biases must be 16-byte aligned", who);
-  if (ldx < c->D || ldx % 8 || ldx >= 1 << 23) return fail(LLATTN_ERR_LAYOUT, "%s: rows of x: a stride of %lld elements (a multiple of 8 in [D, 2^23))", who, (long long)ldx);
-  if (!ws || bytes < need || !aligned16(ws)) return fail(LLATTN_ERR_WORKSPACE, "%s: needs %zu workspace bytes (got %zu)", who, need, bytes);
+  if (ldx < c->D || ldx % 8 || ldx >= 1 << 23)
+    return fail(LLATTN_ERR_LAYOUT, "%s: rows of x: a stride of %lld elements (a multiple of 8 in [D, 2^23))", who, (long long)ldx);
+  if (need > 1 && (!ws || bytes < need || !aligned16(ws)))
+    return fail(LLATTN_ERR_WORKSPACE, "%s: needs %zu workspace bytes (got %zu)", who, need, bytes);
   return LLATTN_OK;
 }
 
@@ -865,19 +875,21 @@ extern "C" size_t llattn_gated_bytes(const llattn_gated_cfg* c, int32_t which) {
     fail(LLATTN_ERR_SHAPE, "llattn_gated_bytes: unknown buffer %d", which);
     return 0;
   }
-  return bytes_of(c, plan_of(c), which);
+  const bool thin = which == ALONE && c->rows <= kThinRows;
+  return bytes_of(c, plan_of(c, which == BACKWARD ? OF_BACKWARD : which == KEPT || thin ? SIZES : OF_FORWARD), which);
 }
 
 extern "C" int32_t llattn_gated_fwd(const llattn_gated_cfg* c, const void* x, int64_t ldx, const llattn_gated_weights* w, void* kept,
                                     void* y, void* workspace, size_t workspace_bytes, void* stream) {
   if (const int32_t rc = check("llattn_gated_fwd", c)) return rc;
-  const Plan plan = plan_of(c);
+  const bool thin = !kept && c->rows <= kThinRows;
+  const Plan plan = plan_of(c, thin ? SIZES : OF_FORWARD);
   const size_t need = bytes_of(c, plan, kept ? FORWARD : ALONE);
   if (const int32_t rc = check_operands("llattn_gated_fwd", c, x, ldx, w, workspace, workspace_bytes, need)) return rc;
   if (!y || !aligned16(y) || !aligned16(kept)) return fail(LLATTN_ERR_LAYOUT, "llattn_gated_fwd: null y, or y or kept not 16-byte aligned");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
-  if (!kept && c->rows <= kThinRows) {
+  if (thin) {
     ThinArgs gate{}, out{};
     gate.M = out.M = c->rows;
     gate.N = out.K = c->F; gate.K = c->D; out.N = c->D_out;
@@ -925,7 +937,7 @@ extern "C" int32_t llattn_gated_bwd(const llattn_gated_cfg* c, const void* x, in
                                     const void* kept, const void* dy, const llattn_gated_grads* g, void* workspace,
                                     size_t workspace_bytes, void* stream) {
   if (const int32_t rc = check("llattn_gated_bwd", c)) return rc;
-  const Plan plan = plan_of(c);
+  const Plan plan = plan_of(c, OF_BACKWARD);
   if (const int32_t rc = check_operands("llattn_gated_bwd", c, x, ldx, w, workspace, workspace_bytes, bytes_of(c, plan, BACKWARD))) return rc;
   if (!kept || !dy || !g) return fail(LLATTN_ERR_LAYOUT, "llattn_gated_bwd: null kept, dy or gradients");
   for (const void* q : {kept, dy, (const void*)g->dx, (const void*)g->dW1, (const void*)g->dW3, (const void*)g->dW2})

@@ -60,7 +60,7 @@ def _buffer(cfg, which, device):
     n = L.load().llattn_gated_bytes(ctypes.byref(cfg), which)
     if n == 0:
         L.check(L.ERR_SHAPE, "llattn_gated_bytes")
-    return torch.empty((n,), dtype=torch.uint8, device=device), n
+    return torch.empty((n,), dtype=torch.uint8, device=device) if n > 1 else None, n
 
 
 def _forward(x, act, ps, saved):
@@ -82,7 +82,7 @@ def _forward(x, act, ps, saved):
         work, n = _buffer(cfg, L.GATED_FORWARD if saved else L.GATED_ALONE, dev)
         with L.on_device(dev):
             ops._call("llattn_gated_fwd", ctypes.byref(cfg), xb.data_ptr(), xb.stride(0),
-                  ctypes.byref(L.LlattnGatedWeights(*map(_ptr, ws), *map(_ptr, bs))), _ptr(kept), y.data_ptr(), work.data_ptr(), n,
+                  ctypes.byref(L.LlattnGatedWeights(*map(_ptr, ws), *map(_ptr, bs))), _ptr(kept), y.data_ptr(), _ptr(work), n,
                   L.stream_ptr(dev), work=6 * N * D * Fd)
     if po:
         y = y[:, :Do]

@@ -224,6 +224,8 @@ def test_gated_sizes_refused(kw):
     for which in range(4):
         assert L.load().llattn_gated_bytes(ctypes.byref(_gated_cfg(**kw)), which) == 0 and L.load().llattn_last_error()
         assert L.load().llattn_gated_bytes(ctypes.byref(_gated_cfg()), which) > 0
+    # enough tiles: no parts of y, and no workspace of a forward that keeps h
+    assert L.load().llattn_gated_bytes(ctypes.byref(_gated_cfg(rows=4096, D_out=4096)), L.GATED_FORWARD) == 1
     for which in (-1, 4):
         assert L.load().llattn_gated_bytes(ctypes.byref(_gated_cfg()), which) == 0
 
