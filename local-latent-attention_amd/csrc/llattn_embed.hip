@@ -438,6 +438,8 @@ __device__ __forceinline__ Block block_at(const Keys& s, int counted, int c, int
   const int64_t last = (int64_t)c * size + size - 1;
   if (last >= counted) return Block{make_int2(0, 0), 0, -1};
   const int key = key_at(s, (int)last);
+  // the keys lie in the caller's memory: one written to since the rows were ordered changes sums, and reads nothing outside
+  if (s.keys && (uint32_t)key >= (uint32_t)s.R) return Block{make_int2(0, 0), 0, -1};
   const int2 run = run_of(s, key);
   const int at = ((int)last - run.x) / size * size;
   return Block{run, key, at + size <= run.y - run.x ? at : -1};

@@ -351,3 +351,19 @@ def test_two_graphs_at_once():
         torch.cuda.synchronize()
         for _, out, want, _, _ in runs:
             assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("value", [-1, 4999, 5000, 1 << 20, (1 << 31) - 1, 1 << 40])
+def test_indices_written_over_before_the_backward(value):
+    # past the version counter, which refuses the backward otherwise: the tokens' sums are anything, the positions' right
+    w, p = (t.requires_grad_() for t in _tables(5000, 700, 136, F32))
+    ids = _ids((4, 700), 5000)
+    y = _embed(ids, w, p, positions=torch.arange(700, device=DEV).expand(4, 700).contiguous())
+    ids.data.fill_(value)
+    dw, dp = torch.autograd.grad(y, (w, p), torch.ones_like(y))
+    assert dw.shape == w.shape and torch.equal(dp, torch.full_like(dp, 4.0))
+    ids = _ids((4, 700), 5000)
+    y = _embed(ids, w, p)
+    ids.fill_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(y, (w, p), torch.ones_like(y))
