@@ -4,7 +4,7 @@
 //
 // The gradients are sums over the rows of one key (a token or a position), so the rows are ordered by key first.  That waits for no
 // gradient, so a training pass does it behind the forward, where the chip is idle until the host has come to the backward (packed
-// rows, 8192 x 1536: 143 us with it in the backward, 128; the sort is 19 us).  One launch, a workgroup for each residue class of keys
+// rows, 8192 x 1536: 143 us with it in the backward, 128; the sort was 19 us then, 12 now).  One launch, a workgroup for each residue class of keys
 // (key mod buckets), which reads all keys, keeps its own in their order and counts them out by key.  The order of the keys among
 // themselves is of no use here; the residues spread a text's frequent tokens, whose numbers are close, over the workgroups.  Where
 // positions are n % T the order is known.
@@ -18,7 +18,7 @@
 //
 // What bounds it: memory.  Forward: a table row read and a row written per token; backward: dout read once for each
 // table, the tables' gradients written whole.  us in training passes of 32768 rows x 1408 fp32, 32000 tokens, 2048 positions: forward
-// 57 (250 MB), order 21 (latency: half of it the reading of the keys by 256 workgroups), sums of 32 rows 20, of 1024 5, the tables
+// 57 (250 MB), order 20 (latency: half of it the reading of the keys by 256 workgroups), sums of 32 rows 20, of 1024 5, the tables
 // 68 (380 MB); a copy runs at 5.0 TB/s.  Few tokens take none but the last of these launches (embed_scan_kernel).
 #include <algorithm>
 
@@ -191,9 +191,10 @@ struct SortArgs {
 };
 
 // The keys of a workgroup's waves, 64 at a time, stay in registers between the counting and the collecting where they are no
-// more than kSteps times 64 a wave (32768 rows); others are read again.
-constexpr int kSteps = 32;
-__global__ __launch_bounds__(64 * kWaves) void embed_sort_kernel(const SortArgs a) {
+// more than STEPS times 64 a wave (16384 rows, 32768 rows); others are read again.  64 registers at most: two workgroups on a CU, of the
+// two sets.  (8192 rows in two sets 12.0 us with 16 steps, 14.8 with 32, 19.4 with 76 registers; 32768 rows 25.4 with 16, 20.4 with 32.)
+template <int STEPS>
+__global__ __launch_bounds__(64 * kWaves, 8) void embed_sort_kernel(const SortArgs a) {
   __shared__ int2 list[kList];
   __shared__ int count[kWaves][kKeys];
   __shared__ int eq_of[kWaves], lt_of[kWaves], all_of[kWaves], sums[kKeys / 64];
@@ -205,18 +206,18 @@ __global__ __launch_bounds__(64 * kWaves) void embed_sort_kernel(const SortArgs 
   const int64_t lo = min((int64_t)a.rows, w * seg), hi = min((int64_t)a.rows, lo + seg);
   constexpr uint32_t kNone = 0xffffffffu;
   const uint32_t padding = s.padding < 0 ? kNone : (uint32_t)s.padding;
-  uint32_t key[kSteps];
+  uint32_t key[STEPS];
   const auto read = [&](int64_t n0) {  // the keys n0 + 64 u + lane; kNone: none that has a run
 #pragma unroll
-    for (int u0 = 0; u0 < kSteps; u0 += 16) {
+    for (int u0 = 0; u0 < STEPS; u0 += 8) {
       if (n0 + 64 * u0 >= hi) {
 #pragma unroll
-        for (int u = 0; u < 16; ++u) key[u0 + u] = kNone;
+        for (int u = 0; u < 8; ++u) key[u0 + u] = kNone;
         continue;
       }
-      uint2 raw[16];
+      uint2 raw[8];
 #pragma unroll
-      for (int u = 0; u < 16; ++u) {
+      for (int u = 0; u < 8; ++u) {
         const int64_t n = n0 + 64 * (u0 + u) + lane;
         raw[u] = make_uint2(kNone, 0);
         if (n < hi) {
@@ -225,17 +226,17 @@ __global__ __launch_bounds__(64 * kWaves) void embed_sort_kernel(const SortArgs 
         }
       }
 #pragma unroll
-      for (int u = 0; u < 16; ++u)
+      for (int u = 0; u < 8; ++u)
         key[u0 + u] = raw[u].y == 0 && raw[u].x < (uint32_t)s.R && raw[u].x != padding ? raw[u].x : kNone;
     }
   };
-  // a key's residue class; past every one for none
-  const auto bucket = [&](uint32_t k) { return k == kNone ? kNone : k & (uint32_t)mask; };
+  // a key's residue class; past every one for none (keys are below 2^31)
+  const auto bucket = [&](uint32_t k) { return k & ((uint32_t)mask | 0x80000000u); };
   int eq = 0, lt = 0, all = 0;
-  for (int64_t n = lo; n < hi; n += 64 * kSteps) {
+  for (int64_t n = lo; n < hi; n += 64 * STEPS) {
     read(n);
 #pragma unroll
-    for (int u = 0; u < kSteps; ++u) {
+    for (int u = 0; u < STEPS; ++u) {
       if (n + 64 * u >= hi) continue;
       const uint32_t k = bucket(key[u]);
       eq += __popcll(__ballot(k == (uint32_t)b));
@@ -262,10 +263,10 @@ __global__ __launch_bounds__(64 * kWaves) void embed_sort_kernel(const SortArgs 
   // this bucket's rows in their order
   int2* const kept = n_list <= kList ? list : s.list + base;
   if (eq) {
-    for (int64_t n = lo; n < hi; n += 64 * kSteps) {
-      if (seg > 64 * kSteps) read(n);
+    for (int64_t n = lo; n < hi; n += 64 * STEPS) {
+      if (seg > 64 * STEPS) read(n);
 #pragma unroll
-      for (int u = 0; u < kSteps; ++u) {
+      for (int u = 0; u < STEPS; ++u) {
         const bool mine = bucket(key[u]) == (uint32_t)b;
         const uint64_t m = __ballot(mine);
         if (!m) continue;
@@ -812,7 +813,9 @@ extern "C" int32_t llattn_embed_order(const llattn_embed_cfg* c, const void* ids
   SortArgs s = sets_of(c, ids, pos, order);
   s.first[1] = tokens ? s.set[0].buckets : 0;
   s.first[2] = s.first[1] + (positions && c->P ? s.set[1].buckets : 0);
-  if (s.first[2]) hipLaunchKernelGGL(embed_sort_kernel, dim3(s.first[2]), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream), s);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (s.first[2] && c->rows <= 16 * 64 * kWaves) hipLaunchKernelGGL(embed_sort_kernel<16>, dim3(s.first[2]), dim3(64 * kWaves), 0, st, s);
+  else if (s.first[2]) hipLaunchKernelGGL(embed_sort_kernel<32>, dim3(s.first[2]), dim3(64 * kWaves), 0, st, s);
   return check_launch("llattn_embed_order");
 }
 
