@@ -78,6 +78,10 @@ CASES = [
     (1100, 2, 3, 4, 36, F32, 1.0, "even", False),            # positions of 1100 rows each
     (2, 64, 200001, 70, 40, F32, 1.0, "even", False),        # more than 256 buckets
     (8, 512, 32000, 512, 136, BF16, 1.0, "frequent", True),
+    (16, 1024, 3000, 1024, 24, F32, 1.0, "frequent", True),  # as many rows as 16 steps of keys hold, and one more
+    (5, 3277, 3000, 3277, 24, BF16, 1.0, "frequent", True),
+    (1, 32769, 700, 32769, 8, F32, 1.0, "frequent", True),   # more than 32 steps hold
+    (4, 10001, 150000, 10001, 16, F32, 1.0, "even", False),
 ]
 
 
