@@ -191,10 +191,12 @@ struct SortArgs {
 };
 
 // The keys of a workgroup's waves, 64 at a time, stay in registers between the counting and the collecting where they are no
-// more than STEPS times 64 a wave (16384 rows, 32768 rows); others are read again.  64 registers at most: two workgroups on a CU, of the
-// two sets.  (8192 rows in two sets 12.0 us with 16 steps, 14.8 with 32, 19.4 with 76 registers; 32768 rows 25.4 with 16, 20.4 with 32.)
+// more than STEPS times 64 a wave (16384 rows, 32768 rows); others are read again.  With 16 steps in 64 registers, two workgroups on a CU:
+// those of both sets at a time.  (8192 rows in two sets 12.0 us, 14.8 with 32 steps, 19.4 with those in 76 registers; 32768 rows 25.4 with
+// 16 steps, 20.4 with 32.  In 64 registers these spill, and a launch with scratch memory slows its neighbours: forward 58 -> 61 us, the
+// tables' gradients 68 -> 72.)
 template <int STEPS>
-__global__ __launch_bounds__(64 * kWaves, 8) void embed_sort_kernel(const SortArgs a) {
+__global__ __launch_bounds__(64 * kWaves, STEPS <= 16 ? 8 : 4) void embed_sort_kernel(const SortArgs a) {
   __shared__ int2 list[kList];
   __shared__ int count[kWaves][kKeys];
   __shared__ int eq_of[kWaves], lt_of[kWaves], all_of[kWaves], sums[kKeys / 64];
@@ -479,6 +481,7 @@ __global__ __launch_bounds__(256) void embed_leaf_kernel(const BwdArgs a) {
   if (b.at < 0) return;
   Sum<T> sum;
   sum.zero();
+  // 8 rows ahead (32768 x 1408: 20.6 us; 4 21.2, 16 31.6, with fewer waves)
   add_rows<T, RAGGED, 8>(sum, kLeaf, k, a.D,
                          [&](int i) { return static_cast<const T*>(a.dout) + (int64_t)row_at(s, b.run, b.key, b.at + i) * a.D; });
   store_sums(a.leaf[set] + (int64_t)k.row * a.Dp, sum, k);
@@ -522,7 +525,7 @@ __device__ __forceinline__ void store_row(const BwdArgs& a, int set, const Task&
 // Rows of the tables' gradients, of a whole run each: the blocks of 1024, those of 32 behind them, the rows behind those.  Most runs are
 // empty or short, so what counts is the number of waves at work and not what each has in flight: with 8 (bf16: 6) on a SIMD
 // instead of 6 (4), two sums and two rows (bf16: four) ahead instead of four, 52305 rows x 1536 bf16 take 43 us for 49, 34048 x 1408
-// fp32 68 for 71.
+// fp32 68 for 71.  (One register of the bf16 form spills then, 11 where rows are ragged; 5 waves, without that, 46.)
 template <typename T> constexpr bool kWide = std::is_same_v<T, float>;
 template <typename T, bool RAGGED>
 __global__ __launch_bounds__(256, kWide<T> ? 8 : 6) void embed_bwd_kernel(const BwdArgs a) {
