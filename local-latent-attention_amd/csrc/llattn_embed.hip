@@ -243,7 +243,8 @@ __global__ __launch_bounds__(64 * kWaves, STEPS <= 16 ? 8 : 4) void embed_sort_k
       const uint32_t k = bucket(key[u]);
       eq += __popcll(__ballot(k == (uint32_t)b));
       lt += __popcll(__ballot(k < (uint32_t)b));
-      if (b == 0) all += __popcll(__ballot(k != kNone));
+      // by the key: a residue class of none is not kNone.  Positions of the order past these rows are never written
+      if (b == 0) all += __popcll(__ballot(key[u] != kNone));
     }
   }
   if (lane == 0) {

@@ -371,3 +371,34 @@ def test_indices_written_over_before_the_backward(value):
     ids.fill_(0)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         torch.autograd.grad(y, (w, p), torch.ones_like(y))
+
+
+@pytest.mark.parametrize("n", [1100, 5000, 16384, 40001])  # 16 and 32 steps of keys, and more
+def test_many_rows_without_a_run(n):
+    """Most rows padded or out of range, more of them than are looked through: the order counts the others alone, and the sums over
+    blocks read nothing behind those."""
+    from llattn_amd import embedding
+    V, P, D = 50, 9, 24
+    w, p = (t.requires_grad_() for t in _tables(V, P, D, F32))
+    g = torch.Generator().manual_seed(n)
+    ids = torch.where(torch.rand(n, generator=g) < 0.3, torch.randint(0, V, (n,), generator=g), 5)
+    ids[::7], ids[3::11] = -1, V
+    pos = torch.where(torch.rand(n, generator=g) < 0.6, torch.randint(0, P, (n,), generator=g), P + 3)
+    ids, pos = ids.to(DEV), pos.to(DEV)
+    _, i, q, cfg = embedding._forward(ids, w, p, pos, 1.0, 5)
+    order = embedding._order(i, q, cfg, True, True)
+    want = [int(((ids >= 0) & (ids < V) & (ids != 5)).sum()), int((pos < P).sum())]
+    assert order[:8].view(torch.int32).tolist() == want
+    dy = torch.randn(n, D, generator=g).to(DEV)
+    for scale in (1.0, -2.5):
+        dw, dp = torch.autograd.grad(_embed(ids, w, p, positions=pos, padding_idx=5, scale=scale), (w, p), dy)
+        _check_sums(dw, ids, dy, V, scale, skip=5)
+        _check_sums(dp, pos, dy, P, 1.0)
+
+
+def test_rows_of_padding_alone():
+    w, p = (t.requires_grad_() for t in _tables(3000, 700, 136, BF16))
+    ids = torch.full((8, 700), 17, device=DEV)
+    y = _embed(ids, w, p, positions=torch.full_like(ids, -1), padding_idx=17)
+    dw, dp = torch.autograd.grad(y, (w, p), torch.ones_like(y))
+    assert bool(y.isnan().all()) and bool((dw == 0).all()) and bool((dp == 0).all())
