@@ -35,6 +35,12 @@ constexpr int kWaves = 16;         // of a sorting workgroup
 constexpr int kList = 4096;        // rows of a bucket held in LDS
 constexpr int kMostRows = 1 << 22; // of a table: 8192 buckets
 
+// What each of a sorting workgroup's waves takes of n entries, in whole steps of 64.  n is anything below 2^31: unsigned, for the
+// sum of n and the waves, the waves' ends and the steps past the last entry go beyond that.
+__host__ __device__ constexpr uint32_t share_of(uint32_t n) { return ((n + kWaves - 1) / kWaves + 63) / 64 * 64; }
+static_assert(share_of(0x7fffffff) == 1u << 27 && share_of(0x7ffffff0) == 1u << 27 && share_of(0) == 0 && share_of(1) == 64,
+              "the waves' shares of the most rows");
+
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_f __attribute__((aligned(4)));
 typedef u32x4 u32x4_h __attribute__((aligned(2)));
@@ -204,7 +210,7 @@ __global__ __launch_bounds__(64 * kWaves, STEPS <= 16 ? 8 : 4) void embed_sort_k
   const Keys& s = a.set[which];
   const int b = blockIdx.x - a.first[which], mask = s.buckets - 1, shift = 31 - __builtin_clz(s.buckets);
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t seg = ((a.rows + kWaves - 1) / kWaves + 63) / 64 * 64;
+  const int64_t seg = share_of(a.rows);
   const int64_t lo = min((int64_t)a.rows, w * seg), hi = min((int64_t)a.rows, lo + seg);
   constexpr uint32_t kNone = 0xffffffffu;
   const uint32_t padding = s.padding < 0 ? kNone : (uint32_t)s.padding;
@@ -280,9 +286,8 @@ __global__ __launch_bounds__(64 * kWaves, STEPS <= 16 ? 8 : 4) void embed_sort_k
   }
   __syncthreads();
   // counted out by key: each wave counts a stretch of the list, the counts are added up by key and, within a key, by wave
-  const int step = ((n_list + kWaves - 1) / kWaves + 63) / 64 * 64;
-  const int from = min(n_list, w * step), to = min(n_list, from + step);
-  for (int i = from + lane; i < to; i += 64) atomicAdd(&count[w][kept[i].y], 1);
+  const uint32_t listed = n_list, step = share_of(listed), from = min(listed, w * step), to = min(listed, from + step);
+  for (uint32_t i = from + lane; i < to; i += 64) atomicAdd(&count[w][kept[i].y], 1);
   __syncthreads();
   const int k = threadIdx.x;
   if (w * 64 < s.per) {
@@ -318,7 +323,7 @@ __global__ __launch_bounds__(64 * kWaves, STEPS <= 16 ? 8 : 4) void embed_sort_k
     s.runs[b * s.per + k] = eq ? make_int2(first, first + eq) : make_int2(0, 0);
   }
   __syncthreads();
-  for (int i = from; i < to; i += 64) {
+  for (uint32_t i = from; i < to; i += 64) {
     const bool live = i + lane < to;
     const int2 x = live ? kept[i + lane] : make_int2(0, 0);
     uint64_t m = __ballot(live);  // the lanes of the same key

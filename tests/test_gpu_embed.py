@@ -402,3 +402,28 @@ def test_rows_of_padding_alone():
     y = _embed(ids, w, p, positions=torch.full_like(ids, -1), padding_idx=17)
     dw, dp = torch.autograd.grad(y, (w, p), torch.ones_like(y))
     assert bool(y.isnan().all()) and bool((dw == 0).all()) and bool((dp == 0).all())
+
+
+def test_the_most_rows():
+    """2^31 - 1 rows, nearly all of one token, so that the rows, a wave's share of them and a key's run lie next to 2^31.  Whole numbers:
+    column 0 counts the rows, and a sum of them takes two additions that are rounded (the blocks of 1024, below 2^21 of them, are
+    exact); column 1 has single rows next to where the shares of 2^27 end, powers of two that add up exactly."""
+    N = (1 << 31) - 1
+    ids = torch.full((N,), 2, dtype=torch.int32, device=DEV)
+    few = {0: 0, 77: 1, 1 << 30: 1, N - 1: 0}
+    for at, token in few.items():
+        ids[at] = token
+    w = torch.tensor([[1.0, 2.0], [3.0, 4.0], [5.0, 6.0]], device=DEV, requires_grad=True)
+    out = _embed(ids, w)
+    assert out.shape == (N, 2) and all(torch.equal(out[at], w.detach()[t]) for at, t in few.items())
+    assert torch.equal(out[N - 2], w.detach()[2]) and torch.equal(out[N // 3], w.detach()[2])
+    dy = torch.zeros(N, 2, device=DEV)
+    dy[:, 0] = 1.0
+    edges = [k * (1 << 27) + d for k in (1, 5, 9, 13, 15) for d in (-1, 0)] + [1, N - 2]
+    for k, at in enumerate(edges):
+        dy[at, 1] = 2.0 ** k
+    for at in few:
+        dy[at, 1] = 7.0
+    dw, = torch.autograd.grad(out, w, dy)
+    assert dw[:2].tolist() == [[2.0, 14.0], [2.0, 14.0]]
+    assert float(dw[2, 1]) == 2.0 ** len(edges) - 1 and abs(float(dw[2, 0]) - (N - 4)) <= 2 * U * N
