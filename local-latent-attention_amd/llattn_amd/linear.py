@@ -68,13 +68,15 @@ def pack_params(groups):
         dst = (ctypes.c_void_p * k)(*[sg[1].data_ptr() for sg in chunk])
         n = (ctypes.c_int64 * k)(*[sg[2] for sg in chunk])
         dt = (ctypes.c_int32 * k)(*[sg[3] for sg in chunk])
-        if any(sg[4] is not None for sg in chunk):
-            tdst = (ctypes.c_void_p * k)(*[sg[4] for sg in chunk])
-            tld = (ctypes.c_int64 * k)(*[sg[5] for sg in chunk])
-            rows = (ctypes.c_int32 * k)(*[sg[6] for sg in chunk])
-            _call("llattn_cast_transposed", k, src, dst, n, dt, tdst, tld, rows, L.stream_ptr(chunk[0][0].device))
-        else:
-            _call("llattn_cast", k, src, dst, n, dt, L.stream_ptr(chunk[0][0].device))
+        device = chunk[0][0].device
+        with L.on_device(device):
+            if any(sg[4] is not None for sg in chunk):
+                tdst = (ctypes.c_void_p * k)(*[sg[4] for sg in chunk])
+                tld = (ctypes.c_int64 * k)(*[sg[5] for sg in chunk])
+                rows = (ctypes.c_int32 * k)(*[sg[6] for sg in chunk])
+                _call("llattn_cast_transposed", k, src, dst, n, dt, tdst, tld, rows, L.stream_ptr(device))
+            else:
+                _call("llattn_cast", k, src, dst, n, dt, L.stream_ptr(device))
     return outs
 
 

@@ -267,6 +267,29 @@ def test_gated_refusals():
         gated_feed_forward(x, *_layers(3, 5, 2))
 
 
+@pytest.mark.parametrize("transposed", [False, True])
+def test_weights_are_cast_on_their_own_device(transposed, monkeypatch):
+    """The launch that rounds fp32 weights stands under their device, whichever one is current: a stream of another device's would
+    be refused, and the default streams, which have no handle, are not told apart."""
+    import contextlib
+    from llattn_amd import linear, ops
+    inside, calls = [], []
+
+    @contextlib.contextmanager
+    def on_device(device):
+        inside.append(device)
+        yield
+        inside.pop()
+    monkeypatch.setattr(L, "on_device", on_device)
+    monkeypatch.setattr(L, "require_gpu", lambda *t: None)
+    monkeypatch.setattr(L, "stream_ptr", lambda device: None)
+    monkeypatch.setattr(ops, "_call", lambda name, *a, **k: calls.append((name, list(inside))))
+    ws = [torch.zeros(8, 16) for _ in range(2 * linear.MAX_SEGS + 1)]
+    linear.pack_params([([w], BF16, transposed) for w in ws])
+    name = "llattn_cast_transposed" if transposed else "llattn_cast"
+    assert calls == [(name, [torch.device("cpu")])] * 3 and not inside
+
+
 # ---------------------------------------------------------------------------
 # the model
 # ---------------------------------------------------------------------------
