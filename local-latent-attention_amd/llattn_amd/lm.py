@@ -71,9 +71,26 @@ class FeedForward(nn.Module):
 GATES = {"swiglu": "silu", "geglu": "gelu"}
 
 
+def _plain(module: nn.Module, kind: type) -> bool:
+    """Whether a call of ``module`` is ``kind``'s forward on its own parameters and nothing else, so that an operator may read those
+    in its place: no forward of its own (an adapter's, a quantised layer's), no hooks (also those that make the weight before the
+    call), and parameters that are tensors of no other kind."""
+    t = type(module)
+    return (getattr(t, "forward", None) is kind.forward and t.__call__ is nn.Module.__call__ and "forward" not in module.__dict__
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
+            and all(type(p) in (nn.Parameter, torch.Tensor) for p in module._parameters.values() if p is not None))
+
+
+def _plain_layers(layers, dropout: nn.Module) -> bool:
+    """Whether ``layers`` are linear layers that nothing stands around, and ``dropout`` does nothing."""
+    return not _has_any_global_hook() and all(_plain(m, nn.Linear) for m in layers) and _plain(dropout, nn.Dropout) \
+        and (dropout.p == 0.0 or not dropout.training)
+
+
 class GatedFeedForward(nn.Module):
     """``w2(act(w1 x) * w3 x)``, the gated kind of :class:`FeedForward` (``config.ffn``: ``"swiglu"`` or ``"geglu"``).  On the GPU
-    under bf16 autocast, or in bf16 throughout, it runs as :func:`llattn_amd.gated.gated_feed_forward`."""
+    under bf16 autocast, or in bf16 throughout, it runs as :func:`llattn_amd.gated.gated_feed_forward` where its projections are
+    plain linear layers, without hooks; others are called one by one."""
 
     def __init__(self, config: ModelConfig) -> None:
         super().__init__()
@@ -85,14 +102,20 @@ class GatedFeedForward(nn.Module):
         self.fused = True  # False: separate torch ops (a comparison model sets it)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        autocast = torch.is_autocast_enabled("cuda")
-        bf16 = torch.get_autocast_dtype("cuda") == torch.bfloat16 if autocast else \
-            x.dtype == torch.bfloat16 == self.w1.weight.dtype == self.w3.weight.dtype == self.w2.weight.dtype
-        if self.fused and x.is_cuda and bf16 and (self.dropout.p == 0.0 or not self.training):
+        if self.fused and x.is_cuda and self._fusable(x):
             from .gated import gated_feed_forward
             return gated_feed_forward(x, self.w1, self.w3, self.w2, self.act)
         act = F.silu if self.act == "silu" else F.gelu
         return self.dropout(self.w2(act(self.w1(x)) * self.w3(x)))
+
+    def _fusable(self, x: torch.Tensor) -> bool:
+        """Whether the products are bf16 ones of plain linear layers and dropout does nothing."""
+        layers = (self.w1, self.w3, self.w2)
+        if not _plain_layers(layers, self.dropout):
+            return False
+        if torch.is_autocast_enabled("cuda"):
+            return torch.get_autocast_dtype("cuda") == torch.bfloat16
+        return x.dtype == torch.bfloat16 and all(m.weight.dtype == torch.bfloat16 for m in layers)
 
 
 def build_feed_forward(config: ModelConfig) -> nn.Module:

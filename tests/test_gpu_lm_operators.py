@@ -148,3 +148,28 @@ def test_generation_with_a_gated_model():
         out = m.generate(prompt, 4)
         again = m.generate(prompt, 4)
     assert out.shape == (1, 13) and torch.equal(out, again) and torch.equal(out[:, :9], prompt)
+
+
+@pytest.mark.parametrize("name", ["w1", "w3", "w2"])
+def test_projections_with_something_around_them(name):
+    """An adapter, or a hook, on one projection shows in the result: the model's is that of its layers called one by one."""
+    from llattn_amd.config import ModelConfig
+    from llattn_amd.lm import GatedFeedForward
+    torch.manual_seed(0)
+    ff = GatedFeedForward(ModelConfig(d_model=64, d_ff=136, ffn="swiglu")).to(DEV, torch.bfloat16)
+    x = torch.randn(40, 64, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    one_by_one = lambda: ff.w2(torch.nn.functional.silu(ff.w1(x)) * ff.w3(x))  # noqa: E731
+    with torch.no_grad():
+        clean = ff(x)
+        hook = getattr(ff, name).register_forward_hook(lambda m, a, y: y * 3)
+        assert torch.equal(ff(x), one_by_one()) and not torch.allclose(ff(x), clean, rtol=0.1)
+        hook.remove()
+        assert torch.equal(ff(x), clean)
+
+        class Adapter(torch.nn.Linear):
+            def forward(self, v):
+                return super().forward(v) * 3
+        m = Adapter(*reversed(getattr(ff, name).weight.shape)).to(DEV, torch.bfloat16)
+        m.load_state_dict(getattr(ff, name).state_dict())
+        setattr(ff, name, m)
+        assert torch.equal(ff(x), one_by_one()) and not torch.allclose(ff(x), clean, rtol=0.1)

@@ -313,6 +313,64 @@ def test_models_with_a_gate():
         _model(ffn="relu")
 
 
+class _Adapter(torch.nn.Linear):
+    """A linear layer that adds something of its own."""
+
+    def forward(self, x):
+        return super().forward(x) + 1
+
+
+def _stood_around(ff, name):
+    """The ways in which a layer of a feed-forward comes to be more than its weight and bias: (what it is, undo)."""
+    m = getattr(ff, name)
+
+    def own(_):
+        a = _Adapter(m.in_features, m.out_features).to(m.weight)
+        a.load_state_dict(m.state_dict())
+        setattr(ff, name, a)
+        return lambda: setattr(ff, name, m)
+
+    def wrapped(_):
+        setattr(ff, name, torch.nn.Sequential(m))
+        return lambda: setattr(ff, name, m)
+
+    def replaced(_):
+        m.forward = lambda x: torch.nn.functional.linear(x, m.weight, m.bias) + 1
+        return lambda: delattr(m, "forward")
+
+    def weight_made_before(_):
+        torch.nn.utils.weight_norm(m)
+        return lambda: torch.nn.utils.remove_weight_norm(m)
+    hooks = [lambda _: m.register_forward_hook(lambda *a: a[2] + 1).remove, lambda _: m.register_forward_pre_hook(lambda *a: None).remove,
+             lambda _: m.register_full_backward_hook(lambda *a: None).remove, lambda _: m.register_full_backward_pre_hook(lambda *a: None).remove,
+             lambda _: torch.nn.modules.module.register_module_forward_hook(lambda *a: None).remove]
+    return [own, wrapped, replaced, weight_made_before, *hooks]
+
+
+@pytest.mark.parametrize("name", ["w1", "w3", "w2"])
+def test_projections_that_the_gated_feed_forward_leaves_alone(name):
+    """Layers with a forward of their own, replaced ones and hooked ones are called, not read."""
+    ff, x = _model(ffn="swiglu").blocks[0].ff.bfloat16(), torch.zeros(1, dtype=BF16)
+    assert ff._fusable(x)
+    for way in _stood_around(ff, name):
+        undo = way(ff)
+        assert not ff._fusable(x)
+        undo()
+        assert ff._fusable(x)
+    torch.nn.utils.parametrize.register_parametrization(getattr(ff, name), "weight", torch.nn.Identity())
+    assert ff._fusable(x)  # its weight is what a call reads
+
+
+def test_dropout_of_a_gated_feed_forward():
+    ff, x = _model(ffn="geglu").blocks[0].ff.bfloat16(), torch.zeros(1, dtype=BF16)
+    ff.dropout.p = 0.5
+    assert not ff._fusable(x) and ff.eval()._fusable(x)
+    ff.dropout.train()  # alone: as dropout is switched on to sample from a model
+    assert not ff._fusable(x)
+    ff.dropout = torch.nn.Identity()
+    assert not ff._fusable(x)
+
+
 def test_lookups_on_the_cpu_are_torchs():
     m = _model()
     ids = torch.zeros(2, 5, dtype=torch.int64)
