@@ -173,3 +173,25 @@ def test_projections_with_something_around_them(name):
         m.load_state_dict(getattr(ff, name).state_dict())
         setattr(ff, name, m)
         assert torch.equal(ff(x), one_by_one()) and not torch.allclose(ff(x), clean, rtol=0.1)
+
+
+@pytest.mark.parametrize("name", ["w1", "w2"])
+def test_ungated_projections_with_something_around_them(name):
+    from llattn_amd.config import ModelConfig
+    from llattn_amd.lm import FeedForward
+    torch.manual_seed(0)
+    ff = FeedForward(ModelConfig(d_model=64, d_ff=136)).to(DEV)
+    x = torch.randn(40, 64, generator=torch.Generator().manual_seed(1)).to(DEV)
+    one_by_one = lambda: ff.w2(torch.nn.functional.gelu(ff.w1(x)))  # noqa: E731
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        clean = ff(x)
+        hook = getattr(ff, name).register_forward_hook(lambda m, a, y: y * 3)
+        assert torch.equal(ff(x), one_by_one()) and not torch.allclose(ff(x), clean, rtol=0.1)
+        hook.remove()
+        assert torch.equal(ff(x), clean)
+        layer = getattr(ff, name)
+        layer.forward = lambda v: torch.nn.functional.linear(v, layer.weight, layer.bias) * 3
+        assert torch.equal(ff(x), one_by_one()) and not torch.allclose(ff(x), clean, rtol=0.1)
+        del layer.forward
+        ff.dropout = torch.nn.Identity()
+        assert torch.equal(ff(x), one_by_one())
