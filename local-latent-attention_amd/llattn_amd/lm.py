@@ -114,9 +114,11 @@ class GatedFeedForward(nn.Module):
         layers = (self.w1, self.w3, self.w2)
         if not _plain_layers(layers, self.dropout):
             return False
-        if torch.is_autocast_enabled("cuda"):
-            return torch.get_autocast_dtype("cuda") == torch.bfloat16
-        return x.dtype == torch.bfloat16 and all(m.weight.dtype == torch.bfloat16 for m in layers)
+        types = {x.dtype, *[m.weight.dtype for m in layers]}
+        if torch.is_autocast_enabled("cuda"):  # which takes more types than the operator does
+            types |= {m.bias.dtype for m in layers if m.bias is not None}
+            return torch.get_autocast_dtype("cuda") == torch.bfloat16 and types <= {torch.float32, torch.bfloat16}
+        return types == {torch.bfloat16}
 
 
 def build_feed_forward(config: ModelConfig) -> nn.Module:

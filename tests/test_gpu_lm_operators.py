@@ -195,3 +195,35 @@ def test_ungated_projections_with_something_around_them(name):
         del layer.forward
         ff.dropout = torch.nn.Identity()
         assert torch.equal(ff(x), one_by_one())
+
+
+@pytest.mark.parametrize("what", ["x", "w3", "bias"])
+def test_types_that_autocast_takes(what):
+    """Half-precision inputs or layers under bf16 autocast, which the operator refuses: torch's products, as without it."""
+    from llattn_amd.config import ModelConfig
+    from llattn_amd.lm import GatedFeedForward
+    torch.manual_seed(0)
+    ff = GatedFeedForward(ModelConfig(d_model=64, d_ff=136, ffn="swiglu")).to(DEV)
+    x = torch.randn(40, 64, generator=torch.Generator().manual_seed(1)).to(DEV)
+    if what == "x":
+        x = x.half()
+    elif what == "w3":
+        ff.w3.half()
+    else:
+        ff.w1.bias = torch.nn.Parameter(ff.w1.bias.detach().half())
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        y = ff(x)
+        assert y.dtype is torch.bfloat16 and torch.equal(y, ff.w2(torch.nn.functional.silu(ff.w1(x)) * ff.w3(x)))
+
+
+def test_fp32_biases_of_a_half_precision_layer():
+    """Without autocast the operator takes them, which torch's products do not."""
+    from llattn_amd.config import ModelConfig
+    from llattn_amd.lm import GatedFeedForward
+    ff = GatedFeedForward(ModelConfig(d_model=64, d_ff=136, ffn="swiglu")).to(DEV, torch.bfloat16)
+    x = torch.randn(40, 64, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    with torch.no_grad():
+        want = ff(x)
+        for m in (ff.w1, ff.w3, ff.w2):
+            m.bias = torch.nn.Parameter(m.bias.detach().float())
+        assert torch.equal(ff(x), want)
