@@ -265,8 +265,8 @@ class LocalLatentLM(nn.Module):
                 m.weight.requires_grad for m in tables):
             return False
         if type(self.norm) is not RMSNorm or _has_any_global_hook() or any(
-                type(m) is not nn.Embedding or m.max_norm is not None or m.sparse or m.scale_grad_by_freq or not m.weight.is_cuda
-                or m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in tables):
+                type(m) is not nn.Embedding or not _plain(m, nn.Embedding) or m.max_norm is not None or m.sparse or m.scale_grad_by_freq
+                or not m.weight.is_cuda for m in tables):
             return False
         types = {m.weight.dtype for m in tables}
         return len(types) == 1 and types <= {torch.float32, torch.bfloat16} and self.position.padding_idx is None \

@@ -227,3 +227,18 @@ def test_fp32_biases_of_a_half_precision_layer():
         for m in (ff.w1, ff.w3, ff.w2):
             m.bias = torch.nn.Parameter(m.bias.detach().float())
         assert torch.equal(ff(x), want)
+
+
+@pytest.mark.parametrize("name", ["embedding", "position"])
+def test_tables_whose_call_is_replaced(name):
+    """A forward put on one table itself is what the model calls, with gradients and without."""
+    m = _model(fused_embeddings=True)
+    ids, table = _tokens(1, 20)[0], getattr(m, name)
+    with torch.no_grad():
+        clean = m.hidden(ids)
+    table.forward = lambda i: 3 * torch.nn.functional.embedding(i, table.weight)
+    assert not m._fused_embeddings(ids)
+    with torch.no_grad():
+        assert not m._fused_embeddings(ids) and not torch.allclose(m.hidden(ids), clean, rtol=0.1)
+    del table.forward
+    assert m._fused_embeddings(ids)
