@@ -126,9 +126,87 @@ def grad_norm(tensors) -> torch.Tensor:
     return norm
 
 
+def _span(t: torch.Tensor):
+    """(first byte, one past the last) of the memory that a tensor of one element at least lies in."""
+    at = t.data_ptr()
+    return at, at + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+_MEET_STEPS = 1 << 16
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors whose spans intersect share memory, which interleaved slices of one buffer do not.
+
+    Elements of a lie at sum x_k s_k, x_k < n_k along its axes, those of b likewise at y_k (where the elements' sizes differ, in bytes,
+    with an element's own as one more axis).  With n_k - 1 - y_k in y_k's place both are sums with positive steps, and the
+    question is whether their sum takes one value: by the largest step first, as often as those below can make up for.  Two that are
+    not told apart in 2^16 steps (axes that interleave in no order) count as one."""
+    size = a.element_size()
+    goal = b.data_ptr() - a.data_ptr()
+    bytewise = b.element_size() != size or goal % size != 0
+    goal //= 1 if bytewise else size
+    steps: dict[int, int] = {}
+    for t in (a, b):
+        unit = t.element_size() if bytewise else 1
+        axes = [(n - 1, s * unit) for n, s in zip(t.shape, t.stride()) if n > 1 and s]
+        for n, s in axes + [(unit - 1, 1)]:
+            steps[s] = steps.get(s, 0) + n
+            goal += n * s if t is b else 0
+    order = sorted(((s, n) for s, n in steps.items() if n), reverse=True)
+    rest, divisor = [0], [0]  # what the steps from the k-th on add up to at most, and what divides them; from the last
+    for s, n in reversed(order):
+        rest.append(rest[-1] + n * s)
+        divisor.append(math.gcd(divisor[-1], s))
+    rest.reverse()
+    divisor.reverse()
+    left = _MEET_STEPS
+
+    def found(k, goal):
+        nonlocal left
+        left -= 1
+        if not 0 <= goal <= rest[k]:
+            return False
+        if goal == 0 or left < 0:
+            return True
+        if goal % divisor[k]:
+            return False
+        s, n = order[k]
+        first, last = max(0, -((rest[k + 1] - goal) // s)), min(n, goal // s)
+        return any(found(k + 1, goal - x * s) for x in range(first, last + 1))
+    return found(0, goal)
+
+
+def _refuse_overlap(who: str, tensors, out) -> None:
+    """As the C call does for contiguous tensors, which are all that it sees: what is written overlaps nothing else, neither another
+    tensor that is written nor an input but its own in place."""
+    written = tensors if out is None else out
+    spans = [(*_span(t), i, t, True) for i, t in enumerate(written) if t.numel()]
+    if out is not None:
+        spans += [(*_span(t), i, t, False) for i, t in enumerate(tensors) if t.numel()]
+    spans.sort(key=lambda s: s[0])
+    held = []
+    for span in spans:
+        at, _, i, t, is_written = span
+        held = [h for h in held if h[1] > at]
+        for _, _, j, o, was_written in held:
+            if not (is_written or was_written):
+                continue
+            if is_written and was_written:
+                what = f"tensors {j} and {i}, which are written, overlap"
+            elif i == j and t.data_ptr() == o.data_ptr() and t.stride() == o.stride():
+                continue  # in place
+            else:
+                what = f"output {i if is_written else j} overlaps gradient {j if is_written else i}"
+            if _meet(t, o):
+                raise ValueError(f"{who}: {what}")
+        held.append(span)
+
+
 def _pairs(who: str, tensors, out):
     """Contiguous (sources, destinations) for gradients that are not all so; and (tensor, destination) pairs to be copied back."""
     src, dst, back = [], [], []
+    copied = False  # the C call does not see all tensors where they lie
     for i, g in enumerate(tensors):
         g = g.detach()
         o = g if out is None else out[i].detach()
@@ -136,6 +214,7 @@ def _pairs(who: str, tensors, out):
         f = _flat(g) if same else None  # both in one order of the axes: that of memory
         d = _flat(o) if same else o if o.is_contiguous() else None
         if f is None or d is None:
+            copied = True
             f = g.contiguous()
             if not o.is_contiguous():  # not in one stretch: scaled apart
                 if torch._debug_has_internal_overlap(o) == 1:
@@ -146,6 +225,8 @@ def _pairs(who: str, tensors, out):
                 d = o
         src.append(f)
         dst.append(d)
+    if copied:
+        _refuse_overlap(who, tensors, out)
     return src, dst, back
 
 

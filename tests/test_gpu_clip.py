@@ -256,3 +256,19 @@ def test_sparse_tensors_are_refused(where):
                 clip_grad_norm([t], 1.0)
             else:
                 clip_grad_norm([g], 1.0, out=[t])
+
+
+def test_strided_tensors_that_overlap_are_refused():
+    """As contiguous ones are; interleaved slices of one buffer are not refused, and each is scaled once."""
+    from llattn_amd import clip_grad_norm
+    a = _make([(60, 80)])[0]
+    keep = a.clone()
+    even, odd = a[:, ::2], a[:, 1::2]
+    for g, out in (([even, even], None), ([even, a], None), ([a[:, :50], a[:, 40:]], None), ([even, odd], [odd, even]),
+                   ([a[:, :60]], [a[:, :60].t()]), ([even], [a[:, 1:41]])):
+        with pytest.raises(ValueError, match="overlap|shapes"):
+            clip_grad_norm(g, 0.1, out=out)
+    assert torch.equal(a, keep)
+    _check(clip_grad_norm([even, odd], 0.5), [even, odd], [keep[:, ::2], keep[:, 1::2]], 0.5)
+    a.copy_(keep)
+    _check(clip_grad_norm([even, odd], 0.5, out=[even, odd]), [even, odd], [keep[:, ::2], keep[:, 1::2]], 0.5)

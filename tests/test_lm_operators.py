@@ -206,6 +206,50 @@ def test_flat_views():
         assert clip._flat(t) is None
 
 
+def _bytes(t):
+    """The bytes of a tensor's elements, one by one."""
+    at = {t.data_ptr()}
+    for n, s in zip(t.shape, t.stride()):
+        at = {v + k * s * t.element_size() for v in at for k in range(n)}
+    return {v + k for v in at for k in range(t.element_size())}
+
+
+def test_tensors_that_share_memory():
+    """Strided pieces of one buffer, of equal and of different types, against their bytes one by one."""
+    g = torch.Generator().manual_seed(0)
+    draw = lambda lo, hi: int(torch.randint(lo, hi, (), generator=g))  # noqa: E731
+    flat, found = torch.zeros(400), [0, 0]
+
+    def piece():
+        base = (flat, flat.view(BF16))[draw(0, 2)]
+        shape = [draw(1, 5) for _ in range(draw(1, 4))]
+        return base.as_strided(shape, [draw(0, 14) for _ in shape], draw(0, 60))
+    for _ in range(3000):
+        a, b = piece(), piece()
+        want = bool(_bytes(a) & _bytes(b))
+        assert clip._meet(a, b) == want == clip._meet(b, a), (a.shape, a.stride(), b.shape, b.stride())
+        found[want] += 1
+    assert min(found) > 300
+    big = torch.empty(1 << 13, 1 << 12, device="meta").as_strided((1 << 12, 1 << 11), (1 << 13, 2))
+    assert clip._meet(big, big)
+
+
+def test_strided_gradients_that_overlap_are_refused():
+    a, b = torch.ones(6, 8), torch.ones(8, 6)
+    even, odd = a[:, ::2], a[:, 1::2]
+    for g, out in (([even, odd], None), ([a[::2], a[1::2]], None), ([a[:, :4], a[:, 4:]], None), ([a[:3, ::3], a[3:, ::2]], None), ([even], [odd]), ([even], [even]),
+                   ([even, odd], [even, odd]), ([even], [b[:6, :4]]), ([even, even], [b[:6, :4], b.new_zeros(6, 4)]), ([a.t()], [b]),
+                   ([a[:, ::2], a[:0]], None)):
+        clip._refuse_overlap("clip", g, out)
+    for g, out, what in (([even, even], None, "overlap"), ([even, a], None, "overlap"), ([a[:, ::2], a[:, ::3]], None, "overlap"),
+                         ([a[:, :5], a[:, 4:]], None, "overlap"), ([even, odd], [odd, even], "overlaps gradient"),
+                         ([a[:, :4]], [a[:, 1:5]], "output 0 overlaps gradient 0"), ([a[:6, :6]], [a[:6, :6].t()], "output 0 overlaps gradient 0"),
+                         ([even, odd], [b[:6, :4], b[1:7, :4]], "written"), ([a, b.t()], [torch.ones(6, 8), a], "output 1 overlaps gradient 0"),
+                         ([a[:, ::2], a.view(BF16)[:, 5:9]], None, "overlap")):
+        with pytest.raises(ValueError, match=what):
+            clip._refuse_overlap("clip", g, out)
+
+
 # ---------------------------------------------------------------------------
 # gated feed-forward
 # ---------------------------------------------------------------------------
