@@ -39,7 +39,7 @@ typedef struct llattn_embed_cfg {
   int32_t dtype;        /* LLATTN_F32 or LLATTN_BF16 */
   int32_t index_bytes;
   int64_t padding;      /* a token without gradient, or -1 */
-  float scale;
+  float scale;          /* finite */
 } llattn_embed_cfg;
 
 int32_t llattn_embed_fwd(const llattn_embed_cfg* cfg, const void* ids, const void* pos, const void* W, int64_t ldw,

@@ -21,6 +21,7 @@
 // 57 (250 MB), order 20 (latency: half of it the reading of the keys by 256 workgroups), sums of 32 rows 20, of 1024 5, the tables
 // 68 (380 MB); a copy runs at 5.0 TB/s.  Few tokens take none but the last of these launches (embed_scan_kernel).
 #include <algorithm>
+#include <cmath>
 
 #include "llattn_abi.h"
 #include "llattn_device.h"
@@ -673,6 +674,7 @@ int32_t check(const char* who, const llattn_embed_cfg* c, bool has_pos) {
     return fail(LLATTN_ERR_SHAPE, "%s: T %d must be in [1, P %d] and divide the rows (%lld)", who, c->T, c->P, (long long)c->rows);
   if (c->dtype != LLATTN_F32 && c->dtype != LLATTN_BF16) return fail(LLATTN_ERR_DTYPE, "%s: unknown dtype %d", who, c->dtype);
   if (c->index_bytes != 4 && c->index_bytes != 8) return fail(LLATTN_ERR_DTYPE, "%s: indices of %d bytes", who, c->index_bytes);
+  if (!std::isfinite(c->scale)) return fail(LLATTN_ERR_SHAPE, "%s: scale %g is not finite", who, (double)c->scale);
   if (c->padding < -1 || c->padding >= c->V) return fail(LLATTN_ERR_SHAPE, "%s: padding %lld outside [-1, V)", who, (long long)c->padding);
   return LLATTN_OK;
 }

@@ -16,6 +16,7 @@ from . import _lib as L
 from . import ops
 
 MOST = 1 << 22  # rows of a table
+LARGEST = torch.finfo(torch.float32).max  # size of the scale
 _INDEX = (torch.int64, torch.int32)
 
 
@@ -152,6 +153,8 @@ def embed(ids: torch.Tensor, weight: torch.Tensor, position: torch.Tensor | None
         raise ValueError(f"embed: {ids.shape[-1]} tokens in a row and {P} positions")
     if type(scale) is not float and not isinstance(scale, Real):
         raise ValueError(f"embed: scale must be a number, got {type(scale).__name__}")
+    if not -LARGEST <= scale <= LARGEST:  # an infinite one would make NaN of the rows that no token names
+        raise ValueError(f"embed: scale must be finite in fp32, got {scale}")
     padding = -1
     if padding_idx is not None:
         if not isinstance(padding_idx, Integral) or not -V <= padding_idx < V:

@@ -54,6 +54,19 @@ def test_embed_sizes_refused(kw):
         assert L.load().llattn_embed_bytes(ctypes.byref(_cfg(**kw)), 0, which) == 0 and L.load().llattn_last_error()
 
 
+@pytest.mark.parametrize("scale", [float("inf"), float("-inf"), float("nan")])
+def test_scales_that_are_not_finite_are_refused(scale):
+    """They would reach the rows of the gradient that no token names, which are zero."""
+    assert L.load().llattn_embed_bytes(ctypes.byref(_cfg(scale=scale)), 0, 0) == 0 and b"finite" in L.load().llattn_last_error()
+    assert L.load().llattn_embed_fwd(ctypes.byref(_cfg(scale=scale)), AT, None, AT, 8, AT, 8, AT, None) == 1
+    ids, w = torch.zeros(2, 3, dtype=torch.int64), torch.zeros(5, 4)
+    for s in (scale, 3.5e38, 10 ** 400):  # infinite in fp32, or in 64 bits
+        with pytest.raises(ValueError, match="finite"):
+            embed(ids, w, scale=s)
+    with pytest.raises(RuntimeError, match="MI355X"):
+        embed(ids, w, scale=3.4e38)
+
+
 def test_embed_sizes_taken():
     def n(cfg, has_pos):
         return tuple(L.load().llattn_embed_bytes(ctypes.byref(cfg), has_pos, k) for k in (L.EMBED_ORDER, L.EMBED_BACKWARD))
