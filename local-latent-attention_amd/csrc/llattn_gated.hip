@@ -237,7 +237,7 @@ __device__ __forceinline__ void gated_tiles(const GatedArgs& a, unsigned char* s
   auto source = [&](const uint16_t* p, int64_t ld, bool t, int o, int n, int k, int K) {
     StepSrc s;
     s.addr = reinterpret_cast<uint64_t>(p + (t ? o + (int64_t)k * 64 * ld : o * ld + (int64_t)k * 64));
-    s.full = t ? extent_of(64, ld, n) : extent_of(n, ld, 64);  // not t: chunks past the last k are masked (RowOp::at)
+    s.full = t ? extent_of(64, ld, n) : rows_extent(n, ld, K);  // not t: chunks past the last k are masked (RowOp::at)
     s.tail = t ? extent_of(K & 63 ? K & 63 : 64, ld, n) : s.full;
     s.inc = t ? (uint32_t)(128 * ld) : 128u;
     return s;

@@ -249,10 +249,15 @@ struct StepSrc {
   }
 };
 // (rows - 1) ld + cols elements in bytes, as an extent (rows, cols >= 1)
-__device__ __forceinline__ uint32_t extent_of(int rows, int64_t ld, int cols) {
+__host__ __device__ constexpr uint32_t extent_of(int rows, int64_t ld, int cols) {
   const uint64_t n = (uint64_t)((int64_t)(rows - 1) * ld + cols) * 2;
   return n > kOffPastK ? kOffPastK : (uint32_t)n;
 }
+// The extent of a 64-k step of rows with k along them.  Chunks of a row past the last k are masked (kmask); of rows shorter than a
+// step the extent ends with the last one's own elements, or the row behind it would begin inside the extent.
+__host__ __device__ constexpr uint32_t rows_extent(int rows, int64_t ld, int K) { return extent_of(rows, ld, K < 64 ? K : 64); }
+static_assert(rows_extent(5, 40, 40) == 5 * 40 * 2 && rows_extent(1, 8, 8) == 16 && rows_extent(3, 72, 72) == (2 * 72 + 64) * 2 &&
+                  rows_extent(3, 128, 8) == (2 * 128 + 8) * 2, "no row behind the last begins inside the extent");
 
 // One wave's copy of 64 x 16 bytes into the 1 KB LDS block at byte address lds + AT (buffer_load ... lds, as dma_block).
 template <int AT>

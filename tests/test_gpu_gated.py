@@ -414,3 +414,27 @@ def test_vectorised_calls_are_refused():
     x = torch.randn(2, 5, 16, device=DEV, dtype=BF16)
     with pytest.raises(RuntimeError):
         torch.vmap(lambda v: _ffn(v, *layers))(x)
+
+
+@pytest.mark.parametrize("N", [1, 5, 40, 64, 70, 200])
+@pytest.mark.parametrize("sizes", [(8, 8, 8), (40, 136, 24), (136, 24, 40), (56, 200, 56)], ids=str)
+def test_nothing_behind_the_operands_is_read(N, sizes):
+    """x, the weights and dy end where NaN begin: of rows shorter than 64 elements too, no result depends on what lies behind them."""
+    D, F, Do = sizes
+    g = torch.Generator().manual_seed(N)
+
+    def held(rows, cols, behind, size=1.0):
+        t = torch.full((rows * cols + 4096,), behind, dtype=BF16, device=DEV)
+        t[:rows * cols] = (torch.randn(rows * cols, generator=torch.Generator().manual_seed(rows * 1000 + cols)) * size).to(BF16).to(DEV)
+        return t[:rows * cols].view(rows, cols)
+
+    def results(behind):
+        layers = _layers(D, F, Do)
+        for m in layers:
+            m.weight = torch.nn.Parameter(held(*m.weight.shape, behind, m.weight.shape[1] ** -0.5))
+        x, dy = held(N, D, behind).requires_grad_(), held(N, Do, behind)
+        out = _grads(x, layers, "gelu", dy)
+        with torch.no_grad():
+            return out + [_ffn(x, *layers, act="gelu")]
+    for name, a, b in zip((*NAMES, "y alone"), results(float("nan")), results(0.0)):
+        assert bool(a.isfinite().all()) and torch.equal(a, b), name
