@@ -128,7 +128,7 @@ __global__ __launch_bounds__(S::THREADS, WGS * S::W / 4) void head_kernel(const 
   auto source = [&](const uint16_t* p, int64_t ld, bool t, int o, int n, int k0) {  // n of the operand's rows (t: columns) from o on
     StepSrc s;
     s.addr = reinterpret_cast<uint64_t>(p + (t ? o + (int64_t)k0 * 64 * ld : o * ld + (int64_t)k0 * 64));
-    s.full = t ? extent_of(64, ld, n) : extent_of(n, ld, 64);  // not t: chunks past the last k are masked (RowOp::at)
+    s.full = t ? extent_of(64, ld, n) : rows_extent(n, ld, a.K);  // not t: chunks past the last k are masked (RowOp::at)
     s.tail = t ? extent_of(a.K & 63 ? a.K & 63 : 64, ld, n) : s.full;
     s.inc = t ? (uint32_t)(128 * ld) : 128u;
     return s;

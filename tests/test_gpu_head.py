@@ -431,3 +431,21 @@ def test_gradients_of_any_size_row_by_row(size):
     t1[1] = 5
     gh, = torch.autograd.grad(_loss(h, w, t1, reduction="none"), h, g)
     assert not torch.isfinite(gh[1]).any() and torch.isfinite(gh[2:]).all() and torch.isfinite(gh[0]).all()
+
+
+@pytest.mark.parametrize("N,D,V", [(1, 8, 1), (5, 24, 70), (70, 40, 509), (200, 56, 1000)])
+@pytest.mark.parametrize("piece", [0, 256])
+def test_nothing_behind_the_operands_is_read(N, D, V, piece):
+    """h and the weight end where NaN begin: of rows shorter than 64 elements too, no result depends on what lies behind them."""
+    h0, w0, t = _inputs(N, D, V)
+
+    def results(behind):
+        leaves = []
+        for v in (h0, w0):
+            flat = torch.full((v.numel() + 4096,), behind, dtype=BF16, device=DEV)
+            flat[:v.numel()] = v.flatten()
+            leaves.append(flat[:v.numel()].view(v.shape).requires_grad_())
+        loss = _loss(*leaves, t, reduction="sum", piece=piece)
+        return [loss.detach(), *torch.autograd.grad(loss, leaves)]
+    for a, b in zip(results(float("nan")), results(0.0)):
+        assert bool(a.isfinite().all()) and torch.equal(a, b)
