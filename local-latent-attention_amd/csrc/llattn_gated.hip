@@ -86,7 +86,7 @@ __device__ __forceinline__ void activation(int act, float a, float& f, float& df
 // which it would empty of the operands: the gate's product 220 -> 209 us there, its gradients' beside dW2 258 -> 240, the next
 // products, which read h and d, 98 -> 92 and 198 -> 182.
 struct Float24 {
-  static __host__ __device__ __forceinline__ int64_t elements(int64_t rows, int cols) { return (rows + 15) / 16 * 16 * cols; }
+  static __host__ __device__ constexpr int64_t elements(int64_t rows, int cols) { return (rows + 15) / 16 * 16 * cols; }
   static __device__ __forceinline__ int64_t place(int row, int col, int cols) {
     return (((int64_t)(row >> 4) * (cols >> 3) + (col >> 3)) * 16 + (row & 15)) * 8;
   }
@@ -717,7 +717,7 @@ constexpr int tile_m(int kind) { return kind == WIDE ? 256 : kTm[kind]; }
 constexpr int tile_n(int kind) { return kind == WIDE ? 192 : kTn[kind]; }
 
 // As tiling(), without thin tiles and with wide ones
-Tiling choose(int64_t M, int64_t N, int steps, int most, bool wide) {
+constexpr Tiling choose(int64_t M, int64_t N, int steps, int most, bool wide) {
   Tiling best = tiling(std::max<int64_t>(M, 65), N, steps, most);
   for (int S = 1; wide && S <= most && (S == 1 || steps / S >= 4); ++S) {
     const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 192) * S;
@@ -794,7 +794,7 @@ struct Plan {
 };
 // The sizes, and the tilings of a direction's products and what follows from them (a microsecond or two of the host's for each)
 enum { SIZES = 0, OF_FORWARD = 1, OF_BACKWARD = 2 };
-Plan plan_of(const llattn_gated_cfg* c, int which) {
+constexpr Plan tilings_of(const llattn_gated_cfg* c, int which) {
   Plan p{};
   const auto steps = [](int k) { return (k + 63) / 64; };
   const auto part = [](const Tiling& t, int64_t m, int64_t n, bool folded) { return t.splits > 1 || folded ? up((size_t)t.splits * m * n * 4) : 0; };
@@ -823,8 +823,13 @@ Plan plan_of(const llattn_gated_cfg* c, int which) {
     p.part[1] = part(p.dx, p.rows, c->D, p.low);
     p.part[2] = part(p.dw, 2 * (int64_t)p.half, c->D, false);
     p.part[3] = part(p.dw2, c->D_out, c->F, false);
-    p.colsum = up(std::max(llattn_colsum_workspace_size(p.rows, c->F), llattn_colsum_workspace_size(c->rows, c->D_out)));
   }
+  return p;
+}
+Plan plan_of(const llattn_gated_cfg* c, int which) {
+  Plan p = tilings_of(c, which);
+  if (which == OF_BACKWARD)
+    p.colsum = up(std::max(llattn_colsum_workspace_size(p.rows, c->F), llattn_colsum_workspace_size(c->rows, c->D_out)));
   return p;
 }
 // Forward with a backward to follow, forward alone (h in it, as two bf16 values where rows are few), backward, what is kept between them

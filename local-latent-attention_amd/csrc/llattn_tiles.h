@@ -81,7 +81,7 @@ struct ColOp {
   }
 };
 
-inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Workgroups: tiles of 64 x 128, 128 x 128 and 256 x 256.
 enum Kind { THIN = 0, SQUARE = 1, BIG = 2, KINDS = 3 };
@@ -116,7 +116,7 @@ struct Tiling { int kind, splits; double us; };
 
 // The tiles of an M x N product over `steps` 64-wide k steps, and the splits of its contraction (at most `most`): the least
 // expected time, in rounds of whole tiles over the 256 CUs, the partial sums written and read at 4.5 TB/s.
-inline Tiling tiling(int64_t M, int64_t N, int steps, int most) {
+constexpr Tiling tiling(int64_t M, int64_t N, int steps, int most) {
   Tiling best{SQUARE, 1, 1e30};
   for (int kind = M <= 64 ? THIN : SQUARE; kind < KINDS; ++kind) {
     if (most > 1 && kind == THIN) continue;  // gradients: 128 x 128 and larger

@@ -421,7 +421,6 @@ def test_vectorised_calls_are_refused():
 def test_nothing_behind_the_operands_is_read(N, sizes):
     """x, the weights and dy end where NaN begin: of rows shorter than 64 elements too, no result depends on what lies behind them."""
     D, F, Do = sizes
-    g = torch.Generator().manual_seed(N)
 
     def held(rows, cols, behind, size=1.0):
         t = torch.full((rows * cols + 4096,), behind, dtype=BF16, device=DEV)
@@ -438,3 +437,61 @@ def test_nothing_behind_the_operands_is_read(N, sizes):
             return out + [_ffn(x, *layers, act="gelu")]
     for name, a, b in zip((*NAMES, "y alone"), results(float("nan")), results(0.0)):
         assert bool(a.isfinite().all()) and torch.equal(a, b), name
+
+
+# Sizes whose products take the larger tiles, and which of them do (tests/test_lm_operators.py holds the choice to this list): rows and
+# columns end inside tiles, with biases and without, both activations, weight gradients of both types.  "split": the contraction is.
+LARGE = [
+    ((333, 1408, 4096, 1408, "silu", False, BF16, F32), {"dw": "WIDE"}),
+    ((4100, 1536, 1024, 1536, "gelu", True, BF16, BF16), {"gate": "BIG"}),
+    ((8190, 1408, 1200, 1408, "silu", True, BF16, BF16), {"out": "WIDE", "dx": "WIDE"}),
+    ((5000, 777, 3001, 777, "gelu", True, F32, F32), {"gate": "BIG", "dx": "BIG split"}),  # more tiles of the gate than run at a time
+    ((9432, 1160, 200, 1160, "silu", True, BF16, F32), {"out": "BIG", "dx": "BIG"}),
+    ((4542, 89, 6841, 521, "silu", True, BF16, F32), {"gate": "BIG", "out": "WIDE split", "dgate": "BIG", "dw2": "BIG split"}),
+    ((73, 1792, 2536, 3896, "gelu", False, BF16, BF16), {"dw": "WIDE", "dw2": "WIDE"}),
+    ((70, 2001, 3877, 3488, "silu", True, BF16, F32), {"dw": "BIG", "dw2": "BIG"}),
+    ((9469, 136, 3832, 8, "gelu", False, BF16, BF16), {"gate": "BIG", "dx": "WIDE split", "dw": "WIDE split"}),
+    ((5105, 824, 2555, 8, "silu", False, BF16, F32), {"gate": "BIG", "dx": "BIG split", "dw": "BIG split"}),
+    ((1219, 24, 4176, 3267, "gelu", True, BF16, BF16), {"gate": "BIG", "out": "BIG split", "dw2": "BIG"}),
+    ((10806, 8, 792, 2408, "silu", True, BF16, F32), {"out": "BIG", "dgate": "BIG", "dw2": "WIDE split"}),
+]
+
+
+@pytest.fixture
+def unwritten_memory_is_nan():
+    """New buffers hold NaN: what is read of them without having been written shows."""
+    held = torch.utils.deterministic.fill_uninitialized_memory, torch.are_deterministic_algorithms_enabled()
+    torch.utils.deterministic.fill_uninitialized_memory = True
+    torch.use_deterministic_algorithms(True, warn_only=True)
+    yield
+    torch.utils.deterministic.fill_uninitialized_memory = held[0]
+    torch.use_deterministic_algorithms(held[1])
+
+
+@pytest.mark.parametrize("case", [c for c, _ in LARGE], ids=lambda c: "-".join(str(v).replace("torch.", "") for v in c))
+def test_values_and_gradients_on_the_larger_tiles(case, unwritten_memory_is_nan):
+    test_values_and_gradients(case)
+
+
+@pytest.mark.parametrize("shape", [c[:4] for c, _ in LARGE], ids=str)
+def test_whole_numbers_on_the_larger_tiles(shape):
+    test_whole_numbers_are_exact(shape)
+
+
+@pytest.mark.parametrize("N", [1, 5, 33, 64, 65, 200])
+@pytest.mark.parametrize("sizes", [(72, 136, 40), (264, 520, 264), (777, 1001, 250)], ids=str)
+def test_nothing_is_read_that_was_not_written(N, sizes, unwritten_memory_is_nan):
+    D, F, Do = sizes
+    layers = _layers(D, F, Do)
+    g = torch.Generator().manual_seed(N)
+    x = torch.randn(N, D, generator=g).to(BF16).to(DEV).requires_grad_()
+    dy = torch.randn(N, Do, generator=g).to(BF16).to(DEV)
+    assert bool(torch.empty(1000, dtype=torch.uint8, device=DEV).eq(255).all())
+    got = _grads(x, layers, "silu", dy)
+    with torch.no_grad():
+        got.append(_ffn(x, *layers))
+    torch.utils.deterministic.fill_uninitialized_memory = False
+    want = _grads(x, layers, "silu", dy)
+    for name, a, b in zip((*NAMES, "y alone"), got, want + [got[-1]]):
+        assert bool(a.isfinite().all()), name
+        assert torch.equal(a, b), (name, int((a != b).sum()), float((a.double() - b.double()).abs().max()), (a != b).nonzero()[:4].tolist())

@@ -347,6 +347,33 @@ def test_weights_are_cast_on_their_own_device(transposed, monkeypatch):
     assert calls == [(name, [torch.device("cpu")])] * 3 and not inside
 
 
+def test_which_tiles_the_larger_cases_take(tmp_path):
+    """The sizes that tests/test_gpu_gated.py keeps for the kernels of larger tiles do take those, by the library's own choice."""
+    from llattn_amd import _build
+    from test_gpu_gated import CASES, LARGE
+    up = lambda n: -(-n // 8) * 8  # noqa: E731
+    lines = ['#include "llattn_gated.hip"', "namespace llattn { namespace {"]
+    taken = set()
+    for k, (case, kinds) in enumerate([*LARGE, *((c, {}) for c in CASES)]):
+        N, D, F, Do = case[0], *map(up, case[1:4])
+        lines.append(f"constexpr llattn_gated_cfg c{k}{{{N}, {D}, {F}, {Do}, 0, 0, 0}};")
+        for product in ("gate", "out", "dgate", "dx", "dw", "dw2"):
+            kind, *split = kinds.get(product, "SQUARE").split()
+            way = "OF_FORWARD" if product in ("gate", "out") else "OF_BACKWARD"
+            at = f"tilings_of(&c{k}, {way}).{product}"
+            lines.append(f"static_assert({at}.kind == {kind}, \"{case} {product}\");")
+            if kind != "SQUARE":
+                lines.append(f"static_assert(({at}.splits > 1) == {str(bool(split)).lower()}, \"{case} {product}\");")
+                taken.add((product, kind, bool(split)))
+    assert taken == {("gate", "BIG", False), ("dgate", "BIG", False),
+                     *((p, k, s) for p in ("out", "dx", "dw", "dw2") for k in ("BIG", "WIDE") for s in (False, True))}
+    src = tmp_path / "tilings.hip"
+    src.write_text("\n".join([*lines, "} }"]))
+    run = subprocess.run([_build.hipcc(), f"--offload-arch={_build.ARCH}", "--offload-host-only", "-fsyntax-only", "-std=c++17",
+                          f"-I{_build.INCLUDE_DIR}", f"-I{_build.SRC_DIR}", str(src)], capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr[-2000:]
+
+
 # ---------------------------------------------------------------------------
 # the model
 # ---------------------------------------------------------------------------
