@@ -427,3 +427,35 @@ def test_the_most_rows():
     dw, = torch.autograd.grad(out, w, dy)
     assert dw[:2].tolist() == [[2.0, 14.0], [2.0, 14.0]]
     assert float(dw[2, 1]) == 2.0 ** len(edges) - 1 and abs(float(dw[2, 0]) - (N - 4)) <= 2 * U * N
+
+
+@pytest.mark.parametrize("want", ["both", "tokens", "positions"])
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("N,T", [(600, 300), (2800, 700), (40000, 2000)])
+def test_nothing_is_read_that_was_not_written(N, T, given, want):
+    """New buffers filled with ones in every bit (NaN, and -1 as an index; the indices and gradients lie within wider memory, so that
+    even such an index reads what is there): the same bits."""
+    V, P, D = 300, T + 5, 40
+    g = torch.Generator().manual_seed(N)
+    w, p = _tables(V, P, D, F32)
+    w.requires_grad_(want != "positions")
+    p.requires_grad_(want != "tokens")
+    held = [torch.randint(-3, n, (N + 64,), generator=g).to(DEV) for n in (V + 3, P + 3)]
+    ids, pos = (h[32:N + 32].view(-1, T) for h in held)
+    dy = torch.randn(N + 64, D, generator=g).to(DEV)[32:N + 32].view(-1, T, D)
+
+    def call():
+        y = _embed(ids, w, p, positions=pos if given else None, padding_idx=7)
+        return [y.detach(), *torch.autograd.grad(y, [t for t in (w, p) if t.requires_grad], dy)]
+    clean = call()
+    was = torch.utils.deterministic.fill_uninitialized_memory
+    torch.use_deterministic_algorithms(True, warn_only=True)
+    torch.utils.deterministic.fill_uninitialized_memory = True
+    try:
+        assert bool(torch.empty(1000, dtype=torch.uint8, device=DEV).eq(255).all())
+        got = call()
+    finally:
+        torch.use_deterministic_algorithms(False)
+        torch.utils.deterministic.fill_uninitialized_memory = was
+    assert bool(torch.equal(got[0].nan_to_num(nan=7.0), clean[0].nan_to_num(nan=7.0)))
+    assert all(torch.equal(a, b) and bool(a.isfinite().all()) for a, b in zip(got[1:], clean[1:]))
