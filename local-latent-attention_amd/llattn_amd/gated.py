@@ -83,7 +83,7 @@ def _forward(x, act, ps, saved):
         with L.on_device(dev):
             ops._call("llattn_gated_fwd", ctypes.byref(cfg), xb.data_ptr(), xb.stride(0),
                   ctypes.byref(L.LlattnGatedWeights(*map(_ptr, ws), *map(_ptr, bs))), _ptr(kept), y.data_ptr(), _ptr(work), n,
-                  L.stream_ptr(dev), work=6 * N * D * Fd)
+                  L.stream_ptr(dev), work=2 * N * Fd * (2 * D + Do))
     if po:
         y = y[:, :Do]
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], Do), cfg, (xb, *ws, kept)
@@ -120,7 +120,7 @@ def _backward(ctx, dy):
         ops._call("llattn_gated_bwd", ctypes.byref(cfg), xb.data_ptr(), xb.stride(0),
               ctypes.byref(L.LlattnGatedWeights(w1.data_ptr(), w3.data_ptr(), w2.data_ptr(), None, None, None)), kept.data_ptr(),
               d.data_ptr(), ctypes.byref(L.LlattnGatedGrads(*map(_ptr, grads))), work.data_ptr(), n, L.stream_ptr(dev),
-              work=12 * N * D * Fd)
+              work=4 * N * Fd * (2 * D + Do))
     if dx is not None:
         if D > x_shape[-1]:
             dx = dx[:, :x_shape[-1]]

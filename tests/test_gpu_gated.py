@@ -495,3 +495,19 @@ def test_nothing_is_read_that_was_not_written(N, sizes, unwritten_memory_is_nan)
     for name, a, b in zip((*NAMES, "y alone"), got, want + [got[-1]]):
         assert bool(a.isfinite().all()), name
         assert torch.equal(a, b), (name, int((a != b).sum()), float((a.double() - b.double()).abs().max()), (a != b).nonzero()[:4].tolist())
+
+
+def test_the_work_that_calls_log():
+    """Operations of the products: 2 N F for each column of x read twice and of y written once, and twice that backward."""
+    from llattn_amd import ops
+    N, D, F, Do = 70, 16, 24, 40
+    layers = _layers(D, F, Do)
+    x = torch.ones(N, D, dtype=BF16, device=DEV, requires_grad=True)
+    ops.EVENT_LOG = []
+    try:
+        _grads(x, layers, "silu", torch.ones(N, Do, dtype=BF16, device=DEV))
+        work = {name: w for name, _, _, w in ops.EVENT_LOG}
+    finally:
+        ops.EVENT_LOG = None
+    n = 2 * N * F * (2 * D + Do)
+    assert work["llattn_gated_fwd"] == n and work["llattn_gated_bwd"] == 2 * n
