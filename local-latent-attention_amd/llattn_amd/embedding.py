@@ -117,7 +117,7 @@ def _check_integers(name: str, t: torch.Tensor) -> None:
 def embed(ids: torch.Tensor, weight: torch.Tensor, position: torch.Tensor | None = None,
           positions: torch.Tensor | None = None, scale: float = 1.0, padding_idx: int | None = None) -> torch.Tensor:
     """``scale * weight[ids] + position[positions]`` for ``ids [..., T]``, ``weight [V, D]`` and ``position [P, D]``
-    (fp32 or bf16, one type; any strides), computed in fp32 and rounded once to that type.
+    (fp32 or bf16, one type; any strides) and a finite ``scale``, computed in fp32 and rounded once to that type.
 
     Without ``positions`` (integers of ``ids``' shape, for packed documents or single tokens at their places) the tokens
     of the last axis stand at positions 0, 1, ...; without ``position`` nothing is added.  An id outside ``[0, V)`` or a

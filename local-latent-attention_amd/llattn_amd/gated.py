@@ -160,7 +160,9 @@ def gated_feed_forward(x: torch.Tensor, w1: torch.nn.Linear, w3: torch.nn.Linear
     ``w1`` and ``w3`` map D to F, ``w2`` F to any width, each with a bias or without.  ``x`` and the weights are bf16 or fp32,
     fp32 ones rounded to bf16 as under autocast; sums are fp32, gradients come in their input's type, those of weights and
     biases from fp32 sums, ``x``'s rounded to bf16 before it is widened.  Widths that are not multiples of 8 are padded in copies.
-    Fewer than 2^23 rows.  Differentiable once, in reverse mode.  GPU only."""
+    Fewer than 2^23 rows; a row's bits depend on how many are beside it (other kernels up to 16, 32 and 64 rows, and its gated product is
+    rounded to bf16 above 64).  The layers' weights and biases are read, their forwards and hooks are not run.  Differentiable
+    once, in reverse mode.  GPU only."""
     if act not in ACTS:
         raise ValueError(f"gated_feed_forward: act must be one of {tuple(ACTS)}, got {act!r}")
     ps = [_param(m, n) for m in (w1, w3, w2) for n in ("weight", "bias")]

@@ -204,7 +204,9 @@ class LocalLatentLM(nn.Module):
         return {k: v / count for k, v in totals.items()} if count else {}
 
     def hidden(self, input_ids: torch.Tensor) -> torch.Tensor:
-        """The final-norm hidden states ``[B, T, D]`` that the tied head maps to logits."""
+        """The final-norm hidden states ``[B, T, D]`` that the tied head maps to logits.  An id outside the vocabulary gives rows of NaN
+        where the lookups run as :func:`~llattn_amd.embedding.embed` (on the GPU wherever no gradient is asked for), with nothing said:
+        ids are the caller's to check.  Elsewhere torch's lookup raises, or stops the device."""
         _, seq_len = input_ids.shape
         if self._fused_embeddings(input_ids):
             x = embed(input_ids, self.embedding.weight, self.position.weight, padding_idx=self.embedding.padding_idx)
