@@ -33,6 +33,7 @@ from torch.utils.checkpoint import checkpoint
 from .clip import clip_grad_norm_
 from .config import MODEL_PRESETS, ModelConfig, build_attention
 from .embedding import MOST as MOST_EMBEDDINGS, embed
+from .ffn import _param
 from .norm import add_rms_norm, rms_norm
 
 
@@ -63,7 +64,7 @@ class FeedForward(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         # bf16 autocast on the GPU without active dropout: both products on the MFMA GEMM, GELU in their epilogues
         if (self.fused and x.is_cuda and torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16
-                and _plain_layers((self.w1, self.w2), self.dropout)):
+                and _plain_layers(("w1", "w2"), self)):
             from .ffn import feed_forward
             return feed_forward(x, self.w1, self.w2)
         return self.dropout(self.w2(F.gelu(self.w1(x))))
@@ -72,20 +73,35 @@ class FeedForward(nn.Module):
 GATES = {"swiglu": "silu", "geglu": "gelu"}
 
 
+_TYPES = {torch.float32, torch.bfloat16}
+_DENSE = (nn.Parameter, torch.Tensor, type(None))
+
+
 def _plain(module: nn.Module, kind: type) -> bool:
     """Whether a call of ``module`` is ``kind``'s forward on its own parameters and nothing else, so that an operator may read those
     in its place: no forward of its own (an adapter's, a quantised layer's), no hooks (also those that make the weight before the
     call), and parameters that are tensors of no other kind."""
-    t = type(module)
-    return (getattr(t, "forward", None) is kind.forward and t.__call__ is nn.Module.__call__ and "forward" not in module.__dict__
-            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
-            and all(type(p) in (nn.Parameter, torch.Tensor) for p in module._parameters.values() if p is not None))
+    t, held = type(module), module.__dict__
+    if t is not kind and (getattr(t, "forward", None) is not kind.forward or t.__call__ is not nn.Module.__call__):
+        return False
+    if "forward" in held or held["_forward_hooks"] or held["_forward_pre_hooks"] or held["_backward_hooks"] or held["_backward_pre_hooks"]:
+        return False
+    for p in held["_parameters"].values():
+        if type(p) not in _DENSE:
+            return False
+    return True
 
 
-def _plain_layers(layers, dropout: nn.Module) -> bool:
-    """Whether ``layers`` are linear layers that nothing stands around, and ``dropout`` does nothing."""
-    return not _has_any_global_hook() and all(_plain(m, nn.Linear) for m in layers) and _plain(dropout, nn.Dropout) \
-        and (dropout.p == 0.0 or not dropout.training)
+def _plain_layers(names, ff: nn.Module) -> bool:
+    """Whether the layers of ``ff`` of these names are linear ones that nothing stands around, and its dropout does nothing."""
+    if _has_any_global_hook():
+        return False
+    layers = ff._modules
+    for name in names:
+        if not _plain(layers[name], nn.Linear):
+            return False
+    dropout = layers["dropout"]
+    return _plain(dropout, nn.Dropout) and (dropout.p == 0.0 or not dropout.training)
 
 
 class GatedFeedForward(nn.Module):
@@ -111,14 +127,16 @@ class GatedFeedForward(nn.Module):
 
     def _fusable(self, x: torch.Tensor) -> bool:
         """Whether the products are bf16 ones of plain linear layers and dropout does nothing."""
-        layers = (self.w1, self.w3, self.w2)
-        if not _plain_layers(layers, self.dropout):
+        if not _plain_layers(("w1", "w3", "w2"), self):
             return False
-        types = {x.dtype, *[m.weight.dtype for m in layers]}
-        if torch.is_autocast_enabled("cuda"):  # which takes more types than the operator does
-            types |= {m.bias.dtype for m in layers if m.bias is not None}
-            return torch.get_autocast_dtype("cuda") == torch.bfloat16 and types <= {torch.float32, torch.bfloat16}
-        return types == {torch.bfloat16}
+        layers = self._modules["w1"], self._modules["w3"], self._modules["w2"]
+        weights = [_param(m, "weight").dtype for m in layers]
+        if not torch.is_autocast_enabled("cuda"):
+            return x.dtype is torch.bfloat16 and weights.count(torch.bfloat16) == 3
+        if torch.get_autocast_dtype("cuda") is not torch.bfloat16:
+            return False
+        biases = [b.dtype for m in layers if (b := _param(m, "bias")) is not None]
+        return _TYPES.issuperset((x.dtype, *weights, *biases))  # autocast takes more types than the operator does
 
 
 def build_feed_forward(config: ModelConfig) -> nn.Module:
